@@ -350,6 +350,131 @@ void ommx_b200_reset_launch_count(void);
 /* Tensor maps encoded since load: decode calls on planes that were decoded before encode none. */
 int64_t ommx_b200_tensor_map_encodings(void);
 
+/* ---- the 4-bit cache --------------------------------------------------------------------------
+ * A paged KV cache of its own beside the OMMX planes: keys and values of a token in 4 bits, a bf16 scale and zero for each
+ * 32 channels (160 bytes a token and kv head at head_dim 128).  No counterpart in the reference.
+ *
+ * records: [num_pages][n_kv_heads][page_size / 16][20 * head_dim] bytes.  A record holds 16 tokens of one kv head, in 32-bit
+ * words, G = head_dim / 32:
+ *   key codes         word (tau * 4 + t) * G + j       channels 32 j + 8 t + 0..7 of token tau, four bits each, lowest first
+ *   value codes       word (32 h + 4 g + t) * G + j    channels 32 j + 4 g + 0..3 of token 8 h + 2 t (low half) and the next (high)
+ *   key parameters    word tau * G + j                 bf16 scale << 16 | bf16 zero of channels 32 j + 0..31
+ *   value parameters  the same
+ * value = zero + scale * code, where for the 32 values x: zero = min x rounded down to bf16, scale = (max x - zero) / 15 *
+ * (1 - 2^-20) rounded up to bf16 (0 below 2^-96), code = (x - zero) * ((1 - 2^-20) / scale) rounded, in fp32.  NaN counts as 0
+ * and values beyond 2^126 as that (OMMX_ST_NONFINITE where one is not finite).
+ * summary (optional): bf16 [num_pages][n_kv_heads][2][head_dim], each page's channel maxima and minima of the stored keys' inputs,
+ * rounded outwards; what ommx_b200_kv4_select reads.
+ *
+ * A page that takes rows belongs to one sequence.  Lengths, tables and row ranges are read on the device: nothing synchronises, and
+ * a captured graph follows them.  Bad ones are reported in *status and skipped.
+ */
+typedef struct ommx_kv4_cache {
+    void *records;                  /* 16-byte aligned */
+    void *summary;                  /* 16-byte aligned, or NULL */
+    int32_t num_pages, n_kv_heads;
+    int32_t head_dim;               /* 64 or 128 */
+    int32_t page_size;              /* 16, 32, 64, 128 or 256 */
+} ommx_kv4_cache;
+
+typedef struct ommx_kv4_seqs {
+    const int32_t *b_seq_len;       /* [batch] tokens of each sequence, those this call appends among them */
+    const void *page_table;         /* [batch, pages_per_seq] int32 or int64 */
+    int64_t page_table_stride;      /* elements from row to row */
+    int32_t table_is_int64, pages_per_seq, batch;
+} ommx_kv4_seqs;
+
+typedef struct ommx_kv4_append_args {
+    ommx_kv4_cache cache;
+    ommx_kv4_seqs seqs;
+    const void *k_new, *v_new;      /* [num_rows, n_kv_heads, head_dim], last dimension contiguous */
+    int32_t dtype;                  /* OMMX_DT_* of k_new, v_new, q and q_out */
+    int32_t num_rows;
+    int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+    const int32_t *row_start;       /* [batch + 1]: rows row_start[b] .. row_start[b + 1] are the last tokens of sequence b; NULL: row b
+                                       is the last token of sequence b.  Rows behind row_start[batch] are left alone */
+    const void *q;                  /* [num_rows, n_q_heads, head_dim] to be rotated into q_out, or NULL; q_out may be q */
+    void *q_out;
+    int32_t n_q_heads;
+    int64_t q_stride_t, q_stride_h, qo_stride_t, qo_stride_h;
+    const float *cos, *sin;         /* [num_positions, rot_dim / 2], rows cs_stride apart; rows start on 16-byte boundaries */
+    int64_t cs_stride;
+    int32_t num_positions;
+    int32_t rot_dim;                /* channels rotated: 0 (none), 32, 64, 128 */
+    int32_t interleaved;            /* 0: pairs (c, c + rot_dim / 2), 1: pairs (2 i, 2 i + 1) */
+    const void *positions;          /* [num_rows] rotation positions, or NULL: the tokens' places in their sequences */
+    int32_t positions_is_int64;
+    int32_t *status;
+} ommx_kv4_append_args;
+
+/* Rotate the new rows' keys (and queries), quantize keys and values, store them, and keep the page summaries.  One launch. */
+int ommx_b200_kv4_append(const ommx_kv4_append_args *args, void *stream);
+
+typedef struct ommx_kv4_gather_args {
+    ommx_kv4_cache cache;
+    ommx_kv4_seqs seqs;
+    void *k, *v;                    /* [num_rows, n_kv_heads, head_dim], last dimension contiguous */
+    int32_t dtype;                  /* OMMX_DT_* of k and v */
+    int32_t num_rows;
+    int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+    const int32_t *row_start;       /* as in ommx_kv4_append_args */
+    int32_t *status;
+} ommx_kv4_gather_args;
+
+/* Read the last rows of every sequence back (all of them: row_start from the lengths).  One launch. */
+int ommx_b200_kv4_gather(const ommx_kv4_gather_args *args, void *stream);
+
+typedef struct ommx_kv4_decode_args {
+    ommx_kv4_cache cache;
+    ommx_kv4_seqs seqs;
+    const void *q;                  /* [batch, n_q_heads, head_dim], last dimension contiguous */
+    int32_t q_dtype;                /* OMMX_DT_BF16 or OMMX_DT_F16 */
+    int32_t n_q_heads;              /* a multiple of n_kv_heads */
+    int64_t q_stride_b, q_stride_h;
+    void *o;                        /* [batch, n_q_heads, head_dim] */
+    int32_t o_dtype;                /* OMMX_DT_* */
+    int64_t o_stride_b, o_stride_h;
+    float *lse;                     /* [batch, n_q_heads], natural logarithm; -inf (and o = 0) for a sequence of no tokens */
+    int64_t lse_stride_b;
+    const int32_t *selected;        /* [batch, n_kv_heads, num_selected] places of pages in their sequence, or NULL: all pages.  The first
+                                       min(num_selected, pages of the sequence) count; one below 0 is passed over */
+    int32_t num_selected;
+    float *workspace;               /* ommx_b200_kv4_workspace_floats() of them, 16-byte aligned; calls that overlap need their own */
+    int64_t workspace_floats;
+    int32_t max_seq_len;            /* an upper bound of b_seq_len that sizes the grid, 0: what the table can hold */
+    float sm_scale, logit_cap;      /* logits: cap * tanh(q.k * sm_scale / cap); cap 0: none */
+    int32_t *status;
+} ommx_kv4_decode_args;
+
+/* Attention of one query row per sequence over the cache, or over selected pages of it.  Two launches. */
+int ommx_b200_kv4_decode(const ommx_kv4_decode_args *args, void *stream);
+/* floats of workspace that a decode call needs on the current device */
+int64_t ommx_b200_kv4_workspace_floats(int32_t head_dim);
+
+typedef struct ommx_kv4_select_args {
+    ommx_kv4_cache cache;           /* summary is read, records are not */
+    ommx_kv4_seqs seqs;
+    const void *q;                  /* [batch, n_q_heads, head_dim], last dimension contiguous */
+    int32_t q_dtype;                /* OMMX_DT_BF16 or OMMX_DT_F16 */
+    int32_t n_q_heads;
+    int64_t q_stride_b, q_stride_h;
+    int32_t *selected;              /* out [batch, n_kv_heads, num_selected]: places of pages, ascending, then -1 */
+    int32_t num_selected;
+    int32_t first_pages, last_pages; /* always among them */
+    void *workspace;                /* ommx_b200_kv4_select_workspace_bytes() of them, 16-byte aligned */
+    int64_t workspace_bytes;
+    int32_t *status;
+} ommx_kv4_select_args;
+
+/*
+ * The num_selected pages of each sequence and kv head whose keys can meet its query heads best.  A page's score is the largest, over
+ * the query heads, of sum_c max(q_c M_c, q_c m_c) with its maxima M and minima m, in whole numbers: q * 2^(6 - e) rounded to
+ * +-127 (2^e the leading power of the kv head's largest |q|), M and m * (63/64) 2^(5 - f) rounded (2^f that of the page's
+ * largest), times 2^f.  No rounding depends on an order, so neither does the choice; ties go to the lower page.
+ */
+int ommx_b200_kv4_select(const ommx_kv4_select_args *args, void *stream);
+int64_t ommx_b200_kv4_select_workspace_bytes(int32_t batch, int32_t n_kv_heads, int32_t pages_per_seq);
+
 #ifdef __cplusplus
 }
 #endif

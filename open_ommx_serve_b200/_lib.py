@@ -85,6 +85,47 @@ class KVAppendArgs(C.Structure):
                 ("write_pos", C.c_void_p), ("index_is_int64", C.c_int32)]
 
 
+class KV4Cache(C.Structure):
+    _fields_ = [("records", C.c_void_p), ("summary", C.c_void_p), ("num_pages", C.c_int32), ("n_kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("page_size", C.c_int32)]
+
+
+class KV4Seqs(C.Structure):
+    _fields_ = [("b_seq_len", C.c_void_p), ("page_table", C.c_void_p), ("page_table_stride", C.c_int64),
+                ("table_is_int64", C.c_int32), ("pages_per_seq", C.c_int32), ("batch", C.c_int32)]
+
+
+class KV4AppendArgs(C.Structure):
+    _fields_ = [("cache", KV4Cache), ("seqs", KV4Seqs), ("k_new", C.c_void_p), ("v_new", C.c_void_p), ("dtype", C.c_int32),
+                ("num_rows", C.c_int32), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64), ("v_stride_t", C.c_int64),
+                ("v_stride_h", C.c_int64), ("row_start", C.c_void_p), ("q", C.c_void_p), ("q_out", C.c_void_p),
+                ("n_q_heads", C.c_int32), ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64), ("qo_stride_t", C.c_int64),
+                ("qo_stride_h", C.c_int64), ("cos", C.c_void_p), ("sin", C.c_void_p), ("cs_stride", C.c_int64),
+                ("num_positions", C.c_int32), ("rot_dim", C.c_int32), ("interleaved", C.c_int32), ("positions", C.c_void_p),
+                ("positions_is_int64", C.c_int32), ("status", C.c_void_p)]
+
+
+class KV4GatherArgs(C.Structure):
+    _fields_ = [("cache", KV4Cache), ("seqs", KV4Seqs), ("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32),
+                ("num_rows", C.c_int32), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64), ("v_stride_t", C.c_int64),
+                ("v_stride_h", C.c_int64), ("row_start", C.c_void_p), ("status", C.c_void_p)]
+
+
+class KV4DecodeArgs(C.Structure):
+    _fields_ = [("cache", KV4Cache), ("seqs", KV4Seqs), ("q", C.c_void_p), ("q_dtype", C.c_int32), ("n_q_heads", C.c_int32),
+                ("q_stride_b", C.c_int64), ("q_stride_h", C.c_int64), ("o", C.c_void_p), ("o_dtype", C.c_int32),
+                ("o_stride_b", C.c_int64), ("o_stride_h", C.c_int64), ("lse", C.c_void_p), ("lse_stride_b", C.c_int64),
+                ("selected", C.c_void_p), ("num_selected", C.c_int32), ("workspace", C.c_void_p), ("workspace_floats", C.c_int64),
+                ("max_seq_len", C.c_int32), ("sm_scale", C.c_float), ("logit_cap", C.c_float), ("status", C.c_void_p)]
+
+
+class KV4SelectArgs(C.Structure):
+    _fields_ = [("cache", KV4Cache), ("seqs", KV4Seqs), ("q", C.c_void_p), ("q_dtype", C.c_int32), ("n_q_heads", C.c_int32),
+                ("q_stride_b", C.c_int64), ("q_stride_h", C.c_int64), ("selected", C.c_void_p), ("num_selected", C.c_int32),
+                ("first_pages", C.c_int32), ("last_pages", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+                ("status", C.c_void_p)]
+
+
 class LaunchPlan(C.Structure):
     _fields_ = [(name, C.c_int32) for name in ("ctas", "cluster", "shares", "ctas_per_share", "groups_per_share")]
 
@@ -105,6 +146,12 @@ SYMBOLS = {
                                            C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "ommx_b200_kv_gather_inputs": (C.c_int, [C.POINTER(KVPool), C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
                                              C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "ommx_b200_kv4_append": (C.c_int, [C.POINTER(KV4AppendArgs), C.c_void_p]),
+    "ommx_b200_kv4_gather": (C.c_int, [C.POINTER(KV4GatherArgs), C.c_void_p]),
+    "ommx_b200_kv4_decode": (C.c_int, [C.POINTER(KV4DecodeArgs), C.c_void_p]),
+    "ommx_b200_kv4_workspace_floats": (C.c_int64, [C.c_int32]),
+    "ommx_b200_kv4_select": (C.c_int, [C.POINTER(KV4SelectArgs), C.c_void_p]),
+    "ommx_b200_kv4_select_workspace_bytes": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
     "ommx_b200_peer_alloc": (C.c_int, [C.c_size_t, C.POINTER(C.c_void_p), C.c_void_p]),
     "ommx_b200_peer_open": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "ommx_b200_peer_close": (C.c_int, [C.c_void_p]),

@@ -20,9 +20,12 @@
 #include <torch/csrc/utils/object_ptr.h>
 
 #include <cctype>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "../../include/ommx_b200.h"
 
@@ -593,6 +596,329 @@ PyObject *py_kv_gather_tail(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- the 4-bit cache --------------------------------------------------------------------------------
+// Arguments that do not fit raise here, with the reason; whether they are on the GPU is asked last, so that the other refusals hold
+// without one.
+struct Refusal { PyObject *type; std::string text; };
+[[noreturn]] void refuse(const std::string &text) { throw Refusal{PyExc_ValueError, text}; }
+std::string shape_text(const Tensor &t) {
+    std::string s = "[";
+    for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+    return s + "]";
+}
+
+struct KV4Call {
+    const char *who;
+    std::vector<std::pair<const char *, const Tensor *>> given;            // whose devices are compared at the end
+
+    const Tensor *tensor(PyObject *o, const char *name, bool needed = true) {
+        if (o == Py_None) {
+            if (needed) refuse(std::string(who) + ": " + name + " is needed");
+            return nullptr;
+        }
+        const Tensor *t = as_tensor(o);
+        if (!t) throw Refusal{PyExc_TypeError, std::string(who) + ": " + name + " must be a tensor"};
+        given.emplace_back(name, t);
+        return t;
+    }
+    void expect(bool ok, const std::string &text) const { if (!ok) refuse(std::string(who) + ": " + text); }
+    int64_t integer(PyObject *o, const char *name, int64_t lo) const {
+        int64_t v = 0;
+        if (!as_long(o, &v)) throw Refusal{PyExc_TypeError, std::string(who) + ": " + name + " must be an integer"};
+        expect(v >= lo && v <= INT32_MAX, std::string(name) + " = " + std::to_string(v) + " is out of range");
+        return v;
+    }
+    double number(PyObject *o, const char *name) const {
+        double v = 0;
+        if (!as_double(o, &v)) throw Refusal{PyExc_TypeError, std::string(who) + ": " + name + " must be a number"};
+        return v;
+    }
+    // [a, b, D] with a contiguous last dimension
+    const Tensor *rows(PyObject *o, const char *name, int64_t a, int64_t b, int64_t d, at::ScalarType type, bool needed = true) {
+        const Tensor *t = tensor(o, name, needed);
+        if (!t) return t;
+        expect(t->dim() == 3 && t->size(0) == a && t->size(1) == b && t->size(2) == d,
+               std::string(name) + " is " + shape_text(*t) + ", wanted [" + std::to_string(a) + ", " + std::to_string(b) + ", " + std::to_string(d) + "]");
+        expect(t->scalar_type() == type, std::string(name) + " has another dtype than it should: " + c10::toString(t->scalar_type()) + ", wanted " + c10::toString(type));
+        expect(t->size(2) <= 1 || t->stride(2) == 1, std::string(name) + "'s last dimension must be contiguous");
+        return t;
+    }
+    // rows that a kernel writes: no two of them in one place
+    void distinct(const Tensor &t, const char *name) const {
+        for (int i = 0; i < 2; ++i) expect(t.size(i) <= 1 || t.stride(i) != 0, std::string(name) + " must not be expanded: its rows are written");
+    }
+    void records(PyObject *o, ommx_kv4_cache *c) {
+        const Tensor *t = tensor(o, "records");
+        expect(t->dim() == 4 && t->scalar_type() == at::kByte && t->is_contiguous(), "records must be a contiguous uint8 tensor [pages, kv heads, page_size / 16, 20 * head_dim]");
+        const int64_t D = t->size(3) / 20;
+        expect(t->size(3) == 20 * D && t->size(0) <= INT32_MAX && t->size(1) > 0 && t->size(1) <= 4096 && t->size(2) >= 1 && t->size(2) <= 16,
+               "records is " + shape_text(*t) + ", wanted [pages, kv heads, page_size / 16, 20 * head_dim]");
+        c->records = t->data_ptr();
+        c->num_pages = (int32_t)t->size(0); c->n_kv_heads = (int32_t)t->size(1); c->page_size = 16 * (int32_t)t->size(2); c->head_dim = (int32_t)D;
+    }
+    void summary(PyObject *o, const ommx_kv4_cache &c, void **to) {
+        const Tensor *t = tensor(o, "summary", false);
+        if (!t) return;
+        expect(t->dim() == 4 && t->scalar_type() == at::kBFloat16 && t->is_contiguous() && t->size(0) == c.num_pages && t->size(1) == c.n_kv_heads && t->size(2) == 2 &&
+                   t->size(3) == c.head_dim, "summary must be a contiguous bfloat16 tensor [pages, kv heads, 2, head_dim] of the records' sizes");
+        *to = t->data_ptr();
+    }
+    void seqs(PyObject *table, PyObject *len, ommx_kv4_seqs *s) {
+        const Tensor *l = tensor(len, "b_seq_len"), *t = tensor(table, "page_table");
+        expect(l->dim() == 1 && l->scalar_type() == at::kInt && l->is_contiguous(), "b_seq_len must be a contiguous int32 tensor [batch]");
+        expect(t->dim() == 2 && (t->scalar_type() == at::kInt || t->scalar_type() == at::kLong) && (t->size(1) <= 1 || t->stride(1) == 1),
+               "page_table must be an int32 or int64 tensor [batch, pages] with contiguous rows");
+        expect(t->size(0) == l->size(0), "page_table has " + std::to_string(t->size(0)) + " rows for " + std::to_string(l->size(0)) + " lengths");
+        expect(l->size(0) <= INT32_MAX && t->size(1) <= INT32_MAX, "too many sequences or pages");
+        s->b_seq_len = (const int32_t *)l->data_ptr();
+        s->page_table = t->data_ptr(); s->page_table_stride = t->stride(0); s->table_is_int64 = t->scalar_type() == at::kLong;
+        s->pages_per_seq = (int32_t)t->size(1); s->batch = (int32_t)l->size(0);
+    }
+    const int32_t *row_start(PyObject *o, int64_t batch, int64_t rows) {
+        const Tensor *t = tensor(o, "row_start", false);
+        if (!t) {
+            expect(rows == batch, "without row_start there is one row for each of the " + std::to_string(batch) + " sequences, not " + std::to_string(rows));
+            return nullptr;
+        }
+        expect(t->dim() == 1 && t->scalar_type() == at::kInt && t->is_contiguous() && t->size(0) == batch + 1, "row_start must be a contiguous int32 tensor [batch + 1]");
+        return (const int32_t *)t->data_ptr();
+    }
+    int32_t *status(PyObject *o) {
+        const Tensor *t = tensor(o, "status", false);
+        if (!t) return nullptr;
+        expect(t->scalar_type() == at::kInt && t->numel() >= 1, "status must be an int32 tensor");
+        return (int32_t *)t->data_ptr();
+    }
+    // a workspace of the caller's, or one of this call
+    void *workspace(PyObject *o, at::ScalarType type, int64_t need, const at::Device &dev, Tensor *own) {
+        const Tensor *t = tensor(o, "workspace", false);
+        if (!t) {
+            if (need == 0) return nullptr;
+            const c10::cuda::CUDAGuard guard(dev);
+            *own = fresh({need}, at::TensorOptions().device(dev).dtype(type));
+            return own->data_ptr();
+        }
+        expect(t->scalar_type() == type && t->is_contiguous() && t->numel() >= need,
+               std::string("workspace must be a contiguous ") + c10::toString(type) + " tensor of at least " + std::to_string(need) + " values");
+        return t->data_ptr();
+    }
+    at::Device device() const {
+        const at::Device dev = given.front().second->device();
+        for (auto &g : given) {
+            if (!g.second->is_cuda()) throw Refusal{PyExc_RuntimeError, std::string(who) + " needs CUDA tensors (no CPU path): " + g.first + " is on " + g.second->device().str()};
+            expect(g.second->device() == dev, std::string(g.first) + " is on " + g.second->device().str() + ", " + given.front().first + " on " + dev.str());
+        }
+        return dev;
+    }
+};
+void head_size(const KV4Call &c, const ommx_kv4_cache &k) {
+    if (k.head_dim != 64 && k.head_dim != 128) throw Refusal{PyExc_NotImplementedError, std::string(c.who) + ": head_dim " + std::to_string(k.head_dim) + " (this build serves 64 and 128)"};
+    if (k.page_size & (k.page_size - 1)) throw Refusal{PyExc_NotImplementedError, std::string(c.who) + ": page_size " + std::to_string(k.page_size) + " (this build serves 16, 32, 64, 128 and 256)"};
+}
+int32_t type_code(const KV4Call &c, const Tensor &t, const char *name, bool f32) {
+    int32_t code = 0;
+    c.expect(dtype_code(t, &code) && (f32 || code != OMMX_DT_F32), std::string(name) + " must be bfloat16" + (f32 ? ", float16 or float32" : " or float16"));
+    return code;
+}
+#define KV4_TRY try {
+#define KV4_END } catch (const Refusal &r) { PyErr_SetString(r.type, r.text.c_str()); return nullptr; }
+
+// kv4_append(k_new, v_new, records, page_table, b_seq_len, row_start, q, q_out, cos, sin, positions, interleaved, summary, status)
+PyObject *py_kv4_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    KV4_TRY
+    if (n != 14) { PyErr_SetString(PyExc_TypeError, "kv4_append: wrong argument count"); return nullptr; }
+    KV4Call c{"ommx_kv4_append"};
+    ommx_kv4_append_args d;
+    memset(&d, 0, sizeof(d));
+    c.records(a[2], &d.cache);
+    head_size(c, d.cache);
+    c.seqs(a[3], a[4], &d.seqs);
+    const Tensor *k = c.tensor(a[0], "k_new");
+    c.expect(k->dim() == 3 && k->size(0) <= INT32_MAX, "k_new must be [rows, kv heads, head_dim]");
+    d.dtype = type_code(c, *k, "k_new", true);
+    const int64_t T = k->size(0), H = d.cache.n_kv_heads, D = d.cache.head_dim;
+    k = c.rows(a[0], "k_new", T, H, D, k->scalar_type());
+    const Tensor *v = c.rows(a[1], "v_new", T, H, D, k->scalar_type());
+    d.k_new = k->data_ptr(); d.v_new = v->data_ptr(); d.num_rows = (int32_t)T;
+    d.k_stride_t = k->stride(0); d.k_stride_h = k->stride(1); d.v_stride_t = v->stride(0); d.v_stride_h = v->stride(1);
+    d.row_start = c.row_start(a[5], d.seqs.batch, T);
+    const Tensor *cos = c.tensor(a[8], "cos", false), *sin = c.tensor(a[9], "sin", false), *q = c.tensor(a[6], "q", false);
+    c.expect(!cos == !sin, "cos and sin come together");
+    if (cos) {
+        for (const Tensor *t : {cos, sin})
+            c.expect(t->dim() == 2 && t->scalar_type() == at::kFloat && (t->size(1) <= 1 || t->stride(1) == 1), "cos and sin must be float32 tensors [positions, rot_dim / 2] with contiguous rows");
+        c.expect(cos->sizes() == sin->sizes() && cos->strides() == sin->strides() && cos->size(0) >= 1 && cos->size(0) <= INT32_MAX, "cos and sin must have the same size and strides, and a row");
+        c.expect(((uintptr_t)cos->data_ptr() | (uintptr_t)sin->data_ptr() | (uintptr_t)(cos->stride(0) * 4)) % 16 == 0, "rows of cos and sin must start on 16-byte boundaries");
+        c.expect(2 * cos->size(1) <= D, "cos and sin turn " + std::to_string(2 * cos->size(1)) + " channels of heads of " + std::to_string(D));
+        const int64_t rot = 2 * cos->size(1);
+        if (rot != 32 && rot != 64 && rot != 128) throw Refusal{PyExc_NotImplementedError, "ommx_kv4_append: a rotation of " + std::to_string(rot) + " channels (this build rotates 32, 64 or 128)"};
+        d.cos = (const float *)cos->data_ptr(); d.sin = (const float *)sin->data_ptr(); d.cs_stride = cos->stride(0);
+        d.num_positions = (int32_t)cos->size(0); d.rot_dim = (int32_t)rot;
+    }
+    bool interleaved = false;
+    c.expect(as_bool(a[11], &interleaved), "interleaved must be a truth value");
+    d.interleaved = interleaved;
+    if (const Tensor *pos = c.tensor(a[10], "positions", false)) {
+        c.expect(cos != nullptr, "positions without cos and sin");
+        c.expect(pos->dim() == 1 && pos->size(0) == T && (T <= 1 || pos->stride(0) == 1) && (pos->scalar_type() == at::kInt || pos->scalar_type() == at::kLong),
+                 "positions must be a contiguous int32 or int64 tensor of one value for each row");
+        d.positions = pos->data_ptr(); d.positions_is_int64 = pos->scalar_type() == at::kLong;
+    }
+    Tensor fresh_q;
+    const Tensor *out = nullptr;
+    if (q) {
+        c.expect(cos != nullptr, "q without cos and sin: there is nothing to do to it");
+        c.expect(q->dim() == 3 && q->size(1) >= 1, "q must be [rows, query heads, head_dim]");
+        q = c.rows(a[6], "q", T, q->size(1), D, k->scalar_type());
+        out = c.rows(a[7], "q_out", T, q->size(1), D, k->scalar_type(), false);
+        if (out) c.distinct(*out, "q_out");
+    } else {
+        c.expect(a[7] == Py_None, "q_out without q");
+    }
+    c.summary(a[12], d.cache, &d.cache.summary);
+    d.status = c.status(a[13]);
+    const at::Device dev = c.device();
+    if (q) {
+        if (!out) {
+            const c10::cuda::CUDAGuard guard(dev);
+            fresh_q = fresh({T, q->size(1), D}, q->options());
+            out = &fresh_q;
+        }
+        d.q = q->data_ptr(); d.q_out = out->data_ptr(); d.n_q_heads = (int32_t)q->size(1);
+        d.q_stride_t = q->stride(0); d.q_stride_h = q->stride(1); d.qo_stride_t = out->stride(0); d.qo_stride_h = out->stride(1);
+    }
+    const int rc = launch(dev, [&](void *stream) { return ommx_b200_kv4_append(&d, stream); });
+    if (rc) return PyLong_FromLong(rc);
+    if (!out) Py_RETURN_NONE;
+    if (!fresh_q.defined()) { Py_INCREF(a[7]); return a[7]; }
+    return THPVariable_Wrap(fresh_q);
+    KV4_END
+    END_HANDLE_TH_ERRORS
+}
+
+// kv4_gather(records, page_table, b_seq_len, k_out, v_out, row_start, status)
+PyObject *py_kv4_gather(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    KV4_TRY
+    if (n != 7) { PyErr_SetString(PyExc_TypeError, "kv4_gather: wrong argument count"); return nullptr; }
+    KV4Call c{"ommx_kv4_gather"};
+    ommx_kv4_gather_args d;
+    memset(&d, 0, sizeof(d));
+    c.records(a[0], &d.cache);
+    head_size(c, d.cache);
+    c.seqs(a[1], a[2], &d.seqs);
+    const Tensor *k = c.tensor(a[3], "k_out");
+    c.expect(k->dim() == 3 && k->size(0) <= INT32_MAX, "k_out must be [rows, kv heads, head_dim]");
+    d.dtype = type_code(c, *k, "k_out", true);
+    const int64_t T = k->size(0), H = d.cache.n_kv_heads, D = d.cache.head_dim;
+    k = c.rows(a[3], "k_out", T, H, D, k->scalar_type());
+    const Tensor *v = c.rows(a[4], "v_out", T, H, D, k->scalar_type());
+    c.distinct(*k, "k_out");
+    c.distinct(*v, "v_out");
+    d.k = k->data_ptr(); d.v = v->data_ptr(); d.num_rows = (int32_t)T;
+    d.k_stride_t = k->stride(0); d.k_stride_h = k->stride(1); d.v_stride_t = v->stride(0); d.v_stride_h = v->stride(1);
+    d.row_start = c.row_start(a[5], d.seqs.batch, T);
+    d.status = c.status(a[6]);
+    return PyLong_FromLong(launch(c.device(), [&](void *stream) { return ommx_b200_kv4_gather(&d, stream); }));
+    KV4_END
+    END_HANDLE_TH_ERRORS
+}
+
+// kv4_decode(q, records, page_table, b_seq_len, o, lse, sm_scale, logit_cap, selected, workspace, max_seq_len, status)
+PyObject *py_kv4_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    KV4_TRY
+    if (n != 12) { PyErr_SetString(PyExc_TypeError, "kv4_decode: wrong argument count"); return nullptr; }
+    KV4Call c{"ommx_kv4_decode_attention"};
+    ommx_kv4_decode_args d;
+    memset(&d, 0, sizeof(d));
+    c.records(a[1], &d.cache);
+    head_size(c, d.cache);
+    c.seqs(a[2], a[3], &d.seqs);
+    const int64_t B = d.seqs.batch, H = d.cache.n_kv_heads, D = d.cache.head_dim;
+    const Tensor *q = c.tensor(a[0], "q");
+    c.expect(q->dim() == 3 && q->size(1) <= INT32_MAX, "q must be [batch, query heads, head_dim]");
+    d.q_dtype = type_code(c, *q, "q", false);
+    const int64_t Hq = q->size(1);
+    q = c.rows(a[0], "q", B, Hq, D, q->scalar_type());
+    if (Hq < H || Hq % H) throw Refusal{PyExc_NotImplementedError, "ommx_kv4_decode_attention: " + std::to_string(Hq) + " query heads are not a multiple of " + std::to_string(H) + " kv heads"};
+    const Tensor *o = c.tensor(a[4], "o");
+    d.o_dtype = type_code(c, *o, "o", true);
+    o = c.rows(a[4], "o", B, Hq, D, o->scalar_type());
+    c.distinct(*o, "o");
+    const Tensor *lse = c.tensor(a[5], "lse");
+    c.expect(lse->dim() == 2 && lse->size(0) == B && lse->size(1) == Hq && lse->scalar_type() == at::kFloat && (Hq <= 1 || lse->stride(1) == 1) && (B <= 1 || lse->stride(0) >= Hq),
+             "lse must be a float32 tensor [batch, query heads] with contiguous rows");
+    d.q = q->data_ptr(); d.n_q_heads = (int32_t)Hq; d.q_stride_b = q->stride(0); d.q_stride_h = q->stride(1);
+    d.o = o->data_ptr(); d.o_stride_b = o->stride(0); d.o_stride_h = o->stride(1);
+    d.lse = (float *)lse->data_ptr(); d.lse_stride_b = lse->stride(0);
+    d.sm_scale = (float)(a[6] == Py_None ? 1.0 / std::sqrt((double)D) : c.number(a[6], "sm_scale"));
+    d.logit_cap = (float)c.number(a[7], "logit_cap");
+    c.expect(d.logit_cap >= 0.0f, "logit_cap must not be negative");
+    if (const Tensor *sel = c.tensor(a[8], "selected", false)) {
+        c.expect(sel->dim() == 3 && sel->scalar_type() == at::kInt && sel->is_contiguous() && sel->size(0) == B && sel->size(1) == H && sel->size(2) <= INT32_MAX,
+                 "selected must be a contiguous int32 tensor [batch, kv heads, pages]");
+        // no list of no pages: every sequence is then one of no tokens, and a null pointer would mean all of them
+        c.expect(sel->size(2) >= 1, "selected must have room for a page");
+        d.selected = (const int32_t *)sel->data_ptr(); d.num_selected = (int32_t)sel->size(2);
+    }
+    if (a[10] != Py_None) d.max_seq_len = (int32_t)c.integer(a[10], "max_seq_len", 0);
+    d.status = c.status(a[11]);
+    if (a[9] != Py_None) c.tensor(a[9], "workspace");
+    const at::Device dev = c.device();
+    Tensor own;
+    {
+        const c10::cuda::CUDAGuard guard(dev);
+        d.workspace_floats = ommx_b200_kv4_workspace_floats((int32_t)D);
+    }
+    d.workspace = (float *)c.workspace(a[9], at::kFloat, d.workspace_floats, dev, &own);
+    return PyLong_FromLong(launch(dev, [&](void *stream) { return ommx_b200_kv4_decode(&d, stream); }));
+    KV4_END
+    END_HANDLE_TH_ERRORS
+}
+
+// kv4_select(q, summary, page_table, b_seq_len, selected, page_size, first_pages, last_pages, workspace, status)
+PyObject *py_kv4_select(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    KV4_TRY
+    if (n != 10) { PyErr_SetString(PyExc_TypeError, "kv4_select: wrong argument count"); return nullptr; }
+    KV4Call c{"ommx_kv4_select_pages"};
+    ommx_kv4_select_args d;
+    memset(&d, 0, sizeof(d));
+    const Tensor *sum = c.tensor(a[1], "summary");
+    c.expect(sum->dim() == 4 && sum->scalar_type() == at::kBFloat16 && sum->is_contiguous() && sum->size(2) == 2 && sum->size(0) <= INT32_MAX && sum->size(1) >= 1 && sum->size(1) <= 4096,
+             "summary must be a contiguous bfloat16 tensor [pages, kv heads, 2, head_dim]");
+    d.cache.summary = sum->data_ptr(); d.cache.records = d.cache.summary;   // not read
+    d.cache.num_pages = (int32_t)sum->size(0); d.cache.n_kv_heads = (int32_t)sum->size(1); d.cache.head_dim = (int32_t)std::min<int64_t>(sum->size(3), INT32_MAX);
+    d.cache.page_size = (int32_t)c.integer(a[5], "page_size", 1);
+    head_size(c, d.cache);
+    c.seqs(a[2], a[3], &d.seqs);
+    const int64_t B = d.seqs.batch, H = d.cache.n_kv_heads, D = d.cache.head_dim;
+    const Tensor *q = c.tensor(a[0], "q");
+    c.expect(q->dim() == 3 && q->size(1) <= INT32_MAX, "q must be [batch, query heads, head_dim]");
+    d.q_dtype = type_code(c, *q, "q", false);
+    const int64_t Hq = q->size(1);
+    q = c.rows(a[0], "q", B, Hq, D, q->scalar_type());
+    if (Hq < H || Hq % H) throw Refusal{PyExc_NotImplementedError, "ommx_kv4_select_pages: " + std::to_string(Hq) + " query heads are not a multiple of " + std::to_string(H) + " kv heads"};
+    const Tensor *sel = c.tensor(a[4], "selected");
+    c.expect(sel->dim() == 3 && sel->scalar_type() == at::kInt && sel->is_contiguous() && sel->size(0) == B && sel->size(1) == H && sel->size(2) <= INT32_MAX,
+             "selected must be a contiguous int32 tensor [batch, kv heads, pages]");
+    d.q = q->data_ptr(); d.n_q_heads = (int32_t)Hq; d.q_stride_b = q->stride(0); d.q_stride_h = q->stride(1);
+    d.selected = (int32_t *)sel->data_ptr(); d.num_selected = (int32_t)sel->size(2);
+    d.first_pages = (int32_t)c.integer(a[6], "first_pages", 0); d.last_pages = (int32_t)c.integer(a[7], "last_pages", 0);
+    c.expect((int64_t)d.first_pages + d.last_pages <= d.num_selected, "first_pages and last_pages must fit into the " + std::to_string(d.num_selected) + " selected ones");
+    d.status = c.status(a[9]);
+    if (a[8] != Py_None) c.tensor(a[8], "workspace");
+    const at::Device dev = c.device();
+    Tensor own;
+    d.workspace_bytes = ommx_b200_kv4_select_workspace_bytes(d.seqs.batch, d.cache.n_kv_heads, d.seqs.pages_per_seq);
+    d.workspace = c.workspace(a[8], at::kByte, d.workspace_bytes, dev, &own);
+    return PyLong_FromLong(launch(dev, [&](void *stream) { return ommx_b200_kv4_select(&d, stream); }));
+    KV4_END
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef METHODS[] = {
     {"decode", (PyCFunction)(void (*)())py_decode, METH_FASTCALL, "paged decode attention; None when an argument needs explaining"},
     {"pack_into", (PyCFunction)(void (*)())py_pack_into, METH_FASTCALL, "quantize and pack into given planes; None when an argument needs explaining"},
@@ -600,6 +926,10 @@ PyMethodDef METHODS[] = {
     {"kv_append", (PyCFunction)(void (*)())py_kv_append, METH_FASTCALL, "decode-step store of a pool"},
     {"kv_append_block", (PyCFunction)(void (*)())py_kv_append_block, METH_FASTCALL, "prefill of one slot of a pool"},
     {"kv_gather_tail", (PyCFunction)(void (*)())py_kv_gather_tail, METH_FASTCALL, "residual rows by position"},
+    {"kv4_append", (PyCFunction)(void (*)())py_kv4_append, METH_FASTCALL, "rows into a 4-bit cache, rotated on the way"},
+    {"kv4_gather", (PyCFunction)(void (*)())py_kv4_gather, METH_FASTCALL, "rows of a 4-bit cache"},
+    {"kv4_decode", (PyCFunction)(void (*)())py_kv4_decode, METH_FASTCALL, "decode attention over a 4-bit cache"},
+    {"kv4_select", (PyCFunction)(void (*)())py_kv4_select, METH_FASTCALL, "the pages of a 4-bit cache that attention reads"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef MODULE = {PyModuleDef_HEAD_INIT, "_host", "torch tensors -> the C ABI of libommx_b200.so", -1, METHODS, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,482 @@
+// The 4-bit cache: attention of one query row per sequence.
+//
+// For query head h of a sequence, over its tokens t:  x_t = sm_scale q.K_t,  o = sum_t exp(x_t) V_t / sum_t exp(x_t), with
+// K_tc = z_tj + s_tj a_tc and V the same (j: the group of 32 channels that c is in, a: codes 0..15). So
+//   q.K_t = sum_j s_tj (sum_c q_c a_tc) + z_tj (sum_c q_c),      o_c = sum_t (p_t s_tj) a_tc + sum_t p_t z_tj:
+// the codes go into the tensor cores as they are. A nibble masked in place is the fp16 subnormal code * 2^-24 (or 2^-20), exact and
+// one LOP3 for two of them; the tokens (of K) and channels (of V) are the rows of an m16n8k16 product and up to eight query heads
+// that share the kv head its columns. Scales meet the sums of K's groups behind the product and the weights of V before it, zeros
+// are fp32 multiply-adds. Queries keep all their bits: a head's are scaled by a power of two into fp16's range.
+//
+// Weights p_t s_tj are rounded to fp16 (2^-12 of each, of either sign): against the running reference r, which covers the logit and
+// the scale, they are 2^12 at most, and those below 2^-36 of the largest are lost. Sums of weights and zeros stay fp32.
+#include "ommx_kv4.cuh"
+
+namespace ommx {
+namespace kv4 {
+
+constexpr int NW = 4;                             // warps to a block, each with tiles of 16 tokens of its own
+constexpr int COLS = 8;                           // query heads side by side
+constexpr int BLOCKS_PER_SM = 4;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float ROOM = 4096.0f;                   // how large a weight may get before its reference moves
+constexpr float LOWEST = -1e30f;
+
+struct DecodeParams {
+    Cache c;
+    Seqs s;
+    const void *q;
+    void *o;
+    float *lse, *work;
+    const int32_t *selected;
+    int64_t q_b, q_h, o_b, o_h, lse_b;
+    int32_t q16, o_type, Hq, group, col_blocks, num_selected, page_shift, least;
+    float sm_scale, cap;
+    int32_t *status;
+};
+
+// ---- how the work is dealt ------------------------------------------------------------------------
+// Units are records (16 tokens of a kv head, or a block of COLS of its query heads), in order of (sequence, kv head, block of heads,
+// place); block i of the grid takes `per` of them in a row. A row (sequence, kv head, block) that lies in one share is finished
+// there; the others' parts meet in the second kernel, which works the same shares out. A block writes at most two parts: of the row
+// that an earlier block began (slot 0) and of the one that a later block goes on with (slot 1).
+__device__ __forceinline__ int pages_of(const DecodeParams &p, int len) { return (len + p.c.page - 1) >> p.page_shift; }
+__device__ __forceinline__ int length_of(const DecodeParams &p, int b) {
+    const int len = p.s.len[b];
+    const int64_t most = (int64_t)p.s.max_pages << p.page_shift;
+    if (len < 0 || len > most) { or_status(p.status, OMMX_ST_BAD_LENGTH); return len < 0 ? 0 : (int)most; }
+    return len;
+}
+__device__ __forceinline__ int tiles_of(const DecodeParams &p, int len) {
+    if (p.selected) return min(pages_of(p, len), p.num_selected) * p.c.parts;
+    return (len + 15) >> 4;
+}
+struct Shares { int64_t per, total; };
+__device__ __forceinline__ Shares shares(const DecodeParams &p, int rows, int blocks, int lane) {
+    int64_t sum = 0;
+    for (int b = lane; b < p.s.B; b += 32) sum += tiles_of(p, length_of(p, b));
+#pragma unroll
+    for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+    Shares r;
+    r.total = sum * rows;
+    r.per = max((r.total + blocks - 1) / blocks, (int64_t)p.least);
+    return r;
+}
+
+// ---- pieces ---------------------------------------------------------------------------------------
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float scale_of(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ float zero_of(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23 & 255u) - 127; }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
+
+__device__ __forceinline__ float load_q(const DecodeParams &p, int64_t at) {
+    if (p.q16) return __half2float(reinterpret_cast<const __half *>(p.q)[at]);
+    return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p.q)[at]);
+}
+__device__ __forceinline__ void store_o(const DecodeParams &p, int64_t at, float v) {
+    if (p.o_type == OMMX_DT_F32) reinterpret_cast<float *>(p.o)[at] = v;
+    else if (p.o_type == OMMX_DT_F16) reinterpret_cast<__half *>(p.o)[at] = __float2half_rn(v);
+    else reinterpret_cast<__nv_bfloat16 *>(p.o)[at] = __float2bfloat16_rn(v);
+}
+
+// A kv head's queries as B fragments. Lane (g, t): head g, channels 32 j + 8 t + 0..7; frag[j][k] holds the channels (0, 4), (1, 5),
+// (2, 6), (3, 7); the second and fourth meet nibbles that are 16 times as large. sums: of two heads' (2 t, 2 t + 1) groups.
+template <int G> struct Query {
+    uint32_t frag[G][4];
+    float sums[G][2], factor[2];                  // in the products' units; what turns those into log2 units
+};
+template <int G> __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int first_head, int n, int lane, Query<G> &q) {
+    const int g = lane >> 2, t = lane & 3;
+    float x[G][8], top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[j][i] = g < n ? load_q(p, b * p.q_b + (first_head + g) * p.q_h + 32 * j + 8 * t + i) : 0.0f;
+            top = fmaxf(top, fabsf(x[j][i]));
+        }
+    top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+    const int e = top > 0.0f ? max(exponent_of(top), -100) : 0;
+    const float up = power_of_two(13 - e);
+    const float factor = p.sm_scale * power_of_two(24 - 13 + e) * (p.cap > 0.0f ? 1.0f : LOG2E);
+    q.factor[0] = __shfl_sync(~0u, factor, 8 * t);
+    q.factor[1] = __shfl_sync(~0u, factor, 8 * t + 4);
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { x[j][i] *= up; sum += x[j][i]; }
+        sum += __shfl_xor_sync(~0u, sum, 1);
+        sum += __shfl_xor_sync(~0u, sum, 2);
+        sum *= 0x1p-24f;
+        q.sums[j][0] = __shfl_sync(~0u, sum, 8 * t);
+        q.sums[j][1] = __shfl_sync(~0u, sum, 8 * t + 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float f = k & 1 ? 0.0625f : 1.0f;
+            q.frag[j][k] = half2_bits(x[j][k] * f, x[j][k + 4] * f);
+        }
+    }
+}
+
+// A warp's running state. acc[j][u]: channels 32 j + 4 g + 2 u (rows g) and + 1 (rows g + 8, 16 times too large), heads 2 t, 2 t + 1.
+template <int G> struct State {
+    float acc[G][2][4], zero[G][2], sum[2], ref[2];
+};
+
+template <int G> __device__ __forceinline__ void clear(State<G> &s) {
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s.acc[j][u][i] = 0.0f;
+        s.zero[j][0] = s.zero[j][1] = 0.0f;
+    }
+    s.sum[0] = s.sum[1] = 0.0f;
+    s.ref[0] = s.ref[1] = LOWEST;
+}
+template <int G> __device__ __forceinline__ void rescale(State<G> &s, float f0, float f1) {
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) { s.acc[j][u][0] *= f0; s.acc[j][u][1] *= f1; s.acc[j][u][2] *= f0; s.acc[j][u][3] *= f1; }
+        s.zero[j][0] *= f0; s.zero[j][1] *= f1;
+    }
+    s.sum[0] *= f0; s.sum[1] *= f1;
+}
+
+// One record, n of its tokens valid (1..16)
+template <int G> __device__ __forceinline__ void attend(const DecodeParams &p, const uint8_t *rec, int n, int lane, const Query<G> &q, State<G> &s) {
+    using W = typename Words<G>::T;
+    const int g = lane >> 2;
+    constexpr uint32_t LO = 0x000F000Fu, HI = 0x00F000F0u;
+    alignas(16) uint32_t k0[G], k1[G], v0[G], v1[G], kp0[G], kp1[G], vp0[G], vp1[G];
+    *reinterpret_cast<W *>(k0) = reinterpret_cast<const W *>(rec)[lane];
+    *reinterpret_cast<W *>(k1) = reinterpret_cast<const W *>(rec)[32 + lane];
+    *reinterpret_cast<W *>(kp0) = reinterpret_cast<const W *>(rec + Rec<G>::KP)[g];
+    *reinterpret_cast<W *>(kp1) = reinterpret_cast<const W *>(rec + Rec<G>::KP)[g + 8];
+    *reinterpret_cast<W *>(v0) = reinterpret_cast<const W *>(rec + Rec<G>::V)[lane];
+    *reinterpret_cast<W *>(v1) = reinterpret_cast<const W *>(rec + Rec<G>::V)[32 + lane];
+    *reinterpret_cast<W *>(vp0) = reinterpret_cast<const W *>(rec + Rec<G>::VP)[g];
+    *reinterpret_cast<W *>(vp1) = reinterpret_cast<const W *>(rec + Rec<G>::VP)[g + 8];
+
+    // ---- logits: x[0], x[1] of token g and heads 2 t, 2 t + 1; x[2], x[3] of token g + 8
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        mma(c, k0[j] & LO, k1[j] & LO, k0[j] & HI, k1[j] & HI, q.frag[j][0], q.frag[j][1]);
+        const uint32_t a = k0[j] >> 8, b = k1[j] >> 8;
+        mma(c, a & LO, b & LO, a & HI, b & HI, q.frag[j][2], q.frag[j][3]);
+        const float s0 = scale_of(kp0[j]), s1 = scale_of(kp1[j]), z0 = zero_of(kp0[j]), z1 = zero_of(kp1[j]);
+        x[0] = fmaf(z0, q.sums[j][0], fmaf(s0, c[0], x[0]));
+        x[1] = fmaf(z0, q.sums[j][1], fmaf(s0, c[1], x[1]));
+        x[2] = fmaf(z1, q.sums[j][0], fmaf(s1, c[2], x[2]));
+        x[3] = fmaf(z1, q.sums[j][1], fmaf(s1, c[3], x[3]));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] *= q.factor[i & 1];
+    if (p.cap > 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = p.cap * LOG2E * tanhf(x[i] / p.cap);
+    }
+    if (n < 16) {                                 // what lies behind the last token may be anything
+        if (g >= n) {
+            x[0] = x[1] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < G; ++j) vp0[j] = 0;
+        }
+        if (g + 8 >= n) {
+            x[2] = x[3] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < G; ++j) vp1[j] = 0;
+        }
+    }
+
+    // ---- weights
+    float top0 = scale_of(vp0[0]), top1 = scale_of(vp1[0]);
+#pragma unroll
+    for (int j = 1; j < G; ++j) { top0 = fmaxf(top0, scale_of(vp0[j])); top1 = fmaxf(top1, scale_of(vp1[j])); }
+    top0 = fmaxf(top0, 0x1p-30f);
+    top1 = fmaxf(top1, 0x1p-30f);
+    float w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = exp2_approx(x[i] - s.ref[i & 1]);
+    const float most = fmaxf(fmaxf(w[0], w[1]) * top0, fmaxf(w[2], w[3]) * top1);
+    if (__any_sync(~0u, !(most <= ROOM))) {
+        // the references move to the largest logit plus exponent of its scales
+        float r0 = fmaxf(x[0] + (exponent_of(top0) + 1), x[2] + (exponent_of(top1) + 1)), r1 = fmaxf(x[1] + (exponent_of(top0) + 1), x[3] + (exponent_of(top1) + 1));
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) {
+            r0 = fmaxf(r0, __shfl_xor_sync(~0u, r0, d));
+            r1 = fmaxf(r1, __shfl_xor_sync(~0u, r1, d));
+        }
+        r0 = fmaxf(s.ref[0], r0);
+        r1 = fmaxf(s.ref[1], r1);
+        rescale(s, exp2_approx(s.ref[0] - r0), exp2_approx(s.ref[1] - r1));
+        s.ref[0] = r0;
+        s.ref[1] = r1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = exp2_approx(x[i] - s.ref[i & 1]);
+    }
+    s.sum[0] += w[0] + w[2];
+    s.sum[1] += w[1] + w[3];
+
+    // ---- values
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+        const float s0 = scale_of(vp0[j]), s1 = scale_of(vp1[j]), z0 = zero_of(vp0[j]), z1 = zero_of(vp1[j]);
+        s.zero[j][0] = fmaf(z1, w[2], fmaf(z0, w[0], s.zero[j][0]));
+        s.zero[j][1] = fmaf(z1, w[3], fmaf(z0, w[1], s.zero[j][1]));
+        const uint32_t b0 = transpose8x8(half2_bits(w[0] * s0, w[1] * s0)), b1 = transpose8x8(half2_bits(w[2] * s1, w[3] * s1));
+        mma(s.acc[j][0], v0[j] & LO, v0[j] & HI, v1[j] & LO, v1[j] & HI, b0, b1);
+        const uint32_t a = v0[j] >> 8, b = v1[j] >> 8;
+        mma(s.acc[j][1], a & LO, a & HI, b & LO, b & HI, b0, b1);
+    }
+}
+
+template <int G> struct Shared {
+    static constexpr int D = 32 * G, PART = COLS * D + 2 * COLS;   // floats of a part in the workspace
+    float o[NW][COLS][D + 4];                     // the padding spreads the heads over the banks
+    float ref[NW][COLS], sum[NW][COLS];
+};
+
+// The warps' states of a row to its output, or to a part: [COLS][D] weighted values, [COLS] references, [COLS] sums
+template <int G>
+__device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Shared<G> &sh, int b, int first_head, int n, float *part, int warp, int lane) {
+    constexpr int D = 32 * G;
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int d = 4; d < 32; d *= 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s.sum[i] += __shfl_xor_sync(~0u, s.sum[i], d);
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) s.zero[j][i] += __shfl_xor_sync(~0u, s.zero[j][i], d);
+    }
+    if (g == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { sh.ref[warp][2 * t + i] = s.ref[i]; sh.sum[warp][2 * t + i] = s.sum[i]; }
+    }
+    __syncthreads();
+    float f[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float top = sh.ref[0][2 * t + i];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) top = fmaxf(top, sh.ref[w][2 * t + i]);
+        f[i] = exp2_approx(s.ref[i] - top);
+    }
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                sh.o[warp][2 * t + (i & 1)][32 * j + 4 * g + 2 * u + (i >> 1)] =
+                    f[i & 1] * fmaf(s.acc[j][u][i], i < 2 ? 0x1p24f : 0x1p20f, s.zero[j][i & 1]);
+    __syncthreads();
+    for (int i = threadIdx.x; i < COLS * D; i += 32 * NW) {
+        const int h = i / D, c = i % D;
+        float v = sh.o[0][h][c], top = sh.ref[0][h], sum = 0.0f;
+#pragma unroll
+        for (int w = 1; w < NW; ++w) { v += sh.o[w][h][c]; top = fmaxf(top, sh.ref[w][h]); }
+#pragma unroll
+        for (int w = 0; w < NW; ++w) sum += sh.sum[w][h] * exp2_approx(sh.ref[w][h] - top);
+        if (part) {
+            part[i] = v;
+            if (c == 0) { part[COLS * D + h] = top; part[COLS * D + COLS + h] = sum; }
+        } else if (h < n) {
+            store_o(p, b * p.o_b + (first_head + h) * p.o_h + c, sum != 0.0f ? v / sum : 0.0f);
+            if (c == 0) p.lse[b * p.lse_b + first_head + h] = sum != 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
+        }
+    }
+    __syncthreads();
+}
+
+template <int G> __global__ void __launch_bounds__(32 * NW, BLOCKS_PER_SM) kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
+    __shared__ Shared<G> sh;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    wait_earlier();
+    let_next_in();
+    const int rows = p.c.H * p.col_blocks;
+    const Shares sr = shares(p, rows, gridDim.x, lane);
+    int64_t u = blockIdx.x * sr.per;
+    const int64_t end = min(u + sr.per, sr.total), start = u;
+    if (u >= end) return;
+    // the sequence that unit u lies in
+    int b = 0, tiles = 0, len = 0;
+    int64_t base = 0;                             // units before sequence b
+    for (int b0 = 0;; b0 += 32) {
+        const int l = b0 + lane < p.s.B ? length_of(p, b0 + lane) : 0, n = tiles_of(p, l);
+        const int sum = warp_inclusive_scan(n, lane);              // of 32 sequences: below 2^31 tiles of 16 tokens
+        const uint32_t past = __ballot_sync(~0u, base + (int64_t)sum * rows > u);
+        if (past) {
+            const int from = __ffs(past) - 1;
+            b = b0 + from;
+            base += (int64_t)__shfl_sync(~0u, sum - n, from) * rows;
+            tiles = __shfl_sync(~0u, n, from);
+            len = __shfl_sync(~0u, l, from);
+            break;
+        }
+        base += (int64_t)__shfl_sync(~0u, sum, 31) * rows;
+    }
+    while (u < end) {
+        while (u >= base + (int64_t)tiles * rows) {               // the next sequence that has any
+            base += (int64_t)tiles * rows;
+            len = length_of(p, ++b);
+            tiles = tiles_of(p, len);
+        }
+        const int row = (int)((u - base) / tiles), i0 = (int)(u - base - (int64_t)row * tiles), i1 = (int)min((int64_t)tiles, i0 + (end - u));
+        const int head = row / p.col_blocks, cb = row % p.col_blocks;
+        const int first_head = head * p.group + cb * COLS, n = min(COLS, p.group - cb * COLS);
+        Query<G> q;
+        State<G> s;
+        load_query<G>(p, b, first_head, n, lane, q);
+        clear(s);
+        const int32_t *sel = p.selected ? p.selected + ((int64_t)b * p.c.H + head) * p.num_selected : nullptr;
+        for (int i = i0 + warp; i < i1; i += NW) {
+            const int slot = i / p.c.parts, part = i - slot * p.c.parts, place = sel ? sel[slot] : slot;
+            const int64_t first = ((int64_t)place << p.page_shift) + 16 * part;
+            if (place < 0 || first >= len) continue;
+            const int64_t id = page_id(p.s, b, place);
+            if (id < 0 || id >= p.c.num_pages) { or_status(p.status, OMMX_ST_BAD_PAGE); continue; }
+            attend<G>(p, p.c.records + ((id * p.c.H + head) * p.c.parts + part) * Rec<G>::BYTES, (int)min((int64_t)16, len - first), lane, q, s);
+        }
+        float *part = nullptr;
+        if (i0 > 0 || i1 < tiles) part = p.work + (2 * (int64_t)blockIdx.x + (base + (int64_t)row * tiles >= start)) * Shared<G>::PART;
+        finish<G>(p, s, sh, b, first_head, n, part, warp, lane);
+        u += i1 - i0;
+    }
+}
+
+// Rows of which several blocks have a part, and those of no tokens. Grid: (rows of a sequence x COLS, sequences); a warp takes every
+// fourth part, a lane four (two) channels.
+template <int G> __global__ void __launch_bounds__(128) kv4_combine_kernel(const __grid_constant__ DecodeParams p, int blocks) {
+    constexpr int D = 32 * G;
+    __shared__ float so[4][D], sr[4], ss[4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int b = blockIdx.y, row = blockIdx.x / COLS, h = blockIdx.x % COLS;
+    const int head = row / p.col_blocks, cb = row % p.col_blocks, hq = head * p.group + cb * COLS + h;
+    wait_earlier();
+    let_next_in();
+    if (h >= p.group - cb * COLS) return;
+    const int rows = p.c.H * p.col_blocks;
+    const Shares sh = shares(p, rows, blocks, lane);
+    int64_t before = 0;
+    for (int i = lane; i < b; i += 32) before += tiles_of(p, length_of(p, i));
+#pragma unroll
+    for (int d = 16; d; d /= 2) before += __shfl_xor_sync(~0u, before, d);
+    const int tiles = tiles_of(p, length_of(p, b));
+    if (tiles == 0) {
+        for (int c = threadIdx.x; c < D; c += 128) store_o(p, b * p.o_b + hq * p.o_h + c, 0.0f);
+        if (threadIdx.x == 0) p.lse[b * p.lse_b + hq] = -INFINITY;
+        return;
+    }
+    const int64_t r0 = before * rows + (int64_t)row * tiles, r1 = r0 + tiles;
+    const int64_t c0 = r0 / sh.per, c1 = (r1 - 1) / sh.per;
+    if (c0 == c1) return;                         // finished where it was computed
+    float top = LOWEST, sum = 0.0f, o[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) o[i] = 0.0f;
+    for (int64_t c = c0 + warp; c <= c1; c += 4) {
+        const float *part = p.work + (2 * c + (r0 >= c * sh.per)) * Shared<G>::PART;
+        const float ref = part[COLS * D + h], add = part[COLS * D + COLS + h], r = fmaxf(top, ref);
+        const float keep = exp2_approx(top - r), take = exp2_approx(ref - r);
+        const float *v = part + h * D + lane * G;
+#pragma unroll
+        for (int i = 0; i < G; ++i) o[i] = fmaf(v[i], take, o[i] * keep);
+        sum = fmaf(add, take, sum * keep);
+        top = r;
+    }
+    if (lane == 0) { sr[warp] = top; ss[warp] = sum; }
+#pragma unroll
+    for (int i = 0; i < G; ++i) so[warp][lane * G + i] = o[i];
+    __syncthreads();
+    float r = sr[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) r = fmaxf(r, sr[w]);
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) sum += ss[w] * exp2_approx(sr[w] - r);
+    for (int c = threadIdx.x; c < D; c += 128) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v = fmaf(so[w][c], exp2_approx(sr[w] - r), v);
+        store_o(p, b * p.o_b + hq * p.o_h + c, sum != 0.0f ? v / sum : 0.0f);
+    }
+    if (threadIdx.x == 0) p.lse[b * p.lse_b + hq] = sum != 0.0f ? (r + log2f(sum)) * LN2 : -INFINITY;
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+static int64_t workspace_floats(int head_dim) {
+    const int64_t part = head_dim == 64 ? Shared<2>::PART : Shared<4>::PART;
+    return 2 * part * BLOCKS_PER_SM * sm_count();
+}
+
+template <int G> static int launch_decode(const DecodeParams &p, int64_t blocks, cudaStream_t st) {
+    if (int rc = launch_dependent(kv4_decode_kernel<G>, dim3((unsigned)blocks), 32 * NW, 0, st, p)) return rc;
+    return launch_dependent(kv4_combine_kernel<G>, dim3(p.c.H * p.col_blocks * COLS, p.s.B), 128, 0, st, p, (int)blocks);
+}
+
+static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
+    if (!a) return fail(OMMX_E_ARG, "kv4_decode: null args");
+    DecodeParams p;
+    memset(&p, 0, sizeof(p));
+    if (int rc = read_cache("kv4_decode", a->cache, &p.c)) return rc;
+    if (int rc = read_seqs("kv4_decode", a->seqs, &p.s)) return rc;
+    if (a->q_dtype != OMMX_DT_BF16 && a->q_dtype != OMMX_DT_F16) return fail(OMMX_E_UNSUPPORTED, "kv4_decode: q must be bfloat16 or float16");
+    if (a->o_dtype != OMMX_DT_F32 && a->o_dtype != OMMX_DT_BF16 && a->o_dtype != OMMX_DT_F16) return fail(OMMX_E_ARG, "kv4_decode: o dtype %d", a->o_dtype);
+    if (a->n_q_heads < p.c.H || a->n_q_heads % p.c.H)
+        return fail(OMMX_E_UNSUPPORTED, "kv4_decode: %d query heads are not a multiple of %d kv heads", a->n_q_heads, p.c.H);
+    if (!(a->logit_cap >= 0.0f)) return fail(OMMX_E_ARG, "kv4_decode: logit_cap must not be negative");
+    if (a->selected && a->num_selected < 0) return fail(OMMX_E_ARG, "kv4_decode: num_selected must not be negative");
+    if (p.s.B > 65535) return fail(OMMX_E_UNSUPPORTED, "kv4_decode: a batch of %d", p.s.B);
+    if (p.s.B == 0) return 0;
+    if (!a->q || !a->o || !a->lse) return fail(OMMX_E_ARG, "kv4_decode: q, o and lse must not be null");
+    if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 || a->workspace_floats < workspace_floats(a->cache.head_dim))
+        return fail(OMMX_E_ARG, "kv4_decode: workspace must be 16-byte aligned and hold %lld floats", (long long)workspace_floats(a->cache.head_dim));
+    p.q = a->q; p.q16 = a->q_dtype == OMMX_DT_F16; p.q_b = a->q_stride_b; p.q_h = a->q_stride_h;
+    p.o = a->o; p.o_type = a->o_dtype; p.o_b = a->o_stride_b; p.o_h = a->o_stride_h;
+    p.lse = a->lse; p.lse_b = a->lse_stride_b;
+    p.work = a->workspace;
+    p.selected = a->selected; p.num_selected = a->num_selected;
+    p.Hq = a->n_q_heads; p.group = a->n_q_heads / p.c.H; p.col_blocks = (p.group + COLS - 1) / COLS;
+    p.page_shift = shift_of(p.c.page);
+    p.sm_scale = a->sm_scale; p.cap = a->logit_cap; p.status = a->status;
+    p.least = NW;
+    // as many blocks as the SMs hold, no more than the work can have
+    int64_t tiles = (int64_t)p.s.max_pages * p.c.parts;
+    if (a->max_seq_len > 0) tiles = tiles < (a->max_seq_len + 15LL) / 16 ? tiles : (a->max_seq_len + 15LL) / 16;
+    if (p.selected) tiles = tiles < (int64_t)p.num_selected * p.c.parts ? tiles : (int64_t)p.num_selected * p.c.parts;
+    const int64_t most = (tiles * p.s.B * p.c.H * p.col_blocks + p.least - 1) / p.least, hold = (int64_t)BLOCKS_PER_SM * sm_count();
+    const int64_t blocks = most < 1 ? 1 : most < hold ? most : hold;
+    return a->cache.head_dim == 64 ? launch_decode<2>(p, blocks, st) : launch_decode<4>(p, blocks, st);
+}
+
+}  // namespace kv4
+}  // namespace ommx
+
+extern "C" int64_t ommx_b200_kv4_workspace_floats(int32_t head_dim) { return head_dim == 64 || head_dim == 128 ? ommx::kv4::workspace_floats(head_dim) : 0; }
+extern "C" int ommx_b200_kv4_decode(const ommx_kv4_decode_args *args, void *stream) { return ommx::kv4::decode(args, (cudaStream_t)stream); }
