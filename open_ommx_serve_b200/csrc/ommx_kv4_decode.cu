@@ -9,15 +9,18 @@
 // are fp32 multiply-adds. Queries keep all their bits: a head's are scaled by a power of two into fp16's range.
 //
 // Weights p_t s_tj are rounded to fp16 (2^-12 of each, of either sign): against the running reference r, which covers the logit and
-// the scale, they are 2^12 at most, and those below 2^-36 of the largest are lost. Sums of weights and zeros stay fp32.
+// the scale, they are 2^12 at most, and those below 2^-36 of the largest are lost. That is an eighth of a bf16 output's own
+// rounding; where the output is finer (fp16, fp32), a second product takes what the rounding left (FINE). Sums of weights and
+// zeros stay fp32.
 #include "ommx_kv4.cuh"
 
 namespace ommx {
 namespace kv4 {
 
-constexpr int NW = 4;                             // warps to a block, each with tiles of 16 tokens of its own
+constexpr int NW = 8;                             // warps to a block, each with tiles of 16 tokens of its own
+constexpr int STAGES = 4;                         // records that a warp has on their way
 constexpr int COLS = 8;                           // query heads side by side
-constexpr int BLOCKS_PER_SM = 4;
+constexpr int BLOCKS_PER_SM = 2;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float ROOM = 4096.0f;                   // how large a weight may get before its reference moves
 constexpr float LOWEST = -1e30f;
@@ -30,7 +33,7 @@ struct DecodeParams {
     float *lse, *work;
     const int32_t *selected;
     int64_t q_b, q_h, o_b, o_h, lse_b;
-    int32_t q16, o_type, Hq, group, col_blocks, num_selected, page_shift, least;
+    int32_t q16, q_wide, o_type, Hq, group, col_blocks, num_selected, page_shift, least;
     float sm_scale, cap;
     int32_t *status;
 };
@@ -68,6 +71,40 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// two fp32 numbers in a register pair
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -82,14 +119,23 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
+__device__ __forceinline__ float2 half2_floats(uint32_t b) { return __half22float2(*reinterpret_cast<const __half2 *>(&b)); }
 __device__ __forceinline__ float scale_of(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 __device__ __forceinline__ float zero_of(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23 & 255u) - 127; }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 
-__device__ __forceinline__ float load_q(const DecodeParams &p, int64_t at) {
-    if (p.q16) return __half2float(reinterpret_cast<const __half *>(p.q)[at]);
-    return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p.q)[at]);
+// eight channels of a query
+__device__ __forceinline__ void load_q8(const DecodeParams &p, int64_t at, float *x) {
+    alignas(16) uint16_t v[8];
+    if (p.q_wide) {
+        *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p.q) + at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = reinterpret_cast<const uint16_t *>(p.q)[at + i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p.q16 ? __half2float(__ushort_as_half(v[i])) : __uint_as_float((uint32_t)v[i] << 16);
 }
 __device__ __forceinline__ void store_o(const DecodeParams &p, int64_t at, float v) {
     if (p.o_type == OMMX_DT_F32) reinterpret_cast<float *>(p.o)[at] = v;
@@ -98,21 +144,21 @@ __device__ __forceinline__ void store_o(const DecodeParams &p, int64_t at, float
 }
 
 // A kv head's queries as B fragments. Lane (g, t): head g, channels 32 j + 8 t + 0..7; frag[j][k] holds the channels (0, 4), (1, 5),
-// (2, 6), (3, 7); the second and fourth meet nibbles that are 16 times as large. sums: of two heads' (2 t, 2 t + 1) groups.
+// (2, 6), (3, 7); the second and fourth meet nibbles that are 16 times as large. What meets the zeros is the sum of a group's
+// channels: three bf16 numbers add up to it, so that one bf16 product of the zeros, as they are stored, and them is exact.
 template <int G> struct Query {
-    uint32_t frag[G][4];
-    float sums[G][2], factor[2];                  // in the products' units; what turns those into log2 units
+    uint32_t frag[G][4], sums[2];
+    float factor[2];                              // of heads 2 t and 2 t + 1: what turns the products' units into log2 units
 };
 template <int G> __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int first_head, int n, int lane, Query<G> &q) {
     const int g = lane >> 2, t = lane & 3;
     float x[G][8], top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < G; ++j)
+    for (int j = 0; j < G; ++j) {
+        load_q8(p, b * p.q_b + (first_head + min(g, n - 1)) * p.q_h + 32 * j + 8 * t, x[j]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[j][i] = g < n ? load_q(p, b * p.q_b + (first_head + g) * p.q_h + 32 * j + 8 * t + i) : 0.0f;
-            top = fmaxf(top, fabsf(x[j][i]));
-        }
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[j][i]));
+    }
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
     const int e = top > 0.0f ? max(exponent_of(top), -100) : 0;
@@ -120,6 +166,7 @@ template <int G> __device__ __forceinline__ void load_query(const DecodeParams &
     const float factor = p.sm_scale * power_of_two(24 - 13 + e) * (p.cap > 0.0f ? 1.0f : LOG2E);
     q.factor[0] = __shfl_sync(~0u, factor, 8 * t);
     q.factor[1] = __shfl_sync(~0u, factor, 8 * t + 4);
+    float sums[G];
 #pragma unroll
     for (int j = 0; j < G; ++j) {
         float sum = 0.0f;
@@ -127,20 +174,32 @@ template <int G> __device__ __forceinline__ void load_query(const DecodeParams &
         for (int i = 0; i < 8; ++i) { x[j][i] *= up; sum += x[j][i]; }
         sum += __shfl_xor_sync(~0u, sum, 1);
         sum += __shfl_xor_sync(~0u, sum, 2);
-        sum *= 0x1p-24f;
-        q.sums[j][0] = __shfl_sync(~0u, sum, 8 * t);
-        q.sums[j][1] = __shfl_sync(~0u, sum, 8 * t + 4);
+        sums[j] = sum * 0x1p-24f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float f = k & 1 ? 0.0625f : 1.0f;
             q.frag[j][k] = half2_bits(x[j][k] * f, x[j][k + 4] * f);
         }
     }
+    // rows of the product: term r of group j at G r + j; lane t holds rows 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
+    const float a = G == 4 && (t & 1) ? sums[G - 2] : sums[0], b2 = G == 4 && (t & 1) ? sums[G - 1] : sums[1];
+    const float a1 = bf16_round_f32(a), b1 = bf16_round_f32(b2), a2 = bf16_round_f32(a - a1), b2r = bf16_round_f32(b2 - b1);
+    const uint32_t terms[4] = {f32_to_bf16_bits(a1) | f32_to_bf16_bits(b1) << 16, f32_to_bf16_bits(a2) | f32_to_bf16_bits(b2r) << 16,
+                               f32_to_bf16_bits(a - a1 - a2) | f32_to_bf16_bits(b2 - b1 - b2r) << 16, 0u};
+    if constexpr (G == 4) {
+        q.sums[0] = t < 2 ? terms[0] : terms[1];
+        q.sums[1] = t < 2 ? terms[2] : 0u;
+    } else {
+        q.sums[0] = t == 0 ? terms[0] : t == 1 ? terms[1] : t == 2 ? terms[2] : 0u;
+        q.sums[1] = 0u;
+    }
 }
 
 // A warp's running state. acc[j][u]: channels 32 j + 4 g + 2 u (rows g) and + 1 (rows g + 8, 16 times too large), heads 2 t, 2 t + 1.
+// zero[i][e]: what the zeros of groups 2 i and 2 i + 1 add, head 2 t + e.
 template <int G> struct State {
-    float acc[G][2][4], zero[G][2], sum[2], ref[2];
+    float acc[G][2][4], sum[2], ref[2];
+    uint64_t zero[G / 2][2];
 };
 
 template <int G> __device__ __forceinline__ void clear(State<G> &s) {
@@ -150,7 +209,7 @@ template <int G> __device__ __forceinline__ void clear(State<G> &s) {
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s.acc[j][u][i] = 0.0f;
-        s.zero[j][0] = s.zero[j][1] = 0.0f;
+        s.zero[j / 2][j & 1] = 0;
     }
     s.sum[0] = s.sum[1] = 0.0f;
     s.ref[0] = s.ref[1] = LOWEST;
@@ -160,46 +219,67 @@ template <int G> __device__ __forceinline__ void rescale(State<G> &s, float f0, 
     for (int j = 0; j < G; ++j) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) { s.acc[j][u][0] *= f0; s.acc[j][u][1] *= f1; s.acc[j][u][2] *= f0; s.acc[j][u][3] *= f1; }
-        s.zero[j][0] *= f0; s.zero[j][1] *= f1;
+        s.zero[j / 2][j & 1] = mul2(s.zero[j / 2][j & 1], j & 1 ? pair(f1, f1) : pair(f0, f0));
     }
     s.sum[0] *= f0; s.sum[1] *= f1;
 }
 
-// One record, n of its tokens valid (1..16)
-template <int G> __device__ __forceinline__ void attend(const DecodeParams &p, const uint8_t *rec, int n, int lane, const Query<G> &q, State<G> &s) {
+// ---- a warp's ring of records: one bulk copy each, completion counted by an mbarrier to a slot ----
+constexpr int MOST_TRIES = 1 << 20;               // of a wait; each sleeps for a while by itself
+__device__ __forceinline__ void send_record(uint32_t to, uint32_t barrier, const uint8_t *rec, int bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(rec ? bytes : 0) : "memory");
+    if (rec)
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(to), "l"(rec), "r"(bytes), "r"(barrier) : "memory");
+}
+__device__ __forceinline__ bool arrived(uint32_t barrier, uint32_t parity) {
+    for (int i = 0; i < MOST_TRIES; ++i) {
+        uint32_t done;
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                     : "=r"(done) : "r"(barrier), "r"(parity) : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+
+// One record in shared memory, n of its tokens valid (1..16)
+template <int G, bool FINE> __device__ __forceinline__ void attend(const DecodeParams &p, const uint8_t *rec, int n, int lane, const Query<G> &q, State<G> &s) {
     using W = typename Words<G>::T;
     const int g = lane >> 2;
     constexpr uint32_t LO = 0x000F000Fu, HI = 0x00F000F0u;
-    alignas(16) uint32_t k0[G], k1[G], v0[G], v1[G], kp0[G], kp1[G], vp0[G], vp1[G];
+    alignas(16) uint32_t k0[G], k1[G], kp0[G], kp1[G], vp0[G], vp1[G];
     *reinterpret_cast<W *>(k0) = reinterpret_cast<const W *>(rec)[lane];
     *reinterpret_cast<W *>(k1) = reinterpret_cast<const W *>(rec)[32 + lane];
     *reinterpret_cast<W *>(kp0) = reinterpret_cast<const W *>(rec + Rec<G>::KP)[g];
     *reinterpret_cast<W *>(kp1) = reinterpret_cast<const W *>(rec + Rec<G>::KP)[g + 8];
-    *reinterpret_cast<W *>(v0) = reinterpret_cast<const W *>(rec + Rec<G>::V)[lane];
-    *reinterpret_cast<W *>(v1) = reinterpret_cast<const W *>(rec + Rec<G>::V)[32 + lane];
     *reinterpret_cast<W *>(vp0) = reinterpret_cast<const W *>(rec + Rec<G>::VP)[g];
     *reinterpret_cast<W *>(vp1) = reinterpret_cast<const W *>(rec + Rec<G>::VP)[g + 8];
 
     // ---- logits: x[0], x[1] of token g and heads 2 t, 2 t + 1; x[2], x[3] of token g + 8
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float x[4];
+    {
+        const bool up = G == 4 && (lane & 1);
+        const uint32_t z0 = __byte_perm(up ? kp0[G - 2] : kp0[0], up ? kp0[G - 1] : kp0[1], 0x5410);
+        const uint32_t z1 = __byte_perm(up ? kp1[G - 2] : kp1[0], up ? kp1[G - 1] : kp1[1], 0x5410);
+        mma_bf16(x, z0, z1, z0, z1, q.sums[0], q.sums[1]);
+    }
 #pragma unroll
     for (int j = 0; j < G; ++j) {
-        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        mma(c, k0[j] & LO, k1[j] & LO, k0[j] & HI, k1[j] & HI, q.frag[j][0], q.frag[j][1]);
+        float c[4];
+        mma_first(c, k0[j] & LO, k1[j] & LO, k0[j] & HI, k1[j] & HI, q.frag[j][0], q.frag[j][1]);
         const uint32_t a = k0[j] >> 8, b = k1[j] >> 8;
         mma(c, a & LO, b & LO, a & HI, b & HI, q.frag[j][2], q.frag[j][3]);
-        const float s0 = scale_of(kp0[j]), s1 = scale_of(kp1[j]), z0 = zero_of(kp0[j]), z1 = zero_of(kp1[j]);
-        x[0] = fmaf(z0, q.sums[j][0], fmaf(s0, c[0], x[0]));
-        x[1] = fmaf(z0, q.sums[j][1], fmaf(s0, c[1], x[1]));
-        x[2] = fmaf(z1, q.sums[j][0], fmaf(s1, c[2], x[2]));
-        x[3] = fmaf(z1, q.sums[j][1], fmaf(s1, c[3], x[3]));
+        const float s0 = scale_of(kp0[j]), s1 = scale_of(kp1[j]);
+        x[0] = fmaf(s0, c[0], x[0]);
+        x[1] = fmaf(s0, c[1], x[1]);
+        x[2] = fmaf(s1, c[2], x[2]);
+        x[3] = fmaf(s1, c[3], x[3]);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] *= q.factor[i & 1];
     if (p.cap > 0.0f) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = p.cap * LOG2E * tanhf(x[i] / p.cap);
+        for (int i = 0; i < 4; ++i) x[i] = p.cap * tanhf(x[i] * q.factor[i & 1] / p.cap);
     }
+    const float f0 = p.cap > 0.0f ? LOG2E : q.factor[0], f1 = p.cap > 0.0f ? LOG2E : q.factor[1];   // x f: logits in powers of two
     if (n < 16) {                                 // what lies behind the last token may be anything
         if (g >= n) {
             x[0] = x[1] = -INFINITY;
@@ -214,18 +294,21 @@ template <int G> __device__ __forceinline__ void attend(const DecodeParams &p, c
     }
 
     // ---- weights
-    float top0 = scale_of(vp0[0]), top1 = scale_of(vp1[0]);
+    // the largest scale of each token; a word taken as a number is its scale and less than a hundredth of it more
+    float top0 = 0x1p-30f, top1 = 0x1p-30f;
 #pragma unroll
-    for (int j = 1; j < G; ++j) { top0 = fmaxf(top0, scale_of(vp0[j])); top1 = fmaxf(top1, scale_of(vp1[j])); }
-    top0 = fmaxf(top0, 0x1p-30f);
-    top1 = fmaxf(top1, 0x1p-30f);
+    for (int j = 0; j < G; j += 2) {
+        top0 = max3(top0, __uint_as_float(vp0[j]), __uint_as_float(vp0[j + 1]));
+        top1 = max3(top1, __uint_as_float(vp1[j]), __uint_as_float(vp1[j + 1]));
+    }
     float w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = exp2_approx(x[i] - s.ref[i & 1]);
+    for (int i = 0; i < 4; ++i) w[i] = exp2_approx(fmaf(x[i], i & 1 ? f1 : f0, -s.ref[i & 1]));
     const float most = fmaxf(fmaxf(w[0], w[1]) * top0, fmaxf(w[2], w[3]) * top1);
     if (__any_sync(~0u, !(most <= ROOM))) {
         // the references move to the largest logit plus exponent of its scales
-        float r0 = fmaxf(x[0] + (exponent_of(top0) + 1), x[2] + (exponent_of(top1) + 1)), r1 = fmaxf(x[1] + (exponent_of(top0) + 1), x[3] + (exponent_of(top1) + 1));
+        const float e0 = (float)(exponent_of(top0) + 1), e1 = (float)(exponent_of(top1) + 1);
+        float r0 = fmaxf(fmaf(x[0], f0, e0), fmaf(x[2], f0, e1)), r1 = fmaxf(fmaf(x[1], f1, e0), fmaf(x[3], f1, e1));
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) {
             r0 = fmaxf(r0, __shfl_xor_sync(~0u, r0, d));
@@ -237,21 +320,37 @@ template <int G> __device__ __forceinline__ void attend(const DecodeParams &p, c
         s.ref[0] = r0;
         s.ref[1] = r1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = exp2_approx(x[i] - s.ref[i & 1]);
+        for (int i = 0; i < 4; ++i) w[i] = exp2_approx(fmaf(x[i], i & 1 ? f1 : f0, -s.ref[i & 1]));
     }
     s.sum[0] += w[0] + w[2];
     s.sum[1] += w[1] + w[3];
 
     // ---- values
+    alignas(16) uint32_t v0[G], v1[G];
+    *reinterpret_cast<W *>(v0) = reinterpret_cast<const W *>(rec + Rec<G>::V)[lane];
+    *reinterpret_cast<W *>(v1) = reinterpret_cast<const W *>(rec + Rec<G>::V)[32 + lane];
+    const uint64_t ww[4] = {pair(w[0], w[0]), pair(w[1], w[1]), pair(w[2], w[2]), pair(w[3], w[3])};
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-        const float s0 = scale_of(vp0[j]), s1 = scale_of(vp1[j]), z0 = zero_of(vp0[j]), z1 = zero_of(vp1[j]);
-        s.zero[j][0] = fmaf(z1, w[2], fmaf(z0, w[0], s.zero[j][0]));
-        s.zero[j][1] = fmaf(z1, w[3], fmaf(z0, w[1], s.zero[j][1]));
-        const uint32_t b0 = transpose8x8(half2_bits(w[0] * s0, w[1] * s0)), b1 = transpose8x8(half2_bits(w[2] * s1, w[3] * s1));
+    for (int j2 = 0; j2 < G; j2 += 2) {
+    const uint64_t s0 = pair(scale_of(vp0[j2]), scale_of(vp0[j2 + 1])), s1 = pair(scale_of(vp1[j2]), scale_of(vp1[j2 + 1]));
+    const uint64_t z0 = pair(zero_of(vp0[j2]), zero_of(vp0[j2 + 1])), z1 = pair(zero_of(vp1[j2]), zero_of(vp1[j2 + 1]));
+    s.zero[j2 / 2][0] = fma2(z1, ww[2], fma2(z0, ww[0], s.zero[j2 / 2][0]));
+    s.zero[j2 / 2][1] = fma2(z1, ww[3], fma2(z0, ww[1], s.zero[j2 / 2][1]));
+    const float2 y2[4] = {unpair(mul2(ww[0], s0)), unpair(mul2(ww[1], s0)), unpair(mul2(ww[2], s1)), unpair(mul2(ww[3], s1))};
+#pragma unroll
+    for (int j = j2; j < j2 + 2; ++j) {
+        const float y[4] = {j & 1 ? y2[0].y : y2[0].x, j & 1 ? y2[1].y : y2[1].x, j & 1 ? y2[2].y : y2[2].x, j & 1 ? y2[3].y : y2[3].x};
+        const uint32_t h0 = half2_bits(y[0], y[1]), h1 = half2_bits(y[2], y[3]), a = v0[j] >> 8, b = v1[j] >> 8;
+        const uint32_t b0 = transpose8x8(h0), b1 = transpose8x8(h1);
         mma(s.acc[j][0], v0[j] & LO, v0[j] & HI, v1[j] & LO, v1[j] & HI, b0, b1);
-        const uint32_t a = v0[j] >> 8, b = v1[j] >> 8;
         mma(s.acc[j][1], a & LO, a & HI, b & LO, b & HI, b0, b1);
+        if constexpr (FINE) {
+            const float2 r0 = half2_floats(h0), r1 = half2_floats(h1);
+            const uint32_t d0 = transpose8x8(half2_bits(y[0] - r0.x, y[1] - r0.y)), d1 = transpose8x8(half2_bits(y[2] - r1.x, y[3] - r1.y));
+            mma(s.acc[j][0], v0[j] & LO, v0[j] & HI, v1[j] & LO, v1[j] & HI, d0, d1);
+            mma(s.acc[j][1], a & LO, a & HI, b & LO, b & HI, d0, d1);
+        }
+    }
     }
 }
 
@@ -266,6 +365,11 @@ template <int G>
 __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Shared<G> &sh, int b, int first_head, int n, float *part, int warp, int lane) {
     constexpr int D = 32 * G;
     const int g = lane >> 2, t = lane & 3;
+    float zero[G][2];
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) zero[j][i] = j & 1 ? unpair(s.zero[j / 2][i]).y : unpair(s.zero[j / 2][i]).x;
 #pragma unroll
     for (int d = 4; d < 32; d *= 2) {
 #pragma unroll
@@ -273,7 +377,7 @@ __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Share
 #pragma unroll
         for (int j = 0; j < G; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) s.zero[j][i] += __shfl_xor_sync(~0u, s.zero[j][i], d);
+            for (int i = 0; i < 2; ++i) zero[j][i] += __shfl_xor_sync(~0u, zero[j][i], d);
     }
     if (g == 0) {
 #pragma unroll
@@ -295,7 +399,7 @@ __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Share
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 sh.o[warp][2 * t + (i & 1)][32 * j + 4 * g + 2 * u + (i >> 1)] =
-                    f[i & 1] * fmaf(s.acc[j][u][i], i < 2 ? 0x1p24f : 0x1p20f, s.zero[j][i & 1]);
+                    f[i & 1] * fmaf(s.acc[j][u][i], i < 2 ? 0x1p24f : 0x1p20f, zero[j][i & 1]);
     __syncthreads();
     for (int i = threadIdx.x; i < COLS * D; i += 32 * NW) {
         const int h = i / D, c = i % D;
@@ -312,12 +416,31 @@ __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Share
             if (c == 0) p.lse[b * p.lse_b + first_head + h] = sum != 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
         }
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");            // what lay here, before the next row's copies
     __syncthreads();
 }
 
-template <int G> __global__ void __launch_bounds__(32 * NW, BLOCKS_PER_SM) kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
-    __shared__ Shared<G> sh;
+template <int G> struct Memory {
+    union {
+        Shared<G> sh;
+        alignas(128) uint8_t ring[NW][STAGES][Rec<G>::BYTES];
+    };
+    uint64_t barriers[NW][STAGES];
+};
+template <int G> struct Floats;
+template <> struct Floats<2> { using T = float2; };
+template <> struct Floats<4> { using T = float4; };
+
+template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PER_SM) kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
+    extern __shared__ __align__(128) uint8_t memory[];
+    Memory<G> &m = *reinterpret_cast<Memory<G> *>(memory);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint8_t *ring = m.ring[warp][0];
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), barriers = (uint32_t)__cvta_generic_to_shared(m.barriers[warp]);
+    if (lane < STAGES) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(barriers + 8 * lane) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
+    uint32_t sent = 0, taken = 0;                 // records since the start
     wait_earlier();
     let_next_in();
     const int rows = p.c.H * p.col_blocks;
@@ -351,37 +474,70 @@ template <int G> __global__ void __launch_bounds__(32 * NW, BLOCKS_PER_SM) kv4_d
         const int row = (int)((u - base) / tiles), i0 = (int)(u - base - (int64_t)row * tiles), i1 = (int)min((int64_t)tiles, i0 + (end - u));
         const int head = row / p.col_blocks, cb = row % p.col_blocks;
         const int first_head = head * p.group + cb * COLS, n = min(COLS, p.group - cb * COLS);
+        const int32_t *sel = p.selected ? p.selected + ((int64_t)b * p.c.H + head) * p.num_selected : nullptr;
+        // the records of 32 of the warp's tiles at a time are looked up by a lane each: address and tokens (0: none)
+        const int mine = (i1 - i0 - warp + NW - 1) / NW;
+        const uint8_t *rec = nullptr;
+        int valid = 0;
+        auto look_up = [&](int k) {
+            const int i = i0 + warp + (k + lane) * NW, slot = i / p.c.parts, part = i - slot * p.c.parts;
+            rec = nullptr;
+            valid = 0;
+            if (i >= i1) return;
+            const int place = sel ? sel[slot] : slot;
+            const int64_t first = ((int64_t)place << p.page_shift) + 16 * part;
+            if (place < 0 || first >= len) return;
+            const int64_t id = page_id(p.s, b, place);
+            if (id < 0 || id >= p.c.num_pages) { or_status(p.status, OMMX_ST_BAD_PAGE); return; }
+            rec = p.c.records + ((id * p.c.H + head) * p.c.parts + part) * Rec<G>::BYTES;
+            valid = (int)min((int64_t)16, len - first);
+        };
+        // tile k is sent STAGES - 1 tiles ahead, by the lane that looked it up
+        uint32_t counts = 0;                          // tokens of the tiles on their way, eight bits each, the next one lowest
+        auto send = [&](int k) {
+            if (k < mine) {
+                if ((k & 31) == 0) look_up(k);
+                const uint32_t slot = sent++ % STAGES;
+                if (lane == (k & 31)) send_record(ring_at + slot * Rec<G>::BYTES, barriers + 8 * slot, rec, Rec<G>::BYTES);
+                counts = counts >> 8 | (uint32_t)__shfl_sync(~0u, valid, k & 31) << (8 * (STAGES - 1));
+            } else {
+                counts >>= 8;
+            }
+        };
+#pragma unroll
+        for (int k = 0; k < STAGES - 1; ++k) send(k);
         Query<G> q;
         State<G> s;
         load_query<G>(p, b, first_head, n, lane, q);
         clear(s);
-        const int32_t *sel = p.selected ? p.selected + ((int64_t)b * p.c.H + head) * p.num_selected : nullptr;
-        for (int i = i0 + warp; i < i1; i += NW) {
-            const int slot = i / p.c.parts, part = i - slot * p.c.parts, place = sel ? sel[slot] : slot;
-            const int64_t first = ((int64_t)place << p.page_shift) + 16 * part;
-            if (place < 0 || first >= len) continue;
-            const int64_t id = page_id(p.s, b, place);
-            if (id < 0 || id >= p.c.num_pages) { or_status(p.status, OMMX_ST_BAD_PAGE); continue; }
-            attend<G>(p, p.c.records + ((id * p.c.H + head) * p.c.parts + part) * Rec<G>::BYTES, (int)min((int64_t)16, len - first), lane, q, s);
+        for (int k = 0; k < mine; ++k) {
+            send(k + STAGES - 1);
+            const int n = counts & 255u;
+            const uint32_t slot = taken % STAGES;
+            const bool here = arrived(barriers + 8 * slot, taken++ / STAGES & 1);
+            if (!here) or_status(p.status, OMMX_ST_TIMEOUT);
+            if (n && here) attend<G, FINE>(p, ring + slot * Rec<G>::BYTES, n, lane, q, s);
+            __syncwarp();                             // before the slot is filled again
         }
+        __syncthreads();                              // the ring is the merge's memory too
         float *part = nullptr;
         if (i0 > 0 || i1 < tiles) part = p.work + (2 * (int64_t)blockIdx.x + (base + (int64_t)row * tiles >= start)) * Shared<G>::PART;
-        finish<G>(p, s, sh, b, first_head, n, part, warp, lane);
+        finish<G>(p, s, m.sh, b, first_head, n, part, warp, lane);
         u += i1 - i0;
     }
 }
 
-// Rows of which several blocks have a part, and those of no tokens. Grid: (rows of a sequence x COLS, sequences); a warp takes every
-// fourth part, a lane four (two) channels.
-template <int G> __global__ void __launch_bounds__(128) kv4_combine_kernel(const __grid_constant__ DecodeParams p, int blocks) {
+// Rows of which several blocks have a part, and those of no tokens. Grid: (rows of a sequence x COLS, sequences). The references and
+// sums of all parts are read at once; then a warp takes every CW-th part, a lane G channels, UNROLL parts on their way.
+// The lengths are read before the wait: this kernel starts when every block of the one before has waited for what came earlier.
+constexpr int CW = 8, UNROLL = 5, MOST_PARTS = 512;
+template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_kernel(const __grid_constant__ DecodeParams p, int blocks) {
     constexpr int D = 32 * G;
-    __shared__ float so[4][D], sr[4], ss[4];
+    using V = typename Floats<G>::T;
+    __shared__ float so[CW][D], weight[MOST_PARTS], sr[CW], ss[CW];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int b = blockIdx.y, row = blockIdx.x / COLS, h = blockIdx.x % COLS;
     const int head = row / p.col_blocks, cb = row % p.col_blocks, hq = head * p.group + cb * COLS + h;
-    wait_earlier();
-    let_next_in();
-    if (h >= p.group - cb * COLS) return;
     const int rows = p.c.H * p.col_blocks;
     const Shares sh = shares(p, rows, blocks, lane);
     int64_t before = 0;
@@ -389,55 +545,92 @@ template <int G> __global__ void __launch_bounds__(128) kv4_combine_kernel(const
 #pragma unroll
     for (int d = 16; d; d /= 2) before += __shfl_xor_sync(~0u, before, d);
     const int tiles = tiles_of(p, length_of(p, b));
-    if (tiles == 0) {
-        for (int c = threadIdx.x; c < D; c += 128) store_o(p, b * p.o_b + hq * p.o_h + c, 0.0f);
+    const int64_t r0 = before * rows + (int64_t)row * tiles, r1 = r0 + tiles;
+    const int c0 = (int)(r0 / sh.per), n = tiles ? (int)((r1 - 1) / sh.per) - c0 + 1 : 0;
+    const bool late = r0 >= c0 * sh.per;          // the row begins in block c0: its part there is the second one
+    wait_earlier();
+    let_next_in();
+    if (h >= p.group - cb * COLS || n == 1) return;                         // not a head, or finished where it was computed
+    if (n == 0) {
+        for (int c = threadIdx.x; c < D; c += 32 * CW) store_o(p, b * p.o_b + hq * p.o_h + c, 0.0f);
         if (threadIdx.x == 0) p.lse[b * p.lse_b + hq] = -INFINITY;
         return;
     }
-    const int64_t r0 = before * rows + (int64_t)row * tiles, r1 = r0 + tiles;
-    const int64_t c0 = r0 / sh.per, c1 = (r1 - 1) / sh.per;
-    if (c0 == c1) return;                         // finished where it was computed
-    float top = LOWEST, sum = 0.0f, o[G];
+    auto part = [&](int i) { return p.work + (int64_t)(2 * (c0 + i) + (i == 0 && late)) * Shared<G>::PART; };
+    float top = LOWEST, sum = 0.0f;
+    for (int i = threadIdx.x; i < n; i += 32 * CW) {
+        const float r = part(i)[COLS * D + h], s = part(i)[COLS * D + COLS + h], m = fmaxf(top, r);
+        weight[i] = r;
+        sum = fmaf(s, exp2_approx(r - m), sum * exp2_approx(top - m));
+        top = m;
+    }
+    V v[UNROLL];
+    auto load = [&](int i0) {
 #pragma unroll
-    for (int i = 0; i < G; ++i) o[i] = 0.0f;
-    for (int64_t c = c0 + warp; c <= c1; c += 4) {
-        const float *part = p.work + (2 * c + (r0 >= c * sh.per)) * Shared<G>::PART;
-        const float ref = part[COLS * D + h], add = part[COLS * D + COLS + h], r = fmaxf(top, ref);
-        const float keep = exp2_approx(top - r), take = exp2_approx(ref - r);
-        const float *v = part + h * D + lane * G;
+        for (int u = 0; u < UNROLL; ++u)
+            if (i0 + u * CW < n) v[u] = reinterpret_cast<const V *>(part(i0 + u * CW) + h * D)[lane];
+    };
+    load(warp);                                   // on their way while the references meet
 #pragma unroll
-        for (int i = 0; i < G; ++i) o[i] = fmaf(v[i], take, o[i] * keep);
-        sum = fmaf(add, take, sum * keep);
-        top = r;
+    for (int d = 16; d; d /= 2) {
+        const float r = __shfl_xor_sync(~0u, top, d), s = __shfl_xor_sync(~0u, sum, d), m = fmaxf(top, r);
+        sum = fmaf(s, exp2_approx(r - m), sum * exp2_approx(top - m));
+        top = m;
     }
     if (lane == 0) { sr[warp] = top; ss[warp] = sum; }
+    __syncthreads();
+    top = sr[0];
+#pragma unroll
+    for (int w = 1; w < CW; ++w) top = fmaxf(top, sr[w]);
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < CW; ++w) sum = fmaf(ss[w], exp2_approx(sr[w] - top), sum);
+    float o[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) o[i] = 0.0f;
+    for (int i0 = warp; i0 < n; i0 += CW * UNROLL) {
+        if (i0 != warp) load(i0);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+            if (i0 + u * CW < n) {
+                const float f = exp2_approx(weight[i0 + u * CW] - top);
+                const float *x = reinterpret_cast<const float *>(&v[u]);
+#pragma unroll
+                for (int i = 0; i < G; ++i) o[i] = fmaf(x[i], f, o[i]);
+            }
+    }
 #pragma unroll
     for (int i = 0; i < G; ++i) so[warp][lane * G + i] = o[i];
     __syncthreads();
-    float r = sr[0];
+    for (int c = threadIdx.x; c < D; c += 32 * CW) {
+        float x = 0.0f;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) r = fmaxf(r, sr[w]);
-    sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) sum += ss[w] * exp2_approx(sr[w] - r);
-    for (int c = threadIdx.x; c < D; c += 128) {
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) v = fmaf(so[w][c], exp2_approx(sr[w] - r), v);
-        store_o(p, b * p.o_b + hq * p.o_h + c, sum != 0.0f ? v / sum : 0.0f);
+        for (int w = 0; w < CW; ++w) x += so[w][c];
+        store_o(p, b * p.o_b + hq * p.o_h + c, sum != 0.0f ? x / sum : 0.0f);
     }
-    if (threadIdx.x == 0) p.lse[b * p.lse_b + hq] = sum != 0.0f ? (r + log2f(sum)) * LN2 : -INFINITY;
+    if (threadIdx.x == 0) p.lse[b * p.lse_b + hq] = sum != 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
 }
 
 // ---- host ---------------------------------------------------------------------------------------
+static int64_t most_blocks() {
+    const int n = BLOCKS_PER_SM * sm_count();
+    return n < MOST_PARTS ? n : MOST_PARTS;
+}
 static int64_t workspace_floats(int head_dim) {
     const int64_t part = head_dim == 64 ? Shared<2>::PART : Shared<4>::PART;
-    return 2 * part * BLOCKS_PER_SM * sm_count();
+    return 2 * part * most_blocks();
 }
 
-template <int G> static int launch_decode(const DecodeParams &p, int64_t blocks, cudaStream_t st) {
-    if (int rc = launch_dependent(kv4_decode_kernel<G>, dim3((unsigned)blocks), 32 * NW, 0, st, p)) return rc;
-    return launch_dependent(kv4_combine_kernel<G>, dim3(p.c.H * p.col_blocks * COLS, p.s.B), 128, 0, st, p, (int)blocks);
+template <int G, bool FINE> static int launch_decode(const DecodeParams &p, int64_t blocks, cudaStream_t st) {
+    static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may take its shared memory
+    int dev = 0;
+    if (int rc = current_device(&dev)) return rc;
+    if (!(allowed.load(std::memory_order_acquire) >> dev & 1)) {
+        OMMX_CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<G, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Memory<G>)));
+        allowed.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    if (int rc = launch_dependent(kv4_decode_kernel<G, FINE>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G>), st, p)) return rc;
+    return launch_dependent(kv4_combine_kernel<G>, dim3(p.c.H * p.col_blocks * COLS, p.s.B), 32 * CW, 0, st, p, (int)blocks);
 }
 
 static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
@@ -458,6 +651,7 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 || a->workspace_floats < workspace_floats(a->cache.head_dim))
         return fail(OMMX_E_ARG, "kv4_decode: workspace must be 16-byte aligned and hold %lld floats", (long long)workspace_floats(a->cache.head_dim));
     p.q = a->q; p.q16 = a->q_dtype == OMMX_DT_F16; p.q_b = a->q_stride_b; p.q_h = a->q_stride_h;
+    p.q_wide = (reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)(2 * p.q_b) | (uintptr_t)(2 * p.q_h)) % 16 == 0;
     p.o = a->o; p.o_type = a->o_dtype; p.o_b = a->o_stride_b; p.o_h = a->o_stride_h;
     p.lse = a->lse; p.lse_b = a->lse_stride_b;
     p.work = a->workspace;
@@ -470,9 +664,10 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     int64_t tiles = (int64_t)p.s.max_pages * p.c.parts;
     if (a->max_seq_len > 0) tiles = tiles < (a->max_seq_len + 15LL) / 16 ? tiles : (a->max_seq_len + 15LL) / 16;
     if (p.selected) tiles = tiles < (int64_t)p.num_selected * p.c.parts ? tiles : (int64_t)p.num_selected * p.c.parts;
-    const int64_t most = (tiles * p.s.B * p.c.H * p.col_blocks + p.least - 1) / p.least, hold = (int64_t)BLOCKS_PER_SM * sm_count();
+    const int64_t most = (tiles * p.s.B * p.c.H * p.col_blocks + p.least - 1) / p.least, hold = most_blocks();
     const int64_t blocks = most < 1 ? 1 : most < hold ? most : hold;
-    return a->cache.head_dim == 64 ? launch_decode<2>(p, blocks, st) : launch_decode<4>(p, blocks, st);
+    if (a->o_dtype == OMMX_DT_BF16) return a->cache.head_dim == 64 ? launch_decode<2, false>(p, blocks, st) : launch_decode<4, false>(p, blocks, st);
+    return a->cache.head_dim == 64 ? launch_decode<2, true>(p, blocks, st) : launch_decode<4, true>(p, blocks, st);
 }
 
 }  // namespace kv4
