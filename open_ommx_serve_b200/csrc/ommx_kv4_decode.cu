@@ -5,7 +5,8 @@
 //   q.K_t = sum_j s_tj (sum_c q_c a_tc) + z_tj (sum_c q_c),      o_c = sum_t (p_t s_tj) a_tc + sum_t p_t z_tj:
 // the codes go into the tensor cores as they are. A nibble masked in place is the fp16 subnormal code * 2^-24 (or 2^-20), exact and
 // one LOP3 for two of them; the tokens (of K) and channels (of V) are the rows of an m16n8k16 product and up to eight query heads
-// that share the kv head its columns. Scales meet the sums of K's groups behind the product and the weights of V before it, zeros
+// that share the kv head its columns. Of V, one row takes two nibbles as they lie, lower + 16 upper, and another the upper one
+// alone: their difference is the lower one's, a mask saved. Scales meet the sums of K's groups behind the product and the weights of V before it, zeros
 // are fp32 multiply-adds. Queries keep all their bits: a head's are scaled by a power of two into fp16's range.
 //
 // Weights p_t s_tj are rounded to fp16 (2^-12 of each, of either sign): against the running reference r, which covers the logit and
@@ -18,7 +19,8 @@ namespace ommx {
 namespace kv4 {
 
 constexpr int NW = 8;                             // warps to a block, each with tiles of 16 tokens of its own
-constexpr int STAGES = 4;                         // records that a warp has on their way
+constexpr int STAGES = 4, AHEAD = STAGES - 1;     // records that a warp holds, and those of them on their way
+constexpr int FULL = 0x101010;                    // sixteen tokens in each of those
 constexpr int COLS = 8;                           // query heads side by side
 constexpr int BLOCKS_PER_SM = 2;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -68,37 +70,16 @@ __device__ __forceinline__ Shares shares(const DecodeParams &p, int rows, int bl
 
 // ---- pieces ---------------------------------------------------------------------------------------
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
-}
-// two fp32 numbers in a register pair
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t x) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
@@ -107,7 +88,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -148,7 +129,7 @@ __device__ __forceinline__ void store_o(const DecodeParams &p, int64_t at, float
 // channels: three bf16 numbers add up to it, so that one bf16 product of the zeros, as they are stored, and them is exact.
 template <int G> struct Query {
     uint32_t frag[G][4], sums[2];
-    float factor[2];                              // of heads 2 t and 2 t + 1: what turns the products' units into log2 units
+    float factor[2], raw[2];                      // of heads 2 t and 2 t + 1: the products' units in powers of two; with a cap: in its units
 };
 template <int G> __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int first_head, int n, int lane, Query<G> &q) {
     const int g = lane >> 2, t = lane & 3;
@@ -163,9 +144,13 @@ template <int G> __device__ __forceinline__ void load_query(const DecodeParams &
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
     const int e = top > 0.0f ? max(exponent_of(top), -100) : 0;
     const float up = power_of_two(13 - e);
-    const float factor = p.sm_scale * power_of_two(24 - 13 + e) * (p.cap > 0.0f ? 1.0f : LOG2E);
-    q.factor[0] = __shfl_sync(~0u, factor, 8 * t);
-    q.factor[1] = __shfl_sync(~0u, factor, 8 * t + 4);
+    const float factor = p.sm_scale * power_of_two(24 - 13 + e);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float f = __shfl_sync(~0u, factor, 8 * t + 4 * i);
+        q.raw[i] = f / p.cap;
+        q.factor[i] = p.cap > 0.0f ? p.cap * LOG2E : f * LOG2E;
+    }
     float sums[G];
 #pragma unroll
     for (int j = 0; j < G; ++j) {
@@ -195,11 +180,10 @@ template <int G> __device__ __forceinline__ void load_query(const DecodeParams &
     }
 }
 
-// A warp's running state. acc[j][u]: channels 32 j + 4 g + 2 u (rows g) and + 1 (rows g + 8, 16 times too large), heads 2 t, 2 t + 1.
-// zero[i][e]: what the zeros of groups 2 i and 2 i + 1 add, head 2 t + e.
+// A warp's running state. acc[j][u]: 2^-24 (channel 32 j + 4 g + 2 u, and 16 times the next one) in rows g, the latter alone in rows
+// g + 8; heads 2 t, 2 t + 1.
 template <int G> struct State {
-    float acc[G][2][4], sum[2], ref[2];
-    uint64_t zero[G / 2][2];
+    float acc[G][2][4], zero[G][2], sum[2], ref[2];
 };
 
 template <int G> __device__ __forceinline__ void clear(State<G> &s) {
@@ -209,7 +193,7 @@ template <int G> __device__ __forceinline__ void clear(State<G> &s) {
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s.acc[j][u][i] = 0.0f;
-        s.zero[j / 2][j & 1] = 0;
+        s.zero[j][0] = s.zero[j][1] = 0.0f;
     }
     s.sum[0] = s.sum[1] = 0.0f;
     s.ref[0] = s.ref[1] = LOWEST;
@@ -219,27 +203,24 @@ template <int G> __device__ __forceinline__ void rescale(State<G> &s, float f0, 
     for (int j = 0; j < G; ++j) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) { s.acc[j][u][0] *= f0; s.acc[j][u][1] *= f1; s.acc[j][u][2] *= f0; s.acc[j][u][3] *= f1; }
-        s.zero[j / 2][j & 1] = mul2(s.zero[j / 2][j & 1], j & 1 ? pair(f1, f1) : pair(f0, f0));
+        s.zero[j][0] *= f0; s.zero[j][1] *= f1;
     }
     s.sum[0] *= f0; s.sum[1] *= f1;
 }
 
-// ---- a warp's ring of records: one bulk copy each, completion counted by an mbarrier to a slot ----
-constexpr int MOST_TRIES = 1 << 20;               // of a wait; each sleeps for a while by itself
-__device__ __forceinline__ void send_record(uint32_t to, uint32_t barrier, const uint8_t *rec, int bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(rec ? bytes : 0) : "memory");
-    if (rec)
-        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                     ::"r"(to), "l"(rec), "r"(bytes), "r"(barrier) : "memory");
+// ---- a warp's ring of records: 16 bytes a lane at a time, a group of copies for each record ----
+// Bulk copies counted by mbarriers move the same bytes, but a record's barrier, wait and copy took a warp 90 cycles of a scheduler
+// against 25 of these (8 x 64K tokens, 8 kv heads: 144 us).
+template <int G> __device__ __forceinline__ void fetch(uint32_t to, const uint8_t *rec, int lane) {   // both at the lane's 16 bytes
+#pragma unroll
+    for (int i = 0; i < Rec<G>::BYTES; i += 512)
+        if (i + 512 <= Rec<G>::BYTES || i + 16 * lane < Rec<G>::BYTES)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i), "l"(rec + i) : "memory");
 }
-__device__ __forceinline__ bool arrived(uint32_t barrier, uint32_t parity) {
-    for (int i = 0; i < MOST_TRIES; ++i) {
-        uint32_t done;
-        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                     : "=r"(done) : "r"(barrier), "r"(parity) : "memory");
-        if (done) return true;
-    }
-    return false;
+__device__ __forceinline__ void close_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void fetched() {                // all but the last N groups
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    __syncwarp();
 }
 
 // One record in shared memory, n of its tokens valid (1..16)
@@ -277,9 +258,9 @@ template <int G, bool FINE> __device__ __forceinline__ void attend(const DecodeP
     }
     if (p.cap > 0.0f) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = p.cap * tanhf(x[i] * q.factor[i & 1] / p.cap);
+        for (int i = 0; i < 4; ++i) x[i] = tanhf(x[i] * q.raw[i & 1]);
     }
-    const float f0 = p.cap > 0.0f ? LOG2E : q.factor[0], f1 = p.cap > 0.0f ? LOG2E : q.factor[1];   // x f: logits in powers of two
+    const float f0 = q.factor[0], f1 = q.factor[1];                         // x f: logits in powers of two
     if (n < 16) {                                 // what lies behind the last token may be anything
         if (g >= n) {
             x[0] = x[1] = -INFINITY;
@@ -329,28 +310,24 @@ template <int G, bool FINE> __device__ __forceinline__ void attend(const DecodeP
     alignas(16) uint32_t v0[G], v1[G];
     *reinterpret_cast<W *>(v0) = reinterpret_cast<const W *>(rec + Rec<G>::V)[lane];
     *reinterpret_cast<W *>(v1) = reinterpret_cast<const W *>(rec + Rec<G>::V)[32 + lane];
-    const uint64_t ww[4] = {pair(w[0], w[0]), pair(w[1], w[1]), pair(w[2], w[2]), pair(w[3], w[3])};
 #pragma unroll
-    for (int j2 = 0; j2 < G; j2 += 2) {
-    const uint64_t s0 = pair(scale_of(vp0[j2]), scale_of(vp0[j2 + 1])), s1 = pair(scale_of(vp1[j2]), scale_of(vp1[j2 + 1]));
-    const uint64_t z0 = pair(zero_of(vp0[j2]), zero_of(vp0[j2 + 1])), z1 = pair(zero_of(vp1[j2]), zero_of(vp1[j2 + 1]));
-    s.zero[j2 / 2][0] = fma2(z1, ww[2], fma2(z0, ww[0], s.zero[j2 / 2][0]));
-    s.zero[j2 / 2][1] = fma2(z1, ww[3], fma2(z0, ww[1], s.zero[j2 / 2][1]));
-    const float2 y2[4] = {unpair(mul2(ww[0], s0)), unpair(mul2(ww[1], s0)), unpair(mul2(ww[2], s1)), unpair(mul2(ww[3], s1))};
-#pragma unroll
-    for (int j = j2; j < j2 + 2; ++j) {
-        const float y[4] = {j & 1 ? y2[0].y : y2[0].x, j & 1 ? y2[1].y : y2[1].x, j & 1 ? y2[2].y : y2[2].x, j & 1 ? y2[3].y : y2[3].x};
-        const uint32_t h0 = half2_bits(y[0], y[1]), h1 = half2_bits(y[2], y[3]), a = v0[j] >> 8, b = v1[j] >> 8;
+    for (int j = 0; j < G; ++j) {
+        const float s0 = scale_of(vp0[j]), s1 = scale_of(vp1[j]), z0 = zero_of(vp0[j]), z1 = zero_of(vp1[j]);
+        s.zero[j][0] = fmaf(z1, w[2], fmaf(z0, w[0], s.zero[j][0]));
+        s.zero[j][1] = fmaf(z1, w[3], fmaf(z0, w[1], s.zero[j][1]));
+        const float y[4] = {w[0] * s0, w[1] * s0, w[2] * s1, w[3] * s1};
+        const uint32_t h0 = half2_bits(y[0], y[1]), h1 = half2_bits(y[2], y[3]);
+        // bytes 0, 2 and 1, 3 in half words of their own
+        const uint32_t a = v0[j] & 0x00FF00FFu, b = v1[j] & 0x00FF00FFu, c = __byte_perm(v0[j], 0, 0x4341), d = __byte_perm(v1[j], 0, 0x4341);
         const uint32_t b0 = transpose8x8(h0), b1 = transpose8x8(h1);
-        mma(s.acc[j][0], v0[j] & LO, v0[j] & HI, v1[j] & LO, v1[j] & HI, b0, b1);
-        mma(s.acc[j][1], a & LO, a & HI, b & LO, b & HI, b0, b1);
+        mma(s.acc[j][0], a, a & HI, b, b & HI, b0, b1);
+        mma(s.acc[j][1], c, c & HI, d, d & HI, b0, b1);
         if constexpr (FINE) {
             const float2 r0 = half2_floats(h0), r1 = half2_floats(h1);
             const uint32_t d0 = transpose8x8(half2_bits(y[0] - r0.x, y[1] - r0.y)), d1 = transpose8x8(half2_bits(y[2] - r1.x, y[3] - r1.y));
-            mma(s.acc[j][0], v0[j] & LO, v0[j] & HI, v1[j] & LO, v1[j] & HI, d0, d1);
-            mma(s.acc[j][1], a & LO, a & HI, b & LO, b & HI, d0, d1);
+            mma(s.acc[j][0], a, a & HI, b, b & HI, d0, d1);
+            mma(s.acc[j][1], c, c & HI, d, d & HI, d0, d1);
         }
-    }
     }
 }
 
@@ -369,7 +346,7 @@ __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Share
 #pragma unroll
     for (int j = 0; j < G; ++j)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) zero[j][i] = j & 1 ? unpair(s.zero[j / 2][i]).y : unpair(s.zero[j / 2][i]).x;
+        for (int i = 0; i < 2; ++i) zero[j][i] = s.zero[j][i];
 #pragma unroll
     for (int d = 4; d < 32; d *= 2) {
 #pragma unroll
@@ -399,7 +376,7 @@ __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Share
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 sh.o[warp][2 * t + (i & 1)][32 * j + 4 * g + 2 * u + (i >> 1)] =
-                    f[i & 1] * fmaf(s.acc[j][u][i], i < 2 ? 0x1p24f : 0x1p20f, zero[j][i & 1]);
+                    f[i & 1] * fmaf(i < 2 ? s.acc[j][u][i] - s.acc[j][u][i + 2] : s.acc[j][u][i], i < 2 ? 0x1p24f : 0x1p20f, zero[j][i & 1]);
     __syncthreads();
     for (int i = threadIdx.x; i < COLS * D; i += 32 * NW) {
         const int h = i / D, c = i % D;
@@ -416,16 +393,12 @@ __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Share
             if (c == 0) p.lse[b * p.lse_b + first_head + h] = sum != 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
         }
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");            // what lay here, before the next row's copies
     __syncthreads();
 }
 
-template <int G> struct Memory {
-    union {
-        Shared<G> sh;
-        alignas(128) uint8_t ring[NW][STAGES][Rec<G>::BYTES];
-    };
-    uint64_t barriers[NW][STAGES];
+template <int G> union Memory {
+    Shared<G> sh;
+    uint8_t ring[NW][STAGES][Rec<G>::BYTES];
 };
 template <int G> struct Floats;
 template <> struct Floats<2> { using T = float2; };
@@ -436,11 +409,8 @@ template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PE
     Memory<G> &m = *reinterpret_cast<Memory<G> *>(memory);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint8_t *ring = m.ring[warp][0];
-    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), barriers = (uint32_t)__cvta_generic_to_shared(m.barriers[warp]);
-    if (lane < STAGES) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(barriers + 8 * lane) : "memory");
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    __syncwarp();
-    uint32_t sent = 0, taken = 0;                 // records since the start
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + 16 * lane;
+    const uint8_t *records = p.c.records + 16 * lane;
     wait_earlier();
     let_next_in();
     const int rows = p.c.H * p.col_blocks;
@@ -475,50 +445,64 @@ template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PE
         const int head = row / p.col_blocks, cb = row % p.col_blocks;
         const int first_head = head * p.group + cb * COLS, n = min(COLS, p.group - cb * COLS);
         const int32_t *sel = p.selected ? p.selected + ((int64_t)b * p.c.H + head) * p.num_selected : nullptr;
-        // the records of 32 of the warp's tiles at a time are looked up by a lane each: address and tokens (0: none)
-        const int mine = (i1 - i0 - warp + NW - 1) / NW;
-        const uint8_t *rec = nullptr;
-        int valid = 0;
-        auto look_up = [&](int k) {
-            const int i = i0 + warp + (k + lane) * NW, slot = i / p.c.parts, part = i - slot * p.c.parts;
-            rec = nullptr;
+        // 32 of the warp's records at a time are looked up by a lane each, while the 32 before are on their way: which one it is and how
+        // many of its tokens are valid (0: there is none). `odd`: those of less than 16.
+        const int mine = (i1 - i0 - warp + NW - 1) / NW, part_shift = p.page_shift - 4;
+        auto look_up = [&](int k, uint32_t &rec, int &valid) {
+            const int i = i0 + warp + (k + lane) * NW, slot = i >> part_shift, part = i & (p.c.parts - 1);
+            rec = 0;                                  // a record that is not meant is fetched too, and not used
             valid = 0;
             if (i >= i1) return;
             const int place = sel ? sel[slot] : slot;
             const int64_t first = ((int64_t)place << p.page_shift) + 16 * part;
             if (place < 0 || first >= len) return;
-            const int64_t id = page_id(p.s, b, place);
-            if (id < 0 || id >= p.c.num_pages) { or_status(p.status, OMMX_ST_BAD_PAGE); return; }
-            rec = p.c.records + ((id * p.c.H + head) * p.c.parts + part) * Rec<G>::BYTES;
+            const int64_t page = page_id(p.s, b, place);
+            if (page < 0 || page >= p.c.num_pages) { or_status(p.status, OMMX_ST_BAD_PAGE); return; }
+            rec = (uint32_t)((page * p.c.H + head) * p.c.parts + part);    // below 2^32: there is no memory for more
             valid = (int)min((int64_t)16, len - first);
         };
-        // tile k is sent STAGES - 1 tiles ahead, by the lane that looked it up
-        uint32_t counts = 0;                          // tokens of the tiles on their way, eight bits each, the next one lowest
-        auto send = [&](int k) {
-            if (k < mine) {
-                if ((k & 31) == 0) look_up(k);
-                const uint32_t slot = sent++ % STAGES;
-                if (lane == (k & 31)) send_record(ring_at + slot * Rec<G>::BYTES, barriers + 8 * slot, rec, Rec<G>::BYTES);
-                counts = counts >> 8 | (uint32_t)__shfl_sync(~0u, valid, k & 31) << (8 * (STAGES - 1));
-            } else {
-                counts >>= 8;
-            }
-        };
+        // `rec`, `valid`: of the AHEAD first ones, then of 32 at a time, AHEAD of those in use
+        uint32_t rec, next_rec;
+        int valid, next_valid, flying = 0;            // flying: valid tokens of those on their way, eight bits each, the next one lowest
+        look_up(0, rec, valid);
+        look_up(AHEAD, next_rec, next_valid);
 #pragma unroll
-        for (int k = 0; k < STAGES - 1; ++k) send(k);
+        for (int k = 0; k < AHEAD; ++k) {
+            if (k < mine) fetch<G>(ring_at + k * Rec<G>::BYTES, records + (uint64_t)__shfl_sync(~0u, rec, k) * Rec<G>::BYTES, lane);
+            flying |= __shfl_sync(~0u, valid, k) << (8 * k);
+            close_group();
+        }
         Query<G> q;
         State<G> s;
         load_query<G>(p, b, first_head, n, lane, q);
         clear(s);
-        for (int k = 0; k < mine; ++k) {
-            send(k + STAGES - 1);
-            const int n = counts & 255u;
-            const uint32_t slot = taken % STAGES;
-            const bool here = arrived(barriers + 8 * slot, taken++ / STAGES & 1);
-            if (!here) or_status(p.status, OMMX_ST_TIMEOUT);
-            if (n && here) attend<G, FINE>(p, ring + slot * Rec<G>::BYTES, n, lane, q, s);
-            __syncwarp();                             // before the slot is filled again
+        for (int k0 = 0; k0 < mine; k0 += 32) {
+            rec = next_rec;
+            valid = next_valid;
+            look_up(k0 + 32 + AHEAD, next_rec, next_valid);
+            const int left = mine - k0, now = min(32, left);
+            if (flying == FULL && __all_sync(~0u, valid == 16 || lane + AHEAD >= left)) {
+                for (int k = 0; k < now; ++k) {
+                    if (k + AHEAD < left)
+                        fetch<G>(ring_at + (k + AHEAD) % STAGES * Rec<G>::BYTES, records + (uint64_t)__shfl_sync(~0u, rec, k) * Rec<G>::BYTES, lane);
+                    close_group();
+                    fetched<AHEAD>();
+                    attend<G, FINE>(p, ring + k % STAGES * Rec<G>::BYTES, 16, lane, q, s);
+                    __syncwarp();                     // before the slot is filled again
+                }
+            } else {
+                for (int k = 0; k < now; ++k) {
+                    if (k + AHEAD < left)
+                        fetch<G>(ring_at + (k + AHEAD) % STAGES * Rec<G>::BYTES, records + (uint64_t)__shfl_sync(~0u, rec, k) * Rec<G>::BYTES, lane);
+                    close_group();
+                    fetched<AHEAD>();
+                    if (flying & 255) attend<G, FINE>(p, ring + k % STAGES * Rec<G>::BYTES, flying & 255, lane, q, s);
+                    flying = flying >> 8 | __shfl_sync(~0u, valid, k) << (8 * (AHEAD - 1));
+                    __syncwarp();
+                }
+            }
         }
+        fetched<0>();
         __syncthreads();                              // the ring is the merge's memory too
         float *part = nullptr;
         if (i0 > 0 || i1 < tiles) part = p.work + (2 * (int64_t)blockIdx.x + (base + (int64_t)row * tiles >= start)) * Shared<G>::PART;
@@ -659,6 +643,7 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     p.Hq = a->n_q_heads; p.group = a->n_q_heads / p.c.H; p.col_blocks = (p.group + COLS - 1) / COLS;
     p.page_shift = shift_of(p.c.page);
     p.sm_scale = a->sm_scale; p.cap = a->logit_cap; p.status = a->status;
+    if (p.c.num_pages == 0) p.c.records = reinterpret_cast<uint8_t *>(p.work);   // what is fetched for a page that is not there
     p.least = NW;
     // as many blocks as the SMs hold, no more than the work can have
     int64_t tiles = (int64_t)p.s.max_pages * p.c.parts;
