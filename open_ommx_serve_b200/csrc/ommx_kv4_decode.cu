@@ -26,6 +26,7 @@ constexpr int BLOCKS_PER_SM = 2;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float ROOM = 4096.0f;                   // how large a weight may get before its reference moves
 constexpr float LOWEST = -1e30f;
+constexpr int WHOLE = 4 * NW;                     // records of a row that one block takes at most where it could share it
 
 struct DecodeParams {
     Cache c;
@@ -35,7 +36,7 @@ struct DecodeParams {
     float *lse, *work;
     const int32_t *selected;
     int64_t q_b, q_h, o_b, o_h, lse_b;
-    int32_t q16, q_wide, o_type, Hq, group, col_blocks, num_selected, page_shift, least;
+    int32_t q16, q_wide, o_type, Hq, group, col_blocks, num_selected, page_shift, least, whole;
     float sm_scale, cap;
     int32_t *status;
 };
@@ -52,19 +53,18 @@ __device__ __forceinline__ int length_of(const DecodeParams &p, int b) {
     if (len < 0 || len > most) { or_status(p.status, OMMX_ST_BAD_LENGTH); return len < 0 ? 0 : (int)most; }
     return len;
 }
-__device__ __forceinline__ int tiles_of(const DecodeParams &p, int len) {
+__device__ __forceinline__ int units_of(const DecodeParams &p, int len) {
     if (p.selected) return min(pages_of(p, len), p.num_selected) * p.c.parts;
     return (len + 15) >> 4;
 }
-struct Shares { int64_t per, total; };
-__device__ __forceinline__ Shares shares(const DecodeParams &p, int rows, int blocks, int lane) {
-    int64_t sum = 0;
-    for (int b = lane; b < p.s.B; b += 32) sum += tiles_of(p, length_of(p, b));
-#pragma unroll
-    for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+struct Shares { uint32_t per, total; };           // the host refuses what 32 bits do not count
+__device__ __forceinline__ Shares shares(const DecodeParams &p, uint32_t rows, uint32_t blocks, int lane) {
+    uint32_t sum = 0;
+    for (int b = lane; b < p.s.B; b += 32) sum += units_of(p, length_of(p, b));
+    sum = __reduce_add_sync(~0u, sum);
     Shares r;
     r.total = sum * rows;
-    r.per = max((r.total + blocks - 1) / blocks, (int64_t)p.least);
+    r.per = max((r.total + blocks - 1) / blocks, (uint32_t)p.least);
     return r;
 }
 
@@ -131,19 +131,37 @@ template <int G> struct Query {
     uint32_t frag[G][4], sums[2];
     float factor[2], raw[2];                      // of heads 2 t and 2 t + 1: the products' units in powers of two; with a cap: in its units
 };
-template <int G> __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int first_head, int n, int lane, Query<G> &q) {
+// Warp j < G takes group j of all heads; largest values, sums and fragments meet in shared memory. All warps call it.
+template <int G> struct QueryMemory {
+    uint4 frag[G][32];
+    float top[COLS][G], sum[COLS][G];
+};
+template <int G>
+__device__ __forceinline__ void load_query(const DecodeParams &p, int b, int first_head, int n, int warp, int lane, QueryMemory<G> &m, Query<G> &q) {
     const int g = lane >> 2, t = lane & 3;
-    float x[G][8], top = 0.0f;
+    float x[8];
+    if (warp < G) {
+        load_q8(p, b * p.q_b + (first_head + min(g, n - 1)) * p.q_h + 32 * warp + 8 * t, x);
+        float top = fabsf(x[0]), sum = x[0];
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-        load_q8(p, b * p.q_b + (first_head + min(g, n - 1)) * p.q_h + 32 * j + 8 * t, x[j]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[j][i]));
+        for (int i = 1; i < 8; ++i) { top = fmaxf(top, fabsf(x[i])); sum += x[i]; }
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+        sum += __shfl_xor_sync(~0u, sum, 1);
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+        sum += __shfl_xor_sync(~0u, sum, 2);
+        if (t == 0) { m.top[g][warp] = top; m.sum[g][warp] = sum; }
     }
-    top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+    __syncthreads();
+    float top = m.top[g][0];
+#pragma unroll
+    for (int j = 1; j < G; ++j) top = fmaxf(top, m.top[g][j]);
     const int e = top > 0.0f ? max(exponent_of(top), -100) : 0;
     const float up = power_of_two(13 - e);
+    if (warp < G) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= i & 1 ? up * 0.0625f : up;      // odd nibbles are 16 times as large
+        m.frag[warp][lane] = make_uint4(half2_bits(x[0], x[4]), half2_bits(x[1], x[5]), half2_bits(x[2], x[6]), half2_bits(x[3], x[7]));
+    }
     const float factor = p.sm_scale * power_of_two(24 - 13 + e);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -151,32 +169,24 @@ template <int G> __device__ __forceinline__ void load_query(const DecodeParams &
         q.raw[i] = f / p.cap;
         q.factor[i] = p.cap > 0.0f ? p.cap * LOG2E : f * LOG2E;
     }
-    float sums[G];
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { x[j][i] *= up; sum += x[j][i]; }
-        sum += __shfl_xor_sync(~0u, sum, 1);
-        sum += __shfl_xor_sync(~0u, sum, 2);
-        sums[j] = sum * 0x1p-24f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float f = k & 1 ? 0.0625f : 1.0f;
-            q.frag[j][k] = half2_bits(x[j][k] * f, x[j][k + 4] * f);
-        }
-    }
     // rows of the product: term r of group j at G r + j; lane t holds rows 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
-    const float a = G == 4 && (t & 1) ? sums[G - 2] : sums[0], b2 = G == 4 && (t & 1) ? sums[G - 1] : sums[1];
-    const float a1 = bf16_round_f32(a), b1 = bf16_round_f32(b2), a2 = bf16_round_f32(a - a1), b2r = bf16_round_f32(b2 - b1);
-    const uint32_t terms[4] = {f32_to_bf16_bits(a1) | f32_to_bf16_bits(b1) << 16, f32_to_bf16_bits(a2) | f32_to_bf16_bits(b2r) << 16,
-                               f32_to_bf16_bits(a - a1 - a2) | f32_to_bf16_bits(b2 - b1 - b2r) << 16, 0u};
+    const int j = G == 4 ? 2 * (t & 1) : 0;
+    const float a = m.sum[g][j] * (up * 0x1p-24f), c = m.sum[g][j + 1] * (up * 0x1p-24f);
+    const float a1 = bf16_round_f32(a), c1 = bf16_round_f32(c), a2 = bf16_round_f32(a - a1), c2 = bf16_round_f32(c - c1);
+    const uint32_t term1 = f32_to_bf16_bits(a1) | f32_to_bf16_bits(c1) << 16, term2 = f32_to_bf16_bits(a2) | f32_to_bf16_bits(c2) << 16,
+                   term3 = f32_to_bf16_bits(a - a1 - a2) | f32_to_bf16_bits(c - c1 - c2) << 16;
     if constexpr (G == 4) {
-        q.sums[0] = t < 2 ? terms[0] : terms[1];
-        q.sums[1] = t < 2 ? terms[2] : 0u;
+        q.sums[0] = t < 2 ? term1 : term2;
+        q.sums[1] = t < 2 ? term3 : 0u;
     } else {
-        q.sums[0] = t == 0 ? terms[0] : t == 1 ? terms[1] : t == 2 ? terms[2] : 0u;
+        q.sums[0] = t == 0 ? term1 : t == 1 ? term2 : t == 2 ? term3 : 0u;
         q.sums[1] = 0u;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+        const uint4 f = m.frag[i][lane];
+        q.frag[i][0] = f.x; q.frag[i][1] = f.y; q.frag[i][2] = f.z; q.frag[i][3] = f.w;
     }
 }
 
@@ -334,19 +344,24 @@ template <int G, bool FINE> __device__ __forceinline__ void attend(const DecodeP
 template <int G> struct Shared {
     static constexpr int D = 32 * G, PART = COLS * D + 2 * COLS;   // floats of a part in the workspace
     float o[NW][COLS][D + 4];                     // the padding spreads the heads over the banks
-    float ref[NW][COLS], sum[NW][COLS];
 };
+template <int G> struct Floats;
+template <> struct Floats<2> { using T = float2; };
+template <> struct Floats<4> { using T = float4; };
+template <int G> __device__ __forceinline__ void store_o(const DecodeParams &p, int64_t at, const float (&v)[G]) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) store_o(p, at + i, v[i]);
+}
 
-// The warps' states of a row to its output, or to a part: [COLS][D] weighted values, [COLS] references, [COLS] sums
+// The warps' states of a row to its output, or to a part: [COLS][D] weighted values, [COLS] references, [COLS] sums. Warp h finishes
+// head h, a lane G channels.
 template <int G>
-__device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Shared<G> &sh, int b, int first_head, int n, float *part, int warp, int lane) {
+__device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Shared<G> &sh, float (&ref)[COLS][NW], float (&sum)[COLS][NW], int b,
+                                       int first_head, int n, float *part, int warp, int lane) {
+    static_assert(NW == COLS, "a warp finishes a head");
+    using V = typename Floats<G>::T;
     constexpr int D = 32 * G;
     const int g = lane >> 2, t = lane & 3;
-    float zero[G][2];
-#pragma unroll
-    for (int j = 0; j < G; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) zero[j][i] = s.zero[j][i];
 #pragma unroll
     for (int d = 4; d < 32; d *= 2) {
 #pragma unroll
@@ -354,55 +369,73 @@ __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Share
 #pragma unroll
         for (int j = 0; j < G; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) zero[j][i] += __shfl_xor_sync(~0u, zero[j][i], d);
+            for (int i = 0; i < 2; ++i) s.zero[j][i] += __shfl_xor_sync(~0u, s.zero[j][i], d);
     }
     if (g == 0) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) { sh.ref[warp][2 * t + i] = s.ref[i]; sh.sum[warp][2 * t + i] = s.sum[i]; }
+        for (int i = 0; i < 2; ++i) { ref[2 * t + i][warp] = s.ref[i]; sum[2 * t + i][warp] = s.sum[i]; }
     }
-    __syncthreads();
+    __syncthreads();                              // and the ring, whose memory `sh` is, is done with
     float f[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        float top = sh.ref[0][2 * t + i];
+        float top = ref[2 * t + i][0];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) top = fmaxf(top, sh.ref[w][2 * t + i]);
+        for (int w = 1; w < NW; ++w) top = fmaxf(top, ref[2 * t + i][w]);
         f[i] = exp2_approx(s.ref[i] - top);
     }
 #pragma unroll
     for (int j = 0; j < G; ++j)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                sh.o[warp][2 * t + (i & 1)][32 * j + 4 * g + 2 * u + (i >> 1)] =
-                    f[i & 1] * fmaf(i < 2 ? s.acc[j][u][i] - s.acc[j][u][i + 2] : s.acc[j][u][i], i < 2 ? 0x1p24f : 0x1p20f, zero[j][i & 1]);
-    __syncthreads();
-    for (int i = threadIdx.x; i < COLS * D; i += 32 * NW) {
-        const int h = i / D, c = i % D;
-        float v = sh.o[0][h][c], top = sh.ref[0][h], sum = 0.0f;
-#pragma unroll
-        for (int w = 1; w < NW; ++w) { v += sh.o[w][h][c]; top = fmaxf(top, sh.ref[w][h]); }
-#pragma unroll
-        for (int w = 0; w < NW; ++w) sum += sh.sum[w][h] * exp2_approx(sh.ref[w][h] - top);
-        if (part) {
-            part[i] = v;
-            if (c == 0) { part[COLS * D + h] = top; part[COLS * D + COLS + h] = sum; }
-        } else if (h < n) {
-            store_o(p, b * p.o_b + (first_head + h) * p.o_h + c, sum != 0.0f ? v / sum : 0.0f);
-            if (c == 0) p.lse[b * p.lse_b + first_head + h] = sum != 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
+        for (int i = 0; i < 2; ++i) {
+            float *to = &sh.o[warp][2 * t + i][32 * j + 4 * g];
+            const float z = s.zero[j][i];
+            *reinterpret_cast<float4 *>(to) = make_float4(f[i] * fmaf(s.acc[j][0][i] - s.acc[j][0][i + 2], 0x1p24f, z), f[i] * fmaf(s.acc[j][0][i + 2], 0x1p20f, z),
+                                                          f[i] * fmaf(s.acc[j][1][i] - s.acc[j][1][i + 2], 0x1p24f, z), f[i] * fmaf(s.acc[j][1][i + 2], 0x1p20f, z));
         }
+    float top = ref[warp][0], all = 0.0f;
+#pragma unroll
+    for (int w = 1; w < NW; ++w) top = fmaxf(top, ref[warp][w]);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) all = fmaf(sum[warp][w], exp2_approx(ref[warp][w] - top), all);
+    __syncthreads();
+    float v[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) v[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        const V x = *reinterpret_cast<const V *>(&sh.o[w][warp][lane * G]);
+#pragma unroll
+        for (int i = 0; i < G; ++i) v[i] += reinterpret_cast<const float *>(&x)[i];
+    }
+    if (part) {
+        *reinterpret_cast<V *>(part + warp * D + lane * G) = *reinterpret_cast<const V *>(v);
+        if (lane == 0) { part[COLS * D + warp] = top; part[COLS * D + COLS + warp] = all; }
+    } else if (warp < n) {
+        const float inverse = all != 0.0f ? 1.0f / all : 0.0f;
+#pragma unroll
+        for (int i = 0; i < G; ++i) v[i] = all != 0.0f ? v[i] * inverse : 0.0f;
+        store_o(p, b * p.o_b + (first_head + warp) * p.o_h + lane * G, v);
+        if (lane == 0) p.lse[b * p.lse_b + first_head + warp] = all != 0.0f ? (top + log2f(all)) * LN2 : -INFINITY;
     }
     __syncthreads();
 }
 
-template <int G> union Memory {
-    Shared<G> sh;
-    uint8_t ring[NW][STAGES][Rec<G>::BYTES];
+template <int G> struct Memory {
+    union {
+        Shared<G> sh;
+        uint8_t ring[NW][STAGES][Rec<G>::BYTES];
+    };
+    QueryMemory<G> query;
+    float ref[COLS][NW], sum[COLS][NW];
 };
-template <int G> struct Floats;
-template <> struct Floats<2> { using T = float2; };
-template <> struct Floats<4> { using T = float4; };
+
+// A row of no tokens
+template <int G> __device__ __forceinline__ void nothing(const DecodeParams &p, int b, int row) {
+    const int cb = row % p.col_blocks, first = (row / p.col_blocks) * p.group + cb * COLS, n = min(COLS, p.group - cb * COLS);
+    for (int i = threadIdx.x; i < n * 32 * G; i += blockDim.x) store_o(p, b * p.o_b + (first + i / (32 * G)) * p.o_h + i % (32 * G), 0.0f);
+    if (threadIdx.x < n) p.lse[b * p.lse_b + first + threadIdx.x] = -INFINITY;
+}
 
 template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PER_SM) kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
     extern __shared__ __align__(128) uint8_t memory[];
@@ -413,35 +446,44 @@ template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PE
     const uint8_t *records = p.c.records + 16 * lane;
     wait_earlier();
     let_next_in();
-    const int rows = p.c.H * p.col_blocks;
-    const Shares sr = shares(p, rows, gridDim.x, lane);
-    int64_t u = blockIdx.x * sr.per;
-    const int64_t end = min(u + sr.per, sr.total), start = u;
-    if (u >= end) return;
-    // the sequence that unit u lies in
-    int b = 0, tiles = 0, len = 0;
-    int64_t base = 0;                             // units before sequence b
-    for (int b0 = 0;; b0 += 32) {
-        const int l = b0 + lane < p.s.B ? length_of(p, b0 + lane) : 0, n = tiles_of(p, l);
-        const int sum = warp_inclusive_scan(n, lane);              // of 32 sequences: below 2^31 tiles of 16 tokens
-        const uint32_t past = __ballot_sync(~0u, base + (int64_t)sum * rows > u);
-        if (past) {
-            const int from = __ffs(past) - 1;
-            b = b0 + from;
-            base += (int64_t)__shfl_sync(~0u, sum - n, from) * rows;
-            tiles = __shfl_sync(~0u, n, from);
-            len = __shfl_sync(~0u, l, from);
-            break;
+    const uint32_t rows = p.c.H * p.col_blocks;
+    uint32_t u, end, start, base = 0;             // this block's units; units before sequence b
+    int b = 0, units = 0, len = 0;
+    if (p.whole) {                                // a block to a row
+        b = blockIdx.x / rows;
+        len = length_of(p, b);
+        units = units_of(p, len);
+        start = u = (blockIdx.x - b * rows) * units;
+        end = u + units;
+        if (units == 0) { nothing<G>(p, b, blockIdx.x - b * rows); return; }
+    } else {
+        const Shares sr = shares(p, rows, gridDim.x, lane);
+        start = u = blockIdx.x * sr.per;
+        if (u >= sr.total) return;
+        end = min(u + sr.per, sr.total);
+        // the sequence that unit u lies in
+        for (int b0 = 0;; b0 += 32) {
+            if (b0 >= p.s.B) return;              // lengths past max_seq_len, more units than 32 bits count
+            const int l = b0 + lane < p.s.B ? length_of(p, b0 + lane) : 0, n = units_of(p, l);
+            const uint32_t sum = warp_inclusive_scan(n, lane), past = __ballot_sync(~0u, base + sum * rows > u);
+            if (past) {
+                const int from = __ffs(past) - 1;
+                b = b0 + from;
+                base += __shfl_sync(~0u, sum - n, from) * rows;
+                units = __shfl_sync(~0u, n, from);
+                len = __shfl_sync(~0u, l, from);
+                break;
+            }
+            base += __shfl_sync(~0u, sum, 31) * rows;
         }
-        base += (int64_t)__shfl_sync(~0u, sum, 31) * rows;
     }
     while (u < end) {
-        while (u >= base + (int64_t)tiles * rows) {               // the next sequence that has any
-            base += (int64_t)tiles * rows;
+        while (u >= base + units * rows) {        // the next sequence that has any
+            base += units * rows;
             len = length_of(p, ++b);
-            tiles = tiles_of(p, len);
+            units = units_of(p, len);
         }
-        const int row = (int)((u - base) / tiles), i0 = (int)(u - base - (int64_t)row * tiles), i1 = (int)min((int64_t)tiles, i0 + (end - u));
+        const int row = (u - base) / units, i0 = u - base - row * units, i1 = min((uint32_t)units, i0 + (end - u));
         const int head = row / p.col_blocks, cb = row % p.col_blocks;
         const int first_head = head * p.group + cb * COLS, n = min(COLS, p.group - cb * COLS);
         const int32_t *sel = p.selected ? p.selected + ((int64_t)b * p.c.H + head) * p.num_selected : nullptr;
@@ -474,7 +516,7 @@ template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PE
         }
         Query<G> q;
         State<G> s;
-        load_query<G>(p, b, first_head, n, lane, q);
+        load_query<G>(p, b, first_head, n, warp, lane, m.query, q);
         clear(s);
         for (int k0 = 0; k0 < mine; k0 += 32) {
             rec = next_rec;
@@ -503,10 +545,9 @@ template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PE
             }
         }
         fetched<0>();
-        __syncthreads();                              // the ring is the merge's memory too
         float *part = nullptr;
-        if (i0 > 0 || i1 < tiles) part = p.work + (2 * (int64_t)blockIdx.x + (base + (int64_t)row * tiles >= start)) * Shared<G>::PART;
-        finish<G>(p, s, m.sh, b, first_head, n, part, warp, lane);
+        if (i0 > 0 || i1 < units) part = p.work + (2 * (int64_t)blockIdx.x + (base + row * units >= start)) * Shared<G>::PART;
+        finish<G>(p, s, m.sh, m.ref, m.sum, b, first_head, n, part, warp, lane);
         u += i1 - i0;
     }
 }
@@ -522,15 +563,13 @@ template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_kernel(c
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int b = blockIdx.y, row = blockIdx.x / COLS, h = blockIdx.x % COLS;
     const int head = row / p.col_blocks, cb = row % p.col_blocks, hq = head * p.group + cb * COLS + h;
-    const int rows = p.c.H * p.col_blocks;
+    const uint32_t rows = p.c.H * p.col_blocks;
     const Shares sh = shares(p, rows, blocks, lane);
-    int64_t before = 0;
-    for (int i = lane; i < b; i += 32) before += tiles_of(p, length_of(p, i));
-#pragma unroll
-    for (int d = 16; d; d /= 2) before += __shfl_xor_sync(~0u, before, d);
-    const int tiles = tiles_of(p, length_of(p, b));
-    const int64_t r0 = before * rows + (int64_t)row * tiles, r1 = r0 + tiles;
-    const int c0 = (int)(r0 / sh.per), n = tiles ? (int)((r1 - 1) / sh.per) - c0 + 1 : 0;
+    uint32_t before = 0;
+    for (int i = lane; i < b; i += 32) before += units_of(p, length_of(p, i));
+    before = __reduce_add_sync(~0u, before);
+    const uint32_t units = units_of(p, length_of(p, b)), r0 = before * rows + row * units, c0 = r0 / sh.per;
+    const int n = units ? (int)((r0 + units - 1) / sh.per - c0) + 1 : 0;
     const bool late = r0 >= c0 * sh.per;          // the row begins in block c0: its part there is the second one
     wait_earlier();
     let_next_in();
@@ -540,7 +579,7 @@ template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_kernel(c
         if (threadIdx.x == 0) p.lse[b * p.lse_b + hq] = -INFINITY;
         return;
     }
-    auto part = [&](int i) { return p.work + (int64_t)(2 * (c0 + i) + (i == 0 && late)) * Shared<G>::PART; };
+    auto part = [&](int i) { return p.work + (2 * (int64_t)(c0 + i) + (i == 0 && late)) * Shared<G>::PART; };
     float top = LOWEST, sum = 0.0f;
     for (int i = threadIdx.x; i < n; i += 32 * CW) {
         const float r = part(i)[COLS * D + h], s = part(i)[COLS * D + COLS + h], m = fmaxf(top, r);
@@ -614,6 +653,7 @@ template <int G, bool FINE> static int launch_decode(const DecodeParams &p, int6
         allowed.fetch_or(1ull << dev, std::memory_order_release);
     }
     if (int rc = launch_dependent(kv4_decode_kernel<G, FINE>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G>), st, p)) return rc;
+    if (p.whole) return 0;
     return launch_dependent(kv4_combine_kernel<G>, dim3(p.c.H * p.col_blocks * COLS, p.s.B), 32 * CW, 0, st, p, (int)blocks);
 }
 
@@ -649,8 +689,14 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     int64_t tiles = (int64_t)p.s.max_pages * p.c.parts;
     if (a->max_seq_len > 0) tiles = tiles < (a->max_seq_len + 15LL) / 16 ? tiles : (a->max_seq_len + 15LL) / 16;
     if (p.selected) tiles = tiles < (int64_t)p.num_selected * p.c.parts ? tiles : (int64_t)p.num_selected * p.c.parts;
-    const int64_t most = (tiles * p.s.B * p.c.H * p.col_blocks + p.least - 1) / p.least, hold = most_blocks();
-    const int64_t blocks = most < 1 ? 1 : most < hold ? most : hold;
+    const int64_t rows = (int64_t)p.s.B * p.c.H * p.col_blocks;
+    if (tiles * rows >= 1LL << 31 || rows * COLS >= 1LL << 31)
+        return fail(OMMX_E_UNSUPPORTED, "kv4_decode: %lld rows of up to %lld records (2^31 in all are counted): give max_seq_len", (long long)rows, (long long)tiles);
+    // As many blocks as the SMs hold, no more than the work can have. Rows that are short for certain go whole to a block each, and
+    // the second kernel is not needed.
+    p.whole = tiles <= WHOLE;
+    const int64_t most = (tiles * rows + p.least - 1) / p.least, hold = most_blocks();
+    const int64_t blocks = p.whole ? rows : most < 1 ? 1 : most < hold ? most : hold;
     if (a->o_dtype == OMMX_DT_BF16) return a->cache.head_dim == 64 ? launch_decode<2, false>(p, blocks, st) : launch_decode<4, false>(p, blocks, st);
     return a->cache.head_dim == 64 ? launch_decode<2, true>(p, blocks, st) : launch_decode<4, true>(p, blocks, st);
 }
