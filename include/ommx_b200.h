@@ -439,16 +439,18 @@ typedef struct ommx_kv4_decode_args {
     const int32_t *selected;        /* [batch, n_kv_heads, num_selected] places of pages in their sequence, or NULL: all pages.  The first
                                        min(num_selected, pages of the sequence) count; one below 0 is passed over */
     int32_t num_selected;
-    float *workspace;               /* ommx_b200_kv4_workspace_floats() of them, 16-byte aligned; calls that overlap need their own */
+    float *workspace;               /* 16-byte aligned; calls that overlap need their own */
     int64_t workspace_floats;
     int32_t max_seq_len;            /* an upper bound of b_seq_len that sizes the grid, 0: what the table can hold */
     float sm_scale, logit_cap;      /* logits: cap * tanh(q.k * sm_scale / cap); cap 0: none */
     int32_t *status;
 } ommx_kv4_decode_args;
 
-/* Attention of one query row per sequence over the cache, or over selected pages of it.  Two launches. */
+/* Attention of one query row per sequence over the cache, or over selected pages of it.  Two launches; one where no sequence has
+ * more than 512 tokens by max_seq_len, the table's width or num_selected. */
 int ommx_b200_kv4_decode(const ommx_kv4_decode_args *args, void *stream);
-/* floats of workspace that a decode call needs on the current device */
+/* floats of workspace that this call needs on the current device (0: none; its pointers are not looked at), and that any call needs */
+int64_t ommx_b200_kv4_decode_workspace_floats(const ommx_kv4_decode_args *args);
 int64_t ommx_b200_kv4_workspace_floats(int32_t head_dim);
 
 typedef struct ommx_kv4_select_args {

@@ -149,6 +149,7 @@ SYMBOLS = {
     "ommx_b200_kv4_append": (C.c_int, [C.POINTER(KV4AppendArgs), C.c_void_p]),
     "ommx_b200_kv4_gather": (C.c_int, [C.POINTER(KV4GatherArgs), C.c_void_p]),
     "ommx_b200_kv4_decode": (C.c_int, [C.POINTER(KV4DecodeArgs), C.c_void_p]),
+    "ommx_b200_kv4_decode_workspace_floats": (C.c_int64, [C.POINTER(KV4DecodeArgs)]),
     "ommx_b200_kv4_workspace_floats": (C.c_int64, [C.c_int32]),
     "ommx_b200_kv4_select": (C.c_int, [C.POINTER(KV4SelectArgs), C.c_void_p]),
     "ommx_b200_kv4_select_workspace_bytes": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),

@@ -98,8 +98,8 @@ def ommx_kv4_decode_attention(q: torch.Tensor, records: torch.Tensor, page_table
     ``D ** -0.5``; ``logit_cap`` c makes a logit ``c tanh(x / c)``.  A sequence of no tokens gives ``o = 0``, ``lse = -inf``.
     ``selected`` (int32 ``[batch, n_kv_heads, n]``, as ``ommx_kv4_select_pages`` writes it) limits a kv head to these places of
     the page table; the first ``min(n, pages)`` entries count, one below 0 is passed over, one listed twice counts twice.
-    ``max_seq_len`` sizes the grid (the table's width without it); ``workspace`` (fp32, ``kv4_workspace_floats(D)`` values) is
-    allocated per call when not given; calls that run side by side need their own."""
+    ``max_seq_len`` sizes the grid (the table's width without it; up to 512 tokens it is one launch); ``workspace`` (fp32,
+    ``kv4_workspace_floats(D)`` values) is allocated per call when needed and not given; calls that run side by side need their own."""
     _check((_HOST or _host()).kv4_decode(q, records, page_table, b_seq_len, o, lse, sm_scale, logit_cap, selected, workspace, max_seq_len, status),
            "ommx_b200_kv4_decode")
 

@@ -607,9 +607,13 @@ std::string shape_text(const Tensor &t) {
     return s + "]";
 }
 
+// the text is made only where it is needed: a dozen strings were 3 us of a call
+#define KV4_EXPECT(call, ok, ...) do { if (!(ok)) (call).wrong(__VA_ARGS__); } while (0)
+
 struct KV4Call {
     const char *who;
-    std::vector<std::pair<const char *, const Tensor *>> given;            // whose devices are compared at the end
+    std::pair<const char *, const Tensor *> given[24] = {};                 // whose devices are compared at the end
+    int n_given = 0;
 
     const Tensor *tensor(PyObject *o, const char *name, bool needed = true) {
         if (o == Py_None) {
@@ -618,14 +622,14 @@ struct KV4Call {
         }
         const Tensor *t = as_tensor(o);
         if (!t) throw Refusal{PyExc_TypeError, std::string(who) + ": " + name + " must be a tensor"};
-        given.emplace_back(name, t);
+        if (n_given < 24) given[n_given++] = {name, t};
         return t;
     }
-    void expect(bool ok, const std::string &text) const { if (!ok) refuse(std::string(who) + ": " + text); }
+    [[noreturn]] void wrong(const std::string &text) const { refuse(std::string(who) + ": " + text); }
     int64_t integer(PyObject *o, const char *name, int64_t lo) const {
         int64_t v = 0;
         if (!as_long(o, &v)) throw Refusal{PyExc_TypeError, std::string(who) + ": " + name + " must be an integer"};
-        expect(v >= lo && v <= INT32_MAX, std::string(name) + " = " + std::to_string(v) + " is out of range");
+        KV4_EXPECT(*this, v >= lo && v <= INT32_MAX, std::string(name) + " = " + std::to_string(v) + " is out of range");
         return v;
     }
     double number(PyObject *o, const char *name) const {
@@ -637,21 +641,21 @@ struct KV4Call {
     const Tensor *rows(PyObject *o, const char *name, int64_t a, int64_t b, int64_t d, at::ScalarType type, bool needed = true) {
         const Tensor *t = tensor(o, name, needed);
         if (!t) return t;
-        expect(t->dim() == 3 && t->size(0) == a && t->size(1) == b && t->size(2) == d,
+        KV4_EXPECT(*this, t->dim() == 3 && t->size(0) == a && t->size(1) == b && t->size(2) == d,
                std::string(name) + " is " + shape_text(*t) + ", wanted [" + std::to_string(a) + ", " + std::to_string(b) + ", " + std::to_string(d) + "]");
-        expect(t->scalar_type() == type, std::string(name) + " has another dtype than it should: " + c10::toString(t->scalar_type()) + ", wanted " + c10::toString(type));
-        expect(t->size(2) <= 1 || t->stride(2) == 1, std::string(name) + "'s last dimension must be contiguous");
+        KV4_EXPECT(*this, t->scalar_type() == type, std::string(name) + " has another dtype than it should: " + c10::toString(t->scalar_type()) + ", wanted " + c10::toString(type));
+        KV4_EXPECT(*this, t->size(2) <= 1 || t->stride(2) == 1, std::string(name) + "'s last dimension must be contiguous");
         return t;
     }
     // rows that a kernel writes: no two of them in one place
     void distinct(const Tensor &t, const char *name) const {
-        for (int i = 0; i < 2; ++i) expect(t.size(i) <= 1 || t.stride(i) != 0, std::string(name) + " must not be expanded: its rows are written");
+        for (int i = 0; i < 2; ++i) KV4_EXPECT(*this, t.size(i) <= 1 || t.stride(i) != 0, std::string(name) + " must not be expanded: its rows are written");
     }
     void records(PyObject *o, ommx_kv4_cache *c) {
         const Tensor *t = tensor(o, "records");
-        expect(t->dim() == 4 && t->scalar_type() == at::kByte && t->is_contiguous(), "records must be a contiguous uint8 tensor [pages, kv heads, page_size / 16, 20 * head_dim]");
+        KV4_EXPECT(*this, t->dim() == 4 && t->scalar_type() == at::kByte && t->is_contiguous(), "records must be a contiguous uint8 tensor [pages, kv heads, page_size / 16, 20 * head_dim]");
         const int64_t D = t->size(3) / 20;
-        expect(t->size(3) == 20 * D && t->size(0) <= INT32_MAX && t->size(1) > 0 && t->size(1) <= 4096 && t->size(2) >= 1 && t->size(2) <= 16,
+        KV4_EXPECT(*this, t->size(3) == 20 * D && t->size(0) <= INT32_MAX && t->size(1) > 0 && t->size(1) <= 4096 && t->size(2) >= 1 && t->size(2) <= 16,
                "records is " + shape_text(*t) + ", wanted [pages, kv heads, page_size / 16, 20 * head_dim]");
         c->records = t->data_ptr();
         c->num_pages = (int32_t)t->size(0); c->n_kv_heads = (int32_t)t->size(1); c->page_size = 16 * (int32_t)t->size(2); c->head_dim = (int32_t)D;
@@ -659,17 +663,17 @@ struct KV4Call {
     void summary(PyObject *o, const ommx_kv4_cache &c, void **to) {
         const Tensor *t = tensor(o, "summary", false);
         if (!t) return;
-        expect(t->dim() == 4 && t->scalar_type() == at::kBFloat16 && t->is_contiguous() && t->size(0) == c.num_pages && t->size(1) == c.n_kv_heads && t->size(2) == 2 &&
+        KV4_EXPECT(*this, t->dim() == 4 && t->scalar_type() == at::kBFloat16 && t->is_contiguous() && t->size(0) == c.num_pages && t->size(1) == c.n_kv_heads && t->size(2) == 2 &&
                    t->size(3) == c.head_dim, "summary must be a contiguous bfloat16 tensor [pages, kv heads, 2, head_dim] of the records' sizes");
         *to = t->data_ptr();
     }
     void seqs(PyObject *table, PyObject *len, ommx_kv4_seqs *s) {
         const Tensor *l = tensor(len, "b_seq_len"), *t = tensor(table, "page_table");
-        expect(l->dim() == 1 && l->scalar_type() == at::kInt && l->is_contiguous(), "b_seq_len must be a contiguous int32 tensor [batch]");
-        expect(t->dim() == 2 && (t->scalar_type() == at::kInt || t->scalar_type() == at::kLong) && (t->size(1) <= 1 || t->stride(1) == 1),
+        KV4_EXPECT(*this, l->dim() == 1 && l->scalar_type() == at::kInt && l->is_contiguous(), "b_seq_len must be a contiguous int32 tensor [batch]");
+        KV4_EXPECT(*this, t->dim() == 2 && (t->scalar_type() == at::kInt || t->scalar_type() == at::kLong) && (t->size(1) <= 1 || t->stride(1) == 1),
                "page_table must be an int32 or int64 tensor [batch, pages] with contiguous rows");
-        expect(t->size(0) == l->size(0), "page_table has " + std::to_string(t->size(0)) + " rows for " + std::to_string(l->size(0)) + " lengths");
-        expect(l->size(0) <= INT32_MAX && t->size(1) <= INT32_MAX, "too many sequences or pages");
+        KV4_EXPECT(*this, t->size(0) == l->size(0), "page_table has " + std::to_string(t->size(0)) + " rows for " + std::to_string(l->size(0)) + " lengths");
+        KV4_EXPECT(*this, l->size(0) <= INT32_MAX && t->size(1) <= INT32_MAX, "too many sequences or pages");
         s->b_seq_len = (const int32_t *)l->data_ptr();
         s->page_table = t->data_ptr(); s->page_table_stride = t->stride(0); s->table_is_int64 = t->scalar_type() == at::kLong;
         s->pages_per_seq = (int32_t)t->size(1); s->batch = (int32_t)l->size(0);
@@ -677,16 +681,16 @@ struct KV4Call {
     const int32_t *row_start(PyObject *o, int64_t batch, int64_t rows) {
         const Tensor *t = tensor(o, "row_start", false);
         if (!t) {
-            expect(rows == batch, "without row_start there is one row for each of the " + std::to_string(batch) + " sequences, not " + std::to_string(rows));
+            KV4_EXPECT(*this, rows == batch, "without row_start there is one row for each of the " + std::to_string(batch) + " sequences, not " + std::to_string(rows));
             return nullptr;
         }
-        expect(t->dim() == 1 && t->scalar_type() == at::kInt && t->is_contiguous() && t->size(0) == batch + 1, "row_start must be a contiguous int32 tensor [batch + 1]");
+        KV4_EXPECT(*this, t->dim() == 1 && t->scalar_type() == at::kInt && t->is_contiguous() && t->size(0) == batch + 1, "row_start must be a contiguous int32 tensor [batch + 1]");
         return (const int32_t *)t->data_ptr();
     }
     int32_t *status(PyObject *o) {
         const Tensor *t = tensor(o, "status", false);
         if (!t) return nullptr;
-        expect(t->scalar_type() == at::kInt && t->numel() >= 1, "status must be an int32 tensor");
+        KV4_EXPECT(*this, t->scalar_type() == at::kInt && t->numel() >= 1, "status must be an int32 tensor");
         return (int32_t *)t->data_ptr();
     }
     // a workspace of the caller's, or one of this call
@@ -698,15 +702,16 @@ struct KV4Call {
             *own = fresh({need}, at::TensorOptions().device(dev).dtype(type));
             return own->data_ptr();
         }
-        expect(t->scalar_type() == type && t->is_contiguous() && t->numel() >= need,
+        KV4_EXPECT(*this, t->scalar_type() == type && t->is_contiguous() && t->numel() >= need,
                std::string("workspace must be a contiguous ") + c10::toString(type) + " tensor of at least " + std::to_string(need) + " values");
         return t->data_ptr();
     }
     at::Device device() const {
-        const at::Device dev = given.front().second->device();
-        for (auto &g : given) {
+        const at::Device dev = given[0].second->device();
+        for (int i = 0; i < n_given; ++i) {
+            const auto &g = given[i];
             if (!g.second->is_cuda()) throw Refusal{PyExc_RuntimeError, std::string(who) + " needs CUDA tensors (no CPU path): " + g.first + " is on " + g.second->device().str()};
-            expect(g.second->device() == dev, std::string(g.first) + " is on " + g.second->device().str() + ", " + given.front().first + " on " + dev.str());
+            KV4_EXPECT(*this, g.second->device() == dev, std::string(g.first) + " is on " + g.second->device().str() + ", " + given[0].first + " on " + dev.str());
         }
         return dev;
     }
@@ -717,7 +722,7 @@ void head_size(const KV4Call &c, const ommx_kv4_cache &k) {
 }
 int32_t type_code(const KV4Call &c, const Tensor &t, const char *name, bool f32) {
     int32_t code = 0;
-    c.expect(dtype_code(t, &code) && (f32 || code != OMMX_DT_F32), std::string(name) + " must be bfloat16" + (f32 ? ", float16 or float32" : " or float16"));
+    KV4_EXPECT(c, dtype_code(t, &code) && (f32 || code != OMMX_DT_F32), std::string(name) + " must be bfloat16" + (f32 ? ", float16 or float32" : " or float16"));
     return code;
 }
 #define KV4_TRY try {
@@ -735,7 +740,7 @@ PyObject *py_kv4_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     head_size(c, d.cache);
     c.seqs(a[3], a[4], &d.seqs);
     const Tensor *k = c.tensor(a[0], "k_new");
-    c.expect(k->dim() == 3 && k->size(0) <= INT32_MAX, "k_new must be [rows, kv heads, head_dim]");
+    KV4_EXPECT(c, k->dim() == 3 && k->size(0) <= INT32_MAX, "k_new must be [rows, kv heads, head_dim]");
     d.dtype = type_code(c, *k, "k_new", true);
     const int64_t T = k->size(0), H = d.cache.n_kv_heads, D = d.cache.head_dim;
     k = c.rows(a[0], "k_new", T, H, D, k->scalar_type());
@@ -744,37 +749,37 @@ PyObject *py_kv4_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     d.k_stride_t = k->stride(0); d.k_stride_h = k->stride(1); d.v_stride_t = v->stride(0); d.v_stride_h = v->stride(1);
     d.row_start = c.row_start(a[5], d.seqs.batch, T);
     const Tensor *cos = c.tensor(a[8], "cos", false), *sin = c.tensor(a[9], "sin", false), *q = c.tensor(a[6], "q", false);
-    c.expect(!cos == !sin, "cos and sin come together");
+    KV4_EXPECT(c, !cos == !sin, "cos and sin come together");
     if (cos) {
         for (const Tensor *t : {cos, sin})
-            c.expect(t->dim() == 2 && t->scalar_type() == at::kFloat && (t->size(1) <= 1 || t->stride(1) == 1), "cos and sin must be float32 tensors [positions, rot_dim / 2] with contiguous rows");
-        c.expect(cos->sizes() == sin->sizes() && cos->strides() == sin->strides() && cos->size(0) >= 1 && cos->size(0) <= INT32_MAX, "cos and sin must have the same size and strides, and a row");
-        c.expect(((uintptr_t)cos->data_ptr() | (uintptr_t)sin->data_ptr() | (uintptr_t)(cos->stride(0) * 4)) % 16 == 0, "rows of cos and sin must start on 16-byte boundaries");
-        c.expect(2 * cos->size(1) <= D, "cos and sin turn " + std::to_string(2 * cos->size(1)) + " channels of heads of " + std::to_string(D));
+            KV4_EXPECT(c, t->dim() == 2 && t->scalar_type() == at::kFloat && (t->size(1) <= 1 || t->stride(1) == 1), "cos and sin must be float32 tensors [positions, rot_dim / 2] with contiguous rows");
+        KV4_EXPECT(c, cos->sizes() == sin->sizes() && cos->strides() == sin->strides() && cos->size(0) >= 1 && cos->size(0) <= INT32_MAX, "cos and sin must have the same size and strides, and a row");
+        KV4_EXPECT(c, ((uintptr_t)cos->data_ptr() | (uintptr_t)sin->data_ptr() | (uintptr_t)(cos->stride(0) * 4)) % 16 == 0, "rows of cos and sin must start on 16-byte boundaries");
+        KV4_EXPECT(c, 2 * cos->size(1) <= D, "cos and sin turn " + std::to_string(2 * cos->size(1)) + " channels of heads of " + std::to_string(D));
         const int64_t rot = 2 * cos->size(1);
         if (rot != 32 && rot != 64 && rot != 128) throw Refusal{PyExc_NotImplementedError, "ommx_kv4_append: a rotation of " + std::to_string(rot) + " channels (this build rotates 32, 64 or 128)"};
         d.cos = (const float *)cos->data_ptr(); d.sin = (const float *)sin->data_ptr(); d.cs_stride = cos->stride(0);
         d.num_positions = (int32_t)cos->size(0); d.rot_dim = (int32_t)rot;
     }
     bool interleaved = false;
-    c.expect(as_bool(a[11], &interleaved), "interleaved must be a truth value");
+    KV4_EXPECT(c, as_bool(a[11], &interleaved), "interleaved must be a truth value");
     d.interleaved = interleaved;
     if (const Tensor *pos = c.tensor(a[10], "positions", false)) {
-        c.expect(cos != nullptr, "positions without cos and sin");
-        c.expect(pos->dim() == 1 && pos->size(0) == T && (T <= 1 || pos->stride(0) == 1) && (pos->scalar_type() == at::kInt || pos->scalar_type() == at::kLong),
+        KV4_EXPECT(c, cos != nullptr, "positions without cos and sin");
+        KV4_EXPECT(c, pos->dim() == 1 && pos->size(0) == T && (T <= 1 || pos->stride(0) == 1) && (pos->scalar_type() == at::kInt || pos->scalar_type() == at::kLong),
                  "positions must be a contiguous int32 or int64 tensor of one value for each row");
         d.positions = pos->data_ptr(); d.positions_is_int64 = pos->scalar_type() == at::kLong;
     }
     Tensor fresh_q;
     const Tensor *out = nullptr;
     if (q) {
-        c.expect(cos != nullptr, "q without cos and sin: there is nothing to do to it");
-        c.expect(q->dim() == 3 && q->size(1) >= 1, "q must be [rows, query heads, head_dim]");
+        KV4_EXPECT(c, cos != nullptr, "q without cos and sin: there is nothing to do to it");
+        KV4_EXPECT(c, q->dim() == 3 && q->size(1) >= 1, "q must be [rows, query heads, head_dim]");
         q = c.rows(a[6], "q", T, q->size(1), D, k->scalar_type());
         out = c.rows(a[7], "q_out", T, q->size(1), D, k->scalar_type(), false);
         if (out) c.distinct(*out, "q_out");
     } else {
-        c.expect(a[7] == Py_None, "q_out without q");
+        KV4_EXPECT(c, a[7] == Py_None, "q_out without q");
     }
     c.summary(a[12], d.cache, &d.cache.summary);
     d.status = c.status(a[13]);
@@ -809,7 +814,7 @@ PyObject *py_kv4_gather(PyObject *, PyObject *const *a, Py_ssize_t n) {
     head_size(c, d.cache);
     c.seqs(a[1], a[2], &d.seqs);
     const Tensor *k = c.tensor(a[3], "k_out");
-    c.expect(k->dim() == 3 && k->size(0) <= INT32_MAX, "k_out must be [rows, kv heads, head_dim]");
+    KV4_EXPECT(c, k->dim() == 3 && k->size(0) <= INT32_MAX, "k_out must be [rows, kv heads, head_dim]");
     d.dtype = type_code(c, *k, "k_out", true);
     const int64_t T = k->size(0), H = d.cache.n_kv_heads, D = d.cache.head_dim;
     k = c.rows(a[3], "k_out", T, H, D, k->scalar_type());
@@ -838,7 +843,7 @@ PyObject *py_kv4_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
     c.seqs(a[2], a[3], &d.seqs);
     const int64_t B = d.seqs.batch, H = d.cache.n_kv_heads, D = d.cache.head_dim;
     const Tensor *q = c.tensor(a[0], "q");
-    c.expect(q->dim() == 3 && q->size(1) <= INT32_MAX, "q must be [batch, query heads, head_dim]");
+    KV4_EXPECT(c, q->dim() == 3 && q->size(1) <= INT32_MAX, "q must be [batch, query heads, head_dim]");
     d.q_dtype = type_code(c, *q, "q", false);
     const int64_t Hq = q->size(1);
     q = c.rows(a[0], "q", B, Hq, D, q->scalar_type());
@@ -848,19 +853,19 @@ PyObject *py_kv4_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
     o = c.rows(a[4], "o", B, Hq, D, o->scalar_type());
     c.distinct(*o, "o");
     const Tensor *lse = c.tensor(a[5], "lse");
-    c.expect(lse->dim() == 2 && lse->size(0) == B && lse->size(1) == Hq && lse->scalar_type() == at::kFloat && (Hq <= 1 || lse->stride(1) == 1) && (B <= 1 || lse->stride(0) >= Hq),
+    KV4_EXPECT(c, lse->dim() == 2 && lse->size(0) == B && lse->size(1) == Hq && lse->scalar_type() == at::kFloat && (Hq <= 1 || lse->stride(1) == 1) && (B <= 1 || lse->stride(0) >= Hq),
              "lse must be a float32 tensor [batch, query heads] with contiguous rows");
     d.q = q->data_ptr(); d.n_q_heads = (int32_t)Hq; d.q_stride_b = q->stride(0); d.q_stride_h = q->stride(1);
     d.o = o->data_ptr(); d.o_stride_b = o->stride(0); d.o_stride_h = o->stride(1);
     d.lse = (float *)lse->data_ptr(); d.lse_stride_b = lse->stride(0);
     d.sm_scale = (float)(a[6] == Py_None ? 1.0 / std::sqrt((double)D) : c.number(a[6], "sm_scale"));
     d.logit_cap = (float)c.number(a[7], "logit_cap");
-    c.expect(d.logit_cap >= 0.0f, "logit_cap must not be negative");
+    KV4_EXPECT(c, d.logit_cap >= 0.0f, "logit_cap must not be negative");
     if (const Tensor *sel = c.tensor(a[8], "selected", false)) {
-        c.expect(sel->dim() == 3 && sel->scalar_type() == at::kInt && sel->is_contiguous() && sel->size(0) == B && sel->size(1) == H && sel->size(2) <= INT32_MAX,
+        KV4_EXPECT(c, sel->dim() == 3 && sel->scalar_type() == at::kInt && sel->is_contiguous() && sel->size(0) == B && sel->size(1) == H && sel->size(2) <= INT32_MAX,
                  "selected must be a contiguous int32 tensor [batch, kv heads, pages]");
         // no list of no pages: every sequence is then one of no tokens, and a null pointer would mean all of them
-        c.expect(sel->size(2) >= 1, "selected must have room for a page");
+        KV4_EXPECT(c, sel->size(2) >= 1, "selected must have room for a page");
         d.selected = (const int32_t *)sel->data_ptr(); d.num_selected = (int32_t)sel->size(2);
     }
     if (a[10] != Py_None) d.max_seq_len = (int32_t)c.integer(a[10], "max_seq_len", 0);
@@ -870,7 +875,7 @@ PyObject *py_kv4_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
     Tensor own;
     {
         const c10::cuda::CUDAGuard guard(dev);
-        d.workspace_floats = ommx_b200_kv4_workspace_floats((int32_t)D);
+        d.workspace_floats = ommx_b200_kv4_decode_workspace_floats(&d);
     }
     d.workspace = (float *)c.workspace(a[9], at::kFloat, d.workspace_floats, dev, &own);
     return PyLong_FromLong(launch(dev, [&](void *stream) { return ommx_b200_kv4_decode(&d, stream); }));
@@ -887,7 +892,7 @@ PyObject *py_kv4_select(PyObject *, PyObject *const *a, Py_ssize_t n) {
     ommx_kv4_select_args d;
     memset(&d, 0, sizeof(d));
     const Tensor *sum = c.tensor(a[1], "summary");
-    c.expect(sum->dim() == 4 && sum->scalar_type() == at::kBFloat16 && sum->is_contiguous() && sum->size(2) == 2 && sum->size(0) <= INT32_MAX && sum->size(1) >= 1 && sum->size(1) <= 4096,
+    KV4_EXPECT(c, sum->dim() == 4 && sum->scalar_type() == at::kBFloat16 && sum->is_contiguous() && sum->size(2) == 2 && sum->size(0) <= INT32_MAX && sum->size(1) >= 1 && sum->size(1) <= 4096,
              "summary must be a contiguous bfloat16 tensor [pages, kv heads, 2, head_dim]");
     d.cache.summary = sum->data_ptr(); d.cache.records = d.cache.summary;   // not read
     d.cache.num_pages = (int32_t)sum->size(0); d.cache.n_kv_heads = (int32_t)sum->size(1); d.cache.head_dim = (int32_t)std::min<int64_t>(sum->size(3), INT32_MAX);
@@ -896,18 +901,18 @@ PyObject *py_kv4_select(PyObject *, PyObject *const *a, Py_ssize_t n) {
     c.seqs(a[2], a[3], &d.seqs);
     const int64_t B = d.seqs.batch, H = d.cache.n_kv_heads, D = d.cache.head_dim;
     const Tensor *q = c.tensor(a[0], "q");
-    c.expect(q->dim() == 3 && q->size(1) <= INT32_MAX, "q must be [batch, query heads, head_dim]");
+    KV4_EXPECT(c, q->dim() == 3 && q->size(1) <= INT32_MAX, "q must be [batch, query heads, head_dim]");
     d.q_dtype = type_code(c, *q, "q", false);
     const int64_t Hq = q->size(1);
     q = c.rows(a[0], "q", B, Hq, D, q->scalar_type());
     if (Hq < H || Hq % H) throw Refusal{PyExc_NotImplementedError, "ommx_kv4_select_pages: " + std::to_string(Hq) + " query heads are not a multiple of " + std::to_string(H) + " kv heads"};
     const Tensor *sel = c.tensor(a[4], "selected");
-    c.expect(sel->dim() == 3 && sel->scalar_type() == at::kInt && sel->is_contiguous() && sel->size(0) == B && sel->size(1) == H && sel->size(2) <= INT32_MAX,
+    KV4_EXPECT(c, sel->dim() == 3 && sel->scalar_type() == at::kInt && sel->is_contiguous() && sel->size(0) == B && sel->size(1) == H && sel->size(2) <= INT32_MAX,
              "selected must be a contiguous int32 tensor [batch, kv heads, pages]");
     d.q = q->data_ptr(); d.n_q_heads = (int32_t)Hq; d.q_stride_b = q->stride(0); d.q_stride_h = q->stride(1);
     d.selected = (int32_t *)sel->data_ptr(); d.num_selected = (int32_t)sel->size(2);
     d.first_pages = (int32_t)c.integer(a[6], "first_pages", 0); d.last_pages = (int32_t)c.integer(a[7], "last_pages", 0);
-    c.expect((int64_t)d.first_pages + d.last_pages <= d.num_selected, "first_pages and last_pages must fit into the " + std::to_string(d.num_selected) + " selected ones");
+    KV4_EXPECT(c, (int64_t)d.first_pages + d.last_pages <= d.num_selected, "first_pages and last_pages must fit into the " + std::to_string(d.num_selected) + " selected ones");
     d.status = c.status(a[9]);
     if (a[8] != Py_None) c.tensor(a[8], "workspace");
     const at::Device dev = c.device();

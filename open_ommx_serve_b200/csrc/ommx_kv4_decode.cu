@@ -657,6 +657,16 @@ template <int G, bool FINE> static int launch_decode(const DecodeParams &p, int6
     return launch_dependent(kv4_combine_kernel<G>, dim3(p.c.H * p.col_blocks * COLS, p.s.B), 32 * CW, 0, st, p, (int)blocks);
 }
 
+// records that a row of the call can have
+static int64_t most_units(const ommx_kv4_decode_args *a) {
+    const int64_t parts = a->cache.page_size / 16;
+    int64_t n = a->seqs.pages_per_seq * parts;
+    if (a->max_seq_len > 0) n = n < (a->max_seq_len + 15LL) / 16 ? n : (a->max_seq_len + 15LL) / 16;
+    if (a->selected) n = n < a->num_selected * parts ? n : a->num_selected * parts;
+    return n;
+}
+static int64_t workspace_floats(const ommx_kv4_decode_args *a) { return most_units(a) <= WHOLE ? 0 : workspace_floats(a->cache.head_dim); }
+
 static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     if (!a) return fail(OMMX_E_ARG, "kv4_decode: null args");
     DecodeParams p;
@@ -672,8 +682,9 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     if (p.s.B > 65535) return fail(OMMX_E_UNSUPPORTED, "kv4_decode: a batch of %d", p.s.B);
     if (p.s.B == 0) return 0;
     if (!a->q || !a->o || !a->lse) return fail(OMMX_E_ARG, "kv4_decode: q, o and lse must not be null");
-    if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 || a->workspace_floats < workspace_floats(a->cache.head_dim))
-        return fail(OMMX_E_ARG, "kv4_decode: workspace must be 16-byte aligned and hold %lld floats", (long long)workspace_floats(a->cache.head_dim));
+    const int64_t need = workspace_floats(a);
+    if (need && (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 || a->workspace_floats < need))
+        return fail(OMMX_E_ARG, "kv4_decode: workspace must be 16-byte aligned and hold %lld floats", (long long)need);
     p.q = a->q; p.q16 = a->q_dtype == OMMX_DT_F16; p.q_b = a->q_stride_b; p.q_h = a->q_stride_h;
     p.q_wide = (reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)(2 * p.q_b) | (uintptr_t)(2 * p.q_h)) % 16 == 0;
     p.o = a->o; p.o_type = a->o_dtype; p.o_b = a->o_stride_b; p.o_h = a->o_stride_h;
@@ -683,19 +694,17 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     p.Hq = a->n_q_heads; p.group = a->n_q_heads / p.c.H; p.col_blocks = (p.group + COLS - 1) / COLS;
     p.page_shift = shift_of(p.c.page);
     p.sm_scale = a->sm_scale; p.cap = a->logit_cap; p.status = a->status;
-    if (p.c.num_pages == 0) p.c.records = reinterpret_cast<uint8_t *>(p.work);   // what is fetched for a page that is not there
+    if (p.c.num_pages == 0) return fail(OMMX_E_ARG, "kv4_decode: a cache of no pages");   // what is fetched for a page that is not there
     p.least = NW;
     // as many blocks as the SMs hold, no more than the work can have
-    int64_t tiles = (int64_t)p.s.max_pages * p.c.parts;
-    if (a->max_seq_len > 0) tiles = tiles < (a->max_seq_len + 15LL) / 16 ? tiles : (a->max_seq_len + 15LL) / 16;
-    if (p.selected) tiles = tiles < (int64_t)p.num_selected * p.c.parts ? tiles : (int64_t)p.num_selected * p.c.parts;
+    const int64_t units = most_units(a);
     const int64_t rows = (int64_t)p.s.B * p.c.H * p.col_blocks;
-    if (tiles * rows >= 1LL << 31 || rows * COLS >= 1LL << 31)
-        return fail(OMMX_E_UNSUPPORTED, "kv4_decode: %lld rows of up to %lld records (2^31 in all are counted): give max_seq_len", (long long)rows, (long long)tiles);
+    if (units * rows >= 1LL << 31 || rows * COLS >= 1LL << 31)
+        return fail(OMMX_E_UNSUPPORTED, "kv4_decode: %lld rows of up to %lld records (2^31 in all are counted): give max_seq_len", (long long)rows, (long long)units);
     // As many blocks as the SMs hold, no more than the work can have. Rows that are short for certain go whole to a block each, and
     // the second kernel is not needed.
-    p.whole = tiles <= WHOLE;
-    const int64_t most = (tiles * rows + p.least - 1) / p.least, hold = most_blocks();
+    p.whole = units <= WHOLE;
+    const int64_t most = (units * rows + p.least - 1) / p.least, hold = most_blocks();
     const int64_t blocks = p.whole ? rows : most < 1 ? 1 : most < hold ? most : hold;
     if (a->o_dtype == OMMX_DT_BF16) return a->cache.head_dim == 64 ? launch_decode<2, false>(p, blocks, st) : launch_decode<4, false>(p, blocks, st);
     return a->cache.head_dim == 64 ? launch_decode<2, true>(p, blocks, st) : launch_decode<4, true>(p, blocks, st);
@@ -704,5 +713,8 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
 }  // namespace kv4
 }  // namespace ommx
 
+extern "C" int64_t ommx_b200_kv4_decode_workspace_floats(const ommx_kv4_decode_args *args) {
+    return !args || (args->cache.head_dim != 64 && args->cache.head_dim != 128) ? 0 : ommx::kv4::workspace_floats(args);
+}
 extern "C" int64_t ommx_b200_kv4_workspace_floats(int32_t head_dim) { return head_dim == 64 || head_dim == 128 ? ommx::kv4::workspace_floats(head_dim) : 0; }
 extern "C" int ommx_b200_kv4_decode(const ommx_kv4_decode_args *args, void *stream) { return ommx::kv4::decode(args, (cudaStream_t)stream); }

@@ -9,7 +9,8 @@
 namespace ommx {
 namespace kv4 {
 
-constexpr int SCORE_WARPS = 4, PICK_THREADS = 1024;
+constexpr int SCORE_WARPS = 8, PICK_THREADS = 1024;
+constexpr int MOST_HEADS = 160;                   // query heads to a kv head: their fragments lie in 40 KB of shared memory
 
 struct SelectParams {
     Cache c;
@@ -19,7 +20,7 @@ struct SelectParams {
     int64_t q_b, q_h;
     uint32_t *keys;                               // [B][H][max_pages]
     int32_t *selected;
-    int32_t q16, group, col_blocks, n, first, last, page_shift;
+    int32_t q16, q_wide, group, col_blocks, n, first, last, page_shift;
     int32_t *status;
 };
 
@@ -34,9 +35,17 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t b = __float_as_uint(x);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float load_q(const SelectParams &p, int64_t at) {
-    if (p.q16) return __half2float(reinterpret_cast<const __half *>(p.q)[at]);
-    return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p.q)[at]);
+// eight channels of a query
+__device__ __forceinline__ void load_q8(const SelectParams &p, int64_t at, float *x) {
+    alignas(16) uint16_t v[8];
+    if (p.q_wide) {
+        *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p.q) + at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = reinterpret_cast<const uint16_t *>(p.q)[at + i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p.q16 ? __half2float(__ushort_as_half(v[i])) : __uint_as_float((uint32_t)v[i] << 16);
 }
 __device__ __forceinline__ void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -58,93 +67,128 @@ __device__ __forceinline__ uint32_t bytes_of(uint32_t x01, uint32_t x23, uint32_
     return __byte_perm(fma_bf16x2(x01, cc, MAGIC), fma_bf16x2(x23, cc, MAGIC), 0x6420) & 0x7F7F7F7Fu;
 }
 
+// A kv head's queries in 8 bits, as B fragments of lane (g, t) = head g, channels 32 j + 8 t + 0..7: what is above 0, and what is below.
+// The whole block calls it; sums: of a head's channels.
+template <int G> __device__ __forceinline__ void quantize_query(const SelectParams &p, int b, int h, uint4 *frag, int *sums, uint32_t *top) {
+    constexpr int D = 32 * G, CHUNKS = D / 8, THREADS = 32 * SCORE_WARPS;
+    const int chunks = p.group * CHUNKS;
+    for (int i = threadIdx.x; i < p.col_blocks * 8; i += THREADS) sums[i] = 0;
+    if (threadIdx.x == 0) *top = 0;
+    for (int i = chunks + threadIdx.x; i < p.col_blocks * 8 * CHUNKS; i += THREADS)         // heads that are not there
+        frag[((i / CHUNKS / 8) * G + i % CHUNKS / 4) * 32 + (i / CHUNKS % 8) * 4 + i % 4] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    const int64_t at = b * p.q_b + (int64_t)h * p.group * p.q_h;
+    float x[8];
+    uint32_t most = 0;
+    for (int i = threadIdx.x; i < chunks; i += THREADS) {
+        load_q8(p, at + (int64_t)(i / CHUNKS) * p.q_h + i % CHUNKS * 8, x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) most = max(most, x[k] == x[k] ? __float_as_uint(fabsf(x[k])) : 0u);
+    }
+    most = __reduce_max_sync(~0u, most);
+    if ((threadIdx.x & 31) == 0) atomicMax(top, most);
+    __syncthreads();
+    const float largest = __uint_as_float(*top);
+    const int e = (int)(*top >> 23) - 127;                                  // q of subnormal size: all 0 either way
+    const float up = largest > 0.0f ? __uint_as_float((uint32_t)min(max(6 - e + 127, 1), 254) << 23) : 0.0f;
+    for (int i = threadIdx.x; i < chunks; i += THREADS) {
+        if (chunks > THREADS) load_q8(p, at + (int64_t)(i / CHUNKS) * p.q_h + i % CHUNKS * 8, x);
+        uint32_t plus[2] = {0, 0}, minus[2] = {0, 0};
+        int sum = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int v = max(-127, min(127, __float2int_rn(x[k] * up)));
+            sum += v;
+            plus[k >> 2] |= (uint32_t)max(v, 0) << (8 * (k & 3));
+            minus[k >> 2] |= ((uint32_t)min(v, 0) & 255u) << (8 * (k & 3));
+        }
+        const int head = i / CHUNKS, c = i % CHUNKS;
+        frag[((head / 8) * G + c / 4) * 32 + (head % 8) * 4 + c % 4] = make_uint4(plus[0], plus[1], minus[0], minus[1]);
+        atomicAdd(&sums[head], sum);
+    }
+    __syncthreads();
+}
+
 // Grid: (blocks of a sequence's pages, kv heads, sequences). A warp scores 16 pages at a time: lane (g, t) holds channels
-// 32 j + 8 t + 0..7 of pages g and g + 8 as the rows of m16n8k32 products, up to eight query heads are the columns.
+// 32 j + 8 t + 0..7 of pages g and g + 8 as the rows of m16n8k32 products, up to eight query heads are the columns. The first pages
+// are on their way while the block works out the queries.
 template <int G> __global__ void __launch_bounds__(32 * SCORE_WARPS) kv4_score_kernel(const __grid_constant__ SelectParams p) {
     constexpr int D = 32 * G;
+    extern __shared__ uint4 frag[];               // [col_blocks][G][32]
+    int *sums = reinterpret_cast<int *>(frag + p.col_blocks * G * 32);      // [col_blocks][8], and the largest |q|
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int h = blockIdx.y, b = blockIdx.z;
     wait_earlier();
     let_next_in();
-    const int pages = pages_of(p, b);
-    if (pages <= p.n) return;                                               // all of them: nothing to compare
-    const int tile0 = blockIdx.x * SCORE_WARPS + warp, tiles = (pages + 15) >> 4;
-    if (tile0 >= tiles) return;
-    // the kv head's queries in 8 bits
-    float top = 0.0f;
-    for (int i = lane; i < p.group * D; i += 32) top = fmaxf(top, fabsf(load_q(p, b * p.q_b + (int64_t)(h * p.group + i / D) * p.q_h + i % D)));
-#pragma unroll
-    for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-    const int e = (int)(__float_as_uint(top) >> 23) - 127;                  // q of subnormal size: all 0 either way
-    const float up = top > 0.0f ? __uint_as_float((uint32_t)min(max(6 - e + 127, 1), 254) << 23) : 0.0f;
-
-    for (int tile = tile0; tile < tiles; tile += gridDim.x * SCORE_WARPS) {
-        uint32_t a[2][2][G][2];                                             // [page g, g + 8][M, m][j][half]
-        float weight[2];
+    const int pages = pages_of(p, b), tiles = (pages + 15) >> 4;
+    if (pages <= p.n || blockIdx.x * SCORE_WARPS >= tiles) return;          // all of them: nothing to compare; or none for this block
+    uint4 x[2][2][G];                             // [page g, g + 8][M, m][j]
+    uint32_t there = 0;
+    auto load = [&](int tile) {
+        there = 0;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int page = tile * 16 + 8 * r + g;
-            uint4 x[2][G];
             int64_t id = -1;
             if (page < pages) {
                 id = page_id(p.s, b, page);
                 if (id < 0 || id >= p.c.num_pages) { or_status(p.status, OMMX_ST_BAD_PAGE); id = -1; }
             }
+            there |= (uint32_t)(id >= 0) << r;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int j = 0; j < G; ++j)
-                    x[m][j] = id < 0 ? make_uint4(0, 0, 0, 0)
-                                     : *reinterpret_cast<const uint4 *>(p.summary + ((id * p.c.H + h) * 2 + m) * D + 32 * j + 8 * t);
+                    x[r][m][j] = id < 0 ? make_uint4(0, 0, 0, 0)
+                                        : *reinterpret_cast<const uint4 *>(p.summary + ((id * p.c.H + h) * 2 + m) * D + 32 * j + 8 * t);
+        }
+    };
+    int tile = blockIdx.x * SCORE_WARPS + warp;
+    if (tile < tiles) load(tile);
+    quantize_query<G>(p, b, h, frag, sums, reinterpret_cast<uint32_t *>(sums + p.col_blocks * 8));
+    for (; tile < tiles; tile += gridDim.x * SCORE_WARPS) {
+        uint32_t a[2][2][G][2];                                             // [page g, g + 8][M, m][j][half]
+        float weight[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
             uint32_t most = 0;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int j = 0; j < G; ++j) {
-                    most = max_bf16x2(max_bf16x2(most, x[m][j].x & 0x7FFF7FFFu), x[m][j].y & 0x7FFF7FFFu);
-                    most = max_bf16x2(max_bf16x2(most, x[m][j].z & 0x7FFF7FFFu), x[m][j].w & 0x7FFF7FFFu);
+                    const uint4 v = x[r][m][j];
+                    most = max_bf16x2(max_bf16x2(most, v.x & 0x7FFF7FFFu), v.y & 0x7FFF7FFFu);
+                    most = max_bf16x2(max_bf16x2(most, v.z & 0x7FFF7FFFu), v.w & 0x7FFF7FFFu);
                 }
             uint32_t one = max(most & 0xFFFFu, most >> 16);
             one = max(one, __shfl_xor_sync(~0u, one, 1));
             one = max(one, __shfl_xor_sync(~0u, one, 2));
             const int f = max((int)(one >> 7) - 127, -100);
             const uint32_t c = ((uint32_t)(5 - f - 1 + 127) << 7) | 0x7Cu;  // (63 / 64) 2^(5 - f) = (63 / 32) 2^(4 - f) in bf16
-            weight[r] = __uint_as_float((uint32_t)(f - 26 + 127) << 23);
-            if (id < 0) weight[r] = 0.0f;
+            weight[r] = there >> r & 1 ? __uint_as_float((uint32_t)(f - 26 + 127) << 23) : 0.0f;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int j = 0; j < G; ++j) {
-                    a[r][m][j][0] = bytes_of(x[m][j].x, x[m][j].y, c | c << 16);
-                    a[r][m][j][1] = bytes_of(x[m][j].z, x[m][j].w, c | c << 16);
+                    a[r][m][j][0] = bytes_of(x[r][m][j].x, x[r][m][j].y, c | c << 16);
+                    a[r][m][j][1] = bytes_of(x[r][m][j].z, x[r][m][j].w, c | c << 16);
                 }
         }
+        const int next = tile + gridDim.x * SCORE_WARPS;
+        if (next < tiles) load(next);
         int best[2] = {INT32_MIN, INT32_MIN};
         for (int cb = 0; cb < p.col_blocks; ++cb) {
-            const int n = min(8, p.group - 8 * cb);
-            int sum = 0, acc[4] = {0, 0, 0, 0};
+            int acc[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < G; ++j) {
-                uint32_t plus[2] = {0, 0}, minus[2] = {0, 0};
-                if (g < n) {
-                    const int64_t at = b * p.q_b + (int64_t)(h * p.group + 8 * cb + g) * p.q_h + 32 * j + 8 * t;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int v = max(-127, min(127, __float2int_rn(load_q(p, at + i) * up)));
-                        sum += v;
-                        plus[i >> 2] |= (uint32_t)max(v, 0) << (8 * (i & 3));
-                        minus[i >> 2] |= ((uint32_t)min(v, 0) & 255u) << (8 * (i & 3));
-                    }
-                }
-                mma_u8s8(acc, a[0][0][j][0], a[1][0][j][0], a[0][0][j][1], a[1][0][j][1], plus[0], plus[1]);
-                mma_u8s8(acc, a[0][1][j][0], a[1][1][j][0], a[0][1][j][1], a[1][1][j][1], minus[0], minus[1]);
+                const uint4 q = frag[(cb * G + j) * 32 + lane];
+                mma_u8s8(acc, a[0][0][j][0], a[1][0][j][0], a[0][0][j][1], a[1][0][j][1], q.x, q.y);
+                mma_u8s8(acc, a[0][1][j][0], a[1][1][j][0], a[0][1][j][1], a[1][1][j][1], q.z, q.w);
             }
-            sum += __shfl_xor_sync(~0u, sum, 1);
-            sum += __shfl_xor_sync(~0u, sum, 2);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int off = 64 * __shfl_sync(~0u, sum, 8 * t + 4 * i);  // the bytes are 64 too large
-                if (2 * t + i < n) { best[0] = max(best[0], acc[i] - off); best[1] = max(best[1], acc[2 + i] - off); }
+                const int head = 8 * cb + 2 * t + i, off = 64 * sums[head];  // the bytes are 64 too large
+                if (head < p.group) { best[0] = max(best[0], acc[i] - off); best[1] = max(best[1], acc[2 + i] - off); }
             }
         }
 #pragma unroll
@@ -152,9 +196,7 @@ template <int G> __global__ void __launch_bounds__(32 * SCORE_WARPS) kv4_score_k
             best[r] = max(best[r], __shfl_xor_sync(~0u, best[r], 1));
             best[r] = max(best[r], __shfl_xor_sync(~0u, best[r], 2));
             const int page = tile * 16 + 8 * r + g;
-            if (t == 0 && page < pages)
-                p.keys[((int64_t)b * p.c.H + h) * p.s.max_pages + page] =
-                    page < p.first || page >= pages - p.last ? ~0u : ordered(__int2float_rn(best[r]) * weight[r]);
+            if (t == 0 && page < pages) p.keys[((int64_t)b * p.c.H + h) * p.s.max_pages + page] = ordered(__int2float_rn(best[r]) * weight[r]);
         }
     }
 }
@@ -175,11 +217,14 @@ __device__ __forceinline__ int2 block_exclusive_scan(int2 v, int2 *shared, int2 
     return make_int2(before.x + s.x - v.x, before.y + s.y - v.y);
 }
 
-// The n largest keys of a row, ties to the lowest page: a digit of eight bits at a time from the top, then one ordered pass.
+// The n largest keys of a row, ties to the lowest page. What lies between the smallest key and the largest is cut into BINS equal
+// parts, the part that holds the last key taken again, until it is one value: the keys of a row share their leading bits, and counts
+// by those would be atomics on a few words. Up to KEPT keys a thread stay in registers.
+constexpr int BINS = 2048, KEPT = 8;
 __global__ void __launch_bounds__(PICK_THREADS) kv4_pick_kernel(const __grid_constant__ SelectParams p) {
-    __shared__ int histogram[256];
+    __shared__ int histogram[BINS];
     __shared__ int2 scan[PICK_THREADS / 32];
-    __shared__ uint32_t chosen;
+    __shared__ uint32_t low, high;
     __shared__ int left;
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
     wait_earlier();
@@ -190,45 +235,73 @@ __global__ void __launch_bounds__(PICK_THREADS) kv4_pick_kernel(const __grid_con
         for (int i = tid; i < p.n; i += PICK_THREADS) out[i] = i < pages ? i : -1;
         return;
     }
+    // thread t has keys t * each .. : the order of the threads is the order of the pages
     const uint32_t *keys = p.keys + ((int64_t)b * p.c.H + h) * p.s.max_pages;
-    uint32_t prefix = 0, mask = 0;
-    int want = p.n;                               // how many of the keys that begin with `prefix` are taken
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) histogram[tid] = 0;
+    const int each = (pages + PICK_THREADS - 1) / PICK_THREADS, from = min(pages, tid * each), to = min(pages, from + each);
+    uint32_t kept[KEPT];
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) kept[i] = from + i < to ? keys[from + i] : 0;
+    if (tid == 0) { low = ~0u; high = 0; }
+    __syncthreads();
+    // f(key, page) for each of the thread's keys that are not taken anyway
+    auto each_key = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < KEPT; ++i)
+            if (from + i < to && from + i >= p.first && from + i < pages - p.last) f(kept[i]);
+        for (int i = max(from + KEPT, p.first); i < min(to, pages - p.last); ++i) f(keys[i]);
+    };
+    uint32_t a = ~0u, z = 0;
+    each_key([&](uint32_t k) { a = min(a, k); z = max(z, k); });
+    a = __reduce_min_sync(~0u, a);
+    z = __reduce_max_sync(~0u, z);
+    if ((tid & 31) == 0) { atomicMin(&low, a); atomicMax(&high, z); }
+    __syncthreads();
+    a = low;
+    int width = 32 - __clz(high - a);             // bits of what the keys span
+    int want = p.n - p.first - p.last;            // how many of the keys from `a` on, below a + 2^width, are taken
+    while (width > 0) {
+        const int shift = max(0, width - 11);
+        for (int i = tid; i < BINS; i += PICK_THREADS) histogram[i] = 0;
         __syncthreads();
-        for (int i = tid; i < pages; i += PICK_THREADS) {
-            const uint32_t k = keys[i];
-            if ((k & mask) == prefix) atomicAdd(&histogram[k >> shift & 255u], 1);
+        each_key([&](uint32_t k) {
+            const uint32_t d = k - a;
+            if (width == 32 || d >> width == 0) atomicAdd(&histogram[d >> shift], 1);
+        });
+        __syncthreads();
+        // from the top: thread t has bins BINS - 1 - 2 t and the one below
+        const int hi = histogram[BINS - 1 - 2 * tid], lo = histogram[BINS - 2 - 2 * tid];
+        int2 all;
+        const int before = block_exclusive_scan(make_int2(hi + lo, 0), scan, &all).x;
+        if (before < want && before + hi + lo >= want) {
+            const bool upper = before + hi >= want;
+            left = want - before - (upper ? 0 : hi);
+            low = a + ((uint32_t)(BINS - (upper ? 1 : 2) - 2 * tid) << shift);
         }
         __syncthreads();
-        if (tid < 32) {                           // lane l: digits 255 - 8 l .. 248 - 8 l
-            int mine = 0;
-            for (int i = 0; i < 8; ++i) mine += histogram[255 - 8 * tid - i];
-            const int upto = warp_inclusive_scan(mine, tid);
-            if (upto >= want && upto - mine < want) {
-                int above = upto - mine, d = 255 - 8 * tid;
-                while (above + histogram[d] < want) above += histogram[d--];
-                chosen = prefix | (uint32_t)d << shift;
-                left = want - above;
-            }
-        }
-        __syncthreads();
-        prefix = chosen;
+        a = low;
         want = left;
-        mask |= 255u << shift;
+        width = shift;
         __syncthreads();
     }
-    // keys above `prefix`, and the first `want` equal to it, in order
-    const int each = (pages + PICK_THREADS - 1) / PICK_THREADS, from = min(pages, tid * each), to = min(pages, from + each);
+    // keys above `a`, and the first `want` equal to it, in order
+    auto taken = [&](int i) { return i < p.first || i >= pages - p.last; };
     int2 mine = make_int2(0, 0), total;
-    for (int i = from; i < to; ++i) { mine.x += keys[i] > prefix; mine.y += keys[i] == prefix; }
+    if (p.n - p.first - p.last == 0) { a = ~0u; want = 0; }
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i)
+        if (from + i < to) { mine.x += taken(from + i) || kept[i] > a; mine.y += !taken(from + i) && kept[i] == a; }
+    for (int i = from + KEPT; i < to; ++i) { mine.x += taken(i) || keys[i] > a; mine.y += !taken(i) && keys[i] == a; }
     int2 at = block_exclusive_scan(mine, scan, &total);
-    for (int i = from; i < to; ++i) {
-        const bool more = keys[i] > prefix, same = keys[i] == prefix;
+    auto put = [&](int i, uint32_t k) {
+        const bool more = taken(i) || k > a, same = !taken(i) && k == a;
         if (more || (same && at.y < want)) out[at.x + min(at.y, want)] = i;
         at.x += more;
         at.y += same;
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i)
+        if (from + i < to) put(from + i, kept[i]);
+    for (int i = from + KEPT; i < to; ++i) put(i, keys[i]);
 }
 
 static int64_t select_workspace(int64_t B, int64_t H, int64_t pages) { return (B * H * pages * 4 + 15) / 16 * 16; }
@@ -242,6 +315,8 @@ static int select(const ommx_kv4_select_args *a, cudaStream_t st) {
     if (a->q_dtype != OMMX_DT_BF16 && a->q_dtype != OMMX_DT_F16) return fail(OMMX_E_UNSUPPORTED, "kv4_select: q must be bfloat16 or float16");
     if (a->n_q_heads < p.c.H || a->n_q_heads % p.c.H)
         return fail(OMMX_E_UNSUPPORTED, "kv4_select: %d query heads are not a multiple of %d kv heads", a->n_q_heads, p.c.H);
+    if (a->n_q_heads / p.c.H > MOST_HEADS)
+        return fail(OMMX_E_UNSUPPORTED, "kv4_select: %d query heads to a kv head (this build serves %d)", a->n_q_heads / p.c.H, MOST_HEADS);
     if (a->first_pages < 0 || a->last_pages < 0 || (int64_t)a->first_pages + a->last_pages > a->num_selected)
         return fail(OMMX_E_ARG, "kv4_select: first_pages %d and last_pages %d must fit into %d selected ones", a->first_pages, a->last_pages, a->num_selected);
     if (p.s.B > 65535) return fail(OMMX_E_UNSUPPORTED, "kv4_select: a batch of %d", p.s.B);
@@ -253,6 +328,7 @@ static int select(const ommx_kv4_select_args *a, cudaStream_t st) {
         return fail(OMMX_E_ARG, "kv4_select: workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
     p.summary = (const uint16_t *)a->cache.summary;
     p.q = a->q; p.q16 = a->q_dtype == OMMX_DT_F16; p.q_b = a->q_stride_b; p.q_h = a->q_stride_h;
+    p.q_wide = (reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)(2 * p.q_b) | (uintptr_t)(2 * p.q_h)) % 16 == 0;
     p.keys = (uint32_t *)a->workspace;
     p.selected = a->selected; p.n = a->num_selected; p.first = a->first_pages; p.last = a->last_pages;
     p.group = a->n_q_heads / p.c.H; p.col_blocks = (p.group + 7) / 8;
@@ -260,10 +336,11 @@ static int select(const ommx_kv4_select_args *a, cudaStream_t st) {
     p.status = a->status;
     if (p.s.max_pages > p.n) {
         const int64_t rows = (int64_t)p.s.B * p.c.H, most = (p.s.max_pages + 16LL * SCORE_WARPS - 1) / (16 * SCORE_WARPS);
-        const int64_t fill = (8LL * sm_count() + rows - 1) / rows;          // eight blocks to an SM
+        const int64_t fill = (4LL * sm_count() + rows - 1) / rows;          // about four blocks to an SM
+        const size_t smem = (size_t)p.col_blocks * (a->cache.head_dim * 16 + 32) + 16;
         const dim3 grid((unsigned)(most < fill ? most : fill), p.c.H, p.s.B);
-        const int rc = a->cache.head_dim == 64 ? launch_dependent(kv4_score_kernel<2>, grid, 32 * SCORE_WARPS, 0, st, p)
-                                               : launch_dependent(kv4_score_kernel<4>, grid, 32 * SCORE_WARPS, 0, st, p);
+        const int rc = a->cache.head_dim == 64 ? launch_dependent(kv4_score_kernel<2>, grid, 32 * SCORE_WARPS, smem, st, p)
+                                               : launch_dependent(kv4_score_kernel<4>, grid, 32 * SCORE_WARPS, smem, st, p);
         if (rc) return rc;
     }
     return launch_dependent(kv4_pick_kernel, dim3(p.c.H, p.s.B), PICK_THREADS, 0, st, p);

@@ -186,9 +186,16 @@ def test_the_c_abi_refuses_before_it_launches():
     d.logit_cap = 0.0
     says(lib.ommx_b200_kv4_decode, d, -1, "null")
     d.q = d.o = d.lse = 4096
+    assert lib.ommx_b200_kv4_decode_workspace_floats(C.byref(d)) == 0                       # 48 tokens: one launch without any
+    d.seqs.pages_per_seq = 100
+    assert lib.ommx_b200_kv4_decode_workspace_floats(C.byref(d)) == kv4_workspace_floats(64) > 0
     says(lib.ommx_b200_kv4_decode, d, -1, "workspace")
     d.workspace, d.workspace_floats = 4096, kv4_workspace_floats(64) - 1
     says(lib.ommx_b200_kv4_decode, d, -1, "workspace")
+    d.workspace_floats, d.seqs.pages_per_seq, d.seqs.batch = 1 << 40, 1 << 24, 100
+    says(lib.ommx_b200_kv4_decode, d, -2, "max_seq_len")
+    d.cache.num_pages, d.cache.records = 0, None
+    says(lib.ommx_b200_kv4_decode, d, -1, "no pages")
     s = _lib.KV4SelectArgs(cache=a.cache, seqs=a.seqs, q_dtype=_lib.OMMX_DT_F16, n_q_heads=4, num_selected=2, first_pages=1, last_pages=2)
     says(lib.ommx_b200_kv4_select, s, -1, "fit into")
     s.last_pages = 1
