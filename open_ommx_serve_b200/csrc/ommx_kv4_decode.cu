@@ -42,10 +42,17 @@ struct DecodeParams {
 };
 
 // ---- how the work is dealt ------------------------------------------------------------------------
-// Units are records (16 tokens of a kv head, or a block of COLS of its query heads), in order of (sequence, kv head, block of heads,
-// place); block i of the grid takes `per` of them in a row. A row (sequence, kv head, block) that lies in one share is finished
-// there; the others' parts meet in the second kernel, which works the same shares out. A block writes at most two parts: of the row
-// that an earlier block began (slot 0) and of the one that a later block goes on with (slot 1).
+// Units are records (16 tokens of a kv head, for a block of COLS of its query heads); a row (sequence, kv head, block of heads) is a
+// run of them. Lengths are known on the device alone, so every block works the same deal out, and so does the second kernel:
+// * a block to a row, where the host knows that rows are short (`whole`);
+// * else every row is cut into pieces of at most `per` units, a block to a piece, with the smallest `per` for which there are blocks
+//   enough;
+// * or, where that would leave a block with over BEGIN units more than an even share, all rows end to end are cut into such shares,
+//   whatever rows they touch. A second piece costs a block some 4 us, half of it hidden by the SM's other block (64K tokens: 26.7 us
+//   with seven such blocks of 296, 24.3 with none; 32 sequences of 700..8191: 66.9 with even shares, 74.8 with pieces up to 28 longer).
+// A piece that is a whole row is finished where it is computed; the others' parts meet in the second kernel. A block has at most two
+// of those, of the row that an earlier block began (its slot 0) and of the one that a later block goes on with (slot 1).
+constexpr int BEGIN = 12;
 __device__ __forceinline__ int pages_of(const DecodeParams &p, int len) { return (len + p.c.page - 1) >> p.page_shift; }
 __device__ __forceinline__ int length_of(const DecodeParams &p, int b) {
     const int len = p.s.len[b];
@@ -57,15 +64,37 @@ __device__ __forceinline__ int units_of(const DecodeParams &p, int len) {
     if (p.selected) return min(pages_of(p, len), p.num_selected) * p.c.parts;
     return (len + 15) >> 4;
 }
-struct Shares { uint32_t per, total; };           // the host refuses what 32 bits do not count
-__device__ __forceinline__ Shares shares(const DecodeParams &p, uint32_t rows, uint32_t blocks, int lane) {
-    uint32_t sum = 0;
-    for (int b = lane; b < p.s.B; b += 32) sum += units_of(p, length_of(p, b));
-    sum = __reduce_add_sync(~0u, sum);
-    Shares r;
-    r.total = sum * rows;
-    r.per = max((r.total + blocks - 1) / blocks, (uint32_t)p.least);
-    return r;
+struct Deal { uint32_t per, total; bool pieces; };   // the host refuses what 32 bits do not count
+__device__ __forceinline__ uint32_t pieces_of(uint32_t units, uint32_t per) { return (units + per - 1) / per; }
+__device__ __forceinline__ Deal deal(const DecodeParams &p, uint32_t rows, uint32_t blocks, int lane) {
+    uint32_t sum = 0, some = 0, most = 0;
+    const uint32_t own = lane < p.s.B ? units_of(p, length_of(p, lane)) : 0;
+    for (int b = lane; b < p.s.B; b += 32) {
+        const uint32_t n = b == lane ? own : units_of(p, length_of(p, b));
+        sum += n;
+        some += n > 0;
+        most = max(most, n);
+    }
+    Deal d;
+    d.total = __reduce_add_sync(~0u, sum) * rows;
+    const uint32_t full = __reduce_add_sync(~0u, some) * rows;
+    most = __reduce_max_sync(~0u, most);
+    const uint32_t even = max((d.total + blocks - 1) / blocks, (uint32_t)p.least);
+    d.per = even;
+    d.pieces = false;
+    if (full == 0 || full > blocks) return d;
+    // pieces of `per` take total / per + full blocks at most; fewer may do
+    uint32_t lo = even, hi = min(max(most, even), full < blocks ? max(even, d.total / (blocks - full) + 1) : 0xFFFFFFFFu);
+#pragma unroll 1
+    for (int i = 0; i < 6 && lo < hi; ++i) {
+        const uint32_t per = i == 0 ? lo : (lo + hi) / 2;
+        uint32_t n = pieces_of(own, per);
+        for (int b = lane + 32; b < p.s.B; b += 32) n += pieces_of(units_of(p, length_of(p, b)), per);
+        if (__reduce_add_sync(~0u, n) * rows <= blocks) hi = per;
+        else lo = per + 1;
+    }
+    if (hi <= even + BEGIN) { d.per = hi; d.pieces = true; }
+    return d;
 }
 
 // ---- pieces ---------------------------------------------------------------------------------------
@@ -447,34 +476,44 @@ template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PE
     wait_earlier();
     let_next_in();
     const uint32_t rows = p.c.H * p.col_blocks;
-    uint32_t u, end, start, base = 0;             // this block's units; units before sequence b
+    uint32_t u, end, base = 0;                    // this block's units; units before sequence b
+    uint32_t second = ~0u;                        // a row that begins here or later leaves its part in the second slot
     int b = 0, units = 0, len = 0;
     if (p.whole) {                                // a block to a row
         b = blockIdx.x / rows;
         len = length_of(p, b);
         units = units_of(p, len);
-        start = u = (blockIdx.x - b * rows) * units;
+        u = (blockIdx.x - b * rows) * units;
         end = u + units;
         if (units == 0) { nothing<G>(p, b, blockIdx.x - b * rows); return; }
     } else {
-        const Shares sr = shares(p, rows, gridDim.x, lane);
-        start = u = blockIdx.x * sr.per;
-        if (u >= sr.total) return;
-        end = min(u + sr.per, sr.total);
-        // the sequence that unit u lies in
+        const Deal d = deal(p, rows, gridDim.x, lane);
+        // the sequence that this block's (first) unit lies in; `at`, `base`: this block and the first of the sequence, in pieces or units
+        const uint32_t at = d.pieces ? blockIdx.x : blockIdx.x * d.per;
+        if (!d.pieces && at >= d.total) return;
+        uint32_t before = 0;
         for (int b0 = 0;; b0 += 32) {
-            if (b0 >= p.s.B) return;              // lengths past max_seq_len, more units than 32 bits count
+            if (b0 >= p.s.B) return;              // no piece for this block (or lengths past max_seq_len, more than 32 bits count)
             const int l = b0 + lane < p.s.B ? length_of(p, b0 + lane) : 0, n = units_of(p, l);
-            const uint32_t sum = warp_inclusive_scan(n, lane), past = __ballot_sync(~0u, base + sum * rows > u);
+            const uint32_t v = d.pieces ? pieces_of(n, d.per) : n, sum = warp_inclusive_scan(v, lane), past = __ballot_sync(~0u, before + sum * rows > at);
             if (past) {
                 const int from = __ffs(past) - 1;
                 b = b0 + from;
-                base += __shfl_sync(~0u, sum - n, from) * rows;
+                before += __shfl_sync(~0u, sum - v, from) * rows;
                 units = __shfl_sync(~0u, n, from);
                 len = __shfl_sync(~0u, l, from);
                 break;
             }
-            base += __shfl_sync(~0u, sum, 31) * rows;
+            before += __shfl_sync(~0u, sum, 31) * rows;
+        }
+        if (d.pieces) {                           // piece `part` of `parts` of a row; units are counted from the sequence's first
+            const uint32_t parts = pieces_of(units, d.per), row = (at - before) / parts, part = at - before - row * parts;
+            u = row * units + (uint32_t)((uint64_t)units * part / parts);
+            end = row * units + (uint32_t)((uint64_t)units * (part + 1) / parts);
+        } else {
+            base = before;
+            second = u = at;
+            end = min(u + d.per, d.total);
         }
     }
     while (u < end) {
@@ -546,7 +585,7 @@ template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PE
         }
         fetched<0>();
         float *part = nullptr;
-        if (i0 > 0 || i1 < units) part = p.work + (2 * (int64_t)blockIdx.x + (base + row * units >= start)) * Shared<G>::PART;
+        if (i0 > 0 || i1 < units) part = p.work + (2 * (int64_t)blockIdx.x + (base + row * units >= second)) * Shared<G>::PART;
         finish<G>(p, s, m.sh, m.ref, m.sum, b, first_head, n, part, warp, lane);
         u += i1 - i0;
     }
@@ -564,13 +603,25 @@ template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_kernel(c
     const int b = blockIdx.y, row = blockIdx.x / COLS, h = blockIdx.x % COLS;
     const int head = row / p.col_blocks, cb = row % p.col_blocks, hq = head * p.group + cb * COLS + h;
     const uint32_t rows = p.c.H * p.col_blocks;
-    const Shares sh = shares(p, rows, blocks, lane);
+    const Deal d = deal(p, rows, blocks, lane);
+    const uint32_t units = units_of(p, length_of(p, b));
     uint32_t before = 0;
-    for (int i = lane; i < b; i += 32) before += units_of(p, length_of(p, i));
-    before = __reduce_add_sync(~0u, before);
-    const uint32_t units = units_of(p, length_of(p, b)), r0 = before * rows + row * units, c0 = r0 / sh.per;
-    const int n = units ? (int)((r0 + units - 1) / sh.per - c0) + 1 : 0;
-    const bool late = r0 >= c0 * sh.per;          // the row begins in block c0: its part there is the second one
+    for (int i = lane; i < b; i += 32) {
+        const uint32_t n = units_of(p, length_of(p, i));
+        before += d.pieces ? pieces_of(n, d.per) : n;
+    }
+    before = __reduce_add_sync(~0u, before) * rows;
+    uint32_t c0, n;
+    bool late = false;                            // the row begins inside block c0: its part there is the second one
+    if (d.pieces) {
+        n = pieces_of(units, d.per);
+        c0 = before + row * n;
+    } else {
+        const uint32_t r0 = before + row * units;
+        c0 = r0 / d.per;
+        n = units ? (r0 + units - 1) / d.per - c0 + 1 : 0;
+        late = r0 >= c0 * d.per;
+    }
     wait_earlier();
     let_next_in();
     if (h >= p.group - cb * COLS || n == 1) return;                         // not a head, or finished where it was computed
@@ -581,7 +632,7 @@ template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_kernel(c
     }
     auto part = [&](int i) { return p.work + (2 * (int64_t)(c0 + i) + (i == 0 && late)) * Shared<G>::PART; };
     float top = LOWEST, sum = 0.0f;
-    for (int i = threadIdx.x; i < n; i += 32 * CW) {
+    for (int i = threadIdx.x; i < (int)n; i += 32 * CW) {
         const float r = part(i)[COLS * D + h], s = part(i)[COLS * D + COLS + h], m = fmaxf(top, r);
         weight[i] = r;
         sum = fmaf(s, exp2_approx(r - m), sum * exp2_approx(top - m));
@@ -591,7 +642,7 @@ template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_kernel(c
     auto load = [&](int i0) {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
-            if (i0 + u * CW < n) v[u] = reinterpret_cast<const V *>(part(i0 + u * CW) + h * D)[lane];
+            if (i0 + u * CW < (int)n) v[u] = reinterpret_cast<const V *>(part(i0 + u * CW) + h * D)[lane];
     };
     load(warp);                                   // on their way while the references meet
 #pragma unroll
@@ -611,11 +662,11 @@ template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_kernel(c
     float o[G];
 #pragma unroll
     for (int i = 0; i < G; ++i) o[i] = 0.0f;
-    for (int i0 = warp; i0 < n; i0 += CW * UNROLL) {
+    for (int i0 = warp; i0 < (int)n; i0 += CW * UNROLL) {
         if (i0 != warp) load(i0);
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
-            if (i0 + u * CW < n) {
+            if (i0 + u * CW < (int)n) {
                 const float f = exp2_approx(weight[i0 + u * CW] - top);
                 const float *x = reinterpret_cast<const float *>(&v[u]);
 #pragma unroll
@@ -695,7 +746,7 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     p.page_shift = shift_of(p.c.page);
     p.sm_scale = a->sm_scale; p.cap = a->logit_cap; p.status = a->status;
     if (p.c.num_pages == 0) return fail(OMMX_E_ARG, "kv4_decode: a cache of no pages");   // what is fetched for a page that is not there
-    p.least = NW;
+    p.least = 2 * NW;
     // as many blocks as the SMs hold, no more than the work can have
     const int64_t units = most_units(a);
     const int64_t rows = (int64_t)p.s.B * p.c.H * p.col_blocks;

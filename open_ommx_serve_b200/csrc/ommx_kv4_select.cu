@@ -201,32 +201,31 @@ template <int G> __global__ void __launch_bounds__(32 * SCORE_WARPS) kv4_score_k
     }
 }
 
-__device__ __forceinline__ int2 block_exclusive_scan(int2 v, int2 *shared, int2 *total) {
+// Sums of a block's threads before this one's, of two small numbers at once (each sum below 2^31). `shared`: one value a warp.
+__device__ __forceinline__ int2 block_exclusive_scan(int2 v, int2 *shared) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int2 s = make_int2(warp_inclusive_scan(v.x, lane), warp_inclusive_scan(v.y, lane));
+    const int2 s = make_int2(warp_inclusive_scan(v.x, lane), warp_inclusive_scan(v.y, lane));
     if (lane == 31) shared[warp] = s;
     __syncthreads();
-    int2 before = make_int2(0, 0), all = before;
-    for (int w = 0; w < PICK_THREADS / 32; ++w) {
-        if (w == warp) before = all;
-        all.x += shared[w].x;
-        all.y += shared[w].y;
-    }
-    __syncthreads();
-    *total = all;
-    return make_int2(before.x + s.x - v.x, before.y + s.y - v.y);
+    const int2 w = shared[lane];                  // as many warps as lanes
+    const int x = __reduce_add_sync(~0u, lane < warp ? w.x : 0), y = __reduce_add_sync(~0u, lane < warp ? w.y : 0);
+    return make_int2(x + s.x - v.x, y + s.y - v.y);
 }
 
 // The n largest keys of a row, ties to the lowest page. What lies between the smallest key and the largest is cut into BINS equal
-// parts, the part that holds the last key taken again, until it is one value: the keys of a row share their leading bits, and counts
-// by those would be atomics on a few words. Up to KEPT keys a thread stay in registers.
+// parts, the part that holds the last key taken again, until no more than a warp's worth are in it, which then rank themselves: the
+// keys of a row share their leading bits, and counts by those would be atomics on a few words. Up to KEPT keys a thread stay in
+// registers.
 constexpr int BINS = 2048, KEPT = 8;
 __global__ void __launch_bounds__(PICK_THREADS) kv4_pick_kernel(const __grid_constant__ SelectParams p) {
+    static_assert(PICK_THREADS == 1024 && BINS == 2 * PICK_THREADS, "a warp to a lane, two bins to a thread");
     __shared__ int histogram[BINS];
-    __shared__ int2 scan[PICK_THREADS / 32];
-    __shared__ uint32_t low, high;
-    __shared__ int left;
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    __shared__ int2 scan[32];
+    __shared__ uint32_t few[32], low, high;
+    __shared__ int left, inside, listed;
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+    if (tid == 0) { low = ~0u; high = 0; listed = 0; }
+    histogram[tid] = histogram[tid + PICK_THREADS] = 0;
     wait_earlier();
     let_next_in();
     const int pages = pages_of(p, b);
@@ -241,9 +240,7 @@ __global__ void __launch_bounds__(PICK_THREADS) kv4_pick_kernel(const __grid_con
     uint32_t kept[KEPT];
 #pragma unroll
     for (int i = 0; i < KEPT; ++i) kept[i] = from + i < to ? keys[from + i] : 0;
-    if (tid == 0) { low = ~0u; high = 0; }
-    __syncthreads();
-    // f(key, page) for each of the thread's keys that are not taken anyway
+    // f(key) for each of the thread's keys that are not taken anyway
     auto each_key = [&](auto f) {
 #pragma unroll
         for (int i = 0; i < KEPT; ++i)
@@ -254,44 +251,61 @@ __global__ void __launch_bounds__(PICK_THREADS) kv4_pick_kernel(const __grid_con
     each_key([&](uint32_t k) { a = min(a, k); z = max(z, k); });
     a = __reduce_min_sync(~0u, a);
     z = __reduce_max_sync(~0u, z);
-    if ((tid & 31) == 0) { atomicMin(&low, a); atomicMax(&high, z); }
+    __syncthreads();
+    if (lane == 0) { atomicMin(&low, a); atomicMax(&high, z); }
     __syncthreads();
     a = low;
     int width = 32 - __clz(high - a);             // bits of what the keys span
     int want = p.n - p.first - p.last;            // how many of the keys from `a` on, below a + 2^width, are taken
-    while (width > 0) {
+    auto within = [&](uint32_t k) { return width == 32 || (k - a) >> width == 0; };
+    while (width > 0 && want > 0) {
         const int shift = max(0, width - 11);
-        for (int i = tid; i < BINS; i += PICK_THREADS) histogram[i] = 0;
-        __syncthreads();
-        each_key([&](uint32_t k) {
-            const uint32_t d = k - a;
-            if (width == 32 || d >> width == 0) atomicAdd(&histogram[d >> shift], 1);
-        });
+        each_key([&](uint32_t k) { if (within(k)) atomicAdd(&histogram[(k - a) >> shift], 1); });
         __syncthreads();
         // from the top: thread t has bins BINS - 1 - 2 t and the one below
         const int hi = histogram[BINS - 1 - 2 * tid], lo = histogram[BINS - 2 - 2 * tid];
-        int2 all;
-        const int before = block_exclusive_scan(make_int2(hi + lo, 0), scan, &all).x;
+        const int before = block_exclusive_scan(make_int2(hi + lo, 0), scan).x;
         if (before < want && before + hi + lo >= want) {
             const bool upper = before + hi >= want;
             left = want - before - (upper ? 0 : hi);
+            inside = upper ? hi : lo;
             low = a + ((uint32_t)(BINS - (upper ? 1 : 2) - 2 * tid) << shift);
         }
+        histogram[BINS - 1 - 2 * tid] = histogram[BINS - 2 - 2 * tid] = 0;
         __syncthreads();
         a = low;
         want = left;
         width = shift;
+        if (inside <= 32) break;
         __syncthreads();
     }
+    if (width > 0 && want > 0) {                  // the `want`-th of the few that lie in this part
+        const int count = inside;
+        each_key([&](uint32_t k) { if (within(k)) few[atomicAdd(&listed, 1)] = k; });
+        __syncthreads();
+        const uint32_t mine = lane < count ? few[lane] : 0;
+        int above = 0, same = 0;
+        for (int i = 0; i < count; ++i) {
+            const uint32_t k = __shfl_sync(~0u, mine, i);
+            above += k > mine;
+            same += k == mine;
+        }
+        const uint32_t found = __ballot_sync(~0u, lane < count && above < want && above + same >= want);
+        const int one = __ffs(found) - 1;         // equal ones all say so
+        a = __shfl_sync(~0u, mine, one);
+        want -= __shfl_sync(~0u, above, one);
+    }
+    if (p.n == p.first + p.last) a = ~0u;         // keys are below that
     // keys above `a`, and the first `want` equal to it, in order
     auto taken = [&](int i) { return i < p.first || i >= pages - p.last; };
-    int2 mine = make_int2(0, 0), total;
-    if (p.n - p.first - p.last == 0) { a = ~0u; want = 0; }
+    int2 mine = make_int2(0, 0);
+    auto count = [&](int i, uint32_t k) { mine.x += taken(i) || k > a; mine.y += !taken(i) && k == a; };
 #pragma unroll
     for (int i = 0; i < KEPT; ++i)
-        if (from + i < to) { mine.x += taken(from + i) || kept[i] > a; mine.y += !taken(from + i) && kept[i] == a; }
-    for (int i = from + KEPT; i < to; ++i) { mine.x += taken(i) || keys[i] > a; mine.y += !taken(i) && keys[i] == a; }
-    int2 at = block_exclusive_scan(mine, scan, &total);
+        if (from + i < to) count(from + i, kept[i]);
+    for (int i = from + KEPT; i < to; ++i) count(i, keys[i]);
+    __syncthreads();                              // `scan` is read above
+    int2 at = block_exclusive_scan(mine, scan);
     auto put = [&](int i, uint32_t k) {
         const bool more = taken(i) || k > a, same = !taken(i) && k == a;
         if (more || (same && at.y < want)) out[at.x + min(at.y, want)] = i;
@@ -336,7 +350,7 @@ static int select(const ommx_kv4_select_args *a, cudaStream_t st) {
     p.status = a->status;
     if (p.s.max_pages > p.n) {
         const int64_t rows = (int64_t)p.s.B * p.c.H, most = (p.s.max_pages + 16LL * SCORE_WARPS - 1) / (16 * SCORE_WARPS);
-        const int64_t fill = (4LL * sm_count() + rows - 1) / rows;          // about four blocks to an SM
+        const int64_t fill = (2LL * sm_count() + rows - 1) / rows;          // two blocks to an SM, which is what it holds
         const size_t smem = (size_t)p.col_blocks * (a->cache.head_dim * 16 + 32) + 16;
         const dim3 grid((unsigned)(most < fill ? most : fill), p.c.H, p.s.B);
         const int rc = a->cache.head_dim == 64 ? launch_dependent(kv4_score_kernel<2>, grid, 32 * SCORE_WARPS, smem, st, p)
