@@ -43,7 +43,8 @@ struct DecodeParams {
 
 // ---- how the work is dealt ------------------------------------------------------------------------
 // Units are records (16 tokens of a kv head, for a block of COLS of its query heads); a row (sequence, kv head, block of heads) is a
-// run of them. Lengths are known on the device alone, so every block works the same deal out, and so does the second kernel:
+// run of them. Lengths are known on the device alone, so every block works the same deal out, and leaves it for the
+// second kernel:
 // * a block to a row, where the host knows that rows are short (`whole`);
 // * else every row is cut into pieces of at most `per` units, a block to a piece, with the smallest `per` for which there are blocks
 //   enough;
@@ -52,7 +53,7 @@ struct DecodeParams {
 //   with seven such blocks of 296, 24.3 with none; 32 sequences of 700..8191: 66.9 with even shares, 74.8 with pieces up to 28 longer).
 // A piece that is a whole row is finished where it is computed; the others' parts meet in the second kernel. A block has at most two
 // of those, of the row that an earlier block began (its slot 0) and of the one that a later block goes on with (slot 1).
-constexpr int BEGIN = 12;
+constexpr int BEGIN = 12, HEAD = 4;               // HEAD: floats in front of the parts, which hold the deal
 __device__ __forceinline__ int pages_of(const DecodeParams &p, int len) { return (len + p.c.page - 1) >> p.page_shift; }
 __device__ __forceinline__ int length_of(const DecodeParams &p, int b) {
     const int len = p.s.len[b];
@@ -488,6 +489,7 @@ template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PE
         if (units == 0) { nothing<G>(p, b, blockIdx.x - b * rows); return; }
     } else {
         const Deal d = deal(p, rows, gridDim.x, lane);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<uint2 *>(p.work) = make_uint2(d.per, d.pieces);
         // the sequence that this block's (first) unit lies in; `at`, `base`: this block and the first of the sequence, in pieces or units
         const uint32_t at = d.pieces ? blockIdx.x : blockIdx.x * d.per;
         if (!d.pieces && at >= d.total) return;
@@ -585,70 +587,132 @@ template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PE
         }
         fetched<0>();
         float *part = nullptr;
-        if (i0 > 0 || i1 < units) part = p.work + (2 * (int64_t)blockIdx.x + (base + row * units >= second)) * Shared<G>::PART;
+        if (i0 > 0 || i1 < units) part = p.work + HEAD + (2 * (int64_t)blockIdx.x + (base + row * units >= second)) * Shared<G>::PART;
         finish<G>(p, s, m.sh, m.ref, m.sum, b, first_head, n, part, warp, lane);
         u += i1 - i0;
     }
 }
 
-// Rows of which several blocks have a part, and those of no tokens. Grid: (rows of a sequence x COLS, sequences). The references and
-// sums of all parts are read at once; then a warp takes every CW-th part, a lane G channels, UNROLL parts on their way.
-// The lengths are read before the wait: this kernel starts when every block of the one before has waited for what came earlier.
+// Where the parts of a row are: those of blocks first .. first + count - 1, the first one in its slot 1 if `late`. A whole warp calls
+// it, before the wait for the first kernel: this one starts when every block of that has waited for what came earlier, so the lengths
+// are there, and only the deal is not.
+struct Parts { uint32_t first, count; bool late; };
+__device__ __forceinline__ Parts parts_of(const DecodeParams &p, int b, uint32_t row, int lane) {
+    const uint32_t rows = p.c.H * p.col_blocks, units = units_of(p, length_of(p, b)), own = lane < b ? units_of(p, length_of(p, lane)) : 0;
+    wait_earlier();
+    const uint2 d = *reinterpret_cast<const uint2 *>(p.work);
+    uint32_t before = d.y ? pieces_of(own, d.x) : own;
+    for (int i = lane + 32; i < b; i += 32) {
+        const uint32_t v = units_of(p, length_of(p, i));
+        before += d.y ? pieces_of(v, d.x) : v;
+    }
+    before = __reduce_add_sync(~0u, before) * rows;
+    Parts r;
+    if (units == 0) return {0, 0, false};
+    if (d.y) {
+        r.count = pieces_of(units, d.x);
+        r.first = before + row * r.count;
+        r.late = false;
+    } else {
+        const uint32_t r0 = before + row * units;
+        r.first = r0 / d.x;
+        r.count = (r0 + units - 1) / d.x - r.first + 1;
+        r.late = r0 >= r.first * d.x;
+    }
+    return r;
+}
+template <int G> __device__ __forceinline__ const float *part_at(const DecodeParams &p, const Parts &r, int i) {
+    return p.work + HEAD + (2 * (int64_t)(r.first + i) + (i == 0 && r.late)) * Shared<G>::PART;
+}
+template <int G> __device__ __forceinline__ void zeros(const DecodeParams &p, int b, int hq, int lane) {      // a head of no tokens
+#pragma unroll
+    for (int i = 0; i < G; ++i) store_o(p, b * p.o_b + hq * p.o_h + lane * G + i, 0.0f);
+    if (lane == 0) p.lse[b * p.lse_b + hq] = -INFINITY;
+}
+
+// Rows of which several blocks have a part, and those of no tokens, where rows are many: a block to a row, a warp to a head, a lane
+// to G channels. Grid: (rows of a sequence, sequences).
+template <int G> __global__ void __launch_bounds__(32 * COLS) kv4_combine_row_kernel(const __grid_constant__ DecodeParams p) {
+    using V = typename Floats<G>::T;
+    constexpr int D = 32 * G;
+    const int lane = threadIdx.x & 31, h = threadIdx.x >> 5, b = blockIdx.y, row = blockIdx.x;
+    const int head = row / p.col_blocks, cb = row % p.col_blocks, hq = head * p.group + cb * COLS + h;
+    const Parts r = parts_of(p, b, row, lane);
+    let_next_in();
+    if (h >= p.group - cb * COLS || r.count == 1) return;                   // not a head, or finished where it was computed
+    if (r.count == 0) { zeros<G>(p, b, hq, lane); return; }
+    float top = LOWEST, sum = 0.0f, o[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) o[i] = 0.0f;
+    for (int i0 = 0; i0 < (int)r.count; i0 += 4) {
+        V v[4];
+        float ref[4], add[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const bool on = i0 + u < (int)r.count;
+            const float *part = part_at<G>(p, r, on ? i0 + u : i0);
+            v[u] = reinterpret_cast<const V *>(part + h * D)[lane];
+            ref[u] = on ? part[COLS * D + h] : LOWEST;
+            add[u] = on ? part[COLS * D + COLS + h] : 0.0f;
+        }
+        const float next = fmaxf(fmaxf(fmaxf(ref[0], ref[1]), fmaxf(ref[2], ref[3])), top), keep = exp2_approx(top - next);
+        sum *= keep;
+#pragma unroll
+        for (int i = 0; i < G; ++i) o[i] *= keep;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i0 + u < (int)r.count) {
+                const float f = exp2_approx(ref[u] - next);
+                sum = fmaf(add[u], f, sum);
+#pragma unroll
+                for (int i = 0; i < G; ++i) o[i] = fmaf(reinterpret_cast<const float *>(&v[u])[i], f, o[i]);
+            }
+        top = next;
+    }
+    const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int i = 0; i < G; ++i) o[i] = sum != 0.0f ? o[i] * inverse : 0.0f;
+    store_o(p, b * p.o_b + hq * p.o_h + lane * G, o);
+    if (lane == 0) p.lse[b * p.lse_b + hq] = sum != 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
+}
+
+// The same where rows are few and their parts many: a block to a head. The references and sums of all parts are read at once; then a
+// warp takes every CW-th part, UNROLL of them on their way. Grid: (rows of a sequence x COLS, sequences).
 constexpr int CW = 8, UNROLL = 5, MOST_PARTS = 512;
-template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_kernel(const __grid_constant__ DecodeParams p, int blocks) {
+template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_head_kernel(const __grid_constant__ DecodeParams p) {
     constexpr int D = 32 * G;
     using V = typename Floats<G>::T;
     __shared__ float so[CW][D], weight[MOST_PARTS], sr[CW], ss[CW];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int b = blockIdx.y, row = blockIdx.x / COLS, h = blockIdx.x % COLS;
     const int head = row / p.col_blocks, cb = row % p.col_blocks, hq = head * p.group + cb * COLS + h;
-    const uint32_t rows = p.c.H * p.col_blocks;
-    const Deal d = deal(p, rows, blocks, lane);
-    const uint32_t units = units_of(p, length_of(p, b));
-    uint32_t before = 0;
-    for (int i = lane; i < b; i += 32) {
-        const uint32_t n = units_of(p, length_of(p, i));
-        before += d.pieces ? pieces_of(n, d.per) : n;
-    }
-    before = __reduce_add_sync(~0u, before) * rows;
-    uint32_t c0, n;
-    bool late = false;                            // the row begins inside block c0: its part there is the second one
-    if (d.pieces) {
-        n = pieces_of(units, d.per);
-        c0 = before + row * n;
-    } else {
-        const uint32_t r0 = before + row * units;
-        c0 = r0 / d.per;
-        n = units ? (r0 + units - 1) / d.per - c0 + 1 : 0;
-        late = r0 >= c0 * d.per;
-    }
-    wait_earlier();
+    const Parts r = parts_of(p, b, row, lane);
     let_next_in();
+    const int n = r.count;
     if (h >= p.group - cb * COLS || n == 1) return;                         // not a head, or finished where it was computed
     if (n == 0) {
-        for (int c = threadIdx.x; c < D; c += 32 * CW) store_o(p, b * p.o_b + hq * p.o_h + c, 0.0f);
-        if (threadIdx.x == 0) p.lse[b * p.lse_b + hq] = -INFINITY;
+        if (warp == 0) zeros<G>(p, b, hq, lane);
         return;
-    }
-    auto part = [&](int i) { return p.work + (2 * (int64_t)(c0 + i) + (i == 0 && late)) * Shared<G>::PART; };
-    float top = LOWEST, sum = 0.0f;
-    for (int i = threadIdx.x; i < (int)n; i += 32 * CW) {
-        const float r = part(i)[COLS * D + h], s = part(i)[COLS * D + COLS + h], m = fmaxf(top, r);
-        weight[i] = r;
-        sum = fmaf(s, exp2_approx(r - m), sum * exp2_approx(top - m));
-        top = m;
     }
     V v[UNROLL];
     auto load = [&](int i0) {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
-            if (i0 + u * CW < (int)n) v[u] = reinterpret_cast<const V *>(part(i0 + u * CW) + h * D)[lane];
+            if (i0 + u * CW < n) v[u] = reinterpret_cast<const V *>(part_at<G>(p, r, i0 + u * CW) + h * D)[lane];
     };
     load(warp);                                   // on their way while the references meet
+    float top = LOWEST, sum = 0.0f;
+    for (int i = threadIdx.x; i < n; i += 32 * CW) {
+        const float *part = part_at<G>(p, r, i);
+        const float ref = part[COLS * D + h], s = part[COLS * D + COLS + h], m = fmaxf(top, ref);
+        weight[i] = ref;
+        sum = fmaf(s, exp2_approx(ref - m), sum * exp2_approx(top - m));
+        top = m;
+    }
 #pragma unroll
     for (int d = 16; d; d /= 2) {
-        const float r = __shfl_xor_sync(~0u, top, d), s = __shfl_xor_sync(~0u, sum, d), m = fmaxf(top, r);
-        sum = fmaf(s, exp2_approx(r - m), sum * exp2_approx(top - m));
+        const float ref = __shfl_xor_sync(~0u, top, d), s = __shfl_xor_sync(~0u, sum, d), m = fmaxf(top, ref);
+        sum = fmaf(s, exp2_approx(ref - m), sum * exp2_approx(top - m));
         top = m;
     }
     if (lane == 0) { sr[warp] = top; ss[warp] = sum; }
@@ -662,11 +726,11 @@ template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_kernel(c
     float o[G];
 #pragma unroll
     for (int i = 0; i < G; ++i) o[i] = 0.0f;
-    for (int i0 = warp; i0 < (int)n; i0 += CW * UNROLL) {
+    for (int i0 = warp; i0 < n; i0 += CW * UNROLL) {
         if (i0 != warp) load(i0);
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
-            if (i0 + u * CW < (int)n) {
+            if (i0 + u * CW < n) {
                 const float f = exp2_approx(weight[i0 + u * CW] - top);
                 const float *x = reinterpret_cast<const float *>(&v[u]);
 #pragma unroll
@@ -692,7 +756,7 @@ static int64_t most_blocks() {
 }
 static int64_t workspace_floats(int head_dim) {
     const int64_t part = head_dim == 64 ? Shared<2>::PART : Shared<4>::PART;
-    return 2 * part * most_blocks();
+    return HEAD + 2 * part * most_blocks();
 }
 
 template <int G, bool FINE> static int launch_decode(const DecodeParams &p, int64_t blocks, cudaStream_t st) {
@@ -705,7 +769,10 @@ template <int G, bool FINE> static int launch_decode(const DecodeParams &p, int6
     }
     if (int rc = launch_dependent(kv4_decode_kernel<G, FINE>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G>), st, p)) return rc;
     if (p.whole) return 0;
-    return launch_dependent(kv4_combine_kernel<G>, dim3(p.c.H * p.col_blocks * COLS, p.s.B), 32 * CW, 0, st, p, (int)blocks);
+    // a row has some blocks / rows parts
+    const int rows = p.c.H * p.col_blocks;
+    if ((int64_t)rows * p.s.B * COLS >= blocks) return launch_dependent(kv4_combine_row_kernel<G>, dim3(rows, p.s.B), 32 * COLS, 0, st, p);
+    return launch_dependent(kv4_combine_head_kernel<G>, dim3(rows * COLS, p.s.B), 32 * CW, 0, st, p);
 }
 
 // records that a row of the call can have
