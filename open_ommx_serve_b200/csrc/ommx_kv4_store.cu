@@ -1,4 +1,6 @@
 // The 4-bit cache: appending rows (rotation, quantization, page summaries) and reading rows back.
+#include <type_traits>
+
 #include "ommx_kv4.cuh"
 
 namespace ommx {
@@ -15,17 +17,19 @@ template <> __device__ __forceinline__ __half from_f32(float v) { return __float
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 
 // eight channels; WIDE: the address is a multiple of 16 bytes
-template <typename T, bool WIDE> __device__ __forceinline__ void load8(const T *p, float *x) {
+template <typename T> struct alignas(16) Eight { T v[8]; };
+template <typename T, bool WIDE> __device__ __forceinline__ void fetch8(const T *p, Eight<T> &x) {
     if constexpr (!WIDE) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i]);
+        for (int i = 0; i < 8; ++i) x.v[i] = p[i];
     } else {
-        alignas(16) T v[8];
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(v) / 16; ++i) reinterpret_cast<uint4 *>(v)[i] = reinterpret_cast<const uint4 *>(p)[i];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32(v[i]);
+        for (int i = 0; i < (int)sizeof(x) / 16; ++i) reinterpret_cast<uint4 *>(&x)[i] = reinterpret_cast<const uint4 *>(p)[i];
     }
+}
+template <typename T> __device__ __forceinline__ void unpack8(const Eight<T> &e, float *x) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(e.v[i]);
 }
 template <typename T, bool WIDE> __device__ __forceinline__ void store8(T *p, const float *x) {
     if constexpr (!WIDE) {
@@ -76,7 +80,7 @@ struct AppendParams {
     const float *cos, *sin;
     int64_t cs_stride;
     const void *positions;
-    int32_t positions64, num_positions, rot, interleaved, Hq, page_shift, kv_blocks, q_rows;
+    int32_t positions64, num_positions, rot, interleaved, Hq, page_shift, kv_blocks, blocks, q_rows, split;
     int32_t *status;
 };
 
@@ -89,65 +93,55 @@ __device__ __forceinline__ int rope_row(const AppendParams &p, int row, int pos)
     return (int)at;
 }
 
-// Rotation of a lane's channels 32 j + 8 t + 0..7 of a key, the four lanes t of a row together. Pairs (c, c + rot / 2) lie in one
-// lane for rot >= 64, in lanes t and t ^ 2 for rot = 32; pairs (2 i, 2 i + 1) always in one.
-template <int G> __device__ __forceinline__ void rotate_key(const AppendParams &p, float (&x)[G][8], int at, int t) {
-    const float *cos = p.cos + at * p.cs_stride, *sin = p.sin + at * p.cs_stride;
+// Rotation of eight channels c .. c + 7 of a key, below p.rot. Pairs (c, c + rot / 2): y holds the partners; pairs (2 i, 2 i + 1): both
+// lie here.
+__device__ __forceinline__ void rotate_key(const AppendParams &p, float (&x)[8], const float (&y)[8], int at, int c) {
+    const int half = p.rot / 2;
     if (p.interleaved) {
+        float cs[4], sn[4];
+        load_f32<4>(p.cos + at * p.cs_stride + c / 2, cs);
+        load_f32<4>(p.sin + at * p.cs_stride + c / 2, sn);
 #pragma unroll
-        for (int j = 0; j < G; ++j)
-            if (32 * j < p.rot) {
-                float c[4], s[4];
-                load_f32<4>(cos + 16 * j + 4 * t, c);
-                load_f32<4>(sin + 16 * j + 4 * t, s);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) turn(x[j][2 * i], x[j][2 * i + 1], c[i], s[i]);
-            }
+        for (int i = 0; i < 4; ++i) turn(x[2 * i], x[2 * i + 1], cs[i], sn[i]);
         return;
     }
-    if (p.rot == 32) {
-        float c[8], s[8];
-        load_f32<8>(cos + 8 * (t & 1), c);
-        load_f32<8>(sin + 8 * (t & 1), s);
+    const bool upper = c >= half;
+    const int64_t from = at * p.cs_stride + (upper ? c - half : c);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float mine = x[0][i], other = __shfl_xor_sync(~0u, mine, 2);
-            if (t < 2) turn(mine, other, c[i], s[i]);
-            else { turn(other, mine, c[i], s[i]); }
-            x[0][i] = mine;
+    for (int k = 0; k < 8; k += 4) {
+        float cs[4], sn[4];
+        load_f32<4>(p.cos + from + k, cs);
+        load_f32<4>(p.sin + from + k, sn);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float s = __fmul_rn(y[k + i], sn[i]);
+            x[k + i] = __fadd_rn(__fmul_rn(x[k + i], cs[i]), upper ? s : -s);
         }
-        return;
     }
-    // rot = 64: groups 0, 1; rot = 128: groups 0, 2 and 1, 3
-#pragma unroll
-    for (int j = 0; j < G / 2; ++j)
-        if (64 * j < p.rot) {
-            float c[8], s[8];
-            load_f32<8>(cos + 32 * j + 8 * t, c);
-            load_f32<8>(sin + 32 * j + 8 * t, s);
-            if (G == 2 || p.rot == 64) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) turn(x[0][i], x[1][i], c[i], s[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) turn(x[j][i], x[j + G / 2][i], c[i], s[i]);
-            }
-        }
 }
 
+// of three, NaN if one is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // Codes and parameters of one group of 32 channels, eight in each of the four lanes of a row: the lane's word of codes, and the
 // group's word of parameters. `bad`: x held a value that is not finite.
 __device__ __forceinline__ uint32_t quantize_group(float (&x)[8], uint32_t *params, bool *bad) {
-    float check = 0.0f;
+    float lo = min3_nan(min3_nan(min3_nan(x[0], x[1], x[2]), x[3], x[4]), x[5], fminf(x[6], x[7]));
+    float hi = max3_nan(max3_nan(max3_nan(x[0], x[1], x[2]), x[3], x[4]), x[5], max3_nan(x[6], x[7], x[7]));
+    if (!(hi <= LARGEST && lo >= -LARGEST)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) check = fmaf(x[i], 0.0f, check);           // NaN as soon as one of them is not finite
-    float lo = x[0], hi = x[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) { lo = fminf(lo, x[i]); hi = fmaxf(hi, x[i]); }
-    if (check != 0.0f || hi > LARGEST || lo < -LARGEST) {
-        *bad = *bad || check != 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] != x[i] ? 0.0f : fminf(fmaxf(x[i], -LARGEST), LARGEST);
+        for (int i = 0; i < 8; ++i) {
+            *bad = *bad || !(fabsf(x[i]) < INFINITY);
+            x[i] = x[i] != x[i] ? 0.0f : fminf(fmaxf(x[i], -LARGEST), LARGEST);
+        }
         lo = hi = x[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) { lo = fminf(lo, x[i]); hi = fmaxf(hi, x[i]); }
@@ -181,185 +175,185 @@ __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
 }
 constexpr uint32_t NOTHING = 0xFF80FF80u;                                  // -inf twice
 
-template <int G> __device__ __forceinline__ void store_words(void *to, const uint32_t (&w)[G]) {
-    if constexpr (G == 4) *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-    else *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
-}
-
-// One warp appends up to 16 rows that share a record. Four lanes to a row, eight rows at a time; eight channels of every group to
-// a lane, so that key words, parameters and pairs of the rotation need no exchange beyond two shuffles of a group's extremes.
+// One warp appends up to 16 rows that share a record, ROWS of them at a time: lane ((row, j), t) has channels 32 j + 8 t + 0..7, so a
+// group's extremes meet in two shuffles, and 64 registers do. The next rows are on their way while these are quantized. A key's
+// partners in the rotation are loaded too (from the first-level cache), not exchanged.
 template <typename T, int G, bool WIDE>
 __device__ __forceinline__ void append_part(const AppendParams &p, uint8_t *rec, int head, int first_row, int first_pos, int tau0, int n,
-                                            int lane, uint32_t (&best)[2 * G * 4]) {
-    const int g = lane >> 2, t = lane & 3;
+                                            int lane, uint32_t (&best)[2][4]) {
+    constexpr int ROWS = 8 / G;
+    const int t = lane & 3, j = lane / 4 % G, odd = lane / (4 * G) & 1, c = 32 * j + 8 * t;
+    const bool rotates = c < p.rot, partner = rotates && !p.interleaved;
+    const int other = c < p.rot / 2 ? p.rot / 2 : -p.rot / 2;               // where the partners lie
     bool bad = false;
+    Eight<T> kk = {}, yy = {}, vv = {};
+    int tau = tau0 / ROWS * ROWS + lane / (4 * G);                          // the lane's token of the record; row tau - tau0 of the n
+    const T *k = reinterpret_cast<const T *>(p.k) + (int64_t)(first_row + tau - tau0) * p.k_t + (int64_t)head * p.k_h + c;
+    const T *v = reinterpret_cast<const T *>(p.v) + (int64_t)(first_row + tau - tau0) * p.v_t + (int64_t)head * p.v_h + c;
+    const int64_t k_step = ROWS * p.k_t, v_step = ROWS * p.v_t;
+    auto fetch = [&] {
+        if (tau >= tau0 && tau < tau0 + n) {
+            fetch8<T, WIDE>(k, kk);
+            if (partner) fetch8<T, WIDE>(k + other, yy);
+            fetch8<T, WIDE>(v, vv);
+        }
+        k += k_step;
+        v += v_step;
+    };
 #pragma unroll 1
-    for (int half = 0; half < 2; ++half) {
-        const int tau = 8 * half + g, i = tau - tau0;                       // the lane's token of the record, its row of the n
-        if (tau0 + n <= 8 * half || tau0 >= 8 * half + 8) continue;
+    for (int last = tau0 + n - 1, base = tau0 / ROWS * ROWS; base <= last; base += ROWS) {
+        const int here = tau, i = here - tau0;
         bool on = i >= 0 && i < n;
         const int at = on ? rope_row(p, first_row + i, first_pos + i) : 0;
         on = on && at >= 0;
-        float x[G][8];
-        uint32_t word[G], par[G];
-        const T *k = reinterpret_cast<const T *>(p.k) + (int64_t)(first_row + i) * p.k_t + (int64_t)head * p.k_h + 8 * t;
-        const T *v = reinterpret_cast<const T *>(p.v) + (int64_t)(first_row + i) * p.v_t + (int64_t)head * p.v_h + 8 * t;
+        fetch();
+        tau += ROWS;
+        float x[8], y[8];
+        unpack8(kk, x);
+        if (rotates) {
+            unpack8(yy, y);
+            rotate_key(p, x, y, max(at, 0), c);
 #pragma unroll
-        for (int j = 0; j < G; ++j) {
-            if (on) load8<T, WIDE>(k + 32 * j, x[j]);
-            else for (int e = 0; e < 8; ++e) x[j][e] = 0.0f;
+            for (int e = 0; e < 8; ++e) x[e] = to_f32(from_f32<T>(x[e]));   // what a separate rotation would have stored
         }
-        if (p.rot) {
-            rotate_key<G>(p, x, max(at, 0), t);
-#pragma unroll
-            for (int j = 0; j < G; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[j][e] = to_f32(from_f32<T>(x[j][e]));   // what a separate rotation would have stored
-        }
-#pragma unroll
-        for (int j = 0; j < G; ++j) word[j] = quantize_group(x[j], &par[j], &bad);
+        uint32_t par, word = quantize_group(x, &par, &bad);
         if (on) {
-            store_words<G>(rec + 4 * G * (tau * 4 + t), word);
-            if (t == 0) store_words<G>(rec + Rec<G>::KP + 4 * G * tau, par);
+            uint32_t *words = reinterpret_cast<uint32_t *>(rec);
+            words[(here * 4 + t) * G + j] = word;
+            if (t == 0) words[Rec<G>::KP / 4 + here * G + j] = par;
             if (p.summary) {
 #pragma unroll
-                for (int j = 0; j < G; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float a = x[j][2 * e], b = x[j][2 * e + 1];
-                        uint32_t &hi = best[j * 4 + e], &lo = best[(G + j) * 4 + e];
-                        hi = max_bf16x2(hi, ceil_bf16(a) | ceil_bf16(b) << 16);
-                        lo = max_bf16x2(lo, (floor_bf16(a) | floor_bf16(b) << 16) ^ 0x80008000u);
+                for (int e = 0; e < 4; ++e) {
+                    const float a = x[2 * e], b = x[2 * e + 1];
+                    uint32_t up, down;
+                    if constexpr (std::is_same<T, __nv_bfloat16>::value) {          // what came from bf16 is bf16
+                        up = down = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+                    } else {
+                        up = ceil_bf16(a) | ceil_bf16(b) << 16;
+                        down = floor_bf16(a) | floor_bf16(b) << 16;
                     }
+                    best[0][e] = max_bf16x2(best[0][e], up);
+                    best[1][e] = max_bf16x2(best[1][e], down ^ 0x80008000u);
+                }
             }
         }
-        // values: a word needs two tokens, and a lane's word of eight channels is two half words of four
-#pragma unroll
-        for (int j = 0; j < G; ++j) {
-            if (on) load8<T, WIDE>(v + 32 * j, x[j]);
-            else for (int e = 0; e < 8; ++e) x[j][e] = 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < G; ++j) word[j] = quantize_group(x[j], &par[j], &bad);
-        const bool both = __shfl_xor_sync(~0u, (int)on, 4) && on;
-        const int pair = g >> 1, odd = g & 1;                               // tokens 8 half + 2 pair + {0, 1}
-        uint32_t two[G];
-#pragma unroll
-        for (int j = 0; j < G; ++j) {
-            // the even token's lane makes the words of channel quad 2 t, the odd one's those of 2 t + 1
-            const uint32_t other = __shfl_xor_sync(~0u, word[j], 4);
-            two[j] = odd ? __byte_perm(other, word[j], 0x7632) : __byte_perm(word[j], other, 0x5410);
-        }
-        uint8_t *vc = rec + Rec<G>::V;
+        // values: a word holds four channels of two tokens; the even token's lane makes those of channel quad 2 t, the odd one's of 2 t + 1
+        unpack8(vv, x);
+        word = quantize_group(x, &par, &bad);
+        const bool both = __shfl_xor_sync(~0u, (int)on, 4 * G) && on;
+        const uint32_t theirs = __shfl_xor_sync(~0u, word, 4 * G);
+        uint8_t *quad = rec + Rec<G>::V + 4 * (G * (32 * (here >> 3) + 8 * t + (here >> 1 & 3)) + j);
         if (both) {
-            store_words<G>(vc + 4 * G * (32 * half + 4 * (2 * t + odd) + pair), two);
+            *reinterpret_cast<uint32_t *>(quad + 16 * G * odd) = odd ? __byte_perm(theirs, word, 0x7632) : __byte_perm(word, theirs, 0x5410);
         } else if (on) {
-#pragma unroll
-            for (int j = 0; j < G; ++j) {
-                *reinterpret_cast<uint16_t *>(vc + 4 * (G * (32 * half + 4 * (2 * t) + pair) + j) + 2 * odd) = (uint16_t)word[j];
-                *reinterpret_cast<uint16_t *>(vc + 4 * (G * (32 * half + 4 * (2 * t + 1) + pair) + j) + 2 * odd) = (uint16_t)(word[j] >> 16);
-            }
+            *reinterpret_cast<uint16_t *>(quad + 2 * odd) = (uint16_t)word;
+            *reinterpret_cast<uint16_t *>(quad + 16 * G + 2 * odd) = (uint16_t)(word >> 16);
         }
-        if (on && t == 0) store_words<G>(rec + Rec<G>::VP + 4 * G * tau, par);
+        if (on && t == 0) *reinterpret_cast<uint32_t *>(rec + Rec<G>::VP + 4 * (here * G + j)) = par;
     }
     if (bad) or_status(p.status, OMMX_ST_NONFINITE);
 }
 
-// Largest over the eight rows of a warp, halving what a lane holds at every step. Lane (g, t) ends with four registers (eight
-// channels): of 2 G runs of four, run g for G = 4, run g / 2 for G = 2.
-template <int G> __device__ __forceinline__ void reduce_rows(uint32_t (&a)[2 * G * 4], int lane) {
-    int n = 2 * G * 4;
-#pragma unroll
-    for (int d = 16; d >= 4; d /= 2) {
-        if (n > 4) {
-            n /= 2;
-#pragma unroll
-            for (int i = 0; i < G * 4; ++i)
-                if (i < n) {
-                    const bool up = lane & d;
-                    const uint32_t give = up ? a[i] : a[i + n], keep = up ? a[i + n] : a[i];
-                    a[i] = max_bf16x2(keep, __shfl_xor_sync(~0u, give, d));
-                }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = max_bf16x2(a[i], __shfl_xor_sync(~0u, a[i], d));
-        }
-    }
-}
+constexpr int WARPS = 4;
 
-constexpr int WARPS = 4, Q_ROWS = 4;
-
-// Grid: (runs of rows that share a page, kv_blocks + query blocks). The first kv_blocks blocks of a run take its keys and values, a
-// warp to 16 tokens of a head (pages over 64 tokens: a warp to several of them); the others rotate the query rows, q_rows each.
+// Grid: `blocks` for each run of rows that share a page. The first kv_blocks of a run take its keys and values, a warp to 16 tokens of a
+// head (pages over 64 tokens: a warp to several of them); the others rotate the query rows, q_rows each. Lying side by side, the
+// first, which the quantizer's instructions bound, and the second, which memory does, share the SMs.
 template <typename T, int G, bool WIDE>
-__global__ void __launch_bounds__(32 * WARPS) kv4_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 5 : 7) kv4_append_kernel(const __grid_constant__ AppendParams p) {
     constexpr int D = 32 * G;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     wait_earlier();
     let_next_in();
     Run run;
-    if (!find_run(p.s, p.rows, p.page_shift, blockIdx.x, lane, &run, p.status)) return;
+    const int runs_at = blockIdx.x / p.blocks, block = blockIdx.x - runs_at * p.blocks;
+    if (!find_run(p.s, p.rows, p.page_shift, runs_at, lane, &run, p.status)) return;
     const int page = 1 << p.page_shift;
 
-    if ((int)blockIdx.y >= p.kv_blocks) {                                   // ---- query rows
+    if (block >= p.kv_blocks) {                                   // ---- query rows
         int p0 = run.p0, p1 = run.p1;
         if (p.q_rows < page) {
-            const int from = (run.p0 & -page) + ((int)blockIdx.y - p.kv_blocks) * p.q_rows;
+            const int from = (run.p0 & -page) + (block - p.kv_blocks) * p.q_rows;
             p0 = max(p0, from);
             p1 = min(p1, from + p.q_rows);
         }
-        const int items = (p1 - p0) * p.Hq * (D / 16);
-#pragma unroll 2
-        for (int i = threadIdx.x; i < items; i += 32 * WARPS) {
-            const int c = i % (D / 16), r = i / (D / 16) / p.Hq, h = i / (D / 16) - r * p.Hq;
+        // a thread to sixteen channels of a row: their angles are loaded once for all heads, and two heads are on their way
+        constexpr int CHUNKS = D / 16, TURNS = 2;
+        const int slots = 32 * WARPS / CHUNKS, rows = p1 - p0, lots = max(1, slots / max(rows, 1));   // threads to a chunk: rows x lots
+        const int c = threadIdx.x % CHUNKS, slot = threadIdx.x / CHUNKS;
+        for (int r = slot / lots; r < rows; r += slots / lots) {
             const int row = run.row + p0 - run.p0 + r, at = rope_row(p, row, p0 + r);
             if (at < 0) continue;
             const bool turned = 16 * c < p.rot;
             const int first = turned && !p.interleaved ? 8 * c : 16 * c, second = turned && !p.interleaved ? 8 * c + p.rot / 2 : 16 * c + 8;
-            const T *in = reinterpret_cast<const T *>(p.q) + (int64_t)row * p.q_t + (int64_t)h * p.q_h;
-            T *out = reinterpret_cast<T *>(p.q_out) + (int64_t)row * p.o_t + (int64_t)h * p.o_h;
-            float x[16];
-            load8<T, WIDE>(in + first, x);
-            load8<T, WIDE>(in + second, x + 8);
+            float cs[8], sn[8];
             if (turned) {
-                float cs[8], sn[8];
                 load_f32<8>(p.cos + at * p.cs_stride + 8 * c, cs);
                 load_f32<8>(p.sin + at * p.cs_stride + 8 * c, sn);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (p.interleaved) turn(x[2 * e], x[2 * e + 1], cs[e], sn[e]);
-                    else turn(x[e], x[8 + e], cs[e], sn[e]);
-                }
             }
-            store8<T, WIDE>(out + first, x);
-            store8<T, WIDE>(out + second, x + 8);
+            const T *in = reinterpret_cast<const T *>(p.q) + (int64_t)row * p.q_t;
+            T *out = reinterpret_cast<T *>(p.q_out) + (int64_t)row * p.o_t;
+            for (int h0 = slot % lots; h0 < p.Hq; h0 += TURNS * lots) {
+                Eight<T> raw[TURNS][2];
+#pragma unroll
+                for (int u = 0; u < TURNS; ++u)
+                    if (h0 + u * lots < p.Hq) {
+                        fetch8<T, WIDE>(in + (h0 + u * lots) * p.q_h + first, raw[u][0]);
+                        fetch8<T, WIDE>(in + (h0 + u * lots) * p.q_h + second, raw[u][1]);
+                    }
+#pragma unroll
+                for (int u = 0; u < TURNS; ++u)
+                    if (h0 + u * lots < p.Hq) {
+                        float x[16];
+                        unpack8(raw[u][0], x);
+                        unpack8(raw[u][1], x + 8);
+                        if (turned) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                if (p.interleaved) turn(x[2 * e], x[2 * e + 1], cs[e], sn[e]);
+                                else turn(x[e], x[8 + e], cs[e], sn[e]);
+                            }
+                        }
+                        store8<T, WIDE>(out + (h0 + u * lots) * p.o_h + first, x);
+                        store8<T, WIDE>(out + (h0 + u * lots) * p.o_h + second, x + 8);
+                    }
+            }
         }
         return;
     }
 
     // ---- keys and values
-    const int warps_a_head = min(p.c.parts, WARPS), heads = WARPS / warps_a_head;
-    const int head = blockIdx.y * heads + warp / warps_a_head;
+    const int pieces = p.c.parts * p.split, warps_a_head = min(pieces, WARPS), heads = WARPS / warps_a_head, size = 16 / p.split;
+    const int head = block * heads + warp / warps_a_head;
     const int at = run.p0 >> p.page_shift;
     int64_t id = -1;
     if (at < p.s.max_pages) id = page_id(p.s, run.b, at);
     else or_status(p.status, OMMX_ST_BAD_LENGTH);
     if (at < p.s.max_pages && (id < 0 || id >= p.c.num_pages)) { or_status(p.status, OMMX_ST_BAD_PAGE); id = -1; }
     if (id < 0) return;                                                     // the whole block: one run, one page
-    uint32_t best[2 * G * 4];
+    uint32_t best[2][4];                          // maxima and negated minima of the lane's eight channels
 #pragma unroll
-    for (int i = 0; i < 2 * G * 4; ++i) best[i] = NOTHING;
+    for (int i = 0; i < 4; ++i) best[0][i] = best[1][i] = NOTHING;
     if (head < p.c.H)
-        for (int part = warp % warps_a_head; part < p.c.parts; part += warps_a_head) {
-            const int base = (run.p0 & -page) + 16 * part, p0 = max(run.p0, base), p1 = min(run.p1, base + 16);
+        for (int piece = warp % warps_a_head; piece < pieces; piece += warps_a_head) {
+            const int part = piece / p.split, base = (run.p0 & -page) + 16 * part;
+            const int p0 = max(run.p0, base + piece % p.split * size), p1 = min(run.p1, base + (piece % p.split + 1) * size);
             if (p0 >= p1) continue;
             uint8_t *rec = p.c.records + ((id * p.c.H + head) * p.c.parts + part) * Rec<G>::BYTES;
             append_part<T, G, WIDE>(p, rec, head, run.row + p0 - run.p0, p0, p0 - base, p1 - p0, lane, best);
         }
     if (!p.summary) return;
-    reduce_rows<G>(best, lane);
+#pragma unroll
+    for (int d = 4 * G; d < 32; d *= 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            best[0][i] = max_bf16x2(best[0][i], __shfl_xor_sync(~0u, best[0][i], d));
+            best[1][i] = max_bf16x2(best[1][i], __shfl_xor_sync(~0u, best[1][i], d));
+        }
+    // the first row's lanes go on with the maxima, the second's with the minima
     __shared__ uint4 shared[WARPS][32];
-    uint4 own = make_uint4(best[0], best[1], best[2], best[3]);
+    const bool low = lane / (4 * G) & 1;
+    uint4 own = low ? make_uint4(best[1][0], best[1][1], best[1][2], best[1][3]) : make_uint4(best[0][0], best[0][1], best[0][2], best[0][3]);
     if (warps_a_head > 1) {
         shared[warp][lane] = own;
         __syncthreads();
@@ -369,13 +363,10 @@ __global__ void __launch_bounds__(32 * WARPS) kv4_append_kernel(const __grid_con
             own = make_uint4(max_bf16x2(own.x, o.x), max_bf16x2(own.y, o.y), max_bf16x2(own.z, o.z), max_bf16x2(own.w, o.w));
         }
     }
-    if (head >= p.c.H) return;
-    const int g = lane >> 2, t = lane & 3, r = G == 4 ? g : g >> 1;         // r: run of four of 2 G
-    if (G == 2 && (g & 1)) return;
-    const bool low = r >= G;
-    uint4 *to = reinterpret_cast<uint4 *>(p.summary + ((id * p.c.H + head) * 2 + low) * D + 32 * (r % G) + 8 * t);
-    const uint32_t sign = low ? 0x80008000u : 0u;
+    if (head >= p.c.H || lane >= 8 * G) return;
     if (own.x == NOTHING) return;                                           // none of its rows was stored
+    uint4 *to = reinterpret_cast<uint4 *>(p.summary + ((id * p.c.H + head) * 2 + low) * D + 32 * (lane / 4 % G) + 8 * (lane & 3));
+    const uint32_t sign = low ? 0x80008000u : 0u;
     if (run.p0 & (page - 1)) {                                              // the page held tokens before: theirs count too
         const uint4 o = *to;
         own = make_uint4(max_bf16x2(own.x, o.x ^ sign), max_bf16x2(own.y, o.y ^ sign), max_bf16x2(own.z, o.z ^ sign), max_bf16x2(own.w, o.w ^ sign));
@@ -488,16 +479,23 @@ static int append(const ommx_kv4_append_args *a, cudaStream_t st) {
     p.rot = a->rot_dim; p.interleaved = a->interleaved; p.Hq = a->q ? a->n_q_heads : 0;
     p.page_shift = shift_of(p.c.page);
     p.status = a->status;
-    const int heads = WARPS / (p.c.parts < WARPS ? p.c.parts : WARPS);
+    // A record to a warp, or to two or four where there are fewer records than warps that the SMs hold (2049 rows of 4 heads: 14.8 us
+    // with one, 10.2 with four)
+    p.split = 1;
+    while (p.split < 4 && a->num_rows >= 16LL * p.split * p.s.B && (int64_t)a->num_rows * p.c.H / (16 * p.split) < 28LL * sm_count()) p.split *= 2;
+    const int pieces = p.c.parts * p.split, heads = WARPS / (pieces < WARPS ? pieces : WARPS);
     p.kv_blocks = (p.c.H + heads - 1) / heads;
-    p.q_rows = a->row_start ? Q_ROWS : p.c.page;
-    const int q_blocks = !a->q ? 0 : a->row_start ? p.c.page / Q_ROWS : 1;
+    // Query rows to a block: at most 16, and fewer until there are two blocks to an SM, but no more blocks to a run than it has rows
     const int64_t runs = most_runs(a->num_rows, p.s.B, p.c.page, a->row_start == nullptr);
-    if (p.kv_blocks + q_blocks > 65535) return fail(OMMX_E_UNSUPPORTED, "kv4_append: %d kv heads", p.c.H);
+    p.q_rows = p.c.page;
+    while (p.c.page / p.q_rows < a->num_rows / runs && (p.q_rows > 16 || runs * (p.c.page / p.q_rows) < 2LL * sm_count())) p.q_rows /= 2;
+    const int q_blocks = !a->q ? 0 : p.c.page / p.q_rows;
+    p.blocks = p.kv_blocks + q_blocks;
+    if (runs * p.blocks >= 1LL << 31) return fail(OMMX_E_UNSUPPORTED, "kv4_append: %d rows of %d kv heads in one call", a->num_rows, p.c.H);
     const int bytes = a->dtype == OMMX_DT_F32 ? 4 : 2;
     const bool wide = aligned16(a->k_new, p.k_t, p.k_h, bytes) && aligned16(a->v_new, p.v_t, p.v_h, bytes) &&
                       (!a->q || (aligned16(a->q, p.q_t, p.q_h, bytes) && aligned16(a->q_out, p.o_t, p.o_h, bytes)));
-    return launch_dependent(KV4_PICK(kv4_append_kernel, a->dtype, G, wide), dim3((unsigned)runs, p.kv_blocks + q_blocks), 32 * WARPS, 0, st, p);
+    return launch_dependent(KV4_PICK(kv4_append_kernel, a->dtype, G, wide), dim3((unsigned)(runs * p.blocks)), 32 * WARPS, 0, st, p);
 }
 
 static int gather(const ommx_kv4_gather_args *a, cudaStream_t st) {
