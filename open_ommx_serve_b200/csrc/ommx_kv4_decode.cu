@@ -13,20 +13,22 @@
 // the scale, they are 2^12 at most, and those below 2^-36 of the largest are lost. That is an eighth of a bf16 output's own
 // rounding; where the output is finer (fp16, fp32), a second product takes what the rounding left (FINE). Sums of weights and
 // zeros stay fp32.
+#include <type_traits>
+
 #include "ommx_kv4.cuh"
 
 namespace ommx {
 namespace kv4 {
 
-constexpr int NW = 8;                             // warps to a block, each with tiles of 16 tokens of its own
+constexpr int WARPS_PER_SM = 16;                  // as many as the registers hold; a block is NW of them, each with records of its own
 constexpr int STAGES = 4, AHEAD = STAGES - 1;     // records that a warp holds, and those of them on their way
 constexpr int FULL = 0x101010;                    // sixteen tokens in each of those
 constexpr int COLS = 8;                           // query heads side by side
-constexpr int BLOCKS_PER_SM = 2;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float ROOM = 4096.0f;                   // how large a weight may get before its reference moves
 constexpr float LOWEST = -1e30f;
-constexpr int WHOLE = 4 * NW;                     // records of a row that one block takes at most where it could share it
+constexpr int MOST_PARTS = 768;                   // blocks of a call that shares rows
+constexpr int WHOLE = 32;                         // records of a row that one block takes at most where it could share it
 
 struct DecodeParams {
     Cache c;
@@ -371,8 +373,9 @@ template <int G, bool FINE> __device__ __forceinline__ void attend(const DecodeP
     }
 }
 
-template <int G> struct Shared {
-    static constexpr int D = 32 * G, PART = COLS * D + 2 * COLS;   // floats of a part in the workspace
+template <int G> constexpr int PART = COLS * 32 * G + 2 * COLS;            // floats of a part in the workspace
+template <int G, int NW> struct Shared {
+    static constexpr int D = 32 * G;
     float o[NW][COLS][D + 4];                     // the padding spreads the heads over the banks
 };
 template <int G> struct Floats;
@@ -383,12 +386,12 @@ template <int G> __device__ __forceinline__ void store_o(const DecodeParams &p, 
     for (int i = 0; i < G; ++i) store_o(p, at + i, v[i]);
 }
 
-// The warps' states of a row to its output, or to a part: [COLS][D] weighted values, [COLS] references, [COLS] sums. Warp h finishes
-// head h, a lane G channels.
-template <int G>
-__device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Shared<G> &sh, float (&ref)[COLS][NW], float (&sum)[COLS][NW], int b,
+// The warps' states of a row to its output, or to a part: [COLS][D] weighted values, [COLS] references, [COLS] sums. A warp
+// finishes every NW-th head, a lane G channels.
+template <int G, int NW>
+__device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Shared<G, NW> &sh, float (&ref)[COLS][NW], float (&sum)[COLS][NW], int b,
                                        int first_head, int n, float *part, int warp, int lane) {
-    static_assert(NW == COLS, "a warp finishes a head");
+    static_assert(NW >= G, "a warp to a group of channels when queries are loaded");
     using V = typename Floats<G>::T;
     constexpr int D = 32 * G;
     const int g = lane >> 2, t = lane & 3;
@@ -423,37 +426,39 @@ __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Share
             *reinterpret_cast<float4 *>(to) = make_float4(f[i] * fmaf(s.acc[j][0][i] - s.acc[j][0][i + 2], 0x1p24f, z), f[i] * fmaf(s.acc[j][0][i + 2], 0x1p20f, z),
                                                           f[i] * fmaf(s.acc[j][1][i] - s.acc[j][1][i + 2], 0x1p24f, z), f[i] * fmaf(s.acc[j][1][i + 2], 0x1p20f, z));
         }
-    float top = ref[warp][0], all = 0.0f;
-#pragma unroll
-    for (int w = 1; w < NW; ++w) top = fmaxf(top, ref[warp][w]);
-#pragma unroll
-    for (int w = 0; w < NW; ++w) all = fmaf(sum[warp][w], exp2_approx(ref[warp][w] - top), all);
     __syncthreads();
-    float v[G];
+    for (int h = warp; h < COLS; h += NW) {
+        float top = ref[h][0], all = 0.0f;
 #pragma unroll
-    for (int i = 0; i < G; ++i) v[i] = 0.0f;
+        for (int w = 1; w < NW; ++w) top = fmaxf(top, ref[h][w]);
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        const V x = *reinterpret_cast<const V *>(&sh.o[w][warp][lane * G]);
+        for (int w = 0; w < NW; ++w) all = fmaf(sum[h][w], exp2_approx(ref[h][w] - top), all);
+        float v[G];
 #pragma unroll
-        for (int i = 0; i < G; ++i) v[i] += reinterpret_cast<const float *>(&x)[i];
-    }
-    if (part) {
-        *reinterpret_cast<V *>(part + warp * D + lane * G) = *reinterpret_cast<const V *>(v);
-        if (lane == 0) { part[COLS * D + warp] = top; part[COLS * D + COLS + warp] = all; }
-    } else if (warp < n) {
-        const float inverse = all != 0.0f ? 1.0f / all : 0.0f;
+        for (int i = 0; i < G; ++i) v[i] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < G; ++i) v[i] = all != 0.0f ? v[i] * inverse : 0.0f;
-        store_o(p, b * p.o_b + (first_head + warp) * p.o_h + lane * G, v);
-        if (lane == 0) p.lse[b * p.lse_b + first_head + warp] = all != 0.0f ? (top + log2f(all)) * LN2 : -INFINITY;
+        for (int w = 0; w < NW; ++w) {
+            const V x = *reinterpret_cast<const V *>(&sh.o[w][h][lane * G]);
+#pragma unroll
+            for (int i = 0; i < G; ++i) v[i] += reinterpret_cast<const float *>(&x)[i];
+        }
+        if (part) {
+            *reinterpret_cast<V *>(part + h * D + lane * G) = *reinterpret_cast<const V *>(v);
+            if (lane == 0) { part[COLS * D + h] = top; part[COLS * D + COLS + h] = all; }
+        } else if (h < n) {
+            const float inverse = all != 0.0f ? 1.0f / all : 0.0f;
+#pragma unroll
+            for (int i = 0; i < G; ++i) v[i] = all != 0.0f ? v[i] * inverse : 0.0f;
+            store_o(p, b * p.o_b + (first_head + h) * p.o_h + lane * G, v);
+            if (lane == 0) p.lse[b * p.lse_b + first_head + h] = all != 0.0f ? (top + log2f(all)) * LN2 : -INFINITY;
+        }
     }
     __syncthreads();
 }
 
-template <int G> struct Memory {
+template <int G, int NW> struct Memory {
     union {
-        Shared<G> sh;
+        Shared<G, NW> sh;
         uint8_t ring[NW][STAGES][Rec<G>::BYTES];
     };
     QueryMemory<G> query;
@@ -467,9 +472,9 @@ template <int G> __device__ __forceinline__ void nothing(const DecodeParams &p, 
     if (threadIdx.x < n) p.lse[b * p.lse_b + first + threadIdx.x] = -INFINITY;
 }
 
-template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PER_SM) kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
+template <int G, bool FINE, int NW> __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
     extern __shared__ __align__(128) uint8_t memory[];
-    Memory<G> &m = *reinterpret_cast<Memory<G> *>(memory);
+    Memory<G, NW> &m = *reinterpret_cast<Memory<G, NW> *>(memory);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint8_t *ring = m.ring[warp][0];
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + 16 * lane;
@@ -587,8 +592,8 @@ template <int G, bool FINE> __global__ void __launch_bounds__(32 * NW, BLOCKS_PE
         }
         fetched<0>();
         float *part = nullptr;
-        if (i0 > 0 || i1 < units) part = p.work + HEAD + (2 * (int64_t)blockIdx.x + (base + row * units >= second)) * Shared<G>::PART;
-        finish<G>(p, s, m.sh, m.ref, m.sum, b, first_head, n, part, warp, lane);
+        if (i0 > 0 || i1 < units) part = p.work + HEAD + (2 * (int64_t)blockIdx.x + (base + row * units >= second)) * PART<G>;
+        finish<G, NW>(p, s, m.sh, m.ref, m.sum, b, first_head, n, part, warp, lane);
         u += i1 - i0;
     }
 }
@@ -622,7 +627,7 @@ __device__ __forceinline__ Parts parts_of(const DecodeParams &p, int b, uint32_t
     return r;
 }
 template <int G> __device__ __forceinline__ const float *part_at(const DecodeParams &p, const Parts &r, int i) {
-    return p.work + HEAD + (2 * (int64_t)(r.first + i) + (i == 0 && r.late)) * Shared<G>::PART;
+    return p.work + HEAD + (2 * (int64_t)(r.first + i) + (i == 0 && r.late)) * PART<G>;
 }
 template <int G> __device__ __forceinline__ void zeros(const DecodeParams &p, int b, int hq, int lane) {      // a head of no tokens
 #pragma unroll
@@ -678,7 +683,7 @@ template <int G> __global__ void __launch_bounds__(32 * COLS) kv4_combine_row_ke
 
 // The same where rows are few and their parts many: a block to a head. The references and sums of all parts are read at once; then a
 // warp takes every CW-th part, UNROLL of them on their way. Grid: (rows of a sequence x COLS, sequences).
-constexpr int CW = 8, UNROLL = 5, MOST_PARTS = 512;
+constexpr int CW = 8, UNROLL = 5;
 template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_head_kernel(const __grid_constant__ DecodeParams p) {
     constexpr int D = 32 * G;
     using V = typename Floats<G>::T;
@@ -750,24 +755,24 @@ template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_head_ker
 }
 
 // ---- host ---------------------------------------------------------------------------------------
-static int64_t most_blocks() {
-    const int n = BLOCKS_PER_SM * sm_count();
+static int64_t most_blocks(int warps) {
+    const int n = WARPS_PER_SM / warps * sm_count();
     return n < MOST_PARTS ? n : MOST_PARTS;
 }
 static int64_t workspace_floats(int head_dim) {
-    const int64_t part = head_dim == 64 ? Shared<2>::PART : Shared<4>::PART;
-    return HEAD + 2 * part * most_blocks();
+    const int64_t part = head_dim == 64 ? PART<2> : PART<4>;
+    return HEAD + 2 * part * most_blocks(4);
 }
 
-template <int G, bool FINE> static int launch_decode(const DecodeParams &p, int64_t blocks, cudaStream_t st) {
+template <int G, bool FINE, int NW> static int launch_decode(const DecodeParams &p, int64_t blocks, cudaStream_t st) {
     static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may take its shared memory
     int dev = 0;
     if (int rc = current_device(&dev)) return rc;
     if (!(allowed.load(std::memory_order_acquire) >> dev & 1)) {
-        OMMX_CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<G, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Memory<G>)));
+        OMMX_CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<G, FINE, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Memory<G, NW>)));
         allowed.fetch_or(1ull << dev, std::memory_order_release);
     }
-    if (int rc = launch_dependent(kv4_decode_kernel<G, FINE>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G>), st, p)) return rc;
+    if (int rc = launch_dependent(kv4_decode_kernel<G, FINE, NW>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G, NW>), st, p)) return rc;
     if (p.whole) return 0;
     // a row has some blocks / rows parts
     const int rows = p.c.H * p.col_blocks;
@@ -813,19 +818,29 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     p.page_shift = shift_of(p.c.page);
     p.sm_scale = a->sm_scale; p.cap = a->logit_cap; p.status = a->status;
     if (p.c.num_pages == 0) return fail(OMMX_E_ARG, "kv4_decode: a cache of no pages");   // what is fetched for a page that is not there
-    p.least = 2 * NW;
     // as many blocks as the SMs hold, no more than the work can have
     const int64_t units = most_units(a);
     const int64_t rows = (int64_t)p.s.B * p.c.H * p.col_blocks;
     if (units * rows >= 1LL << 31 || rows * COLS >= 1LL << 31)
         return fail(OMMX_E_UNSUPPORTED, "kv4_decode: %lld rows of up to %lld records (2^31 in all are counted): give max_seq_len", (long long)rows, (long long)units);
-    // As many blocks as the SMs hold, no more than the work can have. Rows that are short for certain go whole to a block each, and
-    // the second kernel is not needed.
+    // Blocks of eight warps where rows are few, so that a row has few parts, of four where they are many: then blocks often go on from
+    // one row to the next, and an SM's others work meanwhile (64 sequences of 200..2000 tokens, 8 kv heads: 43 us with four, 54 with
+    // eight; one of 64K: 25.4 and 24.4). As many blocks as the SMs hold, no more than the work can have. Rows that are short for
+    // certain go whole to a block each, and the second kernel is not needed.
+    const int warps = rows >= 64 ? 4 : 8;
+    p.least = 2 * warps;
     p.whole = units <= WHOLE;
-    const int64_t most = (units * rows + p.least - 1) / p.least, hold = most_blocks();
+    const int64_t most = (units * rows + p.least - 1) / p.least, hold = most_blocks(warps);
     const int64_t blocks = p.whole ? rows : most < 1 ? 1 : most < hold ? most : hold;
-    if (a->o_dtype == OMMX_DT_BF16) return a->cache.head_dim == 64 ? launch_decode<2, false>(p, blocks, st) : launch_decode<4, false>(p, blocks, st);
-    return a->cache.head_dim == 64 ? launch_decode<2, true>(p, blocks, st) : launch_decode<4, true>(p, blocks, st);
+    auto launch = [&](auto g, auto fine) {
+        constexpr int G = decltype(g)::value;
+        constexpr bool FINE = decltype(fine)::value;
+        return warps == 4 ? launch_decode<G, FINE, 4>(p, blocks, st) : launch_decode<G, FINE, 8>(p, blocks, st);
+    };
+    using std::integral_constant;
+    if (a->o_dtype == OMMX_DT_BF16)
+        return a->cache.head_dim == 128 ? launch(integral_constant<int, 4>(), std::false_type()) : launch(integral_constant<int, 2>(), std::false_type());
+    return a->cache.head_dim == 128 ? launch(integral_constant<int, 4>(), std::true_type()) : launch(integral_constant<int, 2>(), std::true_type());
 }
 
 }  // namespace kv4
