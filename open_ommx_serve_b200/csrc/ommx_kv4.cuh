@@ -48,17 +48,20 @@ __device__ __forceinline__ void wait_earlier() { asm volatile("griddepcontrol.wa
 __device__ __forceinline__ void let_next_in() { asm volatile("griddepcontrol.launch_dependents;"); }
 
 template <typename K, typename... A>
-int launch_dependent(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream, const A &...args) {
+int launch_dependent(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream, int cluster, const A &...args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     OMMX_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
     count_launch();
     return 0;

@@ -47,15 +47,15 @@ struct DecodeParams {
 // Units are records (16 tokens of a kv head, for a block of COLS of its query heads); a row (sequence, kv head, block of heads) is a
 // run of them. Lengths are known on the device alone, so every block works the same deal out, and leaves it for the
 // second kernel:
-// * a block to a row, where the host knows that rows are short (`whole`);
+// * a block to a row, where the host knows that rows are short (`whole`), or a cluster of blocks, which exchange their parts themselves;
 // * else every row is cut into pieces of at most `per` units, a block to a piece, with the smallest `per` for which there are blocks
 //   enough;
 // * or, where that would leave a block with over BEGIN units more than an even share, all rows end to end are cut into such shares,
-//   whatever rows they touch. A second piece costs a block some 4 us, half of it hidden by the SM's other block (64K tokens: 26.7 us
-//   with seven such blocks of 296, 24.3 with none; 32 sequences of 700..8191: 66.9 with even shares, 74.8 with pieces up to 28 longer).
+//   whatever rows they touch. A second piece costs a block some 4 us, half of it hidden by the SM's other blocks (64K tokens: 26.7 us
+//   with seven such blocks of 296, 24.4 with none; 64 sequences of 200..2000 tokens: 43.3 with even shares, 38.3 with pieces).
 // A piece that is a whole row is finished where it is computed; the others' parts meet in the second kernel. A block has at most two
 // of those, of the row that an earlier block began (its slot 0) and of the one that a later block goes on with (slot 1).
-constexpr int BEGIN = 12, HEAD = 4;               // HEAD: floats in front of the parts, which hold the deal
+constexpr int BEGIN = 64, HEAD = 4;               // HEAD: floats in front of the parts, which hold the deal
 __device__ __forceinline__ int pages_of(const DecodeParams &p, int len) { return (len + p.c.page - 1) >> p.page_shift; }
 __device__ __forceinline__ int length_of(const DecodeParams &p, int b) {
     const int len = p.s.len[b];
@@ -463,6 +463,7 @@ template <int G, int NW> struct Memory {
     };
     QueryMemory<G> query;
     float ref[COLS][NW], sum[COLS][NW];
+    alignas(16) float merged[PART<G>];            // of this block, where a cluster shares a row
 };
 
 // A row of no tokens
@@ -472,7 +473,63 @@ template <int G> __device__ __forceinline__ void nothing(const DecodeParams &p, 
     if (threadIdx.x < n) p.lse[b * p.lse_b + first + threadIdx.x] = -INFINITY;
 }
 
-template <int G, bool FINE, int NW> __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
+// ---- a row shared by a cluster's blocks: their parts meet in distributed shared memory ----
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 peer_float4(uint32_t at, uint32_t rank) {
+    uint32_t there;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
+    return v;
+}
+__device__ __forceinline__ float peer_float(uint32_t at, uint32_t rank) {
+    uint32_t there;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+    return v;
+}
+// Head h is finished by block h mod n of the cluster, by its warp h.
+constexpr int MOST_CLUSTER = 8;
+template <int G> __device__ __forceinline__ void merge_cluster(const DecodeParams &p, const float *merged, int b, int first_head, int heads, int h, int lane) {
+    constexpr int D = 32 * G, LANES = D / 4;      // lanes that have four channels
+    const uint32_t n = cluster_size(), at = (uint32_t)__cvta_generic_to_shared(merged);
+    cluster_barrier();
+    if (h < heads && h % n == cluster_rank()) {
+        float4 v[MOST_CLUSTER];
+        float ref[MOST_CLUSTER], sum[MOST_CLUSTER];
+#pragma unroll
+        for (int r = 0; r < MOST_CLUSTER; ++r) {
+            const uint32_t from = r < (int)n ? r : 0;
+            v[r] = peer_float4(at + 4 * (h * D + 4 * (lane % LANES)), from);
+            ref[r] = r < (int)n ? peer_float(at + 4 * (COLS * D + h), from) : LOWEST;
+            sum[r] = r < (int)n ? peer_float(at + 4 * (COLS * D + COLS + h), from) : 0.0f;
+        }
+        float top = ref[0], all = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int r = 1; r < MOST_CLUSTER; ++r) top = fmaxf(top, ref[r]);
+#pragma unroll
+        for (int r = 0; r < MOST_CLUSTER; ++r)
+            if (r < (int)n) {
+                const float f = exp2_approx(ref[r] - top);
+                all = fmaf(sum[r], f, all);
+                o[0] = fmaf(v[r].x, f, o[0]); o[1] = fmaf(v[r].y, f, o[1]); o[2] = fmaf(v[r].z, f, o[2]); o[3] = fmaf(v[r].w, f, o[3]);
+            }
+        const float inverse = all != 0.0f ? 1.0f / all : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = all != 0.0f ? o[i] * inverse : 0.0f;
+        if (lane < LANES) store_o(p, b * p.o_b + (first_head + h) * p.o_h + 4 * lane, o);
+        if (lane == 0) p.lse[b * p.lse_b + first_head + h] = all != 0.0f ? (top + log2f(all)) * LN2 : -INFINITY;
+    }
+    cluster_barrier();                            // no block leaves before its peers have read its part
+}
+
+template <int G, bool FINE, int NW, bool CLUSTER>
+__global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
     extern __shared__ __align__(128) uint8_t memory[];
     Memory<G, NW> &m = *reinterpret_cast<Memory<G, NW> *>(memory);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -485,7 +542,19 @@ template <int G, bool FINE, int NW> __global__ void __launch_bounds__(32 * NW, W
     uint32_t u, end, base = 0;                    // this block's units; units before sequence b
     uint32_t second = ~0u;                        // a row that begins here or later leaves its part in the second slot
     int b = 0, units = 0, len = 0;
-    if (p.whole) {                                // a block to a row
+    if (CLUSTER) {                                // a cluster to a row
+        const uint32_t n = cluster_size(), rank = cluster_rank(), at = blockIdx.x / n;
+        b = at / rows;
+        len = length_of(p, b);
+        units = units_of(p, len);
+        if (units == 0) {                         // for all of the cluster
+            if (rank == 0) nothing<G>(p, b, at - b * rows);
+            return;
+        }
+        u = (at - b * rows) * units;
+        end = u + units * (rank + 1) / n;
+        u += units * rank / n;
+    } else if (p.whole) {                         // a block to a row
         b = blockIdx.x / rows;
         len = length_of(p, b);
         units = units_of(p, len);
@@ -523,7 +592,7 @@ template <int G, bool FINE, int NW> __global__ void __launch_bounds__(32 * NW, W
             end = min(u + d.per, d.total);
         }
     }
-    while (u < end) {
+    while (CLUSTER || u < end) {
         while (u >= base + units * rows) {        // the next sequence that has any
             base += units * rows;
             len = length_of(p, ++b);
@@ -591,6 +660,11 @@ template <int G, bool FINE, int NW> __global__ void __launch_bounds__(32 * NW, W
             }
         }
         fetched<0>();
+        if constexpr (CLUSTER) {
+            finish<G, NW>(p, s, m.sh, m.ref, m.sum, b, first_head, n, m.merged, warp, lane);
+            merge_cluster<G>(p, m.merged, b, first_head, n, warp, lane);
+            return;
+        }
         float *part = nullptr;
         if (i0 > 0 || i1 < units) part = p.work + HEAD + (2 * (int64_t)blockIdx.x + (base + row * units >= second)) * PART<G>;
         finish<G, NW>(p, s, m.sh, m.ref, m.sum, b, first_head, n, part, warp, lane);
@@ -764,20 +838,20 @@ static int64_t workspace_floats(int head_dim) {
     return HEAD + 2 * part * most_blocks(4);
 }
 
-template <int G, bool FINE, int NW> static int launch_decode(const DecodeParams &p, int64_t blocks, cudaStream_t st) {
+template <int G, bool FINE, int NW, bool CLUSTER> static int launch_decode(const DecodeParams &p, int64_t blocks, int cluster, cudaStream_t st) {
     static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may take its shared memory
     int dev = 0;
     if (int rc = current_device(&dev)) return rc;
     if (!(allowed.load(std::memory_order_acquire) >> dev & 1)) {
-        OMMX_CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<G, FINE, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Memory<G, NW>)));
+        OMMX_CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<G, FINE, NW, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Memory<G, NW>)));
         allowed.fetch_or(1ull << dev, std::memory_order_release);
     }
-    if (int rc = launch_dependent(kv4_decode_kernel<G, FINE, NW>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G, NW>), st, p)) return rc;
-    if (p.whole) return 0;
+    if (int rc = launch_dependent(kv4_decode_kernel<G, FINE, NW, CLUSTER>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G, NW>), st, cluster, p)) return rc;
+    if (p.whole || CLUSTER) return 0;
     // a row has some blocks / rows parts
     const int rows = p.c.H * p.col_blocks;
-    if ((int64_t)rows * p.s.B * COLS >= blocks) return launch_dependent(kv4_combine_row_kernel<G>, dim3(rows, p.s.B), 32 * COLS, 0, st, p);
-    return launch_dependent(kv4_combine_head_kernel<G>, dim3(rows * COLS, p.s.B), 32 * CW, 0, st, p);
+    if ((int64_t)rows * p.s.B * COLS >= blocks) return launch_dependent(kv4_combine_row_kernel<G>, dim3(rows, p.s.B), 32 * COLS, 0, st, 1, p);
+    return launch_dependent(kv4_combine_head_kernel<G>, dim3(rows * COLS, p.s.B), 32 * CW, 0, st, 1, p);
 }
 
 // records that a row of the call can have
@@ -831,11 +905,17 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     p.least = 2 * warps;
     p.whole = units <= WHOLE;
     const int64_t most = (units * rows + p.least - 1) / p.least, hold = most_blocks(warps);
-    const int64_t blocks = p.whole ? rows : most < 1 ? 1 : most < hold ? most : hold;
+    // Rows of middling length, and few, go to a cluster of eight-warp blocks each, as many as fit at once: no second kernel
+    // (4096 tokens, 8 kv heads: 10.4 us with two, 8.3 with clusters; past 256 records the blocks that stay idle cost more)
+    int cluster = 1;
+    while (!p.whole && cluster < MOST_CLUSTER && 2 * cluster * rows <= most_blocks(8)) cluster *= 2;
+    if (units > 32 * cluster) cluster = 1;
+    const int64_t blocks = p.whole ? rows : cluster > 1 ? cluster * rows : most < 1 ? 1 : most < hold ? most : hold;
     auto launch = [&](auto g, auto fine) {
         constexpr int G = decltype(g)::value;
         constexpr bool FINE = decltype(fine)::value;
-        return warps == 4 ? launch_decode<G, FINE, 4>(p, blocks, st) : launch_decode<G, FINE, 8>(p, blocks, st);
+        if (cluster > 1) return launch_decode<G, FINE, 8, true>(p, blocks, cluster, st);
+        return warps == 4 ? launch_decode<G, FINE, 4, false>(p, blocks, 1, st) : launch_decode<G, FINE, 8, false>(p, blocks, 1, st);
     };
     using std::integral_constant;
     if (a->o_dtype == OMMX_DT_BF16)

@@ -353,11 +353,11 @@ static int select(const ommx_kv4_select_args *a, cudaStream_t st) {
         const int64_t fill = (2LL * sm_count() + rows - 1) / rows;          // two blocks to an SM, which is what it holds
         const size_t smem = (size_t)p.col_blocks * (a->cache.head_dim * 16 + 32) + 16;
         const dim3 grid((unsigned)(most < fill ? most : fill), p.c.H, p.s.B);
-        const int rc = a->cache.head_dim == 64 ? launch_dependent(kv4_score_kernel<2>, grid, 32 * SCORE_WARPS, smem, st, p)
-                                               : launch_dependent(kv4_score_kernel<4>, grid, 32 * SCORE_WARPS, smem, st, p);
+        const int rc = a->cache.head_dim == 64 ? launch_dependent(kv4_score_kernel<2>, grid, 32 * SCORE_WARPS, smem, st, 1, p)
+                                               : launch_dependent(kv4_score_kernel<4>, grid, 32 * SCORE_WARPS, smem, st, 1, p);
         if (rc) return rc;
     }
-    return launch_dependent(kv4_pick_kernel, dim3(p.c.H, p.s.B), PICK_THREADS, 0, st, p);
+    return launch_dependent(kv4_pick_kernel, dim3(p.c.H, p.s.B), PICK_THREADS, 0, st, 1, p);
 }
 
 }  // namespace kv4

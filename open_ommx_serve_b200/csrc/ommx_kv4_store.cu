@@ -495,7 +495,7 @@ static int append(const ommx_kv4_append_args *a, cudaStream_t st) {
     const int bytes = a->dtype == OMMX_DT_F32 ? 4 : 2;
     const bool wide = aligned16(a->k_new, p.k_t, p.k_h, bytes) && aligned16(a->v_new, p.v_t, p.v_h, bytes) &&
                       (!a->q || (aligned16(a->q, p.q_t, p.q_h, bytes) && aligned16(a->q_out, p.o_t, p.o_h, bytes)));
-    return launch_dependent(KV4_PICK(kv4_append_kernel, a->dtype, G, wide), dim3((unsigned)(runs * p.blocks)), 32 * WARPS, 0, st, p);
+    return launch_dependent(KV4_PICK(kv4_append_kernel, a->dtype, G, wide), dim3((unsigned)(runs * p.blocks)), 32 * WARPS, 0, st, 1, p);
 }
 
 static int gather(const ommx_kv4_gather_args *a, cudaStream_t st) {
@@ -517,7 +517,7 @@ static int gather(const ommx_kv4_gather_args *a, cudaStream_t st) {
     const int bytes = a->dtype == OMMX_DT_F32 ? 4 : 2;
     const bool wide = aligned16(a->k, p.k_t, p.k_h, bytes) && aligned16(a->v, p.v_t, p.v_h, bytes);
     const int64_t runs = most_runs(a->num_rows, p.s.B, 16, a->row_start == nullptr);
-    return launch_dependent(KV4_PICK(kv4_gather_kernel, a->dtype, a->cache.head_dim / 32, wide), dim3((unsigned)runs), 32 * WARPS, 0, st, p);
+    return launch_dependent(KV4_PICK(kv4_gather_kernel, a->dtype, a->cache.head_dim / 32, wide), dim3((unsigned)runs), 32 * WARPS, 0, st, 1, p);
 }
 
 }  // namespace kv4
