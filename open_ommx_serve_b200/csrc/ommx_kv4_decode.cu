@@ -5,8 +5,7 @@
 //   q.K_t = sum_j s_tj (sum_c q_c a_tc) + z_tj (sum_c q_c),      o_c = sum_t (p_t s_tj) a_tc + sum_t p_t z_tj:
 // the codes go into the tensor cores as they are. A nibble masked in place is the fp16 subnormal code * 2^-24 (or 2^-20), exact and
 // one LOP3 for two of them; the tokens (of K) and channels (of V) are the rows of an m16n8k16 product and up to eight query heads
-// that share the kv head its columns. Of V, one row takes two nibbles as they lie, lower + 16 upper, and another the upper one
-// alone: their difference is the lower one's, a mask saved. Scales meet the sums of K's groups behind the product and the weights of V before it, zeros
+// that share the kv head its columns. Scales meet the sums of K's groups behind the product and the weights of V before it, zeros
 // are fp32 multiply-adds. Queries keep all their bits: a head's are scaled by a power of two into fp16's range.
 //
 // Weights p_t s_tj are rounded to fp16 (2^-12 of each, of either sign): against the running reference r, which covers the logit and
@@ -21,8 +20,8 @@ namespace ommx {
 namespace kv4 {
 
 constexpr int WARPS_PER_SM = 16;                  // as many as the registers hold; a block is NW of them, each with records of its own
-constexpr int STAGES = 4, AHEAD = STAGES - 1;     // records that a warp holds, and those of them on their way
-constexpr int FULL = 0x101010;                    // sixteen tokens in each of those
+constexpr int STAGES = 3, AHEAD = STAGES - 1;     // records that a warp holds, and those of them on their way
+constexpr int FULL = 0x1010;                      // sixteen tokens in each of those
 constexpr int COLS = 8;                           // query heads side by side
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float ROOM = 4096.0f;                   // how large a weight may get before its reference moves
@@ -222,13 +221,19 @@ __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int fir
     }
 }
 
-// A warp's running state. acc[j][u]: 2^-24 (channel 32 j + 4 g + 2 u, and 16 times the next one) in rows g, the latter alone in rows
-// g + 8; heads 2 t, 2 t + 1.
+// A warp's running state. acc[j][u]: 2^-24 channel 32 j + 4 g + 2 u (rows g), 2^-20 the next one (rows g + 8); heads 2 t, 2 t + 1.
+// The tensor cores cut what they add to a sum, so long sums of codes, none of them negative, fall short: by some 2^-26 of the sum a
+// record, which is much of an output that the zeros nearly cancel (8e-4 of it after 110 records of 64K tokens that weigh alike). So
+// `acc` is added to `whole` in shared memory every 64 records, every 32 where the output is finer than bf16 (2 % of the time).
 template <int G> struct State {
     float acc[G][2][4], zero[G][2], sum[2], ref[2];
+    float *whole;                                 // the lane's first of 8 G values, 32 apart
+    bool some;                                    // there is something there
 };
 
-template <int G> __device__ __forceinline__ void clear(State<G> &s) {
+template <int G> __device__ __forceinline__ void clear(State<G> &s, float *whole) {
+    s.whole = whole;
+    s.some = false;
 #pragma unroll
     for (int j = 0; j < G; ++j) {
 #pragma unroll
@@ -248,6 +253,23 @@ template <int G> __device__ __forceinline__ void rescale(State<G> &s, float f0, 
         s.zero[j][0] *= f0; s.zero[j][1] *= f1;
     }
     s.sum[0] *= f0; s.sum[1] *= f1;
+    if (s.some)
+#pragma unroll
+        for (int i = 0; i < 8 * G; ++i) s.whole[32 * i] *= i & 1 ? f1 : f0;
+}
+template <int G> __device__ __forceinline__ void put_by(State<G> &s) {      // acc to `whole`
+#pragma unroll
+    for (int i = 0; i < 8 * G; ++i) {
+        float &a = s.acc[i / 8][i / 4 % 2][i % 4];
+        s.whole[32 * i] = s.some ? s.whole[32 * i] + a : a;
+        a = 0.0f;
+    }
+    s.some = true;
+}
+template <int G> __device__ __forceinline__ void take_back(State<G> &s) {
+    if (s.some)
+#pragma unroll
+        for (int i = 0; i < 8 * G; ++i) s.acc[i / 8][i / 4 % 2][i % 4] += s.whole[32 * i];
 }
 
 // ---- a warp's ring of records: 16 bytes a lane at a time, a group of copies for each record ----
@@ -359,16 +381,15 @@ template <int G, bool FINE> __device__ __forceinline__ void attend(const DecodeP
         s.zero[j][1] = fmaf(z1, w[3], fmaf(z0, w[1], s.zero[j][1]));
         const float y[4] = {w[0] * s0, w[1] * s0, w[2] * s1, w[3] * s1};
         const uint32_t h0 = half2_bits(y[0], y[1]), h1 = half2_bits(y[2], y[3]);
-        // bytes 0, 2 and 1, 3 in half words of their own
-        const uint32_t a = v0[j] & 0x00FF00FFu, b = v1[j] & 0x00FF00FFu, c = __byte_perm(v0[j], 0, 0x4341), d = __byte_perm(v1[j], 0, 0x4341);
+        const uint32_t a = v0[j] >> 8, b = v1[j] >> 8;
         const uint32_t b0 = transpose8x8(h0), b1 = transpose8x8(h1);
-        mma(s.acc[j][0], a, a & HI, b, b & HI, b0, b1);
-        mma(s.acc[j][1], c, c & HI, d, d & HI, b0, b1);
+        mma(s.acc[j][0], v0[j] & LO, v0[j] & HI, v1[j] & LO, v1[j] & HI, b0, b1);
+        mma(s.acc[j][1], a & LO, a & HI, b & LO, b & HI, b0, b1);
         if constexpr (FINE) {
             const float2 r0 = half2_floats(h0), r1 = half2_floats(h1);
             const uint32_t d0 = transpose8x8(half2_bits(y[0] - r0.x, y[1] - r0.y)), d1 = transpose8x8(half2_bits(y[2] - r1.x, y[3] - r1.y));
-            mma(s.acc[j][0], a, a & HI, b, b & HI, d0, d1);
-            mma(s.acc[j][1], c, c & HI, d, d & HI, d0, d1);
+            mma(s.acc[j][0], v0[j] & LO, v0[j] & HI, v1[j] & LO, v1[j] & HI, d0, d1);
+            mma(s.acc[j][1], a & LO, a & HI, b & LO, b & HI, d0, d1);
         }
     }
 }
@@ -423,8 +444,8 @@ __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Share
         for (int i = 0; i < 2; ++i) {
             float *to = &sh.o[warp][2 * t + i][32 * j + 4 * g];
             const float z = s.zero[j][i];
-            *reinterpret_cast<float4 *>(to) = make_float4(f[i] * fmaf(s.acc[j][0][i] - s.acc[j][0][i + 2], 0x1p24f, z), f[i] * fmaf(s.acc[j][0][i + 2], 0x1p20f, z),
-                                                          f[i] * fmaf(s.acc[j][1][i] - s.acc[j][1][i + 2], 0x1p24f, z), f[i] * fmaf(s.acc[j][1][i + 2], 0x1p20f, z));
+            *reinterpret_cast<float4 *>(to) = make_float4(f[i] * fmaf(s.acc[j][0][i], 0x1p24f, z), f[i] * fmaf(s.acc[j][0][i + 2], 0x1p20f, z),
+                                                          f[i] * fmaf(s.acc[j][1][i], 0x1p24f, z), f[i] * fmaf(s.acc[j][1][i + 2], 0x1p20f, z));
         }
     __syncthreads();
     for (int h = warp; h < COLS; h += NW) {
@@ -461,6 +482,7 @@ template <int G, int NW> struct Memory {
         Shared<G, NW> sh;
         uint8_t ring[NW][STAGES][Rec<G>::BYTES];
     };
+    float whole[NW][8 * G][32];
     QueryMemory<G> query;
     float ref[COLS][NW], sum[COLS][NW];
     alignas(16) float merged[PART<G>];            // of this block, where a cluster shares a row
@@ -533,6 +555,7 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv4_decode_kernel(
     extern __shared__ __align__(128) uint8_t memory[];
     Memory<G, NW> &m = *reinterpret_cast<Memory<G, NW> *>(memory);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int BY = FINE ? 32 : 64;            // records to a partial sum
     const uint8_t *ring = m.ring[warp][0];
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + 16 * lane;
     const uint8_t *records = p.c.records + 16 * lane;
@@ -632,8 +655,9 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv4_decode_kernel(
         Query<G> q;
         State<G> s;
         load_query<G>(p, b, first_head, n, warp, lane, m.query, q);
-        clear(s);
+        clear(s, m.whole[warp][0] + lane);
         for (int k0 = 0; k0 < mine; k0 += 32) {
+            if (k0 % BY == 0 && k0) put_by(s);
             rec = next_rec;
             valid = next_valid;
             look_up(k0 + 32 + AHEAD, next_rec, next_valid);
@@ -660,6 +684,7 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv4_decode_kernel(
             }
         }
         fetched<0>();
+        take_back(s);
         if constexpr (CLUSTER) {
             finish<G, NW>(p, s, m.sh, m.ref, m.sum, b, first_head, n, m.merged, warp, lane);
             merge_cluster<G>(p, m.merged, b, first_head, n, warp, lane);

@@ -553,3 +553,23 @@ def test_row_starts_out_of_order_stay_inside():
         assert torch.equal(cache["records"][spare], before[spare])
         ko = torch.full((4, H, D), 2.0, device=DEV)
         ommx_kv4_gather(cache["records"], table, length, ko, ko.clone(), row_start=torch.tensor(start, dtype=torch.int32, device=DEV))
+
+
+@pytest.mark.parametrize("dtype,allowed", [(torch.bfloat16, 2.0 ** -9), (torch.float32, 0.0)])
+def test_long_even_sums_keep_their_bits(dtype, allowed):
+    """130 thousand tokens that weigh alike: the output is what is left of codes and zeros that nearly cancel, so what a sum of hundreds
+    of products loses would show.  Of a value's error a weight's rounding gives 2^-12 of its group's range R at most, of either sign:
+    averaged over N tokens 2^-12 R / sqrt(N).  A sum that is cut by up to half a step in 2^23 at each of 64 additions (bf16 output;
+    32 else, where weights have 22 bits) is off by 2^-18 (2^-19) of itself, 15 scales <= R.  Both are doubled for the tail; outputs of bf16
+    are rounded by 2^-9 of themselves."""
+    n, D = 131072, 128
+    cache, table, length = filled([n], 1, D, 64, seed=101)
+    q = torch.zeros(1, 4, D, dtype=torch.bfloat16, device=DEV)
+    o, lse = torch.empty(1, 4, D, dtype=dtype, device=DEV), torch.empty(1, 4, device=DEV)
+    ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse)
+    k, v = ref.sequence(cache["records"], table[0], n)
+    want = v.mean(1)                                                        # [1, D]
+    R = float((v.unflatten(-1, (-1, 32)).amax(-1) - v.unflatten(-1, (-1, 32)).amin(-1)).max())
+    off = 2 * (2.0 ** -12 * R / math.sqrt(n) + 2.0 ** -18 * R) if dtype == torch.bfloat16 else 2 * 2.0 ** -19 * R
+    assert float((o[0].double() - want).abs().max()) <= off + allowed * float(want.abs().max())
+    assert abs(float(lse[0, 0]) - math.log(n)) < 1e-4
