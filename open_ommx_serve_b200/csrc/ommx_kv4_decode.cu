@@ -254,8 +254,8 @@ template <int G> __device__ __forceinline__ void rescale(State<G> &s, float f0, 
     }
     s.sum[0] *= f0; s.sum[1] *= f1;
     if (s.some)
-#pragma unroll
-        for (int i = 0; i < 8 * G; ++i) s.whole[32 * i] *= i & 1 ? f1 : f0;
+#pragma unroll 1
+        for (int i = 0; i < 8 * G; i += 2) { s.whole[32 * i] *= f0; s.whole[32 * i + 32] *= f1; }
 }
 template <int G> __device__ __forceinline__ void put_by(State<G> &s) {      // acc to `whole`
 #pragma unroll
@@ -482,10 +482,13 @@ template <int G, int NW> struct Memory {
         Shared<G, NW> sh;
         uint8_t ring[NW][STAGES][Rec<G>::BYTES];
     };
-    float whole[NW][8 * G][32];
+    // two blocks (of four warps, four) have to stay below 196 KB: the first-level cache is halved past that, and 64K tokens took 1 us more
+    union {
+        float whole[NW][8 * G][32];
+        alignas(16) float merged[PART<G>];        // of this block, where a cluster shares a row; its warps have taken theirs back
+    };
     QueryMemory<G> query;
     float ref[COLS][NW], sum[COLS][NW];
-    alignas(16) float merged[PART<G>];            // of this block, where a cluster shares a row
 };
 
 // A row of no tokens
@@ -656,6 +659,9 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv4_decode_kernel(
         State<G> s;
         load_query<G>(p, b, first_head, n, warp, lane, m.query, q);
         clear(s, m.whole[warp][0] + lane);
+        // the slot in use and the one that is filled next, which is the one used before
+        int read = 0, write = AHEAD * Rec<G>::BYTES;
+        auto advance = [&] { write = read; read = read == AHEAD * Rec<G>::BYTES ? 0 : read + Rec<G>::BYTES; };
         for (int k0 = 0; k0 < mine; k0 += 32) {
             if (k0 % BY == 0 && k0) put_by(s);
             rec = next_rec;
@@ -665,19 +671,21 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv4_decode_kernel(
             if (flying == FULL && __all_sync(~0u, valid == 16 || lane + AHEAD >= left)) {
                 for (int k = 0; k < now; ++k) {
                     if (k + AHEAD < left)
-                        fetch<G>(ring_at + (k + AHEAD) % STAGES * Rec<G>::BYTES, records + (uint64_t)__shfl_sync(~0u, rec, k) * Rec<G>::BYTES, lane);
+                        fetch<G>(ring_at + write, records + (uint64_t)__shfl_sync(~0u, rec, k) * Rec<G>::BYTES, lane);
                     close_group();
                     fetched<AHEAD>();
-                    attend<G, FINE>(p, ring + k % STAGES * Rec<G>::BYTES, 16, lane, q, s);
+                    attend<G, FINE>(p, ring + read, 16, lane, q, s);
+                    advance();
                     __syncwarp();                     // before the slot is filled again
                 }
             } else {
                 for (int k = 0; k < now; ++k) {
                     if (k + AHEAD < left)
-                        fetch<G>(ring_at + (k + AHEAD) % STAGES * Rec<G>::BYTES, records + (uint64_t)__shfl_sync(~0u, rec, k) * Rec<G>::BYTES, lane);
+                        fetch<G>(ring_at + write, records + (uint64_t)__shfl_sync(~0u, rec, k) * Rec<G>::BYTES, lane);
                     close_group();
                     fetched<AHEAD>();
-                    if (flying & 255) attend<G, FINE>(p, ring + k % STAGES * Rec<G>::BYTES, flying & 255, lane, q, s);
+                    if (flying & 255) attend<G, FINE>(p, ring + read, flying & 255, lane, q, s);
+                    advance();
                     flying = flying >> 8 | __shfl_sync(~0u, valid, k) << (8 * (AHEAD - 1));
                     __syncwarp();
                 }

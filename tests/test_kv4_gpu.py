@@ -573,3 +573,26 @@ def test_long_even_sums_keep_their_bits(dtype, allowed):
     off = 2 * (2.0 ** -12 * R / math.sqrt(n) + 2.0 ** -18 * R) if dtype == torch.bfloat16 else 2 * 2.0 ** -19 * R
     assert float((o[0].double() - want).abs().max()) <= off + allowed * float(want.abs().max())
     assert abs(float(lse[0, 0]) - math.log(n)) < 1e-4
+
+
+@pytest.mark.parametrize("D,page,B,n,od", [(128, 16, 64, 8101, torch.bfloat16), (64, 64, 100, 6007, torch.float32), (128, 32, 9, 65003, torch.float32)])
+def test_more_records_to_a_warp_than_it_looks_up_at_once(D, page, B, n, od):
+    """Sequences that share their pages (one prompt, many continuations): hundreds of records to a warp, several lookups, partial sums."""
+    H, Hq = 8, 16
+    cache, table, _ = filled([n], H, D, page, seed=111)
+    table = table.expand(B, -1).contiguous()
+    lens = [n - 37 * b for b in range(B)]
+    q = torch.randn(B, Hq, D, generator=torch.Generator().manual_seed(5)).bfloat16().to(DEV)
+    o, lse = torch.empty(B, Hq, D, dtype=od, device=DEV), torch.empty(B, Hq, device=DEV)
+    length = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse)
+    k, v = ref.sequence(cache["records"], table[0], n)
+    for b in range(0, B, 4):
+        wo, wl = ref.attention(q[b], list(k[:, :lens[b]]), list(v[:, :lens[b]]), D ** -0.5)
+        off, drift = bounds(q[b], k, v, D ** -0.5, od)
+        assert float((o[b].double() - wo).abs().max()) <= off, b
+        assert float((lse[b].double() - wl).abs().max()) <= drift + 2.0 ** -22 * float(wl.abs().max()), b
+    again, lse2 = torch.empty_like(o), torch.empty_like(lse)
+    for _ in range(3):
+        ommx_kv4_decode_attention(q, cache["records"], table, length, again, lse2)
+        assert torch.equal(o, again) and torch.equal(lse, lse2)
