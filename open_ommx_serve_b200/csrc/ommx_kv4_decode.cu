@@ -10,8 +10,13 @@
 //
 // Weights p_t s_tj are rounded to fp16 (2^-12 of each, of either sign): against the running reference r, which covers the logit and
 // the scale, they are 2^12 at most, and those below 2^-36 of the largest are lost. That is an eighth of a bf16 output's own
-// rounding; where the output is finer (fp16, fp32), a second product takes what the rounding left (FINE). Sums of weights and
-// zeros stay fp32.
+// rounding; where the output is finer (fp16, fp32), a second product takes what the rounding left (FINE: 32 ragged sequences 57 us
+// without, 64 with). Sums of weights and zeros stay fp32.
+//
+// What bounds it: a record's 160 bytes a token are read once, so HBM, and beside it the schedulers: a record is some 320 instructions
+// of a warp, 17 of them products that hold a scheduler 8 cycles, in which its multiply-adds wait. 8 x 64K tokens, 8 kv heads, 32
+// query heads: 136 us (4.9 TB/s, 75 % of the copy rate); 110 with the copies left out, 112 with the arithmetic left out. e4m3 products
+// for K (half the masks, twice the depth) were slower, 173: their operands are converted.
 #include <type_traits>
 
 #include "ommx_kv4.cuh"
@@ -273,8 +278,8 @@ template <int G> __device__ __forceinline__ void take_back(State<G> &s) {
 }
 
 // ---- a warp's ring of records: 16 bytes a lane at a time, a group of copies for each record ----
-// Bulk copies counted by mbarriers move the same bytes, but a record's barrier, wait and copy took a warp 90 cycles of a scheduler
-// against 25 of these (8 x 64K tokens, 8 kv heads: 144 us).
+// Bulk copies counted by mbarriers move the same bytes with fewer instructions, but a record's arrival, wait and copy held a scheduler
+// longer than five of these do (8 x 64K tokens, 8 kv heads: 146.6 us against 141.9 when both were tried).
 template <int G> __device__ __forceinline__ void fetch(uint32_t to, const uint8_t *rec, int lane) {   // both at the lane's 16 bytes
 #pragma unroll
     for (int i = 0; i < Rec<G>::BYTES; i += 512)

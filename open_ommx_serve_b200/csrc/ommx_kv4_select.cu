@@ -3,7 +3,8 @@
 // score(page) = max over the query heads of a kv head of  sum_c max(q_c M_c, q_c m_c) = q+ . M + q- . m  (M, m: the page's channel
 // maxima and minima, q+ and q-: q where it is above and below 0): no key of the page has a larger product with q. It is computed
 // in whole numbers, q in 8 bits and M, m in 7, on the tensor cores: exact in any order, so the choice repeats on every device and
-// however the work is cut. M and m are read once, 4 D bytes a page and kv head.
+// however the work is cut. M and m are read once, 4 D bytes a page and kv head: 8192 pages x 8 heads 7.4 us (4.5 TB/s), and as much
+// again to pick 256 of them, a block to a kv head, which is latency: lengths, keys, five rounds of the block.
 #include "ommx_kv4.cuh"
 
 namespace ommx {
