@@ -860,7 +860,7 @@ PyObject *py_kv4_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
     d.lse = (float *)lse->data_ptr(); d.lse_stride_b = lse->stride(0);
     d.sm_scale = (float)(a[6] == Py_None ? 1.0 / std::sqrt((double)D) : c.number(a[6], "sm_scale"));
     d.logit_cap = (float)c.number(a[7], "logit_cap");
-    KV4_EXPECT(c, d.logit_cap >= 0.0f, "logit_cap must not be negative");
+    KV4_EXPECT(c, d.logit_cap >= 0.0f && std::isfinite(d.logit_cap), "logit_cap must be finite and not negative");
     if (const Tensor *sel = c.tensor(a[8], "selected", false)) {
         KV4_EXPECT(c, sel->dim() == 3 && sel->scalar_type() == at::kInt && sel->is_contiguous() && sel->size(0) == B && sel->size(1) == H && sel->size(2) <= INT32_MAX,
                  "selected must be a contiguous int32 tensor [batch, kv heads, pages]");

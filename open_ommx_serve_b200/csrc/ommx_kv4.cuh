@@ -135,10 +135,12 @@ inline int read_cache(const char *who, const ommx_kv4_cache &c, Cache *to) {
     *to = {(uint8_t *)c.records, c.num_pages, c.n_kv_heads, c.page_size, c.page_size / 16};
     return 0;
 }
-inline int read_seqs(const char *who, const ommx_kv4_seqs &s, Seqs *to) {
+inline int read_seqs(const char *who, const ommx_kv4_seqs &s, const Cache &c, Seqs *to) {
     if (s.batch < 0 || s.pages_per_seq < 0) return fail(OMMX_E_ARG, "%s: batch and pages_per_seq must not be negative", who);
     if (s.batch && (!s.b_seq_len || (!s.page_table && s.pages_per_seq))) return fail(OMMX_E_ARG, "%s: b_seq_len and page_table must not be null", who);
-    *to = {s.b_seq_len, s.page_table, s.page_table_stride, s.table_is_int64, s.pages_per_seq, s.batch};
+    // places are counted in 32 bits, a page and more to spare
+    const int32_t most = 0x7FFFFC00 / c.page;
+    *to = {s.b_seq_len, s.page_table, s.page_table_stride, s.table_is_int64, s.pages_per_seq < most ? s.pages_per_seq : most, s.batch};
     return 0;
 }
 

@@ -17,6 +17,7 @@
 // of a warp, 17 of them products that hold a scheduler 8 cycles, in which its multiply-adds wait. 8 x 64K tokens, 8 kv heads, 32
 // query heads: 136 us (4.9 TB/s, 75 % of the copy rate); 110 with the copies left out, 112 with the arithmetic left out. e4m3 products
 // for K (half the masks, twice the depth) were slower, 173: their operands are converted.
+#include <cmath>
 #include <type_traits>
 
 #include "ommx_kv4.cuh"
@@ -59,6 +60,7 @@ struct DecodeParams {
 //   with seven such blocks of 296, 24.4 with none; 64 sequences of 200..2000 tokens: 43.3 with even shares, 38.3 with pieces).
 // A piece that is a whole row is finished where it is computed; the others' parts meet in the second kernel. A block has at most two
 // of those, of the row that an earlier block began (its slot 0) and of the one that a later block goes on with (slot 1).
+constexpr uint32_t OVER = 2;                      // in the deal's place: there is none
 constexpr int BEGIN = 64, HEAD = 4;               // HEAD: floats in front of the parts, which hold the deal
 __device__ __forceinline__ int pages_of(const DecodeParams &p, int len) { return (len + p.c.page - 1) >> p.page_shift; }
 __device__ __forceinline__ int length_of(const DecodeParams &p, int b) {
@@ -71,10 +73,11 @@ __device__ __forceinline__ int units_of(const DecodeParams &p, int len) {
     if (p.selected) return min(pages_of(p, len), p.num_selected) * p.c.parts;
     return (len + 15) >> 4;
 }
-struct Deal { uint32_t per, total; bool pieces; };   // the host refuses what 32 bits do not count
+struct Deal { uint32_t per, total; bool pieces, over; };   // over: lengths far past max_seq_len, of more units than 32 bits count
 __device__ __forceinline__ uint32_t pieces_of(uint32_t units, uint32_t per) { return (units + per - 1) / per; }
 __device__ __forceinline__ Deal deal(const DecodeParams &p, uint32_t rows, uint32_t blocks, int lane) {
-    uint32_t sum = 0, some = 0, most = 0;
+    uint64_t sum = 0;
+    uint32_t some = 0, most = 0;
     const uint32_t own = lane < p.s.B ? units_of(p, length_of(p, lane)) : 0;
     for (int b = lane; b < p.s.B; b += 32) {
         const uint32_t n = b == lane ? own : units_of(p, length_of(p, b));
@@ -83,13 +86,17 @@ __device__ __forceinline__ Deal deal(const DecodeParams &p, uint32_t rows, uint3
         most = max(most, n);
     }
     Deal d;
-    d.total = __reduce_add_sync(~0u, sum) * rows;
+#pragma unroll
+    for (int i = 16; i; i /= 2) sum += __shfl_xor_sync(~0u, sum, i);
+    d.over = sum * rows >> 31;
+    d.total = d.over ? 0 : (uint32_t)sum * rows;
     const uint32_t full = __reduce_add_sync(~0u, some) * rows;
     most = __reduce_max_sync(~0u, most);
     const uint32_t even = max((d.total + blocks - 1) / blocks, (uint32_t)p.least);
     d.per = even;
     d.pieces = false;
-    if (full == 0 || full > blocks) return d;
+    if (d.over) or_status(p.status, OMMX_ST_BAD_LENGTH);
+    if (d.over || full == 0 || full > blocks) return d;
     // pieces of `per` take total / per + full blocks at most; fewer may do
     uint32_t lo = even, hi = min(max(most, even), full < blocks ? max(even, d.total / (blocks - full) + 1) : 0xFFFFFFFFu);
 #pragma unroll 1
@@ -496,6 +503,11 @@ template <int G, int NW> struct Memory {
     float ref[COLS][NW], sum[COLS][NW];
 };
 
+__device__ __forceinline__ bool too_many(const DecodeParams &p, uint32_t units, uint32_t rows) {
+    const bool over = (uint64_t)units * rows >> 31;
+    if (over) or_status(p.status, OMMX_ST_BAD_LENGTH);
+    return over;
+}
 // A row of no tokens
 template <int G> __device__ __forceinline__ void nothing(const DecodeParams &p, int b, int row) {
     const int cb = row % p.col_blocks, first = (row / p.col_blocks) * p.group + cb * COLS, n = min(COLS, p.group - cb * COLS);
@@ -578,6 +590,7 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv4_decode_kernel(
         b = at / rows;
         len = length_of(p, b);
         units = units_of(p, len);
+        if (too_many(p, units, rows)) units = 0;
         if (units == 0) {                         // for all of the cluster
             if (rank == 0) nothing<G>(p, b, at - b * rows);
             return;
@@ -589,12 +602,13 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv4_decode_kernel(
         b = blockIdx.x / rows;
         len = length_of(p, b);
         units = units_of(p, len);
+        if (too_many(p, units, rows)) units = 0;
         u = (blockIdx.x - b * rows) * units;
         end = u + units;
         if (units == 0) { nothing<G>(p, b, blockIdx.x - b * rows); return; }
     } else {
         const Deal d = deal(p, rows, gridDim.x, lane);
-        if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<uint2 *>(p.work) = make_uint2(d.per, d.pieces);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<uint2 *>(p.work) = make_uint2(d.per, d.over ? OVER : d.pieces);
         // the sequence that this block's (first) unit lies in; `at`, `base`: this block and the first of the sequence, in pieces or units
         const uint32_t at = d.pieces ? blockIdx.x : blockIdx.x * d.per;
         if (!d.pieces && at >= d.total) return;
@@ -725,7 +739,7 @@ __device__ __forceinline__ Parts parts_of(const DecodeParams &p, int b, uint32_t
     }
     before = __reduce_add_sync(~0u, before) * rows;
     Parts r;
-    if (units == 0) return {0, 0, false};
+    if (units == 0 || d.y == OVER) return {0, 0, false};
     if (d.y) {
         r.count = pieces_of(units, d.x);
         r.first = before + row * r.count;
@@ -907,12 +921,12 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     DecodeParams p;
     memset(&p, 0, sizeof(p));
     if (int rc = read_cache("kv4_decode", a->cache, &p.c)) return rc;
-    if (int rc = read_seqs("kv4_decode", a->seqs, &p.s)) return rc;
+    if (int rc = read_seqs("kv4_decode", a->seqs, p.c, &p.s)) return rc;
     if (a->q_dtype != OMMX_DT_BF16 && a->q_dtype != OMMX_DT_F16) return fail(OMMX_E_UNSUPPORTED, "kv4_decode: q must be bfloat16 or float16");
     if (a->o_dtype != OMMX_DT_F32 && a->o_dtype != OMMX_DT_BF16 && a->o_dtype != OMMX_DT_F16) return fail(OMMX_E_ARG, "kv4_decode: o dtype %d", a->o_dtype);
     if (a->n_q_heads < p.c.H || a->n_q_heads % p.c.H)
         return fail(OMMX_E_UNSUPPORTED, "kv4_decode: %d query heads are not a multiple of %d kv heads", a->n_q_heads, p.c.H);
-    if (!(a->logit_cap >= 0.0f)) return fail(OMMX_E_ARG, "kv4_decode: logit_cap must not be negative");
+    if (!(a->logit_cap >= 0.0f) || !std::isfinite(a->logit_cap)) return fail(OMMX_E_ARG, "kv4_decode: logit_cap must be finite and not negative");
     if (a->selected && a->num_selected < 0) return fail(OMMX_E_ARG, "kv4_decode: num_selected must not be negative");
     if (p.s.B > 65535) return fail(OMMX_E_UNSUPPORTED, "kv4_decode: a batch of %d", p.s.B);
     if (p.s.B == 0) return 0;

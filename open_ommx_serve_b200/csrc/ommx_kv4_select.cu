@@ -326,7 +326,7 @@ static int select(const ommx_kv4_select_args *a, cudaStream_t st) {
     SelectParams p;
     memset(&p, 0, sizeof(p));
     if (int rc = read_cache("kv4_select", a->cache, &p.c)) return rc;
-    if (int rc = read_seqs("kv4_select", a->seqs, &p.s)) return rc;
+    if (int rc = read_seqs("kv4_select", a->seqs, p.c, &p.s)) return rc;
     if (a->q_dtype != OMMX_DT_BF16 && a->q_dtype != OMMX_DT_F16) return fail(OMMX_E_UNSUPPORTED, "kv4_select: q must be bfloat16 or float16");
     if (a->n_q_heads < p.c.H || a->n_q_heads % p.c.H)
         return fail(OMMX_E_UNSUPPORTED, "kv4_select: %d query heads are not a multiple of %d kv heads", a->n_q_heads, p.c.H);

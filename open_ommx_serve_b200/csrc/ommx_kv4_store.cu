@@ -454,7 +454,7 @@ static int append(const ommx_kv4_append_args *a, cudaStream_t st) {
     AppendParams p;
     memset(&p, 0, sizeof(p));
     if (int rc = read_cache("kv4_append", a->cache, &p.c)) return rc;
-    if (int rc = read_seqs("kv4_append", a->seqs, &p.s)) return rc;
+    if (int rc = read_seqs("kv4_append", a->seqs, p.c, &p.s)) return rc;
     if (a->num_rows < 0) return fail(OMMX_E_ARG, "kv4_append: num_rows must not be negative");
     if (!known_dtype(a->dtype)) return fail(OMMX_E_ARG, "kv4_append: dtype %d is none of float32, bfloat16, float16", a->dtype);
     if (p.s.B == 0 || a->num_rows == 0) return 0;
@@ -505,7 +505,7 @@ static int gather(const ommx_kv4_gather_args *a, cudaStream_t st) {
     GatherParams p;
     memset(&p, 0, sizeof(p));
     if (int rc = read_cache("kv4_gather", a->cache, &p.c)) return rc;
-    if (int rc = read_seqs("kv4_gather", a->seqs, &p.s)) return rc;
+    if (int rc = read_seqs("kv4_gather", a->seqs, p.c, &p.s)) return rc;
     if (a->num_rows < 0) return fail(OMMX_E_ARG, "kv4_gather: num_rows must not be negative");
     if (!known_dtype(a->dtype)) return fail(OMMX_E_ARG, "kv4_gather: dtype %d is none of float32, bfloat16, float16", a->dtype);
     if (p.s.B == 0 || a->num_rows == 0) return 0;

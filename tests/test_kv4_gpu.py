@@ -596,3 +596,59 @@ def test_more_records_to_a_warp_than_it_looks_up_at_once(D, page, B, n, od):
     for _ in range(3):
         ommx_kv4_decode_attention(q, cache["records"], table, length, again, lse2)
         assert torch.equal(o, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("H,width", [(8, 30), (8, 250), (2, 250), (16, 2000)])
+def test_a_captured_call_follows_its_lengths(H, width):
+    """One graph, replayed with other lengths, past `max_seq_len` too: whole rows, clusters, and rows shared by two kernels."""
+    D, page, B, Hq = 128, 16, 3, 16
+    cache, table, _ = filled([width * page], H, D, page, seed=121)
+    table = table[:, :width].expand(B, -1).contiguous()
+    q = torch.randn(B, Hq, D, generator=torch.Generator().manual_seed(6)).bfloat16().to(DEV)
+    o, lse = torch.empty(B, Hq, D, device=DEV), torch.empty(B, Hq, device=DEV)
+    length = torch.tensor([1, 2, 3], dtype=torch.int32, device=DEV)
+    work = torch.empty(kv4_workspace_floats(D), device=DEV)
+    for most in (None, 40):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse, workspace=work, max_seq_len=most)
+        for lens in ([0, 0, 0], [width * page, 1, 0], [17, width * page // 2 + 3, 100], [width * page] * 3):
+            length.copy_(torch.tensor(lens, dtype=torch.int32))
+            o.fill_(7), lse.fill_(7)
+            graph.replay()
+            check_attention(cache, table, lens, q, o, lse)
+
+
+def test_calls_behind_one_another_on_their_own_stream():
+    """Selection, attention and an append of other rows back to back, each begun while the one before still runs: nothing is read early."""
+    lens, H, D, page = [3000, 1234], 4, 128, 32
+    cache, table, length = filled(lens, H, D, page, seed=131)
+    gen = torch.Generator().manual_seed(7)
+    table = torch.cat((table, table[:, -1:]), 1)
+    steps = [torch.randn(2, 8 + 2 * H, D, generator=gen).bfloat16().to(DEV) for _ in range(12)]
+    cos, sin = (x.to(DEV) for x in angles(4000, D))
+
+    def run(wait):
+        c = {k: v.clone() for k, v in cache.items()}
+        n, out = length.clone(), []
+        for x in steps:
+            q, sel = torch.empty(2, 8, D, dtype=torch.bfloat16, device=DEV), torch.empty(2, H, 9, dtype=torch.int32, device=DEV)
+            o, lse = torch.empty(2, 8, D, device=DEV), torch.empty(2, 8, device=DEV)
+            for call in (lambda: n.add_(1),
+                         lambda: ommx_kv4_append(x[:, 8:8 + H], x[:, 8 + H:], c["records"], table, n, q=x[:, :8], q_out=q, cos=cos, sin=sin, summary=c["summary"]),
+                         lambda: ommx_kv4_select_pages(q, c["summary"], table, n, sel, page_size=page),
+                         lambda: ommx_kv4_decode_attention(q, c["records"], table, n, o, lse, selected=sel),
+                         lambda: ommx_kv4_decode_attention(q, c["records"], table, n, o[:, :], lse, selected=sel, max_seq_len=1)):
+                call()
+                if wait:
+                    torch.cuda.synchronize()
+            out += [q, sel, o, lse]
+        return [c["records"], c["summary"]] + out
+
+    slow = run(True)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        fast = run(False)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(slow, fast))

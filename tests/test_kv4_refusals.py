@@ -92,7 +92,7 @@ def test_decode_refuses(change, error, text):
 
 
 @pytest.mark.parametrize("more,text", [
-    (dict(logit_cap=-1.0), "logit_cap"), (dict(logit_cap=float("nan")), "logit_cap"), (dict(selected=torch.zeros(B, H, 3)), "selected"),
+    (dict(logit_cap=-1.0), "logit_cap"), (dict(logit_cap=float("nan")), "logit_cap"), (dict(logit_cap=float("inf")), "logit_cap"), (dict(selected=torch.zeros(B, H, 3)), "selected"),
     (dict(selected=torch.zeros(B, H + 1, 3, dtype=torch.int32)), "selected"), (dict(selected=torch.zeros(B, H, 0, dtype=torch.int32)), "selected"),
     (dict(max_seq_len=-1), "max_seq_len"), (dict(max_seq_len=1 << 40), "max_seq_len")])
 def test_decode_refuses_options(more, text):
