@@ -387,9 +387,10 @@ struct GatherParams {
     int32_t *status;
 };
 
-// Grid: runs of rows that share a record of 16 tokens; a warp to a head of it.
+// Grid: runs of rows that share a record of 16 tokens; a warp to a head of it (up to GATHER_WARPS at once).
+constexpr int GATHER_WARPS = 8;
 template <typename T, int G, bool WIDE>
-__global__ void __launch_bounds__(32 * WARPS) kv4_gather_kernel(const __grid_constant__ GatherParams p) {
+__global__ void __launch_bounds__(32 * GATHER_WARPS) kv4_gather_kernel(const __grid_constant__ GatherParams p) {
     using W = typename Words<G>::T;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     wait_earlier();
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv4_gather_kernel(const __grid_con
     const int64_t id = page_id(p.s, run.b, at);
     if (id < 0 || id >= p.c.num_pages) { or_status(p.status, OMMX_ST_BAD_PAGE); return; }
     const int tau0 = run.p0 & 15, n = run.p1 - run.p0;
-    for (int head = warp; head < p.c.H; head += WARPS) {
+    for (int head = warp; head < p.c.H; head += blockDim.x / 32) {
         const uint8_t *rec = p.c.records + ((id * p.c.H + head) * p.c.parts + part) * Rec<G>::BYTES;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -519,7 +520,10 @@ static int gather(const ommx_kv4_gather_args *a, cudaStream_t st) {
     const int bytes = a->dtype == OMMX_DT_F32 ? 4 : 2;
     const bool wide = aligned16(a->k, p.k_t, p.k_h, bytes) && aligned16(a->v, p.v_t, p.v_h, bytes);
     const int64_t runs = most_runs(a->num_rows, p.s.B, 16, a->row_start == nullptr);
-    return launch_dependent(KV4_PICK(kv4_gather_kernel, a->dtype, a->cache.head_dim / 32, wide), dim3((unsigned)runs), 32 * WARPS, 0, st, 1, p);
+    // a warp to each head where a wave of blocks takes all (one row of 8 heads: 2.8 us, 3.9 with four warps), four warps where there
+    // are several, which then overlap (64K tokens, D = 64: 34.8 us, 37.9 with eight)
+    const int warps = runs < 4LL * sm_count() ? GATHER_WARPS : GATHER_WARPS / 2;
+    return launch_dependent(KV4_PICK(kv4_gather_kernel, a->dtype, a->cache.head_dim / 32, wide), dim3((unsigned)runs), 32 * (p.c.H < warps ? p.c.H : warps), 0, st, 1, p);
 }
 
 }  // namespace kv4
