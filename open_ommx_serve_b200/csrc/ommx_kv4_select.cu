@@ -227,9 +227,12 @@ __global__ void __launch_bounds__(PICK_THREADS) kv4_pick_kernel(const __grid_con
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
     if (tid == 0) { low = ~0u; high = 0; listed = 0; }
     histogram[tid] = histogram[tid + PICK_THREADS] = 0;
+    // behind the scores' kernel the lengths are there before the wait: this one starts when all its blocks have waited for what came earlier
+    const bool scored = p.s.max_pages > p.n;
+    int pages = scored ? pages_of(p, b) : 0;
     wait_earlier();
     let_next_in();
-    const int pages = pages_of(p, b);
+    if (!scored) pages = pages_of(p, b);
     int32_t *out = p.selected + ((int64_t)b * p.c.H + h) * p.n;
     if (pages <= p.n) {
         for (int i = tid; i < p.n; i += PICK_THREADS) out[i] = i < pages ? i : -1;
