@@ -177,8 +177,8 @@ constexpr uint32_t NOTHING = 0xFF80FF80u;                                  // -i
 
 // One warp appends up to 16 rows that share a record, ROWS of them at a time: lane ((row, j), t) has channels 32 j + 8 t + 0..7, so a
 // group's extremes meet in two shuffles. A key's partners in the rotation are loaded too (from the first-level cache), not exchanged.
-// Bounds: a row of K and V is 512 bytes in and 160 out at D = 128, some 300 instructions of a warp, and two rows' latency at a time:
-// 8192 rows x 8 heads take 25 us where their bytes take 7, one row 4.1. Eight rows at a time with all groups to a lane (127 registers)
+// Bounds: a row of K and V is 512 bytes in and 160 out at D = 128, and some 285 instructions of a warp: 8192 rows x 8 heads take 25 us
+// (64 % of the issue slots) where their bytes take 7, one row 4.0. Eight rows at a time with all groups to a lane (127 registers)
 // took 22, and 7.0 for one row; the next rows' loads ahead of these rows' work 25.5 (96 registers, fewer warps).
 template <typename T, int G, bool WIDE>
 __device__ __forceinline__ void append_part(const AppendParams &p, uint8_t *rec, int head, int first_row, int first_pos, int tau0, int n,
