@@ -177,7 +177,7 @@ constexpr uint32_t NOTHING = 0xFF80FF80u;                                  // -i
 
 // One warp appends up to 16 rows that share a record, ROWS of them at a time: lane ((row, j), t) has channels 32 j + 8 t + 0..7, so a
 // group's extremes meet in two shuffles. A key's partners in the rotation are loaded too (from the first-level cache), not exchanged.
-// Bounds: a row of K and V is 512 bytes in and 160 out at D = 128, and some 285 instructions of a warp: 8192 rows x 8 heads take 25 us
+// Bounds: a row of K and V is 512 bytes in and 160 out at D = 128, and some 285 instructions of a warp: 8192 rows x 8 heads take 24 us
 // (64 % of the issue slots) where their bytes take 7, one row 4.0. Eight rows at a time with all groups to a lane (127 registers)
 // took 22, and 7.0 for one row; the next rows' loads ahead of these rows' work 25.5 (96 registers, fewer warps).
 template <typename T, int G, bool WIDE>
@@ -193,6 +193,12 @@ __device__ __forceinline__ void append_part(const AppendParams &p, uint8_t *rec,
     const T *k = reinterpret_cast<const T *>(p.k) + (int64_t)(first_row + tau - tau0) * p.k_t + (int64_t)head * p.k_h + c;
     const T *v = reinterpret_cast<const T *>(p.v) + (int64_t)(first_row + tau - tau0) * p.v_t + (int64_t)head * p.v_h + c;
     const int64_t k_step = ROWS * p.k_t, v_step = ROWS * p.v_t;
+    uint32_t *words = reinterpret_cast<uint32_t *>(rec) + (tau * 4 + t) * G + j;         // of the lane's token
+    uint32_t *params = reinterpret_cast<uint32_t *>(rec + Rec<G>::KP) + tau * G + j;
+    uint8_t *const quads = rec + Rec<G>::V + 4 * (G * 8 * t + j);
+    const bool summary = p.summary, placed = !p.positions;
+    // places in their sequences are rotation positions, all of them in the tables: nothing to look at row by row
+    const bool sure = !p.rot || (placed && first_pos + n <= p.num_positions);
     auto fetch = [&] {
         if (tau >= tau0 && tau < tau0 + n) {
             fetch8<T, WIDE>(k, kk);
@@ -206,24 +212,26 @@ __device__ __forceinline__ void append_part(const AppendParams &p, uint8_t *rec,
     for (int last = tau0 + n - 1, base = tau0 / ROWS * ROWS; base <= last; base += ROWS) {
         const int here = tau, i = here - tau0;
         bool on = i >= 0 && i < n;
-        const int at = on ? rope_row(p, first_row + i, first_pos + i) : 0;
-        on = on && at >= 0;
+        int at = first_pos + i;
+        if (!sure) {
+            at = on ? rope_row(p, first_row + i, at) : 0;
+            on = on && at >= 0;
+        }
         fetch();
         tau += ROWS;
         float x[8], y[8];
         unpack8(kk, x);
         if (rotates) {
             unpack8(yy, y);
-            rotate_key(p, x, y, max(at, 0), c);
+            rotate_key(p, x, y, on ? at : 0, c);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = to_f32(from_f32<T>(x[e]));   // what a separate rotation would have stored
         }
         uint32_t par, word = quantize_group(x, &par, &bad);
         if (on) {
-            uint32_t *words = reinterpret_cast<uint32_t *>(rec);
-            words[(here * 4 + t) * G + j] = word;
-            if (t == 0) words[Rec<G>::KP / 4 + here * G + j] = par;
-            if (p.summary) {
+            *words = word;
+            if (t == 0) *params = par;
+            if (summary) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float a = x[2 * e], b = x[2 * e + 1];
@@ -244,14 +252,16 @@ __device__ __forceinline__ void append_part(const AppendParams &p, uint8_t *rec,
         word = quantize_group(x, &par, &bad);
         const bool both = __shfl_xor_sync(~0u, (int)on, 4 * G) && on;
         const uint32_t theirs = __shfl_xor_sync(~0u, word, 4 * G);
-        uint8_t *quad = rec + Rec<G>::V + 4 * (G * (32 * (here >> 3) + 8 * t + (here >> 1 & 3)) + j);
+        uint8_t *quad = quads + 4 * G * (32 * (here >> 3) + (here >> 1 & 3));
         if (both) {
             *reinterpret_cast<uint32_t *>(quad + 16 * G * odd) = odd ? __byte_perm(theirs, word, 0x7632) : __byte_perm(word, theirs, 0x5410);
         } else if (on) {
             *reinterpret_cast<uint16_t *>(quad + 2 * odd) = (uint16_t)word;
             *reinterpret_cast<uint16_t *>(quad + 16 * G + 2 * odd) = (uint16_t)(word >> 16);
         }
-        if (on && t == 0) *reinterpret_cast<uint32_t *>(rec + Rec<G>::VP + 4 * (here * G + j)) = par;
+        if (on && t == 0) params[(Rec<G>::VP - Rec<G>::KP) / 4] = par;
+        words += ROWS * 4 * G;
+        params += ROWS * G;
     }
     if (bad) or_status(p.status, OMMX_ST_NONFINITE);
 }
