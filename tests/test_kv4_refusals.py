@@ -198,7 +198,9 @@ def test_the_c_abi_refuses_before_it_launches():
     says(lib.ommx_b200_kv4_decode, d, -1, "no pages")
     s = _lib.KV4SelectArgs(cache=a.cache, seqs=a.seqs, q_dtype=_lib.OMMX_DT_F16, n_q_heads=4, num_selected=2, first_pages=1, last_pages=2)
     says(lib.ommx_b200_kv4_select, s, -1, "fit into")
-    s.last_pages = 1
+    s.last_pages, s.n_q_heads = 1, 2 * 161
+    says(lib.ommx_b200_kv4_select, s, -2, "query heads to a kv head")
+    s.n_q_heads = 4
     says(lib.ommx_b200_kv4_select, s, -1, "null")
     s.q = s.selected = 4096
     says(lib.ommx_b200_kv4_select, s, -1, "summary")
