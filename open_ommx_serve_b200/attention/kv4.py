@@ -95,7 +95,7 @@ def ommx_kv4_decode_attention(q: torch.Tensor, records: torch.Tensor, page_table
     """Attention of one (rotated) query row per sequence, written to ``o`` ``[batch, n_q_heads, D]`` and ``lse`` (fp32).
 
     ``q`` bf16 or fp16, ``o`` bf16, fp16 or fp32; any number of query heads to a kv head.  ``sm_scale`` defaults to
-    ``D ** -0.5``; ``logit_cap`` c makes a logit ``c tanh(x / c)``.  A sequence of no tokens gives ``o = 0``, ``lse = -inf``.
+    ``D ** -0.5`` and may be any finite number; ``logit_cap`` c makes a logit ``c tanh(x / c)``.  A sequence of no tokens gives ``o = 0``, ``lse = -inf``.
     ``selected`` (int32 ``[batch, n_kv_heads, n]``, as ``ommx_kv4_select_pages`` writes it) limits a kv head to these places of
     the page table; the first ``min(n, pages)`` entries count, one below 0 is passed over, one listed twice counts twice.
     ``max_seq_len`` sizes the grid (the table's width without it; up to 512 tokens it is one launch); ``workspace`` (fp32,

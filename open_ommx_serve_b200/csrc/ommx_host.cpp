@@ -859,6 +859,7 @@ PyObject *py_kv4_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
     d.o = o->data_ptr(); d.o_stride_b = o->stride(0); d.o_stride_h = o->stride(1);
     d.lse = (float *)lse->data_ptr(); d.lse_stride_b = lse->stride(0);
     d.sm_scale = (float)(a[6] == Py_None ? 1.0 / std::sqrt((double)D) : c.number(a[6], "sm_scale"));
+    KV4_EXPECT(c, std::isfinite(d.sm_scale), "sm_scale must be finite in 32 bits");
     d.logit_cap = (float)c.number(a[7], "logit_cap");
     KV4_EXPECT(c, d.logit_cap >= 0.0f && std::isfinite(d.logit_cap), "logit_cap must be finite and not negative");
     if (const Tensor *sel = c.tensor(a[8], "selected", false)) {

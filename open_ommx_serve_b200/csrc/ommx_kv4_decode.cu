@@ -210,7 +210,8 @@ __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int fir
     for (int i = 0; i < 2; ++i) {
         const float f = __shfl_sync(~0u, factor, 8 * t + 4 * i);
         q.raw[i] = f / p.cap;
-        q.factor[i] = p.cap > 0.0f ? p.cap * LOG2E : f * LOG2E;
+        // never 0, so that a masked logit can be an infinity of the other sign: without a cap |x| < 2^124, and x times this is nothing
+        q.factor[i] = p.cap > 0.0f ? p.cap * LOG2E : f * LOG2E != 0.0f ? f * LOG2E : 0x1p-149f;
     }
     // rows of the product: term r of group j at G r + j; lane t holds rows 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
     const int j = G == 4 ? 2 * (t & 1) : 0;
@@ -338,13 +339,16 @@ template <int G, bool FINE> __device__ __forceinline__ void attend(const DecodeP
     }
     const float f0 = q.factor[0], f1 = q.factor[1];                         // x f: logits in powers of two
     if (n < 16) {                                 // what lies behind the last token may be anything
+        const float out0 = copysignf(INFINITY, -f0), out1 = copysignf(INFINITY, -f1);   // logits of -inf, whatever the scale's sign
         if (g >= n) {
-            x[0] = x[1] = -INFINITY;
+            x[0] = out0;
+            x[1] = out1;
 #pragma unroll
             for (int j = 0; j < G; ++j) vp0[j] = 0;
         }
         if (g + 8 >= n) {
-            x[2] = x[3] = -INFINITY;
+            x[2] = out0;
+            x[3] = out1;
 #pragma unroll
             for (int j = 0; j < G; ++j) vp1[j] = 0;
         }
@@ -927,6 +931,7 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     if (a->n_q_heads < p.c.H || a->n_q_heads % p.c.H)
         return fail(OMMX_E_UNSUPPORTED, "kv4_decode: %d query heads are not a multiple of %d kv heads", a->n_q_heads, p.c.H);
     if (!(a->logit_cap >= 0.0f) || !std::isfinite(a->logit_cap)) return fail(OMMX_E_ARG, "kv4_decode: logit_cap must be finite and not negative");
+    if (!std::isfinite(a->sm_scale)) return fail(OMMX_E_ARG, "kv4_decode: sm_scale must be finite");
     if (a->selected && a->num_selected < 0) return fail(OMMX_E_ARG, "kv4_decode: num_selected must not be negative");
     if (p.s.B > 65535) return fail(OMMX_E_UNSUPPORTED, "kv4_decode: a batch of %d", p.s.B);
     if (p.s.B == 0) return 0;

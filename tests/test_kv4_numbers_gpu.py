@@ -1,0 +1,86 @@
+"""Attention over the 4-bit cache where numbers are unusual: scales of logits of every sign, values of every size the cache holds, weights
+far below the largest.  Every output is held to a bound of its own, for its head and its group of 32 channels.
+
+Bounds, with p the softmax in 64 bits, s, z and V the cached scales, zeros and values of a group, n tokens:
+* a weight times a scale is rounded to fp16, by 2^-11 of it at most, and its codes are 15 at most: 2^-11 * 15 sum p s; where the output is
+  finer than bf16 the rest is rounded once more: 2^-21 * 15 sum p s;
+* the largest product p s of a warp (over its tokens and all groups) lies above 2^10 in the units that fp16 has, whose steps are 2^-24: what is
+  lost of a small one is half a step, 2^-35 of the largest, so n * 15 * 2^-35 max p s in all;
+* logits are fp32 sums of a few hundred terms, off by 2^-17 of |q|.|K| sm_scale at most (and 2^-20 for the exponential): a weight is
+  off by that share d, an output by 2 d (sum p |V| + |o|) <= 4 d sum p |V|;
+* sums of up to some hundred terms in 32 bits, those of codes cut by up to 2^-23 at each of 64 additions: 2^-17 (15 sum p s + sum p |z|);
+* the output is rounded by half a step.
+The log-sum-exp is off by d and by 2^-22 of itself.
+"""
+import math
+
+import pytest
+import torch
+
+import kv4_reference as ref
+from test_kv4_gpu import DEV, filled, rows_of, tables
+from open_ommx_serve_b200 import ommx_kv4_alloc, ommx_kv4_append, ommx_kv4_decode_attention
+
+pytestmark = pytest.mark.gpu
+
+
+def value_parameters(records, table, length):
+    """Scales and zeros of a sequence's values: [H, length, D / 32] each, in 64 bits."""
+    S, D = records.shape[2], records.shape[3] // 20
+    rec = records[table[:-(-length // (16 * S))].long()]
+    words = rec[..., 18 * D:].contiguous().view(torch.int32).unflatten(-1, (16, D // 32)).transpose(0, 1).flatten(1, 3)[:, :length]
+    return (words & -65536).view(torch.float32).double(), (words << 16).view(torch.float32).double()
+
+
+def expected(q, records, table, n, sm_scale, cap, o_dtype):
+    """o, lse of one sequence in 64 bits, and how far from them a kernel may be: q [Hq, D]."""
+    k, v = ref.sequence(records, table, n)
+    s, z = value_parameters(records, table, n)
+    group = q.shape[0] // k.shape[0]
+    eps = torch.finfo(o_dtype).eps / 2
+    outs = []
+    for h in range(q.shape[0]):
+        kk, vv, ss, zz = (x[h // group] for x in (k, v, s, z))
+        x = kk @ q[h].double() * sm_scale
+        d = 2.0 ** -17 * float((kk.abs() @ q[h].double().abs()).max()) * abs(sm_scale) + 2.0 ** -20
+        if cap:
+            x = cap * torch.tanh(x / cap)
+        p = torch.softmax(x, 0)
+        o, lse = p @ vv, torch.logsumexp(x, 0)
+        codes = 15 * (p @ ss)                                                # of each group
+        lost = 15 * n * 2.0 ** -35 * float((p[:, None] * ss).max())
+        off = (codes * (2.0 ** -11 if o_dtype == torch.bfloat16 else 2.0 ** -21) + lost + 2.0 ** -17 * (codes + p @ zz.abs())).repeat_interleave(32)
+        outs.append((o, lse, off + 4 * d * (p @ vv.abs()) + eps * o.abs(), d + 2.0 ** -22 * abs(float(lse))))
+    return outs
+
+
+def check(cache, table, lens, q, o, lse, sm_scale=None, cap=0.0):
+    sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else sm_scale
+    for b, n in enumerate(lens):
+        for h, (wo, wl, off, drift) in enumerate(expected(q[b], cache["records"], table[b], n, sm_scale, cap, o.dtype)):
+            worst = ((o[b, h].double() - wo).abs() / off.clamp(min=1e-300)).max()
+            assert float(worst) <= 1, (b, h, n, float(worst))
+            assert abs(float(lse[b, h]) - float(wl)) <= drift, (b, h, n, float(lse[b, h]), float(wl), drift)
+
+
+# ---- the scale of the logits ---------------------------------------------------------------------------------------
+FORMS = [
+    # D, H, Hq, lens: a block to a row, a cluster to one, pieces of rows, even shares of all rows
+    (128, 2, 6, [17, 250, 1, 5]),
+    (128, 2, 8, [4001]),
+    (64, 2, 2, [9001, 33]),
+    (128, 8, 8, [611] + [300 + 3 * i for i in range(79)]),
+]
+
+
+@pytest.mark.parametrize("D,H,Hq,lens", FORMS)
+@pytest.mark.parametrize("sm_scale,cap", [(0.0, 0.0), (-0.3, 0.0), (-0.05, 4.0), (0.0, 2.0), (1e-44, 0.0)])
+def test_logit_scales_of_zero_and_below(D, H, Hq, lens, sm_scale, cap):
+    """Tokens behind a sequence's end stay out whatever the scale's sign; a scale of 0 gives the mean."""
+    cache, table, length = filled(lens, H, D, 16, seed=141)
+    q = torch.randn(len(lens), Hq, D, generator=torch.Generator().manual_seed(142)).bfloat16().to(DEV)
+    o, lse = torch.full((len(lens), Hq, D), 7.0, device=DEV), torch.full((len(lens), Hq), 7.0, device=DEV)
+    ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse, sm_scale=sm_scale, logit_cap=cap, max_seq_len=max(lens))
+    few = list(range(len(lens)))[:6]
+    check(cache, table, [lens[b] for b in few], q, o, lse, sm_scale, cap)
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all()

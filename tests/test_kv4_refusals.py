@@ -218,3 +218,12 @@ def test_struct_layouts_match_the_header():
         body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct %s \{(.*?)\} %s;" % (struct, struct), header, re.S).group(1), flags=re.S)
         names = [n.strip().lstrip("*") for decl in body.split(";") if decl.strip() for n in re.sub(r"^(const\s+)?\w+\s+", "", decl.strip()).split(",")]
         assert names == [f[0] for f in cls._fields_], struct
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), 1e300])
+def test_a_logit_scale_that_is_no_32_bit_number_is_refused(bad):
+    with pytest.raises(ValueError, match="sm_scale"):
+        decode(base(), sm_scale=bad)
+    d = _lib.KV4DecodeArgs(cache=_lib.KV4Cache(4096, None, 4, 2, 64, 16), seqs=_lib.KV4Seqs(4096, 4096, 3, 0, 3, 2), q_dtype=_lib.OMMX_DT_BF16, n_q_heads=4)
+    d.sm_scale = bad if abs(bad) != 1e300 else float("inf")
+    assert _lib.load().ommx_b200_kv4_decode(C.byref(d), None) == -1 and "sm_scale" in _lib.last_error()
