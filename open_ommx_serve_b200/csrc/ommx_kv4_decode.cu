@@ -30,7 +30,10 @@ constexpr int STAGES = 3, AHEAD = STAGES - 1;     // records that a warp holds, 
 constexpr int FULL = 0x1010;                      // sixteen tokens in each of those
 constexpr int COLS = 8;                           // query heads side by side
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr float ROOM = 4096.0f;                   // how large a weight may get before its reference moves
+// Weights w = 2^(x - ref) are held near 2^-ABOVE: they meet zeros of up to 2^126, and a sum of 2^24 such products at HEAVY stays below 2^127.
+// Products of weights and scales, w s unit, go to fp16: near 2^TOP, and up to ROOM before the references move.
+constexpr int ABOVE = 30, TOP = 0;
+constexpr float HEAVY = 0x1p-23f, ROOM = 4096.0f;
 constexpr float LOWEST = -1e30f;
 constexpr int MOST_PARTS = 768;                   // blocks of a call that shares rows
 constexpr int WHOLE = 32;                         // records of a row that one block takes at most where it could share it
@@ -148,6 +151,10 @@ __device__ __forceinline__ float scale_of(uint32_t w) { return __uint_as_float(w
 __device__ __forceinline__ float zero_of(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23 & 255u) - 127; }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
+// of a reference and a sum of weights, which lie near 2^-ABOVE
+__device__ __forceinline__ float log_sum(float ref, float sum) {
+    return sum != 0.0f ? ((ref - ABOVE) + log2f(sum * power_of_two(ABOVE))) * LN2 : -INFINITY;
+}
 
 // eight channels of a query
 __device__ __forceinline__ void load_q8(const DecodeParams &p, int64_t at, float *x) {
@@ -240,6 +247,7 @@ __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int fir
 // `acc` is added to `whole` in shared memory every 64 records, every 32 where the output is finer than bf16 (2 % of the time).
 template <int G> struct State {
     float acc[G][2][4], zero[G][2], sum[2], ref[2];
+    float unit[2];                                // a power of two that only `acc` has in it
     float *whole;                                 // the lane's first of 8 G values, 32 apart
     bool some;                                    // there is something there
 };
@@ -257,18 +265,28 @@ template <int G> __device__ __forceinline__ void clear(State<G> &s, float *whole
     }
     s.sum[0] = s.sum[1] = 0.0f;
     s.ref[0] = s.ref[1] = LOWEST;
+    s.unit[0] = s.unit[1] = 1.0f;
 }
-template <int G> __device__ __forceinline__ void rescale(State<G> &s, float f0, float f1) {
+// The references of head i move: to whole numbers, so that nothing is rounded. `logit`: the record's largest; `product`: that of logits and
+// their scales' exponents. A unit stays within normal numbers: where scales are the smallest (2^-96), products stay below 2^TOP.
+template <int G> __device__ __forceinline__ void move(State<G> &s, int i, float logit, float product) {
+    const int was = exponent_of(s.unit[i]);
+    const float ref = fmaxf(s.ref[i], ceilf(logit) + ABOVE);
+    const float over = ceilf(fmaxf(s.ref[i] + (float)(TOP - was), product) - ref);         // 2^over: the largest product
+    const int now = TOP - (int)fminf(fmaxf(over, (float)(TOP - 126)), (float)(TOP + 126));
+    const float f = exp2_approx(s.ref[i] - ref), a = exp2_approx(s.ref[i] - ref + (float)(now - was));
+    s.ref[i] = ref;
+    s.unit[i] = power_of_two(now);
 #pragma unroll
     for (int j = 0; j < G; ++j) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) { s.acc[j][u][0] *= f0; s.acc[j][u][1] *= f1; s.acc[j][u][2] *= f0; s.acc[j][u][3] *= f1; }
-        s.zero[j][0] *= f0; s.zero[j][1] *= f1;
+        for (int u = 0; u < 2; ++u) { s.acc[j][u][i] *= a; s.acc[j][u][i + 2] *= a; }
+        s.zero[j][i] *= f;
     }
-    s.sum[0] *= f0; s.sum[1] *= f1;
+    s.sum[i] *= f;
     if (s.some)
 #pragma unroll 1
-        for (int i = 0; i < 8 * G; i += 2) { s.whole[32 * i] *= f0; s.whole[32 * i + 32] *= f1; }
+        for (int k = i; k < 8 * G; k += 2) s.whole[32 * k] *= a;
 }
 template <int G> __device__ __forceinline__ void put_by(State<G> &s) {      // acc to `whole`
 #pragma unroll
@@ -356,32 +374,31 @@ template <int G, bool FINE> __device__ __forceinline__ void attend(const DecodeP
 
     // ---- weights
     // the largest scale of each token; a word taken as a number is its scale and less than a hundredth of it more
-    float top0 = 0x1p-30f, top1 = 0x1p-30f;
+    float top0 = 0.0f, top1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < G; j += 2) {
         top0 = max3(top0, __uint_as_float(vp0[j]), __uint_as_float(vp0[j + 1]));
         top1 = max3(top1, __uint_as_float(vp1[j]), __uint_as_float(vp1[j + 1]));
     }
-    float w[4];
+    float w[4], y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = exp2_approx(fmaf(x[i], i & 1 ? f1 : f0, -s.ref[i & 1]));
-    const float most = fmaxf(fmaxf(w[0], w[1]) * top0, fmaxf(w[2], w[3]) * top1);
-    if (__any_sync(~0u, !(most <= ROOM))) {
-        // the references move to the largest logit plus exponent of its scales
+    for (int i = 0; i < 4; ++i) { w[i] = exp2_approx(fmaf(x[i], i & 1 ? f1 : f0, -s.ref[i & 1])); y[i] = w[i] * s.unit[i & 1]; }
+    const float heavy = fmaxf(max3(w[0], w[1], w[2]), w[3]), most = fmaxf(fmaxf(y[0], y[1]) * top0, fmaxf(y[2], y[3]) * top1);
+    if (__any_sync(~0u, !(heavy <= HEAVY && most <= ROOM))) {
         const float e0 = (float)(exponent_of(top0) + 1), e1 = (float)(exponent_of(top1) + 1);
-        float r0 = fmaxf(fmaf(x[0], f0, e0), fmaf(x[2], f0, e1)), r1 = fmaxf(fmaf(x[1], f1, e0), fmaf(x[3], f1, e1));
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) {
-            r0 = fmaxf(r0, __shfl_xor_sync(~0u, r0, d));
-            r1 = fmaxf(r1, __shfl_xor_sync(~0u, r1, d));
+        for (int i = 0; i < 2; ++i) {
+            const float f = i ? f1 : f0;
+            float l = fmaxf(x[i] * f, x[i + 2] * f), r = fmaxf(fmaf(x[i], f, e0), fmaf(x[i + 2], f, e1));
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) {
+                l = fmaxf(l, __shfl_xor_sync(~0u, l, d));
+                r = fmaxf(r, __shfl_xor_sync(~0u, r, d));
+            }
+            move(s, i, l, r);
         }
-        r0 = fmaxf(s.ref[0], r0);
-        r1 = fmaxf(s.ref[1], r1);
-        rescale(s, exp2_approx(s.ref[0] - r0), exp2_approx(s.ref[1] - r1));
-        s.ref[0] = r0;
-        s.ref[1] = r1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = exp2_approx(fmaf(x[i], i & 1 ? f1 : f0, -s.ref[i & 1]));
+        for (int i = 0; i < 4; ++i) { w[i] = exp2_approx(fmaf(x[i], i & 1 ? f1 : f0, -s.ref[i & 1])); y[i] = w[i] * s.unit[i & 1]; }
     }
     s.sum[0] += w[0] + w[2];
     s.sum[1] += w[1] + w[3];
@@ -395,15 +412,15 @@ template <int G, bool FINE> __device__ __forceinline__ void attend(const DecodeP
         const float s0 = scale_of(vp0[j]), s1 = scale_of(vp1[j]), z0 = zero_of(vp0[j]), z1 = zero_of(vp1[j]);
         s.zero[j][0] = fmaf(z1, w[2], fmaf(z0, w[0], s.zero[j][0]));
         s.zero[j][1] = fmaf(z1, w[3], fmaf(z0, w[1], s.zero[j][1]));
-        const float y[4] = {w[0] * s0, w[1] * s0, w[2] * s1, w[3] * s1};
-        const uint32_t h0 = half2_bits(y[0], y[1]), h1 = half2_bits(y[2], y[3]);
+        const float m[4] = {y[0] * s0, y[1] * s0, y[2] * s1, y[3] * s1};
+        const uint32_t h0 = half2_bits(m[0], m[1]), h1 = half2_bits(m[2], m[3]);
         const uint32_t a = v0[j] >> 8, b = v1[j] >> 8;
         const uint32_t b0 = transpose8x8(h0), b1 = transpose8x8(h1);
         mma(s.acc[j][0], v0[j] & LO, v0[j] & HI, v1[j] & LO, v1[j] & HI, b0, b1);
         mma(s.acc[j][1], a & LO, a & HI, b & LO, b & HI, b0, b1);
         if constexpr (FINE) {
             const float2 r0 = half2_floats(h0), r1 = half2_floats(h1);
-            const uint32_t d0 = transpose8x8(half2_bits(y[0] - r0.x, y[1] - r0.y)), d1 = transpose8x8(half2_bits(y[2] - r1.x, y[3] - r1.y));
+            const uint32_t d0 = transpose8x8(half2_bits(m[0] - r0.x, m[1] - r0.y)), d1 = transpose8x8(half2_bits(m[2] - r1.x, m[3] - r1.y));
             mma(s.acc[j][0], v0[j] & LO, v0[j] & HI, v1[j] & LO, v1[j] & HI, d0, d1);
             mma(s.acc[j][1], a & LO, a & HI, b & LO, b & HI, d0, d1);
         }
@@ -446,22 +463,23 @@ __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Share
         for (int i = 0; i < 2; ++i) { ref[2 * t + i][warp] = s.ref[i]; sum[2 * t + i][warp] = s.sum[i]; }
     }
     __syncthreads();                              // and the ring, whose memory `sh` is, is done with
-    float f[2];
+    float f[2], back[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         float top = ref[2 * t + i][0];
 #pragma unroll
         for (int w = 1; w < NW; ++w) top = fmaxf(top, ref[2 * t + i][w]);
         f[i] = exp2_approx(s.ref[i] - top);
+        back[i] = power_of_two(20 - exponent_of(s.unit[i]));                // 2^20 / unit
     }
 #pragma unroll
     for (int j = 0; j < G; ++j)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             float *to = &sh.o[warp][2 * t + i][32 * j + 4 * g];
-            const float z = s.zero[j][i];
-            *reinterpret_cast<float4 *>(to) = make_float4(f[i] * fmaf(s.acc[j][0][i], 0x1p24f, z), f[i] * fmaf(s.acc[j][0][i + 2], 0x1p20f, z),
-                                                          f[i] * fmaf(s.acc[j][1][i], 0x1p24f, z), f[i] * fmaf(s.acc[j][1][i + 2], 0x1p20f, z));
+            const float z = s.zero[j][i], even = 16.0f * back[i];
+            *reinterpret_cast<float4 *>(to) = make_float4(f[i] * fmaf(s.acc[j][0][i], even, z), f[i] * fmaf(s.acc[j][0][i + 2], back[i], z),
+                                                          f[i] * fmaf(s.acc[j][1][i], even, z), f[i] * fmaf(s.acc[j][1][i + 2], back[i], z));
         }
     __syncthreads();
     for (int h = warp; h < COLS; h += NW) {
@@ -487,7 +505,7 @@ __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Share
 #pragma unroll
             for (int i = 0; i < G; ++i) v[i] = all != 0.0f ? v[i] * inverse : 0.0f;
             store_o(p, b * p.o_b + (first_head + h) * p.o_h + lane * G, v);
-            if (lane == 0) p.lse[b * p.lse_b + first_head + h] = all != 0.0f ? (top + log2f(all)) * LN2 : -INFINITY;
+            if (lane == 0) p.lse[b * p.lse_b + first_head + h] = log_sum(top, all);
         }
     }
     __syncthreads();
@@ -569,7 +587,7 @@ template <int G> __device__ __forceinline__ void merge_cluster(const DecodeParam
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = all != 0.0f ? o[i] * inverse : 0.0f;
         if (lane < LANES) store_o(p, b * p.o_b + (first_head + h) * p.o_h + 4 * lane, o);
-        if (lane == 0) p.lse[b * p.lse_b + first_head + h] = all != 0.0f ? (top + log2f(all)) * LN2 : -INFINITY;
+        if (lane == 0) p.lse[b * p.lse_b + first_head + h] = log_sum(top, all);
     }
     cluster_barrier();                            // no block leaves before its peers have read its part
 }
@@ -808,7 +826,7 @@ template <int G> __global__ void __launch_bounds__(32 * COLS) kv4_combine_row_ke
 #pragma unroll
     for (int i = 0; i < G; ++i) o[i] = sum != 0.0f ? o[i] * inverse : 0.0f;
     store_o(p, b * p.o_b + hq * p.o_h + lane * G, o);
-    if (lane == 0) p.lse[b * p.lse_b + hq] = sum != 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
+    if (lane == 0) p.lse[b * p.lse_b + hq] = log_sum(top, sum);
 }
 
 // The same where rows are few and their parts many: a block to a head. The references and sums of all parts are read at once; then a
@@ -881,7 +899,7 @@ template <int G> __global__ void __launch_bounds__(32 * CW) kv4_combine_head_ker
         for (int w = 0; w < CW; ++w) x += so[w][c];
         store_o(p, b * p.o_b + hq * p.o_h + c, sum != 0.0f ? x / sum : 0.0f);
     }
-    if (threadIdx.x == 0) p.lse[b * p.lse_b + hq] = sum != 0.0f ? (top + log2f(sum)) * LN2 : -INFINITY;
+    if (threadIdx.x == 0) p.lse[b * p.lse_b + hq] = log_sum(top, sum);
 }
 
 // ---- host ---------------------------------------------------------------------------------------

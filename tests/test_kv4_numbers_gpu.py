@@ -84,3 +84,58 @@ def test_logit_scales_of_zero_and_below(D, H, Hq, lens, sm_scale, cap):
     few = list(range(len(lens)))[:6]
     check(cache, table, [lens[b] for b in few], q, o, lse, sm_scale, cap)
     assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+
+
+# ---- the size of the values ----------------------------------------------------------------------------------------
+def cache_of(k, v, page=16):
+    """One sequence per entry of the lists k, v ([tokens, H, D]): (cache, table, lens tensor, lens)."""
+    lens = [len(x) for x in k]
+    table, P = tables(lens, page)
+    cache = ommx_kv4_alloc(P, k[0].shape[1], k[0].shape[2], page_size=page, device=DEV)
+    start, length = rows_of(lens, lens)
+    ommx_kv4_append(torch.cat(k).to(DEV), torch.cat(v).to(DEV), cache["records"], table.to(DEV), length.to(DEV), row_start=start.to(DEV))
+    return cache, table.to(DEV), length.to(DEV), lens
+
+
+SIZES = [1e-30, 1e-24, 1e-20, 1e-16, 1e-12, 1e-3, 1e5, 1e12, 1e20, 1e30, 6e36]
+
+
+@pytest.mark.parametrize("form", range(len(FORMS)))
+@pytest.mark.parametrize("o_dtype", [torch.bfloat16, torch.float32])
+def test_values_of_every_size(form, o_dtype):
+    """Random values and constant ones from 2^-100 to near the 2^126 that the cache holds, with equal weights and others."""
+    D, H, Hq, lens = FORMS[form]
+    if lens[0] > 5000:
+        lens = [4500, 33]                         # still in pieces, two launches
+    few = list(range(len(lens)))[:4]
+    gen = torch.Generator().manual_seed(151)
+    k = torch.randn(sum(lens), H, D, generator=gen)
+    v = torch.randn(sum(lens), H, D, generator=gen)
+    q = torch.randn(len(lens), Hq, D, generator=gen)
+    q[:, ::2] = 0
+    q = q.bfloat16().to(DEV)
+    o, lse = torch.empty(len(lens), Hq, D, dtype=o_dtype, device=DEV), torch.empty(len(lens), Hq, device=DEV)
+    for size in SIZES:
+        for values in (v * size, torch.full_like(v, size), torch.full_like(v, -size)):
+            cache, table, length, _ = cache_of(k.split(lens), values.split(lens))
+            ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse, max_seq_len=max(lens))
+            check(cache, table, [lens[b] for b in few], q, o, lse)
+
+
+@pytest.mark.parametrize("o_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("small,large", [(1.0, 1e36), (1e-20, 1e20), (1e-28, 1e8), (1e-25, 1e-5), (1.0, 0.0)])
+def test_values_of_several_sizes_together(small, large, o_dtype):
+    """Tokens that differ in size by up to 2^120, the large ones first, last, in between, heavy and light: sums of weights keep every token,
+    whatever their values."""
+    n, D = 700, 128
+    gen = torch.Generator().manual_seed(152)
+    at = [torch.arange(n) < 3, torch.arange(n) >= n - 3, torch.arange(n) % 50 == 7, torch.arange(n) % 2 == 0]
+    k = [0.05 * torch.randn(n, 1, D, generator=gen) + a[:, None, None].float() for a in at]          # large ones are heavy, or light
+    v = [torch.randn(n, 1, D, generator=gen) * torch.where(a, large, small)[:, None, None] for a in at]
+    cache, table, length, lens = cache_of(k, v)
+    for most in (None, n, 256 * 16):
+        for weight in (0.0, 0.08, -0.08, 0.4, -0.4):
+            q = torch.full((4, 2, D), weight).bfloat16().to(DEV)
+            o, lse = torch.empty(4, 2, D, dtype=o_dtype, device=DEV), torch.empty(4, 2, device=DEV)
+            ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse, max_seq_len=most)
+            check(cache, table, lens, q, o, lse)
