@@ -8,10 +8,17 @@
 // that share the kv head its columns. Scales meet the sums of K's groups behind the product and the weights of V before it, zeros
 // are fp32 multiply-adds. Queries keep all their bits: a head's are scaled by a power of two into fp16's range.
 //
-// Weights p_t s_tj are rounded to fp16 (2^-12 of each, of either sign): against the running reference r, which covers the logit and
-// the scale, they are 2^12 at most, and those below 2^-36 of the largest are lost. That is an eighth of a bf16 output's own
+// A weight w_t = exp(x_t) stays fp32 where it meets a zero and in the sum, against a reference of the logits alone: values of any size the
+// cache holds leave no token out. Products w_t s_tj are rounded to fp16, by 2^-11 at most, in a unit that the largest of them sets: below
+// 2^-23 of it they have fewer bits (fp16's smallest step is 2^-24), and are off by 2^-34 of it at most. That is less than a bf16 output's own
 // rounding; where the output is finer (fp16, fp32), a second product takes what the rounding left (FINE: 32 ragged sequences 57 us
 // without, 64 with). Sums of weights and zeros stay fp32.
+//
+// What the tensor cores cut is then the largest error of a record: they line the addends of a product up with the largest and cut them 25 bits
+// below its leading one (an emulation of that gives the kernel's errors), where a subnormal counts as 2^-14. A masked nibble lies 10 bits
+// below that (the odd ones, 16 times as large, 6), so an addend loses up to 2^-15 of one code of the record's heaviest token - or, in a
+// logit, of the group's largest |q| -: 2^-15 of a group's range a record at most, of the heaviest token's share in the output. Nibbles
+// moved up to bits 6..9 would lose 2^-21, for some 48 shifts a record.
 //
 // What bounds it: a record's 160 bytes a token are read once, so HBM, and beside it the schedulers: a record is some 320 instructions
 // of a warp, 17 of them products that hold a scheduler 8 cycles, in which its multiply-adds wait. 8 x 64K tokens, 8 kv heads, 32
@@ -31,9 +38,10 @@ constexpr int FULL = 0x1010;                      // sixteen tokens in each of t
 constexpr int COLS = 8;                           // query heads side by side
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // Weights w = 2^(x - ref) are held near 2^-ABOVE: they meet zeros of up to 2^126, and a sum of 2^24 such products at HEAVY stays below 2^127.
-// Products of weights and scales, w s unit, go to fp16: near 2^TOP, and up to ROOM before the references move.
-constexpr int ABOVE = 30, TOP = 0;
-constexpr float HEAVY = 0x1p-23f, ROOM = 4096.0f;
+// Products of weights and scales, w s unit, go to fp16: the largest one lies above 2^(TOP - 2) when the references have moved, and may grow to ROOM
+// before they move again. More of fp16's range below it would cost moves (TOP 8, 11, 12: 8 x 64K tokens 137.9, 138.6, 139.3 us).
+constexpr int ABOVE = 30, TOP = 11;
+constexpr float HEAVY = 0x1p-23f, ROOM = 60000.0f;
 constexpr float LOWEST = -1e30f;
 constexpr int MOST_PARTS = 768;                   // blocks of a call that shares rows
 constexpr int WHOLE = 32;                         // records of a row that one block takes at most where it could share it

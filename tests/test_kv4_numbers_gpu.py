@@ -4,13 +4,20 @@ far below the largest.  Every output is held to a bound of its own, for its head
 Bounds, with p the softmax in 64 bits, s, z and V the cached scales, zeros and values of a group, n tokens:
 * a weight times a scale is rounded to fp16, by 2^-11 of it at most, and its codes are 15 at most: 2^-11 * 15 sum p s; where the output is
   finer than bf16 the rest is rounded once more: 2^-21 * 15 sum p s;
-* the largest product p s of a warp (over its tokens and all groups) lies above 2^10 in the units that fp16 has, whose steps are 2^-24: what is
-  lost of a small one is half a step, 2^-35 of the largest, so n * 15 * 2^-35 max p s in all;
-* logits are fp32 sums of a few hundred terms, off by 2^-17 of |q|.|K| sm_scale at most (and 2^-20 for the exponential): a weight is
-  off by that share d, an output by 2 d (sum p |V| + |o|) <= 4 d sum p |V|;
-* sums of up to some hundred terms in 32 bits, those of codes cut by up to 2^-23 at each of 64 additions: 2^-17 (15 sum p s + sum p |z|);
+* the largest product p s of a warp (over its tokens and all groups) lies above 2^9 in the units that fp16 has, whose steps are 2^-24: what is
+  lost of a small one is half a step, 2^-34 of the largest, so n * 15 * 2^-34 max p s in all;
+* the tensor cores line the addends of a product of 16 up with the largest and cut them 25 bits below its leading one.  A masked nibble is an
+  fp16 subnormal, code * 2^-24, that counts as 2^-14 there: an addend (16 and the sum so far) loses up to 2^-15 of one code of the record's
+  heaviest token, 17 * 2^-15 max p s a record, 18 with the product of what the rounding left; and the sum, where it is the largest, up to
+  2^-23 of itself at each of 64 additions: 2^-17 * 15 sum p s;
+* the same in the two products of a group's logits, 33 * 2^-15 max |q| s_K of the group (its channels); beside it they are fp32 sums of a
+  few hundred terms, off by 2^-17 of |q|.|K|.  Times sm_scale, and with 2^-20 for the exponential, that is the share d by which a weight
+  is off, an output by 2 d (sum p |V| + |o|) <= 4 d sum p |V|;
+* sums of zeros and of weights are 32-bit chains.  A warp has n / 64 records at most (four warps or more share a row in turns); a lane adds two
+  tokens' zeros of each, n / 32 additions and up to 64 more to merge, each rounded by 2^-24 of the sum, all the same way where all addends
+  are alike: (n / 32 + 64) 2^-24 sum p |z|, and of weights, one addition a record, (n / 64 + 64) 2^-24 of the output;
 * the output is rounded by half a step.
-The log-sum-exp is off by d and by 2^-22 of itself.
+The log-sum-exp is off by d, by the share that the sum of weights is, and by 2^-22 of itself.
 """
 import math
 
@@ -24,39 +31,44 @@ from open_ommx_serve_b200 import ommx_kv4_alloc, ommx_kv4_append, ommx_kv4_decod
 pytestmark = pytest.mark.gpu
 
 
-def value_parameters(records, table, length):
-    """Scales and zeros of a sequence's values: [H, length, D / 32] each, in 64 bits."""
+def parameters(records, table, length, at):
+    """Scales and zeros of a sequence's keys (at 16) or values (18): [H, length, D / 32] each, in 64 bits."""
     S, D = records.shape[2], records.shape[3] // 20
     rec = records[table[:-(-length // (16 * S))].long()]
-    words = rec[..., 18 * D:].contiguous().view(torch.int32).unflatten(-1, (16, D // 32)).transpose(0, 1).flatten(1, 3)[:, :length]
+    words = rec[..., at * D:(at + 2) * D].contiguous().view(torch.int32).unflatten(-1, (16, D // 32)).transpose(0, 1).flatten(1, 3)[:, :length]
     return (words & -65536).view(torch.float32).double(), (words << 16).view(torch.float32).double()
 
 
 def expected(q, records, table, n, sm_scale, cap, o_dtype):
     """o, lse of one sequence in 64 bits, and how far from them a kernel may be: q [Hq, D]."""
     k, v = ref.sequence(records, table, n)
-    s, z = value_parameters(records, table, n)
+    (s, z), (sk, _) = parameters(records, table, n, 18), parameters(records, table, n, 16)
     group = q.shape[0] // k.shape[0]
     eps = torch.finfo(o_dtype).eps / 2
     outs = []
     for h in range(q.shape[0]):
-        kk, vv, ss, zz = (x[h // group] for x in (k, v, s, z))
+        kk, vv, ss, zz, sq = (x[h // group] for x in (k, v, s, z, sk))
         x = kk @ q[h].double() * sm_scale
-        d = 2.0 ** -17 * float((kk.abs() @ q[h].double().abs()).max()) * abs(sm_scale) + 2.0 ** -20
+        top = q[h].double().abs().unflatten(0, (-1, 32)).amax(-1)            # of each group
+        d = float((2.0 ** -17 * (kk.abs() @ q[h].double().abs()) + 33 * 2.0 ** -15 * (sq @ top)).max()) * abs(sm_scale) + 2.0 ** -20
         if cap:
             x = cap * torch.tanh(x / cap)
         p = torch.softmax(x, 0)
         o, lse = p @ vv, torch.logsumexp(x, 0)
         codes = 15 * (p @ ss)                                                # of each group
-        lost = 15 * n * 2.0 ** -35 * float((p[:, None] * ss).max())
-        off = (codes * (2.0 ** -11 if o_dtype == torch.bfloat16 else 2.0 ** -21) + lost + 2.0 ** -17 * (codes + p @ zz.abs())).repeat_interleave(32)
-        outs.append((o, lse, off + 4 * d * (p @ vv.abs()) + eps * o.abs(), d + 2.0 ** -22 * abs(float(lse))))
+        ps = p[:, None] * ss
+        heaviest = torch.cat((ps, ps.new_zeros(-n % 16, ps.shape[1]))).unflatten(0, (-1, 16)).amax(1).sum(0)
+        lost = 15 * n * 2.0 ** -34 * float(ps.max()) + 18 * 2.0 ** -15 * heaviest
+        off = (codes * (2.0 ** -11 if o_dtype == torch.bfloat16 else 2.0 ** -21) + lost + 2.0 ** -17 * codes + (n / 32 + 64) * 2.0 ** -24 * (p @ zz.abs())).repeat_interleave(32)
+        share = (n / 64 + 64) * 2.0 ** -24
+        outs.append((o, lse, off + 4 * d * (p @ vv.abs()) + (eps + share) * o.abs(), d + share + 2.0 ** -22 * abs(float(lse))))
     return outs
 
 
-def check(cache, table, lens, q, o, lse, sm_scale=None, cap=0.0):
+def check(cache, table, lens, q, o, lse, sm_scale=None, cap=0.0, which=None):
     sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else sm_scale
-    for b, n in enumerate(lens):
+    for b in which or range(len(lens)):
+        n = lens[b]
         for h, (wo, wl, off, drift) in enumerate(expected(q[b], cache["records"], table[b], n, sm_scale, cap, o.dtype)):
             worst = ((o[b, h].double() - wo).abs() / off.clamp(min=1e-300)).max()
             assert float(worst) <= 1, (b, h, n, float(worst))
@@ -81,8 +93,7 @@ def test_logit_scales_of_zero_and_below(D, H, Hq, lens, sm_scale, cap):
     q = torch.randn(len(lens), Hq, D, generator=torch.Generator().manual_seed(142)).bfloat16().to(DEV)
     o, lse = torch.full((len(lens), Hq, D), 7.0, device=DEV), torch.full((len(lens), Hq), 7.0, device=DEV)
     ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse, sm_scale=sm_scale, logit_cap=cap, max_seq_len=max(lens))
-    few = list(range(len(lens)))[:6]
-    check(cache, table, [lens[b] for b in few], q, o, lse, sm_scale, cap)
+    check(cache, table, lens, q, o, lse, sm_scale, cap, which=range(min(len(lens), 6)))
     assert torch.isfinite(o).all() and torch.isfinite(lse).all()
 
 
@@ -107,7 +118,6 @@ def test_values_of_every_size(form, o_dtype):
     D, H, Hq, lens = FORMS[form]
     if lens[0] > 5000:
         lens = [4500, 33]                         # still in pieces, two launches
-    few = list(range(len(lens)))[:4]
     gen = torch.Generator().manual_seed(151)
     k = torch.randn(sum(lens), H, D, generator=gen)
     v = torch.randn(sum(lens), H, D, generator=gen)
@@ -119,7 +129,7 @@ def test_values_of_every_size(form, o_dtype):
         for values in (v * size, torch.full_like(v, size), torch.full_like(v, -size)):
             cache, table, length, _ = cache_of(k.split(lens), values.split(lens))
             ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse, max_seq_len=max(lens))
-            check(cache, table, [lens[b] for b in few], q, o, lse)
+            check(cache, table, lens, q, o, lse, which=range(min(len(lens), 4)))
 
 
 @pytest.mark.parametrize("o_dtype", [torch.bfloat16, torch.float32])
@@ -139,3 +149,25 @@ def test_values_of_several_sizes_together(small, large, o_dtype):
             o, lse = torch.empty(4, 2, D, dtype=o_dtype, device=DEV), torch.empty(4, 2, device=DEV)
             ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse, max_seq_len=most)
             check(cache, table, lens, q, o, lse)
+
+
+# ---- a few tokens that outweigh all others ------------------------------------------------------------------------
+@pytest.mark.parametrize("o_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,H,B,n", [(128, 8, 80, 15001), (64, 1, 1, 6001), (128, 4, 1, 130), (128, 2, 1, 4001)])
+def test_tokens_far_below_the_heaviest_keep_their_bits(D, H, B, n, o_dtype):
+    """Four tokens weigh 2^12 to 2^24 times as much as each of the thousands behind them, which all have the same weight and value, so that what
+    is lost of one is lost of all; one group's values are 2^-10 of the others'.  The largest case has hundreds of records to a warp."""
+    gen = torch.Generator().manual_seed(161)
+    k, v = torch.zeros(n, H, D), torch.randn(1, H, D, generator=gen).repeat(n, 1, 1)
+    heavy = [0, 16, 32, 48]
+    k[heavy] = 1.0
+    v[heavy] = torch.randn(4, H, D, generator=gen)
+    v[..., 32:64] *= 2.0 ** -10
+    cache, table, _, _ = cache_of([k], [v])
+    table = table.expand(B, -1).contiguous()
+    length = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    powers = torch.tensor([12, 15, 16.3, 18.7, 20, 20.6, 22.2, 24])
+    q = (powers * math.log(2) / D ** 0.5).repeat(H)[None, :, None].expand(B, 8 * H, D).bfloat16().to(DEV)
+    o, lse = torch.empty(*q.shape, dtype=o_dtype, device=DEV), torch.empty(*q.shape[:2], device=DEV)
+    ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse)
+    check(cache, table, [n] * B, q, o, lse, which=sorted({0, B // 2, B - 1}))
