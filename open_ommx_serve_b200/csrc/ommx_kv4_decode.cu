@@ -200,9 +200,9 @@ __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int fir
     float x[8];
     if (warp < G) {
         load_q8(p, b * p.q_b + (first_head + min(g, n - 1)) * p.q_h + 32 * warp + 8 * t, x);
-        float top = fabsf(x[0]), sum = x[0];
+        float top = fabsf(x[0]), sum = 0x1p-8f * x[0];                      // 32 of the largest numbers would not have a finite sum
 #pragma unroll
-        for (int i = 1; i < 8; ++i) { top = fmaxf(top, fabsf(x[i])); sum += x[i]; }
+        for (int i = 1; i < 8; ++i) { top = fmaxf(top, fabsf(x[i])); sum += 0x1p-8f * x[i]; }
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
         sum += __shfl_xor_sync(~0u, sum, 1);
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
@@ -220,17 +220,18 @@ __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int fir
         for (int i = 0; i < 8; ++i) x[i] *= i & 1 ? up * 0.0625f : up;      // odd nibbles are 16 times as large
         m.frag[warp][lane] = make_uint4(half2_bits(x[0], x[4]), half2_bits(x[1], x[5]), half2_bits(x[2], x[6]), half2_bits(x[3], x[7]));
     }
-    const float factor = p.sm_scale * power_of_two(24 - 13 + e);
+    // two powers of two: one would pass 32 bits for |q| from 2^117 on
+    const float most = 3.4e38f, factor = fminf(fmaxf(p.sm_scale * 2048.0f * power_of_two(e), -most), most);         // 2^11: 24 - 13
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const float f = __shfl_sync(~0u, factor, 8 * t + 4 * i);
-        q.raw[i] = f / p.cap;
+        q.raw[i] = fminf(fmaxf(f / p.cap, -most), most);
         // never 0, so that a masked logit can be an infinity of the other sign: without a cap |x| < 2^124, and x times this is nothing
-        q.factor[i] = p.cap > 0.0f ? p.cap * LOG2E : f * LOG2E != 0.0f ? f * LOG2E : 0x1p-149f;
+        q.factor[i] = p.cap > 0.0f ? p.cap * LOG2E : f * LOG2E != 0.0f ? fminf(fmaxf(f * LOG2E, -most), most) : 0x1p-149f;
     }
     // rows of the product: term r of group j at G r + j; lane t holds rows 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
     const int j = G == 4 ? 2 * (t & 1) : 0;
-    const float a = m.sum[g][j] * (up * 0x1p-24f), c = m.sum[g][j + 1] * (up * 0x1p-24f);
+    const float a = m.sum[g][j] * (up * 0x1p-16f), c = m.sum[g][j + 1] * (up * 0x1p-16f);
     const float a1 = bf16_round_f32(a), c1 = bf16_round_f32(c), a2 = bf16_round_f32(a - a1), c2 = bf16_round_f32(c - c1);
     const uint32_t term1 = f32_to_bf16_bits(a1) | f32_to_bf16_bits(c1) << 16, term2 = f32_to_bf16_bits(a2) | f32_to_bf16_bits(c2) << 16,
                    term3 = f32_to_bf16_bits(a - a1 - a2) | f32_to_bf16_bits(c - c1 - c2) << 16;

@@ -171,3 +171,20 @@ def test_tokens_far_below_the_heaviest_keep_their_bits(D, H, B, n, o_dtype):
     o, lse = torch.empty(*q.shape, dtype=o_dtype, device=DEV), torch.empty(*q.shape[:2], device=DEV)
     ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse)
     check(cache, table, [n] * B, q, o, lse, which=sorted({0, B // 2, B - 1}))
+
+
+# ---- the size of the queries ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("D,lens", [(128, [40, 17]), (64, [3001])])
+@pytest.mark.parametrize("cap", [0.0, 3.0])
+def test_queries_of_every_size(D, lens, cap):
+    """Queries from 2^-110 to 2^119 against keys as small or large, constant in their groups, so that the logits are ordinary numbers."""
+    gen = torch.Generator().manual_seed(171)
+    n = sum(lens)
+    k = torch.randn(n, 2, D // 32, 1, generator=gen).expand(-1, -1, -1, 32).flatten(-2)
+    v, q0 = torch.randn(n, 2, D, generator=gen), torch.randn(len(lens), 4, D, generator=gen).clamp(-3, 3)
+    for e in (-110, -60, -14, 0, 60, 100, 110, 115, 117):
+        cache, table, length, _ = cache_of((k * 2.0 ** -e).split(lens), v.split(lens))
+        q = (q0 * 2.0 ** e).bfloat16().to(DEV)
+        o, lse = torch.empty(len(lens), 4, D, device=DEV), torch.empty(len(lens), 4, device=DEV)
+        ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse, logit_cap=cap)
+        check(cache, table, lens, q, o, lse, cap=cap)
