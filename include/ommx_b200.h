@@ -392,7 +392,8 @@ typedef struct ommx_kv4_append_args {
     int32_t num_rows;
     int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h;
     const int32_t *row_start;       /* [batch + 1]: rows row_start[b] .. row_start[b + 1] are the last tokens of sequence b; NULL: row b
-                                       is the last token of sequence b.  Rows behind row_start[batch] are left alone */
+                                       is the last token of sequence b.  Rows behind row_start[batch] are left alone; a range below
+                                       0, past num_rows or that ends before it begins is a bad one (OMMX_ST_BAD_LENGTH) */
     const void *q;                  /* [num_rows, n_q_heads, head_dim] to be rotated into q_out, or NULL; q_out may be q */
     void *q_out;
     int32_t n_q_heads;

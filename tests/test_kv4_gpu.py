@@ -652,3 +652,41 @@ def test_calls_behind_one_another_on_their_own_stream():
         fast = run(False)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(slow, fast))
+
+
+@pytest.mark.parametrize("B", [2, 70])
+def test_bad_row_ranges_are_reported_and_their_sequences_skipped(B):
+    """A range below 0, past the rows, or that ends before it begins: nothing of its sequence is stored, rotated or read, the others' is."""
+    H, D, page, T = 2, 64, 16, 2 * B
+    lens = [40 + b for b in range(B)]
+    cache, table, length = filled(lens, H, D, page, seed=141)
+    gen = torch.Generator().manual_seed(142)
+    k, v, q = (torch.randn(T, n, D, generator=gen).bfloat16().to(DEV) for n in (H, H, 4))
+    cos, sin = (x.to(DEV) for x in angles(200, D))
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    good = [2 * b for b in range(B + 1)]
+    for start, wrong in (([-2] + good[1:], [0]), (good[:-1] + [T + 1], [B - 1]), (good[:-1] + [T - 4], [B - 1]), ([T + 7] * (B + 1), list(range(B))),
+                         (good[:-1] + [2 ** 31 - 1], [B - 1]), ([-2 ** 31] + good[1:], [0])):
+        start = torch.tensor(start, dtype=torch.int32, device=DEV)
+        rec, summ, q_out = cache["records"].clone(), cache["summary"].clone(), torch.full_like(q, 5.0)
+        want, w_summ, w_out = rec.clone(), summ.clone(), q_out.clone()
+        status.zero_()
+        ommx_kv4_append(k, v, rec, table, length, row_start=start, q=q, q_out=q_out, cos=cos, sin=sin, summary=summ, status=status)
+        assert int(status) == _lib.ST_BAD_LENGTH
+        ko, vo = torch.full((T, H, D), 2.0, device=DEV), torch.full((T, H, D), 2.0, device=DEV)
+        status.zero_()
+        ommx_kv4_gather(rec, table, length, ko, vo, row_start=start, status=status)
+        assert int(status) == _lib.ST_BAD_LENGTH
+        for b in range(B):                        # each good sequence by a call of its own
+            if b in wrong:
+                continue
+            mine = slice(2 * b, 2 * b + 2)
+            two = torch.tensor([0, 2], dtype=torch.int32, device=DEV)
+            ommx_kv4_append(k[mine], v[mine], want, table[b:b + 1], length[b:b + 1], row_start=two, q=q[mine], q_out=w_out[mine], cos=cos, sin=sin, summary=w_summ)
+            wk, wv = ref.sequence(want, table[b], lens[b])
+            assert torch.equal(ko[mine], wk[:, -2:].transpose(0, 1).float()) and torch.equal(vo[mine], wv[:, -2:].transpose(0, 1).float())
+        assert torch.equal(rec, want) and torch.equal(summ, w_summ) and torch.equal(q_out, w_out)
+        rows = torch.zeros(T, dtype=torch.bool, device=DEV)
+        for b in wrong:
+            rows[2 * b:2 * b + 2] = True
+        assert bool((ko[rows] == 2).all()) and bool((vo[rows] == 2).all())
