@@ -65,7 +65,8 @@ def ommx_kv4_append(k_new: torch.Tensor, v_new: torch.Tensor, records: torch.Ten
     ``k_new`` / ``v_new`` ``[rows, n_kv_heads, D]`` and ``q`` ``[rows, n_q_heads, D]`` in bf16, fp16 or fp32, any strides with a
     contiguous last dimension (slices of one projection's output).  ``b_seq_len`` (int32) counts the new rows: rows
     ``row_start[b] .. row_start[b + 1]`` (int32 ``[batch + 1]``) are the last tokens of sequence ``b``, without it row ``b`` is.
-    Rows behind ``row_start[-1]`` (a padded batch) are left alone, those of ``q_out`` too.  ``page_table`` (int32 or int64
+    Rows behind ``row_start[-1]`` (a padded batch) are left alone, those of ``q_out`` too.  A range that is none of the
+    rows (below 0, past them, ending before it begins) is reported and its sequence skipped.  ``page_table`` (int32 or int64
     ``[batch, pages]``) gives the page of every ``page_size`` tokens; a page that takes rows belongs to one sequence.
 
     ``cos`` / ``sin`` fp32 ``[positions, rot_dim / 2]`` turn the first ``rot_dim`` (32, 64, 128) channels, pairs

@@ -690,3 +690,67 @@ def test_bad_row_ranges_are_reported_and_their_sequences_skipped(B):
         for b in wrong:
             rows[2 * b:2 * b + 2] = True
         assert bool((ko[rows] == 2).all()) and bool((vo[rows] == 2).all())
+
+
+@pytest.mark.parametrize("B,H,group,longest", [(8, 8, 4, 6000), (1, 2, 4, 30000), (3, 4, 2, 700)])
+def test_lengths_that_change_between_calls_that_overlap(B, H, group, longest):
+    """Steps of a length update, an append, a selection and attention in three forms, each begun while the one before still runs and each with
+    outputs of its own: what the later kernels read before they wait is what the step wrote.  Lengths jump, so the deal of records to blocks
+    does too; the first two cases take the second kernel (64 rows of parts, and two)."""
+    D, page, steps = 128, 32, 10
+    cache, table, _ = filled([longest] * B, H, D, page, seed=151)
+    gen = torch.Generator().manual_seed(152)
+    lens = [torch.randint(1, longest + 1, (B,), generator=gen, dtype=torch.int32) for _ in range(steps)]
+    lens[1][:], lens[2][:] = 1, longest
+    lens = [n.to(DEV) for n in lens]
+    rows = [torch.randn(B, (group + 2) * H, D, generator=gen).bfloat16().to(DEV) for _ in range(steps)]
+    cos, sin = (x.to(DEV) for x in angles(longest, D))
+    Hq = group * H
+
+    def run(wait):
+        c = {k: v.clone() for k, v in cache.items()}
+        n = torch.zeros(B, dtype=torch.int32, device=DEV)
+        out = []
+        for x, now in zip(rows, lens):
+            q, sel = torch.empty(B, Hq, D, dtype=torch.bfloat16, device=DEV), torch.empty(B, H, 5, dtype=torch.int32, device=DEV)
+            o, lse = [torch.full((B, Hq, D), 7.0, device=DEV) for _ in range(3)], [torch.full((B, Hq), 7.0, device=DEV) for _ in range(3)]
+            for call in (lambda: n.copy_(now),
+                         lambda: ommx_kv4_append(x[:, Hq:Hq + H], x[:, Hq + H:], c["records"], table, n, q=x[:, :Hq], q_out=q, cos=cos, sin=sin, summary=c["summary"]),
+                         lambda: ommx_kv4_decode_attention(q, c["records"], table, n, o[0], lse[0]),
+                         lambda: ommx_kv4_select_pages(q, c["summary"], table, n, sel, page_size=page),
+                         lambda: ommx_kv4_decode_attention(q, c["records"], table, n, o[1], lse[1], selected=sel),
+                         lambda: ommx_kv4_decode_attention(q, c["records"], table, n, o[2], lse[2], max_seq_len=1)):
+                call()
+                if wait:
+                    torch.cuda.synchronize()
+            out += [q, sel, *o, *lse]
+        return [c["records"], c["summary"]] + out, c
+
+    slow, c = run(True)
+    check_attention(c, table, lens[-1].tolist(), slow[-8], slow[-6], slow[-3])
+    check_attention(c, table, lens[-1].tolist(), slow[-8], slow[-5], slow[-2], selected=slow[-7])
+    check_attention(c, table, lens[-1].tolist(), slow[-8], slow[-4], slow[-1])
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        for _ in range(3):
+            fast, _ = run(False)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(slow, fast))
+
+
+def test_rows_read_back_with_ranges_in_order_and_out():
+    """The clamped form's neighbours: of ranges in and out of order in one call, the good ones' rows come back, the others' stay as they were."""
+    lens, H, D, page = [40, 50, 60], 1, 64, 16
+    cache, table, length = filled(lens, H, D, page, seed=161)
+    wants = [ref.sequence(cache["records"], table[b], lens[b]) for b in range(3)]
+    for start, good in (([-1, 2, 1, 4], [2]), ([2, 0, 3, 3], [1]), ([0, 1, 4, 9], [0, 1])):
+        ko, vo = torch.full((4, H, D), 2.0, device=DEV), torch.full((4, H, D), 3.0, device=DEV)
+        wk, wv = ko.clone(), vo.clone()
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        ommx_kv4_gather(cache["records"], table, length, ko, vo, row_start=torch.tensor(start, dtype=torch.int32, device=DEV), status=status)
+        for b in good:
+            n = start[b + 1] - start[b]
+            for to, want in ((wk, wants[b][0]), (wv, wants[b][1])):
+                to[start[b]:start[b + 1]] = want[:, lens[b] - n:].transpose(0, 1).float()
+        assert torch.equal(ko, wk) and torch.equal(vo, wv) and int(status) == _lib.ST_BAD_LENGTH

@@ -188,3 +188,23 @@ def test_queries_of_every_size(D, lens, cap):
         o, lse = torch.empty(len(lens), 4, D, device=DEV), torch.empty(len(lens), 4, device=DEV)
         ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse, logit_cap=cap)
         check(cache, table, lens, q, o, lse, cap=cap)
+
+
+# ---- weights and values that grow along a sequence -----------------------------------------------------------------
+@pytest.mark.parametrize("o_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("H,n", [(1, 2000), (4, 250), (2, 9000)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_small_values_that_hold_all_the_weight(H, n, o_dtype, sign):
+    """Values grow by 2^30 along the sequence and the weights with them, or against them: then the output is of the size of the first values,
+    some 1e-6, beside last ones of 1e3, and is held to its own size."""
+    D = 128
+    gen = torch.Generator().manual_seed(181)
+    k = 0.1 * torch.randn(n, H, D, generator=gen) + torch.linspace(-4, 4, n)[:, None, None]
+    v = torch.randn(n, H, D, generator=gen) * torch.logspace(-6, 3, n)[:, None, None]
+    cache, table, length, lens = cache_of([k.bfloat16()], [v.bfloat16()])
+    q = (sign * (1 + 0.1 * torch.randn(1, 4 * H, D, generator=gen))).bfloat16().to(DEV)
+    o, lse = torch.empty(1, 4 * H, D, dtype=o_dtype, device=DEV), torch.empty(1, 4 * H, device=DEV)
+    ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse)
+    check(cache, table, lens, q, o, lse)
+    for h, (wo, _, off, _) in enumerate(expected(q[0], cache["records"], table[0], n, D ** -0.5, 0.0, o_dtype)):
+        assert float(off.max()) < 0.5 * float(wo.abs().max()), h             # of the bound itself: an output of zeros would not pass
