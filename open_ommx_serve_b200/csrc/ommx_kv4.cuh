@@ -76,6 +76,24 @@ __device__ __forceinline__ int warp_inclusive_scan(int v, int lane) {
     return v;
 }
 
+// eight channels of a query; P: parameters with q, whether it is fp16 (else bf16) and whether all rows start on 16-byte boundaries
+template <typename P> __device__ __forceinline__ void load_q8(const P &p, int64_t at, float *x) {
+    alignas(16) uint16_t v[8];
+    if (p.q_wide) {
+        *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p.q) + at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = reinterpret_cast<const uint16_t *>(p.q)[at + i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p.q16 ? __half2float(__ushort_as_half(v[i])) : __uint_as_float((uint32_t)v[i] << 16);
+}
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 // Rows of a call that belong to a sequence: [first, end) of the row tensors; the sequence's last rows, in order.
 struct Rows {
     const int32_t *row_start;                     // [B + 1], or null: row b is sequence b's

@@ -54,7 +54,7 @@ struct DecodeParams {
     float *lse, *work;
     const int32_t *selected;
     int64_t q_b, q_h, o_b, o_h, lse_b;
-    int32_t q16, q_wide, o_type, Hq, group, col_blocks, num_selected, page_shift, least, whole;
+    int32_t q16, q_wide, o_type, group, col_blocks, num_selected, page_shift, least, whole;
     float sm_scale, cap;
     int32_t *status;
 };
@@ -164,18 +164,6 @@ __device__ __forceinline__ float log_sum(float ref, float sum) {
     return sum != 0.0f ? ((ref - ABOVE) + log2f(sum * power_of_two(ABOVE))) * LN2 : -INFINITY;
 }
 
-// eight channels of a query
-__device__ __forceinline__ void load_q8(const DecodeParams &p, int64_t at, float *x) {
-    alignas(16) uint16_t v[8];
-    if (p.q_wide) {
-        *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p.q) + at);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = reinterpret_cast<const uint16_t *>(p.q)[at + i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = p.q16 ? __half2float(__ushort_as_half(v[i])) : __uint_as_float((uint32_t)v[i] << 16);
-}
 __device__ __forceinline__ void store_o(const DecodeParams &p, int64_t at, float v) {
     if (p.o_type == OMMX_DT_F32) reinterpret_cast<float *>(p.o)[at] = v;
     else if (p.o_type == OMMX_DT_F16) reinterpret_cast<__half *>(p.o)[at] = __float2half_rn(v);
@@ -525,7 +513,8 @@ template <int G, int NW> struct Memory {
         Shared<G, NW> sh;
         uint8_t ring[NW][STAGES][Rec<G>::BYTES];
     };
-    // two blocks (of four warps, four) have to stay below 196 KB: the first-level cache is halved past that, and 64K tokens took 1 us more
+    // two blocks of eight warps stay below 196 KB, past which the first-level cache is halved (64K tokens took 1 us more); four blocks of four
+    // warps are 2 KB over, and take the smaller cache
     union {
         float whole[NW][8 * G][32];
         alignas(16) float merged[PART<G>];        // of this block, where a cluster shares a row; its warps have taken theirs back
@@ -533,6 +522,7 @@ template <int G, int NW> struct Memory {
     QueryMemory<G> query;
     float ref[COLS][NW], sum[COLS][NW];
 };
+static_assert(2 * (sizeof(Memory<4, 8>) + 1024) <= 196 * 1024, "1 KB of each block is the system's");
 
 __device__ __forceinline__ bool too_many(const DecodeParams &p, uint32_t units, uint32_t rows) {
     const bool over = (uint64_t)units * rows >> 31;
@@ -779,7 +769,7 @@ __device__ __forceinline__ Parts parts_of(const DecodeParams &p, int b, uint32_t
         const uint32_t r0 = before + row * units;
         r.first = r0 / d.x;
         r.count = (r0 + units - 1) / d.x - r.first + 1;
-        r.late = r0 >= r.first * d.x;
+        r.late = true;                            // the first part's block is the one that holds the row's first unit
     }
     return r;
 }
@@ -972,7 +962,7 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     p.lse = a->lse; p.lse_b = a->lse_stride_b;
     p.work = a->workspace;
     p.selected = a->selected; p.num_selected = a->num_selected;
-    p.Hq = a->n_q_heads; p.group = a->n_q_heads / p.c.H; p.col_blocks = (p.group + COLS - 1) / COLS;
+    p.group = a->n_q_heads / p.c.H; p.col_blocks = (p.group + COLS - 1) / COLS;
     p.page_shift = shift_of(p.c.page);
     p.sm_scale = a->sm_scale; p.cap = a->logit_cap; p.status = a->status;
     if (p.c.num_pages == 0) return fail(OMMX_E_ARG, "kv4_decode: a cache of no pages");   // what is fetched for a page that is not there

@@ -36,26 +36,9 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t b = __float_as_uint(x);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-// eight channels of a query
-__device__ __forceinline__ void load_q8(const SelectParams &p, int64_t at, float *x) {
-    alignas(16) uint16_t v[8];
-    if (p.q_wide) {
-        *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p.q) + at);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = reinterpret_cast<const uint16_t *>(p.q)[at + i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = p.q16 ? __half2float(__ushort_as_half(v[i])) : __uint_as_float((uint32_t)v[i] << 16);
-}
 __device__ __forceinline__ void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
 }
 __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t r;

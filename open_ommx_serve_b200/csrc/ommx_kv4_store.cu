@@ -168,11 +168,6 @@ __device__ __forceinline__ uint32_t quantize_group(float (&x)[8], uint32_t *para
 }
 
 // Summary: two bf16 in a register, maxima in the first half of the array and negated minima in the second, so both grow
-__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 constexpr uint32_t NOTHING = 0xFF80FF80u;                                  // -inf twice
 
 // One warp appends up to 16 rows that share a record, ROWS of them at a time: lane ((row, j), t) has channels 32 j + 8 t + 0..7, so a
