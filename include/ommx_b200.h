@@ -444,7 +444,8 @@ typedef struct ommx_kv4_decode_args {
     int64_t workspace_floats;
     int32_t max_seq_len;            /* an upper bound of b_seq_len that sizes the grid, 0: what the table can hold */
     float sm_scale, logit_cap;      /* logits: cap * tanh(q.k * sm_scale / cap); cap 0: none. sm_scale: any finite number, 0 and below too; the
-                                       largest |q| * |sm_scale| * 4096 must be finite in 32 bits */
+                                       largest |q| * |sm_scale| * 4096 must be finite in 32 bits.  Logits are served up to 2^29
+                                       in size: past that 32-bit numbers are over 100 apart */
     int32_t *status;
 } ommx_kv4_decode_args;
 

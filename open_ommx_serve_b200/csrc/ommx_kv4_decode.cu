@@ -39,7 +39,7 @@ constexpr int COLS = 8;                           // query heads side by side
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // Weights w = 2^(x - ref) are held near 2^-ABOVE: they meet zeros of up to 2^126, and a sum of 2^24 such products at HEAVY stays below 2^127.
 // Products of weights and scales, w s unit, go to fp16: the largest one lies above 2^(TOP - 2) when the references have moved, and may grow to ROOM
-// before they move again. More of fp16's range below it would cost moves (TOP 8, 11, 12: 8 x 64K tokens 137.9, 138.6, 139.3 us).
+// before they move again. More of fp16's range below it would cost moves (8 x 64K tokens 137.9 us with TOP 8, 139.3 with 12).
 constexpr int ABOVE = 30, TOP = 11;
 constexpr float HEAVY = 0x1p-23f, ROOM = 60000.0f;
 constexpr float LOWEST = -1e30f;
@@ -264,12 +264,13 @@ template <int G> __device__ __forceinline__ void clear(State<G> &s, float *whole
     s.ref[0] = s.ref[1] = LOWEST;
     s.unit[0] = s.unit[1] = 1.0f;
 }
-// The references of head i move: to whole numbers, so that nothing is rounded. `logit`: the record's largest; `product`: that of logits and
-// their scales' exponents. A unit stays within normal numbers: where scales are the smallest (2^-96), products stay below 2^TOP.
-template <int G> __device__ __forceinline__ void move(State<G> &s, int i, float logit, float product) {
+// The references of head i move to `ref`, a whole number as the one before, so that nothing is rounded. `product`: the record's largest logit
+// plus exponent of its scales, less `ref` (logits may be so large that an exponent added to one is lost). A unit stays within normal
+// numbers: where scales are the smallest (2^-96), products stay below 2^TOP. The largest logit less `ref` is off by half a step of `ref`, 32 at
+// 2^30: up to there a weight is a finite number whatever that is.
+template <int G> __device__ __forceinline__ void move(State<G> &s, int i, float ref, float product) {
     const int was = exponent_of(s.unit[i]);
-    const float ref = fmaxf(s.ref[i], ceilf(logit) + ABOVE);
-    const float over = ceilf(fmaxf(s.ref[i] + (float)(TOP - was), product) - ref);         // 2^over: the largest product
+    const float over = ceilf(fmaxf((s.ref[i] - ref) + (float)(TOP - was), product));       // 2^over: the largest product
     const int now = TOP - (int)fminf(fmaxf(over, (float)(TOP - 126)), (float)(TOP + 126));
     const float f = exp2_approx(s.ref[i] - ref), a = exp2_approx(s.ref[i] - ref + (float)(now - was));
     s.ref[i] = ref;
@@ -386,13 +387,14 @@ template <int G, bool FINE> __device__ __forceinline__ void attend(const DecodeP
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const float f = i ? f1 : f0;
-            float l = fmaxf(x[i] * f, x[i + 2] * f), r = fmaxf(fmaf(x[i], f, e0), fmaf(x[i + 2], f, e1));
+            float l = fmaxf(x[i] * f, x[i + 2] * f);
 #pragma unroll
-            for (int d = 4; d < 32; d *= 2) {
-                l = fmaxf(l, __shfl_xor_sync(~0u, l, d));
-                r = fmaxf(r, __shfl_xor_sync(~0u, r, d));
-            }
-            move(s, i, l, r);
+            for (int d = 4; d < 32; d *= 2) l = fmaxf(l, __shfl_xor_sync(~0u, l, d));
+            const float ref = fmaxf(s.ref[i], ceilf(l) + ABOVE);
+            float r = fmaxf(fmaf(x[i], f, -ref) + e0, fmaf(x[i + 2], f, -ref) + e1);
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) r = fmaxf(r, __shfl_xor_sync(~0u, r, d));
+            move(s, i, ref, r);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) { w[i] = exp2_approx(fmaf(x[i], i & 1 ? f1 : f0, -s.ref[i & 1])); y[i] = w[i] * s.unit[i & 1]; }

@@ -208,3 +208,30 @@ def test_small_values_that_hold_all_the_weight(H, n, o_dtype, sign):
     check(cache, table, lens, q, o, lse)
     for h, (wo, _, off, _) in enumerate(expected(q[0], cache["records"], table[0], n, D ** -0.5, 0.0, o_dtype)):
         assert float(off.max()) < 0.5 * float(wo.abs().max()), h             # of the bound itself: an output of zeros would not pass
+
+
+# ---- the size of the logits ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("D,H,lens", [(128, 2, [1, 17, 250]), (64, 2, [4001]), (128, 1, [9000])])
+@pytest.mark.parametrize("power", [10, 20, 24, 27])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_logits_of_every_size(D, H, lens, power, sign):
+    """Logits of sign * 2^power * 1..4, exact in 32 bits, and values of 3e4: the output is the mean over the tokens of the largest logit.  In
+    bf16 that is 2^-9 of itself off; the weights alike, products of codes off by 2^-11 and 2^-15 of a group's range R (2^-10 in all)."""
+    gen = torch.Generator().manual_seed(191)
+    n = sum(lens)
+    steps = torch.randint(1, 5, (n, H, 1), generator=gen).float()
+    k, v = steps.expand(n, H, D), 3e4 * torch.randn(n, H, D, generator=gen)
+    cache, table, length, _ = cache_of(k.split(lens), v.split(lens))
+    q = torch.ones(len(lens), 3 * H, D, dtype=torch.bfloat16, device=DEV)
+    o, lse = torch.empty(len(lens), 3 * H, D, dtype=torch.bfloat16, device=DEV), torch.empty(len(lens), 3 * H, device=DEV)
+    ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse, sm_scale=sign * 2.0 ** power / D, max_seq_len=max(lens))
+    for b, rows in enumerate(steps.split(lens)):
+        _, cached = ref.sequence(cache["records"], table[b], lens[b])
+        for h in range(3 * H):
+            score = sign * rows[:, h // 3, 0].double().to(DEV)
+            best = cached[h // 3][score == score.max()]
+            want, size = best.mean(0), float(best.abs().max())
+            R = float((best.unflatten(-1, (-1, 32)).amax(-1) - best.unflatten(-1, (-1, 32)).amin(-1)).max())
+            assert float((o[b, h].double() - want).abs().max()) <= 2.0 ** -9 * size + 2.0 ** -10 * R
+            top = float(score.max()) * 2.0 ** power
+            assert abs(float(lse[b, h]) - top) <= math.log(len(best)) + 1e-3 + 2.0 ** -22 * abs(top)
