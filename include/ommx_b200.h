@@ -475,7 +475,7 @@ typedef struct ommx_kv4_select_args {
  * The num_selected pages of each sequence and kv head whose keys can meet its query heads best.  A page's score is the largest, over
  * the query heads, of sum_c max(q_c M_c, q_c m_c) with its maxima M and minima m, in whole numbers: q * 2^(6 - e) rounded to
  * +-127 (2^e the leading power of the kv head's largest |q|), M and m * (63/64) 2^(5 - f) rounded (2^f that of the page's
- * largest), times 2^f.  No rounding depends on an order, so neither does the choice; ties go to the lower page.
+ * largest, f at least -100), times 2^f.  No rounding depends on an order, so neither does the choice; ties go to the lower page.
  */
 int ommx_b200_kv4_select(const ommx_kv4_select_args *args, void *stream);
 int64_t ommx_b200_kv4_select_workspace_bytes(int32_t batch, int32_t n_kv_heads, int32_t pages_per_seq);

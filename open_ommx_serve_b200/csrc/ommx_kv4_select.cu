@@ -72,8 +72,9 @@ template <int G> __device__ __forceinline__ void quantize_query(const SelectPara
     most = __reduce_max_sync(~0u, most);
     if ((threadIdx.x & 31) == 0) atomicMax(top, most);
     __syncthreads();
-    const float largest = __uint_as_float(*top);
-    const int e = (int)(*top >> 23) - 127;                                  // q of subnormal size: all 0 either way
+    const float pre = *top < 0x0D800000u ? 0x1p64f : 1.0f;                  // below 2^-100: 2^(6 - e) would pass 32 bits, or e is not in a subnormal's exponent
+    const float largest = __uint_as_float(*top) * pre;
+    const int e = (int)(__float_as_uint(largest) >> 23) - 127;
     const float up = largest > 0.0f ? __uint_as_float((uint32_t)min(max(6 - e + 127, 1), 254) << 23) : 0.0f;
     for (int i = threadIdx.x; i < chunks; i += THREADS) {
         if (chunks > THREADS) load_q8(p, at + (int64_t)(i / CHUNKS) * p.q_h + i % CHUNKS * 8, x);
@@ -81,7 +82,7 @@ template <int G> __device__ __forceinline__ void quantize_query(const SelectPara
         int sum = 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const int v = max(-127, min(127, __float2int_rn(x[k] * up)));
+            const int v = max(-127, min(127, __float2int_rn(x[k] * pre * up)));
             sum += v;
             plus[k >> 2] |= (uint32_t)max(v, 0) << (8 * (k & 3));
             minus[k >> 2] |= ((uint32_t)min(v, 0) & 255u) << (8 * (k & 3));

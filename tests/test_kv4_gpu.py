@@ -754,3 +754,21 @@ def test_rows_read_back_with_ranges_in_order_and_out():
             for to, want in ((wk, wants[b][0]), (wv, wants[b][1])):
                 to[start[b]:start[b + 1]] = want[:, lens[b] - n:].transpose(0, 1).float()
         assert torch.equal(ko, wk) and torch.equal(vo, wv) and int(status) == _lib.ST_BAD_LENGTH
+
+
+@pytest.mark.parametrize("shift", [-132, -125, -110, -60, 0, 60, 120])
+def test_selection_does_not_depend_on_the_size_of_the_queries(shift):
+    """The same queries, and keys, times a power of two: the same pages, down to the smallest numbers of bf16."""
+    lens, H, D, page, n = [1500], 2, 64, 16, 9
+    cache, table, length = filled(lens, H, D, page, seed=171)
+    q = torch.randint(-1, 3, (1, 6, D), generator=torch.Generator().manual_seed(172)).double()
+    want = ref.select(q[0], cache["summary"].cpu(), table[0].cpu(), lens[0], page, n, 1, 2)
+    sel = torch.empty(1, H, n, dtype=torch.int32, device=DEV)
+    scaled = (q * 2.0 ** shift).bfloat16().to(DEV)
+    assert torch.equal(scaled.cpu().double(), q * 2.0 ** shift)
+    ommx_kv4_select_pages(scaled, cache["summary"], table, length, sel, page_size=page)
+    assert sel[0].tolist() == want
+    if -90 < shift < 100:
+        summary = (cache["summary"].double() * 2.0 ** shift).bfloat16()
+        ommx_kv4_select_pages(q.bfloat16().to(DEV), summary, table, length, sel, page_size=page)
+        assert sel[0].tolist() == want
