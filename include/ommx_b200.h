@@ -449,8 +449,10 @@ typedef struct ommx_kv4_decode_args {
     int32_t *status;
 } ommx_kv4_decode_args;
 
-/* Attention of one query row per sequence over the cache, or over selected pages of it.  Two launches; one where no sequence has
- * more than 512 tokens by max_seq_len, the table's width or num_selected. */
+/* Attention of one query row per sequence over the cache, or over selected pages of it.  A kv head's records are read once for each
+ * eight of its query heads.  Two launches; one where no sequence has more than 512 tokens by max_seq_len, the table's width or
+ * num_selected, or, where rows (sequences x kv heads x eights of query heads) are few enough for clusters, 4096.  A workspace is asked for by
+ * the first of these limits alone, so that its size does not depend on the batch: calls in clusters do not write to it. */
 int ommx_b200_kv4_decode(const ommx_kv4_decode_args *args, void *stream);
 /* floats of workspace that this call needs on the current device (0: none; its pointers are not looked at), and that any call needs */
 int64_t ommx_b200_kv4_decode_workspace_floats(const ommx_kv4_decode_args *args);

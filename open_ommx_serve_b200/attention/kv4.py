@@ -95,12 +95,14 @@ def ommx_kv4_decode_attention(q: torch.Tensor, records: torch.Tensor, page_table
                               max_seq_len: Optional[int] = None, status: Optional[torch.Tensor] = None) -> None:
     """Attention of one (rotated) query row per sequence, written to ``o`` ``[batch, n_q_heads, D]`` and ``lse`` (fp32).
 
-    ``q`` bf16 or fp16, ``o`` bf16, fp16 or fp32; any number of query heads to a kv head.  ``sm_scale`` defaults to
-    ``D ** -0.5`` and may be any finite number; ``logit_cap`` c makes a logit ``c tanh(x / c)``.  A sequence of no tokens gives ``o = 0``, ``lse = -inf``.
+    ``q`` bf16 or fp16, ``o`` bf16, fp16 or fp32; any number of query heads to a kv head, whose cache is read once for each eight of
+    them.  ``sm_scale`` defaults to ``D ** -0.5`` and may be any finite number; ``logit_cap`` c makes a logit ``c tanh(x / c)``.  A
+    sequence of no tokens gives ``o = 0``, ``lse = -inf``.
     ``selected`` (int32 ``[batch, n_kv_heads, n]``, as ``ommx_kv4_select_pages`` writes it) limits a kv head to these places of
     the page table; the first ``min(n, pages)`` entries count, one below 0 is passed over, one listed twice counts twice.
-    ``max_seq_len`` sizes the grid (the table's width without it; up to 512 tokens it is one launch); ``workspace`` (fp32,
-    ``kv4_workspace_floats(D)`` values) is allocated per call when needed and not given; calls that run side by side need their own."""
+    ``max_seq_len`` sizes the grid (the table's width without it; up to 512 tokens, and up to 4096 where sequences and heads are few, it
+    is one launch); ``workspace`` (fp32, ``kv4_workspace_floats(D)`` values) is allocated per call when that may be more than 512 and
+    none is given; calls that run side by side need their own."""
     _check((_HOST or _host()).kv4_decode(q, records, page_table, b_seq_len, o, lse, sm_scale, logit_cap, selected, workspace, max_seq_len, status),
            "ommx_b200_kv4_decode")
 
@@ -112,8 +114,8 @@ def ommx_kv4_select_pages(q: torch.Tensor, summary: torch.Tensor, page_table: to
     places in the page table, ascending, then -1.
 
     All pages where there are at most ``n``; else the first ``first_pages``, the last ``last_pages`` and those of the largest
-    score: a bound of ``q . k`` over the page's keys from its channel maxima and minima, the largest over the kv head's query
-    heads.  Scores are whole numbers (``include/ommx_b200.h``), equal ones go to the lower page: the choice is the same
+    score: an estimate of the largest ``q . k`` of the page's keys from its channel maxima and minima in 7 bits and ``q`` in 8, the
+    largest over the kv head's query heads.  Scores are whole numbers (``include/ommx_b200.h``), equal ones go to the lower page: the choice is the same
     however it is computed.  ``workspace``: uint8, ``kv4_select_workspace_bytes(batch, n_kv_heads, pages)``."""
     _check((_HOST or _host()).kv4_select(q, summary, page_table, b_seq_len, selected, page_size, first_pages, last_pages, workspace, status),
            "ommx_b200_kv4_select")

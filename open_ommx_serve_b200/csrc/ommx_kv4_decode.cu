@@ -11,19 +11,21 @@
 // A weight w_t = exp(x_t) stays fp32 where it meets a zero and in the sum, against a reference of the logits alone: values of any size the
 // cache holds leave no token out. Products w_t s_tj are rounded to fp16, by 2^-11 at most, in a unit that the largest of them sets: below
 // 2^-23 of it they have fewer bits (fp16's smallest step is 2^-24), and are off by 2^-34 of it at most. That is less than a bf16 output's own
-// rounding; where the output is finer (fp16, fp32), a second product takes what the rounding left (FINE: 32 ragged sequences 57 us
-// without, 64 with). Sums of weights and zeros stay fp32.
+// rounding; where the output is finer (fp16, fp32), a second product takes what the rounding left (FINE: 32 ragged sequences 58 us
+// without, 66 with; 8 x 64K tokens 139 and 165). Sums of weights and zeros stay fp32.
 //
 // What the tensor cores cut is then the largest error of a record: they line the addends of a product up with the largest and cut them 25 bits
-// below its leading one (an emulation of that gives the kernel's errors), where a subnormal counts as 2^-14. A masked nibble lies 10 bits
+// below its leading one (an emulation of that gives the kernel's errors to a fifth), where a subnormal counts as 2^-14. A masked nibble lies 10 bits
 // below that (the odd ones, 16 times as large, 6), so an addend loses up to 2^-15 of one code of the record's heaviest token - or, in a
 // logit, of the group's largest |q| -: 2^-15 of a group's range a record at most, of the heaviest token's share in the output. Nibbles
 // moved up to bits 6..9 would lose 2^-21, for some 48 shifts a record.
 //
-// What bounds it: a record's 160 bytes a token are read once, so HBM, and beside it the schedulers: a record is some 320 instructions
-// of a warp, 17 of them products that hold a scheduler 8 cycles, in which its multiply-adds wait. 8 x 64K tokens, 8 kv heads, 32
-// query heads: 136 us (4.9 TB/s, 75 % of the copy rate); 110 with the copies left out, 112 with the arithmetic left out. e4m3 products
-// for K (half the masks, twice the depth) were slower, 173: their operands are converted.
+// What bounds it: a record's 160 bytes a token are read once for each eight query heads of its kv head, so HBM, and beside it the schedulers:
+// a record is some 330 instructions of a warp, 17 of them products that hold a scheduler 8 cycles, in which its multiply-adds wait. 8 x 64K
+// tokens, 8 kv heads, 32 or 64 query heads: 139 us (4.8 TB/s, 74 % of the copy rate), 260 with 128 heads; an earlier form of 136 us took 110
+// with the copies left out, 112 with the arithmetic left out. e4m3 products for K (half the masks, twice the depth) were slower, 173: their
+// operands are converted. The D = 128 forms spill a few registers, outside the loop over records: 33 loads and stores of a warp in 2 x 64K
+// tokens, of 10 thousand instructions.
 #include <cmath>
 #include <type_traits>
 
@@ -241,7 +243,8 @@ __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int fir
 // A warp's running state. acc[j][u]: 2^-24 channel 32 j + 4 g + 2 u (rows g), 2^-20 the next one (rows g + 8); heads 2 t, 2 t + 1.
 // The tensor cores cut what they add to a sum, so long sums of codes, none of them negative, fall short: by some 2^-26 of the sum a
 // record, which is much of an output that the zeros nearly cancel (8e-4 of it after 110 records of 64K tokens that weigh alike). So
-// `acc` is added to `whole` in shared memory every 64 records, every 32 where the output is finer than bf16 (2 % of the time).
+// `acc` is added to `whole` in shared memory every 64 records, every 32 where the output is finer than bf16 and a record
+// is two products (2 % of the time).
 template <int G> struct State {
     float acc[G][2][4], zero[G][2], sum[2], ref[2];
     float unit[2];                                // a power of two that only `acc` has in it

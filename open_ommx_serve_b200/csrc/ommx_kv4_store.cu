@@ -173,8 +173,9 @@ constexpr uint32_t NOTHING = 0xFF80FF80u;                                  // -i
 // One warp appends up to 16 rows that share a record, ROWS of them at a time: lane ((row, j), t) has channels 32 j + 8 t + 0..7, so a
 // group's extremes meet in two shuffles. A key's partners in the rotation are loaded too (from the first-level cache), not exchanged.
 // Bounds: a row of K and V is 512 bytes in and 160 out at D = 128, and some 285 instructions of a warp: 8192 rows x 8 heads take 24 us
-// (64 % of the issue slots) where their bytes take 7, one row 4.0. Eight rows at a time with all groups to a lane (127 registers)
-// took 22, and 7.0 for one row; the next rows' loads ahead of these rows' work 25.5 (96 registers, fewer warps).
+// (64 % of the issue slots; fp32 rows 35) where their bytes take 7 (12), one row 4.0. Eight rows at a time with all groups to a lane (127 registers)
+// took 22, and 7.0 for one row; the next rows' loads ahead of these rows' work 25.5 (96 registers, fewer warps). With 72 registers 16-bit rows
+// spill some: 14 loads and stores of the 550 instructions for two rows of K and V.
 template <typename T, int G, bool WIDE>
 __device__ __forceinline__ void append_part(const AppendParams &p, uint8_t *rec, int head, int first_row, int first_pos, int tau0, int n,
                                             int lane, uint32_t (&best)[2][4]) {
@@ -264,8 +265,10 @@ __device__ __forceinline__ void append_part(const AppendParams &p, uint8_t *rec,
 constexpr int WARPS = 4;
 
 // Grid: `blocks` for each run of rows that share a page. The first kv_blocks of a run take its keys and values, a warp to 16 tokens of a
-// head (pages over 64 tokens: a warp to several of them); the others rotate the query rows, q_rows each. Lying side by side, the
-// first, which the quantizer's instructions bound, and the second, which memory does, share the SMs.
+// head (pages over 64 tokens: a warp to several of them); the others rotate the query rows, q_rows each. The two lie side
+// by side in the grid, but do not hide each other: 8192 rows x 8 kv heads take 24 us, with 32 query heads 48 (their bytes 7 and 28).
+// A run is found by every warp in turn over 32 sequences at a time, which is what a step of many sequences costs: one row each of 61
+// sequences 5.0 us, of 512 21, of 1024 49.
 template <typename T, int G, bool WIDE>
 __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 5 : 7) kv4_append_kernel(const __grid_constant__ AppendParams p) {
     constexpr int D = 32 * G;
