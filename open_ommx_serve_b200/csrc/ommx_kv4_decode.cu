@@ -17,8 +17,8 @@
 // What the tensor cores cut is then the largest error of a record: they line the addends of a product up with the largest and cut them 25 bits
 // below its leading one (an emulation of that gives the kernel's errors to a fifth), where a subnormal counts as 2^-14. A masked nibble lies 10 bits
 // below that (the odd ones, 16 times as large, 6), so an addend loses up to 2^-15 of one code of the record's heaviest token - or, in a
-// logit, of the group's largest |q| -: 2^-15 of a group's range a record at most, of the heaviest token's share in the output. Nibbles
-// moved up to bits 6..9 would lose 2^-21, for some 48 shifts a record.
+// logit, of the group's largest |q| -: 2^-14 of a group's range a record at most (17 addends), of the heaviest token's share in the
+// output. Nibbles moved up to bits 6..9 would lose 2^-21, for some 48 shifts a record.
 //
 // What bounds it: a record's 160 bytes a token are read once for each eight query heads of its kv head, so HBM, and beside it the schedulers:
 // a record is some 330 instructions of a warp, 17 of them products that hold a scheduler 8 cycles, in which its multiply-adds wait. 8 x 64K
