@@ -138,8 +138,8 @@ def _exponent(top, codes):
 
 
 def _power(e):
-    """2^e in fp32, e from -126 to 127"""
-    return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+    """2^e in fp32, e up to 127; 0 below -126"""
+    return ((e.to(torch.int32) + 127).clamp(min=0) << 23).view(torch.float32)
 
 
 def _codes(x, codes):
@@ -247,7 +247,7 @@ def _append_plain(s):
     E = torch.maximum(_exponent(top, kind), held)
     bytes_ = s["codes"].view(torch.uint8)
     old = bytes_[p, :, r].view(CODES[kind]).float()                                          # [blocks, H, 2, 16, D]
-    old = _codes(old * torch.ldexp(torch.ones_like(top), held - E).masked_fill(held == 0, 0.0)[..., None, None], kind).view(torch.uint8)
+    old = _codes(old * _power(held - E).masked_fill(held == 0, 0.0)[..., None, None], kind).view(torch.uint8)
     bytes_[p, :, r] = torch.where((E > held)[..., None, None], old, bytes_[p, :, r])
     s["scales"][p, :, r] = E.to(torch.uint8)
     bytes_[page, :, part, :, tau] = _codes(x * _power(127 - E[of].clamp(min=1))[..., None], kind).view(torch.uint8)
@@ -309,7 +309,7 @@ def _evict_plain(s):
     block, of = torch.unique(seq * (n // 16 + 1) + place // 16, return_inverse=True)
     to = torch.zeros(len(block), H, 2, dtype=torch.int32, device=w.device).index_reduce_(0, of, E, "amax")[of]
     to_page, part, tau = s["to_table"].long()[seq, place // page], place % page // 16, place % 16
-    code = code * torch.ldexp(torch.ones_like(code[..., 0]), E - to).masked_fill(E == 0, 0.0)[..., None]
+    code = code * _power(E - to).masked_fill(E == 0, 0.0)[..., None]
     bytes_[to_page, :, part, :, tau] = _codes(code, kind).view(torch.uint8)
     s["scales"][to_page, :, part] = to.to(torch.uint8)
     s["weight"][to_page, :, place % page] = weight
@@ -348,24 +348,28 @@ def run(state):
 
 
 # ---- in 64 bits, by another route ---------------------------------------------------------------------------------------
+def _power64(e):
+    return ((e.to(torch.int64) + 1023) << 52).view(torch.float64)
+
+
 def _rounded64(x, codes):
     """x (in units) to the nearest code, ties to even"""
     if codes == "int8":
         return torch.round(x)
-    step = torch.exp2(torch.floor(torch.log2(x.abs().clamp(min=2.0 ** -6))) - 3)             # three bits behind the leading one
+    step = _power64(torch.frexp(x.abs().clamp(min=2.0 ** -6))[1] - 4)                        # three bits behind the leading one
     return torch.round(x / step) * step
 
 
 def _unit64(top, codes):
     """The power of two that a block of this largest value is held in; 0 for none."""
-    unit = torch.exp2(torch.ceil(torch.log2(top / TOP[codes])).clamp(min=-126.0))
-    return torch.where(top > 0, unit, 0.0)
+    low = _power64(torch.frexp(top / TOP[codes])[1].clamp(min=-125) - 1)                     # at most what is looked for
+    return torch.where(top > 0, torch.where(top > low * TOP[codes], 2 * low, low), 0.0)
 
 
 def _held64(s, ids, h):
     """Units [blocks, 2] and values [blocks, 2, 16, D] of one kv head's blocks of these pages, in order."""
     E = s["scales"][ids, h].flatten(0, 1).double()
-    unit = torch.where(E > 0, torch.exp2(E - 127), 0.0)
+    unit = torch.where(E > 0, _power64(E - 127), 0.0)
     return unit, s["codes"].view(torch.uint8)[ids, h].view(s["codes"].dtype).to(torch.float32).double().flatten(0, 1) * unit[..., None, None]
 
 
