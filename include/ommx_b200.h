@@ -482,6 +482,123 @@ typedef struct ommx_kv4_select_args {
 int ommx_b200_kv4_select(const ommx_kv4_select_args *args, void *stream);
 int64_t ommx_b200_kv4_select_workspace_bytes(int32_t batch, int32_t n_kv_heads, int32_t pages_per_seq);
 
+/* ---- the 8-bit cache --------------------------------------------------------------------------
+ * A paged KV cache in 8 bits beside the 4-bit one: int8 or e4m3 codes with a power of two for each 16 tokens of a kv head, one for
+ * the keys and one for the values (256 bytes and 1/8 a token and kv head at head_dim 128).  Attention over it sees all tokens, or the
+ * first ones and a sliding window; it can keep account of the weight that each token is attended to with, and tokens can be
+ * evicted by that.  No counterpart in the reference.
+ *
+ * codes: [num_pages][n_kv_heads][page_size / 16][2][16][head_dim] bytes, keys (0) and values (1) of 16 tokens (a block).
+ * scales: [num_pages][n_kv_heads][page_size / 16][2] bytes: E.  value = code * 2^(E - 127).
+ * E is the smallest from 1 on for which the block's largest value is at most 127 (int8) or 448 (e4m3) units, 0 where all are zero;
+ * codes are value / unit to the nearest, ties to even.  NaN counts as 0 and values beyond 2^126 as that (OMMX_ST_NONFINITE where one
+ * is not finite).  A block that holds tokens and takes rows keeps the larger E of the two; codes it holds are rounded to that.
+ * int8 -128 and e4m3's NaN are never written, and count as -128 and, in values that are attended to, 480 units where a caller writes them.
+ * weight (optional): float [num_pages][n_kv_heads][page_size], what each token was attended to with.
+ *
+ * A page that takes rows, weights or kept tokens belongs to one sequence.  Lengths, tables and row ranges are read on the device: nothing
+ * synchronises, and a captured graph follows them.  Bad ones are reported in *status and skipped.
+ */
+#define OMMX_KV8_INT8 0
+#define OMMX_KV8_E4M3 1
+
+typedef struct ommx_kv8_cache {
+    void *codes;                    /* 16-byte aligned */
+    uint8_t *scales;                /* 2-byte aligned */
+    float *weight;                  /* 16-byte aligned, or NULL */
+    int32_t num_pages, n_kv_heads;
+    int32_t head_dim;               /* 64 or 128 */
+    int32_t page_size;              /* 16, 32, 64, 128 or 256 */
+    int32_t code;                   /* OMMX_KV8_* */
+} ommx_kv8_cache;
+
+typedef ommx_kv4_seqs ommx_kv8_seqs;
+
+typedef struct ommx_kv8_append_args {
+    ommx_kv8_cache cache;           /* weight: that of the new tokens is set to 0 */
+    ommx_kv8_seqs seqs;
+    const void *k_new, *v_new;      /* [num_rows, n_kv_heads, head_dim], last dimension contiguous */
+    int32_t dtype;                  /* OMMX_DT_* of k_new and v_new */
+    int32_t num_rows;
+    int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+    const int32_t *row_start;       /* as in ommx_kv4_append_args */
+    int32_t *status;
+} ommx_kv8_append_args;
+
+/* Quantize new rows and store them.  One launch. */
+int ommx_b200_kv8_append(const ommx_kv8_append_args *args, void *stream);
+
+typedef struct ommx_kv8_gather_args {
+    ommx_kv8_cache cache;           /* weight is not read */
+    ommx_kv8_seqs seqs;
+    void *k, *v;                    /* [num_rows, n_kv_heads, head_dim], last dimension contiguous */
+    int32_t dtype;                  /* OMMX_DT_* of k and v */
+    int32_t num_rows;
+    int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+    const int32_t *row_start;       /* as in ommx_kv4_append_args */
+    int32_t *status;
+} ommx_kv8_gather_args;
+
+/* Read the last rows of every sequence back (all of them: row_start from the lengths).  One launch. */
+int ommx_b200_kv8_gather(const ommx_kv8_gather_args *args, void *stream);
+
+typedef struct ommx_kv8_decode_args {
+    ommx_kv8_cache cache;           /* weight: written, for every token of every sequence; NULL: no account is kept */
+    ommx_kv8_seqs seqs;
+    const void *q;                  /* [batch, n_q_heads, head_dim], last dimension contiguous */
+    int32_t q_dtype;                /* OMMX_DT_BF16 or OMMX_DT_F16 */
+    int32_t n_q_heads;              /* a multiple of n_kv_heads */
+    int64_t q_stride_b, q_stride_h;
+    void *o;                        /* [batch, n_q_heads, head_dim] */
+    int32_t o_dtype;                /* OMMX_DT_* */
+    int64_t o_stride_b, o_stride_h;
+    float *lse;                     /* [batch, n_q_heads], natural logarithm; -inf (and o = 0) for a sequence of no tokens */
+    int64_t lse_stride_b;
+    int32_t window, sink_tokens;    /* window > 0: the last `window` tokens and the first sink_tokens are visible; 0: all */
+    const float *weight_before;     /* like cache.weight, and may be it: weight = keep * weight_before + the sum of the attention weights
+                                       of the kv head's query heads; not read with keep = 0 */
+    float keep;
+    float *workspace;               /* 16-byte aligned; calls that overlap need their own */
+    int64_t workspace_floats;
+    int32_t max_seq_len;            /* an upper bound of b_seq_len that sizes the grid and the workspace, 0: what the table can hold.  Weights
+                                       of sequences past it are not kept up (OMMX_ST_BAD_LENGTH) */
+    float sm_scale, logit_cap;      /* logits: cap * tanh(q.k * sm_scale / cap); cap 0: none.  sm_scale: any finite number; the largest
+                                       |q| * |sm_scale| * 2^17 must be finite in 32 bits.  Logits are served up to 2^24 in size */
+    int32_t *status;
+} ommx_kv8_decode_args;
+
+/* Attention of one query row per sequence.  A kv head's records are read once for each eight of its query heads.  Two launches; one where
+ * no sequence sees more than 512 tokens by max_seq_len, the table's width or the window, or, where rows (sequences x kv heads x eights of
+ * query heads) are few enough for clusters, 4096; one more where weights are kept. */
+int ommx_b200_kv8_decode(const ommx_kv8_decode_args *args, void *stream);
+/* floats of workspace that this call needs on the current device (0: none; its pointers are not looked at, but for whether there is a weight) */
+int64_t ommx_b200_kv8_decode_workspace_floats(const ommx_kv8_decode_args *args);
+
+typedef struct ommx_kv8_evict_args {
+    ommx_kv8_cache cache;           /* weight is needed */
+    ommx_kv8_seqs seqs;
+    const void *to_table;           /* [batch, to_pages_per_seq]: the pages that take what is kept, none of them a page of a sequence; NULL: the
+                                       first pages of the sequences themselves */
+    int64_t to_table_stride;
+    int32_t to_table_is_int64, to_pages_per_seq;
+    int32_t *kept;                  /* out [batch, n_kv_heads, budget]: the places that were kept, ascending, then -1 */
+    int32_t budget, sink_tokens, recent_tokens;
+    int32_t *len_out;               /* [batch]: min(b_seq_len, budget); may be b_seq_len, or NULL */
+    void *workspace;                /* ommx_b200_kv8_evict_workspace_bytes() of them, 16-byte aligned */
+    int64_t workspace_bytes;
+    int32_t max_seq_len;            /* an upper bound of b_seq_len that sizes the launch, 0: what the table can hold */
+    int32_t *status;
+} ommx_kv8_evict_args;
+
+/*
+ * Keep `budget` tokens of each sequence and kv head: the first sink_tokens, the last recent_tokens and of the others those of the largest
+ * weight (ties to the lower place, NaN last), moved with their weights to the places 0 .. budget - 1 in their order.  A record of kept
+ * tokens has the largest E that they had; codes are rounded to that.  A sequence of at most `budget` tokens keeps all; one with a page out
+ * of range, or more tokens than its tables hold, is reported and stays as it is.  Two launches.
+ */
+int ommx_b200_kv8_evict(const ommx_kv8_evict_args *args, void *stream);
+int64_t ommx_b200_kv8_evict_workspace_bytes(int32_t batch, int32_t n_kv_heads, int32_t budget);
+
 #ifdef __cplusplus
 }
 #endif

@@ -126,6 +126,39 @@ class KV4SelectArgs(C.Structure):
                 ("status", C.c_void_p)]
 
 
+class KV8Cache(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("weight", C.c_void_p), ("num_pages", C.c_int32), ("n_kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("page_size", C.c_int32), ("code", C.c_int32)]
+
+
+class KV8AppendArgs(C.Structure):
+    _fields_ = [("cache", KV8Cache), ("seqs", KV4Seqs), ("k_new", C.c_void_p), ("v_new", C.c_void_p), ("dtype", C.c_int32),
+                ("num_rows", C.c_int32), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64), ("v_stride_t", C.c_int64),
+                ("v_stride_h", C.c_int64), ("row_start", C.c_void_p), ("status", C.c_void_p)]
+
+
+class KV8GatherArgs(C.Structure):
+    _fields_ = [("cache", KV8Cache), ("seqs", KV4Seqs), ("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32),
+                ("num_rows", C.c_int32), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64), ("v_stride_t", C.c_int64),
+                ("v_stride_h", C.c_int64), ("row_start", C.c_void_p), ("status", C.c_void_p)]
+
+
+class KV8DecodeArgs(C.Structure):
+    _fields_ = [("cache", KV8Cache), ("seqs", KV4Seqs), ("q", C.c_void_p), ("q_dtype", C.c_int32), ("n_q_heads", C.c_int32),
+                ("q_stride_b", C.c_int64), ("q_stride_h", C.c_int64), ("o", C.c_void_p), ("o_dtype", C.c_int32),
+                ("o_stride_b", C.c_int64), ("o_stride_h", C.c_int64), ("lse", C.c_void_p), ("lse_stride_b", C.c_int64),
+                ("window", C.c_int32), ("sink_tokens", C.c_int32), ("weight_before", C.c_void_p), ("keep", C.c_float),
+                ("workspace", C.c_void_p), ("workspace_floats", C.c_int64), ("max_seq_len", C.c_int32), ("sm_scale", C.c_float),
+                ("logit_cap", C.c_float), ("status", C.c_void_p)]
+
+
+class KV8EvictArgs(C.Structure):
+    _fields_ = [("cache", KV8Cache), ("seqs", KV4Seqs), ("to_table", C.c_void_p), ("to_table_stride", C.c_int64),
+                ("to_table_is_int64", C.c_int32), ("to_pages_per_seq", C.c_int32), ("kept", C.c_void_p), ("budget", C.c_int32),
+                ("sink_tokens", C.c_int32), ("recent_tokens", C.c_int32), ("len_out", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64), ("max_seq_len", C.c_int32), ("status", C.c_void_p)]
+
+
 class LaunchPlan(C.Structure):
     _fields_ = [(name, C.c_int32) for name in ("ctas", "cluster", "shares", "ctas_per_share", "groups_per_share")]
 
@@ -153,6 +186,12 @@ SYMBOLS = {
     "ommx_b200_kv4_workspace_floats": (C.c_int64, [C.c_int32]),
     "ommx_b200_kv4_select": (C.c_int, [C.POINTER(KV4SelectArgs), C.c_void_p]),
     "ommx_b200_kv4_select_workspace_bytes": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
+    "ommx_b200_kv8_append": (C.c_int, [C.POINTER(KV8AppendArgs), C.c_void_p]),
+    "ommx_b200_kv8_gather": (C.c_int, [C.POINTER(KV8GatherArgs), C.c_void_p]),
+    "ommx_b200_kv8_decode": (C.c_int, [C.POINTER(KV8DecodeArgs), C.c_void_p]),
+    "ommx_b200_kv8_decode_workspace_floats": (C.c_int64, [C.POINTER(KV8DecodeArgs)]),
+    "ommx_b200_kv8_evict": (C.c_int, [C.POINTER(KV8EvictArgs), C.c_void_p]),
+    "ommx_b200_kv8_evict_workspace_bytes": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
     "ommx_b200_peer_alloc": (C.c_int, [C.c_size_t, C.POINTER(C.c_void_p), C.c_void_p]),
     "ommx_b200_peer_open": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "ommx_b200_peer_close": (C.c_int, [C.c_void_p]),

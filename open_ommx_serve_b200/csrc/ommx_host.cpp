@@ -925,6 +925,180 @@ PyObject *py_kv4_select(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- the 8-bit cache ----
+struct KV8Call : KV4Call {
+    void codes(PyObject *codes, PyObject *scales, ommx_kv8_cache *c) {
+        const Tensor *t = tensor(codes, "codes");
+        KV4_EXPECT(*this, t->dim() == 6 && (t->scalar_type() == at::kChar || t->scalar_type() == at::kFloat8_e4m3fn) && t->is_contiguous(),
+               "codes must be a contiguous int8 or float8_e4m3fn tensor [pages, kv heads, page_size / 16, 2, 16, head_dim]");
+        KV4_EXPECT(*this, t->size(3) == 2 && t->size(4) == 16 && t->size(0) <= INT32_MAX && t->size(1) > 0 && t->size(1) <= 4096 && t->size(2) >= 1 && t->size(2) <= 16 && t->size(5) <= INT32_MAX,
+               "codes is " + shape_text(*t) + ", wanted [pages, kv heads, page_size / 16, 2, 16, head_dim]");
+        c->codes = t->data_ptr();
+        c->num_pages = (int32_t)t->size(0); c->n_kv_heads = (int32_t)t->size(1); c->page_size = 16 * (int32_t)t->size(2); c->head_dim = (int32_t)t->size(5);
+        c->code = t->scalar_type() == at::kChar ? OMMX_KV8_INT8 : OMMX_KV8_E4M3;
+        if (c->head_dim != 64 && c->head_dim != 128) throw Refusal{PyExc_NotImplementedError, std::string(who) + ": head_dim " + std::to_string(c->head_dim) + " (this build serves 64 and 128)"};
+        if (c->page_size & (c->page_size - 1)) throw Refusal{PyExc_NotImplementedError, std::string(who) + ": page_size " + std::to_string(c->page_size) + " (this build serves 16, 32, 64, 128 and 256)"};
+        const Tensor *e = tensor(scales, "scales");
+        KV4_EXPECT(*this, e->dim() == 4 && e->scalar_type() == at::kByte && e->is_contiguous() && e->size(0) == t->size(0) && e->size(1) == t->size(1) && e->size(2) == t->size(2) && e->size(3) == 2,
+               "scales must be a contiguous uint8 tensor [pages, kv heads, page_size / 16, 2] of the codes' sizes");
+        c->scales = (uint8_t *)e->data_ptr();
+    }
+    float *weight(PyObject *o, const char *name, const ommx_kv8_cache &c, bool needed = false) {
+        const Tensor *t = tensor(o, name, needed);
+        if (!t) return nullptr;
+        KV4_EXPECT(*this, t->dim() == 3 && t->scalar_type() == at::kFloat && t->is_contiguous() && t->size(0) == c.num_pages && t->size(1) == c.n_kv_heads && t->size(2) == c.page_size,
+               std::string(name) + " must be a contiguous float32 tensor [pages, kv heads, page_size] of the codes' sizes");
+        return (float *)t->data_ptr();
+    }
+};
+
+// kv8_append(k_new, v_new, codes, scales, page_table, b_seq_len, row_start, weight, status)
+PyObject *py_kv8_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    KV4_TRY
+    if (n != 9) { PyErr_SetString(PyExc_TypeError, "kv8_append: wrong argument count"); return nullptr; }
+    KV8Call c{{"ommx_kv8_append"}};
+    ommx_kv8_append_args d;
+    memset(&d, 0, sizeof(d));
+    c.codes(a[2], a[3], &d.cache);
+    c.seqs(a[4], a[5], &d.seqs);
+    const Tensor *k = c.tensor(a[0], "k_new");
+    KV4_EXPECT(c, k->dim() == 3 && k->size(0) <= INT32_MAX, "k_new must be [rows, kv heads, head_dim]");
+    d.dtype = type_code(c, *k, "k_new", true);
+    const int64_t T = k->size(0), H = d.cache.n_kv_heads, D = d.cache.head_dim;
+    k = c.rows(a[0], "k_new", T, H, D, k->scalar_type());
+    const Tensor *v = c.rows(a[1], "v_new", T, H, D, k->scalar_type());
+    d.k_new = k->data_ptr(); d.v_new = v->data_ptr(); d.num_rows = (int32_t)T;
+    d.k_stride_t = k->stride(0); d.k_stride_h = k->stride(1); d.v_stride_t = v->stride(0); d.v_stride_h = v->stride(1);
+    d.row_start = c.row_start(a[6], d.seqs.batch, T);
+    d.cache.weight = c.weight(a[7], "weight", d.cache);
+    d.status = c.status(a[8]);
+    return PyLong_FromLong(launch(c.device(), [&](void *stream) { return ommx_b200_kv8_append(&d, stream); }));
+    KV4_END
+    END_HANDLE_TH_ERRORS
+}
+
+// kv8_gather(codes, scales, page_table, b_seq_len, k_out, v_out, row_start, status)
+PyObject *py_kv8_gather(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    KV4_TRY
+    if (n != 8) { PyErr_SetString(PyExc_TypeError, "kv8_gather: wrong argument count"); return nullptr; }
+    KV8Call c{{"ommx_kv8_gather"}};
+    ommx_kv8_gather_args d;
+    memset(&d, 0, sizeof(d));
+    c.codes(a[0], a[1], &d.cache);
+    c.seqs(a[2], a[3], &d.seqs);
+    const Tensor *k = c.tensor(a[4], "k_out");
+    KV4_EXPECT(c, k->dim() == 3 && k->size(0) <= INT32_MAX, "k_out must be [rows, kv heads, head_dim]");
+    d.dtype = type_code(c, *k, "k_out", true);
+    const int64_t T = k->size(0), H = d.cache.n_kv_heads, D = d.cache.head_dim;
+    k = c.rows(a[4], "k_out", T, H, D, k->scalar_type());
+    const Tensor *v = c.rows(a[5], "v_out", T, H, D, k->scalar_type());
+    c.distinct(*k, "k_out");
+    c.distinct(*v, "v_out");
+    d.k = k->data_ptr(); d.v = v->data_ptr(); d.num_rows = (int32_t)T;
+    d.k_stride_t = k->stride(0); d.k_stride_h = k->stride(1); d.v_stride_t = v->stride(0); d.v_stride_h = v->stride(1);
+    d.row_start = c.row_start(a[6], d.seqs.batch, T);
+    d.status = c.status(a[7]);
+    return PyLong_FromLong(launch(c.device(), [&](void *stream) { return ommx_b200_kv8_gather(&d, stream); }));
+    KV4_END
+    END_HANDLE_TH_ERRORS
+}
+
+// kv8_decode(q, codes, scales, page_table, b_seq_len, o, lse, sm_scale, logit_cap, window, sink_tokens, weight, weight_before, keep, workspace,
+//            max_seq_len, status)
+PyObject *py_kv8_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    KV4_TRY
+    if (n != 17) { PyErr_SetString(PyExc_TypeError, "kv8_decode: wrong argument count"); return nullptr; }
+    KV8Call c{{"ommx_kv8_decode_attention"}};
+    ommx_kv8_decode_args d;
+    memset(&d, 0, sizeof(d));
+    c.codes(a[1], a[2], &d.cache);
+    c.seqs(a[3], a[4], &d.seqs);
+    const int64_t B = d.seqs.batch, H = d.cache.n_kv_heads, D = d.cache.head_dim;
+    const Tensor *q = c.tensor(a[0], "q");
+    KV4_EXPECT(c, q->dim() == 3 && q->size(1) <= INT32_MAX, "q must be [batch, query heads, head_dim]");
+    d.q_dtype = type_code(c, *q, "q", false);
+    const int64_t Hq = q->size(1);
+    q = c.rows(a[0], "q", B, Hq, D, q->scalar_type());
+    if (Hq < H || Hq % H) throw Refusal{PyExc_NotImplementedError, "ommx_kv8_decode_attention: " + std::to_string(Hq) + " query heads are not a multiple of " + std::to_string(H) + " kv heads"};
+    const Tensor *o = c.tensor(a[5], "o");
+    d.o_dtype = type_code(c, *o, "o", true);
+    o = c.rows(a[5], "o", B, Hq, D, o->scalar_type());
+    c.distinct(*o, "o");
+    const Tensor *lse = c.tensor(a[6], "lse");
+    KV4_EXPECT(c, lse->dim() == 2 && lse->size(0) == B && lse->size(1) == Hq && lse->scalar_type() == at::kFloat && (Hq <= 1 || lse->stride(1) == 1) && (B <= 1 || lse->stride(0) >= Hq),
+             "lse must be a float32 tensor [batch, query heads] with contiguous rows");
+    d.q = q->data_ptr(); d.n_q_heads = (int32_t)Hq; d.q_stride_b = q->stride(0); d.q_stride_h = q->stride(1);
+    d.o = o->data_ptr(); d.o_stride_b = o->stride(0); d.o_stride_h = o->stride(1);
+    d.lse = (float *)lse->data_ptr(); d.lse_stride_b = lse->stride(0);
+    d.sm_scale = (float)(a[7] == Py_None ? 1.0 / std::sqrt((double)D) : c.number(a[7], "sm_scale"));
+    KV4_EXPECT(c, std::isfinite(d.sm_scale), "sm_scale must be finite in 32 bits");
+    d.logit_cap = (float)c.number(a[8], "logit_cap");
+    KV4_EXPECT(c, d.logit_cap >= 0.0f && std::isfinite(d.logit_cap), "logit_cap must be finite and not negative");
+    if (a[9] != Py_None) d.window = (int32_t)c.integer(a[9], "window", 1);
+    d.sink_tokens = (int32_t)c.integer(a[10], "sink_tokens", 0);
+    d.cache.weight = c.weight(a[11], "weight", d.cache);
+    d.weight_before = c.weight(a[12], "weight_before", d.cache);
+    KV4_EXPECT(c, d.cache.weight || !d.weight_before, "weight_before without weight");
+    if (!d.weight_before) d.weight_before = d.cache.weight;
+    d.keep = (float)c.number(a[13], "keep");
+    KV4_EXPECT(c, std::isfinite(d.keep), "keep must be finite in 32 bits");
+    if (a[15] != Py_None) d.max_seq_len = (int32_t)c.integer(a[15], "max_seq_len", 0);
+    d.status = c.status(a[16]);
+    if (a[14] != Py_None) c.tensor(a[14], "workspace");
+    const at::Device dev = c.device();
+    Tensor own;
+    {
+        const c10::cuda::CUDAGuard guard(dev);
+        d.workspace_floats = ommx_b200_kv8_decode_workspace_floats(&d);
+    }
+    d.workspace = (float *)c.workspace(a[14], at::kFloat, d.workspace_floats, dev, &own);
+    return PyLong_FromLong(launch(dev, [&](void *stream) { return ommx_b200_kv8_decode(&d, stream); }));
+    KV4_END
+    END_HANDLE_TH_ERRORS
+}
+
+// kv8_evict(codes, scales, weight, page_table, b_seq_len, kept, sink_tokens, recent_tokens, to_table, len_out, workspace, max_seq_len, status)
+PyObject *py_kv8_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    KV4_TRY
+    if (n != 13) { PyErr_SetString(PyExc_TypeError, "kv8_evict: wrong argument count"); return nullptr; }
+    KV8Call c{{"ommx_kv8_evict"}};
+    ommx_kv8_evict_args d;
+    memset(&d, 0, sizeof(d));
+    c.codes(a[0], a[1], &d.cache);
+    d.cache.weight = c.weight(a[2], "weight", d.cache, true);
+    c.seqs(a[3], a[4], &d.seqs);
+    const int64_t B = d.seqs.batch, H = d.cache.n_kv_heads;
+    const Tensor *kept = c.tensor(a[5], "kept");
+    KV4_EXPECT(c, kept->dim() == 3 && kept->scalar_type() == at::kInt && kept->is_contiguous() && kept->size(0) == B && kept->size(1) == H && kept->size(2) >= 1 && kept->size(2) <= INT32_MAX,
+             "kept must be a contiguous int32 tensor [batch, kv heads, tokens to keep]");
+    d.kept = (int32_t *)kept->data_ptr(); d.budget = (int32_t)kept->size(2);
+    d.sink_tokens = (int32_t)c.integer(a[6], "sink_tokens", 0); d.recent_tokens = (int32_t)c.integer(a[7], "recent_tokens", 0);
+    KV4_EXPECT(c, (int64_t)d.sink_tokens + d.recent_tokens <= d.budget, "sink_tokens and recent_tokens must fit into the " + std::to_string(d.budget) + " tokens that are kept");
+    if (const Tensor *t = c.tensor(a[8], "to_table", false)) {
+        KV4_EXPECT(c, t->dim() == 2 && (t->scalar_type() == at::kInt || t->scalar_type() == at::kLong) && (t->size(1) <= 1 || t->stride(1) == 1) && t->size(0) == B && t->size(1) >= 1 && t->size(1) <= INT32_MAX,
+                 "to_table must be an int32 or int64 tensor [batch, pages] with contiguous rows");
+        d.to_table = t->data_ptr(); d.to_table_stride = t->stride(0); d.to_table_is_int64 = t->scalar_type() == at::kLong; d.to_pages_per_seq = (int32_t)t->size(1);
+    }
+    if (const Tensor *t = c.tensor(a[9], "len_out", false)) {
+        KV4_EXPECT(c, t->dim() == 1 && t->scalar_type() == at::kInt && t->is_contiguous() && t->size(0) == B, "len_out must be a contiguous int32 tensor [batch]");
+        d.len_out = (int32_t *)t->data_ptr();
+    }
+    if (a[11] != Py_None) d.max_seq_len = (int32_t)c.integer(a[11], "max_seq_len", 0);
+    d.status = c.status(a[12]);
+    if (a[10] != Py_None) c.tensor(a[10], "workspace");
+    const at::Device dev = c.device();
+    Tensor own;
+    d.workspace_bytes = ommx_b200_kv8_evict_workspace_bytes(d.seqs.batch, d.cache.n_kv_heads, d.budget);
+    d.workspace = c.workspace(a[10], at::kByte, d.workspace_bytes, dev, &own);
+    return PyLong_FromLong(launch(dev, [&](void *stream) { return ommx_b200_kv8_evict(&d, stream); }));
+    KV4_END
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef METHODS[] = {
     {"decode", (PyCFunction)(void (*)())py_decode, METH_FASTCALL, "paged decode attention; None when an argument needs explaining"},
     {"pack_into", (PyCFunction)(void (*)())py_pack_into, METH_FASTCALL, "quantize and pack into given planes; None when an argument needs explaining"},
@@ -936,6 +1110,10 @@ PyMethodDef METHODS[] = {
     {"kv4_gather", (PyCFunction)(void (*)())py_kv4_gather, METH_FASTCALL, "rows of a 4-bit cache"},
     {"kv4_decode", (PyCFunction)(void (*)())py_kv4_decode, METH_FASTCALL, "decode attention over a 4-bit cache"},
     {"kv4_select", (PyCFunction)(void (*)())py_kv4_select, METH_FASTCALL, "the pages of a 4-bit cache that attention reads"},
+    {"kv8_append", (PyCFunction)(void (*)())py_kv8_append, METH_FASTCALL, "rows into an 8-bit cache"},
+    {"kv8_gather", (PyCFunction)(void (*)())py_kv8_gather, METH_FASTCALL, "rows of an 8-bit cache"},
+    {"kv8_decode", (PyCFunction)(void (*)())py_kv8_decode, METH_FASTCALL, "decode attention over an 8-bit cache"},
+    {"kv8_evict", (PyCFunction)(void (*)())py_kv8_evict, METH_FASTCALL, "keep the tokens of an 8-bit cache that were attended to most"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef MODULE = {PyModuleDef_HEAD_INIT, "_host", "torch tensors -> the C ABI of libommx_b200.so", -1, METHODS, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,885 @@
+// The 8-bit cache: attention of one query row per sequence, over all tokens or the first ones and a sliding window, with an account of
+// each token's weight where it is asked for.
+//
+// For query head h of a sequence, over its visible tokens t:  x_t = sm_scale q.K_t,  o = sum_t exp(x_t) V_t / sum_t exp(x_t), with
+// K_t = 2^ek a_t and V_t = 2^ev b_t for the 16 tokens of a record: a record's scales are two numbers, which meet the sums of its products
+// behind them. Products are m16n8k16 with the codes as A (tokens as rows for K, channels for V) and up to eight query heads that share
+// the kv head as columns:
+//   logits   fp16, exact: codes of either type are fp16 numbers, and a query row times a power of two is (rounded by 2^-39 of its largest
+//            channel at most, where bf16 channels are 2^27 below that);
+//   values   bf16, whose range is that of fp32: a weight y is the sum of two bf16 numbers, off by 2^-17 of itself however small it is, and
+//            no token is left out; codes are bf16 numbers. One record's sum starts at zero and is added in fp32, times its scale: the tensor
+//            cores, which cut what they add, cut 25 bits below a record's own largest product.
+// Values are summed in units of the largest scale a warp has met, and leave it divided by the sum of their weights, so neither the
+// largest nor the smallest numbers a cache holds pass fp32 on the way.
+//
+// What bounds it: a record's 32 D bytes are read once for each eight query heads of its kv head.
+#include <cmath>
+#include <type_traits>
+
+#include "ommx_kv8.cuh"
+#include "ommx_kv_deal.cuh"
+
+namespace ommx {
+namespace kv8 {
+
+using namespace kv;
+
+constexpr int WARPS_PER_SM = 16;                  // a block is NW of them, each with records of its own
+constexpr int STAGES = 3, AHEAD = STAGES - 1;     // records that a warp holds, and those of them on their way
+constexpr uint32_t ALL = 0xFFFFu;                 // sixteen visible tokens
+constexpr int COLS = 8;                           // query heads side by side
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOWEST = -1e30f;
+constexpr int MOST_PARTS = 768;                   // blocks of a call that shares rows
+constexpr int WHOLE = 32;                         // records of a row that one block takes at most where it could share it
+
+// A code as the A operand of values: e4m3 codes moved to a bf16 number's bits are 2^-120 times as large, int8 codes (u - 128) 2^-13 come out
+// of one multiply-add of the subnormal u 2^-133. What weights are multiplied with before they meet e4m3 codes keeps products within fp32
+// (in the weight's own logarithm it would cost it seven bits).
+template <bool E4M3> struct Code {
+    static constexpr float LIFT = E4M3 ? 0x1p80f : 1.0f;
+    static constexpr float BACK = E4M3 ? 0x1p40f : 0x1p13f;                 // undoes both
+};
+constexpr float HEAVY = 128.0f;                   // weights 2^(x - ref) begin near 1; one past this moves the reference
+
+struct DecodeParams {
+    Cache c;
+    Seqs s;
+    const void *q;
+    void *o;
+    float *lse, *work;
+    float *logits;                                // [row of group heads' units][16][group], or null
+    float2 *stats;                                // [B][Hq]: reference and 1 / sum
+    const float *before;                          // what weights add to
+    int64_t q_b, q_h, o_b, o_h, lse_b;
+    int32_t q16, q_wide, o_type, group, col_blocks, page_shift, least, whole, window, sinks, most_units;
+    float sm_scale, cap, keep;
+    int32_t *status;
+};
+
+__device__ __forceinline__ int length_of(const DecodeParams &p, int b) {
+    const int len = p.s.len[b];
+    const int64_t most = (int64_t)p.s.max_pages << p.page_shift;
+    if (len < 0 || len > most) { or_status(p.status, OMMX_ST_BAD_LENGTH); return len < 0 ? 0 : (int)most; }
+    return len;
+}
+// The records of a sequence that hold visible tokens: the first `head`, and those from `head` + `skip` on.
+struct Span { int units, head, skip; };
+__device__ __forceinline__ Span span_of(const DecodeParams &p, int len) {
+    const int all = (len + 15) >> 4;
+    Span s = {all, 0, 0};
+    if (p.window && len > p.window) {
+        const int tail = (len - p.window) >> 4;
+        s.head = min((p.sinks + 15) >> 4, tail);
+        s.skip = tail - s.head;
+        s.units = all - s.skip;
+    }
+    return s;
+}
+__device__ __forceinline__ int units_of(const DecodeParams &p, int len) { return span_of(p, len).units; }
+// Which of a record's tokens are visible, a bit each
+__device__ __forceinline__ uint32_t visible(const DecodeParams &p, int len, int record) {
+    const int first = 16 * record;
+    auto below = [](int n) { return n >= 16 ? ALL : n <= 0 ? 0u : (1u << n) - 1; };
+    uint32_t mask = below(len - first);
+    if (p.window && len > p.window) mask &= ~below(len - p.window - first) | below(p.sinks - first);
+    return mask;
+}
+
+__device__ __forceinline__ void store_o(const DecodeParams &p, int64_t at, float v) {
+    if (p.o_type == OMMX_DT_F32) reinterpret_cast<float *>(p.o)[at] = v;
+    else if (p.o_type == OMMX_DT_F16) reinterpret_cast<__half *>(p.o)[at] = __float2half_rn(v);
+    else reinterpret_cast<__nv_bfloat16 *>(p.o)[at] = __float2bfloat16_rn(v);
+}
+template <int G> __device__ __forceinline__ void store_o(const DecodeParams &p, int64_t at, const float (&v)[G]) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) store_o(p, at + i, v[i]);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
+// A head's reference and sum of weights
+__device__ __forceinline__ void store_sum(const DecodeParams &p, int b, int hq, float ref, float sum) {
+    p.lse[b * p.lse_b + hq] = sum != 0.0f ? (ref + log2f(sum)) * LN2 : -INFINITY;
+    if (p.stats) p.stats[(int64_t)b * p.c.H * p.group + hq] = make_float2(ref, sum != 0.0f ? 1.0f / sum : 0.0f);
+}
+
+// ---- pieces ---------------------------------------------------------------------------------------
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23 & 255u) - 127; }
+
+// four codes of a token to two fp16 pairs
+template <bool E4M3> __device__ __forceinline__ void key_pairs(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    if constexpr (E4M3) {
+        lo = half2_of_e4m3x2(w);
+        hi = half2_of_e4m3x2(w >> 16);
+    } else {
+        const uint32_t u = w ^ 0x80808080u;       // 1024 + 128 + code as an fp16 number
+        const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), off), y = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
+        lo = *reinterpret_cast<const uint32_t *>(&x);
+        hi = *reinterpret_cast<const uint32_t *>(&y);
+    }
+}
+// code `i` of two tokens' words to a bf16 pair, UNIT times as large
+template <bool E4M3> __device__ __forceinline__ uint32_t value_pair(uint32_t a, uint32_t b, int i) {
+    if constexpr (E4M3) {
+        const uint32_t w = __byte_perm(a, b, (4 + i) << 12 | i << 4);       // the codes in the upper bytes
+        return (w & 0x80008000u) | (w >> 4 & 0x07F007F0u);
+    } else {
+        const uint32_t u = (__byte_perm(a, b, (4 + i) << 8 | i) & 0x00FF00FFu) ^ 0x00800080u;
+        uint32_t r;
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(u), "r"(0x7B807B80u), "r"(0xBC80BC80u));   // * 2^120 - 2^-6
+        return r;
+    }
+}
+
+// A kv head's queries as B fragments: lane (g, t) holds head g, channels 8 G t + 4 s + 0..3 for product s
+template <int G> struct Query {
+    uint32_t frag[2 * G][2];
+    float factor[2], raw[2];                      // of heads 2 t and 2 t + 1: the products' units in powers of two; with a cap: in its units
+};
+template <int G> __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int first_head, int n, int lane, Query<G> &q) {
+    const int g = lane >> 2, t = lane & 3;
+    float x[8 * G], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < G; ++i) kv4::load_q8(p, b * p.q_b + (first_head + min(g, n - 1)) * p.q_h + 8 * G * t + 8 * i, x + 8 * i);
+#pragma unroll
+    for (int i = 0; i < 8 * G; ++i) top = fmaxf(top, fabsf(x[i]));
+    top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+    const int e = top > 0.0f ? max(exponent_of(top), -100) : 0;
+    const float up = power_of_two(13 - e);
+#pragma unroll
+    for (int s = 0; s < 2 * G; ++s) {
+        q.frag[s][0] = half2_bits(x[4 * s] * up, x[4 * s + 1] * up);
+        q.frag[s][1] = half2_bits(x[4 * s + 2] * up, x[4 * s + 3] * up);
+    }
+    const float factor = p.sm_scale * 0x1p-13f * power_of_two(e);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float f = __shfl_sync(~0u, factor, 8 * t + 4 * i);
+        q.raw[i] = p.cap > 0.0f ? f / p.cap : f;
+        q.factor[i] = p.cap > 0.0f ? p.cap * LOG2E : f * LOG2E;
+    }
+}
+
+// A warp's running state. acc[i]: channels 4 G g + 2 i (rows g) and the next one (rows g + 8) of heads 2 t, 2 t + 1, in units of 2^(E - 127) UNIT
+template <int G> struct State {
+    float acc[2 * G][4], sum[2], ref[2];
+    int E;
+};
+template <int G> __device__ __forceinline__ void clear(State<G> &s) {
+#pragma unroll
+    for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s.acc[i][j] = 0.0f;
+    s.sum[0] = s.sum[1] = 0.0f;
+    s.ref[0] = s.ref[1] = LOWEST;
+    s.E = 0;
+}
+
+// ---- a warp's ring of records: 16 bytes a lane at a time, a group of copies for each record ----
+// In shared memory a record's 128-byte lines have their 16-byte chunks exchanged, chunk c of line l at c ^ (l & 7) (D = 128) or
+// c ^ (2 l & 6) (two tokens to a line, D = 64), so that both ways of reading - a token's row by four lanes, and a chunk of
+// eight tokens - meet all banks.
+template <int G> __device__ __forceinline__ uint32_t swizzle(int token, int chunk) {
+    if constexpr (G == 4) return 128 * token + 16 * (chunk ^ (token & 7));
+    else return 128 * (token >> 1) + 16 * ((4 * (token & 1) + chunk) ^ (token & 6));
+}
+template <int G> __device__ __forceinline__ void fetch(uint32_t to, const uint8_t *rec, int lane) {
+    // 512 bytes are four lines; every other four the same exchange
+    const int line = lane >> 3, chunk = lane & 7;
+    const uint32_t even = 128 * line + 16 * (G == 4 ? chunk ^ line : chunk ^ (2 * line)), odd = G == 4 ? even ^ 64 : even;
+#pragma unroll
+    for (int i = 0; i < 2 * G; ++i)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 512 * i + (i & 1 ? odd : even)), "l"(rec + 512 * i + 16 * lane) : "memory");
+}
+__device__ __forceinline__ void close_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void fetched() {                // all but the last N groups
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    __syncwarp();
+}
+
+// One record in shared memory; info: which tokens are visible, and above that the exponents of K's and V's scales. `put`: where its logits
+// go, or null
+template <int G, bool E4M3> __device__ __forceinline__ void attend(const DecodeParams &p, const uint8_t *rec, uint32_t info, int lane, const Query<G> &q, State<G> &s,
+                                                                   float *put, int n) {
+    constexpr int D = 32 * G;
+    const int g = lane >> 2, t = lane & 3;
+    // ---- logits: x[0], x[1] of token g and heads 2 t, 2 t + 1; x[2], x[3] of token g + 8
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < G / 2; ++i) {
+        const uint4 a = *reinterpret_cast<const uint4 *>(rec + swizzle<G>(g, G / 2 * t + i));
+        const uint4 b = *reinterpret_cast<const uint4 *>(rec + swizzle<G>(g + 8, G / 2 * t + i));
+        const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t a0, a1, a2, a3;
+            key_pairs<E4M3>(wa[j], a0, a2);
+            key_pairs<E4M3>(wb[j], a1, a3);
+            mma_f16(j & 1 ? z : x, a0, a1, a2, a3, q.frag[4 * i + j][0], q.frag[4 * i + j][1]);
+        }
+    }
+    const float sk = scale_of(info >> 16 & 255u);
+    if (p.cap > 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = tanhf((x[i] + z[i]) * (q.raw[i & 1] * sk)) * q.factor[i & 1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = (x[i] + z[i]) * (q.factor[i & 1] * sk);
+    }
+    if (put) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (2 * t + (i & 1) < n) put[(g + 4 * (i & 2)) * p.group + 2 * t + (i & 1)] = x[i];
+    }
+    const uint32_t mask = info & ALL;
+    if (mask != ALL) {                            // what is not visible may be anything
+        if (!(mask >> g & 1)) x[0] = x[1] = -INFINITY;
+        if (!(mask >> (g + 8) & 1)) x[2] = x[3] = -INFINITY;
+    }
+
+    // ---- weights
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = exp2_approx(x[i] - s.ref[i & 1]);
+    if (__any_sync(~0u, !(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) <= HEAVY))) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float l = fmaxf(x[i], x[i + 2]);
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) l = fmaxf(l, __shfl_xor_sync(~0u, l, d));
+            const float ref = fmaxf(s.ref[i], ceilf(l)), f = exp2_approx(s.ref[i] - ref);
+            s.ref[i] = ref;
+            s.sum[i] *= f;
+#pragma unroll
+            for (int j = 0; j < 2 * G; ++j) { s.acc[j][i] *= f; s.acc[j][i + 2] *= f; }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = exp2_approx(x[i] - s.ref[i & 1]);
+    }
+    s.sum[0] += y[0] + y[2];
+    s.sum[1] += y[1] + y[3];
+    if constexpr (E4M3) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] *= Code<E4M3>::LIFT;
+    }
+    const uint32_t h0 = bf16x2_bits(y[0], y[1]), h1 = bf16x2_bits(y[2], y[3]);
+    const uint32_t b0 = transpose8x8(h0), b1 = transpose8x8(h1);
+    const uint32_t r0 = transpose8x8(bf16x2_bits(y[0] - __uint_as_float(h0 << 16), y[1] - __uint_as_float(h0 & 0xFFFF0000u)));
+    const uint32_t r1 = transpose8x8(bf16x2_bits(y[2] - __uint_as_float(h1 << 16), y[3] - __uint_as_float(h1 & 0xFFFF0000u)));
+
+    // ---- values
+    const int E = info >> 24;
+    if (E > s.E) {
+        const float f = ratio_of(s.E, E);
+#pragma unroll
+        for (int j = 0; j < 2 * G; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s.acc[j][i] *= f;
+        s.E = E;
+    }
+    const float f = ratio_of(E, s.E);
+    uint32_t w[4][G];                             // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9: channels 4 G g + 0 .. 4 G - 1
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int token = 2 * t + (i & 1) + 4 * (i & 2);
+        if constexpr (G == 4) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(rec + 16 * D + swizzle<G>(token, g));
+            w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2 *>(rec + 16 * D + swizzle<G>(token, g >> 1) + 8 * (g & 1));
+            w[i][0] = v.x; w[i][1] = v.y;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 2 * G; ++j) {
+        const int at = 2 * (j & 1);
+        uint32_t a[4];
+        a[0] = value_pair<E4M3>(w[0][j / 2], w[1][j / 2], at);
+        a[1] = value_pair<E4M3>(w[0][j / 2], w[1][j / 2], at + 1);
+        a[2] = value_pair<E4M3>(w[2][j / 2], w[3][j / 2], at);
+        a[3] = value_pair<E4M3>(w[2][j / 2], w[3][j / 2], at + 1);
+        float c[4];
+        mma_bf16_first(c, a, r0, r1);
+        mma_bf16(c, a, b0, b1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.acc[j][i] = fmaf(c[i], f, s.acc[j][i]);
+    }
+}
+
+template <int G> constexpr int PART = COLS * 32 * G + 2 * COLS;            // floats of a part in the workspace: outputs, references, sums
+template <int G, int NW> struct Shared {
+    static constexpr int D = 32 * G;
+    float o[NW][COLS][D + 4];                     // the padding spreads the heads over the banks
+};
+template <int G> struct Floats;
+template <> struct Floats<2> { using T = float2; };
+template <> struct Floats<4> { using T = float4; };
+
+// The warps' states of a row to its output, or to a part: [COLS][D] outputs of its own tokens, [COLS] references, [COLS] sums. A warp
+// finishes every NW-th head, a lane G channels.
+template <int G, bool E4M3, int NW>
+__device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Shared<G, NW> &sh, float (&ref)[COLS][NW], float (&sum)[COLS][NW], int b,
+                                       int first_head, int n, float *part, int warp, int lane) {
+    using V = typename Floats<G>::T;
+    constexpr int D = 32 * G;
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) s.sum[i] += __shfl_xor_sync(~0u, s.sum[i], d);
+        if (g == 0) { ref[2 * t + i][warp] = s.ref[i]; sum[2 * t + i][warp] = s.sum[i]; }
+    }
+    __syncthreads();                              // and the ring, whose memory `sh` is, is done with
+    const float unit = scale_of(s.E);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float back = s.sum[i] != 0.0f ? Code<E4M3>::BACK / s.sum[i] : 0.0f;
+        float *to = &sh.o[warp][2 * t + i][4 * G * g];
+#pragma unroll
+        for (int j = 0; j < 2 * G; j += 2)
+            *reinterpret_cast<float4 *>(to + 2 * j) = make_float4(s.acc[j][i] * back * unit, s.acc[j][i + 2] * back * unit,
+                                                                  s.acc[j + 1][i] * back * unit, s.acc[j + 1][i + 2] * back * unit);
+    }
+    __syncthreads();
+    for (int h = warp; h < COLS; h += NW) {
+        float top = ref[h][0], all = 0.0f;
+#pragma unroll
+        for (int w = 1; w < NW; ++w) top = fmaxf(top, ref[h][w]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) all = fmaf(sum[h][w], exp2_approx(ref[h][w] - top), all);
+        const float inverse = all != 0.0f ? 1.0f / all : 0.0f;
+        float v[G];
+#pragma unroll
+        for (int i = 0; i < G; ++i) v[i] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const V x = *reinterpret_cast<const V *>(&sh.o[w][h][lane * G]);
+            const float f = sum[h][w] * exp2_approx(ref[h][w] - top) * inverse;
+#pragma unroll
+            for (int i = 0; i < G; ++i) v[i] = fmaf(reinterpret_cast<const float *>(&x)[i], f, v[i]);
+        }
+        if (part) {
+            *reinterpret_cast<V *>(part + h * D + lane * G) = *reinterpret_cast<const V *>(v);
+            if (lane == 0) { part[COLS * D + h] = top; part[COLS * D + COLS + h] = all; }
+        } else if (h < n) {
+            store_o(p, b * p.o_b + (first_head + h) * p.o_h + lane * G, v);
+            if (lane == 0) store_sum(p, b, first_head + h, top, all);
+        }
+    }
+    __syncthreads();
+}
+
+template <int G, int NW> struct Memory {
+    union {
+        Shared<G, NW> sh;
+        uint8_t ring[NW][STAGES][1024 * G];
+    };
+    alignas(16) float merged[PART<G>];            // of this block, where a cluster shares a row
+    float ref[COLS][NW], sum[COLS][NW];
+};
+
+__device__ __forceinline__ bool too_many(const DecodeParams &p, uint32_t units, uint32_t rows) {
+    const bool over = (uint64_t)units * rows >> 31;
+    if (over) or_status(p.status, OMMX_ST_BAD_LENGTH);
+    return over;
+}
+// A row of no tokens
+template <int G> __device__ __forceinline__ void nothing(const DecodeParams &p, int b, int row) {
+    const int cb = row % p.col_blocks, first = (row / p.col_blocks) * p.group + cb * COLS, n = min(COLS, p.group - cb * COLS);
+    for (int i = threadIdx.x; i < n * 32 * G; i += blockDim.x) store_o(p, b * p.o_b + (first + i / (32 * G)) * p.o_h + i % (32 * G), 0.0f);
+    if (threadIdx.x < n) store_sum(p, b, first + threadIdx.x, LOWEST, 0.0f);
+}
+
+// ---- a row shared by a cluster's blocks: their parts meet in distributed shared memory ----
+// Head h is finished by block h mod n of the cluster, by its warp h.
+constexpr int MOST_CLUSTER = 8;
+template <int G> __device__ __forceinline__ void merge_cluster(const DecodeParams &p, const float *merged, int b, int first_head, int heads, int h, int lane) {
+    constexpr int D = 32 * G, LANES = D / 4;      // lanes that have four channels
+    const uint32_t n = cluster_size(), at = (uint32_t)__cvta_generic_to_shared(merged);
+    cluster_barrier();
+    if (h < heads && h % n == cluster_rank()) {
+        float4 v[MOST_CLUSTER];
+        float ref[MOST_CLUSTER], sum[MOST_CLUSTER];
+#pragma unroll
+        for (int r = 0; r < MOST_CLUSTER; ++r) {
+            const uint32_t from = r < (int)n ? r : 0;
+            v[r] = peer_float4(at + 4 * (h * D + 4 * (lane % LANES)), from);
+            ref[r] = r < (int)n ? peer_float(at + 4 * (COLS * D + h), from) : LOWEST;
+            sum[r] = r < (int)n ? peer_float(at + 4 * (COLS * D + COLS + h), from) : 0.0f;
+        }
+        float top = ref[0], all = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int r = 1; r < MOST_CLUSTER; ++r) top = fmaxf(top, ref[r]);
+#pragma unroll
+        for (int r = 0; r < MOST_CLUSTER; ++r) { sum[r] *= exp2_approx(ref[r] - top); all += sum[r]; }
+        const float inverse = all != 0.0f ? 1.0f / all : 0.0f;
+#pragma unroll
+        for (int r = 0; r < MOST_CLUSTER; ++r) {
+            const float f = sum[r] * inverse;
+            o[0] = fmaf(v[r].x, f, o[0]); o[1] = fmaf(v[r].y, f, o[1]); o[2] = fmaf(v[r].z, f, o[2]); o[3] = fmaf(v[r].w, f, o[3]);
+        }
+        if (lane < LANES) store_o(p, b * p.o_b + (first_head + h) * p.o_h + 4 * lane, o);
+        if (lane == 0) store_sum(p, b, first_head + h, top, all);
+    }
+    cluster_barrier();                            // no block leaves before its peers have read its part
+}
+
+template <int G, bool E4M3, int NW, bool CLUSTER>
+__global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv8_decode_kernel(const __grid_constant__ DecodeParams p) {
+    extern __shared__ __align__(128) uint8_t memory[];
+    Memory<G, NW> &m = *reinterpret_cast<Memory<G, NW> *>(memory);
+    constexpr int BYTES = 1024 * G;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint8_t *ring = m.ring[warp][0];
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    wait_earlier();
+    let_next_in();
+    const uint32_t rows = p.c.H * p.col_blocks;
+    uint32_t u, end, base = 0;                    // this block's units; units before sequence b
+    uint32_t second = ~0u;                        // a row that begins here or later leaves its part in the second slot
+    int b = 0, len = 0;
+    Span span = {0, 0, 0};
+    if (CLUSTER) {                                // a cluster to a row
+        const uint32_t n = cluster_size(), rank = cluster_rank(), at = blockIdx.x / n;
+        b = at / rows;
+        len = length_of(p, b);
+        span = span_of(p, len);
+        if (too_many(p, span.units, rows)) span.units = 0;
+        if (span.units == 0) {                    // for all of the cluster
+            if (rank == 0) nothing<G>(p, b, at - b * rows);
+            return;
+        }
+        u = (at - b * rows) * span.units;
+        end = u + (uint64_t)span.units * (rank + 1) / n;
+        u += (uint64_t)span.units * rank / n;
+    } else if (p.whole) {                         // a block to a row
+        b = blockIdx.x / rows;
+        len = length_of(p, b);
+        span = span_of(p, len);
+        if (too_many(p, span.units, rows)) span.units = 0;
+        u = (blockIdx.x - b * rows) * span.units;
+        end = u + span.units;
+        if (span.units == 0) { nothing<G>(p, b, blockIdx.x - b * rows); return; }
+    } else {
+        const Deal d = deal(p, rows, gridDim.x, lane);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<uint2 *>(p.work) = make_uint2(d.per, d.over ? OVER : d.pieces);
+        // the sequence that this block's (first) unit lies in; `at`, `before`: this block and the first of the sequence, in pieces or units
+        const uint32_t at = d.pieces ? blockIdx.x : blockIdx.x * d.per;
+        if (!d.pieces && at >= d.total) return;
+        uint32_t before = 0;
+        for (int b0 = 0;; b0 += 32) {
+            if (b0 >= p.s.B) return;              // no piece for this block (or lengths past max_seq_len, more than 32 bits count)
+            const int l = b0 + lane < p.s.B ? length_of(p, b0 + lane) : 0, n = units_of(p, l);
+            const uint32_t v = d.pieces ? pieces_of(n, d.per) : n, sum = warp_inclusive_scan(v, lane), past = __ballot_sync(~0u, before + sum * rows > at);
+            if (past) {
+                const int from = __ffs(past) - 1;
+                b = b0 + from;
+                before += __shfl_sync(~0u, sum - v, from) * rows;
+                len = __shfl_sync(~0u, l, from);
+                span = span_of(p, len);
+                break;
+            }
+            before += __shfl_sync(~0u, sum, 31) * rows;
+        }
+        const uint32_t units = span.units;
+        if (d.pieces) {                           // piece `part` of `parts` of a row; units are counted from the sequence's first
+            const uint32_t parts = pieces_of(units, d.per), row = (at - before) / parts, part = at - before - row * parts;
+            u = row * units + (uint32_t)((uint64_t)units * part / parts);
+            end = row * units + (uint32_t)((uint64_t)units * (part + 1) / parts);
+        } else {
+            base = before;
+            second = u = at;
+            end = min(u + d.per, d.total);
+        }
+    }
+    while (CLUSTER || u < end) {
+        while (u >= base + span.units * rows) {   // the next sequence that has any
+            base += span.units * rows;
+            len = length_of(p, ++b);
+            span = span_of(p, len);
+        }
+        const int units = span.units, row = (u - base) / units, i0 = u - base - row * units, i1 = min((uint32_t)units, i0 + (end - u));
+        const int head = row / p.col_blocks, cb = row % p.col_blocks;
+        const int first_head = head * p.group + cb * COLS, n = min(COLS, p.group - cb * COLS);
+        // 32 of the warp's records at a time are looked up by a lane each, while the 32 before are on their way: which one it is, which of
+        // its tokens are visible (none: there is no record) and its scales.
+        const int mine = (i1 - i0 - warp + NW - 1) / NW;
+        auto look_up = [&](int k, uint32_t &rec, uint32_t &info) {
+            const int i = i0 + warp + (k + lane) * NW, at = i < span.head ? i : i + span.skip, place = at >> (p.page_shift - 4);
+            rec = info = 0;                       // a record that is not meant is fetched too, and not used
+            if (i >= i1) return;
+            const int64_t page = page_id(p.s, b, place);
+            if (page < 0 || page >= p.c.num_pages) { or_status(p.status, OMMX_ST_BAD_PAGE); return; }
+            rec = (uint32_t)((page * p.c.H + head) * p.c.parts + (at & (p.c.parts - 1)));    // below 2^32: there is no memory for more
+            info = visible(p, len, at) | (uint32_t)reinterpret_cast<const uint16_t *>(p.c.scales)[rec] << 16;
+        };
+        // `rec`, `info`: of the AHEAD first ones, then of 32 at a time, AHEAD of those in use
+        uint32_t rec, next_rec, info, next_info, flying[AHEAD];             // flying: of those on their way
+        look_up(0, rec, info);
+        look_up(AHEAD, next_rec, next_info);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (k < mine) fetch<G>(ring_at + k * BYTES, p.c.codes + (uint64_t)__shfl_sync(~0u, rec, k) * BYTES, lane);
+            flying[k] = __shfl_sync(~0u, info, k);
+            close_group();
+        }
+        Query<G> q;
+        State<G> s;
+        load_query<G>(p, b, first_head, n, lane, q);
+        clear(s);
+        float *put = nullptr;
+        if (p.logits) put = p.logits + (((int64_t)b * p.c.H + head) * p.most_units * 16) * p.group + cb * COLS;
+        // the slot in use and the one that is filled next, which is the one used before
+        int read = 0, write = AHEAD * BYTES;
+        for (int k0 = 0; k0 < mine; k0 += 32) {
+            rec = next_rec;
+            info = next_info;
+            look_up(k0 + 32 + AHEAD, next_rec, next_info);
+            const int left = mine - k0, now = min(32, left);
+            for (int k = 0; k < now; ++k) {
+                if (k + AHEAD < left) fetch<G>(ring_at + write, p.c.codes + (uint64_t)__shfl_sync(~0u, rec, k) * BYTES, lane);
+                close_group();
+                fetched<AHEAD>();
+                if (flying[0] & ALL) {
+                    float *to = nullptr;
+                    if (put) {
+                        const int i = i0 + warp + (k0 + k) * NW;
+                        if (i < p.most_units) to = put + (int64_t)i * 16 * p.group;
+                        else or_status(p.status, OMMX_ST_BAD_LENGTH);
+                    }
+                    attend<G, E4M3>(p, ring + read, flying[0], lane, q, s, to, n);
+                }
+#pragma unroll
+                for (int j = 0; j + 1 < AHEAD; ++j) flying[j] = flying[j + 1];
+                flying[AHEAD - 1] = __shfl_sync(~0u, info, k);
+                write = read;
+                read = read == AHEAD * BYTES ? 0 : read + BYTES;
+                __syncwarp();                     // before the slot is filled again
+            }
+        }
+        fetched<0>();
+        if constexpr (CLUSTER) {
+            finish<G, E4M3, NW>(p, s, m.sh, m.ref, m.sum, b, first_head, n, m.merged, warp, lane);
+            merge_cluster<G>(p, m.merged, b, first_head, n, warp, lane);
+            return;
+        }
+        float *part = nullptr;
+        if (i0 > 0 || i1 < units) part = p.work + HEAD + (2 * (int64_t)blockIdx.x + (base + row * units >= second)) * PART<G>;
+        finish<G, E4M3, NW>(p, s, m.sh, m.ref, m.sum, b, first_head, n, part, warp, lane);
+        u += i1 - i0;
+    }
+}
+
+// ---- parts ----------------------------------------------------------------------------------------
+template <int G> __device__ __forceinline__ const float *part_at(const DecodeParams &p, const Parts &r, int i) {
+    return p.work + HEAD + (2 * (int64_t)(r.first + i) + (i == 0 && r.late)) * PART<G>;
+}
+// Reference and sum of a head over the parts that `threads` threads of this one's kind look at, met in a warp
+template <int G> __device__ __forceinline__ void meet(const DecodeParams &p, const Parts &r, int h, int from, int threads, float &top, float &sum) {
+    constexpr int D = 32 * G;
+    top = LOWEST;
+    sum = 0.0f;
+    for (int i = from; i < (int)r.count; i += threads) {
+        const float *part = part_at<G>(p, r, i);
+        const float ref = part[COLS * D + h], s = part[COLS * D + COLS + h], m = fmaxf(top, ref);
+        sum = fmaf(s, exp2_approx(ref - m), sum * exp2_approx(top - m));
+        top = m;
+    }
+#pragma unroll
+    for (int d = 16; d; d /= 2) {
+        const float ref = __shfl_xor_sync(~0u, top, d), s = __shfl_xor_sync(~0u, sum, d), m = fmaxf(top, ref);
+        sum = fmaf(s, exp2_approx(ref - m), sum * exp2_approx(top - m));
+        top = m;
+    }
+}
+template <int G> __device__ __forceinline__ void zeros(const DecodeParams &p, int b, int hq, int lane) {      // a head of no tokens
+#pragma unroll
+    for (int i = 0; i < G; ++i) store_o(p, b * p.o_b + hq * p.o_h + lane * G + i, 0.0f);
+    if (lane == 0) store_sum(p, b, hq, LOWEST, 0.0f);
+}
+
+// Rows of which several blocks have a part, and those of no tokens, where rows are many: a block to a row, a warp to a head, a lane
+// to G channels. Grid: (rows of a sequence, sequences).
+template <int G> __global__ void __launch_bounds__(32 * COLS) kv8_combine_row_kernel(const __grid_constant__ DecodeParams p) {
+    using V = typename Floats<G>::T;
+    constexpr int D = 32 * G;
+    const int lane = threadIdx.x & 31, h = threadIdx.x >> 5, b = blockIdx.y, row = blockIdx.x;
+    const int head = row / p.col_blocks, cb = row % p.col_blocks, hq = head * p.group + cb * COLS + h;
+    const Parts r = parts_of(p, b, row, lane);
+    let_next_in();
+    if (h >= p.group - cb * COLS || r.count == 1) return;                   // not a head, or finished where it was computed
+    if (r.count == 0) { zeros<G>(p, b, hq, lane); return; }
+    float top, sum, o[G];
+    meet<G>(p, r, h, lane, 32, top, sum);
+    const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int i = 0; i < G; ++i) o[i] = 0.0f;
+    for (int i0 = 0; i0 < (int)r.count; i0 += 4) {
+        V v[4];
+        float f[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const bool on = i0 + u < (int)r.count;
+            const float *part = part_at<G>(p, r, on ? i0 + u : i0);
+            v[u] = reinterpret_cast<const V *>(part + h * D)[lane];
+            f[u] = on ? part[COLS * D + COLS + h] * exp2_approx(part[COLS * D + h] - top) * inverse : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < G; ++i) o[i] = fmaf(reinterpret_cast<const float *>(&v[u])[i], f[u], o[i]);
+    }
+    store_o(p, b * p.o_b + hq * p.o_h + lane * G, o);
+    if (lane == 0) store_sum(p, b, hq, top, sum);
+}
+
+// The same where rows are few and their parts many: a block to a head. The references and sums of all parts are read at once; then a
+// warp takes every CW-th part, UNROLL of them on their way. Grid: (rows of a sequence x COLS, sequences).
+constexpr int CW = 8, UNROLL = 5;
+template <int G> __global__ void __launch_bounds__(32 * CW) kv8_combine_head_kernel(const __grid_constant__ DecodeParams p) {
+    constexpr int D = 32 * G;
+    using V = typename Floats<G>::T;
+    __shared__ float so[CW][D], weight[MOST_PARTS], sr[CW], ss[CW];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int b = blockIdx.y, row = blockIdx.x / COLS, h = blockIdx.x % COLS;
+    const int head = row / p.col_blocks, cb = row % p.col_blocks, hq = head * p.group + cb * COLS + h;
+    const Parts r = parts_of(p, b, row, lane);
+    let_next_in();
+    const int n = r.count;
+    if (h >= p.group - cb * COLS || n == 1) return;                         // not a head, or finished where it was computed
+    if (n == 0) {
+        if (warp == 0) zeros<G>(p, b, hq, lane);
+        return;
+    }
+    V v[UNROLL];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+            if (i0 + u * CW < n) v[u] = reinterpret_cast<const V *>(part_at<G>(p, r, i0 + u * CW) + h * D)[lane];
+    };
+    load(warp);                                   // on their way while the references meet
+    float top = LOWEST, sum = 0.0f;
+    for (int i = threadIdx.x; i < n; i += 32 * CW) {
+        const float *part = part_at<G>(p, r, i);
+        weight[i] = part[COLS * D + h];
+    }
+    meet<G>(p, r, h, threadIdx.x, 32 * CW, top, sum);
+    if (lane == 0) { sr[warp] = top; ss[warp] = sum; }
+    __syncthreads();
+    top = sr[0];
+#pragma unroll
+    for (int w = 1; w < CW; ++w) top = fmaxf(top, sr[w]);
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < CW; ++w) sum = fmaf(ss[w], exp2_approx(sr[w] - top), sum);
+    const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
+    float o[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) o[i] = 0.0f;
+    for (int i0 = warp; i0 < n; i0 += CW * UNROLL) {
+        if (i0 != warp) load(i0);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+            if (i0 + u * CW < n) {
+                const float f = part_at<G>(p, r, i0 + u * CW)[COLS * D + COLS + h] * exp2_approx(weight[i0 + u * CW] - top) * inverse;
+                const float *x = reinterpret_cast<const float *>(&v[u]);
+#pragma unroll
+                for (int i = 0; i < G; ++i) o[i] = fmaf(x[i], f, o[i]);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < G; ++i) so[warp][lane * G + i] = o[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < D; c += 32 * CW) {
+        float x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < CW; ++w) x += so[w][c];
+        store_o(p, b * p.o_b + hq * p.o_h + c, x);
+    }
+    if (threadIdx.x == 0) store_sum(p, b, hq, top, sum);
+}
+
+// ---- the account ----------------------------------------------------------------------------------
+// weight = keep * before + the sum of a kv head's query heads' weights, by a thread to a token: the logits are there, and so are their
+// sums. Heads are added in order. Grid: (tokens / 256, H, sequences).
+constexpr int WEIGH_THREADS = 256;
+__global__ void __launch_bounds__(WEIGH_THREADS) kv8_weigh_kernel(const __grid_constant__ DecodeParams p) {
+    wait_earlier();
+    let_next_in();
+    const int t = blockIdx.x * WEIGH_THREADS + threadIdx.x, head = blockIdx.y, b = blockIdx.z;
+    const int len = length_of(p, b);
+    if (t >= len) return;
+    const int64_t page = page_id(p.s, b, t >> p.page_shift);
+    if (page < 0 || page >= p.c.num_pages) return;                          // reported
+    const Span span = span_of(p, len);
+    const int record = t >> 4, unit = record < span.head ? record : record - span.skip;
+    const int64_t at = (page * p.c.H + head) * p.c.page + (t & (p.c.page - 1));
+    float w = p.keep != 0.0f ? p.keep * p.before[at] : 0.0f;
+    if (visible(p, len, record) >> (t & 15) & 1) {
+        if (unit >= p.most_units) return;         // reported
+        const float *x = p.logits + ((((int64_t)b * p.c.H + head) * p.most_units + unit) * 16 + (t & 15)) * p.group;
+        const float2 *stats = p.stats + ((int64_t)b * p.c.H + head) * p.group;
+        float add = 0.0f;
+        for (int h = 0; h < p.group; ++h) {
+            const float2 s = stats[h];
+            add = fmaf(exp2_approx(x[h] - s.x), s.y, add);
+        }
+        w += add;
+    }
+    p.c.weight[at] = w;
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+static int64_t most_blocks(int warps) {
+    const int n = WARPS_PER_SM / warps * sm_count();
+    return n < MOST_PARTS ? n : MOST_PARTS;
+}
+static int64_t parts_floats(int head_dim) {
+    const int64_t part = head_dim == 64 ? PART<2> : PART<4>;
+    return HEAD + 2 * part * most_blocks(4);
+}
+// tokens that a sequence of the call can have, and records of a row
+static int64_t most_tokens(const ommx_kv8_decode_args *a) {
+    const int64_t n = (int64_t)a->seqs.pages_per_seq * a->cache.page_size;
+    return a->max_seq_len > 0 && a->max_seq_len < n ? a->max_seq_len : n;
+}
+static int64_t most_units(const ommx_kv8_decode_args *a) {
+    const int64_t n = (most_tokens(a) + 15) / 16;
+    if (a->window <= 0) return n;
+    const int64_t seen = (a->sink_tokens + 15LL) / 16 + (a->window + 15LL) / 16 + 1;
+    return n < seen ? n : seen;
+}
+static int64_t workspace_floats(const ommx_kv8_decode_args *a) {
+    const int64_t units = most_units(a);
+    int64_t n = units <= WHOLE ? 0 : parts_floats(a->cache.head_dim);
+    if (a->cache.weight) n += 2LL * a->seqs.batch * a->n_q_heads + units * 16 * a->seqs.batch * a->n_q_heads;
+    return (n + 3) / 4 * 4;
+}
+
+template <int G, bool E4M3, int NW, bool CLUSTER> static int launch_decode(const DecodeParams &p, int64_t blocks, int cluster, cudaStream_t st) {
+    static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may take its shared memory
+    int dev = 0;
+    if (int rc = current_device(&dev)) return rc;
+    if (!(allowed.load(std::memory_order_acquire) >> dev & 1)) {
+        OMMX_CUDA_TRY(cudaFuncSetAttribute(kv8_decode_kernel<G, E4M3, NW, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Memory<G, NW>)));
+        allowed.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    if (int rc = launch_dependent(kv8_decode_kernel<G, E4M3, NW, CLUSTER>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G, NW>), st, cluster, p)) return rc;
+    if (p.whole || CLUSTER) return 0;
+    // a row has some blocks / rows parts
+    const int rows = p.c.H * p.col_blocks;
+    if ((int64_t)rows * p.s.B * COLS >= blocks) return launch_dependent(kv8_combine_row_kernel<G>, dim3(rows, p.s.B), 32 * COLS, 0, st, 1, p);
+    return launch_dependent(kv8_combine_head_kernel<G>, dim3(rows * COLS, p.s.B), 32 * CW, 0, st, 1, p);
+}
+
+static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
+    if (!a) return fail(OMMX_E_ARG, "kv8_decode: null args");
+    DecodeParams p;
+    memset(&p, 0, sizeof(p));
+    if (int rc = read_cache("kv8_decode", a->cache, &p.c)) return rc;
+    if (int rc = read_seqs("kv8_decode", a->seqs, p.c, &p.s)) return rc;
+    if (a->q_dtype != OMMX_DT_BF16 && a->q_dtype != OMMX_DT_F16) return fail(OMMX_E_UNSUPPORTED, "kv8_decode: q must be bfloat16 or float16");
+    if (a->o_dtype != OMMX_DT_F32 && a->o_dtype != OMMX_DT_BF16 && a->o_dtype != OMMX_DT_F16) return fail(OMMX_E_ARG, "kv8_decode: o dtype %d", a->o_dtype);
+    if (a->n_q_heads < p.c.H || a->n_q_heads % p.c.H)
+        return fail(OMMX_E_UNSUPPORTED, "kv8_decode: %d query heads are not a multiple of %d kv heads", a->n_q_heads, p.c.H);
+    if (!(a->logit_cap >= 0.0f) || !std::isfinite(a->logit_cap)) return fail(OMMX_E_ARG, "kv8_decode: logit_cap must be finite and not negative");
+    if (!std::isfinite(a->sm_scale)) return fail(OMMX_E_ARG, "kv8_decode: sm_scale must be finite");
+    if (a->window < 0 || a->sink_tokens < 0 || a->max_seq_len < 0) return fail(OMMX_E_ARG, "kv8_decode: window, sink_tokens and max_seq_len must not be negative");
+    if (a->cache.weight && (!std::isfinite(a->keep) || (a->keep != 0.0f && !a->weight_before))) return fail(OMMX_E_ARG, "kv8_decode: keep must be finite, and what is kept must be given");
+    if (p.s.B > 65535 || p.c.H > 65535) return fail(OMMX_E_UNSUPPORTED, "kv8_decode: a batch of %d", p.s.B);
+    if (p.s.B == 0) return 0;
+    if (!a->q || !a->o || !a->lse) return fail(OMMX_E_ARG, "kv8_decode: q, o and lse must not be null");
+    const int64_t need = workspace_floats(a);
+    if (need && (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 || a->workspace_floats < need))
+        return fail(OMMX_E_ARG, "kv8_decode: workspace must be 16-byte aligned and hold %lld floats", (long long)need);
+    p.q = a->q; p.q16 = a->q_dtype == OMMX_DT_F16; p.q_b = a->q_stride_b; p.q_h = a->q_stride_h;
+    p.q_wide = (reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)(2 * p.q_b) | (uintptr_t)(2 * p.q_h)) % 16 == 0;
+    p.o = a->o; p.o_type = a->o_dtype; p.o_b = a->o_stride_b; p.o_h = a->o_stride_h;
+    p.lse = a->lse; p.lse_b = a->lse_stride_b;
+    p.group = a->n_q_heads / p.c.H; p.col_blocks = (p.group + COLS - 1) / COLS;
+    p.page_shift = shift_of(p.c.page);
+    p.window = a->window; p.sinks = a->sink_tokens;
+    p.sm_scale = a->sm_scale; p.cap = a->logit_cap; p.status = a->status;
+    if (p.c.num_pages == 0) return fail(OMMX_E_ARG, "kv8_decode: a cache of no pages");   // what is fetched for a page that is not there
+    // as many blocks as the SMs hold, no more than the work can have
+    const int64_t units = most_units(a);
+    const int64_t rows = (int64_t)p.s.B * p.c.H * p.col_blocks;
+    if (units * rows >= 1LL << 31 || rows * COLS >= 1LL << 31)
+        return fail(OMMX_E_UNSUPPORTED, "kv8_decode: %lld rows of up to %lld records (2^31 in all are counted): give max_seq_len", (long long)rows, (long long)units);
+    p.most_units = (int)units;
+    p.work = a->workspace;
+    if (p.c.weight) {
+        p.stats = reinterpret_cast<float2 *>(a->workspace + (units <= WHOLE ? 0 : parts_floats(a->cache.head_dim)));
+        p.logits = reinterpret_cast<float *>(p.stats + (int64_t)p.s.B * a->n_q_heads);
+        p.before = a->weight_before; p.keep = a->keep;
+    }
+    // Blocks of eight warps where rows are few, so that a row has few parts, of four where they are many: then blocks often go on from
+    // one row to the next, and an SM's others work meanwhile. As many blocks as the SMs hold, no more than the work can have. Rows that
+    // are short for certain go whole to a block each, and the second kernel is not needed.
+    const int warps = rows >= 64 ? 4 : 8;
+    p.least = 2 * warps;
+    const int64_t most = (units * rows + p.least - 1) / p.least, hold = most_blocks(warps);
+    // Rows of middling length, and few, go to a cluster of eight-warp blocks each, as many as fit at once: no second kernel
+    int cluster = 1;
+    while (cluster < MOST_CLUSTER && 2 * cluster * rows <= most_blocks(8)) cluster *= 2;
+    if (units > 32 * cluster) cluster = 1;
+    p.whole = units <= WHOLE / 2 || (units <= WHOLE && cluster == 1);
+    if (p.whole) cluster = 1;
+    const int64_t blocks = p.whole ? rows : cluster > 1 ? cluster * rows : most < 1 ? 1 : most < hold ? most : hold;
+    auto launch = [&](auto g, auto e4m3) {
+        constexpr int G = decltype(g)::value;
+        constexpr bool E4M3 = decltype(e4m3)::value;
+        if (cluster > 1) return launch_decode<G, E4M3, 8, true>(p, blocks, cluster, st);
+        return warps == 4 ? launch_decode<G, E4M3, 4, false>(p, blocks, 1, st) : launch_decode<G, E4M3, 8, false>(p, blocks, 1, st);
+    };
+    using std::integral_constant;
+    int rc;
+    if (a->cache.code == OMMX_KV8_E4M3)
+        rc = a->cache.head_dim == 128 ? launch(integral_constant<int, 4>(), std::true_type()) : launch(integral_constant<int, 2>(), std::true_type());
+    else
+        rc = a->cache.head_dim == 128 ? launch(integral_constant<int, 4>(), std::false_type()) : launch(integral_constant<int, 2>(), std::false_type());
+    const int64_t tokens = most_tokens(a);
+    if (rc || !p.c.weight || !tokens) return rc;
+    return launch_dependent(kv8_weigh_kernel, dim3((unsigned)((tokens + WEIGH_THREADS - 1) / WEIGH_THREADS), p.c.H, p.s.B), WEIGH_THREADS, 0, st, 1, p);
+}
+
+}  // namespace kv8
+}  // namespace ommx
+
+extern "C" int64_t ommx_b200_kv8_decode_workspace_floats(const ommx_kv8_decode_args *args) {
+    return !args || (args->cache.head_dim != 64 && args->cache.head_dim != 128) ? 0 : ommx::kv8::workspace_floats(args);
+}
+extern "C" int ommx_b200_kv8_decode(const ommx_kv8_decode_args *args, void *stream) { return ommx::kv8::decode(args, (cudaStream_t)stream); }

@@ -1,0 +1,111 @@
+// How the paged caches' attention kernels deal their work out, and where a row's parts meet.  P: a kernel's parameters, with s.B, c.H,
+// col_blocks, least, work and status, for which length_of(p, b) and units_of(p, length) say how many units sequence b has.
+#pragma once
+
+#include "ommx_kv4.cuh"
+
+namespace ommx {
+namespace kv {
+
+// Units are records (16 tokens of a kv head, for a block of its query heads); a row (sequence, kv head, block of heads) is a run of
+// them. Lengths are known on the device alone, so every block works the same deal out, and leaves it for the second kernel:
+// * a block to a row, where the host knows that rows are short (`whole`), or a cluster of blocks, which exchange their parts themselves;
+// * else every row is cut into pieces of at most `per` units, a block to a piece, with the smallest `per` for which there are blocks
+//   enough;
+// * or, where that would leave a block with over BEGIN units more than an even share, all rows end to end are cut into such shares,
+//   whatever rows they touch. A second piece costs a block some 4 us, half of it hidden by the SM's other blocks (4-bit cache, 64K tokens:
+//   26.7 us with seven such blocks of 296, 24.4 with none; 64 sequences of 200..2000 tokens: 43.3 with even shares, 38.3 with pieces).
+// A piece that is a whole row is finished where it is computed; the others' parts meet in the second kernel. A block has at most two
+// of those, of the row that an earlier block began (its slot 0) and of the one that a later block goes on with (slot 1).
+constexpr uint32_t OVER = 2;                      // in the deal's place: there is none
+constexpr int BEGIN = 64, HEAD = 4;               // HEAD: floats in front of the parts, which hold the deal
+struct Deal { uint32_t per, total; bool pieces, over; };   // over: lengths far past max_seq_len, of more units than 32 bits count
+__device__ __forceinline__ uint32_t pieces_of(uint32_t units, uint32_t per) { return (units + per - 1) / per; }
+template <typename P> __device__ __forceinline__ Deal deal(const P &p, uint32_t rows, uint32_t blocks, int lane) {
+    uint64_t sum = 0;
+    uint32_t some = 0, most = 0;
+    const uint32_t own = lane < p.s.B ? units_of(p, length_of(p, lane)) : 0;
+    for (int b = lane; b < p.s.B; b += 32) {
+        const uint32_t n = b == lane ? own : units_of(p, length_of(p, b));
+        sum += n;
+        some += n > 0;
+        most = max(most, n);
+    }
+    Deal d;
+#pragma unroll
+    for (int i = 16; i; i /= 2) sum += __shfl_xor_sync(~0u, sum, i);
+    d.over = sum * rows >> 31;
+    d.total = d.over ? 0 : (uint32_t)sum * rows;
+    const uint32_t full = __reduce_add_sync(~0u, some) * rows;
+    most = __reduce_max_sync(~0u, most);
+    const uint32_t even = max((d.total + blocks - 1) / blocks, (uint32_t)p.least);
+    d.per = even;
+    d.pieces = false;
+    if (d.over) or_status(p.status, OMMX_ST_BAD_LENGTH);
+    if (d.over || full == 0 || full > blocks) return d;
+    // pieces of `per` take total / per + full blocks at most; fewer may do
+    uint32_t lo = even, hi = min(max(most, even), full < blocks ? max(even, d.total / (blocks - full) + 1) : 0xFFFFFFFFu);
+#pragma unroll 1
+    for (int i = 0; i < 6 && lo < hi; ++i) {
+        const uint32_t per = i == 0 ? lo : (lo + hi) / 2;
+        uint32_t n = pieces_of(own, per);
+        for (int b = lane + 32; b < p.s.B; b += 32) n += pieces_of(units_of(p, length_of(p, b)), per);
+        if (__reduce_add_sync(~0u, n) * rows <= blocks) hi = per;
+        else lo = per + 1;
+    }
+    if (hi <= even + BEGIN) { d.per = hi; d.pieces = true; }
+    return d;
+}
+
+// Where the parts of a row are: those of blocks first .. first + count - 1, the first one in its slot 1 if `late`. A whole warp calls
+// it, before the wait for the first kernel: this one starts when every block of that has waited for what came earlier, so the lengths
+// are there, and only the deal is not.
+struct Parts { uint32_t first, count; bool late; };
+template <typename P> __device__ __forceinline__ Parts parts_of(const P &p, int b, uint32_t row, int lane) {
+    const uint32_t rows = p.c.H * p.col_blocks, units = units_of(p, length_of(p, b)), own = lane < b ? units_of(p, length_of(p, lane)) : 0;
+    kv4::wait_earlier();
+    const uint2 d = *reinterpret_cast<const uint2 *>(p.work);
+    uint32_t before = d.y ? pieces_of(own, d.x) : own;
+    for (int i = lane + 32; i < b; i += 32) {
+        const uint32_t v = units_of(p, length_of(p, i));
+        before += d.y ? pieces_of(v, d.x) : v;
+    }
+    before = __reduce_add_sync(~0u, before) * rows;
+    Parts r;
+    if (units == 0 || d.y == OVER) return {0, 0, false};
+    if (d.y) {
+        r.count = pieces_of(units, d.x);
+        r.first = before + row * r.count;
+        r.late = false;
+    } else {
+        const uint32_t r0 = before + row * units;
+        r.first = r0 / d.x;
+        r.count = (r0 + units - 1) / d.x - r.first + 1;
+        r.late = true;                            // the first part's block is the one that holds the row's first unit
+    }
+    return r;
+}
+
+// ---- clusters -------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 peer_float4(uint32_t at, uint32_t rank) {
+    uint32_t there;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
+    return v;
+}
+__device__ __forceinline__ float peer_float(uint32_t at, uint32_t rank) {
+    uint32_t there;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+    return v;
+}
+
+}  // namespace kv
+}  // namespace ommx
