@@ -584,8 +584,6 @@ typedef struct ommx_kv8_evict_args {
     int32_t *kept;                  /* out [batch, n_kv_heads, budget]: the places that were kept, ascending, then -1 */
     int32_t budget, sink_tokens, recent_tokens;
     int32_t *len_out;               /* [batch]: min(b_seq_len, budget); may be b_seq_len, or NULL */
-    void *workspace;                /* ommx_b200_kv8_evict_workspace_bytes() of them, 16-byte aligned */
-    int64_t workspace_bytes;
     int32_t max_seq_len;            /* an upper bound of b_seq_len that sizes the launch, 0: what the table can hold */
     int32_t *status;
 } ommx_kv8_evict_args;
@@ -594,10 +592,10 @@ typedef struct ommx_kv8_evict_args {
  * Keep `budget` tokens of each sequence and kv head: the first sink_tokens, the last recent_tokens and of the others those of the largest
  * weight (ties to the lower place, NaN last), moved with their weights to the places 0 .. budget - 1 in their order.  A record of kept
  * tokens has the largest E that they had; codes are rounded to that.  A sequence of at most `budget` tokens keeps all; one with a page out
- * of range, or more tokens than its tables hold, is reported and stays as it is.  Two launches.
+ * of range, or more tokens than its tables hold, is reported and stays as it is.  One launch; two where
+ * len_out is b_seq_len.
  */
 int ommx_b200_kv8_evict(const ommx_kv8_evict_args *args, void *stream);
-int64_t ommx_b200_kv8_evict_workspace_bytes(int32_t batch, int32_t n_kv_heads, int32_t budget);
 
 #ifdef __cplusplus
 }

@@ -155,8 +155,8 @@ class KV8DecodeArgs(C.Structure):
 class KV8EvictArgs(C.Structure):
     _fields_ = [("cache", KV8Cache), ("seqs", KV4Seqs), ("to_table", C.c_void_p), ("to_table_stride", C.c_int64),
                 ("to_table_is_int64", C.c_int32), ("to_pages_per_seq", C.c_int32), ("kept", C.c_void_p), ("budget", C.c_int32),
-                ("sink_tokens", C.c_int32), ("recent_tokens", C.c_int32), ("len_out", C.c_void_p), ("workspace", C.c_void_p),
-                ("workspace_bytes", C.c_int64), ("max_seq_len", C.c_int32), ("status", C.c_void_p)]
+                ("sink_tokens", C.c_int32), ("recent_tokens", C.c_int32), ("len_out", C.c_void_p), ("max_seq_len", C.c_int32),
+                ("status", C.c_void_p)]
 
 
 class LaunchPlan(C.Structure):
@@ -191,7 +191,6 @@ SYMBOLS = {
     "ommx_b200_kv8_decode": (C.c_int, [C.POINTER(KV8DecodeArgs), C.c_void_p]),
     "ommx_b200_kv8_decode_workspace_floats": (C.c_int64, [C.POINTER(KV8DecodeArgs)]),
     "ommx_b200_kv8_evict": (C.c_int, [C.POINTER(KV8EvictArgs), C.c_void_p]),
-    "ommx_b200_kv8_evict_workspace_bytes": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
     "ommx_b200_peer_alloc": (C.c_int, [C.c_size_t, C.POINTER(C.c_void_p), C.c_void_p]),
     "ommx_b200_peer_open": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "ommx_b200_peer_close": (C.c_int, [C.c_void_p]),

@@ -108,7 +108,7 @@ def ommx_kv8_decode_attention(q: torch.Tensor, codes: torch.Tensor, scales: torc
 
 def ommx_kv8_evict(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, page_table: torch.Tensor, b_seq_len: torch.Tensor,
                    kept: torch.Tensor, *, sink_tokens: int = 0, recent_tokens: int = 0, to_table: Optional[torch.Tensor] = None,
-                   len_out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, max_seq_len: Optional[int] = None,
+                   len_out: Optional[torch.Tensor] = None, max_seq_len: Optional[int] = None,
                    status: Optional[torch.Tensor] = None) -> None:
     """Keep ``kept.shape[2]`` tokens of each sequence and kv head, and move them with their weights to the front, in their order.
 
@@ -116,10 +116,9 @@ def ommx_kv8_evict(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tens
     place; NaN last); all of a sequence that has no more.  ``kept`` (int32 ``[batch, n_kv_heads, n]``) gets their places, ascending, then
     -1; ``len_out`` (int32 ``[batch]``, may be ``b_seq_len``) the new lengths.  They take the first pages of the sequence itself or,
     with ``to_table`` (int32 or int64 ``[batch, pages]``), pages that no sequence holds, and then the old ones are left as they were (a
-    prefix that sequences share).  ``max_seq_len`` sizes the launch; ``workspace``: uint8,
-    ``kv8_evict_workspace_bytes(batch, n_kv_heads, n)``; calls that run side by side need their own."""
+    prefix that sequences share).  ``max_seq_len`` sizes the launch."""
     _check((_HOST or _host()).kv8_evict(codes, scales, weight, page_table, b_seq_len, kept, sink_tokens, recent_tokens, to_table, len_out,
-                                        workspace, max_seq_len, status), "ommx_b200_kv8_evict")
+                                        max_seq_len, status), "ommx_b200_kv8_evict")
 
 
 def kv8_workspace_floats(batch: int, n_q_heads: int, head_dim: int, max_seq_len: int, *, window: Optional[int] = None, sink_tokens: int = 0,
@@ -133,10 +132,5 @@ def kv8_workspace_floats(batch: int, n_q_heads: int, head_dim: int, max_seq_len:
     return int(_lib.load().ommx_b200_kv8_decode_workspace_floats(_lib.C.byref(a)))
 
 
-def kv8_evict_workspace_bytes(batch: int, n_kv_heads: int, tokens: int) -> int:
-    """Bytes of workspace that ``ommx_kv8_evict`` needs to keep so many tokens."""
-    return int(_lib.load().ommx_b200_kv8_evict_workspace_bytes(batch, n_kv_heads, tokens))
-
-
 __all__ = ["ommx_kv8_alloc", "ommx_kv8_append", "ommx_kv8_gather", "ommx_kv8_decode_attention", "ommx_kv8_evict",
-           "kv8_workspace_floats", "kv8_evict_workspace_bytes"]
+           "kv8_workspace_floats"]

@@ -1060,11 +1060,11 @@ PyObject *py_kv8_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// kv8_evict(codes, scales, weight, page_table, b_seq_len, kept, sink_tokens, recent_tokens, to_table, len_out, workspace, max_seq_len, status)
+// kv8_evict(codes, scales, weight, page_table, b_seq_len, kept, sink_tokens, recent_tokens, to_table, len_out, max_seq_len, status)
 PyObject *py_kv8_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     KV4_TRY
-    if (n != 13) { PyErr_SetString(PyExc_TypeError, "kv8_evict: wrong argument count"); return nullptr; }
+    if (n != 12) { PyErr_SetString(PyExc_TypeError, "kv8_evict: wrong argument count"); return nullptr; }
     KV8Call c{{"ommx_kv8_evict"}};
     ommx_kv8_evict_args d;
     memset(&d, 0, sizeof(d));
@@ -1087,14 +1087,9 @@ PyObject *py_kv8_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
         KV4_EXPECT(c, t->dim() == 1 && t->scalar_type() == at::kInt && t->is_contiguous() && t->size(0) == B, "len_out must be a contiguous int32 tensor [batch]");
         d.len_out = (int32_t *)t->data_ptr();
     }
-    if (a[11] != Py_None) d.max_seq_len = (int32_t)c.integer(a[11], "max_seq_len", 0);
-    d.status = c.status(a[12]);
-    if (a[10] != Py_None) c.tensor(a[10], "workspace");
-    const at::Device dev = c.device();
-    Tensor own;
-    d.workspace_bytes = ommx_b200_kv8_evict_workspace_bytes(d.seqs.batch, d.cache.n_kv_heads, d.budget);
-    d.workspace = c.workspace(a[10], at::kByte, d.workspace_bytes, dev, &own);
-    return PyLong_FromLong(launch(dev, [&](void *stream) { return ommx_b200_kv8_evict(&d, stream); }));
+    if (a[10] != Py_None) d.max_seq_len = (int32_t)c.integer(a[10], "max_seq_len", 0);
+    d.status = c.status(a[11]);
+    return PyLong_FromLong(launch(c.device(), [&](void *stream) { return ommx_b200_kv8_evict(&d, stream); }));
     KV4_END
     END_HANDLE_TH_ERRORS
 }

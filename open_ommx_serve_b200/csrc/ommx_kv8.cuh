@@ -84,14 +84,39 @@ template <bool E4M3> __device__ __forceinline__ void numbers_of(uint32_t w, floa
         x[3] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7443)) - 8388736.0f;
     }
 }
-// the same codes in a scale 1 / ratio times as large
-template <bool E4M3> __device__ __forceinline__ uint32_t rescaled(uint32_t w, float ratio) {
-    float x[4];
-    numbers_of<E4M3>(w, x);
-    return codes_of<E4M3>(x[0] * ratio, x[1] * ratio, x[2] * ratio, x[3] * ratio);
+// The same codes in a scale 2^by times as large, by >= 1; all is fp16: codes are fp16 numbers, and where a product has more bits than they
+// it rounds to 0 either way. E = 0: the codes stand for zeros.
+struct Rescale { __half2 ratio; };
+__device__ __forceinline__ Rescale rescale_by(int held, int E) {
+    return {__float2half2_rn(ratio_of(held, E))};  // below 2^-24 it is 0, and so are the codes
 }
-template <bool E4M3> __device__ __forceinline__ uint4 rescaled(uint4 w, float ratio) {
-    return make_uint4(rescaled<E4M3>(w.x, ratio), rescaled<E4M3>(w.y, ratio), rescaled<E4M3>(w.z, ratio), rescaled<E4M3>(w.w, ratio));
+template <bool E4M3> __device__ __forceinline__ uint32_t rescaled(uint32_t w, const Rescale &by) {
+    if constexpr (E4M3) {
+        const uint32_t h[2] = {half2_of_e4m3x2(w), half2_of_e4m3x2(w >> 16)};
+        uint32_t r[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const __half2 x = __hmul2(*reinterpret_cast<const __half2 *>(&h[i]), by.ratio);
+            uint16_t e;
+            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(e) : "r"(*reinterpret_cast<const uint32_t *>(&x)));
+            r[i] = e;
+        }
+        return r[0] | r[1] << 16;
+    } else {
+        const uint32_t u = w ^ 0x80808080u;       // 1024 + 128 + code as an fp16 number; the last byte of 1536 + code, rounded as a sum is
+        const __half2 off = __float2half2_rn(1152.0f), round = __float2half2_rn(1536.0f);
+        const uint32_t h[2] = {__byte_perm(u, 0x64646464u, 0x4140), __byte_perm(u, 0x64646464u, 0x4342)};
+        uint32_t r[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const __half2 x = __hfma2(__hsub2(*reinterpret_cast<const __half2 *>(&h[i]), off), by.ratio, round);
+            r[i] = *reinterpret_cast<const uint32_t *>(&x);
+        }
+        return __byte_perm(r[0], r[1], 0x6420);
+    }
+}
+template <bool E4M3> __device__ __forceinline__ uint4 rescaled(uint4 w, const Rescale &by) {
+    return make_uint4(rescaled<E4M3>(w.x, by), rescaled<E4M3>(w.y, by), rescaled<E4M3>(w.z, by), rescaled<E4M3>(w.w, by));
 }
 
 // ---- host: arguments every entry point checks ----

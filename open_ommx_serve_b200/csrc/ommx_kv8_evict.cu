@@ -1,13 +1,13 @@
 // The 8-bit cache: eviction by what tokens were attended to with.
 //
 // Of a sequence of more than `budget` tokens each kv head keeps the first `sinks`, the last `recent` and, of those between, the ones of the
-// largest weight (ties to the lowest place), and they move to the places 0 .. budget - 1 in their order. Two kernels:
-// * pick: the weights' order is that of whole numbers, of which the want-th largest is found by counting: what lies between the smallest
-//   and the largest is cut into 2048 equal parts, and the part that holds it again, three times at most. A cluster of blocks shares a
-//   long row, each with a stretch of its keys in shared memory; counts meet in distributed shared memory. It also notes down what the
-//   moved rows' scales are and will be, so that the scales in the cache are read before they are written.
-// * move: places ascend, and a token never moves up, so a block that reads what a stretch of places takes before it writes that stretch
-//   can work where the tokens lie. Channels do not meet: a row (sequence, kv head) is cut into columns of 32 bytes, a block to each.
+// largest weight (ties to the lowest place), and they move to the places 0 .. budget - 1 in their order. A cluster of blocks to a row
+// (sequence, kv head):
+// * picks: the weights' order is that of whole numbers, of which the want-th largest is found by counting: what lies between the smallest
+//   and the largest is cut into 2048 equal parts, and the part that holds it again, until so few are left that each block takes all of them
+//   and goes on alone. A thread holds its first keys in registers; counts meet in distributed shared memory.
+// * moves: places ascend, and a token never moves up. So once a cluster has read all that a stretch of places takes into its shared
+//   memory it can write that stretch where the tokens lie, and go on to the next.
 #include "ommx_kv8.cuh"
 #include "ommx_kv_deal.cuh"
 
@@ -16,21 +16,22 @@ namespace kv8 {
 
 using namespace kv;
 
-constexpr int PICK_THREADS = 1024, PICK_WARPS = PICK_THREADS / 32, BINS = 2048, MOST_CLUSTER = 8;
-constexpr int MOST_KEYS = 48 * 1024;              // keys that a block holds at most; it reads others again
+constexpr int THREADS = 1024, WARPS = THREADS / 32, BINS = 2048, MOST_CLUSTER = 8;
+constexpr int HELD = 8, TURN = THREADS * HELD;    // keys that a thread holds; a block's turn of keys, a warp has 32 HELD in a row of it
+constexpr int MOST_KEYS = 40 * 1024;              // further keys that a block holds in shared memory; it reads others again
+constexpr int FEW = 4096;                         // keys that each block of a cluster finishes for itself
+constexpr int PLACES = 512;                       // that a block moves at a time
 
 struct EvictParams {
     Cache c;
     Seqs s, to;                                   // `to`: where kept tokens go; only its table
     int32_t *kept, *len_out;
-    int2 *counts;                                 // [B][H]: tokens to move, tokens that are left
-    uint16_t *scales;                             // [B][H][places, places / 16]: of what a place takes, and of its record
-    int32_t budget, sinks, recent, places, keys, page_shift, in_place;      // places: budget up to whole records; keys: that a block holds
+    int32_t budget, sinks, recent, keys, page_shift, in_place;              // keys: behind its first turn that a block holds
     int32_t *status;
 };
-__device__ __forceinline__ int64_t record_of(const EvictParams &p, const Seqs &s, int b, int head, int at) {
-    const int64_t page = page_id(s, b, at >> p.page_shift);
-    return (page * p.c.H + head) * p.c.parts + (at >> 4 & (p.c.parts - 1));
+// row `at` of a sequence's kv head: 16 to a record. Below 2^32: there is no memory for more
+__device__ __forceinline__ uint32_t row_of(const EvictParams &p, int64_t page, int head, int at) {
+    return (uint32_t)((page * p.c.H + head) * p.c.page) + (at & (p.c.page - 1));
 }
 // weights as whole numbers in their order; NaN comes last, and zeros are one
 __device__ __forceinline__ uint32_t ordered(float w) {
@@ -41,112 +42,229 @@ __device__ __forceinline__ uint32_t peer_word(const void *at, uint32_t rank) {
     return __float_as_uint(peer_float((uint32_t)__cvta_generic_to_shared(at), rank));
 }
 
+// What a block knows of the places that it moves
+struct Place { uint32_t from, to; float weight; uint16_t own, scales; };    // rows; exponents of what it takes, and of its record
+
 // Grid: (cluster x H, B).
-__global__ void __launch_bounds__(PICK_THREADS) kv8_pick_kernel(const __grid_constant__ EvictParams p) {
-    extern __shared__ __align__(16) uint32_t keys[];
-    __shared__ int histogram[BINS], warp_sum[2][PICK_WARPS];
-    __shared__ uint32_t low, high;
-    __shared__ int bin, left, more, same, bad;
+template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict_kernel(const __grid_constant__ EvictParams p) {
+    constexpr int D = 32 * G;
+    extern __shared__ __align__(16) uint8_t memory[];                       // keys, then rows
+    uint32_t *keys = reinterpret_cast<uint32_t *>(memory);
+    __shared__ __align__(16) int histogram[BINS];
+    __shared__ uint32_t few[FEW];
+    __shared__ Place places[PLACES];
+    __shared__ int warp_sum[2][WARPS], starts[MOST_CLUSTER + 1], bin, left, inside, listed, more, same, above_here, equal_here, bad, spoilt;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t n = cluster_size(), rank = cluster_rank();
     const int head = blockIdx.x / n, b = blockIdx.y;
-    if (tid == 0) { low = ~0u; high = 0; bad = 0; more = same = 0; }
-    histogram[tid] = histogram[tid + PICK_THREADS] = 0;
+    if (tid == 0) bad = listed = 0;
+    histogram[tid] = histogram[tid + THREADS] = 0;
     wait_earlier();
     let_next_in();
-    int len = p.s.len[b];
+    const int given = p.s.len[b];
     const int64_t room = (int64_t)p.s.max_pages << p.page_shift;
-    int faults = len < 0 || len > room ? OMMX_ST_BAD_LENGTH : 0;
-    if (faults) len = len < 0 ? 0 : (int)room;
-    const int keep = min(len, p.budget);
+    int faults = given < 0 || given > room ? OMMX_ST_BAD_LENGTH : 0;
+    const int len = faults ? 0 : given, keep = min(len, p.budget);
     if (keep > (int64_t)p.to.max_pages << p.page_shift) faults |= OMMX_ST_BAD_LENGTH;
     __syncthreads();
-    // a sequence whose pages are not all there stays as it is: every block of it sees that
+    const bool all = len <= p.budget;
+    int32_t *out = p.kept + ((int64_t)b * p.c.H + head) * p.budget;
+    auto there = [&](int64_t id) { return id >= 0 && id < p.c.num_pages; };
+    // A sequence whose pages are not all there stays as it is, for all of its heads: every block looks at some, and hears of the others'
     if (!faults) {
         bool off = false;
-        for (int i = tid; (int64_t)i << p.page_shift < len; i += PICK_THREADS) { const int64_t id = page_id(p.s, b, i); off |= id < 0 || id >= p.c.num_pages; }
-        for (int i = tid; (int64_t)i << p.page_shift < keep; i += PICK_THREADS) { const int64_t id = page_id(p.to, b, i); off |= id < 0 || id >= p.c.num_pages; }
+        for (int i = rank * THREADS + tid; (int64_t)i << p.page_shift < keep; i += n * THREADS) off |= !there(page_id(p.to, b, i));
+        if (all)
+            for (int i = rank * THREADS + tid; (int64_t)i << p.page_shift < len; i += n * THREADS) off |= !there(page_id(p.s, b, i));
         if (off) bad = 1;
-        __syncthreads();
-        if (bad) faults = OMMX_ST_BAD_PAGE;
     }
-    int32_t *out = p.kept + ((int64_t)b * p.c.H + head) * p.budget;
-    const int share = ((len + (int)n - 1) / (int)n + 31) & ~31, lo = min(len, (int)rank * share), hi = min(len, lo + share);
-    const int moved = faults || (p.in_place && len <= p.budget) ? 0 : keep;
-    if (rank == 0 && tid == 0) {
-        p.counts[(int64_t)b * p.c.H + head] = make_int2(moved, faults ? p.s.len[b] : keep);
-        if (faults) or_status(p.status, faults);
-    }
-    if (faults || len <= p.budget) {
-        for (int i = rank * PICK_THREADS + tid; i < p.budget; i += n * PICK_THREADS) out[i] = !faults && i < len ? i : -1;
-        if (!moved) return;
-    } else {
-        const float *weight = p.c.weight;
-        auto load = [&](int i) { return ordered(weight[record_of(p, p.s, b, head, i) * BLOCK + (i & 15)]); };
-        auto key_at = [&](int i) { return i - lo < p.keys ? keys[i - lo] : load(i); };
-        // keys that are not kept anyway: [first, last) of this block's
-        const int first = max(lo, p.sinks), last = min(hi, len - p.recent);
-        uint32_t a = ~0u, z = 0;
-        for (int i = lo + tid; i < hi; i += PICK_THREADS) {
-            const uint32_t k = load(i);
-            if (i - lo < p.keys) keys[i - lo] = k;
-            if (i >= first && i < last) { a = min(a, k); z = max(z, k); }
+    auto hear = [&] {                             // behind a barrier of the cluster
+        if (warp == 0) {
+            const bool off = __any_sync(~0u, lane < (int)n && peer_word(&bad, lane % n) != 0);
+            if (lane == 0) spoilt = off;
         }
-        a = __reduce_min_sync(~0u, a);
-        z = __reduce_max_sync(~0u, z);
-        if (lane == 0) { atomicMin(&low, a); atomicMax(&high, z); }
+    };
+    auto leave = [&](bool listed) {               // the list and the length of a sequence that is not evicted from
+        if (rank == 0 && tid == 0) {
+            if (faults) or_status(p.status, faults);
+            if (head == 0 && p.len_out) p.len_out[b] = faults ? given : keep;
+        }
+        if (listed)
+            for (int i = rank * THREADS + tid; i < p.budget; i += n * THREADS) out[i] = !faults && i < len ? i : -1;
+    };
+    if (faults) { leave(true); return; }
+    if (all) {
         __syncthreads();
         cluster_barrier();
-        for (uint32_t r = 0; r < n; ++r) { a = min(a, peer_word(&low, r)); z = max(z, peer_word(&high, r)); }
-        a = __reduce_min_sync(~0u, a);
-        z = __reduce_max_sync(~0u, z);
-        // the want-th largest of the keys from `a` on, below a + 2^width
-        int want = p.budget - p.sinks - p.recent, width = 32 - __clz(z - a);
-        if (want == 0) a = ~0u, width = 0;
-        while (width > 0) {
-            const int shift = max(0, width - 11);
-            for (int i = first + tid; i < last; i += PICK_THREADS) {
-                const uint32_t k = key_at(i) - a;
-                if (width == 32 || k >> width == 0) atomicAdd(&histogram[k >> shift], 1);
+        hear();
+        cluster_barrier();
+        if (spoilt) faults = OMMX_ST_BAD_PAGE;
+        leave(true);
+        if (faults || p.in_place) return;
+    } else {
+        // block `rank` has the keys lo .. hi - 1; first .. last - 1 of them are not kept anyway
+        const int share = ((len + (int)n - 1) / (int)n + 31) & ~31, lo = min(len, (int)rank * share), hi = min(len, lo + share);
+        const int first = max(lo, p.sinks), last = min(hi, len - p.recent);
+        const float *weight = p.c.weight;
+        auto load = [&](int i) {
+            const int64_t page = page_id(p.s, b, i >> p.page_shift);
+            return there(page) ? ordered(weight[row_of(p, page, head, i)]) : 0u;
+        };
+        auto place = [&](int turn, int u) { return lo + turn * TURN + warp * (32 * HELD) + u * 32 + lane; };
+        const int turns = (hi - lo + TURN - 1) / TURN;
+        uint32_t held[HELD];
+        bool off = false;
+        for (int turn = 0; turn < turns; ++turn) {
+            int64_t page[HELD];
+            float w[HELD];
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) page[u] = place(turn, u) < hi ? page_id(p.s, b, place(turn, u) >> p.page_shift) : 0;
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) {
+                off |= !there(page[u]);
+                w[u] = place(turn, u) < hi && there(page[u]) ? weight[row_of(p, page[u], head, place(turn, u))] : 0.0f;
             }
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) {
+                const int i = place(turn, u) - lo - TURN;
+                if (turn == 0) held[u] = ordered(w[u]);
+                else if (i < hi - lo - TURN && i < p.keys) keys[i] = ordered(w[u]);
+            }
+        }
+        auto key_at = [&](int i) { return i - lo - TURN < p.keys ? keys[i - lo - TURN] : load(i); };      // behind the first turn
+        // f(key) for each of the thread's keys that is not kept anyway
+        auto each_key = [&](auto f) {
+#pragma unroll
+            for (int u = 0; u < HELD; ++u)
+                if (place(0, u) >= first && place(0, u) < last) f(held[u]);
+            for (int turn = 1; turn < turns; ++turn)
+                for (int u = 0; u < HELD; ++u)
+                    if (place(turn, u) >= first && place(turn, u) < last) f(key_at(place(turn, u)));
+        };
+        if (off) bad = 1;
+        __syncthreads();
+        // The want-th largest of the keys from `a` on, below a + 2^width. First of those above 0, all others taken for the lowest of them; of all
+        // where it is one of these.
+        constexpr uint32_t ZERO = 0x80000000u;
+        const int wanted = p.budget - p.sinks - p.recent;
+        int want = wanted, width = 31;
+        uint32_t a = ZERO;
+        for (bool begun = false; width > 0; begun = true) {
+            const int shift = max(0, width - 11);
+            // the lowest part is not counted: what is not above it is in it, and often it is the one that most are in
+            each_key([&](uint32_t key) {
+                const uint32_t k = key - a;
+                if (key >= a && (width == 32 || k >> width == 0) && k >> shift) atomicAdd(&histogram[k >> shift], 1);
+            });
             __syncthreads();
             cluster_barrier();
-            // from the top: thread t has bins BINS - 1 - 2 t and the one below
-            int upper = 0, lower = 0;
-            for (uint32_t r = 0; r < n; ++r) {
-                upper += (int)peer_word(&histogram[BINS - 1 - 2 * tid], r);
-                lower += (int)peer_word(&histogram[BINS - 2 - 2 * tid], r);
+            if (!begun) hear();
+            // from the top: thread t has bins BINS - 1 - 4 t and the three below
+            int4 mine = make_int4(0, 0, 0, 0);
+            if (tid < BINS / 4) {
+                const uint32_t at = (uint32_t)__cvta_generic_to_shared(&histogram[BINS - 4 - 4 * tid]);
+                float4 v[MOST_CLUSTER];
+#pragma unroll
+                for (int r = 0; r < MOST_CLUSTER; ++r) v[r] = r < (int)n ? peer_float4(at, r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int r = 0; r < MOST_CLUSTER; ++r) {
+                    mine.x += __float_as_int(v[r].x); mine.y += __float_as_int(v[r].y); mine.z += __float_as_int(v[r].z); mine.w += __float_as_int(v[r].w);
+                }
+                if (tid == BINS / 4 - 1) mine.x = 0x3FFFFFFF;
             }
-            int before = warp_inclusive_scan(upper + lower, lane);
+            const int sum = mine.x + mine.y + mine.z + mine.w;
+            int before = warp_inclusive_scan(sum, lane);
             if (lane == 31) warp_sum[0][warp] = before;
             __syncthreads();
-            before += __reduce_add_sync(~0u, lane < warp ? warp_sum[0][lane] : 0) - upper - lower;
-            if (before < want && before + upper + lower >= want) {          // one thread
-                const bool up = before + upper >= want;
-                left = want - before - (up ? 0 : upper);
-                bin = BINS - (up ? 1 : 2) - 2 * tid;
+            before += __reduce_add_sync(~0u, lane < warp ? warp_sum[0][lane] : 0) - sum;
+            if (before < want && before + sum >= want) {                    // one thread, but where none is wanted
+                const int up[4] = {mine.w, mine.z, mine.y, mine.x};
+                int j = 0;
+                while (before + up[j] < want) before += up[j++];
+                left = want - before;
+                inside = up[j];
+                bin = BINS - 1 - 4 * tid - j;
             }
             cluster_barrier();                    // all peers have read
-            histogram[tid] = histogram[tid + PICK_THREADS] = 0;
-            a += (uint32_t)bin << shift;
-            want = left;
-            width = shift;
+            if (!begun && spoilt) { faults = OMMX_ST_BAD_PAGE; break; }
+            histogram[tid] = histogram[tid + THREADS] = 0;
+            if (wanted == 0) { a = ~0u; break; }
+            if (!begun && bin == 0) { a = 0; width = 32; }                  // `want` as it was
+            else { a += (uint32_t)bin << shift; want = left; width = shift; }
+            if (width > 0 && inside <= FEW) {     // all blocks say so
+                each_key([&](uint32_t key) { if ((key - a) >> width == 0) few[atomicAdd(&listed, 1)] = key; });
+                __syncthreads();
+                cluster_barrier();
+                if (warp == 0) {
+                    const int mine = lane < (int)n ? (int)peer_word(&listed, lane % n) : 0, sum = warp_inclusive_scan(mine, lane);
+                    if (lane < MOST_CLUSTER) starts[lane + 1] = sum;
+                    if (lane == 0) starts[0] = 0;
+                }
+                __syncthreads();
+                const int count = starts[n];
+                uint32_t k[FEW / THREADS];
+#pragma unroll
+                for (int j = 0; j < FEW / THREADS; ++j) {
+                    const int i = tid + j * THREADS;
+                    int r = 0;
+                    while (r + 1 < (int)n && i >= starts[r + 1]) ++r;
+                    k[j] = i < count ? peer_word(&few[i - starts[r]], r) - a : 0u;
+                }
+                while (width > 0) {
+                    const int cut = max(0, width - 11);
+#pragma unroll
+                    for (int j = 0; j < FEW / THREADS; ++j)
+                        if (tid + j * THREADS < count && k[j] >> width == 0) atomicAdd(&histogram[k[j] >> cut], 1);
+                    __syncthreads();
+                    const int upper = histogram[BINS - 1 - 2 * tid], lower = histogram[BINS - 2 - 2 * tid];
+                    int over = warp_inclusive_scan(upper + lower, lane);
+                    if (lane == 31) warp_sum[0][warp] = over;
+                    __syncthreads();
+                    over += __reduce_add_sync(~0u, lane < warp ? warp_sum[0][lane] : 0) - upper - lower;
+                    if (over < want && over + upper + lower >= want) {
+                        const bool up = over + upper >= want;
+                        left = want - over - (up ? 0 : upper);
+                        bin = BINS - (up ? 1 : 2) - 2 * tid;
+                    }
+                    histogram[tid] = histogram[tid + THREADS] = 0;
+                    __syncthreads();
+                    const uint32_t from = (uint32_t)bin << cut;
+#pragma unroll
+                    for (int j = 0; j < FEW / THREADS; ++j) k[j] -= from;   // what was below wraps around, and is out of reach
+                    a += from;
+                    want = left;
+                    width = cut;
+                    __syncthreads();
+                }
+                break;
+            }
             __syncthreads();
         }
-        // keys above `a`, and the first `want` equal to it, in order. A warp has a stretch of its own.
-        const int stretch = ((hi - lo + PICK_WARPS - 1) / PICK_WARPS + 31) & ~31, from = min(hi, lo + warp * stretch), to = min(hi, from + stretch);
-        auto look = [&](int i, bool &is_more, bool &is_same) {
-            const uint32_t k = i < to ? key_at(i) : 0;
-            const bool pinned = i < p.sinks || i >= len - p.recent;
-            is_more = i < to && (pinned || k > a);
-            is_same = i < to && !pinned && k == a;
+        leave(faults);
+        if (faults) return;
+        // keys above `a`, and the first `want` equal to it, in order: by turns, warps and 32 at a time
+        uint32_t ms[HELD], es[HELD];
+        auto look = [&](int turn) {               // of a turn: which of each 32 are more, and the same
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) {
+                const int i = place(turn, u);
+                const uint32_t k = i >= hi ? 0u : turn == 0 ? held[u] : key_at(i);
+                const bool pinned = i < p.sinks || i >= len - p.recent;
+                ms[u] = __ballot_sync(~0u, i < hi && (pinned || k > a));
+                es[u] = __ballot_sync(~0u, i < hi && !pinned && k == a);
+            }
+        };
+        auto sum = [&](const uint32_t (&bits)[HELD]) {
+            int c = 0;
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) c += __popc(bits[u]);
+            return c;
         };
         int above = 0, equal = 0;
-        for (int i0 = from; i0 < to; i0 += 32) {
-            bool is_more, is_same;
-            look(i0 + lane, is_more, is_same);
-            above += __popc(__ballot_sync(~0u, is_more));
-            equal += __popc(__ballot_sync(~0u, is_same));
+        for (int turn = turns - 1; turn >= 0; --turn) {                     // the first turn's stay
+            look(turn);
+            above += sum(ms);
+            equal += sum(es);
         }
         if (lane == 0) { warp_sum[0][warp] = above; warp_sum[1][warp] = equal; }
         __syncthreads();
@@ -156,89 +274,106 @@ __global__ void __launch_bounds__(PICK_THREADS) kv8_pick_kernel(const __grid_con
         }
         __syncthreads();
         cluster_barrier();
-        above = __reduce_add_sync(~0u, lane < warp ? warp_sum[0][lane] : 0);
-        equal = __reduce_add_sync(~0u, lane < warp ? warp_sum[1][lane] : 0);
-        for (uint32_t r = 0; r < rank; ++r) { above += (int)peer_word(&more, r); equal += (int)peer_word(&same, r); }
-        for (int i0 = from; i0 < to; i0 += 32) {
-            bool is_more, is_same;
-            look(i0 + lane, is_more, is_same);
-            const uint32_t m = __ballot_sync(~0u, is_more), e = __ballot_sync(~0u, is_same), below = (1u << lane) - 1;
-            const int at = above + __popc(m & below), eq = equal + __popc(e & below);
-            if (is_more || (is_same && eq < want)) out[at + min(eq, want)] = i0 + lane;
-            above += __popc(m);
-            equal += __popc(e);
+        if (warp == 0) {
+            const int m = __reduce_add_sync(~0u, lane < (int)rank ? (int)peer_word(&more, lane % n) : 0);
+            const int e = __reduce_add_sync(~0u, lane < (int)rank ? (int)peer_word(&same, lane % n) : 0);
+            if (lane == 0) { above_here = m; equal_here = e; }
         }
-        cluster_barrier();                        // the list is there; and no block leaves before its peers have read its sums
-    }
-    // ---- scales of what each place takes, and of its record
-    __syncthreads();
-    uint16_t *scales = p.scales + ((int64_t)b * p.c.H + head) * (p.places + p.places / BLOCK);
-    const bool listed = len > p.budget;
-    for (int i0 = (rank * PICK_WARPS + warp) * 32; i0 < keep; i0 += n * PICK_THREADS) {
-        const int i = i0 + lane;
-        uint32_t E = 0;
-        if (i < keep) {
-            const int at = listed ? __ldcg(out + i) : i;
-            E = reinterpret_cast<const uint16_t *>(p.c.scales)[record_of(p, p.s, b, head, at)];
-            scales[i] = (uint16_t)E;
-        }
-        uint32_t most = E;
+        __syncthreads();
+        int above_all = above_here, equal_all = equal_here;
+        for (int turn = 0; turn < turns; ++turn) {
+            if (turn > 0) look(turn);
+            if (turns > 1) {
+                __syncthreads();                  // `warp_sum` is read
+                if (lane == 0) { warp_sum[0][warp] = sum(ms); warp_sum[1][warp] = sum(es); }
+                __syncthreads();
+            }
+            const int m = warp_sum[0][lane], e = warp_sum[1][lane];
+            above = above_all + __reduce_add_sync(~0u, lane < warp ? m : 0);
+            equal = equal_all + __reduce_add_sync(~0u, lane < warp ? e : 0);
+            above_all += __reduce_add_sync(~0u, m);
+            equal_all += __reduce_add_sync(~0u, e);
+            const uint32_t below = (1u << lane) - 1;
 #pragma unroll
-        for (int d = 1; d < 16; d *= 2) most = __vmaxu4(most, __shfl_xor_sync(~0u, most, d));
-        if ((lane & 15) == 0 && i < keep) scales[p.places + i / BLOCK] = (uint16_t)most;
+            for (int u = 0; u < HELD; ++u) {
+                const int at = above + __popc(ms[u] & below), eq = equal + __popc(es[u] & below);
+                if (ms[u] >> lane & 1 || (es[u] >> lane & 1 && eq < want)) out[at + min(eq, want)] = place(turn, u);
+                above += __popc(ms[u]);
+                equal += __popc(es[u]);
+            }
+        }
+        cluster_barrier();                        // the list is there, and no peer reads this block's sums any more
+    }
+    // ---- the move. In shared memory a row is D bytes of keys and D of values; 16 bytes to a thread.
+    constexpr int CHUNKS = D / 8;                 // of a row
+    const int chunk = tid % CHUNKS, which = chunk / (CHUNKS / 2);
+    uint8_t *codes = p.c.codes + which * (16 * D) + 16 * (chunk % (CHUNKS / 2));
+    const uint32_t rows_at = (uint32_t)__cvta_generic_to_shared(memory);
+    for (int base = 0; base < keep; base += n * PLACES) {
+        const int start = base + rank * PLACES, count = max(0, min(PLACES, keep - start));
+        __syncthreads();                          // what the pass before wrote out of here
+        if (tid < PLACES) {
+            Place x = {0, 0, 0.0f, 0, 0};
+            if (tid < count) {
+                const int i = start + tid, at = all ? i : __ldcg(out + i);
+                const int64_t page = page_id(p.s, b, at >> p.page_shift), to = page_id(p.to, b, i >> p.page_shift);
+                x.from = row_of(p, page, head, at);
+                x.to = row_of(p, to, head, i);
+                x.own = reinterpret_cast<const uint16_t *>(p.c.scales)[x.from / BLOCK];
+                x.weight = p.c.weight[x.from];
+            }
+            uint32_t most = x.own;
+#pragma unroll
+            for (int d = 1; d < 16; d *= 2) most = __vmaxu4(most, __shfl_xor_sync(~0u, most, d));
+            x.scales = (uint16_t)most;
+            places[tid] = x;
+        }
+        __syncthreads();
+        for (int i = tid / CHUNKS; i < count; i += THREADS / CHUNKS) {
+            const uint32_t from = places[i].from;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(rows_at + 16 * (i * CHUNKS + chunk)),
+                         "l"(codes + (int64_t)(from / BLOCK) * (32 * D) + (from % BLOCK) * D) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();
+        cluster_barrier();                        // all of the pass is read
+#pragma unroll 4
+        for (int i = tid / CHUNKS; i < count; i += THREADS / CHUNKS) {
+            const Place x = places[i];
+            const int own = x.own >> (8 * which) & 255, E = x.scales >> (8 * which) & 255;
+            if (own == E && x.from == x.to) continue;
+            uint4 w = reinterpret_cast<const uint4 *>(memory)[i * CHUNKS + chunk];
+            if (own != E) w = rescaled<E4M3>(w, rescale_by(own, E));
+            *reinterpret_cast<uint4 *>(codes + (int64_t)(x.to / BLOCK) * (32 * D) + (x.to % BLOCK) * D) = w;
+        }
+        if (tid < count) {
+            const Place x = places[tid];
+            p.c.weight[x.to] = x.weight;
+            if (x.to % BLOCK == 0) reinterpret_cast<uint16_t *>(p.c.scales)[x.to / BLOCK] = x.scales;
+        }
     }
 }
 
-// Grid: (2 D / 32 columns, H, B).  A pass takes MOVE_THREADS / 2 * MOVES places, 16 bytes to a thread and turn.
-constexpr int MOVE_THREADS = 512, MOVES = 4;
-template <int G, bool E4M3>
-__global__ void __launch_bounds__(MOVE_THREADS) kv8_move_kernel(const __grid_constant__ EvictParams p) {
-    constexpr int D = 32 * G, PLACES = MOVE_THREADS / 2 * MOVES;
-    const int which = blockIdx.x / G, column = blockIdx.x % G, head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+// The new lengths where they take the place of the old ones, which other blocks read
+__global__ void kv8_shorten_kernel(const __grid_constant__ EvictParams p, int32_t *len, const int32_t *kept) {
     wait_earlier();
     let_next_in();
-    const int2 count = p.counts[(int64_t)b * p.c.H + head];
-    if (p.len_out && blockIdx.x == 0 && head == 0 && tid == 0) p.len_out[b] = count.y;
-    const int32_t *kept = p.kept + ((int64_t)b * p.c.H + head) * p.budget;
-    const uint16_t *scales = p.scales + ((int64_t)b * p.c.H + head) * (p.places + p.places / BLOCK);
-    const int part = which * 16 * D + column * 32 + (tid & 1) * 16;
-    const bool weighs = which == 0 && column == 0 && (tid & 1) == 0, scaled = column == 0 && (tid & 1) == 0;
-    for (int base = 0; base < count.x; base += PLACES) {
-        uint4 w[MOVES];
-        float weight[MOVES];
-        uint8_t *to[MOVES];
-        int64_t record[MOVES];
-#pragma unroll
-        for (int u = 0; u < MOVES; ++u) {
-            const int i = base + u * (MOVE_THREADS / 2) + tid / 2;
-            to[u] = nullptr;
-            if (i >= count.x) continue;
-            const int at = kept[i];
-            const int64_t from = record_of(p, p.s, b, head, at);
-            const uint8_t *source = p.c.codes + from * (32 * D) + part + (at & 15) * D;
-            record[u] = record_of(p, p.to, b, head, i);
-            w[u] = *reinterpret_cast<const uint4 *>(source);
-            if (weighs) weight[u] = p.c.weight[from * BLOCK + (at & 15)];
-            to[u] = p.c.codes + record[u] * (32 * D) + part + (i & 15) * D;
-            const int own = scales[i] >> (8 * which) & 255, E = scales[p.places + i / BLOCK] >> (8 * which) & 255;
-            if (own != E) w[u] = rescaled<E4M3>(w[u], ratio_of(own, E));
-        }
-        __syncthreads();                          // all of the pass is read
-#pragma unroll
-        for (int u = 0; u < MOVES; ++u) {
-            const int i = base + u * (MOVE_THREADS / 2) + tid / 2;
-            if (!to[u]) continue;
-            *reinterpret_cast<uint4 *>(to[u]) = w[u];
-            if (weighs) p.c.weight[record[u] * BLOCK + (i & 15)] = weight[u];
-            if (scaled && (i & 15) == 0) p.c.scales[2 * record[u] + which] = (uint8_t)(scales[p.places + i / BLOCK] >> (8 * which));
-        }
-    }
+    const int b = blockIdx.x * blockDim.x + threadIdx.x;
+    // the list of a sequence that stayed as it is begins with -1
+    if (b < p.s.B && len[b] > p.budget && kept[(int64_t)b * p.c.H * p.budget] >= 0) len[b] = p.budget;
 }
 
 // ---- host ---------------------------------------------------------------------------------------
-static int64_t places_of(int64_t budget) { return (budget + BLOCK - 1) / BLOCK * BLOCK; }
-static int64_t workspace_bytes(int64_t B, int64_t H, int64_t budget) {
-    return (B * H * 8 + B * H * (places_of(budget) + places_of(budget) / BLOCK) * 2 + 15) / 16 * 16;
+template <int G, bool E4M3> static int launch_evict(const EvictParams &p, int cluster, cudaStream_t st) {
+    static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may take its shared memory
+    int dev = 0;
+    if (int rc = current_device(&dev)) return rc;
+    if (!(allowed.load(std::memory_order_acquire) >> dev & 1)) {
+        OMMX_CUDA_TRY(cudaFuncSetAttribute(kv8_evict_kernel<G, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * MOST_KEYS));
+        allowed.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    const size_t keys = 4 * (size_t)p.keys, rows = (size_t)PLACES * 64 * G;
+    return launch_dependent(kv8_evict_kernel<G, E4M3>, dim3(cluster * p.c.H, p.s.B), THREADS, keys > rows ? keys : rows, st, cluster, p);
 }
 
 static int evict(const ommx_kv8_evict_args *a, cudaStream_t st) {
@@ -256,9 +391,6 @@ static int evict(const ommx_kv8_evict_args *a, cudaStream_t st) {
     if (p.c.num_pages == 0) return fail(OMMX_E_ARG, "kv8_evict: a cache of no pages");
     if (!p.c.weight) return fail(OMMX_E_ARG, "kv8_evict: the cache has no weights");
     if (!a->kept) return fail(OMMX_E_ARG, "kv8_evict: kept must not be null");
-    const int64_t need = workspace_bytes(p.s.B, p.c.H, a->budget);
-    if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 || a->workspace_bytes < need)
-        return fail(OMMX_E_ARG, "kv8_evict: workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
     p.in_place = a->to_table == nullptr;
     p.to = p.s;
     if (a->to_table) {
@@ -266,40 +398,31 @@ static int evict(const ommx_kv8_evict_args *a, cudaStream_t st) {
         to.page_table = a->to_table; to.page_table_stride = a->to_table_stride; to.table_is_int64 = a->to_table_is_int64; to.pages_per_seq = a->to_pages_per_seq;
         if (int rc = read_seqs("kv8_evict", to, p.c, &p.to)) return rc;
     }
-    p.kept = a->kept; p.len_out = a->len_out;
+    const bool shortens = a->len_out == a->seqs.b_seq_len;
+    p.kept = a->kept; p.len_out = shortens ? nullptr : a->len_out;
     p.budget = a->budget; p.sinks = a->sink_tokens; p.recent = a->recent_tokens;
-    p.places = (int)places_of(a->budget);
-    p.counts = (int2 *)a->workspace;
-    p.scales = (uint16_t *)(p.counts + (int64_t)p.s.B * p.c.H);
     p.page_shift = shift_of(p.c.page);
     p.status = a->status;
-    // a cluster to a row where rows are few, but no block for less than 2048 tokens
+    // a cluster to a row where rows are few, but no block for less than 1024 tokens
     int64_t tokens = (int64_t)p.s.max_pages * p.c.page;
     if (a->max_seq_len > 0 && a->max_seq_len < tokens) tokens = a->max_seq_len;
     const int64_t rows = (int64_t)p.s.B * p.c.H;
     int cluster = 1;
-    while (cluster < MOST_CLUSTER && 2 * cluster * rows <= sm_count() && tokens >= 4096LL * cluster) cluster *= 2;
+    while (cluster < MOST_CLUSTER && 2 * cluster * rows <= sm_count() && tokens >= 2048LL * cluster) cluster *= 2;
     const int64_t share = (tokens + cluster - 1) / cluster + 32;
-    p.keys = (int)(share < MOST_KEYS ? share : MOST_KEYS);
-    static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may take its shared memory
-    int dev = 0;
-    if (int rc = current_device(&dev)) return rc;
-    if (!(allowed.load(std::memory_order_acquire) >> dev & 1)) {
-        OMMX_CUDA_TRY(cudaFuncSetAttribute(kv8_pick_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * MOST_KEYS));
-        allowed.fetch_or(1ull << dev, std::memory_order_release);
-    }
-    if (int rc = launch_dependent(kv8_pick_kernel, dim3(cluster * p.c.H, p.s.B), PICK_THREADS, 4 * (size_t)p.keys, st, cluster, p)) return rc;
-    const int G = a->cache.head_dim / 32;
-    const dim3 grid(2 * G, p.c.H, p.s.B);
+    p.keys = (int)(share <= TURN ? 0 : share - TURN < MOST_KEYS ? share - TURN : MOST_KEYS);
+    auto launch = [&](auto g, auto e4m3) { return launch_evict<decltype(g)::value, decltype(e4m3)::value>(p, cluster, st); };
+    using std::integral_constant;
+    int rc;
     if (a->cache.code == OMMX_KV8_E4M3)
-        return G == 4 ? launch_dependent(kv8_move_kernel<4, true>, grid, MOVE_THREADS, 0, st, 1, p) : launch_dependent(kv8_move_kernel<2, true>, grid, MOVE_THREADS, 0, st, 1, p);
-    return G == 4 ? launch_dependent(kv8_move_kernel<4, false>, grid, MOVE_THREADS, 0, st, 1, p) : launch_dependent(kv8_move_kernel<2, false>, grid, MOVE_THREADS, 0, st, 1, p);
+        rc = a->cache.head_dim == 128 ? launch(integral_constant<int, 4>(), std::true_type()) : launch(integral_constant<int, 2>(), std::true_type());
+    else
+        rc = a->cache.head_dim == 128 ? launch(integral_constant<int, 4>(), std::false_type()) : launch(integral_constant<int, 2>(), std::false_type());
+    if (rc || !shortens) return rc;
+    return launch_dependent(kv8_shorten_kernel, dim3((p.s.B + 127) / 128), 128, 0, st, 1, p, a->len_out, (const int32_t *)a->kept);
 }
 
 }  // namespace kv8
 }  // namespace ommx
 
-extern "C" int64_t ommx_b200_kv8_evict_workspace_bytes(int32_t batch, int32_t n_kv_heads, int32_t budget) {
-    return batch < 0 || n_kv_heads < 0 || budget < 0 ? 0 : ommx::kv8::workspace_bytes(batch, n_kv_heads, budget);
-}
 extern "C" int ommx_b200_kv8_evict(const ommx_kv8_evict_args *args, void *stream) { return ommx::kv8::evict(args, (cudaStream_t)stream); }

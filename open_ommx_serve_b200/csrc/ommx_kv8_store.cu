@@ -157,10 +157,10 @@ __global__ void __launch_bounds__(32 * MOST_WARPS) kv8_append_kernel(const __gri
         const int E = max(held, exponent_for<E4M3>(most));
         uint8_t *codes = p.c.codes + record * (32 * D) + which * (16 * D);
         if (tau0 && E > held) {                   // what is there moves to the larger scale
-            const float ratio = ratio_of(held, E);
+            const Rescale by = rescale_by(held, E);
             for (int at = 16 * lane; at < tau0 * D; at += 512) {
                 uint4 *w = reinterpret_cast<uint4 *>(codes + at);
-                *w = rescaled<E4M3>(*w, ratio);
+                *w = rescaled<E4M3>(*w, by);
             }
         }
         const float up = __uint_as_float((uint32_t)(254 - min(E, 254)) << 23);                // 2^(127 - E)

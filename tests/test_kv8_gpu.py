@@ -15,7 +15,7 @@ import torch
 import kv8_reference as ref
 from open_ommx_serve_b200 import _lib
 from open_ommx_serve_b200 import ommx_kv8_alloc, ommx_kv8_append, ommx_kv8_decode_attention, ommx_kv8_evict, ommx_kv8_gather
-from open_ommx_serve_b200.attention.kv8 import kv8_evict_workspace_bytes, kv8_workspace_floats
+from open_ommx_serve_b200.attention.kv8 import kv8_workspace_floats
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -693,7 +693,6 @@ class Layer:
         self.status = i32([0])
         self.H, self.Hq, self.most = H, Hq, pages * page
         self.work = torch.empty(max(1, kv8_workspace_floats(B, Hq, D, self.most, weight=True)), device=DEV)
-        self.evict_work = torch.empty(kv8_evict_workspace_bytes(B, H, 40), dtype=torch.uint8, device=DEV)
 
     def step(self, **more):
         c, q, k, v = self.cache, *self.x.split([self.Hq, self.H, self.H], 1)
@@ -703,8 +702,7 @@ class Layer:
 
     def evict(self):
         c = self.cache
-        ommx_kv8_evict(c["codes"], c["scales"], c["weight"], self.table, self.length, self.kept, sink_tokens=2, recent_tokens=8, len_out=self.length, workspace=self.evict_work,
-                       status=self.status)
+        ommx_kv8_evict(c["codes"], c["scales"], c["weight"], self.table, self.length, self.kept, sink_tokens=2, recent_tokens=8, len_out=self.length, status=self.status)
 
     def state(self):
         return {**self.cache, "length": self.length, "o": self.o, "lse": self.lse, "kept": self.kept, "status": self.status}
@@ -841,7 +839,8 @@ def test_nothing_to_do():
 
 
 def test_launches():
-    """Append and read back are one launch each, attention one or two (three with an account), eviction two."""
+    """Append and read back are one launch each, attention one or two (three with an account), eviction one (two where
+    it shortens the lengths it reads)."""
     lib = _lib.load()
 
     def launches(f):
@@ -858,3 +857,4 @@ def test_launches():
     for n, more, want in ((None, {}, 2), (None, dict(weight=c["weight"]), 3), (None, dict(window=300, sink_tokens=4), 1), (200, {}, 1), (200, dict(weight=c["weight"]), 2)):
         assert launches(lambda: ommx_kv8_decode_attention(q, *where, layer.o, layer.lse, max_seq_len=n, **more)) == want
     assert launches(layer.evict) == 2
+    assert launches(lambda: ommx_kv8_evict(c["codes"], c["scales"], c["weight"], layer.table, layer.length, layer.kept)) == 1

@@ -6,7 +6,7 @@ import torch
 
 from open_ommx_serve_b200 import ommx_kv8_alloc, ommx_kv8_append, ommx_kv8_decode_attention, ommx_kv8_evict, ommx_kv8_gather
 from open_ommx_serve_b200 import _lib
-from open_ommx_serve_b200.attention.kv8 import kv8_evict_workspace_bytes, kv8_workspace_floats
+from open_ommx_serve_b200.attention.kv8 import kv8_workspace_floats
 
 B, H, HQ, D, PAGE = 3, 2, 4, 64, 32
 BF16, E4M3 = torch.bfloat16, torch.float8_e4m3fn
@@ -183,18 +183,15 @@ def test_the_c_entries_refuse_calls():
 
     def evict_with(**change):
         e = c_args(_lib.KV8EvictArgs)
-        e.kept = e.workspace = 256
-        e.budget, e.workspace_bytes = 5, 1 << 30
+        e.kept, e.budget = 256, 5
         for k, v in change.items():
             setattr(e, k, v)
         return lib.ommx_b200_kv8_evict(C.byref(e), None)
 
-    for change, text in ((dict(budget=0), "budget"), (dict(sink_tokens=6), "fit into"), (dict(recent_tokens=-1), "fit into"), (dict(kept=None), "kept"), (dict(workspace_bytes=16), "workspace"),
-                         (dict(workspace=264), "workspace"), (dict(max_seq_len=-1), "max_seq_len")):
+    for change, text in ((dict(budget=0), "budget"), (dict(sink_tokens=6), "fit into"), (dict(recent_tokens=-1), "fit into"), (dict(kept=None), "kept"), (dict(max_seq_len=-1), "max_seq_len")):
         assert evict_with(**change) == -1 and text in _lib.last_error(), change
     e = c_args(_lib.KV8EvictArgs)
-    e.kept = e.workspace = 256
-    e.budget, e.workspace_bytes, e.cache.weight = 5, 1 << 30, None
+    e.kept, e.budget, e.cache.weight = 256, 5, None
     assert lib.ommx_b200_kv8_evict(C.byref(e), None) == -1 and "weights" in _lib.last_error()
 
 
@@ -205,5 +202,3 @@ def test_workspace_sizes():
     assert kv8_workspace_floats(2, 32, 128, 512, weight=True) == 2 * 2 * 32 + 512 * 2 * 32
     assert kv8_workspace_floats(1, 32, 128, 100000, window=300, sink_tokens=4) == 0         # 21 records
     assert kv8_workspace_floats(1, 8, 64, 100000, window=300, sink_tokens=4, weight=True) == 2 * 8 + 21 * 16 * 8
-    assert kv8_evict_workspace_bytes(2, 3, 17) == 6 * 8 + 6 * 34 * 2 + 8                     # 456, up to whole 16 bytes
-    assert kv8_evict_workspace_bytes(-1, 3, 17) == 0
