@@ -232,7 +232,7 @@ template <int N> __device__ __forceinline__ void fetched() {                // a
 
 // One record in shared memory; info: which tokens are visible, and above that the exponents of K's and V's scales. `put`: where its logits
 // go, or null
-template <int G, bool E4M3> __device__ __forceinline__ void attend(const DecodeParams &p, const uint8_t *rec, uint32_t info, int lane, const Query<G> &q, State<G> &s,
+template <int G, bool E4M3, bool FINE> __device__ __forceinline__ void attend(const DecodeParams &p, const uint8_t *rec, uint32_t info, int lane, const Query<G> &q, State<G> &s,
                                                                    float *put, int n) {
     constexpr int D = 32 * G;
     const int g = lane >> 2, t = lane & 3;
@@ -291,16 +291,6 @@ template <int G, bool E4M3> __device__ __forceinline__ void attend(const DecodeP
     }
     s.sum[0] += y[0] + y[2];
     s.sum[1] += y[1] + y[3];
-    if constexpr (E4M3) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] *= Code<E4M3>::LIFT;
-    }
-    const uint32_t h0 = bf16x2_bits(y[0], y[1]), h1 = bf16x2_bits(y[2], y[3]);
-    const uint32_t b0 = transpose8x8(h0), b1 = transpose8x8(h1);
-    const uint32_t r0 = transpose8x8(bf16x2_bits(y[0] - __uint_as_float(h0 << 16), y[1] - __uint_as_float(h0 & 0xFFFF0000u)));
-    const uint32_t r1 = transpose8x8(bf16x2_bits(y[2] - __uint_as_float(h1 << 16), y[3] - __uint_as_float(h1 & 0xFFFF0000u)));
-
-    // ---- values
     const int E = info >> 24;
     if (E > s.E) {
         const float f = ratio_of(s.E, E);
@@ -310,7 +300,17 @@ template <int G, bool E4M3> __device__ __forceinline__ void attend(const DecodeP
             for (int i = 0; i < 4; ++i) s.acc[j][i] *= f;
         s.E = E;
     }
-    const float f = ratio_of(E, s.E);
+    const float f = ratio_of(E, s.E);             // meets the weights, or the record's sums
+    if constexpr (E4M3 || !FINE) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] *= FINE ? Code<E4M3>::LIFT : Code<E4M3>::LIFT * f;
+    }
+    const uint32_t h0 = bf16x2_bits(y[0], y[1]), h1 = bf16x2_bits(y[2], y[3]);
+    const uint32_t b0 = transpose8x8(h0), b1 = transpose8x8(h1);
+    const uint32_t r0 = transpose8x8(bf16x2_bits(y[0] - __uint_as_float(h0 << 16), y[1] - __uint_as_float(h0 & 0xFFFF0000u)));
+    const uint32_t r1 = transpose8x8(bf16x2_bits(y[2] - __uint_as_float(h1 << 16), y[3] - __uint_as_float(h1 & 0xFFFF0000u)));
+
+    // ---- values
     uint32_t w[4][G];                             // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9: channels 4 G g + 0 .. 4 G - 1
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -331,11 +331,16 @@ template <int G, bool E4M3> __device__ __forceinline__ void attend(const DecodeP
         a[1] = value_pair<E4M3>(w[0][j / 2], w[1][j / 2], at + 1);
         a[2] = value_pair<E4M3>(w[2][j / 2], w[3][j / 2], at);
         a[3] = value_pair<E4M3>(w[2][j / 2], w[3][j / 2], at + 1);
-        float c[4];
-        mma_bf16_first(c, a, r0, r1);
-        mma_bf16(c, a, b0, b1);
+        if constexpr (FINE) {
+            float c[4];
+            mma_bf16_first(c, a, r0, r1);
+            mma_bf16(c, a, b0, b1);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s.acc[j][i] = fmaf(c[i], f, s.acc[j][i]);
+            for (int i = 0; i < 4; ++i) s.acc[j][i] = fmaf(c[i], f, s.acc[j][i]);
+        } else {
+            mma_bf16(s.acc[j], a, r0, r1);
+            mma_bf16(s.acc[j], a, b0, b1);
+        }
     }
 }
 
@@ -457,7 +462,7 @@ template <int G> __device__ __forceinline__ void merge_cluster(const DecodeParam
     cluster_barrier();                            // no block leaves before its peers have read its part
 }
 
-template <int G, bool E4M3, int NW, bool CLUSTER>
+template <int G, bool E4M3, bool FINE, int NW, bool CLUSTER>
 __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv8_decode_kernel(const __grid_constant__ DecodeParams p) {
     extern __shared__ __align__(128) uint8_t memory[];
     Memory<G, NW> &m = *reinterpret_cast<Memory<G, NW> *>(memory);
@@ -580,7 +585,7 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv8_decode_kernel(
                         if (i < p.most_units) to = put + (int64_t)i * 16 * p.group;
                         else or_status(p.status, OMMX_ST_BAD_LENGTH);
                     }
-                    attend<G, E4M3>(p, ring + read, flying[0], lane, q, s, to, n);
+                    attend<G, E4M3, FINE>(p, ring + read, flying[0], lane, q, s, to, n);
                 }
 #pragma unroll
                 for (int j = 0; j + 1 < AHEAD; ++j) flying[j] = flying[j + 1];
@@ -789,15 +794,15 @@ static int64_t workspace_floats(const ommx_kv8_decode_args *a) {
     return (n + 3) / 4 * 4;
 }
 
-template <int G, bool E4M3, int NW, bool CLUSTER> static int launch_decode(const DecodeParams &p, int64_t blocks, int cluster, cudaStream_t st) {
+template <int G, bool E4M3, bool FINE, int NW, bool CLUSTER> static int launch_decode(const DecodeParams &p, int64_t blocks, int cluster, cudaStream_t st) {
     static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may take its shared memory
     int dev = 0;
     if (int rc = current_device(&dev)) return rc;
     if (!(allowed.load(std::memory_order_acquire) >> dev & 1)) {
-        OMMX_CUDA_TRY(cudaFuncSetAttribute(kv8_decode_kernel<G, E4M3, NW, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Memory<G, NW>)));
+        OMMX_CUDA_TRY(cudaFuncSetAttribute(kv8_decode_kernel<G, E4M3, FINE, NW, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Memory<G, NW>)));
         allowed.fetch_or(1ull << dev, std::memory_order_release);
     }
-    if (int rc = launch_dependent(kv8_decode_kernel<G, E4M3, NW, CLUSTER>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G, NW>), st, cluster, p)) return rc;
+    if (int rc = launch_dependent(kv8_decode_kernel<G, E4M3, FINE, NW, CLUSTER>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G, NW>), st, cluster, p)) return rc;
     if (p.whole || CLUSTER) return 0;
     // a row has some blocks / rows parts
     const int rows = p.c.H * p.col_blocks;
@@ -855,22 +860,22 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     // Rows of middling length, and few, go to a cluster of eight-warp blocks each, as many as fit at once: no second kernel
     int cluster = 1;
     while (cluster < MOST_CLUSTER && 2 * cluster * rows <= most_blocks(8)) cluster *= 2;
-    if (units > 32 * cluster) cluster = 1;
+    if (units > 36 * cluster) cluster = 1;
     p.whole = units <= WHOLE / 2 || (units <= WHOLE && cluster == 1);
     if (p.whole) cluster = 1;
     const int64_t blocks = p.whole ? rows : cluster > 1 ? cluster * rows : most < 1 ? 1 : most < hold ? most : hold;
-    auto launch = [&](auto g, auto e4m3) {
+    auto launch = [&](auto g, auto e4m3, auto fine) {
         constexpr int G = decltype(g)::value;
-        constexpr bool E4M3 = decltype(e4m3)::value;
-        if (cluster > 1) return launch_decode<G, E4M3, 8, true>(p, blocks, cluster, st);
-        return warps == 4 ? launch_decode<G, E4M3, 4, false>(p, blocks, 1, st) : launch_decode<G, E4M3, 8, false>(p, blocks, 1, st);
+        constexpr bool E4M3 = decltype(e4m3)::value, FINE = decltype(fine)::value;
+        if (cluster > 1) return launch_decode<G, E4M3, FINE, 8, true>(p, blocks, cluster, st);
+        return warps == 4 ? launch_decode<G, E4M3, FINE, 4, false>(p, blocks, 1, st) : launch_decode<G, E4M3, FINE, 8, false>(p, blocks, 1, st);
     };
     using std::integral_constant;
-    int rc;
-    if (a->cache.code == OMMX_KV8_E4M3)
-        rc = a->cache.head_dim == 128 ? launch(integral_constant<int, 4>(), std::true_type()) : launch(integral_constant<int, 2>(), std::true_type());
-    else
-        rc = a->cache.head_dim == 128 ? launch(integral_constant<int, 4>(), std::false_type()) : launch(integral_constant<int, 2>(), std::false_type());
+    auto of_size = [&](auto e4m3, auto fine) {
+        return a->cache.head_dim == 128 ? launch(integral_constant<int, 4>(), e4m3, fine) : launch(integral_constant<int, 2>(), e4m3, fine);
+    };
+    auto of_code = [&](auto fine) { return a->cache.code == OMMX_KV8_E4M3 ? of_size(std::true_type(), fine) : of_size(std::false_type(), fine); };
+    const int rc = a->o_dtype == OMMX_DT_F32 ? of_code(std::true_type()) : of_code(std::false_type());
     const int64_t tokens = most_tokens(a);
     if (rc || !p.c.weight || !tokens) return rc;
     return launch_dependent(kv8_weigh_kernel, dim3((unsigned)((tokens + WEIGH_THREADS - 1) / WEIGH_THREADS), p.c.H, p.s.B), WEIGH_THREADS, 0, st, 1, p);
