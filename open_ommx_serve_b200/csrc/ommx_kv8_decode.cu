@@ -2,17 +2,18 @@
 // each token's weight where it is asked for.
 //
 // For query head h of a sequence, over its visible tokens t:  x_t = sm_scale q.K_t,  o = sum_t exp(x_t) V_t / sum_t exp(x_t), with
-// K_t = 2^ek a_t and V_t = 2^ev b_t for the 16 tokens of a record: a record's scales are two numbers, which meet the sums of its products
-// behind them. Products are m16n8k16 with the codes as A (tokens as rows for K, channels for V) and up to eight query heads that share
-// the kv head as columns:
-//   logits   fp16, exact: codes of either type are fp16 numbers, and a query row times a power of two is (rounded by 2^-39 of its largest
-//            channel at most, where bf16 channels are 2^27 below that);
-//   values   bf16, whose range is that of fp32: a weight y is the sum of two bf16 numbers, off by 2^-17 of itself however small it is, and
-//            no token is left out; codes are bf16 numbers. One record's sum starts at zero and is added in fp32, times its scale: the tensor
-//            cores, which cut what they add, cut 25 bits below a record's own largest product.
-// Values are summed in units of the largest scale a warp has met, and leave it divided by the sum of their weights, so neither the
-// largest nor the smallest numbers a cache holds pass fp32 on the way.
-//
+// K_t = 2^ek a_t and V_t = 2^ev b_t for the 16 tokens of a record: a record's scales are two numbers. Products have the codes as A (tokens as rows
+// for K, channels for V) and up to eight query heads that share the kv head as columns:
+//   logits   int8: 8-bit products (m16n8k32) of the codes as they are and the three bytes of a query row as whole numbers of 23 bits, exact from there
+//            on; a channel is rounded by 2^-22 of the row's largest at most. Fp16 products, whose operands have to be made, took 33 us more of 166 (8 x 64K
+//            tokens, copies left out). e4m3: fp16 products, since 8-bit ones of this type have their operands converted each time (three pieces of a
+//            query: 32 ragged sequences 71 us with fp16, 81 with e4m3); a query row times a power of two is an fp16 number, bf16 channels below 2^-27 of
+//            the largest are rounded by 2^-39 of it;
+//   values   fp16 (m16n8k16), in which the codes are made exactly; weights times scales, y 2^ev, go to fp16 in a unit that the largest of them sets,
+//            a power of two for each head: a token whose weight times scale is 2^-25 of the largest keeps its bits (11), so values of any size
+//            leave no token out. Where the output is finer than bf16 a second product takes what the rounding left (FINE).
+// The tensor cores cut what they add to a sum 24 bits below it, so an output is off by 2^-25 of itself for each record of a warp, 2^-18 for 110 of them
+// (8 x 64K tokens).
 // What bounds it: a record's 32 D bytes are read once for each eight query heads of its kv head.
 #include <cmath>
 #include <type_traits>
@@ -34,14 +35,10 @@ constexpr float LOWEST = -1e30f;
 constexpr int MOST_PARTS = 768;                   // blocks of a call that shares rows
 constexpr int WHOLE = 32;                         // records of a row that one block takes at most where it could share it
 
-// A code as the A operand of values: e4m3 codes moved to a bf16 number's bits are 2^-120 times as large, int8 codes (u - 128) 2^-13 come out
-// of one multiply-add of the subnormal u 2^-133. What weights are multiplied with before they meet e4m3 codes keeps products within fp32
-// (in the weight's own logarithm it would cost it seven bits).
-template <bool E4M3> struct Code {
-    static constexpr float LIFT = E4M3 ? 0x1p80f : 1.0f;
-    static constexpr float BACK = E4M3 ? 0x1p40f : 0x1p13f;                 // undoes both
-};
-constexpr float HEAVY = 128.0f;                   // weights 2^(x - ref) begin near 1; one past this moves the reference
+// Weights w = 2^(x - ref) begin near 1; one past HEAVY moves the reference. Products w 2^(ev - 127) k go to fp16: the largest lies in (2^(TOP - 1), 2^TOP]
+// when the references have moved, and may grow to ROOM before they move again.
+constexpr float HEAVY = 128.0f, ROOM = 60000.0f;
+constexpr int TOP = 11;
 
 struct DecodeParams {
     Cache c;
@@ -104,17 +101,23 @@ __device__ __forceinline__ void store_sum(const DecodeParams &p, int b, int hq, 
 }
 
 // ---- pieces ---------------------------------------------------------------------------------------
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+// Products of bytes. Sums stay below 2^22, so one that begins with the bits of 1.5 * 2^23 is, as a float, that number and the sum
+constexpr float BEGIN_VALUE = 12582912.0f;
+__device__ __forceinline__ void mma_s8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
+    uint32_t d[4] = {__float_as_uint(c[0]), __float_as_uint(c[1]), __float_as_uint(c[2]), __float_as_uint(c[3])};
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = __uint_as_float(d[i]);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -130,45 +133,35 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-__device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
 __device__ __forceinline__ int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23 & 255u) - 127; }
 
-// four codes of a token to two fp16 pairs
-template <bool E4M3> __device__ __forceinline__ void key_pairs(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    if constexpr (E4M3) {
-        lo = half2_of_e4m3x2(w);
-        hi = half2_of_e4m3x2(w >> 16);
-    } else {
-        const uint32_t u = w ^ 0x80808080u;       // 1024 + 128 + code as an fp16 number
-        const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
-        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), off), y = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
-        lo = *reinterpret_cast<const uint32_t *>(&x);
-        hi = *reinterpret_cast<const uint32_t *>(&y);
-    }
-}
-// code `i` of two tokens' words to a bf16 pair, UNIT times as large
-template <bool E4M3> __device__ __forceinline__ uint32_t value_pair(uint32_t a, uint32_t b, int i) {
-    if constexpr (E4M3) {
-        const uint32_t w = __byte_perm(a, b, (4 + i) << 12 | i << 4);       // the codes in the upper bytes
-        return (w & 0x80008000u) | (w >> 4 & 0x07F007F0u);
-    } else {
-        const uint32_t u = (__byte_perm(a, b, (4 + i) << 8 | i) & 0x00FF00FFu) ^ 0x00800080u;
-        uint32_t r;
-        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(u), "r"(0x7B807B80u), "r"(0xBC80BC80u));   // * 2^120 - 2^-6
-        return r;
+// The codes of four channels of two tokens (their words) to fp16 pairs, a channel to each
+template <bool E4M3> __device__ __forceinline__ void value_pairs(uint32_t a, uint32_t b, uint32_t (&pair)[4]) {
+    const uint32_t two[2] = {__byte_perm(a, b, 0x5140), __byte_perm(a, b, 0x7362)};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if constexpr (E4M3) {
+            pair[2 * i] = half2_of_e4m3x2(two[i]);
+            pair[2 * i + 1] = half2_of_e4m3x2(two[i] >> 16);
+        } else {
+            const uint32_t u = two[i] ^ 0x80808080u;                        // 1024 + 128 + code as an fp16 number
+            const __half2 off = __float2half2_rn(1152.0f);
+            const uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);
+            const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&lo), off), y = __hsub2(*reinterpret_cast<const __half2 *>(&hi), off);
+            pair[2 * i] = *reinterpret_cast<const uint32_t *>(&x);
+            pair[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&y);
+        }
     }
 }
 
-// A kv head's queries as B fragments: lane (g, t) holds head g, channels 8 G t + 4 s + 0..3 for product s
-template <int G> struct Query {
-    uint32_t frag[2 * G][2];
+// A kv head's queries as B fragments: lane (g, t) holds head g, channels 8 G t + 8 s + 0..7 for the products s. int8: [s][byte][half of the eight];
+// e4m3: [s][half of the eight][two pairs]
+constexpr int PIECES = 3;
+template <int G, bool E4M3> struct Query {
+    uint32_t frag[G][E4M3 ? 2 : PIECES][2];
     float factor[2], raw[2];                      // of heads 2 t and 2 t + 1: the products' units in powers of two; with a cap: in its units
 };
-template <int G> __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int first_head, int n, int lane, Query<G> &q) {
+template <int G, bool E4M3> __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int first_head, int n, int lane, Query<G, E4M3> &q) {
     const int g = lane >> 2, t = lane & 3;
     float x[8 * G], top = 0.0f;
 #pragma unroll
@@ -178,13 +171,32 @@ template <int G> __device__ __forceinline__ void load_query(const DecodeParams &
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
     const int e = top > 0.0f ? max(exponent_of(top), -100) : 0;
-    const float up = power_of_two(13 - e);
+    constexpr int BITS = E4M3 ? 13 : 21;          // the largest channel lies below 2^(BITS + 1)
+    const float up = power_of_two(BITS - e);
 #pragma unroll
-    for (int s = 0; s < 2 * G; ++s) {
-        q.frag[s][0] = half2_bits(x[4 * s] * up, x[4 * s + 1] * up);
-        q.frag[s][1] = half2_bits(x[4 * s + 2] * up, x[4 * s + 3] * up);
-    }
-    const float factor = p.sm_scale * 0x1p-13f * power_of_two(e);
+    for (int s = 0; s < G; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float *f = x + 8 * s + 4 * h;
+            if constexpr (E4M3) {
+                q.frag[s][h][0] = half2_bits(f[0] * up, f[1] * up);
+                q.frag[s][h][1] = half2_bits(f[2] * up, f[3] * up);
+            } else {
+                int r[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[i] = __float2int_rn(f[i] * up);
+#pragma unroll
+                for (int j = PIECES - 1; j >= 0; --j) {
+                    q.frag[s][j][h] = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        q.frag[s][j][h] |= ((uint32_t)r[i] & 255u) << (8 * i);
+                        r[i] = (r[i] + 128) >> 8;     // of what the last byte, -128 .. 127, leaves
+                    }
+                }
+            }
+        }
+    const float factor = p.sm_scale * power_of_two(-BITS) * power_of_two(e);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const float f = __shfl_sync(~0u, factor, 8 * t + 4 * i);
@@ -193,10 +205,10 @@ template <int G> __device__ __forceinline__ void load_query(const DecodeParams &
     }
 }
 
-// A warp's running state. acc[i]: channels 4 G g + 2 i (rows g) and the next one (rows g + 8) of heads 2 t, 2 t + 1, in units of 2^(E - 127) UNIT
+// A warp's running state. acc[i]: channels 4 G g + 2 i (rows g) and the next one (rows g + 8) of heads 2 t, 2 t + 1, in units of unit[]
 template <int G> struct State {
     float acc[2 * G][4], sum[2], ref[2];
-    int E;
+    float unit[2];                                // a power of two that only `acc` has in it
 };
 template <int G> __device__ __forceinline__ void clear(State<G> &s) {
 #pragma unroll
@@ -205,7 +217,21 @@ template <int G> __device__ __forceinline__ void clear(State<G> &s) {
         for (int j = 0; j < 4; ++j) s.acc[i][j] = 0.0f;
     s.sum[0] = s.sum[1] = 0.0f;
     s.ref[0] = s.ref[1] = LOWEST;
-    s.E = 0;
+    s.unit[0] = s.unit[1] = 1.0f;
+}
+// The references of head i move to `ref`, a whole number as the one before, so that nothing is rounded. E: exponent of a record's scale, `top`: its
+// largest logit less `ref`.
+template <int G> __device__ __forceinline__ void move(State<G> &s, int i, float ref, float top, int E) {
+    const int was = exponent_of(s.unit[i]);
+    const float over = ceilf(fmaxf((s.ref[i] - ref) + (float)(TOP - was), top + (float)(E - 127)));       // 2^over: the largest product
+    const int now = min(TOP - (int)fminf(fmaxf(over, -1000.0f), 1000.0f), 253 - E);                       // a scale times the unit is finite
+    const int held = min(max(now, -126), 126);
+    const float f = exp2_approx(s.ref[i] - ref), a = exp2_approx(s.ref[i] - ref + (float)(held - was));
+    s.ref[i] = ref;
+    s.unit[i] = power_of_two(held);
+    s.sum[i] *= f;
+#pragma unroll
+    for (int j = 0; j < 2 * G; ++j) { s.acc[j][i] *= a; s.acc[j][i + 2] *= a; }
 }
 
 // ---- a warp's ring of records: 16 bytes a lane at a time, a group of copies for each record ----
@@ -232,32 +258,47 @@ template <int N> __device__ __forceinline__ void fetched() {                // a
 
 // One record in shared memory; info: which tokens are visible, and above that the exponents of K's and V's scales. `put`: where its logits
 // go, or null
-template <int G, bool E4M3, bool FINE> __device__ __forceinline__ void attend(const DecodeParams &p, const uint8_t *rec, uint32_t info, int lane, const Query<G> &q, State<G> &s,
+template <int G, bool E4M3, bool FINE> __device__ __forceinline__ void attend(const DecodeParams &p, const uint8_t *rec, uint32_t info, int lane, const Query<G, E4M3> &q, State<G> &s,
                                                                    float *put, int n) {
     constexpr int D = 32 * G;
     const int g = lane >> 2, t = lane & 3;
     // ---- logits: x[0], x[1] of token g and heads 2 t, 2 t + 1; x[2], x[3] of token g + 8
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int SUMS = E4M3 ? 2 : PIECES;       // of half the products each; of a byte each
+    float c[SUMS][4], x[4];
+#pragma unroll
+    for (int j = 0; j < SUMS; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[j][i] = E4M3 ? 0.0f : BEGIN_VALUE;
 #pragma unroll
     for (int i = 0; i < G / 2; ++i) {
         const uint4 a = *reinterpret_cast<const uint4 *>(rec + swizzle<G>(g, G / 2 * t + i));
         const uint4 b = *reinterpret_cast<const uint4 *>(rec + swizzle<G>(g + 8, G / 2 * t + i));
-        const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+        if constexpr (E4M3) {
+            const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t a0, a1, a2, a3;
-            key_pairs<E4M3>(wa[j], a0, a2);
-            key_pairs<E4M3>(wb[j], a1, a3);
-            mma_f16(j & 1 ? z : x, a0, a1, a2, a3, q.frag[4 * i + j][0], q.frag[4 * i + j][1]);
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t k[4] = {half2_of_e4m3x2(wa[j]), half2_of_e4m3x2(wb[j]), half2_of_e4m3x2(wa[j] >> 16), half2_of_e4m3x2(wb[j] >> 16)};
+                mma_f16(c[j & 1], k, q.frag[2 * i + j / 2][j & 1][0], q.frag[2 * i + j / 2][j & 1][1]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) mma_s8(c[j], a.x, b.x, a.y, b.y, q.frag[2 * i][j]);
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) mma_s8(c[j], a.z, b.z, a.w, b.w, q.frag[2 * i + 1][j]);
         }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (E4M3) x[i] = c[0][i] + c[1][i];
+        else x[i] = fmaf(fmaf(c[0][i] - BEGIN_VALUE, 256.0f, c[1][i] - BEGIN_VALUE), 256.0f, c[SUMS - 1][i] - BEGIN_VALUE);
     }
     const float sk = scale_of(info >> 16 & 255u);
     if (p.cap > 0.0f) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = tanhf((x[i] + z[i]) * (q.raw[i & 1] * sk)) * q.factor[i & 1];
+        for (int i = 0; i < 4; ++i) x[i] = tanhf(x[i] * (q.raw[i & 1] * sk)) * q.factor[i & 1];
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = (x[i] + z[i]) * (q.factor[i & 1] * sk);
+        for (int i = 0; i < 4; ++i) x[i] *= q.factor[i & 1] * sk;
     }
     if (put) {
 #pragma unroll
@@ -271,44 +312,36 @@ template <int G, bool E4M3, bool FINE> __device__ __forceinline__ void attend(co
     }
 
     // ---- weights
-    float y[4];
+    const int E = info >> 24;
+    float y[4], f[2], z[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = exp2_approx(x[i] - s.ref[i & 1]);
-    if (__any_sync(~0u, !(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) <= HEAVY))) {
+    for (int i = 0; i < 2; ++i) f[i] = scale_of(E) * s.unit[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { y[i] = exp2_approx(x[i] - s.ref[i & 1]); z[i] = y[i] * f[i & 1]; }
+    const float heavy = fmaxf(max3(y[0], y[1], y[2]), y[3]), most = fmaxf(max3(z[0], z[1], z[2]), z[3]);
+    if (__any_sync(~0u, !(heavy <= HEAVY && most <= ROOM))) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             float l = fmaxf(x[i], x[i + 2]);
 #pragma unroll
             for (int d = 4; d < 32; d *= 2) l = fmaxf(l, __shfl_xor_sync(~0u, l, d));
-            const float ref = fmaxf(s.ref[i], ceilf(l)), f = exp2_approx(s.ref[i] - ref);
-            s.ref[i] = ref;
-            s.sum[i] *= f;
-#pragma unroll
-            for (int j = 0; j < 2 * G; ++j) { s.acc[j][i] *= f; s.acc[j][i + 2] *= f; }
+            const float ref = fmaxf(s.ref[i], ceilf(l));
+            move(s, i, ref, l - ref, E);
+            f[i] = scale_of(E) * s.unit[i];
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = exp2_approx(x[i] - s.ref[i & 1]);
+        for (int i = 0; i < 4; ++i) { y[i] = exp2_approx(x[i] - s.ref[i & 1]); z[i] = y[i] * f[i & 1]; }
     }
     s.sum[0] += y[0] + y[2];
     s.sum[1] += y[1] + y[3];
-    const int E = info >> 24;
-    if (E > s.E) {
-        const float f = ratio_of(s.E, E);
-#pragma unroll
-        for (int j = 0; j < 2 * G; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s.acc[j][i] *= f;
-        s.E = E;
-    }
-    const float f = ratio_of(E, s.E);             // meets the weights, or the record's sums
-    if constexpr (E4M3 || !FINE) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] *= FINE ? Code<E4M3>::LIFT : Code<E4M3>::LIFT * f;
-    }
-    const uint32_t h0 = bf16x2_bits(y[0], y[1]), h1 = bf16x2_bits(y[2], y[3]);
+    const uint32_t h0 = half2_bits(z[0], z[1]), h1 = half2_bits(z[2], z[3]);
     const uint32_t b0 = transpose8x8(h0), b1 = transpose8x8(h1);
-    const uint32_t r0 = transpose8x8(bf16x2_bits(y[0] - __uint_as_float(h0 << 16), y[1] - __uint_as_float(h0 & 0xFFFF0000u)));
-    const uint32_t r1 = transpose8x8(bf16x2_bits(y[2] - __uint_as_float(h1 << 16), y[3] - __uint_as_float(h1 & 0xFFFF0000u)));
+    uint32_t r0 = 0, r1 = 0;
+    if constexpr (FINE) {
+        const float2 n0 = __half22float2(*reinterpret_cast<const __half2 *>(&h0)), n1 = __half22float2(*reinterpret_cast<const __half2 *>(&h1));
+        r0 = transpose8x8(half2_bits(z[0] - n0.x, z[1] - n0.y));
+        r1 = transpose8x8(half2_bits(z[2] - n1.x, z[3] - n1.y));
+    }
 
     // ---- values
     uint32_t w[4][G];                             // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9: channels 4 G g + 0 .. 4 G - 1
@@ -322,24 +355,21 @@ template <int G, bool E4M3, bool FINE> __device__ __forceinline__ void attend(co
             const uint2 v = *reinterpret_cast<const uint2 *>(rec + 16 * D + swizzle<G>(token, g >> 1) + 8 * (g & 1));
             w[i][0] = v.x; w[i][1] = v.y;
         }
+        if (E4M3 && mask != ALL && !(mask >> token & 1)) {                  // a weight of 0 times NaN is not 0
+#pragma unroll
+            for (int j = 0; j < G; ++j) w[i][j] = 0;
+        }
     }
 #pragma unroll
-    for (int j = 0; j < 2 * G; ++j) {
-        const int at = 2 * (j & 1);
-        uint32_t a[4];
-        a[0] = value_pair<E4M3>(w[0][j / 2], w[1][j / 2], at);
-        a[1] = value_pair<E4M3>(w[0][j / 2], w[1][j / 2], at + 1);
-        a[2] = value_pair<E4M3>(w[2][j / 2], w[3][j / 2], at);
-        a[3] = value_pair<E4M3>(w[2][j / 2], w[3][j / 2], at + 1);
-        if constexpr (FINE) {
-            float c[4];
-            mma_bf16_first(c, a, r0, r1);
-            mma_bf16(c, a, b0, b1);
+    for (int j = 0; j < G; ++j) {
+        uint32_t near[4], far[4];                 // of tokens 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
+        value_pairs<E4M3>(w[0][j], w[1][j], near);
+        value_pairs<E4M3>(w[2][j], w[3][j], far);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s.acc[j][i] = fmaf(c[i], f, s.acc[j][i]);
-        } else {
-            mma_bf16(s.acc[j], a, r0, r1);
-            mma_bf16(s.acc[j], a, b0, b1);
+        for (int u = 0; u < 2; ++u) {
+            const uint32_t a[4] = {near[2 * u], near[2 * u + 1], far[2 * u], far[2 * u + 1]};
+            if constexpr (FINE) mma_f16(s.acc[2 * j + u], a, r0, r1);
+            mma_f16(s.acc[2 * j + u], a, b0, b1);
         }
     }
 }
@@ -355,7 +385,7 @@ template <> struct Floats<4> { using T = float4; };
 
 // The warps' states of a row to its output, or to a part: [COLS][D] outputs of its own tokens, [COLS] references, [COLS] sums. A warp
 // finishes every NW-th head, a lane G channels.
-template <int G, bool E4M3, int NW>
+template <int G, int NW>
 __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Shared<G, NW> &sh, float (&ref)[COLS][NW], float (&sum)[COLS][NW], int b,
                                        int first_head, int n, float *part, int warp, int lane) {
     using V = typename Floats<G>::T;
@@ -368,10 +398,9 @@ __device__ __forceinline__ void finish(const DecodeParams &p, State<G> &s, Share
         if (g == 0) { ref[2 * t + i][warp] = s.ref[i]; sum[2 * t + i][warp] = s.sum[i]; }
     }
     __syncthreads();                              // and the ring, whose memory `sh` is, is done with
-    const float unit = scale_of(s.E);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const float back = s.sum[i] != 0.0f ? Code<E4M3>::BACK / s.sum[i] : 0.0f;
+        const float back = s.sum[i] != 0.0f ? 1.0f / s.sum[i] : 0.0f, unit = power_of_two(-exponent_of(s.unit[i]));
         float *to = &sh.o[warp][2 * t + i][4 * G * g];
 #pragma unroll
         for (int j = 0; j < 2 * G; j += 2)
@@ -561,9 +590,9 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv8_decode_kernel(
             flying[k] = __shfl_sync(~0u, info, k);
             close_group();
         }
-        Query<G> q;
+        Query<G, E4M3> q;
         State<G> s;
-        load_query<G>(p, b, first_head, n, lane, q);
+        load_query<G, E4M3>(p, b, first_head, n, lane, q);
         clear(s);
         float *put = nullptr;
         if (p.logits) put = p.logits + (((int64_t)b * p.c.H + head) * p.most_units * 16) * p.group + cb * COLS;
@@ -597,13 +626,13 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv8_decode_kernel(
         }
         fetched<0>();
         if constexpr (CLUSTER) {
-            finish<G, E4M3, NW>(p, s, m.sh, m.ref, m.sum, b, first_head, n, m.merged, warp, lane);
+            finish<G, NW>(p, s, m.sh, m.ref, m.sum, b, first_head, n, m.merged, warp, lane);
             merge_cluster<G>(p, m.merged, b, first_head, n, warp, lane);
             return;
         }
         float *part = nullptr;
         if (i0 > 0 || i1 < units) part = p.work + HEAD + (2 * (int64_t)blockIdx.x + (base + row * units >= second)) * PART<G>;
-        finish<G, E4M3, NW>(p, s, m.sh, m.ref, m.sum, b, first_head, n, part, warp, lane);
+        finish<G, NW>(p, s, m.sh, m.ref, m.sum, b, first_head, n, part, warp, lane);
         u += i1 - i0;
     }
 }
@@ -875,7 +904,7 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
         return a->cache.head_dim == 128 ? launch(integral_constant<int, 4>(), e4m3, fine) : launch(integral_constant<int, 2>(), e4m3, fine);
     };
     auto of_code = [&](auto fine) { return a->cache.code == OMMX_KV8_E4M3 ? of_size(std::true_type(), fine) : of_size(std::false_type(), fine); };
-    const int rc = a->o_dtype == OMMX_DT_F32 ? of_code(std::true_type()) : of_code(std::false_type());
+    const int rc = a->o_dtype != OMMX_DT_BF16 ? of_code(std::true_type()) : of_code(std::false_type());
     const int64_t tokens = most_tokens(a);
     if (rc || !p.c.weight || !tokens) return rc;
     return launch_dependent(kv8_weigh_kernel, dim3((unsigned)((tokens + WEIGH_THREADS - 1) / WEIGH_THREADS), p.c.H, p.s.B), WEIGH_THREADS, 0, st, 1, p);

@@ -82,15 +82,17 @@ def visible(length, window, sinks):
 
 
 def attention(q, k, v, sm_scale, cap=0.0):
-    """q [Hq, D], k / v [H, tokens, D] in 64 bits -> o [Hq, D], lse [Hq], weights [Hq, tokens], and a bound of how far 32 bits put a logit:
-    a sum of D products in a handful of steps, and three roundings of a product."""
+    """q [Hq, D], k / v [H, tokens, D] in 64 bits -> o [Hq, D], lse [Hq], weights [Hq, tokens], and a bound of how far the kernels put a
+    logit: 2^-21 of sum |q||k| for a sum of D products in a handful of steps of 24 bits and three roundings, and each channel of a query rounded by
+    half a step of 2^-21 of the power of two that its row's largest has, 2^-22 of that at most."""
     H = len(k)
     group = q.shape[0] // H
     o, lse = torch.zeros(q.shape, dtype=torch.float64, device=q.device), torch.full((q.shape[0],), -math.inf, dtype=torch.float64, device=q.device)
     p, off = torch.zeros(q.shape[0], k.shape[1], dtype=torch.float64, device=q.device), torch.zeros(q.shape[0], dtype=torch.float64, device=q.device)
     for h in range(q.shape[0] if k.shape[1] else 0):
         x = k[h // group] @ q[h].double() * sm_scale
-        off[h] = 2.0 ** -21 * abs(sm_scale) * (k[h // group].abs() @ q[h].double().abs()).max()
+        near, size = k[h // group].abs(), q[h].double().abs()
+        off[h] = abs(sm_scale) * (2.0 ** -21 * (near @ size) + 2.0 ** -22 * size.max() * near.sum(1)).max()
         if cap:
             x = cap * torch.tanh(x / cap)
         p[h] = torch.softmax(x, 0)
