@@ -27,7 +27,7 @@ namespace kv8 {
 using namespace kv;
 
 constexpr int WARPS_PER_SM = 16;                  // a block is NW of them, each with records of its own
-constexpr int STAGES = 3, AHEAD = STAGES - 1;     // records that a warp holds, and those of them on their way
+constexpr int STAGES = 2, AHEAD = STAGES - 1;     // records that a warp holds, and those of them on their way
 constexpr uint32_t ALL = 0xFFFFu;                 // sixteen visible tokens
 constexpr int COLS = 8;                           // query heads side by side
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -161,11 +161,35 @@ template <int G, bool E4M3> struct Query {
     uint32_t frag[G][E4M3 ? 2 : PIECES][2];
     float factor[2], raw[2];                      // of heads 2 t and 2 t + 1: the products' units in powers of two; with a cap: in its units
 };
-template <int G, bool E4M3> __device__ __forceinline__ void load_query(const DecodeParams &p, int b, int first_head, int n, int lane, Query<G, E4M3> &q) {
-    const int g = lane >> 2, t = lane & 3;
+// The lane's channels as they are, on their way while records are looked up
+template <int G> struct Raw { uint4 v[G]; };
+template <int G> __device__ __forceinline__ void fetch_query(const DecodeParams &p, int b, int first_head, int n, int lane, Raw<G> &raw) {
+    const uint16_t *from = reinterpret_cast<const uint16_t *>(p.q) + b * p.q_b + (first_head + min(lane >> 2, n - 1)) * p.q_h + 8 * G * (lane & 3);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+        if (p.q_wide) {
+            raw.v[i] = reinterpret_cast<const uint4 *>(from)[i];
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = from[8 * i + 2 * j] | (uint32_t)from[8 * i + 2 * j + 1] << 16;
+            raw.v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+template <int G, bool E4M3> __device__ __forceinline__ void make_query(const DecodeParams &p, const Raw<G> &raw, int lane, Query<G, E4M3> &q) {
+    const int t = lane & 3;
     float x[8 * G], top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < G; ++i) kv4::load_q8(p, b * p.q_b + (first_head + min(g, n - 1)) * p.q_h + 8 * G * t + 8 * i, x + 8 * i);
+    for (int i = 0; i < G; ++i) {
+        const uint32_t w[4] = {raw.v[i].x, raw.v[i].y, raw.v[i].z, raw.v[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = p.q16 ? __half22float2(*reinterpret_cast<const __half2 *>(&w[j])) : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+            x[8 * i + 2 * j] = f.x;
+            x[8 * i + 2 * j + 1] = f.y;
+        }
+    }
 #pragma unroll
     for (int i = 0; i < 8 * G; ++i) top = fmaxf(top, fabsf(x[i]));
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
@@ -551,8 +575,9 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv8_decode_kernel(
         const uint32_t units = span.units;
         if (d.pieces) {                           // piece `part` of `parts` of a row; units are counted from the sequence's first
             const uint32_t parts = pieces_of(units, d.per), row = (at - before) / parts, part = at - before - row * parts;
-            u = row * units + (uint32_t)((uint64_t)units * part / parts);
-            end = row * units + (uint32_t)((uint64_t)units * (part + 1) / parts);
+            const uint32_t each = units / parts, more = units - each * parts;    // the first `more` have one more
+            u = row * units + part * each + min(part, more);
+            end = u + each + (part < more);
         } else {
             base = before;
             second = u = at;
@@ -571,28 +596,39 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv8_decode_kernel(
         // 32 of the warp's records at a time are looked up by a lane each, while the 32 before are on their way: which one it is, which of
         // its tokens are visible (none: there is no record) and its scales.
         const int mine = (i1 - i0 - warp + NW - 1) / NW;
-        auto look_up = [&](int k, uint32_t &rec, uint32_t &info) {
-            const int i = i0 + warp + (k + lane) * NW, at = i < span.head ? i : i + span.skip, place = at >> (p.page_shift - 4);
-            rec = info = 0;                       // a record that is not meant is fetched too, and not used
-            if (i >= i1) return;
-            const int64_t page = page_id(p.s, b, place);
-            if (page < 0 || page >= p.c.num_pages) { or_status(p.status, OMMX_ST_BAD_PAGE); return; }
-            rec = (uint32_t)((page * p.c.H + head) * p.c.parts + (at & (p.c.parts - 1)));    // below 2^32: there is no memory for more
-            info = visible(p, len, at) | (uint32_t)reinterpret_cast<const uint16_t *>(p.c.scales)[rec] << 16;
+        auto place_of = [&](int k) { const int i = i0 + warp + (k + lane) * NW; return i < span.head ? i : i + span.skip; };
+        auto page_at = [&](int k) -> int64_t {    // -1: none
+            return i0 + warp + (k + lane) * NW < i1 ? page_id(p.s, b, place_of(k) >> (p.page_shift - 4)) : -1;
+        };
+        auto record_at = [&](int k, int64_t page) -> uint32_t {             // one that is not meant is fetched too, and not used
+            if (page >= p.c.num_pages || (page < 0 && i0 + warp + (k + lane) * NW < i1)) or_status(p.status, OMMX_ST_BAD_PAGE);
+            const bool on = page >= 0 && page < p.c.num_pages;
+            return on ? (uint32_t)((page * p.c.H + head) * p.c.parts + (place_of(k) & (p.c.parts - 1))) : 0u;     // below 2^32: there is no memory for more
+        };
+        auto info_at = [&](int k, int64_t page, uint32_t rec) -> uint32_t {
+            return page >= 0 && page < p.c.num_pages ? visible(p, len, place_of(k)) | (uint32_t)reinterpret_cast<const uint16_t *>(p.c.scales)[rec] << 16 : 0u;
         };
         // `rec`, `info`: of the AHEAD first ones, then of 32 at a time, AHEAD of those in use
         uint32_t rec, next_rec, info, next_info, flying[AHEAD];             // flying: of those on their way
-        look_up(0, rec, info);
-        look_up(AHEAD, next_rec, next_info);
+        Raw<G> raw;
+        {
+            const int64_t page = page_at(0), next = page_at(AHEAD);
+            fetch_query(p, b, first_head, n, lane, raw);
+            rec = record_at(0, page);
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            if (k < mine) fetch<G>(ring_at + k * BYTES, p.c.codes + (uint64_t)__shfl_sync(~0u, rec, k) * BYTES, lane);
-            flying[k] = __shfl_sync(~0u, info, k);
-            close_group();
+            for (int k = 0; k < AHEAD; ++k) {
+                if (k < mine) fetch<G>(ring_at + k * BYTES, p.c.codes + (uint64_t)__shfl_sync(~0u, rec, k) * BYTES, lane);
+                close_group();
+            }
+            info = info_at(0, page, rec);
+            next_rec = record_at(AHEAD, next);
+            next_info = info_at(AHEAD, next, next_rec);
         }
         Query<G, E4M3> q;
         State<G> s;
-        load_query<G, E4M3>(p, b, first_head, n, lane, q);
+        make_query<G, E4M3>(p, raw, lane, q);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) flying[k] = __shfl_sync(~0u, info, k);
         clear(s);
         float *put = nullptr;
         if (p.logits) put = p.logits + (((int64_t)b * p.c.H + head) * p.most_units * 16) * p.group + cb * COLS;
@@ -601,7 +637,11 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv8_decode_kernel(
         for (int k0 = 0; k0 < mine; k0 += 32) {
             rec = next_rec;
             info = next_info;
-            look_up(k0 + 32 + AHEAD, next_rec, next_info);
+            {
+                const int64_t page = page_at(k0 + 32 + AHEAD);
+                next_rec = record_at(k0 + 32 + AHEAD, page);
+                next_info = info_at(k0 + 32 + AHEAD, page, next_rec);
+            }
             const int left = mine - k0, now = min(32, left);
             for (int k = 0; k < now; ++k) {
                 if (k + AHEAD < left) fetch<G>(ring_at + write, p.c.codes + (uint64_t)__shfl_sync(~0u, rec, k) * BYTES, lane);
@@ -677,24 +717,32 @@ template <int G> __global__ void __launch_bounds__(32 * COLS) kv8_combine_row_ke
     if (h >= p.group - cb * COLS || r.count == 1) return;                   // not a head, or finished where it was computed
     if (r.count == 0) { zeros<G>(p, b, hq, lane); return; }
     float top, sum, o[G];
+    constexpr int EACH = 4;                       // parts on their way, the first ones while the references meet
+    V v[EACH];
+    float ref[EACH], add[EACH];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) {
+            const bool on = i0 + u < (int)r.count;
+            const float *part = part_at<G>(p, r, on ? i0 + u : i0);
+            v[u] = reinterpret_cast<const V *>(part + h * D)[lane];
+            ref[u] = part[COLS * D + h];
+            add[u] = on ? part[COLS * D + COLS + h] : 0.0f;
+        }
+    };
+    load(0);
     meet<G>(p, r, h, lane, 32, top, sum);
     const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
     for (int i = 0; i < G; ++i) o[i] = 0.0f;
-    for (int i0 = 0; i0 < (int)r.count; i0 += 4) {
-        V v[4];
-        float f[4];
+    for (int i0 = 0; i0 < (int)r.count; i0 += EACH) {
+        if (i0) load(i0);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const bool on = i0 + u < (int)r.count;
-            const float *part = part_at<G>(p, r, on ? i0 + u : i0);
-            v[u] = reinterpret_cast<const V *>(part + h * D)[lane];
-            f[u] = on ? part[COLS * D + COLS + h] * exp2_approx(part[COLS * D + h] - top) * inverse : 0.0f;
+        for (int u = 0; u < EACH; ++u) {
+            const float f = add[u] * exp2_approx(ref[u] - top) * inverse;
+#pragma unroll
+            for (int i = 0; i < G; ++i) o[i] = fmaf(reinterpret_cast<const float *>(&v[u])[i], f, o[i]);
         }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int i = 0; i < G; ++i) o[i] = fmaf(reinterpret_cast<const float *>(&v[u])[i], f[u], o[i]);
     }
     store_o(p, b * p.o_b + hq * p.o_h + lane * G, o);
     if (lane == 0) store_sum(p, b, hq, top, sum);

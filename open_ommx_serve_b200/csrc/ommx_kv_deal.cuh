@@ -20,7 +20,14 @@ namespace kv {
 constexpr uint32_t OVER = 2;                      // in the deal's place: there is none
 constexpr int BEGIN = 64, HEAD = 4;               // HEAD: floats in front of the parts, which hold the deal
 struct Deal { uint32_t per, total; bool pieces, over; };   // over: lengths far past max_seq_len, of more units than 32 bits count
-__device__ __forceinline__ uint32_t pieces_of(uint32_t units, uint32_t per) { return (units + per - 1) / per; }
+// units / per, rounded up. Shares are no smaller than an even one, so quotients are at most as many as there are blocks, and one in 32 bits that is
+// put right by one is enough: the search below took 1.5 us with divisions, 0.5 so.
+__device__ __forceinline__ uint32_t pieces_of(uint32_t units, uint32_t per) {
+    const uint32_t n = units + per - 1;
+    const uint32_t q = (uint32_t)__fdividef((float)n, (float)per);
+    const int32_t rest = (int32_t)(n - q * per);
+    return rest < 0 ? q - 1 : rest >= (int32_t)per ? q + 1 : q;
+}
 template <typename P> __device__ __forceinline__ Deal deal(const P &p, uint32_t rows, uint32_t blocks, int lane) {
     uint64_t sum = 0;
     uint32_t some = 0, most = 0;
