@@ -326,8 +326,14 @@ template <int G, bool E4M3, bool FINE> __device__ __forceinline__ void attend(co
     }
     if (put) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (2 * t + (i & 1) < n) put[(g + 4 * (i & 2)) * p.group + 2 * t + (i & 1)] = x[i];
+        for (int i = 0; i < 4; i += 2) {
+            float *to = put + (g + 4 * i) * p.group + 2 * t;
+            if (p.group % 2 == 0 && 2 * t < n) *reinterpret_cast<float2 *>(to) = make_float2(x[i], x[i + 1]);
+            else if (2 * t < n) {
+                to[0] = x[i];
+                if (2 * t + 1 < n) to[1] = x[i + 1];
+            }
+        }
     }
     const uint32_t mask = info & ALL;
     if (mask != ALL) {                            // what is not visible may be anything
@@ -706,11 +712,11 @@ template <int G> __device__ __forceinline__ void zeros(const DecodeParams &p, in
 }
 
 // Rows of which several blocks have a part, and those of no tokens, where rows are many: a block to a row, a warp to a head, a lane
-// to G channels. Grid: (rows of a sequence, sequences).
-template <int G> __global__ void __launch_bounds__(32 * COLS) kv8_combine_row_kernel(const __grid_constant__ DecodeParams p) {
+// to G channels. `at`: the row of the sequence.
+template <int G> __device__ __forceinline__ void combine_row(const DecodeParams &p, int b, int row) {
     using V = typename Floats<G>::T;
     constexpr int D = 32 * G;
-    const int lane = threadIdx.x & 31, h = threadIdx.x >> 5, b = blockIdx.y, row = blockIdx.x;
+    const int lane = threadIdx.x & 31, h = threadIdx.x >> 5;
     const int head = row / p.col_blocks, cb = row % p.col_blocks, hq = head * p.group + cb * COLS + h;
     const Parts r = parts_of(p, b, row, lane);
     let_next_in();
@@ -749,14 +755,13 @@ template <int G> __global__ void __launch_bounds__(32 * COLS) kv8_combine_row_ke
 }
 
 // The same where rows are few and their parts many: a block to a head. The references and sums of all parts are read at once; then a
-// warp takes every CW-th part, UNROLL of them on their way. Grid: (rows of a sequence x COLS, sequences).
+// warp takes every CW-th part, UNROLL of them on their way.
 constexpr int CW = 8, UNROLL = 5;
-template <int G> __global__ void __launch_bounds__(32 * CW) kv8_combine_head_kernel(const __grid_constant__ DecodeParams p) {
+template <int G> __device__ __forceinline__ void combine_head(const DecodeParams &p, int b, int row, int h) {
     constexpr int D = 32 * G;
     using V = typename Floats<G>::T;
     __shared__ float so[CW][D], weight[MOST_PARTS], sr[CW], ss[CW];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int b = blockIdx.y, row = blockIdx.x / COLS, h = blockIdx.x % COLS;
     const int head = row / p.col_blocks, cb = row % p.col_blocks, hq = head * p.group + cb * COLS + h;
     const Parts r = parts_of(p, b, row, lane);
     let_next_in();
@@ -815,33 +820,81 @@ template <int G> __global__ void __launch_bounds__(32 * CW) kv8_combine_head_ker
 }
 
 // ---- the account ----------------------------------------------------------------------------------
-// weight = keep * before + the sum of a kv head's query heads' weights, by a thread to a token: the logits are there, and so are their
-// sums. Heads are added in order. Grid: (tokens / 256, H, sequences).
-constexpr int WEIGH_THREADS = 256;
-__global__ void __launch_bounds__(WEIGH_THREADS) kv8_weigh_kernel(const __grid_constant__ DecodeParams p) {
+// weight = keep * before + the sum of a kv head's query heads' weights, by a thread to a token: the logits are there. Heads are added in
+// order. PARTS: their references and sums are not, the block makes them of the parts; the kernel that also joins these would be one to wait
+// for (64K tokens: 43.0 us with a kernel behind it, 42.6 beside it).
+constexpr int THREADS = 256, SHARED_HEADS = 64, EACH_TOKENS = 4, STRETCH = THREADS * EACH_TOKENS;
+template <int G, bool PARTS> __device__ __forceinline__ void weigh(const DecodeParams &p, int b, int head, int first) {
+    __shared__ float2 stats[SHARED_HEADS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     wait_earlier();
     let_next_in();
-    const int t = blockIdx.x * WEIGH_THREADS + threadIdx.x, head = blockIdx.y, b = blockIdx.z;
     const int len = length_of(p, b);
-    if (t >= len) return;
-    const int64_t page = page_id(p.s, b, t >> p.page_shift);
-    if (page < 0 || page >= p.c.num_pages) return;                          // reported
+    if (first >= len) return;
     const Span span = span_of(p, len);
-    const int record = t >> 4, unit = record < span.head ? record : record - span.skip;
-    const int64_t at = (page * p.c.H + head) * p.c.page + (t & (p.c.page - 1));
-    float w = p.keep != 0.0f ? p.keep * p.before[at] : 0.0f;
-    if (visible(p, len, record) >> (t & 15) & 1) {
-        if (unit >= p.most_units) return;         // reported
-        const float *x = p.logits + ((((int64_t)b * p.c.H + head) * p.most_units + unit) * 16 + (t & 15)) * p.group;
-        const float2 *stats = p.stats + ((int64_t)b * p.c.H + head) * p.group;
-        float add = 0.0f;
-        for (int h = 0; h < p.group; ++h) {
-            const float2 s = stats[h];
-            add = fmaf(exp2_approx(x[h] - s.x), s.y, add);
+    int64_t at[EACH_TOKENS];                      // of the token's weight, -1: not kept
+    const float *x[EACH_TOKENS];                  // its logits, or null
+    float before[EACH_TOKENS], add[EACH_TOKENS];
+#pragma unroll
+    for (int u = 0; u < EACH_TOKENS; ++u) {
+        const int t = first + u * THREADS + threadIdx.x, record = t >> 4, unit = record < span.head ? record : record - span.skip;
+        const int64_t page = t < len ? page_id(p.s, b, t >> p.page_shift) : -1;
+        at[u] = page >= 0 && page < p.c.num_pages ? (page * p.c.H + head) * p.c.page + (t & (p.c.page - 1)) : -1;      // not there: reported
+        x[u] = nullptr;
+        if (at[u] >= 0 && (visible(p, len, record) >> (t & 15) & 1)) {
+            if (unit < p.most_units) x[u] = p.logits + ((((int64_t)b * p.c.H + head) * p.most_units + unit) * 16 + (t & 15)) * p.group;
+            else at[u] = -1;                      // past max_seq_len: reported
         }
-        w += add;
+        add[u] = 0.0f;
     }
-    p.c.weight[at] = w;
+#pragma unroll
+    for (int u = 0; u < EACH_TOKENS; ++u) before[u] = at[u] >= 0 && p.keep != 0.0f ? p.before[at[u]] : 0.0f;
+    for (int h0 = 0; h0 < p.group; h0 += SHARED_HEADS) {
+        if (h0) __syncthreads();
+        const int n = min(SHARED_HEADS, p.group - h0);
+        if constexpr (PARTS) {
+            for (int h = warp; h < n; h += THREADS / 32) {
+                const int row = head * p.col_blocks + (h0 + h) / COLS;
+                const Parts r = parts_of(p, b, row, lane);
+                float2 s = make_float2(LOWEST, 0.0f);
+                if (r.count == 1) s = p.stats[((int64_t)b * p.c.H + head) * p.group + h0 + h];
+                else if (r.count > 1) {
+                    float top, sum;
+                    meet<G>(p, r, (h0 + h) % COLS, lane, 32, top, sum);
+                    s = make_float2(top, sum != 0.0f ? 1.0f / sum : 0.0f);
+                }
+                if (lane == 0) stats[h] = s;
+            }
+        } else {
+            for (int h = threadIdx.x; h < n; h += THREADS) stats[h] = p.stats[((int64_t)b * p.c.H + head) * p.group + h0 + h];
+        }
+        __syncthreads();
+        for (int h = 0; h < n; ++h) {
+            const float2 s = stats[h];
+            if (s.y == 0.0f) continue;            // no shares were dealt out
+#pragma unroll
+            for (int u = 0; u < EACH_TOKENS; ++u)
+                if (x[u]) add[u] = fmaf(exp2_approx(x[u][h0 + h] - s.x), s.y, add[u]);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < EACH_TOKENS; ++u)
+        if (at[u] >= 0) p.c.weight[at[u]] = (p.keep != 0.0f ? p.keep * before[u] : 0.0f) + add[u];
+}
+
+// Behind the first kernel: what joins the parts (BY: nothing, a block to a row, a block to a head), and the account's blocks.
+// Grid: (joining blocks of a sequence + blocks of tokens x H, sequences).
+enum { NONE, ROW, HEAD_BLOCKS };
+template <int G, int BY> __global__ void __launch_bounds__(THREADS) kv8_second_kernel(const __grid_constant__ DecodeParams p, int joining) {
+    static_assert(THREADS == 32 * COLS && THREADS == 32 * CW, "one size of blocks");
+    const int b = blockIdx.y, i = blockIdx.x;
+    if (i < joining) {
+        if constexpr (BY == ROW) combine_row<G>(p, b, i);
+        if constexpr (BY == HEAD_BLOCKS) combine_head<G>(p, b, i / COLS, i % COLS);
+        return;
+    }
+    const int blocks = (gridDim.x - joining) / p.c.H, at = i - joining, head = at / blocks;
+    weigh<G, BY != NONE>(p, b, head, (at - head * blocks) * STRETCH);
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -871,7 +924,7 @@ static int64_t workspace_floats(const ommx_kv8_decode_args *a) {
     return (n + 3) / 4 * 4;
 }
 
-template <int G, bool E4M3, bool FINE, int NW, bool CLUSTER> static int launch_decode(const DecodeParams &p, int64_t blocks, int cluster, cudaStream_t st) {
+template <int G, bool E4M3, bool FINE, int NW, bool CLUSTER> static int launch_decode(const DecodeParams &p, int64_t blocks, int cluster, int64_t tokens, cudaStream_t st) {
     static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may take its shared memory
     int dev = 0;
     if (int rc = current_device(&dev)) return rc;
@@ -880,11 +933,14 @@ template <int G, bool E4M3, bool FINE, int NW, bool CLUSTER> static int launch_d
         allowed.fetch_or(1ull << dev, std::memory_order_release);
     }
     if (int rc = launch_dependent(kv8_decode_kernel<G, E4M3, FINE, NW, CLUSTER>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G, NW>), st, cluster, p)) return rc;
-    if (p.whole || CLUSTER) return 0;
     // a row has some blocks / rows parts
-    const int rows = p.c.H * p.col_blocks;
-    if ((int64_t)rows * p.s.B * COLS >= blocks) return launch_dependent(kv8_combine_row_kernel<G>, dim3(rows, p.s.B), 32 * COLS, 0, st, 1, p);
-    return launch_dependent(kv8_combine_head_kernel<G>, dim3(rows * COLS, p.s.B), 32 * CW, 0, st, 1, p);
+    const int rows = p.c.H * p.col_blocks, account = tokens ? (int)((tokens + STRETCH - 1) / STRETCH) * p.c.H : 0;
+    if (p.whole || CLUSTER) {
+        if (!account) return 0;
+        return launch_dependent(kv8_second_kernel<G, NONE>, dim3(account, p.s.B), THREADS, 0, st, 1, p, 0);
+    }
+    if ((int64_t)rows * p.s.B * COLS >= blocks) return launch_dependent(kv8_second_kernel<G, ROW>, dim3(rows + account, p.s.B), THREADS, 0, st, 1, p, rows);
+    return launch_dependent(kv8_second_kernel<G, HEAD_BLOCKS>, dim3(rows * COLS + account, p.s.B), THREADS, 0, st, 1, p, rows * COLS);
 }
 
 static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
@@ -901,7 +957,7 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     if (!std::isfinite(a->sm_scale)) return fail(OMMX_E_ARG, "kv8_decode: sm_scale must be finite");
     if (a->window < 0 || a->sink_tokens < 0 || a->max_seq_len < 0) return fail(OMMX_E_ARG, "kv8_decode: window, sink_tokens and max_seq_len must not be negative");
     if (a->cache.weight && (!std::isfinite(a->keep) || (a->keep != 0.0f && !a->weight_before))) return fail(OMMX_E_ARG, "kv8_decode: keep must be finite, and what is kept must be given");
-    if (p.s.B > 65535 || p.c.H > 65535) return fail(OMMX_E_UNSUPPORTED, "kv8_decode: a batch of %d", p.s.B);
+    if (p.s.B > 65535) return fail(OMMX_E_UNSUPPORTED, "kv8_decode: a batch of %d", p.s.B);
     if (p.s.B == 0) return 0;
     if (!a->q || !a->o || !a->lse) return fail(OMMX_E_ARG, "kv8_decode: q, o and lse must not be null");
     const int64_t need = workspace_floats(a);
@@ -941,21 +997,20 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     p.whole = units <= WHOLE / 2 || (units <= WHOLE && cluster == 1);
     if (p.whole) cluster = 1;
     const int64_t blocks = p.whole ? rows : cluster > 1 ? cluster * rows : most < 1 ? 1 : most < hold ? most : hold;
+    const int64_t tokens = p.c.weight ? most_tokens(a) : 0;                 // that weights are kept of
+    if ((tokens / STRETCH + 1) * p.c.H >= 1LL << 30) return fail(OMMX_E_UNSUPPORTED, "kv8_decode: weights of %lld tokens of %d kv heads: give max_seq_len", (long long)tokens, p.c.H);
     auto launch = [&](auto g, auto e4m3, auto fine) {
         constexpr int G = decltype(g)::value;
         constexpr bool E4M3 = decltype(e4m3)::value, FINE = decltype(fine)::value;
-        if (cluster > 1) return launch_decode<G, E4M3, FINE, 8, true>(p, blocks, cluster, st);
-        return warps == 4 ? launch_decode<G, E4M3, FINE, 4, false>(p, blocks, 1, st) : launch_decode<G, E4M3, FINE, 8, false>(p, blocks, 1, st);
+        if (cluster > 1) return launch_decode<G, E4M3, FINE, 8, true>(p, blocks, cluster, tokens, st);
+        return warps == 4 ? launch_decode<G, E4M3, FINE, 4, false>(p, blocks, 1, tokens, st) : launch_decode<G, E4M3, FINE, 8, false>(p, blocks, 1, tokens, st);
     };
     using std::integral_constant;
     auto of_size = [&](auto e4m3, auto fine) {
         return a->cache.head_dim == 128 ? launch(integral_constant<int, 4>(), e4m3, fine) : launch(integral_constant<int, 2>(), e4m3, fine);
     };
     auto of_code = [&](auto fine) { return a->cache.code == OMMX_KV8_E4M3 ? of_size(std::true_type(), fine) : of_size(std::false_type(), fine); };
-    const int rc = a->o_dtype != OMMX_DT_BF16 ? of_code(std::true_type()) : of_code(std::false_type());
-    const int64_t tokens = most_tokens(a);
-    if (rc || !p.c.weight || !tokens) return rc;
-    return launch_dependent(kv8_weigh_kernel, dim3((unsigned)((tokens + WEIGH_THREADS - 1) / WEIGH_THREADS), p.c.H, p.s.B), WEIGH_THREADS, 0, st, 1, p);
+    return a->o_dtype != OMMX_DT_BF16 ? of_code(std::true_type()) : of_code(std::false_type());
 }
 
 }  // namespace kv8

@@ -839,7 +839,7 @@ def test_nothing_to_do():
 
 
 def test_launches():
-    """Append and read back are one launch each, attention one or two (three with an account), eviction one (two where
+    """Append and read back are one launch each, attention one or two (two with an account), eviction one (two where
     it shortens the lengths it reads)."""
     lib = _lib.load()
 
@@ -854,7 +854,7 @@ def test_launches():
     where = (c["codes"], c["scales"], layer.table, layer.length)
     assert launches(lambda: ommx_kv8_append(k, v, *where)) == 1
     assert launches(lambda: ommx_kv8_gather(*where, k, v)) == 1
-    for n, more, want in ((None, {}, 2), (None, dict(weight=c["weight"]), 3), (None, dict(window=300, sink_tokens=4), 1), (200, {}, 1), (200, dict(weight=c["weight"]), 2)):
+    for n, more, want in ((None, {}, 2), (None, dict(weight=c["weight"]), 2), (None, dict(window=300, sink_tokens=4), 1), (200, {}, 1), (200, dict(weight=c["weight"]), 2)):
         assert launches(lambda: ommx_kv8_decode_attention(q, *where, layer.o, layer.lse, max_seq_len=n, **more)) == want
     assert launches(layer.evict) == 2
     assert launches(lambda: ommx_kv8_evict(c["codes"], c["scales"], c["weight"], layer.table, layer.length, layer.kept)) == 1
