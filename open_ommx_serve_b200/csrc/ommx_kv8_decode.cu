@@ -473,6 +473,7 @@ template <int G, int NW> struct Memory {
     };
     alignas(16) float merged[PART<G>];            // of this block, where a cluster shares a row
     float ref[COLS][NW], sum[COLS][NW];
+    uint32_t fits[NW];                            // of the deal
 };
 
 __device__ __forceinline__ bool too_many(const DecodeParams &p, uint32_t units, uint32_t rows) {
@@ -558,7 +559,8 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv8_decode_kernel(
         end = u + span.units;
         if (span.units == 0) { nothing<G>(p, b, blockIdx.x - b * rows); return; }
     } else {
-        const Deal d = deal(p, rows, gridDim.x, lane);
+        const Lengths own = lengths_of(p, lane);
+        const Deal d = deal(p, own, rows, gridDim.x, lane, warp, NW, m.fits);
         if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<uint2 *>(p.work) = make_uint2(d.per, d.over ? OVER : d.pieces);
         // the sequence that this block's (first) unit lies in; `at`, `before`: this block and the first of the sequence, in pieces or units
         const uint32_t at = d.pieces ? blockIdx.x : blockIdx.x * d.per;
@@ -566,7 +568,15 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv8_decode_kernel(
         uint32_t before = 0;
         for (int b0 = 0;; b0 += 32) {
             if (b0 >= p.s.B) return;              // no piece for this block (or lengths past max_seq_len, more than 32 bits count)
-            const int l = b0 + lane < p.s.B ? length_of(p, b0 + lane) : 0, n = units_of(p, l);
+            int l;
+            uint32_t n;
+            if (b0 < 64) {
+                l = b0 ? own.len[1] : own.len[0];
+                n = b0 ? own.units[1] : own.units[0];
+            } else {
+                l = b0 + lane < p.s.B ? length_of(p, b0 + lane) : 0;
+                n = units_of(p, l);
+            }
             const uint32_t v = d.pieces ? pieces_of(n, d.per) : n, sum = warp_inclusive_scan(v, lane), past = __ballot_sync(~0u, before + sum * rows > at);
             if (past) {
                 const int from = __ffs(past) - 1;
@@ -597,7 +607,7 @@ __global__ void __launch_bounds__(32 * NW, WARPS_PER_SM / NW) kv8_decode_kernel(
             span = span_of(p, len);
         }
         const int units = span.units, row = (u - base) / units, i0 = u - base - row * units, i1 = min((uint32_t)units, i0 + (end - u));
-        const int head = row / p.col_blocks, cb = row % p.col_blocks;
+        const int head = p.col_blocks == 1 ? row : row / p.col_blocks, cb = row - head * p.col_blocks;
         const int first_head = head * p.group + cb * COLS, n = min(COLS, p.group - cb * COLS);
         // 32 of the warp's records at a time are looked up by a lane each, while the 32 before are on their way: which one it is, which of
         // its tokens are visible (none: there is no record) and its scales.

@@ -28,12 +28,24 @@ __device__ __forceinline__ uint32_t pieces_of(uint32_t units, uint32_t per) {
     const int32_t rest = (int32_t)(n - q * per);
     return rest < 0 ? q - 1 : rest >= (int32_t)per ? q + 1 : q;
 }
-template <typename P> __device__ __forceinline__ Deal deal(const P &p, uint32_t rows, uint32_t blocks, int lane) {
-    uint64_t sum = 0;
-    uint32_t some = 0, most = 0;
-    const uint32_t own = lane < p.s.B ? units_of(p, length_of(p, lane)) : 0;
-    for (int b = lane; b < p.s.B; b += 32) {
-        const uint32_t n = b == lane ? own : units_of(p, length_of(p, b));
+// The lengths of the first 64 sequences, two to a lane of each warp, and their units
+struct Lengths { int len[2]; uint32_t units[2]; };
+template <typename P> __device__ __forceinline__ Lengths lengths_of(const P &p, int lane) {
+    Lengths l;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int b = lane + 32 * i;
+        l.len[i] = b < p.s.B ? length_of(p, b) : 0;
+        l.units[i] = b < p.s.B ? units_of(p, l.len[i]) : 0;
+    }
+    return l;
+}
+// All warps of a block call it. `shared`: a word for each.
+template <typename P> __device__ __forceinline__ Deal deal(const P &p, const Lengths &own, uint32_t rows, uint32_t blocks, int lane, int warp, int warps, uint32_t *shared) {
+    uint64_t sum = (uint64_t)own.units[0] + own.units[1];
+    uint32_t some = (own.units[0] > 0) + (own.units[1] > 0), most = max(own.units[0], own.units[1]);
+    for (int b = lane + 64; b < p.s.B; b += 32) {
+        const uint32_t n = units_of(p, length_of(p, b));
         sum += n;
         some += n > 0;
         most = max(most, n);
@@ -50,15 +62,22 @@ template <typename P> __device__ __forceinline__ Deal deal(const P &p, uint32_t 
     d.pieces = false;
     if (d.over) or_status(p.status, OMMX_ST_BAD_LENGTH);
     if (d.over || full == 0 || full > blocks) return d;
-    // pieces of `per` take total / per + full blocks at most; fewer may do
+    // Pieces of `per` take total / per + full blocks at most; fewer may do. Each warp tries one of as many sizes between, and the range is cut to
+    // the one before the smallest that will do (one size after the other: 1.0 us of 32 sequences, 1.7 of 61; so 0.4).
     uint32_t lo = even, hi = min(max(most, even), full < blocks ? max(even, d.total / (blocks - full) + 1) : 0xFFFFFFFFu);
 #pragma unroll 1
-    for (int i = 0; i < 6 && lo < hi; ++i) {
-        const uint32_t per = i == 0 ? lo : (lo + hi) / 2;
-        uint32_t n = pieces_of(own, per);
-        for (int b = lane + 32; b < p.s.B; b += 32) n += pieces_of(units_of(p, length_of(p, b)), per);
-        if (__reduce_add_sync(~0u, n) * rows <= blocks) hi = per;
-        else lo = per + 1;
+    for (int span = 1; span < 64 && lo < hi; span *= warps) {
+        const uint32_t step = (hi - lo + warps - 1) / warps, per = lo + warp * step;        // the first is `lo`
+        uint32_t n = pieces_of(own.units[0], per) + pieces_of(own.units[1], per);
+        for (int b = lane + 64; b < p.s.B; b += 32) n += pieces_of(units_of(p, length_of(p, b)), per);
+        n = __reduce_add_sync(~0u, n);
+        if (lane == 0) shared[warp] = n * rows <= blocks && per < hi;
+        __syncthreads();
+        const uint32_t fits = __ballot_sync(~0u, lane < warps && shared[lane]);
+        const int first = fits ? __ffs(fits) - 1 : warps;
+        if (fits) hi = lo + first * step;
+        if (first) lo = min(lo + (first - 1) * step + 1, hi);
+        __syncthreads();
     }
     if (hi <= even + BEGIN) { d.per = hi; d.pieces = true; }
     return d;
