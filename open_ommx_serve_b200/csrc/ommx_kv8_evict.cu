@@ -45,6 +45,14 @@ __device__ __forceinline__ uint32_t peer_word(const void *at, uint32_t rank) {
 // What a block knows of the places that it moves
 struct Place { uint32_t from, to; float weight; uint16_t own, scales; };    // rows; exponents of what it takes, and of its record
 
+__device__ __forceinline__ int peer_half(const uint16_t *at, uint32_t rank) {
+    uint32_t there;
+    uint16_t v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(rank));
+    asm volatile("ld.shared::cluster.u16 %0, [%1];" : "=h"(v) : "r"(there) : "memory");
+    return v;
+}
+
 // Grid: (cluster x H, B).
 template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict_kernel(const __grid_constant__ EvictParams p) {
     constexpr int D = 32 * G;
@@ -53,11 +61,12 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
     __shared__ __align__(16) int histogram[BINS];
     __shared__ uint32_t few[FEW];
     __shared__ Place places[PLACES];
-    __shared__ int warp_sum[2][WARPS], starts[MOST_CLUSTER + 1], bin, left, inside, listed, more, same, above_here, equal_here, bad, spoilt;
+    __shared__ int warp_sum[2][WARPS], starts[MOST_CLUSTER + 1], bin, left, inside, listed, more, same, above_here, equal_here, first_place, bad, spoilt;
+    __shared__ int firsts[MOST_CLUSTER];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t n = cluster_size(), rank = cluster_rank();
     const int head = blockIdx.x / n, b = blockIdx.y;
-    if (tid == 0) bad = listed = 0;
+    if (tid == 0) bad = listed = more = 0;
     histogram[tid] = histogram[tid + THREADS] = 0;
     wait_earlier();
     let_next_in();
@@ -93,6 +102,9 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
             for (int i = rank * THREADS + tid; i < p.budget; i += n * THREADS) out[i] = !faults && i < len ? i : -1;
     };
     if (faults) { leave(true); return; }
+    const int share = ((len + (int)n - 1) / (int)n + 31) & ~31;
+    const bool short_row = share <= TURN;         // a block lists its tokens in shared memory, behind the rows; else the list is the caller's
+    uint16_t *list = reinterpret_cast<uint16_t *>(memory + PLACES * 2 * D);
     if (all) {
         __syncthreads();
         cluster_barrier();
@@ -103,7 +115,7 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
         if (faults || p.in_place) return;
     } else {
         // block `rank` has the keys lo .. hi - 1; first .. last - 1 of them are not kept anyway
-        const int share = ((len + (int)n - 1) / (int)n + 31) & ~31, lo = min(len, (int)rank * share), hi = min(len, lo + share);
+        const int lo = min(len, (int)rank * share), hi = min(len, lo + share);
         const int first = max(lo, p.sinks), last = min(hi, len - p.recent);
         const float *weight = p.c.weight;
         auto load = [&](int i) {
@@ -149,6 +161,7 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
         const int wanted = p.budget - p.sinks - p.recent;
         int want = wanted, width = 31;
         uint32_t a = ZERO;
+        bool placed = false;                      // the block knows where its first token goes
         for (bool begun = false; width > 0; begun = true) {
             const int shift = max(0, width - 11);
             // the lowest part is not counted: what is not above it is in it, and often it is the one that most are in
@@ -192,13 +205,26 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
             if (!begun && bin == 0) { a = 0; width = 32; }                  // `want` as it was
             else { a += (uint32_t)bin << shift; want = left; width = shift; }
             if (width > 0 && inside <= FEW) {     // all blocks say so
-                each_key([&](uint32_t key) { if ((key - a) >> width == 0) few[atomicAdd(&listed, 1)] = key; });
+                int over = 0;                     // keys above those
+                each_key([&](uint32_t key) {
+                    if ((key - a) >> width == 0) few[atomicAdd(&listed, 1)] = key;
+                    else over += key > a;
+                });
+                over = __reduce_add_sync(~0u, over);
+                if (lane == 0 && over) atomicAdd(&more, over);
                 __syncthreads();
                 cluster_barrier();
                 if (warp == 0) {
                     const int mine = lane < (int)n ? (int)peer_word(&listed, lane % n) : 0, sum = warp_inclusive_scan(mine, lane);
                     if (lane < MOST_CLUSTER) starts[lane + 1] = sum;
                     if (lane == 0) starts[0] = 0;
+                }
+                if (warp == 1) {                  // what the blocks before this one keep whatever the last key is
+                    const int r = lane, from = min(len, r * share), to = min(len, from + share);
+                    const int pinned = to - from - max(0, min(to, len - p.recent) - max(from, p.sinks));
+                    const int sure = __reduce_add_sync(~0u, r < (int)rank ? (int)peer_word(&more, r % n) + pinned : 0);
+                    if (lane == 0) above_here = sure;
+                    if (lane == 1) equal_here = 0;
                 }
                 __syncthreads();
                 const int count = starts[n];
@@ -236,6 +262,19 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
                     width = cut;
                     __syncthreads();
                 }
+                // and of these few: what is left of a key is by how much it is above the last one
+                int m = 0, e = 0;
+#pragma unroll
+                for (int j = 0; j < FEW / THREADS; ++j) {
+                    const bool theirs = tid + j * THREADS < starts[rank];
+                    m += theirs && (int)k[j] > 0;
+                    e += theirs && k[j] == 0;
+                }
+                m = __reduce_add_sync(~0u, m);
+                e = __reduce_add_sync(~0u, e);
+                if (lane == 0 && m) atomicAdd(&above_here, m);
+                if (lane == 0 && e) atomicAdd(&equal_here, e);
+                placed = true;
                 break;
             }
             __syncthreads();
@@ -268,19 +307,23 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
         }
         if (lane == 0) { warp_sum[0][warp] = above; warp_sum[1][warp] = equal; }
         __syncthreads();
-        if (warp == 0) {
-            const int m = __reduce_add_sync(~0u, warp_sum[0][lane]), e = __reduce_add_sync(~0u, warp_sum[1][lane]);
-            if (lane == 0) { more = m; same = e; }
+        if (!placed) {
+            if (warp == 0) {
+                const int m = __reduce_add_sync(~0u, warp_sum[0][lane]), e = __reduce_add_sync(~0u, warp_sum[1][lane]);
+                if (lane == 0) { more = m; same = e; }
+            }
+            __syncthreads();
+            cluster_barrier();
+            if (warp == 0) {
+                const int m = __reduce_add_sync(~0u, lane < (int)rank ? (int)peer_word(&more, lane % n) : 0);
+                const int e = __reduce_add_sync(~0u, lane < (int)rank ? (int)peer_word(&same, lane % n) : 0);
+                if (lane == 0) { above_here = m; equal_here = e; }
+            }
+            __syncthreads();
         }
-        __syncthreads();
-        cluster_barrier();
-        if (warp == 0) {
-            const int m = __reduce_add_sync(~0u, lane < (int)rank ? (int)peer_word(&more, lane % n) : 0);
-            const int e = __reduce_add_sync(~0u, lane < (int)rank ? (int)peer_word(&same, lane % n) : 0);
-            if (lane == 0) { above_here = m; equal_here = e; }
-        }
-        __syncthreads();
         int above_all = above_here, equal_all = equal_here;
+        const int first_here = above_all + min(equal_all, want);
+        if (tid == 0) first_place = first_here;
         for (int turn = 0; turn < turns; ++turn) {
             if (turn > 0) look(turn);
             if (turns > 1) {
@@ -297,12 +340,23 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
 #pragma unroll
             for (int u = 0; u < HELD; ++u) {
                 const int at = above + __popc(ms[u] & below), eq = equal + __popc(es[u] & below);
-                if (ms[u] >> lane & 1 || (es[u] >> lane & 1 && eq < want)) out[at + min(eq, want)] = place(turn, u);
+                if (ms[u] >> lane & 1 || (es[u] >> lane & 1 && eq < want)) {
+                    const int to = at + min(eq, want);
+                    if (short_row) list[to - first_here] = (uint16_t)(place(turn, u) - lo);
+                    else out[to] = place(turn, u);
+                }
                 above += __popc(ms[u]);
                 equal += __popc(es[u]);
             }
         }
+        __syncthreads();
         cluster_barrier();                        // the list is there, and no peer reads this block's sums any more
+        if (short_row) {
+            if (tid < (int)n) firsts[tid] = (int)peer_word(&first_place, tid);
+            __syncthreads();
+            const int end = rank + 1 < n ? firsts[rank + 1] : p.budget;
+            for (int i = first_here + tid; i < end; i += THREADS) out[i] = lo + list[i - first_here];
+        }
     }
     // ---- the move. In shared memory a row is D bytes of keys and D of values; 16 bytes to a thread.
     constexpr int CHUNKS = D / 8;                 // of a row
@@ -315,7 +369,16 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
         if (tid < PLACES) {
             Place x = {0, 0, 0.0f, 0, 0};
             if (tid < count) {
-                const int i = start + tid, at = all ? i : __ldcg(out + i);
+                const int i = start + tid;
+                int at = i;
+                if (!all && short_row) {          // from the list of the block that it is in
+                    int r = 0;
+#pragma unroll
+                    for (int j = 1; j < MOST_CLUSTER; ++j) r = j < (int)n && firsts[j] <= i ? j : r;
+                    at = r * share + peer_half(list + (i - firsts[r]), r);
+                } else if (!all) {
+                    at = __ldcg(out + i);
+                }
                 const int64_t page = page_id(p.s, b, at >> p.page_shift), to = page_id(p.to, b, i >> p.page_shift);
                 x.from = row_of(p, page, head, at);
                 x.to = row_of(p, to, head, i);
@@ -372,7 +435,7 @@ template <int G, bool E4M3> static int launch_evict(const EvictParams &p, int cl
         OMMX_CUDA_TRY(cudaFuncSetAttribute(kv8_evict_kernel<G, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * MOST_KEYS));
         allowed.fetch_or(1ull << dev, std::memory_order_release);
     }
-    const size_t keys = 4 * (size_t)p.keys, rows = (size_t)PLACES * 64 * G;
+    const size_t keys = 4 * (size_t)p.keys, rows = (size_t)PLACES * 64 * G + 2 * TURN;                 // rows and a list
     return launch_dependent(kv8_evict_kernel<G, E4M3>, dim3(cluster * p.c.H, p.s.B), THREADS, keys > rows ? keys : rows, st, cluster, p);
 }
 

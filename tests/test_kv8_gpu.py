@@ -644,6 +644,16 @@ def test_eviction_of_long_rows(L, budget):
         evict([L, 60], 1, 64, 16, I8, budget, 4, min(30, budget - 4), max_len=max_len, apart=max_len == 100)
 
 
+@pytest.mark.parametrize("kind", ["ties", "alike", "zeros", "signs"])
+def test_eviction_of_long_rows_of_like_weights(kind):
+    """More tokens of one weight than a block finishes for itself."""
+    def fill(w):
+        u = torch.rand(w.shape, generator=torch.Generator().manual_seed(3))
+        w.copy_({"ties": (u * 2).floor(), "alike": torch.full_like(u, 0.3), "zeros": torch.where(u < 0.97, 0.0, u), "signs": torch.where(u < 0.5, -1.0, -2.0)}[kind])
+    for max_len in (20000, 100):
+        evict([20000, 60, 9000], 1, 64, 16, E4M3, 2500, 4, 30, weights=fill, max_len=max_len)
+
+
 def test_eviction_where_keys_do_not_fit():
     """Many rows, so that one block has a row of more keys than it holds."""
     lens = [50000] + [30] * 80
