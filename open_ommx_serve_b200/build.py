@@ -21,7 +21,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libommx_b200.so")
 SOURCES = ("ommx_stage1_h8.cu", "ommx_stage1_h4.cu", "ommx_stage1_h2.cu", "ommx_stage1_h1.cu", "ommx_decode.cu", "ommx_pack.cu",
            "ommx_kv4_store.cu", "ommx_kv4_decode.cu", "ommx_kv4_select.cu", "ommx_kv8_store.cu", "ommx_kv8_decode.cu", "ommx_kv8_evict.cu", "ommx_capi.cu")
-HEADERS = ("ommx_common.cuh", "ommx_stage1.cuh", "ommx_decode_tc.cuh", "ommx_kv4.cuh", "ommx_kv8.cuh", "ommx_kv_deal.cuh", "ommx_tables.inc",
+HEADERS = ("ommx_common.cuh", "ommx_stage1.cuh", "ommx_decode_tc.cuh", "ommx_kv4.cuh", "ommx_kv8.cuh", "ommx_kv8_deal.cuh", "ommx_kv_device.cuh", "ommx_tables.inc",
            os.path.join("..", "..", "include", "ommx_b200.h"))
 OBJ = os.path.join(PKG, "build")
 HOST_LIB = HOST_PATH

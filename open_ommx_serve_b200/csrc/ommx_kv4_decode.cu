@@ -30,9 +30,12 @@
 #include <type_traits>
 
 #include "ommx_kv4.cuh"
+#include "ommx_kv_device.cuh"
 
 namespace ommx {
 namespace kv4 {
+
+using namespace kv;
 
 constexpr int WARPS_PER_SM = 16;                  // as many as the registers hold; a block is NW of them, each with records of its own
 constexpr int STAGES = 3, AHEAD = STAGES - 1;     // records that a warp holds, and those of them on their way
@@ -137,30 +140,8 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-    uint32_t y;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float2 half2_floats(uint32_t b) { return __half22float2(*reinterpret_cast<const __half2 *>(&b)); }
 __device__ __forceinline__ float scale_of(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 __device__ __forceinline__ float zero_of(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23 & 255u) - 127; }
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 // of a reference and a sum of weights, which lie near 2^-ABOVE
 __device__ __forceinline__ float log_sum(float ref, float sum) {
     return sum != 0.0f ? ((ref - ABOVE) + log2f(sum * power_of_two(ABOVE))) * LN2 : -INFINITY;
@@ -542,25 +523,6 @@ template <int G> __device__ __forceinline__ void nothing(const DecodeParams &p, 
 }
 
 // ---- a row shared by a cluster's blocks: their parts meet in distributed shared memory ----
-__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float4 peer_float4(uint32_t at, uint32_t rank) {
-    uint32_t there;
-    float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
-    return v;
-}
-__device__ __forceinline__ float peer_float(uint32_t at, uint32_t rank) {
-    uint32_t there;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-    return v;
-}
 // Head h is finished by block h mod n of the cluster, by its warp h.
 constexpr int MOST_CLUSTER = 8;
 template <int G> __device__ __forceinline__ void merge_cluster(const DecodeParams &p, const float *merged, int b, int first_head, int heads, int h, int lane) {

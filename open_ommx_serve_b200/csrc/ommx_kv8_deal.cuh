@@ -1,11 +1,11 @@
-// How the paged caches' attention kernels deal their work out, and where a row's parts meet.  P: a kernel's parameters, with s.B, c.H,
-// col_blocks, least, work and status, for which length_of(p, b) and units_of(p, length) say how many units sequence b has.
+// How the 8-bit cache's attention deals its work out, and where a row's parts are.  P: a kernel's parameters, with s.B, c.H, col_blocks, least,
+// work and status, for which length_of(p, b) and units_of(p, length) say how many units sequence b has.
 #pragma once
 
-#include "ommx_kv4.cuh"
+#include "ommx_kv8.cuh"
 
 namespace ommx {
-namespace kv {
+namespace kv8 {
 
 // Units are records (16 tokens of a kv head, for a block of its query heads); a row (sequence, kv head, block of heads) is a run of
 // them. Lengths are known on the device alone, so every block works the same deal out, and leaves it for the second kernel:
@@ -89,7 +89,7 @@ template <typename P> __device__ __forceinline__ Deal deal(const P &p, const Len
 struct Parts { uint32_t first, count; bool late; };
 template <typename P> __device__ __forceinline__ Parts parts_of(const P &p, int b, uint32_t row, int lane) {
     const uint32_t rows = p.c.H * p.col_blocks, units = units_of(p, length_of(p, b)), own = lane < b ? units_of(p, length_of(p, lane)) : 0;
-    kv4::wait_earlier();
+    wait_earlier();
     const uint2 d = *reinterpret_cast<const uint2 *>(p.work);
     uint32_t before = d.y ? pieces_of(own, d.x) : own;
     for (int i = lane + 32; i < b; i += 32) {
@@ -112,26 +112,5 @@ template <typename P> __device__ __forceinline__ Parts parts_of(const P &p, int 
     return r;
 }
 
-// ---- clusters -------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float4 peer_float4(uint32_t at, uint32_t rank) {
-    uint32_t there;
-    float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
-    return v;
-}
-__device__ __forceinline__ float peer_float(uint32_t at, uint32_t rank) {
-    uint32_t there;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-    return v;
-}
-
-}  // namespace kv
+}  // namespace kv8
 }  // namespace ommx

@@ -19,7 +19,8 @@
 #include <type_traits>
 
 #include "ommx_kv8.cuh"
-#include "ommx_kv_deal.cuh"
+#include "ommx_kv8_deal.cuh"
+#include "ommx_kv_device.cuh"
 
 namespace ommx {
 namespace kv8 {
@@ -93,7 +94,6 @@ template <int G> __device__ __forceinline__ void store_o(const DecodeParams &p, 
 #pragma unroll
     for (int i = 0; i < G; ++i) store_o(p, at + i, v[i]);
 }
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 // A head's reference and sum of weights
 __device__ __forceinline__ void store_sum(const DecodeParams &p, int b, int hq, float ref, float sum) {
     p.lse[b * p.lse_b + hq] = sum != 0.0f ? (ref + log2f(sum)) * LN2 : -INFINITY;
@@ -114,26 +114,6 @@ __device__ __forceinline__ void mma_s8(float (&c)[4], uint32_t a0, uint32_t a1, 
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[i] = __uint_as_float(d[i]);
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-    uint32_t y;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23 & 255u) - 127; }
 
 // The codes of four channels of two tokens (their words) to fp16 pairs, a channel to each
 template <bool E4M3> __device__ __forceinline__ void value_pairs(uint32_t a, uint32_t b, uint32_t (&pair)[4]) {

@@ -9,7 +9,7 @@
 // * moves: places ascend, and a token never moves up. So once a cluster has read all that a stretch of places takes into its shared
 //   memory it can write that stretch where the tokens lie, and go on to the next.
 #include "ommx_kv8.cuh"
-#include "ommx_kv_deal.cuh"
+#include "ommx_kv_device.cuh"
 
 namespace ommx {
 namespace kv8 {
