@@ -493,7 +493,7 @@ int64_t ommx_b200_kv4_select_workspace_bytes(int32_t batch, int32_t n_kv_heads, 
  * E is the smallest from 1 on for which the block's largest value is at most 127 (int8) or 448 (e4m3) units, 0 where all are zero;
  * codes are value / unit to the nearest, ties to even.  NaN counts as 0 and values beyond 2^126 as that (OMMX_ST_NONFINITE where one
  * is not finite).  A block that holds tokens and takes rows keeps the larger E of the two; codes it holds are rounded to that.
- * int8 -128 and e4m3's NaN are never written, and count as -128 and, in values that are attended to, 480 units where a caller writes them.
+ * int8 -128 and e4m3's NaN are never written; where a caller writes them they count as that.
  * weight (optional): float [num_pages][n_kv_heads][page_size], what each token was attended to with.
  *
  * A page that takes rows, weights or kept tokens belongs to one sequence.  Lengths, tables and row ranges are read on the device: nothing
@@ -563,7 +563,8 @@ typedef struct ommx_kv8_decode_args {
     int32_t max_seq_len;            /* an upper bound of b_seq_len that sizes the grid and the workspace, 0: what the table can hold.  Weights
                                        of sequences past it are not kept up (OMMX_ST_BAD_LENGTH) */
     float sm_scale, logit_cap;      /* logits: cap * tanh(q.k * sm_scale / cap); cap 0: none.  sm_scale: any finite number; the largest
-                                       |q| * |sm_scale| * 2^17 must be finite in 32 bits.  Logits are served up to 2^24 in size */
+                                       |q| * |sm_scale| must be finite in 32 bits.  Logits are served up to 2^24 in size; over int8 codes a query
+                                       row's channels count with 2^-22 of the largest.  A row that is not finite gives NaN */
     int32_t *status;
 } ommx_kv8_decode_args;
 
@@ -583,7 +584,7 @@ typedef struct ommx_kv8_evict_args {
     int32_t to_table_is_int64, to_pages_per_seq;
     int32_t *kept;                  /* out [batch, n_kv_heads, budget]: the places that were kept, ascending, then -1 */
     int32_t budget, sink_tokens, recent_tokens;
-    int32_t *len_out;               /* [batch]: min(b_seq_len, budget); may be b_seq_len, or NULL */
+    int32_t *len_out;               /* [batch]: min(b_seq_len, budget); b_seq_len itself, or apart from it, or NULL */
     int32_t max_seq_len;            /* an upper bound of b_seq_len that sizes the launch, 0: what the table can hold */
     int32_t *status;
 } ommx_kv8_evict_args;

@@ -172,8 +172,12 @@ template <int G, bool E4M3> __device__ __forceinline__ void make_query(const Dec
     }
 #pragma unroll
     for (int i = 0; i < 8 * G; ++i) top = fmaxf(top, fabsf(x[i]));
+    bool wild = false;                            // whole numbers hold neither NaN nor infinities: the head's logits are NaN then
+#pragma unroll
+    for (int i = 0; i < 8 * G; ++i) wild |= !(fabsf(x[i]) < INFINITY);
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+    wild = __ballot_sync(~0u, wild) >> (lane & ~3) & 15u;
     const int e = top > 0.0f ? max(exponent_of(top), -100) : 0;
     constexpr int BITS = E4M3 ? 13 : 21;          // the largest channel lies below 2^(BITS + 1)
     const float up = power_of_two(BITS - e);
@@ -200,12 +204,12 @@ template <int G, bool E4M3> __device__ __forceinline__ void make_query(const Dec
                 }
             }
         }
-    const float factor = p.sm_scale * power_of_two(-BITS) * power_of_two(e);
+    const float factor = wild ? NAN : p.sm_scale * power_of_two(-BITS) * power_of_two(e);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const float f = __shfl_sync(~0u, factor, 8 * t + 4 * i);
         q.raw[i] = p.cap > 0.0f ? f / p.cap : f;
-        q.factor[i] = p.cap > 0.0f ? p.cap * LOG2E : f * LOG2E;
+        q.factor[i] = p.cap > 0.0f ? p.cap * LOG2E : f * LOG2E;             // with a cap the NaN is in `raw`
     }
 }
 

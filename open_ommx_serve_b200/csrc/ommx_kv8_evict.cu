@@ -20,6 +20,7 @@ constexpr int THREADS = 1024, WARPS = THREADS / 32, BINS = 2048, MOST_CLUSTER = 
 constexpr int HELD = 8, TURN = THREADS * HELD;    // keys that a thread holds; a block's turn of keys, a warp has 32 HELD in a row of it
 constexpr int MOST_KEYS = 40 * 1024;              // further keys that a block holds in shared memory; it reads others again
 constexpr int FEW = 4096;                         // keys that each block of a cluster finishes for itself
+constexpr int MOST_TOKENS = 0x7FFF0000;           // places are counted in 32 bits, a turn of all blocks and more to spare
 constexpr int PLACES = 512;                       // that a block moves at a time
 
 struct EvictParams {
@@ -71,7 +72,7 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
     wait_earlier();
     let_next_in();
     const int given = p.s.len[b];
-    const int64_t room = (int64_t)p.s.max_pages << p.page_shift;
+    const int64_t room = min((int64_t)p.s.max_pages << p.page_shift, (int64_t)MOST_TOKENS);
     int faults = given < 0 || given > room ? OMMX_ST_BAD_LENGTH : 0;
     const int len = faults ? 0 : given, keep = min(len, p.budget);
     if (keep > (int64_t)p.to.max_pages << p.page_shift) faults |= OMMX_ST_BAD_LENGTH;
@@ -462,6 +463,8 @@ static int evict(const ommx_kv8_evict_args *a, cudaStream_t st) {
         if (int rc = read_seqs("kv8_evict", to, p.c, &p.to)) return rc;
     }
     const bool shortens = a->len_out == a->seqs.b_seq_len;
+    if (a->len_out && !shortens && a->len_out < a->seqs.b_seq_len + p.s.B && a->seqs.b_seq_len < a->len_out + p.s.B)
+        return fail(OMMX_E_ARG, "kv8_evict: len_out must be b_seq_len itself or apart from it");
     p.kept = a->kept; p.len_out = shortens ? nullptr : a->len_out;
     p.budget = a->budget; p.sinks = a->sink_tokens; p.recent = a->recent_tokens;
     p.page_shift = shift_of(p.c.page);

@@ -471,6 +471,57 @@ def test_channels_of_a_query_far_below_its_largest():
     check(q, cache, table.to(DEV), [L], o, lse, sm_scale=2.0 ** 20)
 
 
+@pytest.mark.parametrize("code", [I8, E4M3])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_queries_that_are_not_finite(code, bad, cap):
+    """The head whose row it is gives NaN; the others of its product hold to their bounds (their references move when its do)."""
+    for lens in ([40, 0, 700], [6000, 20, 3000]):
+        table, P = tables(lens, 16)
+        cache = to_gpu(random_cache(P, 2, 128, 16, code))
+        q = torch.randn(3, 12, 128, generator=torch.Generator().manual_seed(0)).bfloat16().to(DEV)
+        o, lse = torch.empty(2, 3, 12, 128, device=DEV), torch.empty(2, 3, 12, device=DEV)
+        for i in range(2):
+            given = q.clone()
+            if i:
+                given[0, 7, 3], given[2, 0, 127] = bad, bad
+            ommx_kv8_decode_attention(given, cache["codes"], cache["scales"], table.to(DEV), i32(lens), o[i], lse[i], logit_cap=cap)
+        hit = torch.zeros(3, 12, dtype=torch.bool, device=DEV)
+        hit[0, 7] = hit[2, 0] = True
+        assert bool(o[1][hit].isnan().all()) and bool(lse[1][hit].isnan().all())
+        check(q, cache, table.to(DEV), lens, torch.where(hit[..., None], o[0], o[1]), torch.where(hit, lse[0], lse[1]), cap=cap)
+
+
+@pytest.mark.parametrize("code,D,H,page", [(I8, 128, 8, 16), (E4M3, 64, 4, 64)])
+def test_offsets_past_32_bits(code, D, H, page):
+    """The same sequences at the front of a small cache and at the back of one of more than 2^32 bytes: append, read back, attend, evict."""
+    need = 12
+    big = 2 ** 32 // (H * page * 2 * D) + 2 * need
+    gen = torch.Generator().manual_seed(3)
+    lens = [5 * page - 3, 4 * page]
+    x, q = rows(sum(lens), H, D, BF16, gen).to(DEV), torch.randn(2, 4 * H, D, generator=gen).bfloat16().to(DEV)
+    got = []
+    for pages in (need, big):
+        c = ommx_kv8_alloc(pages, H, D, page_size=page, dtype=code, weight=True, device=DEV)
+        where = (c["codes"], c["scales"])
+        table = (torch.arange(need, device=DEV, dtype=I32).flip(0).view(2, 6) + (pages - need)).contiguous()
+        length, starts = i32(lens), i32(cumulated(lens))
+        ommx_kv8_append(x[:, :H], x[:, H:], *where, table, length, row_start=starts, weight=c["weight"])
+        o, lse, kept = torch.empty(2, 4 * H, D, device=DEV), torch.empty(2, 4 * H, device=DEV), torch.empty(2, H, 40, dtype=I32, device=DEV)
+        status = i32([0])
+        ommx_kv8_decode_attention(q, *where, table, length, o, lse, weight=c["weight"], keep=0.5, status=status)
+        weights = c["weight"][pages - need:].clone()
+        ommx_kv8_evict(*where, c["weight"], table, length, kept, sink_tokens=1, recent_tokens=3, len_out=length, status=status)
+        k, v = (torch.empty(80, H, D, device=DEV) for _ in range(2))
+        ommx_kv8_gather(*where, table, length, k, v, row_start=i32([0, 40, 80]), status=status)
+        assert int(status) == 0
+        got.append((o, lse, weights, kept, k, v, c["weight"][pages - need:].clone(), c["codes"].view(torch.uint8)[pages - need:].clone(), c["scales"][pages - need:].clone()))
+        assert pages == need or not bool(c["scales"][:need].any())         # what 32 bits would have reached
+        del c, where
+    for a, b in zip(*got):
+        assert same(a, b)
+
+
 def test_strides_alignment_and_padding():
     """q in slices of one projection and off 16-byte boundaries, outputs with gaps, lse rows apart; what lies between stays."""
     lens, page, H, Hq, D = [50, 0, 700], 16, 2, 6, 128

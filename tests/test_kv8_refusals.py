@@ -195,6 +195,14 @@ def test_the_c_entries_refuse_calls():
     assert lib.ommx_b200_kv8_evict(C.byref(e), None) == -1 and "weights" in _lib.last_error()
 
 
+def test_lengths_that_overlap_are_refused():
+    e = c_args(_lib.KV8EvictArgs)
+    e.kept, e.budget = 256, 5
+    for at in (256 + 4, 256 - 4 * (B - 1)):
+        e.len_out = at
+        assert _lib.load().ommx_b200_kv8_evict(C.byref(e), None) == -1 and "len_out" in _lib.last_error()
+
+
 def test_workspace_sizes():
     assert kv8_workspace_floats(4, 32, 128, 512) == 0
     whole = kv8_workspace_floats(1, 32, 128, 513)
