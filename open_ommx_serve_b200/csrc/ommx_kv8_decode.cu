@@ -159,7 +159,8 @@ template <int G> __device__ __forceinline__ void fetch_query(const DecodeParams 
 }
 template <int G, bool E4M3> __device__ __forceinline__ void make_query(const DecodeParams &p, const Raw<G> &raw, int lane, Query<G, E4M3> &q) {
     const int t = lane & 3;
-    float x[8 * G], top = 0.0f;
+    float x[8 * G];
+    uint32_t largest = 0;                         // magnitudes in the order of their bits, two at a time
 #pragma unroll
     for (int i = 0; i < G; ++i) {
         const uint32_t w[4] = {raw.v[i].x, raw.v[i].y, raw.v[i].z, raw.v[i].w};
@@ -168,16 +169,14 @@ template <int G, bool E4M3> __device__ __forceinline__ void make_query(const Dec
             const float2 f = p.q16 ? __half22float2(*reinterpret_cast<const __half2 *>(&w[j])) : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
             x[8 * i + 2 * j] = f.x;
             x[8 * i + 2 * j + 1] = f.y;
+            largest = __vmaxu2(largest, w[j] & 0x7FFF7FFFu);
         }
     }
-#pragma unroll
-    for (int i = 0; i < 8 * G; ++i) top = fmaxf(top, fabsf(x[i]));
-    bool wild = false;                            // whole numbers hold neither NaN nor infinities: the head's logits are NaN then
-#pragma unroll
-    for (int i = 0; i < 8 * G; ++i) wild |= !(fabsf(x[i]) < INFINITY);
-    top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-    wild = __ballot_sync(~0u, wild) >> (lane & ~3) & 15u;
+    largest = max(largest & 0xFFFFu, largest >> 16);
+    largest = max(largest, __shfl_xor_sync(~0u, largest, 1));
+    largest = max(largest, __shfl_xor_sync(~0u, largest, 2));
+    const float top = p.q16 ? __half2float(__ushort_as_half((uint16_t)largest)) : __uint_as_float(largest << 16);
+    const bool wild = !(top < INFINITY);          // whole numbers hold neither NaN nor infinities: the head's logits are NaN then
     const int e = top > 0.0f ? max(exponent_of(top), -100) : 0;
     constexpr int BITS = E4M3 ? 13 : 21;          // the largest channel lies below 2^(BITS + 1)
     const float up = power_of_two(BITS - e);
@@ -190,17 +189,14 @@ template <int G, bool E4M3> __device__ __forceinline__ void make_query(const Dec
                 q.frag[s][h][0] = half2_bits(f[0] * up, f[1] * up);
                 q.frag[s][h][1] = half2_bits(f[2] * up, f[3] * up);
             } else {
-                int r[4];
+                // a whole number and 128 in each of three bytes: what is over in a byte is a digit of -128 .. 127
+                uint32_t r[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) r[i] = __float2int_rn(f[i] * up);
+                for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(fmaf(f[i], up, BEGIN_VALUE)) - __float_as_uint(BEGIN_VALUE) + 0x808080u;
 #pragma unroll
-                for (int j = PIECES - 1; j >= 0; --j) {
-                    q.frag[s][j][h] = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        q.frag[s][j][h] |= ((uint32_t)r[i] & 255u) << (8 * i);
-                        r[i] = (r[i] + 128) >> 8;     // of what the last byte, -128 .. 127, leaves
-                    }
+                for (int j = 0; j < PIECES; ++j) {
+                    const uint32_t byte = PIECES - 1 - j, pick = byte | (byte + 4) << 4;
+                    q.frag[s][j][h] = __byte_perm(__byte_perm(r[0], r[1], pick), __byte_perm(r[2], r[3], pick), 0x5410) ^ 0x80808080u;
                 }
             }
         }
