@@ -17,7 +17,7 @@ namespace kv8 {
 using namespace kv;
 
 constexpr int THREADS = 1024, WARPS = THREADS / 32, BINS = 2048, MOST_CLUSTER = 8;
-constexpr int HELD = 8, TURN = THREADS * HELD;    // keys that a thread holds; a block's turn of keys, a warp has 32 HELD in a row of it
+constexpr int HELD = 8, TURN = THREADS * HELD;    // keys that a thread holds, of consecutive tokens of a page; a block's turn of keys
 constexpr int MOST_KEYS = 40 * 1024;              // further keys that a block holds in shared memory; it reads others again
 constexpr int FEW = 4096;                         // keys that each block of a cluster finishes for itself
 constexpr int MOST_TOKENS = 0x7FFF0000;           // places are counted in 32 bits, a turn of all blocks and more to spare
@@ -123,25 +123,29 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
             const int64_t page = page_id(p.s, b, i >> p.page_shift);
             return there(page) ? ordered(weight[row_of(p, page, head, i)]) : 0u;
         };
-        auto place = [&](int turn, int u) { return lo + turn * TURN + warp * (32 * HELD) + u * 32 + lane; };
+        auto place = [&](int turn, int u) { return lo + turn * TURN + tid * HELD + u; };      // `lo` is a multiple of 32
         const int turns = (hi - lo + TURN - 1) / TURN;
         uint32_t held[HELD];
         bool off = false;
         for (int turn = 0; turn < turns; ++turn) {
-            int64_t page[HELD];
-            float w[HELD];
+            const int i0 = place(turn, 0);
+            float4 w[HELD / 4];
 #pragma unroll
-            for (int u = 0; u < HELD; ++u) page[u] = place(turn, u) < hi ? page_id(p.s, b, place(turn, u) >> p.page_shift) : 0;
+            for (int u = 0; u < HELD / 4; ++u) w[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i0 < hi) {
+                const int64_t page = page_id(p.s, b, i0 >> p.page_shift);
+                off |= !there(page);
+                if (there(page)) {                // tokens behind the last one lie on its page too
 #pragma unroll
-            for (int u = 0; u < HELD; ++u) {
-                off |= !there(page[u]);
-                w[u] = place(turn, u) < hi && there(page[u]) ? weight[row_of(p, page[u], head, place(turn, u))] : 0.0f;
+                    for (int u = 0; u < HELD / 4; ++u) w[u] = *reinterpret_cast<const float4 *>(weight + row_of(p, page, head, i0) + 4 * u);
+                }
             }
 #pragma unroll
             for (int u = 0; u < HELD; ++u) {
+                const uint32_t k = ordered(u % 4 == 0 ? w[u / 4].x : u % 4 == 1 ? w[u / 4].y : u % 4 == 2 ? w[u / 4].z : w[u / 4].w);
                 const int i = place(turn, u) - lo - TURN;
-                if (turn == 0) held[u] = ordered(w[u]);
-                else if (i < hi - lo - TURN && i < p.keys) keys[i] = ordered(w[u]);
+                if (turn == 0) held[u] = k;
+                else if (i < hi - lo - TURN && i < p.keys) keys[i] = k;
             }
         }
         auto key_at = [&](int i) { return i - lo - TURN < p.keys ? keys[i - lo - TURN] : load(i); };      // behind the first turn
@@ -282,29 +286,25 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
         }
         leave(faults);
         if (faults) return;
-        // keys above `a`, and the first `want` equal to it, in order: by turns, warps and 32 at a time
-        uint32_t ms[HELD], es[HELD];
-        auto look = [&](int turn) {               // of a turn: which of each 32 are more, and the same
+        // keys above `a`, and the first `want` equal to it, in order: by turns and threads. Counts of both are summed in the halves of a word.
+        uint32_t ms, es;                          // of a thread's keys of a turn, a bit each
+        auto look = [&](int turn) {
+            ms = es = 0;
 #pragma unroll
             for (int u = 0; u < HELD; ++u) {
                 const int i = place(turn, u);
                 const uint32_t k = i >= hi ? 0u : turn == 0 ? held[u] : key_at(i);
                 const bool pinned = i < p.sinks || i >= len - p.recent;
-                ms[u] = __ballot_sync(~0u, i < hi && (pinned || k > a));
-                es[u] = __ballot_sync(~0u, i < hi && !pinned && k == a);
+                ms |= (uint32_t)(i < hi && (pinned || k > a)) << u;
+                es |= (uint32_t)(i < hi && !pinned && k == a) << u;
             }
-        };
-        auto sum = [&](const uint32_t (&bits)[HELD]) {
-            int c = 0;
-#pragma unroll
-            for (int u = 0; u < HELD; ++u) c += __popc(bits[u]);
-            return c;
+            return __popc(ms) | __popc(es) << 16;
         };
         int above = 0, equal = 0;
-        for (int turn = turns - 1; turn >= 0; --turn) {                     // the first turn's stay
-            look(turn);
-            above += sum(ms);
-            equal += sum(es);
+        for (int turn = turns - 1; turn >= 0; --turn) {                     // the first turn's bits stay
+            const int c = look(turn);
+            above += __reduce_add_sync(~0u, c & 0xFFFF);
+            equal += __reduce_add_sync(~0u, c >> 16);
         }
         if (lane == 0) { warp_sum[0][warp] = above; warp_sum[1][warp] = equal; }
         __syncthreads();
@@ -326,28 +326,26 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
         const int first_here = above_all + min(equal_all, want);
         if (tid == 0) first_place = first_here;
         for (int turn = 0; turn < turns; ++turn) {
-            if (turn > 0) look(turn);
+            const int c = turn > 0 ? look(turn) : __popc(ms) | __popc(es) << 16, scan = warp_inclusive_scan(c, lane);
             if (turns > 1) {
                 __syncthreads();                  // `warp_sum` is read
-                if (lane == 0) { warp_sum[0][warp] = sum(ms); warp_sum[1][warp] = sum(es); }
+                if (lane == 31) { warp_sum[0][warp] = scan & 0xFFFF; warp_sum[1][warp] = scan >> 16; }
                 __syncthreads();
             }
             const int m = warp_sum[0][lane], e = warp_sum[1][lane];
-            above = above_all + __reduce_add_sync(~0u, lane < warp ? m : 0);
-            equal = equal_all + __reduce_add_sync(~0u, lane < warp ? e : 0);
+            above = above_all + __reduce_add_sync(~0u, lane < warp ? m : 0) + ((scan - c) & 0xFFFF);
+            equal = equal_all + __reduce_add_sync(~0u, lane < warp ? e : 0) + ((scan - c) >> 16);
             above_all += __reduce_add_sync(~0u, m);
             equal_all += __reduce_add_sync(~0u, e);
-            const uint32_t below = (1u << lane) - 1;
 #pragma unroll
             for (int u = 0; u < HELD; ++u) {
-                const int at = above + __popc(ms[u] & below), eq = equal + __popc(es[u] & below);
-                if (ms[u] >> lane & 1 || (es[u] >> lane & 1 && eq < want)) {
-                    const int to = at + min(eq, want);
+                if (ms >> u & 1 || (es >> u & 1 && equal < want)) {
+                    const int to = above + min(equal, want);
                     if (short_row) list[to - first_here] = (uint16_t)(place(turn, u) - lo);
                     else out[to] = place(turn, u);
                 }
-                above += __popc(ms[u]);
-                equal += __popc(es[u]);
+                above += ms >> u & 1;
+                equal += es >> u & 1;
             }
         }
         __syncthreads();
