@@ -810,72 +810,101 @@ template <int G> __device__ __forceinline__ void combine_head(const DecodeParams
 }
 
 // ---- the account ----------------------------------------------------------------------------------
-// weight = keep * before + the sum of a kv head's query heads' weights, by a thread to a token: the logits are there. Heads are added in
-// order. PARTS: their references and sums are not, the block makes them of the parts; the kernel that also joins these would be one to wait
+// weight = keep * before + the sum of a kv head's query heads' weights, by a thread to four tokens of a record: the logits are there. Heads are added
+// in order. PARTS: their references and sums are not, the block makes them of the parts; the kernel that also joins these would be one to wait
 // for (64K tokens: 43.0 us with a kernel behind it, 42.6 beside it).
-constexpr int THREADS = 256, SHARED_HEADS = 64, EACH_TOKENS = 4, STRETCH = THREADS * EACH_TOKENS;
-template <int G, bool PARTS> __device__ __forceinline__ void weigh(const DecodeParams &p, int b, int head, int first) {
-    __shared__ float2 stats[SHARED_HEADS];
+constexpr int THREADS = 256, SHARED_HEADS = 64, QUAD = 4, STRETCH = THREADS * QUAD;
+// references and sums of `n` heads from h0 on, by all warps
+template <int G, bool PARTS> __device__ __forceinline__ void stats_of(const DecodeParams &p, int b, int head, int h0, int n, float2 (&stats)[SHARED_HEADS]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if constexpr (PARTS) {
+        for (int h = warp; h < n; h += THREADS / 32) {
+            const int row = head * p.col_blocks + (h0 + h) / COLS;
+            const Parts r = parts_of(p, b, row, lane);
+            float2 s = make_float2(LOWEST, 0.0f);
+            if (r.count == 1) s = p.stats[((int64_t)b * p.c.H + head) * p.group + h0 + h];
+            else if (r.count > 1) {
+                float top, sum;
+                meet<G>(p, r, (h0 + h) % COLS, lane, 32, top, sum);
+                s = make_float2(top, sum != 0.0f ? 1.0f / sum : 0.0f);
+            }
+            if (lane == 0) stats[h] = s;
+        }
+    } else {
+        for (int h = threadIdx.x; h < n; h += THREADS) stats[h] = p.stats[((int64_t)b * p.c.H + head) * p.group + h0 + h];
+    }
+    __syncthreads();
+}
+// Block `block` of `blocks` of a kv head's; it takes every blocks-th stretch, so that references and sums are made once where there are many.
+template <int G, bool PARTS> __device__ __forceinline__ void weigh(const DecodeParams &p, int b, int head, int block, int blocks) {
+    __shared__ float2 stats[SHARED_HEADS];
     wait_earlier();
     let_next_in();
     const int len = length_of(p, b);
-    if (first >= len) return;
+    if (block * STRETCH >= len) return;
     const Span span = span_of(p, len);
-    int64_t at[EACH_TOKENS];                      // of the token's weight, -1: not kept
-    const float *x[EACH_TOKENS];                  // its logits, or null
-    float before[EACH_TOKENS], add[EACH_TOKENS];
-#pragma unroll
-    for (int u = 0; u < EACH_TOKENS; ++u) {
-        const int t = first + u * THREADS + threadIdx.x, record = t >> 4, unit = record < span.head ? record : record - span.skip;
+    const bool few = p.group <= SHARED_HEADS;
+    if (few) stats_of<G, PARTS>(p, b, head, 0, p.group, stats);
+    const bool wide = p.group % 4 == 0;
+    for (int64_t first = (int64_t)block * STRETCH; first < len; first += (int64_t)blocks * STRETCH) {
+        const int t = (int)first + QUAD * threadIdx.x, record = t >> 4, unit = record < span.head ? record : record - span.skip;
         const int64_t page = t < len ? page_id(p.s, b, t >> p.page_shift) : -1;
-        at[u] = page >= 0 && page < p.c.num_pages ? (page * p.c.H + head) * p.c.page + (t & (p.c.page - 1)) : -1;      // not there: reported
-        x[u] = nullptr;
-        if (at[u] >= 0 && (visible(p, len, record) >> (t & 15) & 1)) {
-            if (unit < p.most_units) x[u] = p.logits + ((((int64_t)b * p.c.H + head) * p.most_units + unit) * 16 + (t & 15)) * p.group;
-            else at[u] = -1;                      // past max_seq_len: reported
-        }
-        add[u] = 0.0f;
-    }
-#pragma unroll
-    for (int u = 0; u < EACH_TOKENS; ++u) before[u] = at[u] >= 0 && p.keep != 0.0f ? p.before[at[u]] : 0.0f;
-    for (int h0 = 0; h0 < p.group; h0 += SHARED_HEADS) {
-        if (h0) __syncthreads();
-        const int n = min(SHARED_HEADS, p.group - h0);
-        if constexpr (PARTS) {
-            for (int h = warp; h < n; h += THREADS / 32) {
-                const int row = head * p.col_blocks + (h0 + h) / COLS;
-                const Parts r = parts_of(p, b, row, lane);
-                float2 s = make_float2(LOWEST, 0.0f);
-                if (r.count == 1) s = p.stats[((int64_t)b * p.c.H + head) * p.group + h0 + h];
-                else if (r.count > 1) {
-                    float top, sum;
-                    meet<G>(p, r, (h0 + h) % COLS, lane, 32, top, sum);
-                    s = make_float2(top, sum != 0.0f ? 1.0f / sum : 0.0f);
-                }
-                if (lane == 0) stats[h] = s;
+        const bool there = page >= 0 && page < p.c.num_pages;               // if not, it is reported
+        uint32_t seen = there ? visible(p, len, record) >> (t & 15) & 15u : 0u;
+        uint32_t kept = !there ? 0u : len - t >= QUAD ? 15u : (1u << (len - t)) - 1;
+        if (seen && unit >= p.most_units) { kept &= ~seen; seen = 0; }      // past max_seq_len: reported
+        const int64_t at = (page * p.c.H + head) * p.c.page + (t & (p.c.page - 1));
+        const float *x = p.logits + ((((int64_t)b * p.c.H + head) * p.most_units + unit) * 16 + (t & 15)) * p.group;
+        float4 before = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (kept && p.keep != 0.0f) before = *reinterpret_cast<const float4 *>(p.before + at);
+        float add[QUAD] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int h0 = 0; h0 < p.group; h0 += SHARED_HEADS) {
+            const int n = min(SHARED_HEADS, p.group - h0);
+            if (!few) {
+                __syncthreads();
+                stats_of<G, PARTS>(p, b, head, h0, n, stats);
             }
-        } else {
-            for (int h = threadIdx.x; h < n; h += THREADS) stats[h] = p.stats[((int64_t)b * p.c.H + head) * p.group + h0 + h];
-        }
-        __syncthreads();
-        for (int h = 0; h < n; ++h) {
-            const float2 s = stats[h];
-            if (s.y == 0.0f) continue;            // no shares were dealt out
+            if (wide) {
+                for (int h = 0; h < n; h += 4) {
+                    float4 v[QUAD];
 #pragma unroll
-            for (int u = 0; u < EACH_TOKENS; ++u)
-                if (x[u]) add[u] = fmaf(exp2_approx(x[u][h0 + h] - s.x), s.y, add[u]);
+                    for (int u = 0; u < QUAD; ++u)
+                        if (seen >> u & 1) v[u] = *reinterpret_cast<const float4 *>(x + u * p.group + h0 + h);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 s = stats[h + j];
+                        if (s.y == 0.0f) continue;                          // no shares were dealt out
+#pragma unroll
+                        for (int u = 0; u < QUAD; ++u)
+                            if (seen >> u & 1) add[u] = fmaf(exp2_approx(reinterpret_cast<const float *>(&v[u])[j] - s.x), s.y, add[u]);
+                    }
+                }
+            } else {
+                for (int h = 0; h < n; ++h) {
+                    const float2 s = stats[h];
+                    if (s.y == 0.0f) continue;
+#pragma unroll
+                    for (int u = 0; u < QUAD; ++u)
+                        if (seen >> u & 1) add[u] = fmaf(exp2_approx(x[u * p.group + h0 + h] - s.x), s.y, add[u]);
+                }
+            }
+        }
+        const float4 now = p.keep != 0.0f ? make_float4(fmaf(p.keep, before.x, add[0]), fmaf(p.keep, before.y, add[1]), fmaf(p.keep, before.z, add[2]), fmaf(p.keep, before.w, add[3]))
+                                          : make_float4(add[0], add[1], add[2], add[3]);
+        if (kept == 15u) {
+            *reinterpret_cast<float4 *>(p.c.weight + at) = now;
+        } else {
+#pragma unroll
+            for (int u = 0; u < QUAD; ++u)
+                if (kept >> u & 1) p.c.weight[at + u] = reinterpret_cast<const float *>(&now)[u];
         }
     }
-#pragma unroll
-    for (int u = 0; u < EACH_TOKENS; ++u)
-        if (at[u] >= 0) p.c.weight[at[u]] = (p.keep != 0.0f ? p.keep * before[u] : 0.0f) + add[u];
 }
 
 // Behind the first kernel: what joins the parts (BY: nothing, a block to a row, a block to a head), and the account's blocks.
 // Grid: (joining blocks of a sequence + blocks of tokens x H, sequences).
 enum { NONE, ROW, HEAD_BLOCKS };
-template <int G, int BY> __global__ void __launch_bounds__(THREADS) kv8_second_kernel(const __grid_constant__ DecodeParams p, int joining) {
+template <int G, int BY> __global__ void __launch_bounds__(THREADS, 4) kv8_second_kernel(const __grid_constant__ DecodeParams p, int joining) {
     static_assert(THREADS == 32 * COLS && THREADS == 32 * CW, "one size of blocks");
     const int b = blockIdx.y, i = blockIdx.x;
     if (i < joining) {
@@ -884,7 +913,7 @@ template <int G, int BY> __global__ void __launch_bounds__(THREADS) kv8_second_k
         return;
     }
     const int blocks = (gridDim.x - joining) / p.c.H, at = i - joining, head = at / blocks;
-    weigh<G, BY != NONE>(p, b, head, (at - head * blocks) * STRETCH);
+    weigh<G, BY != NONE>(p, b, head, at - head * blocks, blocks);
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -924,7 +953,10 @@ template <int G, bool E4M3, bool FINE, int NW, bool CLUSTER> static int launch_d
     }
     if (int rc = launch_dependent(kv8_decode_kernel<G, E4M3, FINE, NW, CLUSTER>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G, NW>), st, cluster, p)) return rc;
     // a row has some blocks / rows parts
-    const int rows = p.c.H * p.col_blocks, account = tokens ? (int)((tokens + STRETCH - 1) / STRETCH) * p.c.H : 0;
+    const int rows = p.c.H * p.col_blocks;
+    // the account's blocks: about as many as the SMs hold (8 x 64K tokens: a block to each stretch 242 us in all, so XXX)
+    const int64_t heads = (int64_t)p.c.H * p.s.B, stretches = (tokens + STRETCH - 1) / STRETCH, fill = (4LL * sm_count() + heads - 1) / heads;
+    const int account = (int)(stretches < fill ? stretches : fill) * p.c.H;
     if (p.whole || CLUSTER) {
         if (!account) return 0;
         return launch_dependent(kv8_second_kernel<G, NONE>, dim3(account, p.s.B), THREADS, 0, st, 1, p, 0);
@@ -947,6 +979,7 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     if (!std::isfinite(a->sm_scale)) return fail(OMMX_E_ARG, "kv8_decode: sm_scale must be finite");
     if (a->window < 0 || a->sink_tokens < 0 || a->max_seq_len < 0) return fail(OMMX_E_ARG, "kv8_decode: window, sink_tokens and max_seq_len must not be negative");
     if (a->cache.weight && (!std::isfinite(a->keep) || (a->keep != 0.0f && !a->weight_before))) return fail(OMMX_E_ARG, "kv8_decode: keep must be finite, and what is kept must be given");
+    if (reinterpret_cast<uintptr_t>(a->weight_before) % 16) return fail(OMMX_E_ARG, "kv8_decode: weight_before must be 16-byte aligned");
     if (p.s.B > 65535) return fail(OMMX_E_UNSUPPORTED, "kv8_decode: a batch of %d", p.s.B);
     if (p.s.B == 0) return 0;
     if (!a->q || !a->o || !a->lse) return fail(OMMX_E_ARG, "kv8_decode: q, o and lse must not be null");
@@ -988,7 +1021,6 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     if (p.whole) cluster = 1;
     const int64_t blocks = p.whole ? rows : cluster > 1 ? cluster * rows : most < 1 ? 1 : most < hold ? most : hold;
     const int64_t tokens = p.c.weight ? most_tokens(a) : 0;                 // that weights are kept of
-    if ((tokens / STRETCH + 1) * p.c.H >= 1LL << 30) return fail(OMMX_E_UNSUPPORTED, "kv8_decode: weights of %lld tokens of %d kv heads: give max_seq_len", (long long)tokens, p.c.H);
     auto launch = [&](auto g, auto e4m3, auto fine) {
         constexpr int G = decltype(g)::value;
         constexpr bool E4M3 = decltype(e4m3)::value, FINE = decltype(fine)::value;

@@ -178,7 +178,7 @@ def test_the_c_entries_refuse_calls():
 
     for change, rc, text in ((dict(q_dtype=_lib.OMMX_DT_F32), -2, "q must"), (dict(o_dtype=7), -1, "o dtype"), (dict(n_q_heads=3), -2, "multiple"), (dict(logit_cap=-1.0), -1, "logit_cap"),
                              (dict(sm_scale=INF), -1, "sm_scale"), (dict(window=-1), -1, "window"), (dict(sink_tokens=-1), -1, "sink_tokens"), (dict(keep=NAN), -1, "keep"),
-                             (dict(weight_before=None), -1, "kept must be given"), (dict(lse=None), -1, "null"), (dict(workspace_floats=4), -1, "workspace"), (dict(workspace=260), -1, "workspace")):
+                             (dict(weight_before=None), -1, "kept must be given"), (dict(weight_before=260), -1, "aligned"), (dict(lse=None), -1, "null"), (dict(workspace_floats=4), -1, "workspace"), (dict(workspace=260), -1, "workspace")):
         assert decode_with(**change) == rc and text in _lib.last_error(), change
 
     def evict_with(**change):
