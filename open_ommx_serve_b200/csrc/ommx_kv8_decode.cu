@@ -811,8 +811,7 @@ template <int G> __device__ __forceinline__ void combine_head(const DecodeParams
 
 // ---- the account ----------------------------------------------------------------------------------
 // weight = keep * before + the sum of a kv head's query heads' weights, by a thread to four tokens of a record: the logits are there. Heads are added
-// in order. PARTS: their references and sums are not, the block makes them of the parts; the kernel that also joins these would be one to wait
-// for (64K tokens: 43.0 us with a kernel behind it, 42.6 beside it).
+// in order. PARTS: their references and sums are not, and the block makes them of the parts.
 constexpr int THREADS = 256, SHARED_HEADS = 64, QUAD = 4, STRETCH = THREADS * QUAD;
 // references and sums of `n` heads from h0 on, by all warps
 template <int G, bool PARTS> __device__ __forceinline__ void stats_of(const DecodeParams &p, int b, int head, int h0, int n, float2 (&stats)[SHARED_HEADS]) {
@@ -837,18 +836,25 @@ template <int G, bool PARTS> __device__ __forceinline__ void stats_of(const Deco
 }
 // Block `block` of `blocks` of a kv head's; it takes every blocks-th stretch, so that references and sums are made once where there are many.
 template <int G, bool PARTS> __device__ __forceinline__ void weigh(const DecodeParams &p, int b, int head, int block, int blocks) {
-    __shared__ float2 stats[SHARED_HEADS];
+    __shared__ __align__(16) float2 stats[SHARED_HEADS];
     wait_earlier();
     let_next_in();
     const int len = length_of(p, b);
-    if (block * STRETCH >= len) return;
+    if ((int64_t)block * STRETCH >= len) return;
+    if (PARTS && reinterpret_cast<const uint2 *>(p.work)->y == OVER) return;                 // no shares were dealt out: reported
     const Span span = span_of(p, len);
-    const bool few = p.group <= SHARED_HEADS;
+    const bool few = p.group <= SHARED_HEADS, wide = p.group % 4 == 0;
+    const int64_t step = (int64_t)blocks * STRETCH;
+    auto page_of = [&](int64_t first) -> int64_t {
+        const int64_t t = first + QUAD * threadIdx.x;
+        return t < len ? page_id(p.s, b, (int)(t >> p.page_shift)) : -1;
+    };
+    int64_t next_page = page_of((int64_t)block * STRETCH);                  // of the stretch to come, on its way
     if (few) stats_of<G, PARTS>(p, b, head, 0, p.group, stats);
-    const bool wide = p.group % 4 == 0;
-    for (int64_t first = (int64_t)block * STRETCH; first < len; first += (int64_t)blocks * STRETCH) {
+    for (int64_t first = (int64_t)block * STRETCH; first < len; first += step) {
         const int t = (int)first + QUAD * threadIdx.x, record = t >> 4, unit = record < span.head ? record : record - span.skip;
-        const int64_t page = t < len ? page_id(p.s, b, t >> p.page_shift) : -1;
+        const int64_t page = next_page;
+        next_page = page_of(first + step);
         const bool there = page >= 0 && page < p.c.num_pages;               // if not, it is reported
         uint32_t seen = there ? visible(p, len, record) >> (t & 15) & 15u : 0u;
         uint32_t kept = !there ? 0u : len - t >= QUAD ? 15u : (1u << (len - t)) - 1;
@@ -858,6 +864,9 @@ template <int G, bool PARTS> __device__ __forceinline__ void weigh(const DecodeP
         float4 before = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (kept && p.keep != 0.0f) before = *reinterpret_cast<const float4 *>(p.before + at);
         float add[QUAD] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float *from[QUAD];                  // what is not seen is read from where there is something
+#pragma unroll
+        for (int u = 0; u < QUAD; ++u) from[u] = seen >> u & 1 ? x + u * p.group : p.logits;
         for (int h0 = 0; h0 < p.group; h0 += SHARED_HEADS) {
             const int n = min(SHARED_HEADS, p.group - h0);
             if (!few) {
@@ -868,27 +877,26 @@ template <int G, bool PARTS> __device__ __forceinline__ void weigh(const DecodeP
                 for (int h = 0; h < n; h += 4) {
                     float4 v[QUAD];
 #pragma unroll
-                    for (int u = 0; u < QUAD; ++u)
-                        if (seen >> u & 1) v[u] = *reinterpret_cast<const float4 *>(x + u * p.group + h0 + h);
+                    for (int u = 0; u < QUAD; ++u) v[u] = *reinterpret_cast<const float4 *>(from[u] + h0 + h);
+                    const float4 s01 = *reinterpret_cast<const float4 *>(&stats[h]), s23 = *reinterpret_cast<const float4 *>(&stats[h + 2]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 s = stats[h + j];
-                        if (s.y == 0.0f) continue;                          // no shares were dealt out
-#pragma unroll
-                        for (int u = 0; u < QUAD; ++u)
-                            if (seen >> u & 1) add[u] = fmaf(exp2_approx(reinterpret_cast<const float *>(&v[u])[j] - s.x), s.y, add[u]);
+                    for (int u = 0; u < QUAD; ++u) {
+                        add[u] = fmaf(exp2_approx(v[u].x - s01.x), s01.y, add[u]);
+                        add[u] = fmaf(exp2_approx(v[u].y - s01.z), s01.w, add[u]);
+                        add[u] = fmaf(exp2_approx(v[u].z - s23.x), s23.y, add[u]);
+                        add[u] = fmaf(exp2_approx(v[u].w - s23.z), s23.w, add[u]);
                     }
                 }
             } else {
                 for (int h = 0; h < n; ++h) {
                     const float2 s = stats[h];
-                    if (s.y == 0.0f) continue;
 #pragma unroll
-                    for (int u = 0; u < QUAD; ++u)
-                        if (seen >> u & 1) add[u] = fmaf(exp2_approx(x[u * p.group + h0 + h] - s.x), s.y, add[u]);
+                    for (int u = 0; u < QUAD; ++u) add[u] = fmaf(exp2_approx(from[u][h0 + h] - s.x), s.y, add[u]);
                 }
             }
         }
+#pragma unroll
+        for (int u = 0; u < QUAD; ++u) add[u] = seen >> u & 1 ? add[u] : 0.0f;
         const float4 now = p.keep != 0.0f ? make_float4(fmaf(p.keep, before.x, add[0]), fmaf(p.keep, before.y, add[1]), fmaf(p.keep, before.z, add[2]), fmaf(p.keep, before.w, add[3]))
                                           : make_float4(add[0], add[1], add[2], add[3]);
         if (kept == 15u) {
@@ -896,7 +904,7 @@ template <int G, bool PARTS> __device__ __forceinline__ void weigh(const DecodeP
         } else {
 #pragma unroll
             for (int u = 0; u < QUAD; ++u)
-                if (kept >> u & 1) p.c.weight[at + u] = reinterpret_cast<const float *>(&now)[u];
+                if (kept >> u & 1) p.c.weight[at + u] = u == 0 ? now.x : u == 1 ? now.y : u == 2 ? now.z : now.w;
         }
     }
 }
@@ -904,7 +912,7 @@ template <int G, bool PARTS> __device__ __forceinline__ void weigh(const DecodeP
 // Behind the first kernel: what joins the parts (BY: nothing, a block to a row, a block to a head), and the account's blocks.
 // Grid: (joining blocks of a sequence + blocks of tokens x H, sequences).
 enum { NONE, ROW, HEAD_BLOCKS };
-template <int G, int BY> __global__ void __launch_bounds__(THREADS, 4) kv8_second_kernel(const __grid_constant__ DecodeParams p, int joining) {
+template <int G, int BY> __global__ void __launch_bounds__(THREADS, BY == NONE ? 6 : 4) kv8_second_kernel(const __grid_constant__ DecodeParams p, int joining) {
     static_assert(THREADS == 32 * COLS && THREADS == 32 * CW, "one size of blocks");
     const int b = blockIdx.y, i = blockIdx.x;
     if (i < joining) {
@@ -954,15 +962,22 @@ template <int G, bool E4M3, bool FINE, int NW, bool CLUSTER> static int launch_d
     if (int rc = launch_dependent(kv8_decode_kernel<G, E4M3, FINE, NW, CLUSTER>, dim3((unsigned)blocks), 32 * NW, sizeof(Memory<G, NW>), st, cluster, p)) return rc;
     // a row has some blocks / rows parts
     const int rows = p.c.H * p.col_blocks;
-    // the account's blocks: about as many as the SMs hold (8 x 64K tokens: a block to each stretch 242 us in all, so XXX)
-    const int64_t heads = (int64_t)p.c.H * p.s.B, stretches = (tokens + STRETCH - 1) / STRETCH, fill = (4LL * sm_count() + heads - 1) / heads;
+    // The account's blocks: at most as many as the SMs hold. Where there are stretches for no more than that they stand beside those that join the
+    // parts, and make references and sums themselves; else they come behind them (8 x 64K tokens: 234 us beside, 215 behind; one of 64K 41.4 and 43.0).
+    const int64_t heads = (int64_t)p.c.H * p.s.B, stretches = (tokens + STRETCH - 1) / STRETCH;
+    const bool joins = !p.whole && !CLUSTER, beside = joins && stretches * heads <= 4LL * sm_count();
+    const int64_t fill = (6LL * sm_count() + heads - 1) / heads;
     const int account = (int)(stretches < fill ? stretches : fill) * p.c.H;
-    if (p.whole || CLUSTER) {
-        if (!account) return 0;
-        return launch_dependent(kv8_second_kernel<G, NONE>, dim3(account, p.s.B), THREADS, 0, st, 1, p, 0);
+    if (joins) {
+        const bool by_row = (int64_t)rows * p.s.B * COLS >= blocks;
+        const int joining = by_row ? rows : rows * COLS;
+        const dim3 grid(joining + (beside ? account : 0), p.s.B);
+        const int rc = by_row ? launch_dependent(kv8_second_kernel<G, ROW>, grid, THREADS, 0, st, 1, p, joining)
+                              : launch_dependent(kv8_second_kernel<G, HEAD_BLOCKS>, grid, THREADS, 0, st, 1, p, joining);
+        if (rc) return rc;
     }
-    if ((int64_t)rows * p.s.B * COLS >= blocks) return launch_dependent(kv8_second_kernel<G, ROW>, dim3(rows + account, p.s.B), THREADS, 0, st, 1, p, rows);
-    return launch_dependent(kv8_second_kernel<G, HEAD_BLOCKS>, dim3(rows * COLS + account, p.s.B), THREADS, 0, st, 1, p, rows * COLS);
+    if (beside || !account) return 0;
+    return launch_dependent(kv8_second_kernel<G, NONE>, dim3(account, p.s.B), THREADS, 0, st, 1, p, 0);
 }
 
 static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
