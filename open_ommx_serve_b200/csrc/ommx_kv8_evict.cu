@@ -3,9 +3,9 @@
 // Of a sequence of more than `budget` tokens each kv head keeps the first `sinks`, the last `recent` and, of those between, the ones of the
 // largest weight (ties to the lowest place), and they move to the places 0 .. budget - 1 in their order. A cluster of blocks to a row
 // (sequence, kv head):
-// * picks: the weights' order is that of whole numbers, of which the want-th largest is found by counting: what lies between the smallest
-//   and the largest is cut into 2048 equal parts, and the part that holds it again, until so few are left that each block takes all of them
-//   and goes on alone. A thread holds its first keys in registers; counts meet in distributed shared memory.
+// * picks: the weights' order is that of whole numbers, of which the want-th largest is found by counting: those above 0 (all, where it is none of
+//   these) are cut into 2048 equal parts, and the part that holds it again, until so few are left that each block takes all of them and goes on
+//   alone. A thread holds its first keys in registers; counts meet in distributed shared memory.
 // * moves: places ascend, and a token never moves up. So once a cluster has read all that a stretch of places takes into its shared
 //   memory it can write that stretch where the tokens lie, and go on to the next.
 #include "ommx_kv8.cuh"
@@ -16,12 +16,17 @@ namespace kv8 {
 
 using namespace kv;
 
-constexpr int THREADS = 1024, WARPS = THREADS / 32, BINS = 2048, MOST_CLUSTER = 8;
-constexpr int HELD = 8, TURN = THREADS * HELD;    // keys that a thread holds, of consecutive tokens of a page; a block's turn of keys
-constexpr int MOST_KEYS = 40 * 1024;              // further keys that a block holds in shared memory; it reads others again
+// Blocks of 1024 threads, one to an SM, or, where there are more rows than SMs, of 512, two to an SM, which fill each other's
+// waits (64 sequences of 4608 to 4096 tokens, 8 kv heads: 259 us with one size, 228 so).
+constexpr int BINS = 2048, MOST_CLUSTER = 8;
+constexpr int HELD = 8;                           // keys that a thread holds, of consecutive tokens of a page; TURN: a block's turn of keys
 constexpr int FEW = 4096;                         // keys that each block of a cluster finishes for itself
+template <int THREADS> struct Sizes {
+    static constexpr int TURN = THREADS * HELD;
+    static constexpr int PLACES = THREADS / 2;    // that a block moves at a time
+    static constexpr int MOST_KEYS = 40 * THREADS;                          // further keys that a block holds in shared memory; it reads others again
+};
 constexpr int MOST_TOKENS = 0x7FFF0000;           // places are counted in 32 bits, a turn of all blocks and more to spare
-constexpr int PLACES = 512;                       // that a block moves at a time
 
 struct EvictParams {
     Cache c;
@@ -55,20 +60,26 @@ __device__ __forceinline__ int peer_half(const uint16_t *at, uint32_t rank) {
 }
 
 // Grid: (cluster x H, B).
-template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict_kernel(const __grid_constant__ EvictParams p) {
-    constexpr int D = 32 * G;
+template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv8_evict_kernel(const __grid_constant__ EvictParams p) {
+    constexpr int D = 32 * G, TURN = Sizes<THREADS>::TURN, PLACES = Sizes<THREADS>::PLACES;
+    constexpr int EACH = BINS / THREADS;          // bins of a thread
     extern __shared__ __align__(16) uint8_t memory[];                       // keys, then rows
     uint32_t *keys = reinterpret_cast<uint32_t *>(memory);
     __shared__ __align__(16) int histogram[BINS];
     __shared__ uint32_t few[FEW];
     __shared__ Place places[PLACES];
-    __shared__ int warp_sum[2][WARPS], starts[MOST_CLUSTER + 1], bin, left, inside, listed, more, same, above_here, equal_here, first_place, bad, spoilt;
+    __shared__ int warp_sum[2][32], starts[MOST_CLUSTER + 1], bin, left, inside, listed, more, same, above_here, equal_here, first_place, bad, spoilt;
     __shared__ int firsts[MOST_CLUSTER];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t n = cluster_size(), rank = cluster_rank();
     const int head = blockIdx.x / n, b = blockIdx.y;
     if (tid == 0) bad = listed = more = 0;
-    histogram[tid] = histogram[tid + THREADS] = 0;
+    if (tid < 64) warp_sum[tid / 32][tid % 32] = 0;                         // of warps that there are not
+    auto clear = [&] {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) histogram[tid + i * THREADS] = 0;
+    };
+    clear();
     wait_earlier();
     let_next_in();
     const int given = p.s.len[b];
@@ -205,7 +216,7 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
             }
             cluster_barrier();                    // all peers have read
             if (!begun && spoilt) { faults = OMMX_ST_BAD_PAGE; break; }
-            histogram[tid] = histogram[tid + THREADS] = 0;
+            clear();
             if (wanted == 0) { a = ~0u; break; }
             if (!begun && bin == 0) { a = 0; width = 32; }                  // `want` as it was
             else { a += (uint32_t)bin << shift; want = left; width = shift; }
@@ -247,17 +258,23 @@ template <int G, bool E4M3> __global__ void __launch_bounds__(THREADS) kv8_evict
                     for (int j = 0; j < FEW / THREADS; ++j)
                         if (tid + j * THREADS < count && k[j] >> width == 0) atomicAdd(&histogram[k[j] >> cut], 1);
                     __syncthreads();
-                    const int upper = histogram[BINS - 1 - 2 * tid], lower = histogram[BINS - 2 - 2 * tid];
-                    int over = warp_inclusive_scan(upper + lower, lane);
+                    // from the top: thread t has bins BINS - 1 - EACH t and those below
+                    int mine[EACH], all_mine = 0;
+#pragma unroll
+                    for (int j = 0; j < EACH; ++j) { mine[j] = histogram[BINS - 1 - EACH * tid - j]; all_mine += mine[j]; }
+                    int over = warp_inclusive_scan(all_mine, lane);
                     if (lane == 31) warp_sum[0][warp] = over;
                     __syncthreads();
-                    over += __reduce_add_sync(~0u, lane < warp ? warp_sum[0][lane] : 0) - upper - lower;
-                    if (over < want && over + upper + lower >= want) {
-                        const bool up = over + upper >= want;
-                        left = want - over - (up ? 0 : upper);
-                        bin = BINS - (up ? 1 : 2) - 2 * tid;
+                    over += __reduce_add_sync(~0u, lane < warp ? warp_sum[0][lane] : 0) - all_mine;
+                    if (over < want && over + all_mine >= want) {
+                        bool found = false;
+#pragma unroll
+                        for (int j = 0; j < EACH; ++j) {
+                            if (!found && over + mine[j] >= want) { found = true; left = want - over; bin = BINS - 1 - EACH * tid - j; }
+                            over += mine[j];
+                        }
                     }
-                    histogram[tid] = histogram[tid + THREADS] = 0;
+                    clear();
                     __syncthreads();
                     const uint32_t from = (uint32_t)bin << cut;
 #pragma unroll
@@ -426,16 +443,20 @@ __global__ void kv8_shorten_kernel(const __grid_constant__ EvictParams p, int32_
 }
 
 // ---- host ---------------------------------------------------------------------------------------
-template <int G, bool E4M3> static int launch_evict(const EvictParams &p, int cluster, cudaStream_t st) {
+template <int G, bool E4M3, int THREADS> static int launch_evict(EvictParams p, int64_t tokens, int cluster, cudaStream_t st) {
+    using S = Sizes<THREADS>;
     static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may take its shared memory
     int dev = 0;
     if (int rc = current_device(&dev)) return rc;
     if (!(allowed.load(std::memory_order_acquire) >> dev & 1)) {
-        OMMX_CUDA_TRY(cudaFuncSetAttribute(kv8_evict_kernel<G, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * MOST_KEYS));
+        OMMX_CUDA_TRY(cudaFuncSetAttribute(kv8_evict_kernel<G, E4M3, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * S::MOST_KEYS));
         allowed.fetch_or(1ull << dev, std::memory_order_release);
     }
-    const size_t keys = 4 * (size_t)p.keys, rows = (size_t)PLACES * 64 * G + 2 * TURN;                 // rows and a list
-    return launch_dependent(kv8_evict_kernel<G, E4M3>, dim3(cluster * p.c.H, p.s.B), THREADS, keys > rows ? keys : rows, st, cluster, p);
+    const int64_t share = (tokens + cluster - 1) / cluster + 32;
+    p.keys = (int)(share <= S::TURN ? 0 : share - S::TURN < S::MOST_KEYS ? share - S::TURN : S::MOST_KEYS);
+    const size_t keys = 4 * (size_t)p.keys, rows = (size_t)S::PLACES * 64 * G + 2 * S::TURN;                 // rows and a list
+    static_assert(S::PLACES * 64 * G + 2 * S::TURN <= 4 * S::MOST_KEYS, "the limit that is asked for");
+    return launch_dependent(kv8_evict_kernel<G, E4M3, THREADS>, dim3(cluster * p.c.H, p.s.B), THREADS, keys > rows ? keys : rows, st, cluster, p);
 }
 
 static int evict(const ommx_kv8_evict_args *a, cudaStream_t st) {
@@ -473,9 +494,11 @@ static int evict(const ommx_kv8_evict_args *a, cudaStream_t st) {
     const int64_t rows = (int64_t)p.s.B * p.c.H;
     int cluster = 1;
     while (cluster < MOST_CLUSTER && 2 * cluster * rows <= sm_count() && tokens >= 2048LL * cluster) cluster *= 2;
-    const int64_t share = (tokens + cluster - 1) / cluster + 32;
-    p.keys = (int)(share <= TURN ? 0 : share - TURN < MOST_KEYS ? share - TURN : MOST_KEYS);
-    auto launch = [&](auto g, auto e4m3) { return launch_evict<decltype(g)::value, decltype(e4m3)::value>(p, cluster, st); };
+    auto launch = [&](auto g, auto e4m3) {
+        constexpr int G = decltype(g)::value;
+        constexpr bool E4M3 = decltype(e4m3)::value;
+        return rows > sm_count() ? launch_evict<G, E4M3, 512>(p, tokens, cluster, st) : launch_evict<G, E4M3, 1024>(p, tokens, cluster, st);
+    };
     using std::integral_constant;
     int rc;
     if (a->cache.code == OMMX_KV8_E4M3)

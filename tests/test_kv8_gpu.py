@@ -705,10 +705,20 @@ def test_eviction_of_long_rows_of_like_weights(kind):
         evict([20000, 60, 9000], 1, 64, 16, E4M3, 2500, 4, 30, weights=fill, max_len=max_len)
 
 
-def test_eviction_where_keys_do_not_fit():
-    """Many rows, so that one block has a row of more keys than it holds."""
+@pytest.mark.parametrize("H", [1, 2])
+def test_eviction_where_keys_do_not_fit(H):
+    """Many rows, so that one block, of either size, has a row of more keys than it holds."""
     lens = [50000] + [30] * 80
-    evict(lens, 1, 64, 256, I8, 64, 2, 8)
+    evict(lens, H, 64, 256, I8, 64, 2, 8)
+
+
+@pytest.mark.parametrize("code,D", [(I8, 128), (E4M3, 64)])
+def test_eviction_of_many_rows(code, D):
+    """More rows than SMs: blocks of half the size."""
+    lens = [700, 3, 0, 5000, 333] + [90 + 7 * i for i in range(50)]
+    for apart in (False, True):
+        evict(lens, 3, D, 32, code, 300, 4, 60, apart=apart)
+    evict(lens, 3, D, 32, code, 64, 0, 0, weights=lambda w: w.copy_((torch.rand(w.shape, generator=torch.Generator().manual_seed(1)) * 2).floor()), alias=True)
 
 
 def test_sequences_with_pages_out_of_range_are_not_evicted_from():
