@@ -69,7 +69,7 @@ __device__ __forceinline__ Span span_of(const DecodeParams &p, int len) {
     Span s = {all, 0, 0};
     if (p.window && len > p.window) {
         const int tail = (len - p.window) >> 4;
-        s.head = min((p.sinks + 15) >> 4, tail);
+        s.head = min((int)(((uint32_t)p.sinks + 15) >> 4), tail);
         s.skip = tail - s.head;
         s.units = all - s.skip;
     }

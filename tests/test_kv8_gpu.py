@@ -365,6 +365,28 @@ def test_window_and_first_tokens(window, sinks, code):
     attend([5000, 4999], 1, 8, 128, 32, code, F16, window=window, sink_tokens=sinks, weigh=True, keep=0.0, max_len=None)
 
 
+@pytest.mark.parametrize("code,D", [(I8, 128), (E4M3, 64)])
+def test_first_tokens_and_lengths_near_the_end_of_32_bits(code, D):
+    """More first tokens than any sequence has beside a window; and a sequence of up to 2^31 - 2^10 tokens, as many as are
+    counted, whose table names four pages over and over, through a window."""
+    attend([1, 16, 40, 611, 0, 3000], 2, 4, D, 16, code, window=30, sink_tokens=2 ** 31 - 1, weigh=True, keep=0.5)
+    page, H, Hq, sinks, window = 256, 2, 8, 20, 1000
+    cache = to_gpu(random_cache(4, H, D, page, code))
+    table = (torch.arange(2 ** 31 // page, dtype=I32, device=DEV) % 4).view(1, -1)
+    k, v = ref.sequence(cache["codes"], cache["scales"], torch.arange(4), 4 * page)
+    q = torch.randn(1, Hq, D, device=DEV).bfloat16()
+    for length in (2 ** 31 - 2 ** 10 - x for x in (0, 1, 15, 16, 17)):
+        o, lse, status = torch.empty(1, Hq, D, device=DEV), torch.empty(1, Hq, device=DEV), i32([0])
+        ommx_kv8_decode_attention(q, cache["codes"], cache["scales"], table, i32([length]), o, lse, window=window, sink_tokens=sinks, status=status)
+        assert int(status) == 0
+        at = torch.tensor(list(range(sinks)) + [t % (4 * page) for t in range(length - window, length)])
+        wo, wl, _, off = ref.attention(q[0], k[:, at], v[:, at], D ** -0.5)
+        assert float((o[0].double() - wo).abs().max()) <= (4 * float(off.max()) + 2.0 ** -14) * float(v.abs().max())
+        assert bool(((lse[0].double() - wl).abs() <= off + 2.0 ** -20 + 2.0 ** -22 * wl.abs()).all())
+    ommx_kv8_decode_attention(q, cache["codes"], cache["scales"], table, i32([2 ** 31 - 1]), o, lse, window=window, sink_tokens=sinks, status=status)
+    assert int(status) == _lib.ST_BAD_LENGTH
+
+
 def test_what_is_not_visible_is_not_read():
     """Pages wholly outside the window may be anybody's, or none: their table entries are out of range here."""
     lens, page = [400, 390], 16
