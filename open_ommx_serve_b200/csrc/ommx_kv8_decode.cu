@@ -51,7 +51,7 @@ struct DecodeParams {
     float2 *stats;                                // [B][Hq]: reference and 1 / sum
     const float *before;                          // what weights add to
     int64_t q_b, q_h, o_b, o_h, lse_b;
-    int32_t q16, q_wide, o_type, group, col_blocks, page_shift, least, whole, window, sinks, most_units;
+    int32_t q16, q_wide, o_type, group, col_blocks, page_shift, least, whole, dealt, window, sinks, most_units;
     float sm_scale, cap, keep;
     int32_t *status;
 };
@@ -841,8 +841,9 @@ template <int G, bool PARTS> __device__ __forceinline__ void weigh(const DecodeP
     let_next_in();
     const int len = length_of(p, b);
     if ((int64_t)block * STRETCH >= len) return;
-    if (PARTS && reinterpret_cast<const uint2 *>(p.work)->y == OVER) return;                 // no shares were dealt out: reported
     const Span span = span_of(p, len);
+    // a sequence of more records than are counted was not attended to, or where they are dealt out none was: reported
+    if (p.dealt ? reinterpret_cast<const uint2 *>(p.work)->y == OVER : too_many(p, span.units, p.c.H * p.col_blocks)) return;
     const bool few = p.group <= SHARED_HEADS, wide = p.group % 4 == 0;
     const int64_t step = (int64_t)blocks * STRETCH;
     auto page_of = [&](int64_t first) -> int64_t {
@@ -965,7 +966,7 @@ template <int G, bool E4M3, bool FINE, int NW, bool CLUSTER> static int launch_d
     // The account's blocks: at most as many as the SMs hold. Where there are stretches for no more than that they stand beside those that join the
     // parts, and make references and sums themselves; else they come behind them (8 x 64K tokens: 234 us beside, 215 behind; one of 64K 41.4 and 43.0).
     const int64_t heads = (int64_t)p.c.H * p.s.B, stretches = (tokens + STRETCH - 1) / STRETCH;
-    const bool joins = !p.whole && !CLUSTER, beside = joins && stretches * heads <= 4LL * sm_count();
+    const bool joins = p.dealt, beside = joins && stretches * heads <= 4LL * sm_count();
     const int64_t fill = (6LL * sm_count() + heads - 1) / heads;
     const int account = (int)(stretches < fill ? stretches : fill) * p.c.H;
     if (joins) {
@@ -1034,6 +1035,7 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     if (units > 36 * cluster) cluster = 1;
     p.whole = units <= WHOLE / 2 || (units <= WHOLE && cluster == 1);
     if (p.whole) cluster = 1;
+    p.dealt = !p.whole && cluster == 1;
     const int64_t blocks = p.whole ? rows : cluster > 1 ? cluster * rows : most < 1 ? 1 : most < hold ? most : hold;
     const int64_t tokens = p.c.weight ? most_tokens(a) : 0;                 // that weights are kept of
     auto launch = [&](auto g, auto e4m3, auto fine) {

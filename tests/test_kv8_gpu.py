@@ -610,6 +610,28 @@ def test_lengths_past_max_seq_len():
         assert torch.equal(cache["weight"][ids, :, t % page], before[ids, :, t % page])
 
 
+@pytest.mark.parametrize("most,H", [(200, 32), (500, 18), (3000, 32), (40000, 32)])
+def test_an_account_leaves_sequences_of_too_many_records_alone(most, H):
+    """A sequence of so many records that they are not counted, beside a short one: its weights stay as they were, and where records are dealt out (the
+    last two) both sequences'. Records in a block to a row, a cluster to a row, and in shares with the account beside the join and behind it."""
+    page, D, P = 256, 64, 6
+    cache = to_gpu(random_cache(P, H, D, page, I8))
+    before = cache["weight"].clone()
+    table = (torch.arange(2 ** 31 // page, dtype=I32, device=DEV) % 4).repeat(2, 1)
+    table[1, 0] = 5
+    lens = [2 ** 31 - 2 ** 10, 180]
+    q, o, lse, status = torch.randn(2, H, D, device=DEV).bfloat16(), torch.empty(2, H, D, device=DEV), torch.empty(2, H, device=DEV), i32([0])
+    work = torch.full((kv8_workspace_floats(2, H, D, most, weight=True),), 7.0, device=DEV)
+    ommx_kv8_decode_attention(q, cache["codes"], cache["scales"], table, i32(lens), o, lse, weight=cache["weight"], keep=0.5, workspace=work, max_seq_len=most, status=status)
+    assert int(status) == _lib.ST_BAD_LENGTH
+    assert torch.equal(cache["weight"][:5], before[:5])
+    if most <= 500:
+        short = table[1:, :1].contiguous()
+        check(q[1:], cache, short, lens[1:], o[1:], lse[1:], weight=cache["weight"], before=before, keep=0.5)
+    else:
+        assert torch.equal(cache["weight"], before)
+
+
 # ---- the account of weights ------------------------------------------------------------------------------------------
 def test_weights_accumulate_over_steps():
     lens, page, H, Hq, D = [35, 610, 0], 32, 2, 12, 64
