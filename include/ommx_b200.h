@@ -593,7 +593,7 @@ typedef struct ommx_kv8_evict_args {
  * Keep `budget` tokens of each sequence and kv head: the first sink_tokens, the last recent_tokens and of the others those of the largest
  * weight (ties to the lower place, NaN last), moved with their weights to the places 0 .. budget - 1 in their order.  A record of kept
  * tokens has the largest E that they had; codes are rounded to that.  A sequence of at most `budget` tokens keeps all; one with a page out
- * of range, or more tokens than its tables hold, is reported and stays as it is.  One launch; two where
+ * of range, more tokens than its tables hold, or more than 2^30 - 2^16, is reported and stays as it is.  One launch; two where
  * len_out is b_seq_len.
  */
 int ommx_b200_kv8_evict(const ommx_kv8_evict_args *args, void *stream);

@@ -20,13 +20,14 @@ using namespace kv;
 // waits (64 sequences of 4608 to 4096 tokens, 8 kv heads: 259 us with one size, 228 so).
 constexpr int BINS = 2048, MOST_CLUSTER = 8;
 constexpr int HELD = 8;                           // keys that a thread holds, of consecutive tokens of a page; TURN: a block's turn of keys
+constexpr int LOWEST_BIN = (1 << 30) - 1;         // what the lowest part, which is not counted, is taken to hold
 constexpr int FEW = 4096;                         // keys that each block of a cluster finishes for itself
 template <int THREADS> struct Sizes {
     static constexpr int TURN = THREADS * HELD;
     static constexpr int PLACES = THREADS / 2;    // that a block moves at a time
     static constexpr int MOST_KEYS = 40 * THREADS;                          // further keys that a block holds in shared memory; it reads others again
 };
-constexpr int MOST_TOKENS = 0x7FFF0000;           // places are counted in 32 bits, a turn of all blocks and more to spare
+constexpr int MOST_TOKENS = (1 << 30) - (1 << 16);  // a count of them and one that stands for all (LOWEST_BIN) fit into 32 bits together
 
 struct EvictParams {
     Cache c;
@@ -199,7 +200,7 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
                 for (int r = 0; r < MOST_CLUSTER; ++r) {
                     mine.x += __float_as_int(v[r].x); mine.y += __float_as_int(v[r].y); mine.z += __float_as_int(v[r].z); mine.w += __float_as_int(v[r].w);
                 }
-                if (tid == BINS / 4 - 1) mine.x = 0x3FFFFFFF;
+                if (tid == BINS / 4 - 1) mine.x = LOWEST_BIN;
             }
             const int sum = mine.x + mine.y + mine.z + mine.w;
             int before = warp_inclusive_scan(sum, lane);

@@ -794,6 +794,26 @@ def test_sequences_with_pages_out_of_range_are_not_evicted_from():
             assert same(cache2[name], cache[name]), name
 
 
+def test_sequences_of_more_tokens_than_are_counted_are_not_evicted_from():
+    """Beside one that is. The table of the long one names four pages over and over."""
+    page, H, D, budget = 256, 2, 64, 40
+    cache = random_cache(5, H, D, page, I8)
+    gpu, status = to_gpu(cache), i32([0])
+    table = (torch.arange(2 ** 30 // page, dtype=I32, device=DEV) % 4).repeat(2, 1)
+    table[1, 0] = 4
+    given = [2 ** 30 - 2 ** 16 + 1, 100]
+    kept, len_out = torch.full((2, H, budget), 7, dtype=I32, device=DEV), i32([1, 1])
+    ommx_kv8_evict(gpu["codes"], gpu["scales"], gpu["weight"], table, i32(given), kept, len_out=len_out, status=status)
+    assert int(status) == _lib.ST_BAD_LENGTH
+    assert bool((kept[0] == -1).all()) and len_out.tolist() == [given[0], budget]
+    want = [ref.evict(cache["weight"][4, h, :100].tolist(), 100, budget, 0, 0) for h in range(H)]
+    assert kept[1].tolist() == want
+    short = torch.tensor([[4]])
+    ref.move(cache["codes"], cache["scales"], cache["weight"], short, short, [want])
+    for name in cache:
+        assert same(gpu[name], cache[name]), name
+
+
 # ---- together --------------------------------------------------------------------------------------------------------
 class Layer:
     """A layer's cache and buffers, and a step as a user makes it."""
