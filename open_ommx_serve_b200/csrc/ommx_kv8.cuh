@@ -132,6 +132,32 @@ inline int read_cache(const char *who, const ommx_kv8_cache &c, Cache *to) {
     *to = {(uint8_t *)c.codes, c.scales, c.weight, c.num_pages, c.n_kv_heads, c.page_size, c.page_size / BLOCK};
     return 0;
 }
+// How many clusters of a size (2, 4 or 8) the device holds at once, asked for once: fewer than blocks / size, since a cluster lies on SMs of one
+// group (148 SMs: 33 of eight blocks, two to an SM, and 15 with one). One cluster more than that is a second turn for all.
+struct AtOnce { std::atomic<int> count[MAX_DEVICES][4]; };
+template <typename K> int clusters_at_once(AtOnce &known, K kernel, int threads, size_t smem, int cluster) {
+    int dev = 0, size = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return 0;
+    while (1 << size < cluster) ++size;
+    if (const int held = known.count[dev][size].load(std::memory_order_acquire)) return held - 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = cluster;
+    cfg.blockDim = threads;
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 0) {
+        (void)cudaGetLastError();
+        n = 0;
+    }
+    known.count[dev][size].store(n + 1, std::memory_order_release);
+    return n;
+}
 inline int read_seqs(const char *who, const ommx_kv8_seqs &s, const Cache &c, Seqs *to) {
     kv4::Cache like = {nullptr, c.num_pages, c.H, c.page, c.parts};
     return kv4::read_seqs(who, s, like, to);

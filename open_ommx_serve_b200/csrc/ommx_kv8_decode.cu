@@ -1036,8 +1036,14 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     const int64_t most = (units * rows + p.least - 1) / p.least, hold = most_blocks(warps);
     // Rows of middling length, and few, go to a cluster of eight-warp blocks each, as many as fit at once: no second kernel
     int cluster = 1;
-    while (cluster < MOST_CLUSTER && 2 * cluster * rows <= most_blocks(8)) cluster *= 2;
-    if (units > 36 * cluster) cluster = 1;
+    static AtOnce known[2];                       // of eight and sixteen warps; D = 64 takes less
+    while (cluster < MOST_CLUSTER && 2 * cluster * rows <= most_blocks(8) && rows <= clusters_at_once(known[0], kv8_decode_kernel<4, false, false, 8, true>, 256, sizeof(Memory<4, 8>), 2 * cluster)) cluster *= 2;
+    // of sixteen warps where a row has more records than eight of eight warps should take (8 kv heads: 4400 tokens 10.1 us with eight, 10.7 with sixteen), up
+    // to where all SMs and a join are faster: 5000 tokens 10.9 us so and 13.8 with a join, 8000 12.4 and 14.0, 12000 14.7 and 14.9; of one kv
+    // head 5000 10.7 and 11.1, 7000 11.7 and 11.1
+    const bool wide = cluster == MOST_CLUSTER && units > 36 * cluster && units <= (40 + 6 * rows) * cluster &&
+                      rows <= clusters_at_once(known[1], kv8_decode_kernel<4, false, false, 16, true>, 512, sizeof(Memory<4, 16>), cluster);
+    if (units > 36 * cluster && !wide) cluster = 1;
     p.whole = units <= WHOLE / 2 || (units <= WHOLE && cluster == 1);
     if (p.whole) cluster = 1;
     p.dealt = !p.whole && cluster == 1;
@@ -1046,6 +1052,7 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     auto launch = [&](auto g, auto e4m3, auto fine) {
         constexpr int G = decltype(g)::value;
         constexpr bool E4M3 = decltype(e4m3)::value, FINE = decltype(fine)::value;
+        if (cluster > 1 && wide) return launch_decode<G, E4M3, FINE, 16, true>(p, blocks, cluster, tokens, st);
         if (cluster > 1) return launch_decode<G, E4M3, FINE, 8, true>(p, blocks, cluster, tokens, st);
         return warps == 4 ? launch_decode<G, E4M3, FINE, 4, false>(p, blocks, 1, tokens, st) : launch_decode<G, E4M3, FINE, 8, false>(p, blocks, 1, tokens, st);
     };

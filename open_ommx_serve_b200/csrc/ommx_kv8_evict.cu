@@ -493,12 +493,15 @@ static int evict(const ommx_kv8_evict_args *a, cudaStream_t st) {
     p.page_shift = shift_of(p.c.page);
     p.status = a->status;
     // a cluster to a row where rows are few, but no block for less than 512 tokens (8 kv heads: 4608 to 4096 tokens
-    // 23.0 us so and 27.0 with 1024; 4 sequences of 3000 to 2000 20.9 and 25.5; 1200 to 1000 19.1 and 20.3)
+    // 23.0 us so and 27.0 with 1024; 4 sequences of 3000 to 2000 20.9 and 25.5; 1200 to 1000 19.1 and 20.3),
+    // and as many as run at once (16 rows of 20000 to 4096 tokens: 51.3 us in clusters of eight, of which 15 do, 28.9 in clusters of four)
     int64_t tokens = (int64_t)p.s.max_pages * p.c.page;
     if (a->max_seq_len > 0 && a->max_seq_len < tokens) tokens = a->max_seq_len;
     const int64_t rows = (int64_t)p.s.B * p.c.H;
     int cluster = 1;
-    while (cluster < MOST_CLUSTER && 2 * cluster * rows <= sm_count() && tokens >= 1024LL * cluster) cluster *= 2;
+    static AtOnce known;                          // all forms of 1024 threads take all of an SM's registers
+    auto fit = [&](int n) { return clusters_at_once(known, kv8_evict_kernel<4, false, 1024>, 1024, 4 * Sizes<1024>::MOST_KEYS, n); };
+    while (cluster < MOST_CLUSTER && 2 * cluster * rows <= sm_count() && rows <= fit(2 * cluster) && tokens >= 1024LL * cluster) cluster *= 2;
     auto launch = [&](auto g, auto e4m3) {
         constexpr int G = decltype(g)::value;
         constexpr bool E4M3 = decltype(e4m3)::value;

@@ -8,6 +8,8 @@ divides it included; a weight times its scale goes to fp16, by 2^-12 of itself
 head's weight below 2^-126, where fp32 has no normal numbers, counts as 0: 2^-126 for each head.
 """
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -354,6 +356,40 @@ def test_every_way_of_dealing(lens, H, Hq, code):
     attend(lens, H, Hq, 128, 16, code, BF16)
     attend(lens, H, Hq, 64, 32, code, F16, seed=2, weigh=True, max_len=None)
     attend(lens, H, Hq, 128, 64, code, BF16, out=F32, seed=3, window=333, sink_tokens=5)
+
+
+@pytest.mark.parametrize("lens,H,Hq,D", [([4700], 8, 32, 128), ([5009, 31, 0], 1, 8, 128), ([9000], 8, 32, 64), ([6000, 4999, 1, 16, 17], 3, 9, 64), ([4800] * 2, 7, 7, 128), ([4800] * 2, 8, 8, 128), ([600] * 36, 1, 4, 64)])
+@pytest.mark.parametrize("code", [I8, E4M3])
+def test_clusters_of_every_size(lens, H, Hq, D, code):
+    """Rows in clusters of eight blocks of sixteen warps, just fewer and just more of them than run at once; and as many as would be one more than run at
+    once in clusters of eight of eight warps."""
+    attend(lens, H, Hq, D, 32, code, BF16, weigh=True, keep=0.5)
+    attend(lens, H, Hq, D, 32, code, F16, out=F32)
+
+
+def test_a_first_call_may_be_captured():
+    """In a process of its own: what a call asks of the device for the first time it may ask while a graph is captured."""
+    code = """
+import torch
+from open_ommx_serve_b200 import ommx_kv8_alloc, ommx_kv8_append, ommx_kv8_decode_attention, ommx_kv8_evict
+c = ommx_kv8_alloc(400, 8, 128, weight=True, device="cuda")
+k = torch.randn(5000, 8, 128, device="cuda")
+table, length = torch.arange(400, dtype=torch.int32, device="cuda").view(1, -1), torch.tensor([5000], dtype=torch.int32, device="cuda")
+starts, q, o, lse = torch.tensor([0, 5000], dtype=torch.int32, device="cuda"), torch.randn(1, 8, 128, device="cuda").bfloat16(), torch.empty(1, 8, 128, device="cuda"), torch.empty(1, 8, device="cuda")
+kept, work = torch.empty(1, 8, 100, dtype=torch.int32, device="cuda"), torch.empty(1 << 21, device="cuda")
+def step():
+    ommx_kv8_append(k, k, c["codes"], c["scales"], table, length, row_start=starts, weight=c["weight"])
+    ommx_kv8_decode_attention(q, c["codes"], c["scales"], table, length, o, lse, weight=c["weight"], keep=0.0, workspace=work, max_seq_len=5000)
+    ommx_kv8_evict(c["codes"], c["scales"], c["weight"], table, length, kept)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    step()
+graph.replay()
+first = [x.clone() for x in (o, lse, kept)]
+step()
+assert all(torch.equal(a, b) for a, b in zip(first, (o, lse, kept)))
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (15, 3), (16, 16), (17, 17), (40, 0), (100, 33), (99, 1000), (1000, 4), (2 ** 31 - 1, 2 ** 31 - 1)])
@@ -754,6 +790,12 @@ def test_eviction_where_keys_do_not_fit(H):
     """Many rows, so that one block, of either size, has a row of more keys than it holds."""
     lens = [50000] + [30] * 80
     evict(lens, H, 64, 256, I8, 64, 2, 8)
+
+
+@pytest.mark.parametrize("B,H", [(5, 3), (8, 2), (17, 2), (36, 1)])
+def test_eviction_in_clusters_of_every_size(B, H):
+    """As many rows as clusters of eight blocks run at once and one more, and the same of four."""
+    evict([4200 + 7 * b for b in range(B)], H, 64, 16, I8, 300, 2, 30, seed=B)
 
 
 @pytest.mark.parametrize("code,D", [(I8, 128), (E4M3, 64)])
