@@ -570,7 +570,7 @@ typedef struct ommx_kv8_decode_args {
 
 /* Attention of one query row per sequence.  A kv head's records are read once for each eight of its query heads.  Two launches; one where
  * no sequence sees more than 512 tokens by max_seq_len, the table's width or the window, or, where rows (sequences x kv heads x eights of
- * query heads) are few enough for clusters, 4608 (up to 16000 where they are 15 at most); one more where weights are kept of many tokens, two at least. */
+ * query heads) are few enough for clusters, 4608 (up to 16000 where they are 15 at most), or a window of up to 1500 where there are some 300 to 590 rows; one more where weights are kept of many tokens, two at least. */
 int ommx_b200_kv8_decode(const ommx_kv8_decode_args *args, void *stream);
 /* floats of workspace that this call needs on the current device (0: none; its pointers are not looked at, but for whether there is a weight) */
 int64_t ommx_b200_kv8_decode_workspace_floats(const ommx_kv8_decode_args *args);

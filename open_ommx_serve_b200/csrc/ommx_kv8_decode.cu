@@ -1044,7 +1044,10 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     const bool wide = cluster == MOST_CLUSTER && units > 36 * cluster && units <= (40 + 6 * rows) * cluster &&
                       rows <= clusters_at_once(known[1], kv8_decode_kernel<4, false, false, 16, true>, 512, sizeof(Memory<4, 16>), cluster);
     if (units > 36 * cluster && !wide) cluster = 1;
-    p.whole = units <= WHOLE / 2 || (units <= WHOLE && cluster == 1);
+    // A window makes rows alike, so where there is a block for each and not two they go whole too (61 sequences of 300 to 20000 tokens, 8 kv heads: windows of 600
+    // 21.3 -> 18.0 us, of 1025 30.8 -> 26.7; 50 of 61 sequences too short for one of 1025 18.3 -> 20.6, for 1800 22.6 -> 31.1, which is past the limit)
+    const bool alike = a->window > 0 && cluster == 1 && rows <= hold && 2 * rows > hold && units <= 3 * WHOLE;
+    p.whole = units <= WHOLE / 2 || (units <= WHOLE && cluster == 1) || alike;
     if (p.whole) cluster = 1;
     p.dealt = !p.whole && cluster == 1;
     const int64_t blocks = p.whole ? rows : cluster > 1 ? cluster * rows : most < 1 ? 1 : most < hold ? most : hold;

@@ -423,6 +423,14 @@ def test_first_tokens_and_lengths_near_the_end_of_32_bits(code, D):
     assert int(status) == _lib.ST_BAD_LENGTH
 
 
+@pytest.mark.parametrize("code,D", [(I8, 128), (E4M3, 64)])
+def test_windows_of_many_rows(code, D):
+    """A window's rows in a block each, where there are blocks for all and not for two each; and more rows than that."""
+    lens = [[1200, 0, 650, 17, 900, 1, 601, 600][b % 8] + b // 8 for b in range(50)]
+    attend(lens, 8, 8, D, 16, code, BF16, window=600, sink_tokens=5, weigh=True, keep=0.5)
+    attend([700] * 76, 8, 8, D, 16, code, F16, window=600)
+
+
 def test_what_is_not_visible_is_not_read():
     """Pages wholly outside the window may be anybody's, or none: their table entries are out of range here."""
     lens, page = [400, 390], 16
