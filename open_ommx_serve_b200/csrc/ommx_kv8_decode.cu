@@ -16,7 +16,7 @@
 // (8 x 64K tokens).
 //
 // What bounds it: a record's 32 D bytes are read once for each eight query heads of its kv head, and a warp spends 343 instructions on one (D = 128, int8): the
-// copies alone take 165 us of 8 x 64K tokens, 8 kv heads, the products alone 133, both 180 (6.0 TB/s, 92 % of what a copy reaches); 32 ragged
+// copies alone take 165 us of 8 x 64K tokens, 8 kv heads, the products alone 133, both 171 to 180 (6.0 to 6.3 TB/s, 92 to 96 % of what a copy reaches); 32 ragged
 // sequences of 700 to 8191 tokens 57, 57 and 64. A warp has a ring of its own, so that no barrier stands between a copy and its use: two slots and 16
 // warps to an SM (8 x 64K tokens: 183 us; three slots 192, 12 warps and three slots 188, 20 warps 208). Few and short rows are bound by
 // the chain of launch, lengths, table, records and join: 6.9 us for one of 333 tokens, of which a launch alone takes 2.5.
