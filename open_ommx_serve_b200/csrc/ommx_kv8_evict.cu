@@ -28,7 +28,7 @@ constexpr int FEW = 4096;                         // keys that each block of a c
 template <int THREADS> struct Sizes {
     static constexpr int TURN = THREADS * HELD;
     static constexpr int PLACES = THREADS / 2;    // that a block moves at a time
-    static constexpr int MOST_KEYS = 40 * THREADS;                          // further keys that a block holds in shared memory; it reads others again
+    static constexpr int MOST_KEYS = 36 * THREADS;                          // further keys that a block holds in shared memory; it reads others again
 };
 constexpr int MOST_TOKENS = (1 << 30) - (1 << 16);  // a count of them and one that stands for all (LOWEST_BIN) fit into 32 bits together
 
@@ -69,7 +69,7 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
     constexpr int EACH = BINS / THREADS;          // bins of a thread
     extern __shared__ __align__(16) uint8_t memory[];                       // keys, then rows
     uint32_t *keys = reinterpret_cast<uint32_t *>(memory);
-    __shared__ __align__(16) int histogram[BINS];
+    __shared__ __align__(16) int histograms[2][BINS];                       // the one of a round is read by peers until the next round's barrier
     __shared__ uint32_t few[FEW];
     __shared__ Place places[PLACES];
     __shared__ int warp_sum[2][32], starts[MOST_CLUSTER + 1], bin, left, inside, listed, more, same, above_here, equal_here, first_place, bad, spoilt;
@@ -79,11 +79,12 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
     const int head = blockIdx.x / n, b = blockIdx.y;
     if (tid == 0) bad = listed = more = 0;
     if (tid < 64) warp_sum[tid / 32][tid % 32] = 0;                         // of warps that there are not
-    auto clear = [&] {
+    auto clear = [&](int *histogram) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) histogram[tid + i * THREADS] = 0;
     };
-    clear();
+    clear(histograms[0]);
+    clear(histograms[1]);
     wait_earlier();
     let_next_in();
     const int given = p.s.len[b];
@@ -182,6 +183,7 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
         int want = wanted, width = 31;
         uint32_t a = ZERO;
         bool placed = false;                      // the block knows where its first token goes
+        int *histogram = histograms[0], *other = histograms[1];             // `other`: all zeros but while peers read it
         for (bool begun = false; width > 0; begun = true) {
             const int shift = max(0, width - 11);
             // the lowest part is not counted: what is not above it is in it, and often it is the one that most are in
@@ -192,6 +194,7 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
             __syncthreads();
             cluster_barrier();
             if (!begun) hear();
+            else clear(other);
             // from the top: thread t has bins BINS - 1 - 4 t and the three below
             int4 mine = make_int4(0, 0, 0, 0);
             if (tid < BINS / 4) {
@@ -218,9 +221,12 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
                 inside = up[j];
                 bin = BINS - 1 - 4 * tid - j;
             }
-            cluster_barrier();                    // all peers have read
-            if (!begun && spoilt) { faults = OMMX_ST_BAD_PAGE; break; }
-            clear();
+            __syncthreads();
+            if (!begun && spoilt) {
+                cluster_barrier();                // all peers have read
+                faults = OMMX_ST_BAD_PAGE;
+                break;
+            }
             if (wanted == 0) { a = ~0u; break; }
             if (!begun && bin == 0) { a = 0; width = 32; }                  // `want` as it was
             else { a += (uint32_t)bin << shift; want = left; width = shift; }
@@ -260,12 +266,12 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
                     const int cut = max(0, width - 11);
 #pragma unroll
                     for (int j = 0; j < FEW / THREADS; ++j)
-                        if (tid + j * THREADS < count && k[j] >> width == 0) atomicAdd(&histogram[k[j] >> cut], 1);
+                        if (tid + j * THREADS < count && k[j] >> width == 0) atomicAdd(&other[k[j] >> cut], 1);
                     __syncthreads();
                     // from the top: thread t has bins BINS - 1 - EACH t and those below
                     int mine[EACH], all_mine = 0;
 #pragma unroll
-                    for (int j = 0; j < EACH; ++j) { mine[j] = histogram[BINS - 1 - EACH * tid - j]; all_mine += mine[j]; }
+                    for (int j = 0; j < EACH; ++j) { mine[j] = other[BINS - 1 - EACH * tid - j]; all_mine += mine[j]; }
                     int over = warp_inclusive_scan(all_mine, lane);
                     if (lane == 31) warp_sum[0][warp] = over;
                     __syncthreads();
@@ -278,7 +284,7 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
                             over += mine[j];
                         }
                     }
-                    clear();
+                    clear(other);
                     __syncthreads();
                     const uint32_t from = (uint32_t)bin << cut;
 #pragma unroll
@@ -304,6 +310,9 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
                 break;
             }
             __syncthreads();
+            int *const t = histogram;
+            histogram = other;
+            other = t;
         }
         leave(faults);
         if (faults) return;
@@ -386,36 +395,37 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
     for (int base = 0; base < keep; base += n * PLACES) {
         const int start = base + rank * PLACES, count = max(0, min(PLACES, keep - start));
         __syncthreads();                          // what the pass before wrote out of here
-        if (tid < PLACES) {
-            Place x = {0, 0, 0.0f, 0, 0};
-            if (tid < count) {
-                const int i = start + tid;
-                int at = i;
-                if (!all && short_row) {          // from the list of the block that it is in
-                    int r = 0;
+        Place x = {0, 0, 0.0f, 0, 0};
+        if (tid < count) {
+            const int i = start + tid;
+            int at = i;
+            if (!all && short_row) {              // from the list of the block that it is in
+                int r = 0;
 #pragma unroll
-                    for (int j = 1; j < MOST_CLUSTER; ++j) r = j < (int)n && firsts[j] <= i ? j : r;
-                    at = r * share + peer_half(list + (i - firsts[r]), r);
-                } else if (!all) {
-                    at = __ldcg(out + i);
-                }
-                const int64_t page = page_id(p.s, b, at >> p.page_shift), to = page_id(p.to, b, i >> p.page_shift);
-                x.from = row_of(p, page, head, at);
-                x.to = row_of(p, to, head, i);
-                x.own = reinterpret_cast<const uint16_t *>(p.c.scales)[x.from / BLOCK];
-                x.weight = p.c.weight[x.from];
+                for (int j = 1; j < MOST_CLUSTER; ++j) r = j < (int)n && firsts[j] <= i ? j : r;
+                at = r * share + peer_half(list + (i - firsts[r]), r);
+            } else if (!all) {
+                at = __ldcg(out + i);
             }
-            uint32_t most = x.own;
-#pragma unroll
-            for (int d = 1; d < 16; d *= 2) most = __vmaxu4(most, __shfl_xor_sync(~0u, most, d));
-            x.scales = (uint16_t)most;
-            places[tid] = x;
+            const int64_t page = page_id(p.s, b, at >> p.page_shift), to = page_id(p.to, b, i >> p.page_shift);
+            x.from = row_of(p, page, head, at);
+            x.to = row_of(p, to, head, i);
+            places[tid].from = x.from;
+            x.own = reinterpret_cast<const uint16_t *>(p.c.scales)[x.from / BLOCK];            // on its way beside the rows
+            x.weight = p.c.weight[x.from];
         }
         __syncthreads();
         for (int i = tid / CHUNKS; i < count; i += THREADS / CHUNKS) {
             const uint32_t from = places[i].from;
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(rows_at + 16 * (i * CHUNKS + chunk)),
                          "l"(codes + (int64_t)(from / BLOCK) * (32 * D) + (from % BLOCK) * D) : "memory");
+        }
+        if (tid < PLACES) {
+            uint32_t most = x.own;
+#pragma unroll
+            for (int d = 1; d < 16; d *= 2) most = __vmaxu4(most, __shfl_xor_sync(~0u, most, d));
+            x.scales = (uint16_t)most;
+            places[tid] = x;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
