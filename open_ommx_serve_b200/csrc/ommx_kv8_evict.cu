@@ -8,9 +8,9 @@
 //   alone. A thread holds its first keys in registers; counts meet in distributed shared memory.
 // * moves: places ascend, and a token never moves up. So once a cluster has read all that a stretch of places takes into its shared
 //   memory it can write that stretch where the tokens lie, and go on to the next.
-// What bounds it: where rows are many what moves (64 sequences of 4608 to 4096 tokens, 8 kv heads 228 us; 1.1 GB there and back take 165 of a copy's rate),
-// where they are few the chain: 64K to 4096 tokens, 8 kv heads 28 us in graph replays, of which reading weights takes 2, the first count and its
-// exchange 5.5, the rest of the choice 5, the list 3.7 and the move 7.5.
+// What bounds it: where rows are many what moves (64 sequences of 4608 to 4096 tokens, 8 kv heads 210 us; 1.1 GB there and back take 165 of a copy's rate),
+// where they are few the chain: 64K to 4096 tokens, 8 kv heads 26.5 us in graph replays, of which reading weights takes 2, the first count and its
+// exchange 5, the rest of the choice 5, the list 3.7 and the move 7.
 #include "ommx_kv8.cuh"
 #include "ommx_kv_device.cuh"
 
@@ -20,7 +20,7 @@ namespace kv8 {
 using namespace kv;
 
 // Blocks of 1024 threads, one to an SM, or, where there are more rows than SMs, of 512, two to an SM, which fill each other's
-// waits (64 sequences of 4608 to 4096 tokens, 8 kv heads: 259 us with one size, 228 so).
+// waits (64 sequences of 4608 to 4096 tokens, 8 kv heads: 259 us with one size, 228 so when that was done).
 constexpr int BINS = 2048, MOST_CLUSTER = 8;
 constexpr int HELD = 8;                           // keys that a thread holds, of consecutive tokens of a page; TURN: a block's turn of keys
 constexpr int LOWEST_BIN = (1 << 30) - 1;         // what the lowest part, which is not counted, is taken to hold
