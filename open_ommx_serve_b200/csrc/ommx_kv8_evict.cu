@@ -165,11 +165,21 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
             }
         }
         auto key_at = [&](int i) { return i - lo - TURN < p.keys ? keys[i - lo - TURN] : load(i); };      // behind the first turn
+        // of `held`, a bit each: those that there are, and those that are not kept anyway
+        uint32_t have = 0, live = 0;
+#pragma unroll
+        for (int u = 0; u < HELD; ++u) {
+            have |= (uint32_t)(place(0, u) < hi) << u;
+            live |= (uint32_t)(place(0, u) >= first && place(0, u) < last) << u;
+        }
+        const bool any_held = __any_sync(~0u, have != 0);                   // warps of a short row have none
         // f(key) for each of the thread's keys that is not kept anyway
         auto each_key = [&](auto f) {
+            if (any_held) {
 #pragma unroll
-            for (int u = 0; u < HELD; ++u)
-                if (place(0, u) >= first && place(0, u) < last) f(held[u]);
+                for (int u = 0; u < HELD; ++u)
+                    if (live >> u & 1) f(held[u]);
+            }
             for (int turn = 1; turn < turns; ++turn)
                 for (int u = 0; u < HELD; ++u)
                     if (place(turn, u) >= first && place(turn, u) < last) f(key_at(place(turn, u)));
@@ -320,23 +330,36 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
         uint32_t ms, es;                          // of a thread's keys of a turn, a bit each
         auto look = [&](int turn) {
             ms = es = 0;
+            if (turn == 0) {
+                if (any_held) {
 #pragma unroll
-            for (int u = 0; u < HELD; ++u) {
-                const int i = place(turn, u);
-                const uint32_t k = i >= hi ? 0u : turn == 0 ? held[u] : key_at(i);
-                const bool pinned = i < p.sinks || i >= len - p.recent;
-                ms |= (uint32_t)(i < hi && (pinned || k > a)) << u;
-                es |= (uint32_t)(i < hi && !pinned && k == a) << u;
+                    for (int u = 0; u < HELD; ++u) {
+                        ms |= (uint32_t)(held[u] > a) << u;
+                        es |= (uint32_t)(held[u] == a) << u;
+                    }
+                    ms = (ms & live) | (have & ~live);
+                    es &= live;
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < HELD; ++u) {
+                    const int i = place(turn, u);
+                    const uint32_t k = i >= hi ? 0u : key_at(i);
+                    const bool pinned = i < p.sinks || i >= len - p.recent;
+                    ms |= (uint32_t)(i < hi && (pinned || k > a)) << u;
+                    es |= (uint32_t)(i < hi && !pinned && k == a) << u;
+                }
             }
             return __popc(ms) | __popc(es) << 16;
         };
         int above = 0, equal = 0;
-        for (int turn = turns - 1; turn >= 0; --turn) {                     // the first turn's bits stay
+        for (int turn = turns - 1; turn > 0; --turn) {                      // the first turn's bits stay
             const int c = look(turn);
             above += __reduce_add_sync(~0u, c & 0xFFFF);
             equal += __reduce_add_sync(~0u, c >> 16);
         }
-        if (lane == 0) { warp_sum[0][warp] = above; warp_sum[1][warp] = equal; }
+        const int counts = look(0), scanned = warp_inclusive_scan(counts, lane);
+        if (lane == 31) { warp_sum[0][warp] = above + (scanned & 0xFFFF); warp_sum[1][warp] = equal + (scanned >> 16); }
         __syncthreads();
         if (!placed) {
             if (warp == 0) {
@@ -356,7 +379,7 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
         const int first_here = above_all + min(equal_all, want);
         if (tid == 0) first_place = first_here;
         for (int turn = 0; turn < turns; ++turn) {
-            const int c = turn > 0 ? look(turn) : __popc(ms) | __popc(es) << 16, scan = warp_inclusive_scan(c, lane);
+            const int c = turn > 0 ? look(turn) : counts, scan = turn > 0 ? warp_inclusive_scan(c, lane) : scanned;
             if (turns > 1) {
                 __syncthreads();                  // `warp_sum` is read
                 if (lane == 31) { warp_sum[0][warp] = scan & 0xFFFF; warp_sum[1][warp] = scan >> 16; }
@@ -365,17 +388,18 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
             const int m = warp_sum[0][lane], e = warp_sum[1][lane];
             above = above_all + __reduce_add_sync(~0u, lane < warp ? m : 0) + ((scan - c) & 0xFFFF);
             equal = equal_all + __reduce_add_sync(~0u, lane < warp ? e : 0) + ((scan - c) >> 16);
-            above_all += __reduce_add_sync(~0u, m);
-            equal_all += __reduce_add_sync(~0u, e);
-#pragma unroll
-            for (int u = 0; u < HELD; ++u) {
-                if (ms >> u & 1 || (es >> u & 1 && equal < want)) {
-                    const int to = above + min(equal, want);
+            if (turns > 1) {
+                above_all += __reduce_add_sync(~0u, m);
+                equal_all += __reduce_add_sync(~0u, e);
+            }
+            for (uint32_t bits = ms | es; bits; bits &= bits - 1) {
+                const int u = __ffs(bits) - 1;
+                const uint32_t below = (1u << u) - 1;
+                const int like = equal + __popc(es & below), to = above + __popc(ms & below) + min(like, want);
+                if (ms >> u & 1 || like < want) {
                     if (short_row) list[to - first_here] = (uint16_t)(place(turn, u) - lo);
                     else out[to] = place(turn, u);
                 }
-                above += ms >> u & 1;
-                equal += es >> u & 1;
             }
         }
         __syncthreads();
