@@ -19,9 +19,10 @@ namespace kv8 {
 
 using namespace kv;
 
-// Blocks of 1024 threads, one to an SM, or, where there are more rows than SMs, of 512, two to an SM, which fill each other's
-// waits (64 sequences of 4608 to 4096 tokens, 8 kv heads: 259 us with one size, 228 so when that was done).
-constexpr int BINS = 2048, MOST_CLUSTER = 8;
+// Blocks of 1024 threads, one to an SM, or of 512, two to an SM: where there are more rows than SMs, since they fill each other's waits (64 sequences of 4608
+// to 4096 tokens, 8 kv heads: 259 us with one size, 228 so when that was done), and for rows of up to SHORT tokens, whose blocks wait for barriers (4
+// sequences of 300 to 200 tokens, 4 kv heads 12.3 us with 1024 and 11.5 with 512; one of 700 to 500 14.4 and 14.6).
+constexpr int BINS = 2048, MOST_CLUSTER = 8, SHORT = 640;
 constexpr int HELD = 8;                           // keys that a thread holds, of consecutive tokens of a page; TURN: a block's turn of keys
 constexpr int LOWEST_BIN = (1 << 30) - 1;         // what the lowest part, which is not counted, is taken to hold
 constexpr int FEW = 4096;                         // keys that each block of a cluster finishes for itself
@@ -539,7 +540,7 @@ static int evict(const ommx_kv8_evict_args *a, cudaStream_t st) {
     auto launch = [&](auto g, auto e4m3) {
         constexpr int G = decltype(g)::value;
         constexpr bool E4M3 = decltype(e4m3)::value;
-        return rows > sm_count() ? launch_evict<G, E4M3, 512>(p, tokens, cluster, st) : launch_evict<G, E4M3, 1024>(p, tokens, cluster, st);
+        return rows > sm_count() || tokens <= SHORT ? launch_evict<G, E4M3, 512>(p, tokens, cluster, st) : launch_evict<G, E4M3, 1024>(p, tokens, cluster, st);
     };
     using std::integral_constant;
     int rc;
