@@ -9,8 +9,8 @@
 // * moves: places ascend, and a token never moves up. So once a cluster has read all that a stretch of places takes into its shared
 //   memory it can write that stretch where the tokens lie, and go on to the next.
 // What bounds it: where rows are many what moves (64 sequences of 4608 to 4096 tokens, 8 kv heads 210 us; 1.1 GB there and back take 165 of a copy's rate),
-// where they are few the chain: 64K to 4096 tokens, 8 kv heads 26.5 us in graph replays, of which reading weights takes 2, the first count and its
-// exchange 5, the rest of the choice 5, the list 3.7 and the move 7.
+// where they are few the chain: 64K to 4096 tokens, 8 kv heads 26 us in graph replays, of which reading weights takes 2, the first count and its
+// exchange 4.5, the rest of the choice 5, the list 3 and the move 6.5.
 #include "ommx_kv8.cuh"
 #include "ommx_kv_device.cuh"
 
