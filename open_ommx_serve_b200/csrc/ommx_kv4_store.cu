@@ -2,9 +2,12 @@
 #include <type_traits>
 
 #include "ommx_kv4.cuh"
+#include "ommx_kv_device.cuh"
 
 namespace ommx {
 namespace kv4 {
+
+using kv::max3_nan;
 
 // ---- rows in and out ----------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ float to_f32(T v);
@@ -121,11 +124,6 @@ __device__ __forceinline__ void rotate_key(const AppendParams &p, float (&x)[8],
 }
 
 // of three, NaN if one is
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
 __device__ __forceinline__ float min3_nan(float a, float b, float c) {
     float r;
     asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));

@@ -333,7 +333,9 @@ template <int G, bool E4M3, bool FINE> __device__ __forceinline__ void attend(co
     for (int i = 0; i < 2; ++i) f[i] = scale_of(E) * s.unit[i];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { y[i] = exp2_approx(x[i] - s.ref[i & 1]); z[i] = y[i] * f[i & 1]; }
-    const float heavy = fmaxf(max3(y[0], y[1], y[2]), y[3]), most = fmaxf(max3(z[0], z[1], z[2]), z[3]);
+    // A unit held at its largest while values were zero or tiny may meet a scale with which it is infinite; a weight of 0 then makes a NaN, which
+    // counts as too large: a unit that has moved is finite with the record's scale.
+    const float heavy = fmaxf(max3(y[0], y[1], y[2]), y[3]), most = max3_nan(max3_nan(z[0], z[1], z[2]), z[3], z[3]);
     if (__any_sync(~0u, !(heavy <= HEAVY && most <= ROOM))) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
