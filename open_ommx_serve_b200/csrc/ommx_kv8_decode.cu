@@ -57,7 +57,8 @@ struct DecodeParams {
     const float *before;                          // what weights add to
     int64_t q_b, q_h, o_b, o_h, lse_b;
     int32_t q16, q_wide, o_type, group, col_blocks, page_shift, least, whole, dealt, window, sinks, most_units;
-    float sm_scale, cap, keep;
+    float scale, cap, keep;                       // scale 2^scale_e: sm_scale in powers of two, or with a cap in its units; 0.5 to 1 in size, times LOG2E
+    int32_t scale_e;
     int32_t *status;
 };
 
@@ -144,7 +145,9 @@ template <bool E4M3> __device__ __forceinline__ void value_pairs(uint32_t a, uin
 constexpr int PIECES = 3;
 template <int G, bool E4M3> struct Query {
     uint32_t frag[G][E4M3 ? 2 : PIECES][2];
-    float factor[2], raw[2];                      // of heads 2 t and 2 t + 1: the products' units in powers of two; with a cap: in its units
+    float factor[2];                              // of heads 2 t and 2 t + 1: the products' units, in powers of two or with a cap in its units,
+    int exponent[2];                              // without the powers of two of `exponent` where they are `apart`
+    bool apart;                                   // a factor times a scale may leave fp32's range, or there is a cap
 };
 // The lane's channels as they are, on their way while records are looked up
 template <int G> struct Raw { uint4 v[G]; };
@@ -205,12 +208,14 @@ template <int G, bool E4M3> __device__ __forceinline__ void make_query(const Dec
                 }
             }
         }
-    const float factor = wild ? NAN : p.sm_scale * power_of_two(-BITS) * power_of_two(e);
+    // A factor of 2^-100 to 1 keeps its bits beside every scale, or the logit is nothing, and stays finite
+    const int exponent = p.scale_e + e - BITS;
+    q.apart = p.cap > 0.0f || __any_sync(~0u, exponent > 0 || exponent < -100);
+    const float factor = wild ? NAN : q.apart ? p.scale : p.scale * power_of_two(exponent);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const float f = __shfl_sync(~0u, factor, 8 * t + 4 * i);
-        q.raw[i] = p.cap > 0.0f ? f / p.cap : f;
-        q.factor[i] = p.cap > 0.0f ? p.cap * LOG2E : f * LOG2E;             // with a cap the NaN is in `raw`
+        q.factor[i] = __shfl_sync(~0u, factor, 8 * t + 4 * i);
+        q.exponent[i] = __shfl_sync(~0u, exponent, 8 * t + 4 * i);
     }
 }
 
@@ -301,13 +306,19 @@ template <int G, bool E4M3, bool FINE> __device__ __forceinline__ void attend(co
         if constexpr (E4M3) x[i] = c[0][i] + c[1][i];
         else x[i] = fmaf(fmaf(c[0][i] - BEGIN_VALUE, 256.0f, c[1][i] - BEGIN_VALUE), 256.0f, c[SUMS - 1][i] - BEGIN_VALUE);
     }
-    const float sk = scale_of(info >> 16 & 255u);
-    if (p.cap > 0.0f) {
+    const int EK = info >> 16 & 255u;
+    if (q.apart) {                                // |factor| <= LOG2E: finite; a sum of 0 stays 0, and one below 2^36 times 2^-126 is nothing
+        float f[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = tanhf(x[i] * (q.raw[i & 1] * sk)) * q.factor[i & 1];
+        for (int i = 0; i < 2; ++i) f[i] = q.factor[i] * scale_of(EK ? min(max(EK + q.exponent[i], 1), 254) : 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] *= f[i & 1];
+            if (p.cap > 0.0f) x[i] = tanhf(x[i]) * (p.cap * LOG2E);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] *= q.factor[i & 1] * sk;
+        for (int i = 0; i < 4; ++i) x[i] *= q.factor[i & 1] * scale_of(EK);
     }
     if (put) {
 #pragma unroll
@@ -1016,7 +1027,9 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     p.group = a->n_q_heads / p.c.H; p.col_blocks = (p.group + COLS - 1) / COLS;
     p.page_shift = shift_of(p.c.page);
     p.window = a->window; p.sinks = a->sink_tokens;
-    p.sm_scale = a->sm_scale; p.cap = a->logit_cap; p.status = a->status;
+    p.cap = a->logit_cap; p.status = a->status;
+    p.scale = (float)std::frexp(p.cap > 0.0f ? (double)a->sm_scale / p.cap : (double)a->sm_scale, &p.scale_e);
+    if (!(p.cap > 0.0f)) p.scale *= LOG2E;
     if (p.c.num_pages == 0) return fail(OMMX_E_ARG, "kv8_decode: a cache of no pages");   // what is fetched for a page that is not there
     // as many blocks as the SMs hold, no more than the work can have
     const int64_t units = most_units(a);

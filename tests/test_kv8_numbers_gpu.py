@@ -71,3 +71,47 @@ def test_blocks_of_zeros_before_large_values(run, lens, H, D, large, light, code
     ommx_kv8_decode_attention(q, cache["codes"], cache["scales"], table.to(DEV), i32(lens), o, lse, sm_scale=math.log(2.0), status=status)
     assert int(status) == 0
     hold(q, cache, table.to(DEV), lens, o, lse, math.log(2.0))
+
+
+def attend(lens, H, Hq, D, cache, table, q_scale, sm, dtype=BF16, cap=0.0, out=F32, seed=0):
+    cache = to_gpu(cache)
+    q = (torch.randn(len(lens), Hq, D, generator=torch.Generator().manual_seed(seed)).double() * q_scale).to(dtype).to(DEV)
+    o, lse, status = torch.empty(q.shape, dtype=out, device=DEV), torch.empty(q.shape[:2], device=DEV), i32([0])
+    ommx_kv8_decode_attention(q, cache["codes"], cache["scales"], table.to(DEV), i32(lens), o, lse, sm_scale=sm, logit_cap=cap, status=status)
+    assert int(status) == 0
+    hold(q, cache, table.to(DEV), lens, o, lse, sm, cap)
+
+
+@pytest.mark.parametrize("code,D", [(I8, 128), (E4M3, 128), (I8, 64), (E4M3, 64)])
+@pytest.mark.parametrize("size,sm,E", [(118, -4, 8), (100, -124, 146), (110, -145, 157), (-100, 120, 105),
+                                       (-40, -60, 220), (-60, -50, 230), (60, 60, 3), (0, -130, 245)])
+def test_queries_and_scales_of_every_size(size, sm, E, code, D):
+    """Queries of 2^size, sm_scale 2^sm and keys of unit 2^(E - 127), whose logits are some powers of two."""
+    lens = [40, 900]
+    table, P = tables(lens, 16)
+    cache = random_cache(P, 2, D, 16, code)
+    cache["scales"][..., 0] = E
+    attend(lens, 2, 8, D, cache, table, 2.0 ** size, 2.0 ** sm)
+
+
+@pytest.mark.parametrize("code", [I8, E4M3])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_a_large_channel_that_no_key_has(code, cap):
+    """Queries of one channel, 2^110, which is 0 in every key: all logits are 0, whatever the keys' scales."""
+    lens, D = [40, 900], 128
+    table, P = tables(lens, 16)
+    cache = random_cache(P, 2, D, 16, code, lo=1, hi=246)
+    cache["scales"][..., 1] = 120
+    cache["codes"].view(torch.uint8)[:, :, :, 0, :, 5] = 0
+    q = torch.zeros(2, 4, D)
+    q[..., 5] = 2.0 ** 110
+    q, cache = q.bfloat16().to(DEV), to_gpu(cache)
+    o, lse = torch.empty(q.shape, device=DEV), torch.empty(q.shape[:2], device=DEV)
+    ommx_kv8_decode_attention(q, cache["codes"], cache["scales"], table.to(DEV), i32(lens), o, lse, sm_scale=1.0, logit_cap=cap)
+    for b, n in enumerate(lens):
+        _, v = ref.sequence(cache["codes"], cache["scales"], table[b].to(DEV), n)
+        want = v.mean(1).repeat_interleave(2, 0)
+        size = v.abs().mean(1).repeat_interleave(2, 0)
+        # weights are 1, sums of them exact; values as above
+        assert bool(((o[b].double() - want).abs() <= (2.0 ** -15 + 2.0 ** -21) * size + 2.0 ** -24 * want.abs()).all())
+        assert float((lse[b].double() - math.log(n)).abs().max()) <= 2.0 ** -22 * math.log(n)
