@@ -183,10 +183,19 @@ template <int G, bool E4M3> __device__ __forceinline__ void make_query(const Dec
     largest = max(largest & 0xFFFFu, largest >> 16);
     largest = max(largest, __shfl_xor_sync(~0u, largest, 1));
     largest = max(largest, __shfl_xor_sync(~0u, largest, 2));
-    const float top = p.q16 ? __half2float(__ushort_as_half((uint16_t)largest)) : __uint_as_float(largest << 16);
+    float top = p.q16 ? __half2float(__ushort_as_half((uint16_t)largest)) : __uint_as_float(largest << 16);
     const bool wild = !(top < INFINITY);          // whole numbers hold neither NaN nor infinities: the head's logits are NaN then
-    const int e = top > 0.0f ? max(exponent_of(top), -100) : 0;
     constexpr int BITS = E4M3 ? 13 : 21;          // the largest channel lies below 2^(BITS + 1)
+    constexpr float SMALL = 0x1p-100f;            // rows below it, subnormal ones among them, are raised first: 2^BITS over them is no fp32 number
+    constexpr int RAISE = 64;
+    const bool small = top > 0.0f && top < SMALL;
+    if (__any_sync(~0u, small)) {
+        const float by = small ? power_of_two(RAISE) : 1.0f;
+        top *= by;
+#pragma unroll
+        for (int i = 0; i < 8 * G; ++i) x[i] *= by;
+    }
+    const int e = top > 0.0f ? exponent_of(top) : 0;
     const float up = power_of_two(BITS - e);
 #pragma unroll
     for (int s = 0; s < G; ++s)
@@ -209,7 +218,7 @@ template <int G, bool E4M3> __device__ __forceinline__ void make_query(const Dec
             }
         }
     // A factor of 2^-100 to 1 keeps its bits beside every scale, or the logit is nothing, and stays finite
-    const int exponent = p.scale_e + e - BITS;
+    const int exponent = p.scale_e + e - BITS - (small ? RAISE : 0);
     q.apart = p.cap > 0.0f || __any_sync(~0u, exponent > 0 || exponent < -100);
     const float factor = wild ? NAN : q.apart ? p.scale : p.scale * power_of_two(exponent);
 #pragma unroll

@@ -83,7 +83,7 @@ def attend(lens, H, Hq, D, cache, table, q_scale, sm, dtype=BF16, cap=0.0, out=F
 
 
 @pytest.mark.parametrize("code,D", [(I8, 128), (E4M3, 128), (I8, 64), (E4M3, 64)])
-@pytest.mark.parametrize("size,sm,E", [(118, -4, 8), (100, -124, 146), (110, -145, 157), (-100, 120, 105),
+@pytest.mark.parametrize("size,sm,E", [(-104, 0, 224), (-118, 0, 238), (-128, 0, 245), (-128, 10, 235), (118, -4, 8), (100, -124, 146), (110, -145, 157), (-100, 120, 105),
                                        (-40, -60, 220), (-60, -50, 230), (60, 60, 3), (0, -130, 245)])
 def test_queries_and_scales_of_every_size(size, sm, E, code, D):
     """Queries of 2^size, sm_scale 2^sm and keys of unit 2^(E - 127), whose logits are some powers of two."""
