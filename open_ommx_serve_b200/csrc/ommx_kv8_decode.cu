@@ -1036,7 +1036,9 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     p.group = a->n_q_heads / p.c.H; p.col_blocks = (p.group + COLS - 1) / COLS;
     p.page_shift = shift_of(p.c.page);
     p.window = a->window; p.sinks = a->sink_tokens;
-    p.cap = a->logit_cap; p.status = a->status;
+    // a cap past 2^40 moves a logit of 2^24 by less than its last bit (x^3 / 3 cap^2), and is none: in powers of two the largest ones are infinite
+    p.cap = a->logit_cap <= 0x1p40f ? a->logit_cap : 0.0f;
+    p.status = a->status;
     p.scale = (float)std::frexp(p.cap > 0.0f ? (double)a->sm_scale / p.cap : (double)a->sm_scale, &p.scale_e);
     if (!(p.cap > 0.0f)) p.scale *= LOG2E;
     if (p.c.num_pages == 0) return fail(OMMX_E_ARG, "kv8_decode: a cache of no pages");   // what is fetched for a page that is not there

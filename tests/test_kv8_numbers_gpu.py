@@ -115,3 +115,17 @@ def test_a_large_channel_that_no_key_has(code, cap):
         # weights are 1, sums of them exact; values as above
         assert bool(((o[b].double() - want).abs() <= (2.0 ** -15 + 2.0 ** -21) * size + 2.0 ** -24 * want.abs()).all())
         assert float((lse[b].double() - math.log(n)).abs().max()) <= 2.0 ** -22 * math.log(n)
+
+
+@pytest.mark.parametrize("code", [I8, E4M3])
+@pytest.mark.parametrize("cap", [3.4028234663852886e38, 1e38, 2.0 ** 60, 2.0 ** 41, 2.0 ** 39, 1e6, 1e-30, 1e-38, 1e-45])
+@pytest.mark.parametrize("sm", [0.1, -3.0])
+def test_caps_of_every_size(code, cap, sm):
+    """Some keys are zeros, which no scale of logits makes anything else."""
+    lens = [40, 0, 900]
+    table, P = tables(lens, 16)
+    cache = random_cache(P, 2, 128, 16, code)
+    cache["scales"][::3, ..., 0] = 0
+    cache["codes"].view(torch.uint8)[::3, :, :, 0] = 0
+    lens[1] = 7                                           # on the first page of the pool, which is somebody's
+    attend(lens, 2, 8, 128, cache, table, 1.0, sm, cap=cap)
