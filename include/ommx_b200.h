@@ -32,7 +32,7 @@ extern "C" {
 /* device status bits (OR-ed into *status) */
 #define OMMX_ST_BAD_PAGE     1     /* page id outside [0, num_pages) - access skipped */
 #define OMMX_ST_BAD_GROUP    2     /* group slot outside [0, num_group_slots) - access skipped */
-#define OMMX_ST_NONFINITE    4     /* packer saw NaN/Inf in K or V */
+#define OMMX_ST_NONFINITE    4     /* packer saw NaN/Inf in K or V, an account of weights in a query row */
 #define OMMX_ST_TIMEOUT      8     /* a bounded wait inside a kernel ran out */
 #define OMMX_ST_BAD_LENGTH  16     /* a length past what its tables, its residual buffer or a CTA's split can hold */
 #define OMMX_ST_SCALE_RANGE 32     /* a K or V scale exponent above 11 was clamped in decode (scale step > 2048) */
@@ -564,7 +564,8 @@ typedef struct ommx_kv8_decode_args {
                                        of sequences past it are not kept up (OMMX_ST_BAD_LENGTH) */
     float sm_scale, logit_cap;      /* logits: cap * tanh(q.k * sm_scale / cap); cap 0: none.  sm_scale: any finite number; the largest
                                        |q| * |sm_scale| must be finite in 32 bits.  Logits are served up to 2^24 in size; over int8 codes a query
-                                       row's channels count with 2^-22 of the largest.  A row that is not finite gives NaN */
+                                       row's channels count with 2^-22 of the largest.  A row that is not finite gives NaN for its head, whose
+                                       weights the account leaves out (OMMX_ST_NONFINITE) */
     int32_t *status;
 } ommx_kv8_decode_args;
 

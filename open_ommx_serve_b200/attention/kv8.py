@@ -99,8 +99,8 @@ def ommx_kv8_decode_attention(q: torch.Tensor, codes: torch.Tensor, scales: torc
     sequence of no tokens gives ``o = 0``, ``lse = -inf``; a query row that is not finite NaN, for its head alone.
     ``window``: only the last ``window`` tokens and the first ``sink_tokens`` are visible (all without one); what is not visible is not read.
     ``weight``: every token of a sequence gets ``keep * weight_before`` (default: ``weight`` itself) plus the attention weights, each head's
-    adding up to 1, of the query heads that share its kv head; with ``keep = 0`` those of this step alone.  Their pages belong to one sequence
-    each.
+    adding up to 1, of the query heads that share its kv head; with ``keep = 0`` those of this step alone.  A head whose query row is not finite is
+    left out and reported (``ST_NONFINITE``).  Their pages belong to one sequence each.
     ``max_seq_len`` sizes the grid (the table's width without it); ``workspace`` (fp32, ``kv8_workspace_floats`` values) is
     allocated per call when one is needed and none is given; calls that run side by side need their own."""
     _check((_HOST or _host()).kv8_decode(q, codes, scales, page_table, b_seq_len, o, lse, sm_scale, logit_cap, window, sink_tokens, weight,

@@ -333,10 +333,11 @@ template <int G, bool E4M3, bool FINE> __device__ __forceinline__ void attend(co
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
             float *to = put + (g + 4 * i) * p.group + 2 * t;
-            if (p.group % 2 == 0 && 2 * t < n) *reinterpret_cast<float2 *>(to) = make_float2(x[i], x[i + 1]);
+            const float2 two = make_float2(fmaxf(x[i], LOWEST), fmaxf(x[i + 1], LOWEST));    // the account has no NaN
+            if (p.group % 2 == 0 && 2 * t < n) *reinterpret_cast<float2 *>(to) = two;
             else if (2 * t < n) {
-                to[0] = x[i];
-                if (2 * t + 1 < n) to[1] = x[i + 1];
+                to[0] = two.x;
+                if (2 * t + 1 < n) to[1] = two.y;
             }
         }
     }
@@ -843,6 +844,12 @@ constexpr int THREADS = 256, SHARED_HEADS = 64, QUAD = 4, STRETCH = THREADS * QU
 // references and sums of `n` heads from h0 on, by all warps
 template <int G, bool PARTS> __device__ __forceinline__ void stats_of(const DecodeParams &p, int b, int head, int h0, int n, float2 (&stats)[SHARED_HEADS]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // A head whose query row is not finite is left out: its NaN would stay for all steps to come. Its logits are LOWEST here.
+    auto counted = [&](float2 s) {
+        if (s.y == s.y) return s;
+        or_status(p.status, OMMX_ST_NONFINITE);
+        return make_float2(0.0f, 0.0f);
+    };
     if constexpr (PARTS) {
         for (int h = warp; h < n; h += THREADS / 32) {
             const int row = head * p.col_blocks + (h0 + h) / COLS;
@@ -854,10 +861,10 @@ template <int G, bool PARTS> __device__ __forceinline__ void stats_of(const Deco
                 meet<G>(p, r, (h0 + h) % COLS, lane, 32, top, sum);
                 s = make_float2(top, sum != 0.0f ? 1.0f / sum : 0.0f);
             }
-            if (lane == 0) stats[h] = s;
+            if (lane == 0) stats[h] = counted(s);
         }
     } else {
-        for (int h = threadIdx.x; h < n; h += THREADS) stats[h] = p.stats[((int64_t)b * p.c.H + head) * p.group + h0 + h];
+        for (int h = threadIdx.x; h < n; h += THREADS) stats[h] = counted(p.stats[((int64_t)b * p.c.H + head) * p.group + h0 + h]);
     }
     __syncthreads();
 }

@@ -16,7 +16,7 @@ import pytest
 import torch
 
 import kv8_reference as ref
-from test_kv8_gpu import BF16, DEV, E4M3, F16, F32, I8, i32, random_cache, tables, to_gpu
+from test_kv8_gpu import BF16, DEV, E4M3, F32, I8, i32, random_cache, tables, to_gpu
 from open_ommx_serve_b200 import ommx_kv8_decode_attention
 
 pytestmark = pytest.mark.gpu
