@@ -55,3 +55,48 @@ FORMS = [[40, 0, 200], [1500], [900, 20, 12000], [20000, 4500, 3, 16000, 30000, 
 def test_an_account_leaves_query_rows_out_that_are_not_finite(lens, H, Hq, bad, code, value):
     assert account(lens, H, Hq, 128, code, [(0, h) for h in bad], value=value) == _lib.ST_NONFINITE
     assert account(lens, H, Hq, 64, code, [(0, h) for h in bad], keep=0.0, window=300, sinks=5, value=value) == _lib.ST_NONFINITE
+
+
+@pytest.mark.parametrize("lens", FORMS)
+@pytest.mark.parametrize("H,group", [(1, 65), (2, 70), (1, 128), (2, 100)])
+@pytest.mark.parametrize("code", [I8, E4M3])
+def test_an_account_of_more_heads_than_a_block_holds(lens, H, group, code):
+    """Their references and sums are made 64 at a time for each stretch of tokens: counts that four divides and others, blocks of several stretches."""
+    assert account(lens, H, H * group, 64, code) == 0
+    assert account(lens, H, H * group, 64, code, keep=-1.5, window=1000, sinks=20) == 0
+
+
+def test_an_account_behind_the_join_and_its_launches():
+    """Attention, the join and the account are three launches where the tokens are more than blocks beside the join take at once."""
+    lib, H, D = _lib.load(), 8, 64
+    for lens, want in (([20000] * 4, 3), ([20000], 2), ([200] * 4, 2)):
+        table, P = tables(lens, 64)
+        cache = to_gpu(random_cache(P, H, D, 64, I8))
+        q, table, n = torch.randn(len(lens), H, D, device=DEV).bfloat16(), table.to(DEV), i32(lens)
+        o, lse = torch.empty(q.shape, device=DEV), torch.empty(q.shape[:2], device=DEV)
+        before = lib.ommx_b200_launch_count()
+        ommx_kv8_decode_attention(q, cache["codes"], cache["scales"], table, n, o, lse, weight=cache["weight"], max_seq_len=max(lens))
+        assert lib.ommx_b200_launch_count() - before == want
+
+
+@pytest.mark.parametrize("H", [2, 40])
+def test_the_account_of_a_sequence_beside_ones_past_max_seq_len(H):
+    """Tokens within max_seq_len, in a sequence that is and in those that are not, get their weights; what is past it keeps its own."""
+    lens, page, D, most = [800, 90, 3000], 16, 64, 100
+    table, P = tables(lens, page)
+    cache = to_gpu(random_cache(P, H, D, page, I8))
+    before, q = cache["weight"].clone(), torch.randn(3, 4 * H, D, generator=torch.Generator().manual_seed(1)).bfloat16().to(DEV)
+    o, lse, status = torch.empty(q.shape, device=DEV), torch.empty(q.shape[:2], device=DEV), i32([0])
+    ommx_kv8_decode_attention(q, cache["codes"], cache["scales"], table.to(DEV), i32(lens), o, lse, weight=cache["weight"], keep=0.25, max_seq_len=most, status=status)
+    assert int(status) == _lib.ST_BAD_LENGTH
+    for b, n in enumerate(lens):
+        k, v = ref.sequence(cache["codes"], cache["scales"], table[b].to(DEV), n)
+        _, _, p, off = ref.attention(q[b], k, v, D ** -0.5)
+        add, tol = (x.view(H, 4, n).sum(1) for x in (p, p * (2 * off + 2.0 ** -20)[:, None]))
+        t = torch.arange(n)
+        ids, at = table[b, t // page].long().to(DEV), (t % page).to(DEV)
+        was, now = before[ids, :, at].T.double(), cache["weight"][ids, :, at].T
+        kept = -(-min(n, most) // 16) * 16                # records are counted, not tokens
+        want = 0.25 * was + add
+        assert bool(((now.double() - want).abs() <= tol + 2.0 ** -20 * want.abs() + 4 * 2.0 ** -126)[:, :kept].all())
+        assert torch.equal(now[:, kept:], was[:, kept:].float())
