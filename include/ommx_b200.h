@@ -555,7 +555,7 @@ typedef struct ommx_kv8_decode_args {
     float *lse;                     /* [batch, n_q_heads], natural logarithm; -inf (and o = 0) for a sequence of no tokens */
     int64_t lse_stride_b;
     int32_t window, sink_tokens;    /* window > 0: the last `window` tokens and the first sink_tokens are visible; 0: all */
-    const float *weight_before;     /* like cache.weight, 16-byte aligned, and may be it: weight = keep * weight_before + the sum of the attention weights
+    const float *weight_before;     /* like cache.weight, 16-byte aligned, and it or apart from it: weight = keep * weight_before + the sum of the attention weights
                                        of the kv head's query heads; not read with keep = 0 */
     float keep;
     float *workspace;               /* 16-byte aligned; calls that overlap need their own */

@@ -98,7 +98,7 @@ def ommx_kv8_decode_attention(q: torch.Tensor, codes: torch.Tensor, scales: torc
     them.  ``sm_scale`` defaults to ``D ** -0.5`` and may be any finite number; ``logit_cap`` c makes a logit ``c tanh(x / c)``.  A
     sequence of no tokens gives ``o = 0``, ``lse = -inf``; a query row that is not finite NaN, for its head alone.
     ``window``: only the last ``window`` tokens and the first ``sink_tokens`` are visible (all without one); what is not visible is not read.
-    ``weight``: every token of a sequence gets ``keep * weight_before`` (default: ``weight`` itself) plus the attention weights, each head's
+    ``weight``: every token of a sequence gets ``keep * weight_before`` (``weight`` itself, the default, or apart from it) plus the attention weights, each head's
     adding up to 1, of the query heads that share its kv head; with ``keep = 0`` those of this step alone.  A head whose query row is not finite is
     left out and reported (``ST_NONFINITE``).  Their pages belong to one sequence each.
     ``max_seq_len`` sizes the grid (the table's width without it); ``workspace`` (fp32, ``kv8_workspace_floats`` values) is

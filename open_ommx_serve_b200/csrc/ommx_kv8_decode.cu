@@ -1030,6 +1030,9 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     if (a->window < 0 || a->sink_tokens < 0 || a->max_seq_len < 0) return fail(OMMX_E_ARG, "kv8_decode: window, sink_tokens and max_seq_len must not be negative");
     if (a->cache.weight && (!std::isfinite(a->keep) || (a->keep != 0.0f && !a->weight_before))) return fail(OMMX_E_ARG, "kv8_decode: keep must be finite, and what is kept must be given");
     if (reinterpret_cast<uintptr_t>(a->weight_before) % 16) return fail(OMMX_E_ARG, "kv8_decode: weight_before must be 16-byte aligned");
+    const int64_t weights = (int64_t)p.c.num_pages * p.c.H * p.c.page;
+    if (a->cache.weight && a->keep != 0.0f && a->weight_before != a->cache.weight && a->weight_before < a->cache.weight + weights && a->cache.weight < a->weight_before + weights)
+        return fail(OMMX_E_ARG, "kv8_decode: weight_before must be weight itself or apart from it");
     if (p.s.B > 65535) return fail(OMMX_E_UNSUPPORTED, "kv8_decode: a batch of %d", p.s.B);
     if (p.s.B == 0) return 0;
     if (!a->q || !a->o || !a->lse) return fail(OMMX_E_ARG, "kv8_decode: q, o and lse must not be null");

@@ -203,6 +203,19 @@ def test_lengths_that_overlap_are_refused():
         assert _lib.load().ommx_b200_kv8_evict(C.byref(e), None) == -1 and "len_out" in _lib.last_error()
 
 
+def test_weights_before_that_overlap_are_refused():
+    """A step reads one token's weight before and writes another's: weights a few tokens apart would be read after they are written."""
+    n = 5 * H * PAGE
+    d = c_args(_lib.KV8DecodeArgs)
+    d.q = d.o = d.lse = d.workspace = 256
+    d.q_dtype = d.o_dtype = _lib.OMMX_DT_BF16
+    d.n_q_heads, d.sm_scale, d.keep, d.workspace_floats = HQ, 1.0, 1.0, 1 << 30
+    d.cache.weight = 1 << 20
+    for off in (16, -16, 4 * n - 16, 16 - 4 * n):
+        d.weight_before = (1 << 20) + off
+        assert _lib.load().ommx_b200_kv8_decode(C.byref(d), None) == -1 and "apart" in _lib.last_error()
+
+
 def test_workspace_sizes():
     assert kv8_workspace_floats(4, 32, 128, 512) == 0
     whole = kv8_workspace_floats(1, 32, 128, 513)
