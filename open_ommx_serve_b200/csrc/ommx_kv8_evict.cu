@@ -117,7 +117,7 @@ template <int G, bool E4M3, int THREADS> __global__ void __launch_bounds__(THREA
             if (head == 0 && p.len_out) p.len_out[b] = faults ? given : keep;
         }
         if (listed)
-            for (int i = rank * THREADS + tid; i < p.budget; i += n * THREADS) out[i] = !faults && i < len ? i : -1;
+            for (int64_t i = rank * THREADS + tid; i < p.budget; i += n * THREADS) out[i] = !faults && i < len ? (int)i : -1;
     };
     if (faults) { leave(true); return; }
     const int share = ((len + (int)n - 1) / (int)n + 31) & ~31;
