@@ -931,7 +931,8 @@ static int decode(const ommx_kv4_decode_args *a, cudaStream_t st) {
     p.selected = a->selected; p.num_selected = a->num_selected;
     p.group = a->n_q_heads / p.c.H; p.col_blocks = (p.group + COLS - 1) / COLS;
     p.page_shift = shift_of(p.c.page);
-    p.sm_scale = a->sm_scale; p.cap = a->logit_cap; p.status = a->status;
+    p.sm_scale = a->sm_scale; p.status = a->status;
+    p.cap = a->logit_cap <= 0x1p126f ? a->logit_cap : 0.0f;                 // past that it changes no logit, and is infinite in powers of two
     if (p.c.num_pages == 0) return fail(OMMX_E_ARG, "kv4_decode: a cache of no pages");   // what is fetched for a page that is not there
     // as many blocks as the SMs hold, no more than the work can have
     const int64_t units = most_units(a);

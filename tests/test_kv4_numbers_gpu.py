@@ -97,6 +97,17 @@ def test_logit_scales_of_zero_and_below(D, H, Hq, lens, sm_scale, cap):
     assert torch.isfinite(o).all() and torch.isfinite(lse).all()
 
 
+@pytest.mark.parametrize("D,H,Hq,lens", FORMS)
+@pytest.mark.parametrize("cap", [3.4028234663852886e38, 2.5e38, 1e38])
+def test_caps_near_the_largest_number(D, H, Hq, lens, cap):
+    """They change no logit; from 2^127.5 on they are infinite in powers of two."""
+    cache, table, length = filled(lens, H, D, 16, seed=143)
+    q = torch.randn(len(lens), Hq, D, generator=torch.Generator().manual_seed(144)).bfloat16().to(DEV)
+    o, lse = torch.full((len(lens), Hq, D), 7.0, device=DEV), torch.full((len(lens), Hq), 7.0, device=DEV)
+    ommx_kv4_decode_attention(q, cache["records"], table, length, o, lse, logit_cap=cap, max_seq_len=max(lens))
+    check(cache, table, lens, q, o, lse, cap=cap, which=range(min(len(lens), 6)))
+
+
 # ---- the size of the values ----------------------------------------------------------------------------------------
 def cache_of(k, v, page=16):
     """One sequence per entry of the lists k, v ([tokens, H, D]): (cache, table, lens tensor, lens)."""
