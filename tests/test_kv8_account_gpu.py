@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 def account(lens, H, Hq, D, code, bad=(), keep=0.5, window=None, sinks=0, page=16, max_len=None, value=math.nan):
     """Weights of one call against 64 bits; `bad`: heads (sequence, head) whose query row is not finite, which are left out.  A weight is off by its
-    share d and 2^-20 of itself; a head's below 2^-126 counts as 0."""
+    share d and 2^-20 of itself; a head's below 2^-126 of its reference counts as 0, and the sum that divides it is 1/2 at least."""
     table, P = tables(lens, page)
     cache = to_gpu(random_cache(P, H, D, page, code))
     q = torch.randn(len(lens), Hq, D, generator=torch.Generator().manual_seed(0)).bfloat16().to(DEV)
@@ -39,7 +39,7 @@ def account(lens, H, Hq, D, code, bad=(), keep=0.5, window=None, sinks=0, page=1
         add[:, seen] = p.view(H, group, -1).sum(1)
         tol[:, seen] = (p * (2 * off + 2.0 ** -20)[:, None]).view(H, group, -1).sum(1)
         now = want[ids, :, at].T * keep + add
-        want[ids, :, at], off_all[ids, :, at] = now.T, (tol + 2.0 ** -20 * now.abs() + group * 2.0 ** -126).T
+        want[ids, :, at], off_all[ids, :, at] = now.T, (tol + 2.0 ** -20 * now.abs() + group * 2.0 ** -125).T
     err = (cache["weight"].double() - want).abs()
     assert bool((err <= off_all).all()), (int(cache["weight"].isnan().sum()), float((err - off_all).max()))
     return int(status)
@@ -98,5 +98,5 @@ def test_the_account_of_a_sequence_beside_ones_past_max_seq_len(H):
         was, now = before[ids, :, at].T.double(), cache["weight"][ids, :, at].T
         kept = -(-min(n, most) // 16) * 16                # records are counted, not tokens
         want = 0.25 * was + add
-        assert bool(((now.double() - want).abs() <= tol + 2.0 ** -20 * want.abs() + 4 * 2.0 ** -126)[:, :kept].all())
+        assert bool(((now.double() - want).abs() <= tol + 2.0 ** -20 * want.abs() + 4 * 2.0 ** -125)[:, :kept].all())
         assert torch.equal(now[:, kept:], was[:, kept:].float())

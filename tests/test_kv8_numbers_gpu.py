@@ -5,7 +5,7 @@ Bounds, with p the softmax in 64 bits, V the cached values, s their scales, n to
 * a weight times a scale goes to fp16: by 2^-11 of itself at most, by 2^-21 where the output is finer than bf16 (what the first rounding left is
   rounded once more).  The largest product of a warp lies above 2^10 in the units that fp16 has, whose last steps are 2^-24: half of one is 2^-35 of the
   largest, and codes are 448 at most: n 448 2^-35 max p s;
-* a weight below 2^-126 of its reference counts as 0: n 2^-126 max |V|;
+* a weight below 2^-126 of its reference counts as 0, and the sum that divides it is 1/2 at least: n 2^-125 max |V|;
 * sums of up to 400 records of a warp are cut 24 bits below them: 2^-15 sum p |V|;
 * the output is rounded by half a step.
 The log-sum-exp is off by off + 2^-20 and four roundings of itself.
@@ -34,7 +34,7 @@ def hold(q, cache, table, lens, o, lse, sm, cap=0.0):
         s = torch.where(E > 0, torch.exp2(E - 127), 0.0).repeat_interleave(group, 0)
         v = v.abs().repeat_interleave(group, 0)
         size, d = torch.einsum("ht,htd->hd", p, v), (2 * off + 2.0 ** -20)[:, None]
-        tol = (2 * d + fp16 + 2.0 ** -15) * size + n * (448 * 2.0 ** -35 * (p * s).amax(1)[:, None] + 2.0 ** -126 * v.amax((1, 2))[:, None])
+        tol = (2 * d + fp16 + 2.0 ** -15) * size + n * (448 * 2.0 ** -35 * (p * s).amax(1)[:, None] + 2.0 ** -125 * v.amax((1, 2))[:, None])
         tol = tol + half * wo.abs() + torch.finfo(o.dtype).tiny
         err = (o[b].double() - wo).abs()
         assert bool((err <= tol).all()), (b, n, int(o[b].isnan().sum()), float((err / tol).max()))
