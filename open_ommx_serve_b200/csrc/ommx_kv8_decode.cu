@@ -147,7 +147,7 @@ template <int G, bool E4M3> struct Query {
     uint32_t frag[G][E4M3 ? 2 : PIECES][2];
     float factor[2];                              // of heads 2 t and 2 t + 1: the products' units, in powers of two or with a cap in its units,
     int exponent[2];                              // without the powers of two of `exponent` where they are `apart`
-    bool apart;                                   // a factor times a scale may leave fp32's range, or there is a cap
+    bool apart;                                   // a factor times a scale may leave fp32's range
 };
 // The lane's channels as they are, on their way while records are looked up
 template <int G> struct Raw { uint4 v[G]; };
@@ -219,7 +219,7 @@ template <int G, bool E4M3> __device__ __forceinline__ void make_query(const Dec
         }
     // A factor of 2^-100 to 1 keeps its bits beside every scale, or the logit is nothing, and stays finite
     const int exponent = p.scale_e + e - BITS - (small ? RAISE : 0);
-    q.apart = p.cap > 0.0f || __any_sync(~0u, exponent > 0 || exponent < -100);
+    q.apart = __any_sync(~0u, exponent > 0 || exponent < -100);
     const float factor = wild ? NAN : q.apart ? p.scale : p.scale * power_of_two(exponent);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -316,18 +316,16 @@ template <int G, bool E4M3, bool FINE> __device__ __forceinline__ void attend(co
         else x[i] = fmaf(fmaf(c[0][i] - BEGIN_VALUE, 256.0f, c[1][i] - BEGIN_VALUE), 256.0f, c[SUMS - 1][i] - BEGIN_VALUE);
     }
     const int EK = info >> 16 & 255u;
+    float unit[2] = {q.factor[0] * scale_of(EK), q.factor[1] * scale_of(EK)};
     if (q.apart) {                                // |factor| <= LOG2E: finite; a sum of 0 stays 0, and one below 2^36 times 2^-126 is nothing
-        float f[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) f[i] = q.factor[i] * scale_of(EK ? min(max(EK + q.exponent[i], 1), 254) : 0);
+        for (int i = 0; i < 2; ++i) unit[i] = q.factor[i] * scale_of(EK ? min(max(EK + q.exponent[i], 1), 254) : 0);
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] *= f[i & 1];
-            if (p.cap > 0.0f) x[i] = tanhf(x[i]) * (p.cap * LOG2E);
-        }
-    } else {
+    for (int i = 0; i < 4; ++i) x[i] *= unit[i & 1];
+    if (p.cap > 0.0f) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] *= q.factor[i & 1] * scale_of(EK);
+        for (int i = 0; i < 4; ++i) x[i] = tanhf(x[i]) * (p.cap * LOG2E);
     }
     if (put) {
 #pragma unroll
