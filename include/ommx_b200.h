@@ -493,7 +493,7 @@ int64_t ommx_b200_kv4_select_workspace_bytes(int32_t batch, int32_t n_kv_heads, 
  * E is the smallest from 1 on for which the block's largest value is at most 127 (int8) or 448 (e4m3) units, 0 where all are zero;
  * codes are value / unit to the nearest, ties to even.  NaN counts as 0 and values beyond 2^126 as that (OMMX_ST_NONFINITE where one
  * is not finite).  A block that holds tokens and takes rows keeps the larger E of the two; codes it holds are rounded to that.
- * int8 -128 and e4m3's NaN are never written; where a caller writes them they count as that.
+ * int8 -128 and e4m3's NaN are never written; where a caller writes them they count as that.  E is never above 247, and 254 is the largest that is served.
  * weight (optional): float [num_pages][n_kv_heads][page_size], what each token was attended to with.
  *
  * A page that takes rows, weights or kept tokens belongs to one sequence.  Lengths, tables and row ranges are read on the device: nothing
@@ -562,8 +562,9 @@ typedef struct ommx_kv8_decode_args {
     int64_t workspace_floats;
     int32_t max_seq_len;            /* an upper bound of b_seq_len that sizes the grid and the workspace, 0: what the table can hold.  Weights
                                        of sequences past it are not kept up (OMMX_ST_BAD_LENGTH) */
-    float sm_scale, logit_cap;      /* logits: cap * tanh(q.k * sm_scale / cap); cap 0: none.  sm_scale: any finite number; the largest
-                                       |q| * |sm_scale| must be finite in 32 bits.  Logits are served up to 2^24 in size; over int8 codes a query
+    float sm_scale, logit_cap;      /* logits: cap * tanh(q.k * sm_scale / cap); cap 0, or past 2^40: none.  sm_scale: any finite number; the largest
+                                       |q| * |sm_scale| must be finite in 32 bits.  Logits are served up to 2^24 in size; a token's weight below
+                                       2^-126 of the heaviest counts as 0; over int8 codes a query
                                        row's channels count with 2^-22 of the largest.  A row that is not finite gives NaN for its head, whose
                                        weights the account leaves out (OMMX_ST_NONFINITE) */
     int32_t *status;
@@ -571,7 +572,7 @@ typedef struct ommx_kv8_decode_args {
 
 /* Attention of one query row per sequence.  A kv head's records are read once for each eight of its query heads.  Two launches; one where
  * no sequence sees more than 512 tokens by max_seq_len, the table's width or the window, or, where rows (sequences x kv heads x eights of
- * query heads) are few enough for clusters, 4608 (up to 16000 where they are 15 at most), or a window of up to 1500 where there are some 300 to 590 rows; one more where weights are kept of many tokens, two at least. */
+ * query heads) are few enough for clusters, 4608 (where they are 15 at most 128 (40 + 6 rows): 5888 for one, 11264 for eight, 16640 for fifteen), or a window of up to 1500 where there are some 300 to 590 rows; one more where weights are kept of many tokens, two at least. */
 int ommx_b200_kv8_decode(const ommx_kv8_decode_args *args, void *stream);
 /* floats of workspace that this call needs on the current device (0: none; its pointers are not looked at, but for whether there is a weight) */
 int64_t ommx_b200_kv8_decode_workspace_floats(const ommx_kv8_decode_args *args);

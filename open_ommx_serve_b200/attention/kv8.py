@@ -98,6 +98,7 @@ def ommx_kv8_decode_attention(q: torch.Tensor, codes: torch.Tensor, scales: torc
     them.  ``sm_scale`` defaults to ``D ** -0.5`` and may be any finite number; ``logit_cap`` c makes a logit ``c tanh(x / c)``.  A
     sequence of no tokens gives ``o = 0``, ``lse = -inf``; a query row that is not finite NaN, for its head alone.
     ``window``: only the last ``window`` tokens and the first ``sink_tokens`` are visible (all without one); what is not visible is not read.
+    A token whose weight is below 2^-126 of the heaviest counts for nothing.
     ``weight``: every token of a sequence gets ``keep * weight_before`` (``weight`` itself, the default, or apart from it) plus the attention weights, each head's
     adding up to 1, of the query heads that share its kv head; with ``keep = 0`` those of this step alone.  A head whose query row is not finite is
     left out and reported (``ST_NONFINITE``).  Their pages belong to one sequence each.
@@ -114,7 +115,8 @@ def ommx_kv8_evict(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tens
     """Keep ``kept.shape[2]`` tokens of each sequence and kv head, and move them with their weights to the front, in their order.
 
     Kept are the first ``sink_tokens``, the last ``recent_tokens`` and of the others those of the largest ``weight`` (equal ones: the lower
-    place; NaN last); all of a sequence that has no more.  ``kept`` (int32 ``[batch, n_kv_heads, n]``) gets their places, ascending, then
+    place; NaN last); all of a sequence that has no more.  Appended tokens weigh 0 until a step attends to them, so right after a prompt the lowest
+    places stay: attend a few steps with an account first.  ``kept`` (int32 ``[batch, n_kv_heads, n]``) gets their places, ascending, then
     -1; ``len_out`` (int32 ``[batch]``, may be ``b_seq_len``) the new lengths.  They take the first pages of the sequence itself or,
     with ``to_table`` (int32 or int64 ``[batch, pages]``), pages that no sequence holds, and then the old ones are left as they were (a
     prefix that sequences share).  ``max_seq_len`` sizes the launch."""

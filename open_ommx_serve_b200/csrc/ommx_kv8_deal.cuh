@@ -13,8 +13,9 @@ namespace kv8 {
 // * else every row is cut into pieces of at most `per` units, a block to a piece, with the smallest `per` for which there are blocks
 //   enough;
 // * or, where that would leave a block with over BEGIN units more than an even share, all rows end to end are cut into such shares,
-//   whatever rows they touch. A second piece costs a block some 4 us, half of it hidden by the SM's other blocks (4-bit cache, 64K tokens:
-//   26.7 us with seven such blocks of 296, 24.4 with none; 64 sequences of 200..2000 tokens: 43.3 with even shares, 38.3 with pieces).
+//   whatever rows they touch. A second piece costs a block some 4 us, half of it hidden by the SM's other blocks. us with pieces only up to 0, 16, 32, 64
+//   and 256 units above an even share, and always: 8 x 64K tokens, 8 kv heads 206, 183, 180, 181, 181, 179; 64 sequences of 200 to 2000 44, 42, 42, 39, 39,
+//   39; 100 of 500 to 4000, 2 kv heads 39.5, then 30; 61 of 300 to 20000 159 up to 256, always 179; 32, 40 and 20 ragged ones within 3 %.
 // A piece that is a whole row is finished where it is computed; the others' parts meet in the second kernel. A block has at most two
 // of those, of the row that an earlier block began (its slot 0) and of the one that a later block goes on with (slot 1).
 constexpr uint32_t OVER = 2;                      // in the deal's place: there is none

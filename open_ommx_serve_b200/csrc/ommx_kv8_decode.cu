@@ -7,19 +7,21 @@
 //   logits   int8: 8-bit products (m16n8k32) of the codes as they are and the three bytes of a query row as whole numbers of 23 bits, exact from there
 //            on; a channel is rounded by 2^-22 of the row's largest at most. Fp16 products, whose operands have to be made, took 33 us more of 166 (8 x 64K
 //            tokens, copies left out). e4m3: fp16 products, since 8-bit ones of this type have their operands converted each time (three pieces of a
-//            query: 32 ragged sequences 71 us with fp16, 81 with e4m3); a query row times a power of two is an fp16 number, bf16 channels below 2^-27 of
-//            the largest are rounded by 2^-39 of it;
+//            query: 32 ragged sequences 71 us with fp16, 81 with e4m3); a query row times a power of two is an fp16 number, bf16 channels below 2^-30
+//            of the largest and fp16 ones below 2^-27 are rounded by 2^-38 of it at most;
 //   values   fp16 (m16n8k16), in which the codes are made exactly; weights times scales, y 2^ev, go to fp16 in a unit that the largest of them sets,
 //            a power of two for each head: a token whose weight times scale is 2^-25 of the largest keeps its bits (11), so values of any size
-//            leave no token out. Where the output is finer than bf16 a second product takes what the rounding left (FINE).
+//            leave no token out but those whose weight is below 2^-126 of the heaviest, which fp32 holds as 0. Where the output is finer than bf16 a
+//            second product takes what the rounding left (FINE).
 // The tensor cores cut what they add to a sum 24 bits below it, so an output is off by 2^-25 of itself for each record of a warp, 2^-18 for 110 of them
 // (8 x 64K tokens).
 //
 // What bounds it: a record's 32 D bytes are read once for each eight query heads of its kv head, and a warp spends 343 instructions on one (D = 128, int8): the
-// copies alone take 165 us of 8 x 64K tokens, 8 kv heads, the products alone 133, both 171 to 180 (6.0 to 6.3 TB/s, 92 to 96 % of what a copy reaches); 32 ragged
-// sequences of 700 to 8191 tokens 57, 57 and 64. A warp has a ring of its own, so that no barrier stands between a copy and its use: two slots and 16
+// copies alone take 165 us of 8 x 64K tokens, 8 kv heads, the products alone 133, both 170 to 182 by card (5.9 to 6.3 TB/s, 90 to 97 % of what a copy
+// reaches); 32 ragged sequences of 700 to 8191 tokens 57, 57 and 62 to 64. A warp has a ring of its own, so that no barrier stands between a copy and its use: two slots and 16
 // warps to an SM (8 x 64K tokens: 183 us; three slots 192, 12 warps and three slots 188, 20 warps 208). Few and short rows are bound by
-// the chain of launch, lengths, table, records and join: 6.9 us for one of 333 tokens, of which a launch alone takes 2.5.
+// the chain of launch, lengths, table, records and join: 6.9 us for one of 333 tokens, of which a launch alone takes 2.5. Many short rows are a block
+// each, with that chain in every block: 512 sequences of 100 to 500 tokens are 4096 blocks, 592 at once, 7 turns of 11.4 us (80 us, 49 of them bytes).
 #include <cmath>
 #include <type_traits>
 
@@ -1072,14 +1074,19 @@ static int decode(const ommx_kv8_decode_args *a, cudaStream_t st) {
     int cluster = 1;
     static AtOnce known[2];                       // of eight and sixteen warps; D = 64 takes less
     while (cluster < MOST_CLUSTER && 2 * cluster * rows <= most_blocks(8) && rows <= clusters_at_once(known[0], kv8_decode_kernel<4, false, false, 8, true>, 256, sizeof(Memory<4, 8>), 2 * cluster)) cluster *= 2;
-    // of sixteen warps where a row has more records than eight of eight warps should take (8 kv heads: 4400 tokens 10.1 us with eight, 10.7 with sixteen), up
-    // to where all SMs and a join are faster: 5000 tokens 10.9 us so and 13.8 with a join, 8000 12.4 and 14.0, 12000 14.7 and 14.9; of one kv
-    // head 5000 10.7 and 11.1, 7000 11.7 and 11.1
+    // of sixteen warps where a row has more records than eight of eight warps should take, up to where all SMs and a join are faster, which is later the more
+    // rows there are. us with eight warps, sixteen and a join: 8 rows of 4600 tokens 10.3, 10.8, 12.7, of 6000 11.1, 11.3, 13.4, 8000 12.5, 12.5, 13.6,
+    // 10000 14.2, 13.5, 13.9, 12000 15.6, 14.6, 14.5; where sixteen and a join meet: one row 5900 tokens (10.9), two 6700 (11.6), four 6500 (11.5), eight
+    // 11500 (14.4), twelve 20000 (19.2), fifteen past 20000 (19.4 and 21.6). The line lies within 0.6 us of the better one up to eight rows; past
+    // its end twelve rows of 16000 take 17.9 for 17.1, fifteen of 20000 21.6 for 19.4
     const bool wide = cluster == MOST_CLUSTER && units > 36 * cluster && units <= (40 + 6 * rows) * cluster &&
                       rows <= clusters_at_once(known[1], kv8_decode_kernel<4, false, false, 16, true>, 512, sizeof(Memory<4, 16>), cluster);
     if (units > 36 * cluster && !wide) cluster = 1;
-    // A window makes rows alike, so where there is a block for each and not two they go whole too (61 sequences of 300 to 20000 tokens, 8 kv heads: windows of 600
-    // 21.3 -> 18.0 us, of 1025 30.8 -> 26.7; 50 of 61 sequences too short for one of 1025 18.3 -> 20.6, for 1800 22.6 -> 31.1, which is past the limit)
+    // A window makes rows alike, so where there is a block for each and not two they go whole too. us whole and dealt, for 304, 360, 488 and 584 rows of 8 kv heads
+    // whose sequences have 300 to 20000 tokens: windows of 600 17.1 and 17.5, 17.6 and 21.4, 18.2 and 22.1, 18.8 and 23.5, of 1400 30.7 and 25.7, 31.4 and
+    // 28.8, 33.5 and 37.1, 36.0 and 41.4; 580 rows of one kv head 18.8 and 32.7, 35.4 and 50.8. Where five sequences in six are shorter than the window it is
+    // slower below some 450 rows and windows past 1000 (360 rows of 1025 23.0 and 20.7, of 1400 29.2 and 24.3; 488 rows 23.9 and 25.6): lengths are
+    // not known here
     const bool alike = a->window > 0 && cluster == 1 && rows <= hold && 2 * rows > hold && units <= 3 * WHOLE;
     p.whole = units <= WHOLE / 2 || (units <= WHOLE && cluster == 1) || alike;
     if (p.whole) cluster = 1;

@@ -9,8 +9,10 @@
 // * moves: places ascend, and a token never moves up. So once a cluster has read all that a stretch of places takes into its shared
 //   memory it can write that stretch where the tokens lie, and go on to the next.
 // What bounds it: where rows are many what moves (64 sequences of 4608 to 4096 tokens, 8 kv heads 210 us; 1.1 GB there and back take 165 of a copy's rate),
-// where they are few the chain: 64K to 4096 tokens, 8 kv heads 26 us in graph replays, of which reading weights takes 2, the first count and its
-// exchange 4.5, the rest of the choice 5, the list 3 and the move 6.5.
+// where they are few the chain: 64K to 4096 tokens, 8 kv heads 26 us in graph replays (19 MB are 2.9), of which reading weights takes 2, the first count and its
+// exchange 4.5, the rest of the choice 5, the list 3 and the move 6.5, on 64 of the SMs, since a cluster has eight blocks at most. Short rows are the same
+// chain (700 to 500 tokens 14.4 us). Of 8 x 64K to 4096 (68 us, 23.6 in bytes) a block has 32K keys, which pass through shared memory again at
+// each count and in the list.
 #include "ommx_kv8.cuh"
 #include "ommx_kv_device.cuh"
 

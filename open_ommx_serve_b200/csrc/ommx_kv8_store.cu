@@ -107,8 +107,10 @@ struct AppendParams {
 // Grid: (records that take rows, shares of their 2 H items); an item is the keys or the values of a head, a warp to it. The warp holds its
 // rows (16 at most), whose largest magnitude is an integer maximum, and writes each once. Tokens that the record holds already are read
 // again only where the new rows need a larger scale.
-// What bounds it: memory where rows are many (8192 of 8 kv heads, D = 128, bf16 9.7 us and fp32 13.7, in graph replays; 50 MB take 7.7 of a copy's rate;
-// 65536 rows 69.8 us, 88 % of it), the chain of launch, lengths, table and rows where they are few (one of one sequence 2.5 us, of 512 5.9).
+// What bounds it: memory where rows are many (8192 of 8 kv heads, D = 128, bf16 9.6 us and fp32 13.5, in graph replays; 50 MB take 7.7 of a copy's rate;
+// 65536 rows 69 us, 89 % of it), the chain of launch, lengths, table and rows where they are few (one of one sequence 2.5 us, of 61 too). A row each of many
+// sequences is that chain in every block: 1024 are 2048 blocks, 592 at once, 3.5 turns (10.1 us, for 6.3 MB); with ranges every block also looks
+// through those of all sequences (14.8).
 template <typename T, int G, bool E4M3, bool WIDE>
 __global__ void __launch_bounds__(32 * MOST_WARPS, sizeof(T) == 4 ? 2 : 4) kv8_append_kernel(const __grid_constant__ AppendParams p) {
     constexpr int D = 32 * G, LANES = D / 8, ROWS = 32 / LANES, TURNS = BLOCK / ROWS;
@@ -234,9 +236,9 @@ template <typename T, bool WIDE> __device__ __forceinline__ void store8(T *to, c
     }
 }
 
-// Grid as above; a lane reads 8 codes at a time, so that a warp's store is whole rows: 8192 rows x 8 heads 10.8 us, 14.5 with 16 codes a lane, whose stores
-// left gaps and which took 64 registers. Since then 7.6 in graph replays (outputs of 34 MB that stay in the cache), 65536 rows 67.6: what it reads and writes
-// bounds it, 91 % of a copy's rate.
+// Grid as above; a lane reads 8 codes at a time, so that a warp's store of 16-bit rows is whole rows: 8192 rows x 8 heads 10.8 us, 14.5 with 16 codes a lane,
+// whose stores left gaps and which took 64 registers. Since then 7.6 in graph replays (outputs of 34 MB that stay in the cache), 65536 rows 67.4: what it reads
+// and writes bounds it, 91 % of a copy's rate. fp32 rows are two stores a lane, each of every other 16 bytes: 8192 rows 20.9 us, for bytes of 12.8.
 template <typename T, int G, bool E4M3, bool WIDE>
 __global__ void __launch_bounds__(32 * GATHER_WARPS, 6) kv8_gather_kernel(const __grid_constant__ GatherParams p) {
     constexpr int D = 32 * G, LANES = D / 8, ROWS = 32 / LANES, TURNS = BLOCK / ROWS;
